@@ -56,6 +56,10 @@ extern "C" {
 #define KVC_FLAG_CODE_TOO_LONG   0x100  /* codebook: a code is longer than 32 bits */
 #define KVC_FLAG_NO_SYMBOLS      0x200  /* codebook: empty histogram */
 #define KVC_FLAG_WAIT_TIMEOUT    0x400  /* a bounded device-side wait gave up */
+#define KVC_FLAG_NO_PAGES        0x800  /* page plan: a request was refused (no pages left, or its table row or the token rows are full);
+                                         * page release: more pages than have been taken */
+#define KVC_FLAG_BAD_PAGE        0x1000 /* paged cache: a table entry or a slot outside the pool; its tokens are left out */
+#define KVC_FLAG_BAD_LENGTH      0x2000 /* paged cache: a length or a count of new tokens below 0, or beyond the table row */
 
 typedef void *kvc_stream_t;   /* a cudaStream_t; NULL = the legacy default stream */
 
@@ -368,6 +372,99 @@ int kvc_attn_decode_static(const kvc_cache *k, const kvc_cache *v, int64_t T, in
 /* k_mat_vec_mul_cuda_export (kernels.cu:1192-1273): dense q.k over uncompressed fp16 K
  * [ctx,1,H,128], q [1,H,128] -> out fp16 [ctx,1,H].  Comparison baseline only. */
 int kvc_k_matvec(const void *k, const void *q, void *out, int64_t ctx, int64_t H, kvc_stream_t stream);
+
+/* ---- paged caches: requests of different lengths that come and go --------------------------------------------
+ * No counterpart in the reference, whose caches are rectangular.  A pool holds n_pages pages of page_size tokens; request
+ * b's token t lies in page table[b][t / page_size], row t % page_size; slot = page * page_size + row.  Keys and values are
+ * fp16 or bf16, [page, row, KV head, channel] with the channels next to each other and any strides besides.  free_pages is a stack:
+ * its first head[0] entries are taken.  Lengths, tables, free list and counters live on the device, so that a decode step can
+ * be captured into a graph.  Arguments are passed in memory (8-byte words, then 32-bit ones, in this order).  status may be
+ * null: conditions are not reported then. */
+#define KVC_TYPE_FP16 0
+#define KVC_TYPE_BF16 1
+
+/* Pages for the new_tokens[b] tokens that a step brings behind the lengths[b] tokens of each request.  Request b needs
+ * need[b] = ceil((length + new) / page_size) - ceil(length / page_size) pages more; they come from the free list in request order.
+ * It is served if its pages fit its table row, its tokens fit the `tokens` rows, and need[b] = 0 or head + need[0] + .. + need[b] <= n_pages (the
+ * needs of requests whose row or tokens do not fit do not count); one that is refused keeps its length and raises
+ * KVC_FLAG_NO_PAGES.  Negative lengths and counts are taken as 0.
+ *   starts[B + 1]    the requests' first token rows, served or not: exclusive sums of new_tokens, `tokens` at most
+ *   taken[B]         where in the free list a served request's new pages begin; -1: refused
+ *   lengths_out[B], head_out[1]   behind the step; may be lengths and head
+ *   table            gets the entries of the new pages, nothing else is touched
+ *   slots, positions [tokens]     of token row n of request b: its slot (-1: refused), its position lengths[b] + n - starts[b];
+ *                    rows behind the last request's: -1 and 0 */
+typedef struct {
+    const int32_t *lengths, *new_tokens, *free_pages, *head;
+    int32_t *table;
+    int64_t table_stride, table_width;   /* entries from row to row, entries of a row */
+    int64_t B, n_pages, page_size, tokens;
+    int32_t *lengths_out, *head_out, *starts, *taken, *slots, *positions;
+    int32_t *status;
+} kvc_page_plan_args;
+int kvc_page_plan(const kvc_page_plan_args *args, kvc_stream_t stream);
+
+/* The way back: the pages of every request with done[b] != 0 go to free_pages[head - R .. head - 1] (R of them, in request order), its
+ * length becomes 0, head_out = head - R.  Should R exceed head, the requests behind the last whose pages still fit keep theirs
+ * (KVC_FLAG_NO_PAGES).  lengths_out and head_out may be lengths and head.  first: B + 1 words of scratch. */
+typedef struct {
+    const int32_t *lengths;
+    const uint8_t *done;
+    const int32_t *table;
+    int64_t table_stride, table_width;
+    int32_t *free_pages;
+    const int32_t *head;
+    int64_t B, n_pages, page_size;
+    int32_t *lengths_out, *head_out, *first;
+    int32_t *status;
+} kvc_page_release_args;
+int kvc_page_release(const kvc_page_release_args *args, kvc_stream_t stream);
+
+/* Rotary positions, and the way of a step's keys and values into the pool.  Of a head's D channels the first `rotary` (even) are
+ * rotated in pairs by angle = positions[n] * frequencies[i] (fp64, so that far positions keep their angle): with layout
+ * KVC_ROTARY_HALF channels i and i + rotary / 2, with KVC_ROTARY_INTERLEAVED 2i and 2i + 1; cos and sin are multiplied with `factor`;
+ * inverse != 0 turns the other way.  Computed in fp32, rounded once.  Channels behind them are copied.  rotary = 0: all are.
+ *   q [N, Hq, D] -> q_out, which may be q; Hq = 0: none.
+ *   k, v [N, Hkv, D] -> the rows `slots` of the pools, k rotated and v not; Hkv = 0: none.  A slot below 0 is not stored, one
+ *   behind the pool raises KVC_FLAG_BAD_PAGE and is not stored.  Of two tokens with one slot either may be what stays.
+ * Strides count elements; channels are next to each other.  frequencies: rotary / 2 of them. */
+#define KVC_ROTARY_HALF 0
+#define KVC_ROTARY_INTERLEAVED 1
+typedef struct {
+    const void *q, *k, *v;
+    void *q_out, *kpages, *vpages;
+    const int32_t *positions, *slots;
+    const double *frequencies;
+    int64_t N, Hq, Hkv, D, rotary, n_pages, page_size;
+    int64_t q_token, q_head, k_token, k_head, v_token, v_head, out_token, out_head;
+    int64_t kp_page, kp_row, kp_head, vp_page, vp_row, vp_head;
+    int32_t *status;
+    int32_t layout, inverse, type;
+    float factor;
+} kvc_rotary_args;
+int kvc_rotary_store(const kvc_rotary_args *args, kvc_stream_t stream);
+
+/* One new token per request over its pages: with s_t = scaling * (q . k_t) over the tokens t < lengths[b] (with window > 0 only the last
+ * `window` of them), out = sum exp(s_t) v_t / sum exp(s_t) and lse = log sum exp(s_t) (fp32 [B, Hq], may be null).  No
+ * tokens: out = 0, lse = -inf.  q, out: [B, Hq, D], D 64, 96, 128 or 256, query head h reads KV head h / (Hq / Hkv).  Rows of q and of the
+ * pools start on 16 bytes (pointers and strides).  Tokens behind a length are never read.
+ * workspace: kvc_paged_attn_workspace() bytes, 16-byte aligned, zeroed once before its first use; every call leaves what has to be zero at zero.  A workspace
+ * serves one launch at a time: concurrent streams need their own. */
+typedef struct {
+    const void *q, *kpages, *vpages;
+    const int32_t *table, *lengths;
+    void *out;
+    float *lse;
+    void *workspace;
+    int64_t workspace_bytes, B, Hq, Hkv, D, n_pages, page_size, table_stride, table_width, window;
+    int64_t q_token, q_head, out_token, out_head;
+    int64_t kp_page, kp_row, kp_head, vp_page, vp_row, vp_head;
+    int32_t *status;
+    float scaling;
+    int32_t type;
+} kvc_paged_attn_args;
+int64_t kvc_paged_attn_workspace(int64_t B, int64_t Hq, int64_t Hkv, int64_t D);
+int kvc_paged_attn(const kvc_paged_attn_args *args, kvc_stream_t stream);
 
 #ifdef __cplusplus
 }

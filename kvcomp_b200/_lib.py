@@ -13,13 +13,15 @@ FLAGS = {
     0x001: "ZERO_SCALE", 0x002: "MIN_OVERFLOW", 0x004: "CODE_OVERFLOW", 0x008: "SYMBOL_MISSING",
     0x010: "VECTOR_LONG", 0x020: "BLOCK_LONG", 0x040: "STREAM_FULL", 0x080: "BAD_STREAM",
     0x100: "CODE_TOO_LONG", 0x200: "NO_SYMBOLS", 0x400: "WAIT_TIMEOUT",
+    0x800: "NO_PAGES", 0x1000: "BAD_PAGE", 0x2000: "BAD_LENGTH",
 }
 FLAG_ZERO_SCALE, FLAG_MIN_OVERFLOW, FLAG_CODE_OVERFLOW, FLAG_SYMBOL_MISSING = 0x1, 0x2, 0x4, 0x8
 FLAG_VECTOR_LONG, FLAG_BLOCK_LONG, FLAG_STREAM_FULL, FLAG_BAD_STREAM = 0x10, 0x20, 0x40, 0x80
 FLAG_CODE_TOO_LONG, FLAG_NO_SYMBOLS, FLAG_WAIT_TIMEOUT = 0x100, 0x200, 0x400
+FLAG_NO_PAGES, FLAG_BAD_PAGE, FLAG_BAD_LENGTH = 0x800, 0x1000, 0x2000
 # conditions under which the produced data cannot be trusted (the rest are informational)
 FATAL_FLAGS = FLAG_CODE_OVERFLOW | FLAG_SYMBOL_MISSING | FLAG_BLOCK_LONG | FLAG_STREAM_FULL | \
-    FLAG_BAD_STREAM | FLAG_CODE_TOO_LONG | FLAG_NO_SYMBOLS | FLAG_WAIT_TIMEOUT
+    FLAG_BAD_STREAM | FLAG_CODE_TOO_LONG | FLAG_NO_SYMBOLS | FLAG_WAIT_TIMEOUT | FLAG_BAD_PAGE | FLAG_BAD_LENGTH
 
 MODE_BLOCK, MODE_CHANNEL, MODE_TOKEN, MODE_VECTOR = 0, 1, 2, 3
 
@@ -49,6 +51,13 @@ CACHE_FIELDS = "7q2i4q2i"
 KV_STORE_ARGS = struct.Struct("<11q")
 ATTN_ARGS = struct.Struct("<" + 2 * CACHE_FIELDS + "12qfi")
 STORE_ARGS = struct.Struct("<29q6ifi")
+PAGE_PLAN_ARGS = struct.Struct("<18q")
+PAGE_RELEASE_ARGS = struct.Struct("<14q")
+ROTARY_ARGS = struct.Struct("<31q3if")
+PAGED_ATTN_ARGS = struct.Struct("<29qfi")
+
+TYPE_FP16, TYPE_BF16 = 0, 1
+ROTARY_HALF, ROTARY_INTERLEAVED = 0, 1
 
 
 class KvcError(RuntimeError):
@@ -102,6 +111,11 @@ _SIGNATURES = {
     "kvc_attn_static_capacity": (_i64, []),
     "kvc_attn_decode_static": (_i32, [C.POINTER(Cache), C.POINTER(Cache), _i64, _i64, _i64, _i64, _vp, _f32, _vp, _vp,
                                       _i64, _vp, _i32, _vp, _vp]),
+    "kvc_page_plan": (_i32, [C.c_char_p, _vp]),
+    "kvc_page_release": (_i32, [C.c_char_p, _vp]),
+    "kvc_rotary_store": (_i32, [C.c_char_p, _vp]),
+    "kvc_paged_attn_workspace": (_i64, [_i64, _i64, _i64, _i64]),
+    "kvc_paged_attn": (_i32, [C.c_char_p, _vp]),
     "kvc_k_matvec": (_i32, [_vp, _vp, _vp, _i64, _i64, _vp]),
 }
 
