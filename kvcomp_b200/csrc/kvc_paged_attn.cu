@@ -2,73 +2,459 @@
 //
 // out = sum_t exp(s_t - m) v_t / sum_t exp(s_t - m) with s_t = scaling * q . k_t: one pass over the tokens with a running maximum m
 // and a running sum l; whenever the maximum grows, sum and accumulators are multiplied with exp(m_old - m_new).
+//
+// What bounds it: every key and value is read once and used for Hq / Hkv heads, 4 (Hq / Hkv) operations per 4 bytes: HBM, for any
+// number of heads that a model has.  Everything else is arranged so that the loads never pause:
+//
+// Work is cut into tiles of 64 tokens of a column (a request's KV head), all tiles of all columns in one row; each CTA takes an equal, contiguous
+// share of the row, found from the lengths in the kernel (the host does not know them).  Lengths may be as unequal as they like, and a
+// single long request is spread over the device.  A column that lies in one share is written at once; one that was cut leaves partial results {m, l,
+// sums} in the workspace, and the CTA that finishes last (a counter per column, put back to zero) joins them in the order of the shares, so that
+// the result does not depend on who that was.
+//
+// Four warps take 16 of a tile's tokens each, with a ring of stages of their own that they fill with 16-byte asynchronous copies (any strides,
+// pages that end anywhere) and drain without a barrier; the copies go on over the ends of columns.  The
+// block table's entries are asked for a tile ahead of the copies that need them.
+//
+// The products: 16 tokens x 8 heads, mma.m16n8k16 with the keys as the operand with 16 rows, and O^T = V^T P^T with 16 channels x 8
+// heads, so that few heads waste little.  (tcgen05 wants 64 rows and its operands in shared memory behind barriers of the whole CTA; here the tensor
+// work is a few per cent of the time that the bytes need.)  P is split into two 16-bit pieces, hi + lo, and multiplied twice: the weights keep 21
+// (fp16) or 16 bits (bf16), and the result is rounded once, at the end.  fp16 weights are carried times 2^14, so that the pieces of weights down to 2^-28
+// of the largest are normal numbers and many small ones are not lost.
 #include <cuda_bf16.h>
 #include <math_constants.h>
 #include <string.h>
+
+#include <algorithm>
 
 #include "kvc_common.cuh"
 
 namespace {
 
-template <typename T> __device__ __forceinline__ float to_float(T v);
-template <> __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
-template <> __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <typename T> __device__ __forceinline__ T from_float(float v);
-template <> __device__ __forceinline__ __half from_float(float v) { return __float2half_rn(v); }
-template <> __device__ __forceinline__ __nv_bfloat16 from_float(float v) { return __float2bfloat16_rn(v); }
+constexpr int WARPS = 4, THREADS = WARPS * 32;
+constexpr int TILE = 16 * WARPS;                // tokens of a tile
+constexpr int MAX_CTAS_PER_SM = 4;
+constexpr int MAX_GROUP = 16;                   // query heads that a column serves
 
-constexpr int WARPS = 4;
+struct Div { uint32_t magic, shift; };          // n / d of a divisor known to the host, n < 2^31
 
-// A CTA per (request, query head); its warps take every fourth token, a lane has D / 32 channels.
-template <typename T, int D>
-__global__ void __launch_bounds__(WARPS * 32) paged_attn_kernel(const kvc_paged_attn_args a) {
-    constexpr int E = D / 32;
-    __shared__ float acc_s[WARPS][D], m_s[WARPS], l_s[WARPS];
-    const int h = blockIdx.x, b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int hk = h / (int)(a.Hq / a.Hkv);
-    long long len = a.lengths[b];
-    if (len < 0 || len > a.table_width * a.page_size) {
-        if (threadIdx.x == 0 && a.status) atomicOr(a.status, KVC_FLAG_BAD_LENGTH);
-        len = len < 0 ? 0 : a.table_width * a.page_size;
-    }
-    const long long first = a.window > 0 && len > a.window ? len - a.window : 0;
-    float q[E], acc[E] = {}, m = -CUDART_INF_F, l = 0.0f;
-    for (int e = 0; e < E; e++) q[e] = to_float(reinterpret_cast<const T *>(a.q)[b * a.q_token + h * a.q_head + e * 32 + lane]);
-    for (long long t = first + warp; t < len; t += WARPS) {
-        const int page = a.table[b * a.table_stride + t / a.page_size];
-        if ((unsigned)page >= (unsigned long long)a.n_pages) {
-            if (lane == 0 && a.status) atomicOr(a.status, KVC_FLAG_BAD_PAGE);
-            continue;
-        }
-        const T *k = reinterpret_cast<const T *>(a.kpages) + page * a.kp_page + t % a.page_size * a.kp_row + hk * a.kp_head;
-        const T *v = reinterpret_cast<const T *>(a.vpages) + page * a.vp_page + t % a.page_size * a.vp_row + hk * a.vp_head;
-        float s = 0.0f;
-        for (int e = 0; e < E; e++) s += q[e] * to_float(k[e * 32 + lane]);
-        s = kvc_warp_sum(s) * a.scaling;
-        const float m_new = fmaxf(m, s), scale = m_new == -CUDART_INF_F ? 1.0f : __expf(m - m_new), p = m_new == -CUDART_INF_F ? 0.0f : __expf(s - m_new);
-        m = m_new;
-        l = l * scale + p;
-        for (int e = 0; e < E; e++) acc[e] = acc[e] * scale + p * to_float(v[e * 32 + lane]);
-    }
-    for (int e = 0; e < E; e++) acc_s[warp][e * 32 + lane] = acc[e];
-    if (lane == 0) { m_s[warp] = m; l_s[warp] = l; }
-    __syncthreads();
-    float top = -CUDART_INF_F, sum = 0.0f;
-    for (int w = 0; w < WARPS; w++) top = fmaxf(top, m_s[w]);
-    for (int w = 0; w < WARPS; w++) sum += m_s[w] == -CUDART_INF_F ? 0.0f : l_s[w] * __expf(m_s[w] - top);
-    for (int d = threadIdx.x; d < D; d += WARPS * 32) {
-        float o = 0.0f;
-        for (int w = 0; w < WARPS; w++) o += m_s[w] == -CUDART_INF_F ? 0.0f : acc_s[w][d] * __expf(m_s[w] - top);
-        reinterpret_cast<T *>(a.out)[b * a.out_token + h * a.out_head + d] = from_float<T>(sum == 0.0f ? 0.0f : o / sum);
-    }
-    if (threadIdx.x == 0 && a.lse) a.lse[b * a.Hq + h] = sum == 0.0f ? -CUDART_INF_F : top + logf(sum);
+Div make_div(uint32_t d) {
+    Div r;
+    r.shift = 0;
+    while ((1ull << r.shift) < d) r.shift++;
+    r.magic = (uint32_t)(((1ull << 32) * ((1ull << r.shift) - d)) / d + 1);
+    return r;
 }
+__device__ __forceinline__ int divide(int n, const Div &d) { return (int)((__umulhi(d.magic, (uint32_t)n) + (uint32_t)n) >> d.shift); }
+
+struct Params {
+    kvc_paged_attn_args a;
+    Div page;
+    int group, columns, per_head;               // query heads of a column at most, columns of a request, columns of a KV head
+    float log2_scaling;
+    unsigned *counters;
+    float *parts;
+};
+
+template <typename T> struct Pair;
+template <> struct Pair<__half> {
+    static constexpr float LIFT = 14.0f;
+    static __device__ __forceinline__ uint32_t pack(float a, float b) { const __half2 r = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t *>(&r); }
+    static __device__ __forceinline__ float2 unpack(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2 *>(&v)); }
+    static __device__ __forceinline__ __half one(float a) { return __float2half_rn(a); }
+    static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
+};
+template <> struct Pair<__nv_bfloat16> {
+    static constexpr float LIFT = 0.0f;
+    static __device__ __forceinline__ uint32_t pack(float a, float b) { const __nv_bfloat162 r = __floats2bfloat162_rn(a, b); return *reinterpret_cast<const uint32_t *>(&r); }
+    static __device__ __forceinline__ float2 unpack(uint32_t v) { return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&v)); }
+    static __device__ __forceinline__ __nv_bfloat16 one(float a) { return __float2bfloat16_rn(a); }
+    static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
+};
+
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+// 16 bytes to shared memory, zeros when `on` is false (nothing is read then)
+__device__ __forceinline__ void copy16(uint32_t to, const void *from, bool on) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(on ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ float exp2_approx(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+// where a 16-byte piece of a row lies in a stage: the 8 rows of a matrix load fall on different banks
+template <int D> __device__ __forceinline__ uint32_t piece_at(int row, int piece) {
+    if constexpr (D % 64 == 0) return (uint32_t)(row * (D / 8) + (piece ^ (row & 7))) * 16;       // rows start on bank 0
+    else return (uint32_t)(row * (D / 8) + (piece ^ ((row >> 1) & 3))) * 16;                        // D = 96: every other row starts in the middle
+}
+
+// The tokens of a request that count: [first, len)
+struct Span { int first, len; };
+__device__ __forceinline__ Span span_of(const kvc_paged_attn_args &a, int b, int &flags) {
+    int len = a.lengths[b];
+    const int most = (int)(a.table_width * a.page_size);
+    if (len < 0 || len > most) { flags |= KVC_FLAG_BAD_LENGTH; len = len < 0 ? 0 : most; }
+    Span s;
+    s.len = len;
+    s.first = a.window > 0 && len > a.window ? len - (int)a.window : 0;
+    return s;
+}
+__device__ __forceinline__ int tiles_of(const Span &s) { return (s.len - s.first + TILE - 1) / TILE; }
+
+// A place in the row of tiles: tile `i` of column `c` of request `b`
+struct Place { int b, c, i, n; Span span; };
+__device__ __forceinline__ void next_tile(const kvc_paged_attn_args &a, int columns, Place &p) {
+    if (++p.i < p.n) return;
+    p.i = 0;
+    if (++p.c < columns) return;
+    p.c = 0;
+    int unused = 0;
+    p.n = 0;
+    while (++p.b < a.B) {
+        p.span = span_of(a, p.b, unused);
+        if ((p.n = tiles_of(p.span)) > 0) return;
+    }
+}
+
+template <typename T, int D, int NT, int STAGES>
+__global__ void __launch_bounds__(THREADS) paged_attn_kernel(const __grid_constant__ Params p) {
+    constexpr int KS = D / 16;                              // steps of 16 channels
+    constexpr uint32_t HALF_STAGE = 16 * D * 2, STAGE = 2 * HALF_STAGE;
+    constexpr float LIFT = Pair<T>::LIFT;
+    extern __shared__ __align__(128) uint8_t smem[];        // [warp][stage]: 16 rows of keys, 16 of values
+    __shared__ uint32_t masks[WARPS][STAGES];
+    __shared__ float m_s[WARPS][8 * NT], l_s[WARPS][8 * NT];
+    __shared__ long long scan_s[WARPS];
+    __shared__ Place start_s;
+    __shared__ int last_s;
+    const kvc_paged_attn_args &a = p.a;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, B = (int)a.B;
+    int flags = 0;
+
+    // ---- this CTA's share
+    long long r0, r1, total, shares;
+    {
+        const int chunk = (B + THREADS - 1) / THREADS, b0 = min(B, tid * chunk), b1 = min(B, b0 + chunk);
+        long long mine = 0;
+        for (int b = b0; b < b1; b++) mine += tiles_of(span_of(a, b, flags));
+        long long upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long u = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += u;
+        }
+        if (lane == 31) scan_s[warp] = upto;
+        __syncthreads();
+        long long before = 0, all = 0;
+        for (int w = 0; w < WARPS; w++) {
+            if (w < warp) before += scan_s[w];
+            all += scan_s[w];
+        }
+        before += upto - mine;
+        total = all * p.columns;
+        shares = min((long long)gridDim.x, total);          // none is empty
+        r0 = blockIdx.x < shares ? total * blockIdx.x / shares : total;
+        r1 = blockIdx.x < shares ? total * (blockIdx.x + 1) / shares : total;
+        if (r0 >= before * p.columns && r0 < (before + mine) * p.columns) {
+            Place at;
+            int unused = 0;
+            long long rest = r0 - before * p.columns;
+            for (at.b = b0; ; at.b++) {
+                at.span = span_of(a, at.b, unused);
+                at.n = tiles_of(at.span);
+                if (rest < (long long)at.n * p.columns) break;
+                rest -= (long long)at.n * p.columns;
+            }
+            at.c = (int)(rest / at.n);
+            at.i = (int)(rest % at.n);
+            start_s = at;
+        }
+        __syncthreads();
+    }
+    // requests without tokens
+    for (int b = blockIdx.x; b < B; b += gridDim.x) {
+        if (tiles_of(span_of(a, b, flags)) > 0) continue;
+        for (int i = tid; i < (int)a.Hq * (D / 8); i += THREADS)
+            *reinterpret_cast<uint4 *>(reinterpret_cast<T *>(a.out) + b * a.out_token + i / (D / 8) * a.out_head + i % (D / 8) * 8) = make_uint4(0, 0, 0, 0);
+        if (a.lse) for (int h = tid; h < (int)a.Hq; h += THREADS) a.lse[b * a.Hq + h] = -CUDART_INF_F;
+    }
+    if (r0 >= r1) {
+        if (flags && a.status) atomicOr(a.status, flags);
+        return;
+    }
+
+    // ---- the copies
+    Place ahead = start_s;
+    long long to_copy = r1 - r0;
+    int page = -1;                                          // lanes 0 .. 15: the page of their token of the tile that is copied next
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * STAGES * STAGE;
+    auto ask = [&]() {
+        page = -1;
+        if (to_copy > 0 && lane < 16) {
+            const int t = ahead.span.first + ahead.i * TILE + warp * 16 + lane;
+            if (t < ahead.span.len) page = __ldg(a.table + ahead.b * a.table_stride + divide(t, p.page));
+        }
+    };
+    auto copy_tile = [&](int stage) {
+        if (to_copy > 0) {
+            const int t = ahead.span.first + ahead.i * TILE + warp * 16 + lane;
+            const bool there = lane < 16 && t < ahead.span.len, good = there && (unsigned long long)(unsigned)page < (unsigned long long)a.n_pages;
+            if (there && !good) flags |= KVC_FLAG_BAD_PAGE;
+            const uint32_t mask = __ballot_sync(0xffffffffu, good);
+            if (lane == 0) masks[warp][stage] = mask;
+            if (mask) {
+                const int hk = ahead.c / p.per_head, row = t - divide(t, p.page) * (int)a.page_size;
+                const long long ko = good ? page * a.kp_page + row * a.kp_row + hk * a.kp_head : 0, vo = good ? page * a.vp_page + row * a.vp_row + hk * a.vp_head : 0;
+                const uint32_t to = ring + stage * STAGE;
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const int r = 4 * j + (lane >> 3);
+                    const bool on = mask >> r & 1;
+                    const T *k = reinterpret_cast<const T *>(a.kpages) + __shfl_sync(0xffffffffu, ko, r), *v = reinterpret_cast<const T *>(a.vpages) + __shfl_sync(0xffffffffu, vo, r);
+#pragma unroll
+                    for (int c = 0; c < (D / 8 + 7) / 8; c++) {
+                        const int piece = c * 8 + (lane & 7);
+                        if ((D / 8) % 8 == 0 || piece < D / 8) {
+                            copy16(to + piece_at<D>(r, piece), k + piece * 8, on);
+                            copy16(to + HALF_STAGE + piece_at<D>(r, piece), v + piece * 8, on);
+                        }
+                    }
+                }
+            }
+            next_tile(a, p.columns, ahead);
+            to_copy--;
+        }
+        copies_commit();
+        ask();
+    };
+    ask();
+#pragma unroll 1
+    for (int s = 0; s < STAGES; s++) copy_tile(s);
+
+    // ---- the tiles
+    Place at = start_s;
+    long long left = r1 - r0;
+    int stage = 0;
+    const uint32_t kv_row = lane & 15, kv_piece = lane >> 4;                                // keys: 16 rows, two pieces
+    const uint32_t v_row = (lane & 7) + (lane >> 4) * 8, v_piece = lane >> 3 & 1;           // values: two pieces, 16 rows, transposed
+    while (left > 0) {
+        const int seg = (int)min((long long)(at.n - at.i), left), h0 = at.c / p.per_head * (int)(a.Hq / a.Hkv) + at.c % p.per_head * p.group;
+        const int heads = min(p.group, (int)(a.Hq / a.Hkv) - at.c % p.per_head * p.group);
+        uint32_t q[KS][NT][2];
+        float o[KS][NT][4], m[NT][2], l[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            const int h = nt * 8 + (lane >> 2);
+            const T *from = reinterpret_cast<const T *>(a.q) + at.b * a.q_token + (h0 + h) * a.q_head + (lane & 3) * 2;
+#pragma unroll
+            for (int k = 0; k < KS; k++) {
+                q[k][nt][0] = h < heads ? *reinterpret_cast<const uint32_t *>(from + k * 16) : 0;
+                q[k][nt][1] = h < heads ? *reinterpret_cast<const uint32_t *>(from + k * 16 + 8) : 0;
+                o[k][nt][0] = o[k][nt][1] = o[k][nt][2] = o[k][nt][3] = 0.0f;
+            }
+            m[nt][0] = m[nt][1] = -CUDART_INF_F;
+            l[nt][0] = l[nt][1] = 0.0f;
+        }
+        uint32_t scratch = 0;
+        for (int j = 0; j < seg; j++) {
+            copies_wait<STAGES - 1>();
+            __syncwarp();
+            const uint32_t mask = masks[warp][stage], keys = ring + stage * STAGE, values = keys + HALF_STAGE;
+            if (mask) {
+                float s[2][NT][4] = {};
+#pragma unroll
+                for (int k = 0; k < KS; k++) {
+                    uint32_t f[4];
+                    ldmatrix4(f, keys + piece_at<D>(kv_row, 2 * k + kv_piece));
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) Pair<T>::mma(s[k & 1][nt], f, q[k][nt][0], q[k][nt][1]);
+                }
+                const bool on0 = mask >> (lane >> 2) & 1, on1 = mask >> (8 + (lane >> 2)) & 1;
+                float scale[NT][2];
+                bool grows = false;
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) s[0][nt][e] = (e < 2 ? on0 : on1) ? (s[0][nt][e] + s[1][nt][e]) * p.log2_scaling : -CUDART_INF_F;
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        float top = fmaxf(s[0][nt][e], s[0][nt][e + 2]);
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                        top = fmaxf(top, m[nt][e]);
+                        grows |= top > m[nt][e];
+                        const float base = top == -CUDART_INF_F ? 0.0f : top;
+                        scale[nt][e] = exp2_approx(m[nt][e] - base);
+                        m[nt][e] = top;
+                        s[0][nt][e] = exp2_approx(s[0][nt][e] - base + LIFT);
+                        s[0][nt][e + 2] = exp2_approx(s[0][nt][e + 2] - base + LIFT);
+                        l[nt][e] = l[nt][e] * scale[nt][e] + s[0][nt][e] + s[0][nt][e + 2];
+                    }
+                }
+                if (__any_sync(0xffffffffu, grows)) {
+#pragma unroll
+                    for (int k = 0; k < KS; k++)
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++) {
+                            o[k][nt][0] *= scale[nt][0]; o[k][nt][1] *= scale[nt][1];
+                            o[k][nt][2] *= scale[nt][0]; o[k][nt][3] *= scale[nt][1];
+                        }
+                }
+                uint32_t hi[NT][2], lo[NT][2];
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const uint32_t top = Pair<T>::pack(s[0][nt][2 * e], s[0][nt][2 * e + 1]);
+                        const float2 f = Pair<T>::unpack(top);
+                        hi[nt][e] = transpose8x8(top);
+                        lo[nt][e] = transpose8x8(Pair<T>::pack(s[0][nt][2 * e] - f.x, s[0][nt][2 * e + 1] - f.y));
+                    }
+#pragma unroll
+                for (int k = 0; k < KS; k++) {
+                    uint32_t f[4];
+                    ldmatrix4_trans(f, values + piece_at<D>(v_row, 2 * k + v_piece));
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) {
+                        Pair<T>::mma(o[k][nt], f, hi[nt][0], hi[nt][1]);
+                        Pair<T>::mma(o[k][nt], f, lo[nt][0], lo[nt][1]);
+                    }
+                }
+            }
+            __syncwarp();                                   // everyone has read the stage
+            if (j < seg - 1) copy_tile(stage);
+            else scratch = stage * STAGE;                   // the column's last stage of this CTA holds the warp's sums until they are joined
+            stage = stage + 1 == STAGES ? 0 : stage + 1;
+        }
+        // ---- the warps' results of this column joined
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                float v = l[nt][e];
+                v += __shfl_xor_sync(0xffffffffu, v, 4);
+                v += __shfl_xor_sync(0xffffffffu, v, 8);
+                v += __shfl_xor_sync(0xffffffffu, v, 16);
+                const int h = nt * 8 + (lane & 3) * 2 + e;
+                if (lane < 4) { m_s[warp][h] = m[nt][e]; l_s[warp][h] = v; }
+                if (h < heads) {
+                    float *to = reinterpret_cast<float *>(smem + warp * STAGES * STAGE + scratch) + h * D;
+#pragma unroll
+                    for (int k = 0; k < KS; k++) {
+                        to[(k * 16 + (lane >> 2)) ^ ((h >> 1 & 3) * 8)] = o[k][nt][e];
+                        to[(k * 16 + 8 + (lane >> 2)) ^ ((h >> 1 & 3) * 8)] = o[k][nt][e + 2];
+                    }
+                }
+            }
+        __syncthreads();
+        const bool whole = seg == at.n;                     // the column lies in this share
+        const long long begin = r1 - left - at.i;           // the column's first tile in the row
+        const int w_first = (int)(((begin + 1) * shares - 1) / total), w_last = (int)(((begin + at.n) * shares - 1) / total);
+        const int slot_floats = MAX_GROUP * (D + 2);
+        float *part = p.parts + (2ll * blockIdx.x + (left != r1 - r0)) * slot_floats;
+        for (int i = tid; i < heads * D; i += THREADS) {
+            const int h = i / D, d = i % D;
+            float top = m_s[0][h], sum = 0.0f, v = 0.0f;
+#pragma unroll
+            for (int w = 1; w < WARPS; w++) top = fmaxf(top, m_s[w][h]);
+            const float base = top == -CUDART_INF_F ? 0.0f : top;
+#pragma unroll
+            for (int w = 0; w < WARPS; w++) {
+                const float f = exp2_approx(m_s[w][h] - base);
+                sum += f * l_s[w][h];
+                v += f * reinterpret_cast<const float *>(smem + w * STAGES * STAGE + scratch)[h * D + (d ^ ((h >> 1 & 3) * 8))];
+            }
+            if (whole) {
+                reinterpret_cast<T *>(a.out)[at.b * a.out_token + (h0 + h) * a.out_head + d] = Pair<T>::one(sum == 0.0f ? 0.0f : v / sum);
+                if (d == 0 && a.lse) a.lse[at.b * a.Hq + h0 + h] = sum == 0.0f ? -CUDART_INF_F : (top + log2f(sum) - LIFT) * 0.69314718055994531f;
+            } else {
+                __stcg(part + MAX_GROUP * 2 + i, v);
+                if (d == 0) __stcg(reinterpret_cast<float2 *>(part) + h, make_float2(top, sum));
+            }
+        }
+        __syncthreads();
+        if (!whole) {
+            const long long column = (long long)at.b * p.columns + at.c;
+            if (tid == 0) {
+                __threadfence();
+                last_s = atomicAdd(p.counters + column, 1u) == (unsigned)(w_last - w_first);
+                __threadfence();
+            }
+            __syncthreads();
+            if (last_s) {                                   // all parts are there: joined in the order of the shares
+                if (tid == 0) p.counters[column] = 0;
+                const float *first = p.parts + (2ll * w_first + (begin > total * w_first / shares)) * slot_floats;
+                for (int i = tid; i < heads * D; i += THREADS) {
+                    const int h = i / D, d = i % D;
+                    float top = -CUDART_INF_F, sum = 0.0f, v = 0.0f;
+                    for (int w = w_first; w <= w_last; w++) {
+                        const float *from = w == w_first ? first : p.parts + 2ll * w * slot_floats;
+                        const float2 ml = __ldcg(reinterpret_cast<const float2 *>(from) + h);
+                        const float x = __ldcg(from + MAX_GROUP * 2 + i), now = fmaxf(top, ml.x), base = now == -CUDART_INF_F ? 0.0f : now;
+                        const float f = exp2_approx(top - base), g = exp2_approx(ml.x - base);
+                        sum = sum * f + ml.y * g;
+                        v = v * f + x * g;
+                        top = now;
+                    }
+                    reinterpret_cast<T *>(a.out)[at.b * a.out_token + (h0 + h) * a.out_head + d] = Pair<T>::one(sum == 0.0f ? 0.0f : v / sum);
+                    if (d == 0 && a.lse) a.lse[at.b * a.Hq + h0 + h] = sum == 0.0f ? -CUDART_INF_F : (top + log2f(sum) - LIFT) * 0.69314718055994531f;
+                }
+            }
+        }
+        copy_tile(stage == 0 ? STAGES - 1 : stage - 1);     // (everyone has read the sums)
+        left -= seg;
+        at.i += seg - 1;
+        if (left > 0) next_tile(a, p.columns, at);
+    }
+    copies_wait<0>();
+    if (flags && a.status) atomicOr(a.status, flags);
+}
+
+template <typename T, int D, int NT, int STAGES>
+int launch(const Params &p, long long most_tiles, cudaStream_t stream) {
+    static kvc_launch_slot slot;
+    constexpr size_t shared = (size_t)WARPS * STAGES * 64 * D;
+    auto *kernel = paged_attn_kernel<T, D, NT, STAGES>;
+    int occ = 0;
+    if (int rc = kvc_prepare(slot, reinterpret_cast<const void *>(kernel), THREADS, shared, &occ)) return rc;
+    KVC_REQUIRE(occ > 0, "kvc_paged_attn: the kernel does not fit this device");
+    const long long grid = std::min<long long>(most_tiles, (long long)std::min(occ, MAX_CTAS_PER_SM) * kvc_sm_count());
+    kernel<<<(unsigned)std::max<long long>(grid, 1), THREADS, shared, stream>>>(p);
+    KVC_LAUNCH_OK();
+    return KVC_OK;
+}
+
+// query heads that a column takes at most: 16 where they fit the registers beside the accumulators
+int group_of(int64_t Hq, int64_t Hkv, int64_t D) { return (int)std::min<int64_t>(Hq / Hkv, D > 128 ? 8 : MAX_GROUP); }
+int64_t columns_of(int64_t Hq, int64_t Hkv, int64_t D) { return Hkv * ((Hq / Hkv + group_of(Hq, Hkv, D) - 1) / group_of(Hq, Hkv, D)); }
+int64_t counter_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t D) { return (B * columns_of(Hq, Hkv, D) * 4 + 255) / 256 * 256; }
 
 }  // namespace
 
+// a counter per column; two partial results for every CTA that the device holds
 extern "C" int64_t kvc_paged_attn_workspace(int64_t B, int64_t Hq, int64_t Hkv, int64_t D) {
-    if (B < 0 || Hq <= 0 || Hkv <= 0 || D <= 0) return 0;
-    return 256;
+    if (B < 0 || Hkv <= 0 || Hq < Hkv || D <= 0) return 0;
+    return counter_bytes(B, Hq, Hkv, D) + 2ll * MAX_CTAS_PER_SM * kvc_sm_count() * MAX_GROUP * (D + 2) * 4;
 }
 
 extern "C" int kvc_paged_attn(const kvc_paged_attn_args *args, kvc_stream_t stream) {
@@ -81,7 +467,7 @@ extern "C" int kvc_paged_attn(const kvc_paged_attn_args *args, kvc_stream_t stre
     KVC_REQUIRE(a.page_size > 0 && a.page_size <= (1 << 20) && a.n_pages >= 0 && a.n_pages < (1ll << 31) && a.table_width >= 0 && a.window >= 0, "kvc_paged_attn: bad sizes");
     KVC_REQUIRE(a.table_width * a.page_size < (1ll << 31), "kvc_paged_attn: a table row holds %lld tokens, lengths have 32 bits", (long long)(a.table_width * a.page_size));
     if (a.B == 0) return KVC_OK;
-    KVC_REQUIRE(a.B < 65536, "kvc_paged_attn: %lld requests", (long long)a.B);
+    KVC_REQUIRE(a.B < (1 << 24), "kvc_paged_attn: %lld requests", (long long)a.B);
     KVC_REQUIRE(a.q && a.out && a.lengths && (a.table || a.table_width == 0) && ((a.kpages && a.vpages) || a.n_pages == 0), "kvc_paged_attn: null pointer");
     const uintptr_t at = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.kpages) | reinterpret_cast<uintptr_t>(a.vpages) | reinterpret_cast<uintptr_t>(a.out);
     if (a.Hq == 1) a.q_head = a.out_head = 0;              // (the stride of a dimension of one may be anything)
@@ -96,14 +482,26 @@ extern "C" int kvc_paged_attn(const kvc_paged_attn_args *args, kvc_stream_t stre
         kvc_set_error("kvc_paged_attn: the workspace must hold what kvc_paged_attn_workspace says");
         return KVC_ERR_CAPACITY;
     }
-    const dim3 grid((unsigned)a.Hq, (unsigned)a.B);
-#define KVC_PA(T_, D_) paged_attn_kernel<T_, D_><<<grid, WARPS * 32, 0, kvc_cu(stream)>>>(a)
-    if (a.type == KVC_TYPE_FP16) {
-        if (a.D == 64) KVC_PA(__half, 64); else if (a.D == 96) KVC_PA(__half, 96); else if (a.D == 128) KVC_PA(__half, 128); else KVC_PA(__half, 256);
-    } else {
-        if (a.D == 64) KVC_PA(__nv_bfloat16, 64); else if (a.D == 96) KVC_PA(__nv_bfloat16, 96); else if (a.D == 128) KVC_PA(__nv_bfloat16, 128); else KVC_PA(__nv_bfloat16, 256);
+    Params p;
+    p.a = a;
+    p.page = make_div((uint32_t)a.page_size);
+    p.group = group_of(a.Hq, a.Hkv, a.D);
+    p.columns = (int)columns_of(a.Hq, a.Hkv, a.D);
+    p.per_head = p.columns / (int)a.Hkv;
+    p.log2_scaling = a.scaling * 1.4426950408889634f;
+    p.counters = reinterpret_cast<unsigned *>(a.workspace);
+    p.parts = reinterpret_cast<float *>(reinterpret_cast<uint8_t *>(a.workspace) + counter_bytes(a.B, a.Hq, a.Hkv, a.D));
+    const long long most = a.B * p.columns * ((a.table_width * a.page_size + TILE - 1) / TILE);
+    cudaStream_t s = kvc_cu(stream);
+    const bool wide = p.group > 8;
+#define KVC_PA(T_)                                                                                                             \
+    switch (a.D) {                                                                                                             \
+        case 64: return wide ? launch<T_, 64, 2, 6>(p, most, s) : launch<T_, 64, 1, 6>(p, most, s);                            \
+        case 96: return wide ? launch<T_, 96, 2, 4>(p, most, s) : launch<T_, 96, 1, 4>(p, most, s);                            \
+        case 128: return wide ? launch<T_, 128, 2, 3>(p, most, s) : launch<T_, 128, 1, 3>(p, most, s);                         \
+        default: return launch<T_, 256, 1, 3>(p, most, s);                                                                     \
     }
+    if (a.type == KVC_TYPE_FP16) KVC_PA(__half)
+    KVC_PA(__nv_bfloat16)
 #undef KVC_PA
-    KVC_LAUNCH_OK();
-    return KVC_OK;
 }
