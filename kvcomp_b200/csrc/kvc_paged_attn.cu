@@ -34,6 +34,12 @@ namespace {
 constexpr int WARPS = 4, THREADS = WARPS * 32;
 constexpr int TILE = 16 * WARPS;                // tokens of a tile
 constexpr int MAX_CTAS_PER_SM = 4;
+#ifndef KVC_MIN_TILES
+#define KVC_MIN_TILES 2
+#endif
+#ifndef KVC_S128
+#define KVC_S128 3
+#endif
 constexpr int MAX_GROUP = 16;                   // query heads that a column serves
 
 struct Div { uint32_t magic, shift; };          // n / d of a divisor known to the host, n < 2^31
@@ -51,6 +57,8 @@ struct Params {
     kvc_paged_attn_args a;
     Div page;
     int group, columns, per_head;               // query heads of a column at most, columns of a request, columns of a KV head
+    int most_tokens;                            // of a table row
+    unsigned n_pages;
     float log2_scaling;
     unsigned *counters;
     float *parts;
@@ -109,29 +117,28 @@ template <int D> __device__ __forceinline__ uint32_t piece_at(int row, int piece
 
 // The tokens of a request that count: [first, len)
 struct Span { int first, len; };
-__device__ __forceinline__ Span span_of(const kvc_paged_attn_args &a, int b, int &flags) {
-    int len = a.lengths[b];
-    const int most = (int)(a.table_width * a.page_size);
-    if (len < 0 || len > most) { flags |= KVC_FLAG_BAD_LENGTH; len = len < 0 ? 0 : most; }
+__device__ __forceinline__ Span span_of(const Params &p, int b, int &flags) {
+    int len = p.a.lengths[b];
+    if (len < 0 || len > p.most_tokens) { flags |= KVC_FLAG_BAD_LENGTH; len = len < 0 ? 0 : p.most_tokens; }
     Span s;
     s.len = len;
-    s.first = a.window > 0 && len > a.window ? len - (int)a.window : 0;
+    s.first = p.a.window > 0 && len > p.a.window ? len - (int)p.a.window : 0;
     return s;
 }
 __device__ __forceinline__ int tiles_of(const Span &s) { return (s.len - s.first + TILE - 1) / TILE; }
 
 // A place in the row of tiles: tile `i` of column `c` of request `b`
 struct Place { int b, c, i, n; Span span; };
-__device__ __forceinline__ void next_tile(const kvc_paged_attn_args &a, int columns, Place &p) {
-    if (++p.i < p.n) return;
-    p.i = 0;
-    if (++p.c < columns) return;
-    p.c = 0;
+__device__ __forceinline__ void next_tile(const Params &p, Place &at) {
+    if (++at.i < at.n) return;
+    at.i = 0;
+    if (++at.c < p.columns) return;
+    at.c = 0;
     int unused = 0;
-    p.n = 0;
-    while (++p.b < a.B) {
-        p.span = span_of(a, p.b, unused);
-        if ((p.n = tiles_of(p.span)) > 0) return;
+    at.n = 0;
+    while (++at.b < (int)p.a.B) {
+        at.span = span_of(p, at.b, unused);
+        if ((at.n = tiles_of(at.span)) > 0) return;
     }
 }
 
@@ -139,10 +146,13 @@ template <typename T, int D, int NT, int STAGES>
 __global__ void __launch_bounds__(THREADS) paged_attn_kernel(const __grid_constant__ Params p) {
     constexpr int KS = D / 16;                              // steps of 16 channels
     constexpr uint32_t HALF_STAGE = 16 * D * 2, STAGE = 2 * HALF_STAGE;
+    constexpr int PART = MAX_GROUP * (D + 2);               // floats of a partial result: maxima and sums, sums of values
     constexpr float LIFT = Pair<T>::LIFT;
     extern __shared__ __align__(128) uint8_t smem[];        // [warp][stage]: 16 rows of keys, 16 of values
     __shared__ uint32_t masks[WARPS][STAGES];
-    __shared__ float m_s[WARPS][8 * NT], l_s[WARPS][8 * NT];
+    __shared__ float2 ml_s[WARPS][8 * NT];                  // maximum and sum
+    __shared__ float4 join_v[THREADS];
+    __shared__ float2 join_ml[THREADS];
     __shared__ long long scan_s[WARPS];
     __shared__ Place start_s;
     __shared__ int last_s;
@@ -155,7 +165,7 @@ __global__ void __launch_bounds__(THREADS) paged_attn_kernel(const __grid_consta
     {
         const int chunk = (B + THREADS - 1) / THREADS, b0 = min(B, tid * chunk), b1 = min(B, b0 + chunk);
         long long mine = 0;
-        for (int b = b0; b < b1; b++) mine += tiles_of(span_of(a, b, flags));
+        for (int b = b0; b < b1; b++) mine += tiles_of(span_of(p, b, flags));
         long long upto = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -171,7 +181,7 @@ __global__ void __launch_bounds__(THREADS) paged_attn_kernel(const __grid_consta
         }
         before += upto - mine;
         total = all * p.columns;
-        shares = min((long long)gridDim.x, total);          // none is empty
+        shares = min((long long)gridDim.x, (total + KVC_MIN_TILES - 1) / KVC_MIN_TILES);          // none is empty
         r0 = blockIdx.x < shares ? total * blockIdx.x / shares : total;
         r1 = blockIdx.x < shares ? total * (blockIdx.x + 1) / shares : total;
         if (r0 >= before * p.columns && r0 < (before + mine) * p.columns) {
@@ -179,7 +189,7 @@ __global__ void __launch_bounds__(THREADS) paged_attn_kernel(const __grid_consta
             int unused = 0;
             long long rest = r0 - before * p.columns;
             for (at.b = b0; ; at.b++) {
-                at.span = span_of(a, at.b, unused);
+                at.span = span_of(p, at.b, unused);
                 at.n = tiles_of(at.span);
                 if (rest < (long long)at.n * p.columns) break;
                 rest -= (long long)at.n * p.columns;
@@ -192,7 +202,7 @@ __global__ void __launch_bounds__(THREADS) paged_attn_kernel(const __grid_consta
     }
     // requests without tokens
     for (int b = blockIdx.x; b < B; b += gridDim.x) {
-        if (tiles_of(span_of(a, b, flags)) > 0) continue;
+        if (tiles_of(span_of(p, b, flags)) > 0) continue;
         for (int i = tid; i < (int)a.Hq * (D / 8); i += THREADS)
             *reinterpret_cast<uint4 *>(reinterpret_cast<T *>(a.out) + b * a.out_token + i / (D / 8) * a.out_head + i % (D / 8) * 8) = make_uint4(0, 0, 0, 0);
         if (a.lse) for (int h = tid; h < (int)a.Hq; h += THREADS) a.lse[b * a.Hq + h] = -CUDART_INF_F;
@@ -217,12 +227,12 @@ __global__ void __launch_bounds__(THREADS) paged_attn_kernel(const __grid_consta
     auto copy_tile = [&](int stage) {
         if (to_copy > 0) {
             const int t = ahead.span.first + ahead.i * TILE + warp * 16 + lane;
-            const bool there = lane < 16 && t < ahead.span.len, good = there && (unsigned long long)(unsigned)page < (unsigned long long)a.n_pages;
+            const bool there = lane < 16 && t < ahead.span.len, good = there && (unsigned)page < p.n_pages;
             if (there && !good) flags |= KVC_FLAG_BAD_PAGE;
             const uint32_t mask = __ballot_sync(0xffffffffu, good);
             if (lane == 0) masks[warp][stage] = mask;
             if (mask) {
-                const int hk = ahead.c / p.per_head, row = t - divide(t, p.page) * (int)a.page_size;
+                const int hk = p.per_head == 1 ? ahead.c : ahead.c / p.per_head, row = t - divide(t, p.page) * (int)a.page_size;
                 const long long ko = good ? page * a.kp_page + row * a.kp_row + hk * a.kp_head : 0, vo = good ? page * a.vp_page + row * a.vp_row + hk * a.vp_head : 0;
                 const uint32_t to = ring + stage * STAGE;
 #pragma unroll
@@ -240,27 +250,22 @@ __global__ void __launch_bounds__(THREADS) paged_attn_kernel(const __grid_consta
                     }
                 }
             }
-            next_tile(a, p.columns, ahead);
+            next_tile(p, ahead);
             to_copy--;
         }
         copies_commit();
         ask();
     };
-    ask();
-#pragma unroll 1
-    for (int s = 0; s < STAGES; s++) copy_tile(s);
 
     // ---- the tiles
     Place at = start_s;
-    long long left = r1 - r0;
-    int stage = 0;
-    const uint32_t kv_row = lane & 15, kv_piece = lane >> 4;                                // keys: 16 rows, two pieces
-    const uint32_t v_row = (lane & 7) + (lane >> 4) * 8, v_piece = lane >> 3 & 1;           // values: two pieces, 16 rows, transposed
-    while (left > 0) {
-        const int seg = (int)min((long long)(at.n - at.i), left), h0 = at.c / p.per_head * (int)(a.Hq / a.Hkv) + at.c % p.per_head * p.group;
-        const int heads = min(p.group, (int)(a.Hq / a.Hkv) - at.c % p.per_head * p.group);
-        uint32_t q[KS][NT][2];
-        float o[KS][NT][4], m[NT][2], l[NT][2];
+    uint32_t q[KS][NT][2];
+    float o[KS][NT][4], m[NT][2], l[NT][2];
+    int h0 = 0, heads = 0;
+    auto begin_column = [&]() {                             // (the queries are asked for; they are first used behind the next wait)
+        const int hk = p.per_head == 1 ? at.c : at.c / p.per_head, g = (int)(a.Hq / a.Hkv), sub = (at.c - hk * p.per_head) * p.group;
+        h0 = hk * g + sub;
+        heads = min(p.group, g - sub);
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
             const int h = nt * 8 + (lane >> 2);
@@ -269,13 +274,28 @@ __global__ void __launch_bounds__(THREADS) paged_attn_kernel(const __grid_consta
             for (int k = 0; k < KS; k++) {
                 q[k][nt][0] = h < heads ? *reinterpret_cast<const uint32_t *>(from + k * 16) : 0;
                 q[k][nt][1] = h < heads ? *reinterpret_cast<const uint32_t *>(from + k * 16 + 8) : 0;
-                o[k][nt][0] = o[k][nt][1] = o[k][nt][2] = o[k][nt][3] = 0.0f;
             }
+        }
+    };
+    auto clear = [&]() {
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+            for (int k = 0; k < KS; k++) o[k][nt][0] = o[k][nt][1] = o[k][nt][2] = o[k][nt][3] = 0.0f;
             m[nt][0] = m[nt][1] = -CUDART_INF_F;
             l[nt][0] = l[nt][1] = 0.0f;
         }
-        uint32_t scratch = 0;
-        for (int j = 0; j < seg; j++) {
+    };
+    const long long share = r1 - r0;
+    const uint32_t kv_row = lane & 15, kv_piece = lane >> 4;                                // keys: 16 rows, two pieces
+    const uint32_t v_row = (lane & 7) + (lane >> 4) * 8, v_piece = lane >> 3 & 1;           // values: two pieces, 16 rows, transposed
+    int stage = 0, first_i = at.i;                          // first_i: the first tile of the column that is this CTA's
+    ask();
+    begin_column();
+    clear();
+#pragma unroll 1
+    for (long long n = -STAGES; n < share; n++) {
+        if (n >= 0) {
             copies_wait<STAGES - 1>();
             __syncwarp();
             const uint32_t mask = masks[warp][stage], keys = ring + stage * STAGE, values = keys + HALF_STAGE;
@@ -342,89 +362,147 @@ __global__ void __launch_bounds__(THREADS) paged_attn_kernel(const __grid_consta
                 }
             }
             __syncwarp();                                   // everyone has read the stage
-            if (j < seg - 1) copy_tile(stage);
-            else scratch = stage * STAGE;                   // the column's last stage of this CTA holds the warp's sums until they are joined
-            stage = stage + 1 == STAGES ? 0 : stage + 1;
-        }
-        // ---- the warps' results of this column joined
+            if (at.i == at.n - 1 || n == share - 1) {
+                // ---- the column's end in this share: the warps' results are joined; the stage just read holds their sums meanwhile
+                const uint32_t scratch = stage * STAGE;
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++)
+                for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-            for (int e = 0; e < 2; e++) {
-                float v = l[nt][e];
-                v += __shfl_xor_sync(0xffffffffu, v, 4);
-                v += __shfl_xor_sync(0xffffffffu, v, 8);
-                v += __shfl_xor_sync(0xffffffffu, v, 16);
-                const int h = nt * 8 + (lane & 3) * 2 + e;
-                if (lane < 4) { m_s[warp][h] = m[nt][e]; l_s[warp][h] = v; }
-                if (h < heads) {
-                    float *to = reinterpret_cast<float *>(smem + warp * STAGES * STAGE + scratch) + h * D;
+                    for (int e = 0; e < 2; e++) {
+                        float v = l[nt][e];
+                        v += __shfl_xor_sync(0xffffffffu, v, 4);
+                        v += __shfl_xor_sync(0xffffffffu, v, 8);
+                        v += __shfl_xor_sync(0xffffffffu, v, 16);
+                        const int h = nt * 8 + (lane & 3) * 2 + e;
+                        if (lane < 4) ml_s[warp][h] = make_float2(m[nt][e], v);
+                        if (h < heads) {
+                            float *to = reinterpret_cast<float *>(smem + warp * STAGES * STAGE + scratch) + h * D;
 #pragma unroll
-                    for (int k = 0; k < KS; k++) {
-                        to[(k * 16 + (lane >> 2)) ^ ((h >> 1 & 3) * 8)] = o[k][nt][e];
-                        to[(k * 16 + 8 + (lane >> 2)) ^ ((h >> 1 & 3) * 8)] = o[k][nt][e + 2];
+                            for (int k = 0; k < KS; k++) {
+                                to[(k * 16 + (lane >> 2)) ^ ((h >> 1 & 3) * 8)] = o[k][nt][e];
+                                to[(k * 16 + 8 + (lane >> 2)) ^ ((h >> 1 & 3) * 8)] = o[k][nt][e + 2];
+                            }
+                        }
+                    }
+                const int of_b = at.b, of_h0 = h0, pieces = heads * (D / 4);
+                const bool whole = first_i == 0 && at.i == at.n - 1;        // the column lies in this share
+                const long long column = (long long)at.b * p.columns + at.c, begin = r0 + n - at.i;          // its first tile in the row
+                const int tiles = at.n, slot = 2 * blockIdx.x + (n - (at.i - first_i) > 0);
+                if (n < share - 1) {
+                    next_tile(p, at);
+                    begin_column();                         // on their way while the sums are joined
+                }
+                first_i = 0;
+                clear();
+                __syncthreads();
+                auto write = [&](int i, float top, float sum, const float4 &v) {       // four channels of a result
+                    const int h = of_h0 + i / (D / 4), d = i % (D / 4) * 4;
+                    const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
+                    *reinterpret_cast<uint2 *>(reinterpret_cast<T *>(a.out) + of_b * a.out_token + h * a.out_head + d) =
+                        make_uint2(Pair<T>::pack(v.x * f, v.y * f), Pair<T>::pack(v.z * f, v.w * f));
+                    if (d == 0 && a.lse) a.lse[of_b * a.Hq + h] = sum == 0.0f ? -CUDART_INF_F : (top + log2f(sum) - LIFT) * 0.69314718055994531f;
+                };
+                float *part = p.parts + (long long)slot * PART;
+                for (int i = tid; i < pieces; i += THREADS) {
+                    const int h = i / (D / 4), d = i % (D / 4) * 4;
+                    float2 ml[WARPS];
+                    float top = -CUDART_INF_F, sum = 0.0f;
+#pragma unroll
+                    for (int w = 0; w < WARPS; w++) { ml[w] = ml_s[w][h]; top = fmaxf(top, ml[w].x); }
+                    const float base = top == -CUDART_INF_F ? 0.0f : top;
+                    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                    for (int w = 0; w < WARPS; w++) {
+                        const float f = exp2_approx(ml[w].x - base);
+                        const float4 x = *reinterpret_cast<const float4 *>(smem + w * STAGES * STAGE + scratch + (h * D + (d ^ ((h >> 1 & 3) * 8))) * 4);
+                        sum += f * ml[w].y;
+                        v.x += f * x.x; v.y += f * x.y; v.z += f * x.z; v.w += f * x.w;
+                    }
+                    if (whole) write(i, top, sum, v);
+                    else {
+                        __stcg(reinterpret_cast<float4 *>(part + MAX_GROUP * 2) + i, v);
+                        if (d == 0) __stcg(reinterpret_cast<float2 *>(part) + h, make_float2(top, sum));
                     }
                 }
-            }
-        __syncthreads();
-        const bool whole = seg == at.n;                     // the column lies in this share
-        const long long begin = r1 - left - at.i;           // the column's first tile in the row
-        const int w_first = (int)(((begin + 1) * shares - 1) / total), w_last = (int)(((begin + at.n) * shares - 1) / total);
-        const int slot_floats = MAX_GROUP * (D + 2);
-        float *part = p.parts + (2ll * blockIdx.x + (left != r1 - r0)) * slot_floats;
-        for (int i = tid; i < heads * D; i += THREADS) {
-            const int h = i / D, d = i % D;
-            float top = m_s[0][h], sum = 0.0f, v = 0.0f;
+                __syncthreads();
+                if (!whole) {
+                    const int w_first = (int)(((begin + 1) * shares - 1) / total), w_last = (int)(((begin + tiles) * shares - 1) / total);
+                    if (tid == 0) {
+                        __threadfence();
+                        last_s = atomicAdd(p.counters + column, 1u) == (unsigned)(w_last - w_first);
+                        __threadfence();
+                    }
+                    __syncthreads();
+                    if (last_s) {                           // all parts are there: joined in the order of the shares, by several threads each its own where channels are few
+                        if (tid == 0) p.counters[column] = 0;
+                        const float *const first = p.parts + (2ll * w_first + (begin > total * w_first / shares)) * PART;
+                        const int per = min(pieces, THREADS), ways = THREADS / per, way = tid / per;
+                        for (int i = tid - way * per; i < pieces; i += per) {
+                            const int h = i / (D / 4);
+                            float top = -CUDART_INF_F, sum = 0.0f;
+                            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                            if (way < ways) {
+                                constexpr int AT_ONCE = 8;
+                                for (int w0 = w_first + way; w0 <= w_last; w0 += AT_ONCE * ways) {
+                                    float2 ml[AT_ONCE];
+                                    float4 x[AT_ONCE];
 #pragma unroll
-            for (int w = 1; w < WARPS; w++) top = fmaxf(top, m_s[w][h]);
-            const float base = top == -CUDART_INF_F ? 0.0f : top;
+                                    for (int u = 0; u < AT_ONCE; u++) {
+                                        const int w = w0 + u * ways;
+                                        const float *from = w == w_first ? first : p.parts + 2ll * w * PART;
+                                        ml[u] = make_float2(-CUDART_INF_F, 0.0f);
+                                        x[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                                        if (w <= w_last) {
+                                            ml[u] = __ldcg(reinterpret_cast<const float2 *>(from) + h);
+                                            x[u] = __ldcg(reinterpret_cast<const float4 *>(from + MAX_GROUP * 2) + i);
+                                        }
+                                    }
+                                    float now = top;
 #pragma unroll
-            for (int w = 0; w < WARPS; w++) {
-                const float f = exp2_approx(m_s[w][h] - base);
-                sum += f * l_s[w][h];
-                v += f * reinterpret_cast<const float *>(smem + w * STAGES * STAGE + scratch)[h * D + (d ^ ((h >> 1 & 3) * 8))];
-            }
-            if (whole) {
-                reinterpret_cast<T *>(a.out)[at.b * a.out_token + (h0 + h) * a.out_head + d] = Pair<T>::one(sum == 0.0f ? 0.0f : v / sum);
-                if (d == 0 && a.lse) a.lse[at.b * a.Hq + h0 + h] = sum == 0.0f ? -CUDART_INF_F : (top + log2f(sum) - LIFT) * 0.69314718055994531f;
+                                    for (int u = 0; u < AT_ONCE; u++) now = fmaxf(now, ml[u].x);
+                                    const float base = now == -CUDART_INF_F ? 0.0f : now, f = exp2_approx(top - base);
+                                    sum *= f; v.x *= f; v.y *= f; v.z *= f; v.w *= f;
+#pragma unroll
+                                    for (int u = 0; u < AT_ONCE; u++) {
+                                        const float g = exp2_approx(ml[u].x - base);
+                                        sum += ml[u].y * g;
+                                        v.x += x[u].x * g; v.y += x[u].y * g; v.z += x[u].z * g; v.w += x[u].w * g;
+                                    }
+                                    top = now;
+                                }
+                            }
+                            if (ways > 1) {                 // (the loop is entered once then)
+                                join_v[tid] = v;
+                                join_ml[tid] = make_float2(top, sum);
+                            } else if (way < ways) write(i, top, sum, v);
+                        }
+                        if (ways > 1) {
+                            __syncthreads();
+                            if (tid < pieces) {
+                                float top = -CUDART_INF_F, sum = 0.0f;
+                                float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                                for (int w = 0; w < ways; w++) top = fmaxf(top, join_ml[w * per + tid].x);
+                                const float base = top == -CUDART_INF_F ? 0.0f : top;
+                                for (int w = 0; w < ways; w++) {
+                                    const float2 ml = join_ml[w * per + tid];
+                                    const float4 x = join_v[w * per + tid];
+                                    const float g = exp2_approx(ml.x - base);
+                                    sum += ml.y * g;
+                                    v.x += x.x * g; v.y += x.y * g; v.z += x.z * g; v.w += x.w * g;
+                                }
+                                write(tid, top, sum, v);
+                            }
+                            __syncthreads();
+                        }
+                    }
+                }
             } else {
-                __stcg(part + MAX_GROUP * 2 + i, v);
-                if (d == 0) __stcg(reinterpret_cast<float2 *>(part) + h, make_float2(top, sum));
+                at.i++;
             }
         }
-        __syncthreads();
-        if (!whole) {
-            const long long column = (long long)at.b * p.columns + at.c;
-            if (tid == 0) {
-                __threadfence();
-                last_s = atomicAdd(p.counters + column, 1u) == (unsigned)(w_last - w_first);
-                __threadfence();
-            }
-            __syncthreads();
-            if (last_s) {                                   // all parts are there: joined in the order of the shares
-                if (tid == 0) p.counters[column] = 0;
-                const float *first = p.parts + (2ll * w_first + (begin > total * w_first / shares)) * slot_floats;
-                for (int i = tid; i < heads * D; i += THREADS) {
-                    const int h = i / D, d = i % D;
-                    float top = -CUDART_INF_F, sum = 0.0f, v = 0.0f;
-                    for (int w = w_first; w <= w_last; w++) {
-                        const float *from = w == w_first ? first : p.parts + 2ll * w * slot_floats;
-                        const float2 ml = __ldcg(reinterpret_cast<const float2 *>(from) + h);
-                        const float x = __ldcg(from + MAX_GROUP * 2 + i), now = fmaxf(top, ml.x), base = now == -CUDART_INF_F ? 0.0f : now;
-                        const float f = exp2_approx(top - base), g = exp2_approx(ml.x - base);
-                        sum = sum * f + ml.y * g;
-                        v = v * f + x * g;
-                        top = now;
-                    }
-                    reinterpret_cast<T *>(a.out)[at.b * a.out_token + (h0 + h) * a.out_head + d] = Pair<T>::one(sum == 0.0f ? 0.0f : v / sum);
-                    if (d == 0 && a.lse) a.lse[at.b * a.Hq + h0 + h] = sum == 0.0f ? -CUDART_INF_F : (top + log2f(sum) - LIFT) * 0.69314718055994531f;
-                }
-            }
-        }
-        copy_tile(stage == 0 ? STAGES - 1 : stage - 1);     // (everyone has read the sums)
-        left -= seg;
-        at.i += seg - 1;
-        if (left > 0) next_tile(a, p.columns, at);
+        // the stage that was read is filled again; nothing is read in the first rounds
+        copy_tile(stage);
+        stage = stage + 1 == STAGES ? 0 : stage + 1;
     }
     copies_wait<0>();
     if (flags && a.status) atomicOr(a.status, flags);
@@ -488,6 +566,8 @@ extern "C" int kvc_paged_attn(const kvc_paged_attn_args *args, kvc_stream_t stre
     p.group = group_of(a.Hq, a.Hkv, a.D);
     p.columns = (int)columns_of(a.Hq, a.Hkv, a.D);
     p.per_head = p.columns / (int)a.Hkv;
+    p.most_tokens = (int)(a.table_width * a.page_size);
+    p.n_pages = (unsigned)a.n_pages;
     p.log2_scaling = a.scaling * 1.4426950408889634f;
     p.counters = reinterpret_cast<unsigned *>(a.workspace);
     p.parts = reinterpret_cast<float *>(reinterpret_cast<uint8_t *>(a.workspace) + counter_bytes(a.B, a.Hq, a.Hkv, a.D));
@@ -498,7 +578,7 @@ extern "C" int kvc_paged_attn(const kvc_paged_attn_args *args, kvc_stream_t stre
     switch (a.D) {                                                                                                             \
         case 64: return wide ? launch<T_, 64, 2, 6>(p, most, s) : launch<T_, 64, 1, 6>(p, most, s);                            \
         case 96: return wide ? launch<T_, 96, 2, 4>(p, most, s) : launch<T_, 96, 1, 4>(p, most, s);                            \
-        case 128: return wide ? launch<T_, 128, 2, 3>(p, most, s) : launch<T_, 128, 1, 3>(p, most, s);                         \
+        case 128: return wide ? launch<T_, 128, 2, KVC_S128>(p, most, s) : launch<T_, 128, 1, KVC_S128>(p, most, s);                         \
         default: return launch<T_, 256, 1, 3>(p, most, s);                                                                     \
     }
     if (a.type == KVC_TYPE_FP16) KVC_PA(__half)
