@@ -37,8 +37,17 @@ constexpr int MAX_CTAS_PER_SM = 4;
 #ifndef KVC_MIN_TILES
 #define KVC_MIN_TILES 2
 #endif
-#ifndef KVC_S128
-#define KVC_S128 3
+#ifndef KVC_SC
+#define KVC_SC 3, 4, 4, 3
+#endif
+#ifndef KVC_SC96
+#define KVC_SC96 3, 3, 4, 2
+#endif
+#ifndef KVC_SC128
+#define KVC_SC128 2, 3, 3, 2
+#endif
+#ifndef KVC_SC256
+#define KVC_SC256 3, 1
 #endif
 constexpr int MAX_GROUP = 16;                   // query heads that a column serves
 
@@ -59,7 +68,9 @@ struct Params {
     int group, columns, per_head;               // query heads of a column at most, columns of a request, columns of a KV head
     int most_tokens;                            // of a table row
     unsigned n_pages;
+    uint32_t sign;                              // of the scaling, for two values: the scores' maximum is taken before they are scaled
     float log2_scaling;
+    long long v_less_k;                         // bytes from the keys' pool to the values'
     unsigned *counters;
     float *parts;
 };
@@ -142,8 +153,8 @@ __device__ __forceinline__ void next_tile(const Params &p, Place &at) {
     }
 }
 
-template <typename T, int D, int NT, int STAGES>
-__global__ void __launch_bounds__(THREADS) paged_attn_kernel(const __grid_constant__ Params p) {
+template <typename T, int D, int NT, bool SAME, int STAGES, int CTAS>
+__global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_constant__ Params p) {
     constexpr int KS = D / 16;                              // steps of 16 channels
     constexpr uint32_t HALF_STAGE = 16 * D * 2, STAGE = 2 * HALF_STAGE;
     constexpr int PART = MAX_GROUP * (D + 2);               // floats of a partial result: maxima and sums, sums of values
@@ -161,7 +172,7 @@ __global__ void __launch_bounds__(THREADS) paged_attn_kernel(const __grid_consta
     int flags = 0;
 
     // ---- this CTA's share
-    long long r0, r1, total, shares;
+    long long r0, r1, total, size;                          // (size: tiles of a share)
     {
         const int chunk = (B + THREADS - 1) / THREADS, b0 = min(B, tid * chunk), b1 = min(B, b0 + chunk);
         long long mine = 0;
@@ -181,9 +192,9 @@ __global__ void __launch_bounds__(THREADS) paged_attn_kernel(const __grid_consta
         }
         before += upto - mine;
         total = all * p.columns;
-        shares = min((long long)gridDim.x, (total + KVC_MIN_TILES - 1) / KVC_MIN_TILES);          // none is empty
-        r0 = blockIdx.x < shares ? total * blockIdx.x / shares : total;
-        r1 = blockIdx.x < shares ? total * (blockIdx.x + 1) / shares : total;
+        size = max((long long)KVC_MIN_TILES, (total + gridDim.x - 1) / gridDim.x);
+        r0 = min(total, size * blockIdx.x);
+        r1 = min(total, r0 + size);
         if (r0 >= before * p.columns && r0 < (before + mine) * p.columns) {
             Place at;
             int unused = 0;
@@ -214,7 +225,7 @@ __global__ void __launch_bounds__(THREADS) paged_attn_kernel(const __grid_consta
 
     // ---- the copies
     Place ahead = start_s;
-    long long to_copy = r1 - r0;
+    int to_copy = (int)(r1 - r0);
     int page = -1;                                          // lanes 0 .. 15: the page of their token of the tile that is copied next
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * STAGES * STAGE;
     auto ask = [&]() {
@@ -233,19 +244,24 @@ __global__ void __launch_bounds__(THREADS) paged_attn_kernel(const __grid_consta
             if (lane == 0) masks[warp][stage] = mask;
             if (mask) {
                 const int hk = p.per_head == 1 ? ahead.c : ahead.c / p.per_head, row = t - divide(t, p.page) * (int)a.page_size;
-                const long long ko = good ? page * a.kp_page + row * a.kp_row + hk * a.kp_head : 0, vo = good ? page * a.vp_page + row * a.vp_row + hk * a.vp_head : 0;
+                const T *k16 = reinterpret_cast<const T *>(a.kpages), *v16 = reinterpret_cast<const T *>(a.vpages);
+                if (good) {
+                    k16 += page * a.kp_page + row * (int)a.kp_row + hk * (int)a.kp_head;
+                    if (!SAME) v16 += page * a.vp_page + row * (int)a.vp_row + hk * (int)a.vp_head;
+                }
                 const uint32_t to = ring + stage * STAGE;
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                     const int r = 4 * j + (lane >> 3);
                     const bool on = mask >> r & 1;
-                    const T *k = reinterpret_cast<const T *>(a.kpages) + __shfl_sync(0xffffffffu, ko, r), *v = reinterpret_cast<const T *>(a.vpages) + __shfl_sync(0xffffffffu, vo, r);
+                    const uint8_t *k = reinterpret_cast<const uint8_t *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(k16), r)) + (lane & 7) * 16;
+                    const uint8_t *v = SAME ? k + p.v_less_k : reinterpret_cast<const uint8_t *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(v16), r)) + (lane & 7) * 16;
 #pragma unroll
                     for (int c = 0; c < (D / 8 + 7) / 8; c++) {
-                        const int piece = c * 8 + (lane & 7);
-                        if ((D / 8) % 8 == 0 || piece < D / 8) {
-                            copy16(to + piece_at<D>(r, piece), k + piece * 8, on);
-                            copy16(to + HALF_STAGE + piece_at<D>(r, piece), v + piece * 8, on);
+                        if ((D / 8) % 8 == 0 || c * 8 + (lane & 7) < D / 8) {
+                            const uint32_t at = to + piece_at<D>(r, c * 8 + (lane & 7));
+                            copy16(at, k + c * 128, on);
+                            copy16(at + HALF_STAGE, v + c * 128, on);
                         }
                     }
                 }
@@ -272,8 +288,8 @@ __global__ void __launch_bounds__(THREADS) paged_attn_kernel(const __grid_consta
             const T *from = reinterpret_cast<const T *>(a.q) + at.b * a.q_token + (h0 + h) * a.q_head + (lane & 3) * 2;
 #pragma unroll
             for (int k = 0; k < KS; k++) {
-                q[k][nt][0] = h < heads ? *reinterpret_cast<const uint32_t *>(from + k * 16) : 0;
-                q[k][nt][1] = h < heads ? *reinterpret_cast<const uint32_t *>(from + k * 16 + 8) : 0;
+                q[k][nt][0] = h < heads ? *reinterpret_cast<const uint32_t *>(from + k * 16) ^ p.sign : 0;
+                q[k][nt][1] = h < heads ? *reinterpret_cast<const uint32_t *>(from + k * 16 + 8) ^ p.sign : 0;
             }
         }
     };
@@ -286,51 +302,63 @@ __global__ void __launch_bounds__(THREADS) paged_attn_kernel(const __grid_consta
             l[nt][0] = l[nt][1] = 0.0f;
         }
     };
-    const long long share = r1 - r0;
-    const uint32_t kv_row = lane & 15, kv_piece = lane >> 4;                                // keys: 16 rows, two pieces
-    const uint32_t v_row = (lane & 7) + (lane >> 4) * 8, v_piece = lane >> 3 & 1;           // values: two pieces, 16 rows, transposed
+    const int share = (int)(r1 - r0);
+    // where this lane's rows of a matrix load lie, from the stage's start: keys 16 rows by two pieces, values two pieces by 16 rows
+    uint32_t key_at[4], value_at[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        key_at[k] = piece_at<D>(lane & 15, 2 * k + (lane >> 4));
+        value_at[k] = HALF_STAGE + piece_at<D>((lane & 7) + (lane >> 4) * 8, 2 * k + (lane >> 3 & 1));
+    }
     int stage = 0, first_i = at.i;                          // first_i: the first tile of the column that is this CTA's
     ask();
     begin_column();
     clear();
 #pragma unroll 1
-    for (long long n = -STAGES; n < share; n++) {
+    for (int n = -STAGES; n < share; n++) {
         if (n >= 0) {
             copies_wait<STAGES - 1>();
             __syncwarp();
-            const uint32_t mask = masks[warp][stage], keys = ring + stage * STAGE, values = keys + HALF_STAGE;
+            const uint32_t mask = masks[warp][stage], from = ring + stage * STAGE;
             if (mask) {
                 float s[2][NT][4] = {};
 #pragma unroll
                 for (int k = 0; k < KS; k++) {
                     uint32_t f[4];
-                    ldmatrix4(f, keys + piece_at<D>(kv_row, 2 * k + kv_piece));
+                    ldmatrix4(f, from + key_at[k & 3] + (k >> 2) * 128);
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++) Pair<T>::mma(s[k & 1][nt], f, q[k][nt][0], q[k][nt][1]);
                 }
-                const bool on0 = mask >> (lane >> 2) & 1, on1 = mask >> (8 + (lane >> 2)) & 1;
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) s[0][nt][e] += s[1][nt][e];
+                if (mask != 0xffff) {
+                    const bool on0 = mask >> (lane >> 2) & 1, on1 = mask >> (8 + (lane >> 2)) & 1;
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) s[0][nt][e] = (e < 2 ? on0 : on1) ? s[0][nt][e] : -CUDART_INF_F;
+                }
                 float scale[NT][2];
                 bool grows = false;
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++) {
-#pragma unroll
-                    for (int e = 0; e < 4; e++) s[0][nt][e] = (e < 2 ? on0 : on1) ? (s[0][nt][e] + s[1][nt][e]) * p.log2_scaling : -CUDART_INF_F;
+                for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
                         float top = fmaxf(s[0][nt][e], s[0][nt][e + 2]);
                         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
                         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16)) * p.log2_scaling;
                         top = fmaxf(top, m[nt][e]);
                         grows |= top > m[nt][e];
                         const float base = top == -CUDART_INF_F ? 0.0f : top;
                         scale[nt][e] = exp2_approx(m[nt][e] - base);
                         m[nt][e] = top;
-                        s[0][nt][e] = exp2_approx(s[0][nt][e] - base + LIFT);
-                        s[0][nt][e + 2] = exp2_approx(s[0][nt][e + 2] - base + LIFT);
-                        l[nt][e] = l[nt][e] * scale[nt][e] + s[0][nt][e] + s[0][nt][e + 2];
+                        s[0][nt][e] = exp2_approx(fmaf(s[0][nt][e], p.log2_scaling, LIFT - base));
+                        s[0][nt][e + 2] = exp2_approx(fmaf(s[0][nt][e + 2], p.log2_scaling, LIFT - base));
+                        l[nt][e] = fmaf(l[nt][e], scale[nt][e], s[0][nt][e] + s[0][nt][e + 2]);
                     }
-                }
                 if (__any_sync(0xffffffffu, grows)) {
 #pragma unroll
                     for (int k = 0; k < KS; k++)
@@ -353,7 +381,7 @@ __global__ void __launch_bounds__(THREADS) paged_attn_kernel(const __grid_consta
 #pragma unroll
                 for (int k = 0; k < KS; k++) {
                     uint32_t f[4];
-                    ldmatrix4_trans(f, values + piece_at<D>(v_row, 2 * k + v_piece));
+                    ldmatrix4_trans(f, from + value_at[k & 3] + (k >> 2) * 128);
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++) {
                         Pair<T>::mma(o[k][nt], f, hi[nt][0], hi[nt][1]);
@@ -426,7 +454,7 @@ __global__ void __launch_bounds__(THREADS) paged_attn_kernel(const __grid_consta
                 }
                 __syncthreads();
                 if (!whole) {
-                    const int w_first = (int)(((begin + 1) * shares - 1) / total), w_last = (int)(((begin + tiles) * shares - 1) / total);
+                    const int w_first = (int)(begin / size), w_last = (int)((begin + tiles - 1) / size);
                     if (tid == 0) {
                         __threadfence();
                         last_s = atomicAdd(p.counters + column, 1u) == (unsigned)(w_last - w_first);
@@ -435,7 +463,7 @@ __global__ void __launch_bounds__(THREADS) paged_attn_kernel(const __grid_consta
                     __syncthreads();
                     if (last_s) {                           // all parts are there: joined in the order of the shares, by several threads each its own where channels are few
                         if (tid == 0) p.counters[column] = 0;
-                        const float *const first = p.parts + (2ll * w_first + (begin > total * w_first / shares)) * PART;
+                        const float *const first = p.parts + (2ll * w_first + (begin > size * w_first)) * PART;
                         const int per = min(pieces, THREADS), ways = THREADS / per, way = tid / per;
                         for (int i = tid - way * per; i < pieces; i += per) {
                             const int h = i / (D / 4);
@@ -508,11 +536,11 @@ __global__ void __launch_bounds__(THREADS) paged_attn_kernel(const __grid_consta
     if (flags && a.status) atomicOr(a.status, flags);
 }
 
-template <typename T, int D, int NT, int STAGES>
+template <typename T, int D, int NT, bool SAME, int STAGES, int CTAS>
 int launch(const Params &p, long long most_tiles, cudaStream_t stream) {
     static kvc_launch_slot slot;
     constexpr size_t shared = (size_t)WARPS * STAGES * 64 * D;
-    auto *kernel = paged_attn_kernel<T, D, NT, STAGES>;
+    auto *kernel = paged_attn_kernel<T, D, NT, SAME, STAGES, CTAS>;
     int occ = 0;
     if (int rc = kvc_prepare(slot, reinterpret_cast<const void *>(kernel), THREADS, shared, &occ)) return rc;
     KVC_REQUIRE(occ > 0, "kvc_paged_attn: the kernel does not fit this device");
@@ -520,6 +548,24 @@ int launch(const Params &p, long long most_tiles, cudaStream_t stream) {
     kernel<<<(unsigned)std::max<long long>(grid, 1), THREADS, shared, stream>>>(p);
     KVC_LAUNCH_OK();
     return KVC_OK;
+}
+
+template <typename T, int D, int STAGES, int CTAS, int WIDE_STAGES, int WIDE_CTAS>
+int choose_heads(const Params &p, bool same, long long most, cudaStream_t s) {
+    if constexpr (WIDE_STAGES > 0) {
+        if (p.group > 8) return same ? launch<T, D, 2, true, WIDE_STAGES, WIDE_CTAS>(p, most, s) : launch<T, D, 2, false, WIDE_STAGES, WIDE_CTAS>(p, most, s);
+    }
+    return same ? launch<T, D, 1, true, STAGES, CTAS>(p, most, s) : launch<T, D, 1, false, STAGES, CTAS>(p, most, s);
+}
+
+template <typename T>
+int choose(const Params &p, bool same, long long most, cudaStream_t s) {
+    switch (p.a.D) {
+        case 64: return choose_heads<T, 64, KVC_SC>(p, same, most, s);
+        case 96: return choose_heads<T, 96, KVC_SC96>(p, same, most, s);
+        case 128: return choose_heads<T, 128, KVC_SC128>(p, same, most, s);
+        default: return choose_heads<T, 256, KVC_SC256, 0, 0>(p, same, most, s);
+    }
 }
 
 // query heads that a column takes at most: 16 where they fit the registers beside the accumulators
@@ -555,6 +601,8 @@ extern "C" int kvc_paged_attn(const kvc_paged_attn_args *args, kvc_stream_t stre
     if (a.n_pages <= 1) a.kp_page = a.vp_page = 0;
     const int64_t strides = a.q_token | a.q_head | a.out_token | a.out_head | a.kp_page | a.kp_row | a.kp_head | a.vp_page | a.vp_row | a.vp_head;
     KVC_REQUIRE((at & 15) == 0 && (strides & 7) == 0, "kvc_paged_attn: rows must start on 16 bytes");
+    KVC_REQUIRE(a.kp_row >= 0 && a.kp_head >= 0 && a.vp_row >= 0 && a.vp_head >= 0 && a.kp_page >= 0 && a.vp_page >= 0 && a.kp_row * (a.page_size - 1) + a.kp_head * (a.Hkv - 1) < (1ll << 31) &&
+                    a.vp_row * (a.page_size - 1) + a.vp_head * (a.Hkv - 1) < (1ll << 31), "kvc_paged_attn: a page spans more than 2^31 elements");
     KVC_REQUIRE(a.workspace && (reinterpret_cast<uintptr_t>(a.workspace) & 15) == 0, "kvc_paged_attn: the workspace must be 16-byte aligned");
     if (a.workspace_bytes < kvc_paged_attn_workspace(a.B, a.Hq, a.Hkv, a.D)) {
         kvc_set_error("kvc_paged_attn: the workspace must hold what kvc_paged_attn_workspace says");
@@ -568,20 +616,14 @@ extern "C" int kvc_paged_attn(const kvc_paged_attn_args *args, kvc_stream_t stre
     p.per_head = p.columns / (int)a.Hkv;
     p.most_tokens = (int)(a.table_width * a.page_size);
     p.n_pages = (unsigned)a.n_pages;
-    p.log2_scaling = a.scaling * 1.4426950408889634f;
+    p.sign = a.scaling < 0.0f ? 0x80008000u : 0;
+    p.log2_scaling = std::max(fabsf(a.scaling) * 1.4426950408889634f, 1e-37f);      // (0 times the -inf of a token that is left out is none)
     p.counters = reinterpret_cast<unsigned *>(a.workspace);
     p.parts = reinterpret_cast<float *>(reinterpret_cast<uint8_t *>(a.workspace) + counter_bytes(a.B, a.Hq, a.Hkv, a.D));
     const long long most = a.B * p.columns * ((a.table_width * a.page_size + TILE - 1) / TILE);
     cudaStream_t s = kvc_cu(stream);
-    const bool wide = p.group > 8;
-#define KVC_PA(T_)                                                                                                             \
-    switch (a.D) {                                                                                                             \
-        case 64: return wide ? launch<T_, 64, 2, 6>(p, most, s) : launch<T_, 64, 1, 6>(p, most, s);                            \
-        case 96: return wide ? launch<T_, 96, 2, 4>(p, most, s) : launch<T_, 96, 1, 4>(p, most, s);                            \
-        case 128: return wide ? launch<T_, 128, 2, KVC_S128>(p, most, s) : launch<T_, 128, 1, KVC_S128>(p, most, s);                         \
-        default: return launch<T_, 256, 1, 3>(p, most, s);                                                                     \
-    }
-    if (a.type == KVC_TYPE_FP16) KVC_PA(__half)
-    KVC_PA(__nv_bfloat16)
-#undef KVC_PA
+    KVC_REQUIRE(most / kvc_sm_count() < (1ll << 31), "kvc_paged_attn: too many tokens");
+    p.v_less_k = reinterpret_cast<const uint8_t *>(a.vpages) - reinterpret_cast<const uint8_t *>(a.kpages);
+    const bool same = a.kp_page == a.vp_page && a.kp_row == a.vp_row && a.kp_head == a.vp_head;
+    return a.type == KVC_TYPE_FP16 ? choose<__half>(p, same, most, s) : choose<__nv_bfloat16>(p, same, most, s);
 }

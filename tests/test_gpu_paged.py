@@ -295,10 +295,41 @@ def test_attend_strides(ops, order, D):
     attend(ops, LENGTHS["edges"], 6, 3, D, torch.float16, page=24, order=order)
 
 
+@pytest.mark.parametrize("D", [64, 96, 128, 256])
+@pytest.mark.parametrize("heads", [(4, 2), (20, 2)])
+def test_attend_pools_of_different_strides(ops, D, heads):
+    """Keys with each head's rows together, values token by token with room between the rows."""
+    gen = torch.Generator(device="cuda").manual_seed(D)
+    lengths = LENGTHS["edges"]
+    table, _, _ = plain.tables(np.random.RandomState(D), lengths, 16, 200)
+    kp, vp = plain.pool(gen, 200, 16, 2, D, torch.bfloat16, "cuda", "head"), plain.pool(gen, 200, 16, 2, D, torch.bfloat16, "cuda", "padded")
+    q = torch.randn(len(lengths), heads[0], D, generator=gen, device="cuda").bfloat16()
+    args = (q, kp, vp, dev(table), dev(lengths), 0.1)
+    want, _, bound, _ = plain.attend(*args[:4], lengths, 0.1)
+    near(ops.paged_attn(*args), want, bound)
+    want, _, bound, _ = plain.attend(q, vp, kp, *args[3:4], lengths, 0.1)
+    near(ops.paged_attn(q, vp, kp, *args[3:]), want, bound)
+
+
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 def test_attend_sharp(ops, dtype):
     """Scores in the hundreds: weights from 1 to nothing, the maximum anywhere; with half of one sign only."""
     attend(ops, LENGTHS["edges"] + [3000], 8, 2, 128, dtype, sharp=100.0)
+
+
+@pytest.mark.parametrize("scaling", [-0.3, 0.0, 1e-30, 4.0])
+def test_attend_scalings(ops, scaling):
+    """A negative scaling, none at all (the mean of the values), a large one."""
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    lengths = [0, 1, 5, 77, 300]
+    table, _, _ = plain.tables(np.random.RandomState(2), lengths, 16, 40)
+    kp, vp = (plain.pool(gen, 40, 16, 2, 64, torch.float16, "cuda") for _ in range(2))
+    q = torch.randn(5, 6, 64, generator=gen, device="cuda").half()
+    args = (q, kp, vp, dev(table), dev(lengths), scaling)
+    out, lse = ops.paged_attn(*args, return_lse=True)
+    want, want_lse, bound, lse_bound = plain.attend(*args[:4], lengths, scaling)
+    near(out, want, bound)
+    near(lse[1:], want_lse[1:], lse_bound[1:])
 
 
 def test_attend_small_weights_count(ops):
