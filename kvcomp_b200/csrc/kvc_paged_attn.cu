@@ -21,13 +21,12 @@
 // work is a few per cent of the time that the bytes need.)  P is split into two 16-bit pieces, hi + lo, and multiplied twice: the weights keep 21
 // (fp16) or 16 bits (bf16), and the result is rounded once, at the end.  fp16 weights are carried times 2^14, so that the pieces of weights down to 2^-28
 // of the largest are normal numbers and many small ones are not lost.
-#include <cuda_bf16.h>
 #include <math_constants.h>
 #include <string.h>
 
 #include <algorithm>
 
-#include "kvc_common.cuh"
+#include "kvc_paged.cuh"
 
 namespace {
 
@@ -51,20 +50,9 @@ constexpr int MAX_CTAS_PER_SM = 4;
 #endif
 constexpr int MAX_GROUP = 16;                   // query heads that a column serves
 
-struct Div { uint32_t magic, shift; };          // n / d of a divisor known to the host, n < 2^31
-
-Div make_div(uint32_t d) {
-    Div r;
-    r.shift = 0;
-    while ((1ull << r.shift) < d) r.shift++;
-    r.magic = (uint32_t)(((1ull << 32) * ((1ull << r.shift) - d)) / d + 1);
-    return r;
-}
-__device__ __forceinline__ int divide(int n, const Div &d) { return (int)((__umulhi(d.magic, (uint32_t)n) + (uint32_t)n) >> d.shift); }
-
 struct Params {
     kvc_paged_attn_args a;
-    Div page;
+    kvc_div page;
     int group, columns, per_head;               // query heads of a column at most, columns of a request, columns of a KV head
     int most_tokens;                            // of a table row
     unsigned n_pages;
@@ -232,7 +220,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
         page = -1;
         if (to_copy > 0 && lane < 16) {
             const int t = ahead.span.first + ahead.i * TILE + warp * 16 + lane;
-            if (t < ahead.span.len) page = __ldg(a.table + ahead.b * a.table_stride + divide(t, p.page));
+            if (t < ahead.span.len) page = __ldg(a.table + ahead.b * a.table_stride + kvc_divide(t, p.page));
         }
     };
     auto copy_tile = [&](int stage) {
@@ -243,7 +231,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
             const uint32_t mask = __ballot_sync(0xffffffffu, good);
             if (lane == 0) masks[warp][stage] = mask;
             if (mask) {
-                const int hk = p.per_head == 1 ? ahead.c : ahead.c / p.per_head, row = t - divide(t, p.page) * (int)a.page_size;
+                const int hk = p.per_head == 1 ? ahead.c : ahead.c / p.per_head, row = t - kvc_divide(t, p.page) * (int)a.page_size;
                 const T *k16 = reinterpret_cast<const T *>(a.kpages), *v16 = reinterpret_cast<const T *>(a.vpages);
                 if (good) {
                     k16 += page * a.kp_page + row * (int)a.kp_row + hk * (int)a.kp_head;
@@ -588,7 +576,7 @@ extern "C" int kvc_paged_attn(const kvc_paged_attn_args *args, kvc_stream_t stre
     KVC_REQUIRE(a.type == KVC_TYPE_FP16 || a.type == KVC_TYPE_BF16, "kvc_paged_attn: unknown type %d", a.type);
     KVC_REQUIRE(a.D == 64 || a.D == 96 || a.D == 128 || a.D == 256, "kvc_paged_attn: heads of 64, 96, 128 or 256 channels, got %lld", (long long)a.D);
     KVC_REQUIRE(a.B >= 0 && a.Hkv > 0 && a.Hq > 0 && a.Hq % a.Hkv == 0 && a.Hq < 65536, "kvc_paged_attn: %lld query heads over %lld", (long long)a.Hq, (long long)a.Hkv);
-    KVC_REQUIRE(a.page_size > 0 && a.page_size <= (1 << 20) && a.n_pages >= 0 && a.n_pages < (1ll << 31) && a.table_width >= 0 && a.window >= 0, "kvc_paged_attn: bad sizes");
+    KVC_REQUIRE(a.page_size > 0 && a.page_size <= KVC_MAX_PAGE && a.n_pages >= 0 && a.n_pages < (1ll << 31) && a.table_width >= 0 && a.window >= 0, "kvc_paged_attn: bad sizes");
     KVC_REQUIRE(a.table_width * a.page_size < (1ll << 31), "kvc_paged_attn: a table row holds %lld tokens, lengths have 32 bits", (long long)(a.table_width * a.page_size));
     if (a.B == 0) return KVC_OK;
     KVC_REQUIRE(a.B < (1 << 24), "kvc_paged_attn: %lld requests", (long long)a.B);
@@ -610,7 +598,7 @@ extern "C" int kvc_paged_attn(const kvc_paged_attn_args *args, kvc_stream_t stre
     }
     Params p;
     p.a = a;
-    p.page = make_div((uint32_t)a.page_size);
+    p.page = kvc_make_div((uint32_t)a.page_size);
     p.group = group_of(a.Hq, a.Hkv, a.D);
     p.columns = (int)columns_of(a.Hq, a.Hkv, a.D);
     p.per_head = p.columns / (int)a.Hkv;

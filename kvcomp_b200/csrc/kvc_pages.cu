@@ -1,20 +1,29 @@
 // Paged caches: which pages a step's tokens go to, the way back of finished requests' pages, and the rotation of queries and
 // keys with the way of keys and values into their pages.
-#include <cuda_bf16.h>
 #include <string.h>
 
 #include <algorithm>
 
-#include "kvc_common.cuh"
+#include "kvc_paged.cuh"
 
 namespace {
 
-constexpr int SCAN_THREADS = 1024;
-constexpr int MAX_PAGE = 1 << 20;
+__device__ __forceinline__ void raise_flag(int32_t *status, int flags) {
+    if (flags && status) atomicOr(status, flags);
+}
 
-// ---- sums over the requests -----------------------------------------------------------------------------------
+// ---- pages ----------------------------------------------------------------------------------------------------------
+//
+// Two sums over the requests in their order (tokens, pages) say where each one's rows and pages begin; one CTA makes them, 1024
+// requests at a time, since a launch for a step has little more to do than that.  What is left is 8 bytes for each token or page: where they are few the same CTA
+// writes them behind a barrier, else a second kernel does, which reads what the first has written and never the lengths and the counter, so that
+// these may be changed in place.  (The second kernel begins while the first one runs and waits for it.)
 
-// exclusive sum of a and b over the CTA's threads, and the totals; every thread takes part
+constexpr int SCAN_THREADS = 1024, SMALL_THREADS = 128, FILL_THREADS = 256;
+// Rows that the scanning CTA fills itself.  A second launch costs some 2 us, and so do 4096 rows of one CTA (16 a thread).
+constexpr int FILL_ALONE = 4096;
+
+// exclusive sums of a and b over the CTA's threads, and the totals; every thread takes part
 __device__ __forceinline__ void block_scan2(long long &a, long long &b, long long &total_a, long long &total_b, longlong2 *warps) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     long long ia = a, ib = b;
@@ -26,23 +35,30 @@ __device__ __forceinline__ void block_scan2(long long &a, long long &b, long lon
     __syncthreads();                                        // (the sums of a scan before have been read)
     if (lane == 31) warps[warp] = make_longlong2(ia, ib);
     __syncthreads();
-    long long fa = 0, fb = 0;
-    total_a = total_b = 0;
-    for (int w = 0; w < (int)blockDim.x / 32; w++) {
-        const longlong2 v = warps[w];
-        if (w < warp) { fa += v.x; fb += v.y; }
-        total_a += v.x; total_b += v.y;
+    longlong2 v = lane < (int)blockDim.x / 32 ? warps[lane] : make_longlong2(0, 0);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long ua = __shfl_up_sync(0xffffffffu, v.x, o), ub = __shfl_up_sync(0xffffffffu, v.y, o);
+        if (lane >= o) { v.x += ua; v.y += ub; }
     }
-    a = fa + ia - a;
-    b = fb + ib - b;
+    total_a = __shfl_sync(0xffffffffu, v.x, 31);
+    total_b = __shfl_sync(0xffffffffu, v.y, 31);
+    const long long fa = __shfl_sync(0xffffffffu, v.x, max(warp - 1, 0)), fb = __shfl_sync(0xffffffffu, v.y, max(warp - 1, 0));
+    a = (warp ? fa : 0) + ia - a;
+    b = (warp ? fb : 0) + ib - b;
 }
 
-__device__ __forceinline__ void raise_flag(int32_t *status, int flags) {
-    if (flags && status) atomicOr(status, flags);
+__device__ __forceinline__ long long block_max(long long v, long long *warps) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
+    if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = v;
+    __syncthreads();
+    for (int w = 0; w < (int)blockDim.x / 32; w++) v = max(v, warps[w]);
+    return v;
 }
 
-// the request whose rows hold `row`: the last b with starts[b] <= row among those that have any (starts[B] > row)
-__device__ __forceinline__ int find_row(const int32_t *__restrict__ starts, int B, long long row) {
+// the request whose rows hold `row`: the last b with starts[b] <= row (behind it starts[b + 1] > row: it has some)
+__device__ __forceinline__ int find_row(const int32_t *starts, int B, int row) {
     int lo = 0, hi = B;
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
@@ -51,84 +67,135 @@ __device__ __forceinline__ int find_row(const int32_t *__restrict__ starts, int 
     return lo;
 }
 
-__global__ void __launch_bounds__(SCAN_THREADS) page_plan_kernel(const kvc_page_plan_args a) {
+__device__ __forceinline__ int pages_of(int tokens, const kvc_div &page) { return tokens > 0 ? kvc_divide(tokens - 1, page) + 1 : 0; }
+
+struct PlanParams { kvc_page_plan_args a; kvc_div page; };
+
+// slots and positions of rows [first, first + 4)
+__device__ __forceinline__ void plan_rows(const PlanParams &p, int first, int end) {
+    const kvc_page_plan_args &a = p.a;
+    int slot[4], position[4];
+    int b = -1, behind = 0, start = 0, taken = 0, held = 0, owned = 0, flags = 0;
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        const int n = first + k;
+        slot[k] = -1;
+        position[k] = 0;
+        if (n >= end) continue;
+        if (b < 0 || n >= behind) {
+            if (b < 0) b = find_row(a.starts, (int)a.B, n);
+            else while (a.starts[b + 1] <= n) b++;
+            start = a.starts[b]; behind = a.starts[b + 1];
+            taken = a.taken[b];
+            held = max(a.lengths_out[b], 0) - (taken >= 0 ? max(a.new_tokens[b], 0) : 0);
+            owned = pages_of(held, p.page);
+        }
+        position[k] = held + n - start;
+        if (taken >= 0) {
+            const int at = kvc_divide(position[k], p.page), row = position[k] - at * (int)a.page_size;
+            int32_t *const entry = a.table + b * a.table_stride + at;
+            const int page = at >= owned ? a.free_pages[taken + at - owned] : *entry;
+            if (at >= owned && row == 0) *entry = page;     // (a new page begins with one of these tokens)
+            if ((unsigned)page < (unsigned)a.n_pages) slot[k] = page * (int)a.page_size + row;
+            else flags = KVC_FLAG_BAD_PAGE;
+        }
+    }
+    if (first + 4 <= a.tokens && ((reinterpret_cast<uintptr_t>(a.slots) | reinterpret_cast<uintptr_t>(a.positions)) & 15) == 0) {
+        *reinterpret_cast<int4 *>(a.slots + first) = make_int4(slot[0], slot[1], slot[2], slot[3]);
+        *reinterpret_cast<int4 *>(a.positions + first) = make_int4(position[0], position[1], position[2], position[3]);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            if (first + k < a.tokens) { a.slots[first + k] = slot[k]; a.positions[first + k] = position[k]; }
+    }
+    raise_flag(a.status, flags);
+}
+
+template <int THREADS, bool ALONE>
+__global__ void __launch_bounds__(THREADS) page_plan_kernel(const __grid_constant__ PlanParams p) {
     __shared__ longlong2 warps[32];
+    __shared__ long long largest[32];
+    const kvc_page_plan_args &a = p.a;
+    if (!ALONE) cudaTriggerProgrammaticLaunchCompletion();
     const int B = (int)a.B;
-    const long long ps = a.page_size, head = min(max((long long)a.head[0], 0ll), (long long)a.n_pages);
-    long long rows = 0, pages = 0, given = 0;              // in front of this thread's requests
+    const long long head = min(max((long long)a.head[0], 0ll), (long long)a.n_pages);
+    long long rows = 0, pages = 0, given = 0;               // in front of this round's requests; what this thread's have been given, with all before them
     int flags = a.head[0] != head ? KVC_FLAG_BAD_LENGTH : 0;
-    for (int b0 = 0; b0 < B; b0 += blockDim.x) {
+    for (int b0 = 0; b0 < B; b0 += THREADS) {
         const int b = b0 + threadIdx.x;
-        long long held = 0, add = 0;
+        int held = 0, add = 0;
         if (b < B) { held = a.lengths[b]; add = a.new_tokens[b]; }
         if (held < 0 || add < 0) flags |= KVC_FLAG_BAD_LENGTH;
-        held = held < 0 ? 0 : held; add = add < 0 ? 0 : add;
-        long long start = add, zero = 0, total_rows, unused;
-        block_scan2(start, zero, total_rows, unused, warps);
-        start += rows;
-        const long long owned = (held + ps - 1) / ps, wanted = (held + add + ps - 1) / ps;
-        const bool fits = wanted <= a.table_width && start + add <= a.tokens && held + add < (1ll << 31);
+        held = max(held, 0); add = max(add, 0);
+        const bool counted = (long long)held + add < (1ll << 31);
+        const int owned = pages_of(held, p.page), wanted = counted ? pages_of(held + add, p.page) : 0;
+        bool fits = counted && wanted <= a.table_width;
         const long long need = fits ? wanted - owned : 0;
-        long long before = need, total_need;
-        block_scan2(before, zero, total_need, unused, warps);
-        before += pages;
+        long long start = add, before = need, total_rows, total_pages;
+        block_scan2(start, before, total_rows, total_pages, warps);
+        start += rows; before += pages;
+        fits = fits && start + add <= a.tokens;             // (the requests behind the first whose rows do not fit are refused too: that their needs were summed makes no difference)
         const bool served = fits && (need == 0 || head + before + need <= a.n_pages);
         if (b < B) {
             a.starts[b] = (int32_t)min(start, (long long)a.tokens);
             a.taken[b] = served ? (int32_t)min(head + before, (long long)a.n_pages) : -1;
-            a.lengths_out[b] = (int32_t)(served ? held + add : held);
+            a.lengths_out[b] = served ? held + add : held;
             if (!served) flags |= KVC_FLAG_NO_PAGES;
         }
         if (served && need > 0) given = before + need;
-        rows += total_rows; pages += total_need;
+        rows += total_rows; pages += total_pages;
     }
-    // the served that need pages are the first ones of those that need any: what they took is the largest sum
-    long long best = given;
-    __shared__ long long largest[32];
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
-    if ((threadIdx.x & 31) == 0) largest[threadIdx.x >> 5] = best;
-    __syncthreads();
+    // those that were given pages are the first of those that asked for some: what was taken is the largest sum
+    given = block_max(given, largest);
     if (threadIdx.x == 0) {
-        for (int w = 1; w < SCAN_THREADS / 32; w++) best = max(best, largest[w]);
         a.starts[B] = (int32_t)min(rows, (long long)a.tokens);
-        a.head_out[0] = (int32_t)(head + best);
+        a.head_out[0] = (int32_t)(head + given);
     }
     raise_flag(a.status, flags);
-    __threadfence_block();
-    __syncthreads();
-    const int end = a.starts[B];
-    for (long long n = threadIdx.x; n < a.tokens; n += blockDim.x) {
-        int slot = -1, position = 0;
-        if (n < end) {
-            const int b = find_row(a.starts, B, n), first = a.taken[b];
-            const int add = max(a.new_tokens[b], 0), held = a.lengths_out[b] - (first >= 0 ? add : 0);
-            position = held + (int)n - a.starts[b];
-            if (first >= 0) {
-                const int p = position / (int)ps, owned = (held + (int)ps - 1) / (int)ps;
-                const int page = p >= owned ? a.free_pages[first + p - owned] : a.table[b * a.table_stride + p];
-                if (p >= owned && position % (int)ps == 0) a.table[b * a.table_stride + p] = page;
-                if ((unsigned)page < (unsigned long long)a.n_pages) slot = page * (int)ps + position % (int)ps;
-                else raise_flag(a.status, KVC_FLAG_BAD_PAGE);
-            }
-        }
-        a.slots[n] = slot;
-        a.positions[n] = position;
+    if (ALONE) {
+        __syncthreads();
+        const int end = (int)min(rows, (long long)a.tokens);
+        for (int n = threadIdx.x * 4; n < (int)a.tokens; n += THREADS * 4) plan_rows(p, n, end);
     }
 }
 
-__global__ void __launch_bounds__(SCAN_THREADS) page_release_kernel(const kvc_page_release_args a) {
+__global__ void __launch_bounds__(FILL_THREADS) plan_rows_kernel(const __grid_constant__ PlanParams p) {
+    cudaGridDependencySynchronize();
+    const long long n = 4 * ((long long)blockIdx.x * FILL_THREADS + threadIdx.x);
+    if (n < p.a.tokens) plan_rows(p, (int)n, p.a.starts[p.a.B]);
+}
+
+struct ReleaseParams { kvc_page_release_args a; kvc_div page; };
+
+// entries [i, i + 4) of the `freed` pages that go back; `to` is where the first one goes
+__device__ __forceinline__ void release_rows(const ReleaseParams &p, int i, int freed, int32_t *to) {
+    const kvc_page_release_args &a = p.a;
+    int b = find_row(a.first, (int)a.B, i);
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        if (i + k >= freed) return;
+        while (a.first[b + 1] <= i + k) b++;
+        to[i + k] = a.table[b * a.table_stride + i + k - a.first[b]];
+    }
+}
+
+template <int THREADS, bool ALONE>
+__global__ void __launch_bounds__(THREADS) page_release_kernel(const __grid_constant__ ReleaseParams p) {
     __shared__ longlong2 warps[32];
+    __shared__ long long largest[32];
+    const kvc_page_release_args &a = p.a;
+    if (!ALONE) cudaTriggerProgrammaticLaunchCompletion();
     const int B = (int)a.B;
-    const long long ps = a.page_size, head = min(max((long long)a.head[0], 0ll), (long long)a.n_pages);
+    const long long head = min(max((long long)a.head[0], 0ll), (long long)a.n_pages);
     long long pages = 0, freed = 0;
     int flags = a.head[0] != head ? KVC_FLAG_BAD_LENGTH : 0;
-    for (int b0 = 0; b0 < B; b0 += blockDim.x) {
+    for (int b0 = 0; b0 < B; b0 += THREADS) {
         const int b = b0 + threadIdx.x;
         const bool done = b < B && a.done[b] != 0;
-        long long held = b < B ? a.lengths[b] : 0;
-        if (held < 0 || (held + ps - 1) / ps > a.table_width) { flags |= KVC_FLAG_BAD_LENGTH; held = min(max(held, 0ll), ps * a.table_width); }
-        const long long back = done ? (held + ps - 1) / ps : 0;
+        int held = b < B ? a.lengths[b] : 0;
+        if (held < 0) { flags |= KVC_FLAG_BAD_LENGTH; held = 0; }
+        long long back = done ? pages_of(held, p.page) : 0;
+        if (back > a.table_width) { flags |= KVC_FLAG_BAD_LENGTH; back = a.table_width; }
         long long before = back, zero = 0, total, unused;
         block_scan2(before, zero, total, unused, warps);
         before += pages;
@@ -136,31 +203,50 @@ __global__ void __launch_bounds__(SCAN_THREADS) page_release_kernel(const kvc_pa
         if (done && !fits) flags |= KVC_FLAG_NO_PAGES;
         if (b < B) {
             a.first[b] = (int32_t)min(before, head);
-            a.lengths_out[b] = done && fits ? 0 : (int32_t)held;
+            a.lengths_out[b] = done && fits ? 0 : held;
         }
-        if (fits) freed = max(freed, before + back);
+        if (fits) freed = before + back;
         pages += total;
     }
-    __shared__ long long largest[32];
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) freed = max(freed, __shfl_xor_sync(0xffffffffu, freed, o));
-    if ((threadIdx.x & 31) == 0) largest[threadIdx.x >> 5] = freed;
-    __syncthreads();
-    for (int w = 0; w < SCAN_THREADS / 32; w++) freed = max(freed, largest[w]);
+    freed = block_max(freed, largest);
     if (threadIdx.x == 0) {
         a.first[B] = (int32_t)freed;
         a.head_out[0] = (int32_t)(head - freed);
     }
     raise_flag(a.status, flags);
-    __threadfence_block();
-    __syncthreads();
-    for (long long i = threadIdx.x; i < freed; i += blockDim.x) {
-        const int b = find_row(a.first, B, i);
-        a.free_pages[head - freed + i] = a.table[b * a.table_stride + i - a.first[b]];
+    if (ALONE) {
+        __syncthreads();
+        for (int i = threadIdx.x * 4; i < (int)freed; i += THREADS * 4) release_rows(p, i, (int)freed, a.free_pages + (head - freed));
     }
 }
 
+__global__ void __launch_bounds__(FILL_THREADS) release_rows_kernel(const __grid_constant__ ReleaseParams p) {
+    cudaGridDependencySynchronize();
+    const int freed = p.a.first[p.a.B];
+    for (long long i = 4 * ((long long)blockIdx.x * FILL_THREADS + threadIdx.x); i < freed; i += 4ll * gridDim.x * FILL_THREADS)
+        release_rows(p, (int)i, freed, p.a.free_pages + p.a.head_out[0]);
+}
+
+// `fill` behind `scan` on the stream, launched early
+template <typename P>
+int launch_fill(void (*fill)(const P), unsigned grid, const P &p, cudaStream_t stream) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(FILL_THREADS);
+    cfg.stream = stream;
+    cudaLaunchAttribute early;
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &early;
+    cfg.numAttrs = 1;
+    KVC_CUDA_OK(cudaLaunchKernelEx(&cfg, fill, p));
+    return KVC_OK;
+}
+
 // ---- rotation ---------------------------------------------------------------------------------------------------
+//
+// Every value is read once and written once: HBM for a prompt, latency for a step.  cos and sin are made once for a (token,
+// frequency) and CTA, not once for a head, and wait in shared memory.
 
 template <typename T> __device__ __forceinline__ float to_float(T v);
 template <> __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
@@ -168,19 +254,140 @@ template <> __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return 
 template <typename T> __device__ __forceinline__ T from_float(float v);
 template <> __device__ __forceinline__ __half from_float(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_float(float v) { return __float2bfloat16_rn(v); }
+__device__ __forceinline__ float2 unpack(uint32_t v, __half) { return __half22float2(*reinterpret_cast<const __half2 *>(&v)); }
+__device__ __forceinline__ float2 unpack(uint32_t v, __nv_bfloat16) { return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&v)); }
+__device__ __forceinline__ uint32_t pack(float a, float b, __half) { const __half2 r = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t *>(&r); }
+__device__ __forceinline__ uint32_t pack(float a, float b, __nv_bfloat16) { const __nv_bfloat162 r = __floats2bfloat162_rn(a, b); return *reinterpret_cast<const uint32_t *>(&r); }
 
 // cos and sin of position * frequency.  The turns are counted in fp64: what is left of a far position's angle after its whole
 // turns keeps 2^-53 of the angle, 1e-10 at a million radians; fp32 would keep 0.06.
-__device__ __forceinline__ float2 turn(int position, double frequency, float factor) {
+__device__ __forceinline__ float2 turn(int position, double frequency, float factor, bool inverse) {
     double t = (double)position * (frequency * 0.15915494309189533576888);
     t -= rint(t);
     float s, c;
     sincospif(2.0f * (float)t, &s, &c);
-    return make_float2(c * factor, s * factor);
+    return make_float2(c * factor, inverse ? -s * factor : s * factor);
 }
 
+struct RotaryParams {
+    kvc_rotary_args a;
+    kvc_div page, heads, units;                             // divisors: page size, Hq + 2 Hkv, D / 16
+    int rows;                                               // (token, head) rows of a CTA
+    long long slots;                                        // of the pool
+};
+
+// Where a CTA's tokens go: element offsets of their rows in the pools, -1: nowhere
+struct Place { long long k, v; };
+
+__device__ __forceinline__ Place place_of(const RotaryParams &p, long long n, int &flags) {
+    const kvc_rotary_args &a = p.a;
+    Place r = {-1, -1};
+    const int slot = a.slots[n];
+    if (slot < 0) return r;
+    if (slot >= p.slots) { flags = KVC_FLAG_BAD_PAGE; return r; }
+    const int page = kvc_divide(slot, p.page), row = slot - page * (int)a.page_size;
+    r.k = page * a.kp_page + row * a.kp_row;
+    r.v = page * a.vp_page + row * a.vp_row;
+    return r;
+}
+
+constexpr int ROTARY_THREADS = 256, AT_ONCE = 4, MAX_TOKENS = 32;
+
+// Heads of 16 n channels, rotated by multiples of 16, everything on 16 bytes.  A thread has a unit of 16 channels (8 pairs: two pieces of 16 bytes,
+// half the rotated channels apart, or next to each other) of four rows at a time; the first four are asked for before the
+// angles are made.
 template <typename T>
-__global__ void __launch_bounds__(256) rotary_kernel(const kvc_rotary_args a) {
+__global__ void __launch_bounds__(ROTARY_THREADS, 4) rotary_rows_kernel(const __grid_constant__ RotaryParams p) {
+    extern __shared__ float4 turns[];                       // [token][2 pairs of a unit][unit]: cos, sin, cos, sin
+    __shared__ Place places[MAX_TOKENS];
+    const kvc_rotary_args &a = p.a;
+    const int units = (int)a.D / 16, rotated = (int)a.rotary / 16, H = (int)(a.Hq + 2 * a.Hkv), tid = threadIdx.x;
+    const long long row0 = (long long)blockIdx.x * p.rows, n0 = row0 / H;
+    const int skip = (int)(row0 - n0 * H), rows = (int)min((long long)p.rows, a.N * H - row0);
+    const int tokens = kvc_divide(skip + rows - 1, p.heads) + 1, lanes = ROTARY_THREADS / units, first = kvc_divide(tid, p.units), u = tid - first * units;
+    const bool half = a.layout == KVC_ROTARY_HALF && u < rotated;
+    const int c0 = half ? 8 * u : 16 * u, c1 = half ? 8 * (u + rotated) : 16 * u + 8;
+    uint4 x[AT_ONCE][2];
+    auto load = [&](int from) {
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; j++) {
+            const int r = from + j * lanes;
+            if (first >= lanes || r >= rows) continue;
+            const int t = kvc_divide(skip + r, p.heads), h = skip + r - t * H;
+            const T *at;
+            if (h < a.Hq) at = reinterpret_cast<const T *>(a.q) + (n0 + t) * a.q_token + h * a.q_head;
+            else if (h < a.Hq + a.Hkv) at = reinterpret_cast<const T *>(a.k) + (n0 + t) * a.k_token + (h - a.Hq) * a.k_head;
+            else at = reinterpret_cast<const T *>(a.v) + (n0 + t) * a.v_token + (h - a.Hq - a.Hkv) * a.v_head;
+            x[j][0] = *reinterpret_cast<const uint4 *>(at + c0);
+            x[j][1] = *reinterpret_cast<const uint4 *>(at + c1);
+        }
+    };
+    load(first);
+    const int pairs = (int)a.rotary / 2;
+    for (int t = tid / 32; t < tokens; t += ROTARY_THREADS / 32) {
+        const int position = pairs ? a.positions[n0 + t] : 0;
+        for (int i = tid & 31; i < pairs; i += 32) {
+            const float2 cs = turn(position, a.frequencies[i], a.factor, a.inverse != 0);
+            reinterpret_cast<float2 *>(turns)[((t * 4 + (i & 7) / 2) * rotated + i / 8) * 2 + (i & 1)] = cs;
+        }
+    }
+    if (a.Hkv && tid < tokens) {
+        int flags = 0;
+        places[tid] = place_of(p, n0 + tid, flags);
+        raise_flag(a.status, flags);
+    }
+    __syncthreads();
+    if (first >= lanes) return;
+    for (int from = first; from < rows; from += AT_ONCE * lanes) {
+        if (from != first) load(from);
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; j++) {
+            const int r = from + j * lanes;
+            if (r >= rows) break;
+            const int t = kvc_divide(skip + r, p.heads), h = skip + r - t * H;
+            T *to;
+            if (h < a.Hq) to = reinterpret_cast<T *>(a.q_out) + (n0 + t) * a.out_token + h * a.out_head;
+            else {
+                const bool key = h < a.Hq + a.Hkv;
+                const long long at = key ? places[t].k : places[t].v;
+                if (at < 0) continue;
+                to = key ? reinterpret_cast<T *>(a.kpages) + at + (h - a.Hq) * a.kp_head : reinterpret_cast<T *>(a.vpages) + at + (h - a.Hq - a.Hkv) * a.vp_head;
+            }
+            uint4 y0 = x[j][0], y1 = x[j][1];
+            if (u < rotated && h < a.Hq + a.Hkv) {
+                // pairs: with halves a value of the first piece and its like of the second, else neighbours
+                uint32_t w[8] = {y0.x, y0.y, y0.z, y0.w, y1.x, y1.y, y1.z, y1.w};
+                const float4 *const at_turn = turns + t * 4 * rotated + u;
+                if (half) {
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const float4 cs = at_turn[k * rotated];
+                        const float2 f = unpack(w[k], T()), g = unpack(w[4 + k], T());
+                        w[k] = pack(f.x * cs.x - g.x * cs.y, f.y * cs.z - g.y * cs.w, T());
+                        w[4 + k] = pack(g.x * cs.x + f.x * cs.y, g.y * cs.z + f.y * cs.w, T());
+                    }
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const float4 cs = at_turn[k * rotated];
+                        const float2 f = unpack(w[2 * k], T()), g = unpack(w[2 * k + 1], T());
+                        w[2 * k] = pack(f.x * cs.x - f.y * cs.y, f.y * cs.x + f.x * cs.y, T());
+                        w[2 * k + 1] = pack(g.x * cs.z - g.y * cs.w, g.y * cs.z + g.x * cs.w, T());
+                    }
+                }
+                y0 = make_uint4(w[0], w[1], w[2], w[3]);
+                y1 = make_uint4(w[4], w[5], w[6], w[7]);
+            }
+            *reinterpret_cast<uint4 *>(to + c0) = y0;
+            *reinterpret_cast<uint4 *>(to + c1) = y1;
+        }
+    }
+}
+
+// Any sizes and strides: a thread per pair or copied channel.
+template <typename T>
+__global__ void __launch_bounds__(256) rotary_any_kernel(const __grid_constant__ RotaryParams p) {
+    const kvc_rotary_args &a = p.a;
     const int half = (int)a.rotary / 2, units = (int)a.D - half;
     const long long heads = a.Hq + 2 * a.Hkv, i = (long long)blockIdx.x * 256 + threadIdx.x;
     if (i >= a.N * heads * units) return;
@@ -195,20 +402,18 @@ __global__ void __launch_bounds__(256) rotary_kernel(const kvc_rotary_args a) {
     } else {
         const bool key = h < a.Hq + a.Hkv;
         const long long hk = h - a.Hq - (key ? 0 : a.Hkv);
-        const int slot = a.slots[n];
-        if (slot < 0) return;
-        if (slot >= a.n_pages * a.page_size) { raise_flag(a.status, KVC_FLAG_BAD_PAGE); return; }
-        const long long page = slot / a.page_size, row = slot % a.page_size;
+        int flags = 0;
+        const Place at = place_of(p, n, flags);
+        raise_flag(a.status, flags);
+        if (at.k < 0) return;
         x = key ? reinterpret_cast<const T *>(a.k) + n * a.k_token + hk * a.k_head : reinterpret_cast<const T *>(a.v) + n * a.v_token + hk * a.v_head;
-        y = key ? reinterpret_cast<T *>(a.kpages) + page * a.kp_page + row * a.kp_row + hk * a.kp_head
-                : reinterpret_cast<T *>(a.vpages) + page * a.vp_page + row * a.vp_row + hk * a.vp_head;
+        y = key ? reinterpret_cast<T *>(a.kpages) + at.k + hk * a.kp_head : reinterpret_cast<T *>(a.vpages) + at.v + hk * a.vp_head;
     }
     if (u >= half) { y[half + u] = x[half + u]; return; }
     const int i0 = a.layout == KVC_ROTARY_HALF ? u : 2 * u, i1 = a.layout == KVC_ROTARY_HALF ? u + half : 2 * u + 1;
     const T x0 = x[i0], x1 = x[i1];
     if (h >= a.Hq + a.Hkv) { y[i0] = x0; y[i1] = x1; return; }
-    float2 cs = turn(a.positions[n], a.frequencies[u], a.factor);
-    if (a.inverse) cs.y = -cs.y;
+    const float2 cs = turn(a.positions[n], a.frequencies[u], a.factor, a.inverse != 0);
     const float f0 = to_float(x0), f1 = to_float(x1);
     y[i0] = from_float<T>(f0 * cs.x - f1 * cs.y);
     y[i1] = from_float<T>(f1 * cs.x + f0 * cs.y);
@@ -218,50 +423,104 @@ __global__ void __launch_bounds__(256) rotary_kernel(const kvc_rotary_args a) {
 
 extern "C" int kvc_page_plan(const kvc_page_plan_args *args, kvc_stream_t stream) {
     KVC_REQUIRE(args, "kvc_page_plan: null pointer");
-    kvc_page_plan_args a;
-    memcpy(&a, args, sizeof(a));
-    KVC_REQUIRE(a.B >= 0 && a.B < (1 << 24) && a.n_pages >= 0 && a.page_size > 0 && a.page_size <= MAX_PAGE && a.tokens >= 0 && a.tokens < (1ll << 31),
+    PlanParams p;
+    memcpy(&p.a, args, sizeof(p.a));
+    const kvc_page_plan_args &a = p.a;
+    KVC_REQUIRE(a.B >= 0 && a.B < (1 << 24) && a.n_pages >= 0 && a.page_size > 0 && a.page_size <= KVC_MAX_PAGE && a.tokens >= 0 && a.tokens < (1ll << 31) - 4,
                 "kvc_page_plan: bad sizes");
     KVC_REQUIRE(a.n_pages * a.page_size < (1ll << 31), "kvc_page_plan: slots have 32 bits, the pool %lld tokens", (long long)(a.n_pages * a.page_size));
     KVC_REQUIRE(a.table_width >= 0 && a.table_width < (1ll << 31) && (a.B <= 1 || a.table_stride >= a.table_width), "kvc_page_plan: rows of the table overlap");
     KVC_REQUIRE(a.head && a.head_out && a.starts && (a.B == 0 || (a.lengths && a.new_tokens && a.lengths_out && a.taken)) && (a.free_pages || a.n_pages == 0) &&
                     (a.table || a.B == 0 || a.table_width == 0) && (a.tokens == 0 || (a.slots && a.positions)), "kvc_page_plan: null pointer");
-    page_plan_kernel<<<1, SCAN_THREADS, 0, kvc_cu(stream)>>>(a);
+    p.page = kvc_make_div((uint32_t)a.page_size);
+    cudaStream_t s = kvc_cu(stream);
+    if (a.tokens > FILL_ALONE) {
+        page_plan_kernel<SCAN_THREADS, false><<<1, SCAN_THREADS, 0, s>>>(p);
+        KVC_LAUNCH_OK();
+        return launch_fill(plan_rows_kernel, (unsigned)((a.tokens + 4 * FILL_THREADS - 1) / (4 * FILL_THREADS)), p, s);
+    }
+    if (a.B <= SMALL_THREADS && a.tokens <= 4 * SMALL_THREADS) page_plan_kernel<SMALL_THREADS, true><<<1, SMALL_THREADS, 0, s>>>(p);
+    else page_plan_kernel<SCAN_THREADS, true><<<1, SCAN_THREADS, 0, s>>>(p);
     KVC_LAUNCH_OK();
     return KVC_OK;
 }
 
 extern "C" int kvc_page_release(const kvc_page_release_args *args, kvc_stream_t stream) {
     KVC_REQUIRE(args, "kvc_page_release: null pointer");
-    kvc_page_release_args a;
-    memcpy(&a, args, sizeof(a));
-    KVC_REQUIRE(a.B >= 0 && a.B < (1 << 24) && a.n_pages >= 0 && a.page_size > 0 && a.page_size <= MAX_PAGE && a.n_pages * a.page_size < (1ll << 31),
+    ReleaseParams p;
+    memcpy(&p.a, args, sizeof(p.a));
+    const kvc_page_release_args &a = p.a;
+    KVC_REQUIRE(a.B >= 0 && a.B < (1 << 24) && a.n_pages >= 0 && a.page_size > 0 && a.page_size <= KVC_MAX_PAGE && a.n_pages * a.page_size < (1ll << 31),
                 "kvc_page_release: bad sizes");
     KVC_REQUIRE(a.table_width >= 0 && a.table_width < (1ll << 31) && (a.B <= 1 || a.table_stride >= a.table_width), "kvc_page_release: rows of the table overlap");
     KVC_REQUIRE(a.head && a.head_out && a.first && (a.B == 0 || (a.lengths && a.done && a.lengths_out)) && (a.free_pages || a.n_pages == 0) &&
                     (a.table || a.B == 0 || a.table_width == 0), "kvc_page_release: null pointer");
-    page_release_kernel<<<1, SCAN_THREADS, 0, kvc_cu(stream)>>>(a);
+    p.page = kvc_make_div((uint32_t)a.page_size);
+    cudaStream_t s = kvc_cu(stream);
+    // (how many pages come back is known on the device only: at most so many)
+    const int64_t most = a.table_width == 0 ? 0 : std::min(a.n_pages, a.B * a.table_width);
+    if (most > FILL_ALONE) {
+        page_release_kernel<SCAN_THREADS, false><<<1, SCAN_THREADS, 0, s>>>(p);
+        KVC_LAUNCH_OK();
+        return launch_fill(release_rows_kernel, (unsigned)std::min<int64_t>((most + 4 * FILL_THREADS - 1) / (4 * FILL_THREADS), 4ll * kvc_sm_count()), p, s);
+    }
+    if (a.B <= SMALL_THREADS && most <= 8 * SMALL_THREADS) page_release_kernel<SMALL_THREADS, true><<<1, SMALL_THREADS, 0, s>>>(p);
+    else page_release_kernel<SCAN_THREADS, true><<<1, SCAN_THREADS, 0, s>>>(p);
     KVC_LAUNCH_OK();
     return KVC_OK;
 }
 
 extern "C" int kvc_rotary_store(const kvc_rotary_args *args, kvc_stream_t stream) {
     KVC_REQUIRE(args, "kvc_rotary_store: null pointer");
-    kvc_rotary_args a;
-    memcpy(&a, args, sizeof(a));
+    RotaryParams p;
+    memcpy(&p.a, args, sizeof(p.a));
+    kvc_rotary_args &a = p.a;
     KVC_REQUIRE(a.type == KVC_TYPE_FP16 || a.type == KVC_TYPE_BF16, "kvc_rotary_store: unknown type %d", a.type);
     KVC_REQUIRE(a.layout == KVC_ROTARY_HALF || a.layout == KVC_ROTARY_INTERLEAVED, "kvc_rotary_store: unknown layout %d", a.layout);
     KVC_REQUIRE(a.N >= 0 && a.Hq >= 0 && a.Hkv >= 0 && a.D > 0 && a.D <= 65536 && a.rotary >= 0 && a.rotary <= a.D && a.rotary % 2 == 0,
                 "kvc_rotary_store: bad sizes (head of %lld channels, %lld rotated)", (long long)a.D, (long long)a.rotary);
-    KVC_REQUIRE(a.Hkv == 0 || (a.page_size > 0 && a.page_size <= MAX_PAGE && a.n_pages >= 0 && a.n_pages * a.page_size < (1ll << 31)), "kvc_rotary_store: bad pool");
+    KVC_REQUIRE(a.Hkv == 0 || (a.page_size > 0 && a.page_size <= KVC_MAX_PAGE && a.n_pages >= 0 && a.n_pages * a.page_size < (1ll << 31)), "kvc_rotary_store: bad pool");
     if (a.N == 0 || a.Hq + a.Hkv == 0) return KVC_OK;
     KVC_REQUIRE((a.Hq == 0 || (a.q && a.q_out)) && (a.Hkv == 0 || (a.k && a.v && a.slots && ((a.kpages && a.vpages) || a.n_pages == 0))) &&
                     (a.rotary == 0 || (a.positions && a.frequencies)), "kvc_rotary_store: null pointer");
-    KVC_REQUIRE(a.Hq + 2 * a.Hkv < (1 << 20) && a.N < (1ll << 31), "kvc_rotary_store: too many heads or tokens");
-    const long long n = a.N * (a.Hq + 2 * a.Hkv) * (a.D - a.rotary / 2);
-    KVC_REQUIRE((n + 255) / 256 < (1ll << 31), "kvc_rotary_store: too many elements");
-    auto *kernel = a.type == KVC_TYPE_FP16 ? rotary_kernel<__half> : rotary_kernel<__nv_bfloat16>;
-    kernel<<<(unsigned)((n + 255) / 256), 256, 0, kvc_cu(stream)>>>(a);
+    KVC_REQUIRE(a.Hq < (1 << 20) && a.Hkv < (1 << 20) && a.N < (1ll << 31), "kvc_rotary_store: too many heads or tokens");
+    const long long H = a.Hq + 2 * a.Hkv, rows = a.N * H;
+    p.page = kvc_make_div((uint32_t)std::max<int64_t>(a.page_size, 1));
+    p.heads = kvc_make_div((uint32_t)H);
+    p.slots = a.n_pages * a.page_size;
+    // (the stride of a dimension of one, and what a part that is not there says, may be anything)
+    if (a.Hq == 0) a.q = nullptr, a.q_out = nullptr;
+    if (a.Hkv == 0) a.k = a.v = nullptr, a.kpages = a.vpages = nullptr;
+    if (a.Hq <= 1) a.q_head = a.out_head = 0;
+    if (a.N == 1 || a.Hq == 0) a.q_token = a.out_token = 0;
+    if (a.Hkv <= 1) a.k_head = a.v_head = a.kp_head = a.vp_head = 0;
+    if (a.N == 1 || a.Hkv == 0) a.k_token = a.v_token = 0;
+    if (a.page_size <= 1 || a.Hkv == 0) a.kp_row = a.vp_row = 0;
+    if (a.n_pages <= 1 || a.Hkv == 0) a.kp_page = a.vp_page = 0;
+    const uintptr_t at = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.q_out) | reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) |
+                         reinterpret_cast<uintptr_t>(a.kpages) | reinterpret_cast<uintptr_t>(a.vpages);
+    const int64_t strides = a.q_token | a.q_head | a.k_token | a.k_head | a.v_token | a.v_head | a.out_token | a.out_head | a.kp_page | a.kp_row | a.kp_head | a.vp_page | a.vp_row | a.vp_head;
+    cudaStream_t s = kvc_cu(stream);
+    if ((at & 15) == 0 && (strides & 7) == 0 && a.D % 16 == 0 && a.rotary % 16 == 0 && a.D <= 1024) {
+        const int units = (int)a.D / 16, lanes = ROTARY_THREADS / units;
+        p.units = kvc_make_div((uint32_t)units);
+        // rounds of four rows a thread: as many as leave two CTAs for each that the device holds, so that the angles of a token are made in few of them
+        const long long rounds = rows / ((long long)lanes * AT_ONCE * 8 * kvc_sm_count());
+        p.rows = lanes * AT_ONCE * (int)std::min<long long>(std::max<long long>(rounds, 1), 4);
+        if (rows < (long long)p.rows * 2 * kvc_sm_count()) p.rows = lanes;                    // few: a row for each thread
+        const long long most = std::min<long long>(MAX_TOKENS, 48 * 1024 / (4 * std::max<int64_t>(a.rotary, 1)));      // tokens whose angles have room
+        p.rows = (int)std::min<long long>(p.rows, (most - 1) * H);
+        const long long grid = (rows + p.rows - 1) / p.rows;
+        KVC_REQUIRE(grid < (1ll << 31), "kvc_rotary_store: too many elements");
+        const int tokens = (int)std::min<long long>((p.rows + 2 * H - 2) / H, most);
+        auto *kernel = a.type == KVC_TYPE_FP16 ? rotary_rows_kernel<__half> : rotary_rows_kernel<__nv_bfloat16>;
+        kernel<<<(unsigned)grid, ROTARY_THREADS, (size_t)tokens * a.rotary * 4, s>>>(p);
+    } else {
+        const long long n = rows * (a.D - a.rotary / 2);
+        KVC_REQUIRE((n + 255) / 256 < (1ll << 31), "kvc_rotary_store: too many elements");
+        auto *kernel = a.type == KVC_TYPE_FP16 ? rotary_any_kernel<__half> : rotary_any_kernel<__nv_bfloat16>;
+        kernel<<<(unsigned)((n + 255) / 256), 256, 0, s>>>(p);
+    }
     KVC_LAUNCH_OK();
     return KVC_OK;
 }
