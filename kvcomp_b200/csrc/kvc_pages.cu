@@ -245,8 +245,8 @@ int launch_fill(void (*fill)(const P), unsigned grid, const P &p, cudaStream_t s
 
 // ---- rotation ---------------------------------------------------------------------------------------------------
 //
-// Every value is read once and written once: HBM for a prompt, latency for a step.  cos and sin are made once for a (token,
-// frequency) and CTA, not once for a head, and wait in shared memory.
+// Every value is read once and written once: HBM for a prompt, latency for a step.  cos and sin are made once for a token and several of its
+// heads, in registers, while the first of these are on their way.
 
 template <typename T> __device__ __forceinline__ float to_float(T v);
 template <> __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
@@ -259,24 +259,45 @@ __device__ __forceinline__ float2 unpack(uint32_t v, __nv_bfloat16) { return __b
 __device__ __forceinline__ uint32_t pack(float a, float b, __half) { const __half2 r = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t *>(&r); }
 __device__ __forceinline__ uint32_t pack(float a, float b, __nv_bfloat16) { const __nv_bfloat162 r = __floats2bfloat162_rn(a, b); return *reinterpret_cast<const uint32_t *>(&r); }
 
-// cos and sin of position * frequency.  The turns are counted in fp64: what is left of a far position's angle after its whole
-// turns keeps 2^-53 of the angle, 1e-10 at a million radians; fp32 would keep 0.06.
-__device__ __forceinline__ float2 turn(int position, double frequency, float factor, bool inverse) {
-    double t = (double)position * (frequency * 0.15915494309189533576888);
-    t -= rint(t);
-    float s, c;
-    sincospif(2.0f * (float)t, &s, &c);
-    return make_float2(c * factor, inverse ? -s * factor : s * factor);
+// cos and sin of a position, given the turns of one step.  The turns are counted in fp64: what is left of a far position's angle after its whole
+// turns keeps 2^-53 of the angle, 1e-10 at a million radians; fp32 would keep 0.06.  Of the rest the nearest quarter is taken off, and the series of sine and cosine on
+// [-pi / 4, pi / 4] are left, to the terms below 2^-31.
+constexpr double TURNS_OF_RADIANS = 0.15915494309189533576888;
+__device__ __forceinline__ float2 turn(double position, double turns, float factor) {
+    double whole = position * turns;
+    whole -= rint(whole);
+    const float t = (float)whole, quarter = rintf(4.0f * t), x = fmaf(-0.25f, quarter, t) * 6.2831853071795865f, y = x * x;
+    const int q = (int)quarter;
+    float s = fmaf(y, 1.0f / 362880, -1.0f / 5040), c = fmaf(y, -1.0f / 3628800, 1.0f / 40320);
+    s = fmaf(y, s, 1.0f / 120);
+    c = fmaf(y, c, -1.0f / 720);
+    s = fmaf(y, s, -1.0f / 6);
+    c = fmaf(y, c, 1.0f / 24);
+    s = fmaf(x * y, s, x);
+    c = fmaf(y, c, -0.5f);
+    c = fmaf(y, c, 1.0f);
+    const float a = q & 1 ? s : c, b = q & 1 ? c : s;
+    return make_float2(((q + 1) & 2 ? -a : a) * factor, (q & 2 ? -b : b) * factor);
 }
+
+// Queries, keys or values: a CTA has rows of one of them.  dst: token stride 0 for the pools, where `places` say where a token goes.
+struct Part {
+    const void *src;
+    void *dst;
+    int64_t src_token, src_head, dst_token, dst_head;
+    int heads, chunk, of_token, turned;                     // heads, those that a thread takes, threads' shares of a token, rotated units of a head
+    unsigned first;                                         // CTA
+    kvc_div chunks;                                         // by of_token
+};
 
 struct RotaryParams {
     kvc_rotary_args a;
-    kvc_div page, heads, units;                             // divisors: page size, Hq + 2 Hkv, D / 16
-    int rows;                                               // (token, head) rows of a CTA
+    kvc_div page, units;                                    // divisors: page size, D / 16
     long long slots;                                        // of the pool
+    Part parts[3];
 };
 
-// Where a CTA's tokens go: element offsets of their rows in the pools, -1: nowhere
+// Where a token goes: element offsets of its row in the pools, -1: nowhere
 struct Place { long long k, v; };
 
 __device__ __forceinline__ Place place_of(const RotaryParams &p, long long n, int &flags) {
@@ -291,96 +312,74 @@ __device__ __forceinline__ Place place_of(const RotaryParams &p, long long n, in
     return r;
 }
 
-constexpr int ROTARY_THREADS = 256, AT_ONCE = 4, MAX_TOKENS = 32;
+constexpr int ROTARY_THREADS = 256, ROTARY_CTAS = 3, CHUNK = 4;
 
-// Heads of 16 n channels, rotated by multiples of 16, everything on 16 bytes.  A thread has a unit of 16 channels (8 pairs: two pieces of 16 bytes,
-// half the rotated channels apart, or next to each other) of four rows at a time; the first four are asked for before the
-// angles are made.
+// Heads of 16 n channels, rotated by multiples of 16, everything on 16 bytes.  A thread has a unit of 16 channels (8 pairs: two pieces of 16
+// bytes, half the rotated channels apart, or next to each other) of up to CHUNK heads of a token: its 8 angles serve them all, and no thread waits for another.
+// Queries, keys and values have CTAs of their own, so that all that is picked by kind is picked for a CTA.
+// Measured: 16384 tokens of 40 + 10 + 10 heads of 128 channels (503 MB) 78.5 us, 6.4 TB/s; with the angles of a CTA's tokens in shared memory, made behind a
+// barrier, 84.5 to 89; CHUNK 8 79.2, 5 82.7; at most two heads under way 79.5, two CTAs per SM 88, four (spilling) 97.  32749 tokens of 8 heads (134 MB) 22.7 us, before 28.6.
 template <typename T>
-__global__ void __launch_bounds__(ROTARY_THREADS, 4) rotary_rows_kernel(const __grid_constant__ RotaryParams p) {
-    extern __shared__ float4 turns[];                       // [token][2 pairs of a unit][unit]: cos, sin, cos, sin
-    __shared__ Place places[MAX_TOKENS];
+__global__ void __launch_bounds__(ROTARY_THREADS, ROTARY_CTAS) rotary_rows_kernel(const __grid_constant__ RotaryParams p) {
     const kvc_rotary_args &a = p.a;
-    const int units = (int)a.D / 16, rotated = (int)a.rotary / 16, H = (int)(a.Hq + 2 * a.Hkv), tid = threadIdx.x;
-    const long long row0 = (long long)blockIdx.x * p.rows, n0 = row0 / H;
-    const int skip = (int)(row0 - n0 * H), rows = (int)min((long long)p.rows, a.N * H - row0);
-    const int tokens = kvc_divide(skip + rows - 1, p.heads) + 1, lanes = ROTARY_THREADS / units, first = kvc_divide(tid, p.units), u = tid - first * units;
-    const bool half = a.layout == KVC_ROTARY_HALF && u < rotated;
-    const int c0 = half ? 8 * u : 16 * u, c1 = half ? 8 * (u + rotated) : 16 * u + 8;
-    uint4 x[AT_ONCE][2];
-    auto load = [&](int from) {
+    const int which = blockIdx.x >= p.parts[2].first ? 2 : (blockIdx.x >= p.parts[1].first ? 1 : 0);
+    const Part &part = p.parts[which];
+    const int units = (int)a.D / 16, turned = part.turned, id = (int)((blockIdx.x - part.first) * ROTARY_THREADS + threadIdx.x);
+    const int group = kvc_divide(id, p.units), u = id - group * units, n = kvc_divide(group, part.chunks);
+    if (n >= a.N) return;
+    const int h0 = (group - n * part.of_token) * part.chunk, heads = min(part.chunk, part.heads - h0);
+    const bool half = a.layout == KVC_ROTARY_HALF && u < turned;
+    const int c0 = half ? 8 * u : 16 * u, apart = half ? 8 * turned : 8;
+    const T *src = reinterpret_cast<const T *>(part.src) + n * part.src_token + h0 * part.src_head + c0;
+    T *dst = reinterpret_cast<T *>(part.dst) + n * part.dst_token + h0 * part.dst_head + c0;
+    uint4 x[CHUNK][2];
 #pragma unroll
-        for (int j = 0; j < AT_ONCE; j++) {
-            const int r = from + j * lanes;
-            if (first >= lanes || r >= rows) continue;
-            const int t = kvc_divide(skip + r, p.heads), h = skip + r - t * H;
-            const T *at;
-            if (h < a.Hq) at = reinterpret_cast<const T *>(a.q) + (n0 + t) * a.q_token + h * a.q_head;
-            else if (h < a.Hq + a.Hkv) at = reinterpret_cast<const T *>(a.k) + (n0 + t) * a.k_token + (h - a.Hq) * a.k_head;
-            else at = reinterpret_cast<const T *>(a.v) + (n0 + t) * a.v_token + (h - a.Hq - a.Hkv) * a.v_head;
-            x[j][0] = *reinterpret_cast<const uint4 *>(at + c0);
-            x[j][1] = *reinterpret_cast<const uint4 *>(at + c1);
+    for (int j = 0; j < CHUNK; j++) {
+        if (j < heads) {
+            x[j][0] = *reinterpret_cast<const uint4 *>(src);
+            x[j][1] = *reinterpret_cast<const uint4 *>(src + apart);
         }
-    };
-    load(first);
-    const int pairs = (int)a.rotary / 2;
-    for (int t = tid / 32; t < tokens; t += ROTARY_THREADS / 32) {
-        const int position = pairs ? a.positions[n0 + t] : 0;
-        for (int i = tid & 31; i < pairs; i += 32) {
-            const float2 cs = turn(position, a.frequencies[i], a.factor, a.inverse != 0);
-            reinterpret_cast<float2 *>(turns)[((t * 4 + (i & 7) / 2) * rotated + i / 8) * 2 + (i & 1)] = cs;
-        }
+        src += part.src_head;
     }
-    if (a.Hkv && tid < tokens) {
+    if (which > 0) {
         int flags = 0;
-        places[tid] = place_of(p, n0 + tid, flags);
+        const Place at = place_of(p, n, flags);
         raise_flag(a.status, flags);
+        if (at.k < 0) return;
+        dst += which == 1 ? at.k : at.v;
     }
-    __syncthreads();
-    if (first >= lanes) return;
-    for (int from = first; from < rows; from += AT_ONCE * lanes) {
-        if (from != first) load(from);
+    const bool turns = u < turned;
+    float2 cs[8];
+    if (turns) {
+        const double position = a.inverse ? -(double)a.positions[n] : (double)a.positions[n];
 #pragma unroll
-        for (int j = 0; j < AT_ONCE; j++) {
-            const int r = from + j * lanes;
-            if (r >= rows) break;
-            const int t = kvc_divide(skip + r, p.heads), h = skip + r - t * H;
-            T *to;
-            if (h < a.Hq) to = reinterpret_cast<T *>(a.q_out) + (n0 + t) * a.out_token + h * a.out_head;
-            else {
-                const bool key = h < a.Hq + a.Hkv;
-                const long long at = key ? places[t].k : places[t].v;
-                if (at < 0) continue;
-                to = key ? reinterpret_cast<T *>(a.kpages) + at + (h - a.Hq) * a.kp_head : reinterpret_cast<T *>(a.vpages) + at + (h - a.Hq - a.Hkv) * a.vp_head;
-            }
-            uint4 y0 = x[j][0], y1 = x[j][1];
-            if (u < rotated && h < a.Hq + a.Hkv) {
+        for (int k = 0; k < 8; k++) cs[k] = turn(position, a.frequencies[8 * u + k] * TURNS_OF_RADIANS, a.factor);
+    }
+#pragma unroll
+    for (int j = 0; j < CHUNK; j++) {
+        if (j < heads) {
+            uint32_t w[8] = {x[j][0].x, x[j][0].y, x[j][0].z, x[j][0].w, x[j][1].x, x[j][1].y, x[j][1].z, x[j][1].w};
+            if (turns) {
                 // pairs: with halves a value of the first piece and its like of the second, else neighbours
-                uint32_t w[8] = {y0.x, y0.y, y0.z, y0.w, y1.x, y1.y, y1.z, y1.w};
-                const float4 *const at_turn = turns + t * 4 * rotated + u;
                 if (half) {
 #pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        const float4 cs = at_turn[k * rotated];
-                        const float2 f = unpack(w[k], T()), g = unpack(w[4 + k], T());
-                        w[k] = pack(f.x * cs.x - g.x * cs.y, f.y * cs.z - g.y * cs.w, T());
-                        w[4 + k] = pack(g.x * cs.x + f.x * cs.y, g.y * cs.z + f.y * cs.w, T());
+                    for (int m = 0; m < 4; m++) {
+                        const float2 f = unpack(w[m], T()), g = unpack(w[4 + m], T()), c = cs[2 * m], d = cs[2 * m + 1];
+                        w[m] = pack(f.x * c.x - g.x * c.y, f.y * d.x - g.y * d.y, T());
+                        w[4 + m] = pack(g.x * c.x + f.x * c.y, g.y * d.x + f.y * d.y, T());
                     }
                 } else {
 #pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        const float4 cs = at_turn[k * rotated];
-                        const float2 f = unpack(w[2 * k], T()), g = unpack(w[2 * k + 1], T());
-                        w[2 * k] = pack(f.x * cs.x - f.y * cs.y, f.y * cs.x + f.x * cs.y, T());
-                        w[2 * k + 1] = pack(g.x * cs.z - g.y * cs.w, g.y * cs.z + g.x * cs.w, T());
+                    for (int m = 0; m < 8; m++) {
+                        const float2 f = unpack(w[m], T());
+                        w[m] = pack(f.x * cs[m].x - f.y * cs[m].y, f.y * cs[m].x + f.x * cs[m].y, T());
                     }
                 }
-                y0 = make_uint4(w[0], w[1], w[2], w[3]);
-                y1 = make_uint4(w[4], w[5], w[6], w[7]);
             }
-            *reinterpret_cast<uint4 *>(to + c0) = y0;
-            *reinterpret_cast<uint4 *>(to + c1) = y1;
+            *reinterpret_cast<uint4 *>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+            *reinterpret_cast<uint4 *>(dst + apart) = make_uint4(w[4], w[5], w[6], w[7]);
         }
+        dst += part.dst_head;
     }
 }
 
@@ -413,7 +412,7 @@ __global__ void __launch_bounds__(256) rotary_any_kernel(const __grid_constant__
     const int i0 = a.layout == KVC_ROTARY_HALF ? u : 2 * u, i1 = a.layout == KVC_ROTARY_HALF ? u + half : 2 * u + 1;
     const T x0 = x[i0], x1 = x[i1];
     if (h >= a.Hq + a.Hkv) { y[i0] = x0; y[i1] = x1; return; }
-    const float2 cs = turn(a.positions[n], a.frequencies[u], a.factor, a.inverse != 0);
+    const float2 cs = turn(a.inverse ? -(double)a.positions[n] : (double)a.positions[n], a.frequencies[u] * TURNS_OF_RADIANS, a.factor);
     const float f0 = to_float(x0), f1 = to_float(x1);
     y[i0] = from_float<T>(f0 * cs.x - f1 * cs.y);
     y[i1] = from_float<T>(f1 * cs.x + f0 * cs.y);
@@ -486,7 +485,6 @@ extern "C" int kvc_rotary_store(const kvc_rotary_args *args, kvc_stream_t stream
     KVC_REQUIRE(a.Hq < (1 << 20) && a.Hkv < (1 << 20) && a.N < (1ll << 31), "kvc_rotary_store: too many heads or tokens");
     const long long H = a.Hq + 2 * a.Hkv, rows = a.N * H;
     p.page = kvc_make_div((uint32_t)std::max<int64_t>(a.page_size, 1));
-    p.heads = kvc_make_div((uint32_t)H);
     p.slots = a.n_pages * a.page_size;
     // (the stride of a dimension of one, and what a part that is not there says, may be anything)
     if (a.Hq == 0) a.q = nullptr, a.q_out = nullptr;
@@ -501,20 +499,28 @@ extern "C" int kvc_rotary_store(const kvc_rotary_args *args, kvc_stream_t stream
                          reinterpret_cast<uintptr_t>(a.kpages) | reinterpret_cast<uintptr_t>(a.vpages);
     const int64_t strides = a.q_token | a.q_head | a.k_token | a.k_head | a.v_token | a.v_head | a.out_token | a.out_head | a.kp_page | a.kp_row | a.kp_head | a.vp_page | a.vp_row | a.vp_head;
     cudaStream_t s = kvc_cu(stream);
-    if ((at & 15) == 0 && (strides & 7) == 0 && a.D % 16 == 0 && a.rotary % 16 == 0 && a.D <= 1024) {
-        const int units = (int)a.D / 16, lanes = ROTARY_THREADS / units;
+    if ((at & 15) == 0 && (strides & 7) == 0 && a.D % 16 == 0 && a.rotary % 16 == 0 && rows * (a.D / 16) < (1ll << 31) - ROTARY_THREADS) {
+        const int units = (int)a.D / 16;
         p.units = kvc_make_div((uint32_t)units);
-        // rounds of four rows a thread: as many as leave two CTAs for each that the device holds, so that the angles of a token are made in few of them
-        const long long rounds = rows / ((long long)lanes * AT_ONCE * 8 * kvc_sm_count());
-        p.rows = lanes * AT_ONCE * (int)std::min<long long>(std::max<long long>(rounds, 1), 4);
-        if (rows < (long long)p.rows * 2 * kvc_sm_count()) p.rows = lanes;                    // few: a row for each thread
-        const long long most = std::min<long long>(MAX_TOKENS, 48 * 1024 / (4 * std::max<int64_t>(a.rotary, 1)));      // tokens whose angles have room
-        p.rows = (int)std::min<long long>(p.rows, (most - 1) * H);
-        const long long grid = (rows + p.rows - 1) / p.rows;
-        KVC_REQUIRE(grid < (1ll << 31), "kvc_rotary_store: too many elements");
-        const int tokens = (int)std::min<long long>((p.rows + 2 * H - 2) / H, most);
+        p.parts[0] = {a.q, a.q_out, a.q_token, a.q_head, a.out_token, a.out_head, (int)a.Hq};
+        p.parts[1] = {a.k, a.kpages, a.k_token, a.k_head, 0, a.kp_head, (int)a.Hkv};
+        p.parts[2] = {a.v, a.vpages, a.v_token, a.v_head, 0, a.vp_head, (int)a.Hkv};
+        // heads of a thread: CHUNK share its angles, unless that leaves too few threads for the device's latency
+        const long long threads = (long long)ROTARY_CTAS * ROTARY_THREADS * kvc_sm_count();
+        const int chunk = (int)std::max<long long>(1, std::min<long long>(CHUNK, rows * units / threads));
+        int64_t grid = 0;
+        for (int i = 0; i < 3; i++) {
+            Part &part = p.parts[i];
+            const int chunks = std::max((part.heads + chunk - 1) / chunk, 1);
+            part.chunk = std::max((part.heads + chunks - 1) / chunks, 1);
+            part.of_token = chunks;
+            part.chunks = kvc_make_div((uint32_t)chunks);
+            part.turned = i < 2 ? (int)a.rotary / 16 : 0;
+            part.first = (unsigned)grid;
+            if (part.heads > 0) grid += (a.N * chunks * units + ROTARY_THREADS - 1) / ROTARY_THREADS;
+        }
         auto *kernel = a.type == KVC_TYPE_FP16 ? rotary_rows_kernel<__half> : rotary_rows_kernel<__nv_bfloat16>;
-        kernel<<<(unsigned)grid, ROTARY_THREADS, (size_t)tokens * a.rotary * 4, s>>>(p);
+        kernel<<<(unsigned)grid, ROTARY_THREADS, 0, s>>>(p);
     } else {
         const long long n = rows * (a.D - a.rotary / 2);
         KVC_REQUIRE((n + 255) / 256 < (1ll << 31), "kvc_rotary_store: too many elements");
