@@ -9,7 +9,7 @@
 // Work is cut into tiles of 64 tokens of a column (a request's KV head), all tiles of all columns in one row; each CTA takes an equal, contiguous
 // share of the row, found from the lengths in the kernel (the host does not know them).  Lengths may be as unequal as they like, and a
 // single long request is spread over the device.  A column that lies in one share is written at once; one that was cut leaves partial results {m, l,
-// sums} in the workspace, and the CTA that finishes last (a counter per column, put back to zero) joins them in the order of the shares, so that
+// sums} in the workspace, and the CTA that finishes last (a counter, put back to zero) joins them in the order of the shares, so that
 // the result does not depend on who that was.
 //
 // Four warps take 16 of a tile's tokens each, with a ring of stages of their own that they fill with 16-byte asynchronous copies (any strides,
@@ -33,9 +33,8 @@ namespace {
 constexpr int WARPS = 4, THREADS = WARPS * 32;
 constexpr int TILE = 16 * WARPS;                // tokens of a tile
 constexpr int MAX_CTAS_PER_SM = 4;
-#ifndef KVC_MIN_TILES
-#define KVC_MIN_TILES 2
-#endif
+constexpr int JOINED = 8;                       // partial results that are asked for at once
+constexpr int MIN_TILES = 2;                    // of a share
 #ifndef KVC_SC
 #define KVC_SC 3, 4, 4, 3
 #endif
@@ -57,9 +56,9 @@ struct Params {
     int most_tokens;                            // of a table row
     unsigned n_pages;
     uint32_t sign;                              // of the scaling, for two values: the scores' maximum is taken before they are scaled
-    float log2_scaling;
+    float log2_scaling, per_cta;                // per_cta: a little less than one over the number of CTAs
     long long v_less_k;                         // bytes from the keys' pool to the values'
-    unsigned *counters;
+    unsigned *counters, *group_counters;        // of the places of partial results
     float *parts;
 };
 
@@ -151,8 +150,8 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
     __shared__ uint32_t masks[WARPS][STAGES];
     __shared__ float2 ml_s[WARPS][8 * NT];                  // maximum and sum
     __shared__ float4 join_v[THREADS];
-    __shared__ float2 join_ml[THREADS];
-    __shared__ long long scan_s[WARPS];
+    __shared__ float2 join_ml[THREADS], new_ml[MAX_GROUP];
+    __shared__ int4 scan_s[3][WARPS];
     __shared__ Place start_s;
     __shared__ int last_s;
     const kvc_paged_attn_args &a = p.a;
@@ -160,41 +159,78 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
     int flags = 0;
 
     // ---- this CTA's share
-    long long r0, r1, total, size;                          // (size: tiles of a share)
+    // Whole parts of columns, one for each CTA, where all columns together have no more of them than there are CTAs (few columns): no CTA has two to finish then.  Else
+    // equal shares of the row of all columns' tiles.  (All of it is on the way of the first byte: 32 bits, no division by what is known before.)
+    int r0, r1, size;                                       // tiles [r0, r1) of the row, shares of `size`; or with even != 0: CTA r0, r1 = r0 + 1
+    int even = 0, parts = 1;                                // tiles of a part at most; this column's parts
     {
-        const int chunk = (B + THREADS - 1) / THREADS, b0 = min(B, tid * chunk), b1 = min(B, b0 + chunk);
-        long long mine = 0;
-        for (int b = b0; b < b1; b++) mine += tiles_of(span_of(p, b, flags));
-        long long upto = mine;
+        const int chunk = B <= THREADS ? 1 : (B + THREADS - 1) / THREADS, b0 = min(B, tid * chunk), b1 = min(B, b0 + chunk);
+        const int n0 = b0 < b1 ? tiles_of(span_of(p, b0, flags)) : 0;
+        unsigned mine = n0, some = n0 > 0;
+        for (int b = b0 + 1; b < b1; b++) {
+            const int n = tiles_of(span_of(p, b, flags));
+            mine += n;
+            some += n > 0;
+        }
+        const unsigned sum = __reduce_add_sync(0xffffffffu, mine), columns = __reduce_add_sync(0xffffffffu, some);
+        if (lane == 0) scan_s[0][warp] = make_int4((int)sum, (int)columns, 0, 0);
+        __syncthreads();
+        unsigned total = 0, there = 0;
+#pragma unroll
+        for (int w = 0; w < WARPS; w++) { total += scan_s[0][w].x; there += scan_s[0][w].y; }
+        total *= p.columns;
+        size = max(MIN_TILES, (int)((float)total * p.per_cta));
+        while ((unsigned)size * gridDim.x < total) size += 1 + (size >> 20);       // (the float is a little below the quotient)
+        // the tiles that a part of `tiles` tiles at most needs, for this thread's requests
+        auto count = [&](int tiles) {
+            unsigned k = ((unsigned)n0 + tiles - 1) / (unsigned)tiles;
+            int unused = 0;
+            for (int b = b0 + 1; b < b1; b++) k += ((unsigned)tiles_of(span_of(p, b, unused)) + tiles - 1) / (unsigned)tiles;
+            return k;
+        };
+        if (there * p.columns <= gridDim.x) {
+            const int step = max(1, size / 16);
+            const unsigned k0 = __reduce_add_sync(0xffffffffu, count(size)), k1 = __reduce_add_sync(0xffffffffu, count(size + step)), k2 = __reduce_add_sync(0xffffffffu, count(size + 2 * step));
+            if (lane == 0) scan_s[1][warp] = make_int4((int)k0, (int)k1, (int)k2, 0);
+            __syncthreads();
+            unsigned all0 = 0, all1 = 0, all2 = 0;
+#pragma unroll
+            for (int w = 0; w < WARPS; w++) { all0 += scan_s[1][w].x; all1 += scan_s[1][w].y; all2 += scan_s[1][w].z; }
+            if (all0 * p.columns <= gridDim.x) even = size;
+            else if (all1 * p.columns <= gridDim.x) even = size + step;
+            else if (all2 * p.columns <= gridDim.x) even = size + 2 * step;
+            if (even) mine = count(even);
+        }
+        unsigned upto = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const long long u = __shfl_up_sync(0xffffffffu, upto, o);
+            const unsigned u = __shfl_up_sync(0xffffffffu, upto, o);
             if (lane >= o) upto += u;
         }
-        if (lane == 31) scan_s[warp] = upto;
+        if (lane == 31) scan_s[2][warp] = make_int4((int)upto, 0, 0, 0);
         __syncthreads();
-        long long before = 0, all = 0;
+        unsigned before = upto - mine, all = 0;
+#pragma unroll
         for (int w = 0; w < WARPS; w++) {
-            if (w < warp) before += scan_s[w];
-            all += scan_s[w];
+            if (w < warp) before += scan_s[2][w].x;
+            all += scan_s[2][w].x;
         }
-        before += upto - mine;
-        total = all * p.columns;
-        size = max((long long)KVC_MIN_TILES, (total + gridDim.x - 1) / gridDim.x);
-        r0 = min(total, size * blockIdx.x);
-        r1 = min(total, r0 + size);
-        if (r0 >= before * p.columns && r0 < (before + mine) * p.columns) {
+        before *= p.columns; all *= p.columns;
+        r0 = (int)min((unsigned long long)all, (unsigned long long)(even ? 1 : size) * blockIdx.x);
+        r1 = (int)min(all, (unsigned)r0 + (even ? 1 : size));
+        if ((unsigned)r0 >= before && (unsigned)r0 < before + mine * p.columns) {
             Place at;
             int unused = 0;
-            long long rest = r0 - before * p.columns;
+            unsigned rest = r0 - before, units;
             for (at.b = b0; ; at.b++) {
                 at.span = span_of(p, at.b, unused);
                 at.n = tiles_of(at.span);
-                if (rest < (long long)at.n * p.columns) break;
-                rest -= (long long)at.n * p.columns;
+                units = even ? ((unsigned)at.n + even - 1) / (unsigned)even : at.n;
+                if (rest < units * p.columns) break;
+                rest -= units * p.columns;
             }
-            at.c = (int)(rest / at.n);
-            at.i = (int)(rest % at.n);
+            at.c = (int)(rest / units);
+            at.i = (int)(rest - at.c * units);              // the tile, or the part
             start_s = at;
         }
         __syncthreads();
@@ -212,8 +248,19 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
     }
 
     // ---- the copies
-    Place ahead = start_s;
-    int to_copy = (int)(r1 - r0);
+    Place at = start_s;
+    int share = r1 - r0;
+    if (even) {                                             // part `i` of a column: the same number of tiles for each, the first ones have one more
+        const int i = at.i;
+        parts = (int)(((unsigned)at.n + even - 1) / (unsigned)even);
+        share = (int)((unsigned)at.n / (unsigned)parts);
+        const int more = at.n - share * parts;
+        at.i = i * share + min(i, more);
+        share += i < more;
+        r0 = (int)blockIdx.x - i;                           // the column's first CTA
+    }
+    Place ahead = at;
+    int to_copy = share;
     int page = -1;                                          // lanes 0 .. 15: the page of their token of the tile that is copied next
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * STAGES * STAGE;
     auto ask = [&]() {
@@ -262,7 +309,6 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
     };
 
     // ---- the tiles
-    Place at = start_s;
     uint32_t q[KS][NT][2];
     float o[KS][NT][4], m[NT][2], l[NT][2];
     int h0 = 0, heads = 0;
@@ -290,7 +336,6 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
             l[nt][0] = l[nt][1] = 0.0f;
         }
     };
-    const int share = (int)(r1 - r0);
     // where this lane's rows of a matrix load lie, from the stage's start: keys 16 rows by two pieces, values two pieces by 16 rows
     uint32_t key_at[4], value_at[4];
 #pragma unroll
@@ -400,9 +445,9 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
                             }
                         }
                     }
-                const int of_b = at.b, of_h0 = h0, pieces = heads * (D / 4);
+                const int of_b = at.b, of_h0 = h0, of_heads = heads, pieces = heads * (D / 4);
                 const bool whole = first_i == 0 && at.i == at.n - 1;        // the column lies in this share
-                const long long column = (long long)at.b * p.columns + at.c, begin = r0 + n - at.i;          // its first tile in the row
+                const int begin = r0 + n - at.i;            // its first tile in the row of tiles
                 const int tiles = at.n, slot = 2 * blockIdx.x + (n - (at.i - first_i) > 0);
                 if (n < share - 1) {
                     next_tile(p, at);
@@ -442,47 +487,40 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
                 }
                 __syncthreads();
                 if (!whole) {
-                    const int w_first = (int)(begin / size), w_last = (int)((begin + tiles - 1) / size);
-                    if (tid == 0) {
-                        __threadfence();
-                        last_s = atomicAdd(p.counters + column, 1u) == (unsigned)(w_last - w_first);
-                        __threadfence();
-                    }
-                    __syncthreads();
-                    if (last_s) {                           // all parts are there: joined in the order of the shares, by several threads each its own where channels are few
-                        if (tid == 0) p.counters[column] = 0;
-                        const float *const first = p.parts + (2ll * w_first + (begin > size * w_first)) * PART;
+                    const int w_first = even ? r0 : begin / size, count = even ? parts : (begin + tiles - 1) / size - w_first + 1;
+                    const int first_slot = 2 * w_first + (!even && begin > size * w_first);
+                    // the results of every step-th of `many` CTAs from w on become one: the column's, or one in the first of their places
+                    auto join = [&](int w, int step, int many, bool final) {
                         const int per = min(pieces, THREADS), ways = THREADS / per, way = tid / per;
                         for (int i = tid - way * per; i < pieces; i += per) {
                             const int h = i / (D / 4);
                             float top = -CUDART_INF_F, sum = 0.0f;
                             float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                             if (way < ways) {
-                                constexpr int AT_ONCE = 8;
-                                for (int w0 = w_first + way; w0 <= w_last; w0 += AT_ONCE * ways) {
-                                    float2 ml[AT_ONCE];
-                                    float4 x[AT_ONCE];
+                                for (int u0 = way; u0 < many; u0 += JOINED * ways) {
+                                    float2 ml[JOINED];
+                                    float4 x[JOINED];
 #pragma unroll
-                                    for (int u = 0; u < AT_ONCE; u++) {
-                                        const int w = w0 + u * ways;
-                                        const float *from = w == w_first ? first : p.parts + 2ll * w * PART;
-                                        ml[u] = make_float2(-CUDART_INF_F, 0.0f);
-                                        x[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                                        if (w <= w_last) {
-                                            ml[u] = __ldcg(reinterpret_cast<const float2 *>(from) + h);
-                                            x[u] = __ldcg(reinterpret_cast<const float4 *>(from + MAX_GROUP * 2) + i);
+                                    for (int k = 0; k < JOINED; k++) {
+                                        const int u = u0 + k * ways, from_w = w + u * step;
+                                        const float *from = p.parts + (long long)(from_w == w_first ? first_slot : 2 * from_w) * PART;
+                                        ml[k] = make_float2(-CUDART_INF_F, 0.0f);
+                                        x[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                                        if (u < many) {
+                                            ml[k] = __ldcg(reinterpret_cast<const float2 *>(from) + h);
+                                            x[k] = __ldcg(reinterpret_cast<const float4 *>(from + MAX_GROUP * 2) + i);
                                         }
                                     }
                                     float now = top;
 #pragma unroll
-                                    for (int u = 0; u < AT_ONCE; u++) now = fmaxf(now, ml[u].x);
+                                    for (int k = 0; k < JOINED; k++) now = fmaxf(now, ml[k].x);
                                     const float base = now == -CUDART_INF_F ? 0.0f : now, f = exp2_approx(top - base);
                                     sum *= f; v.x *= f; v.y *= f; v.z *= f; v.w *= f;
 #pragma unroll
-                                    for (int u = 0; u < AT_ONCE; u++) {
-                                        const float g = exp2_approx(ml[u].x - base);
-                                        sum += ml[u].y * g;
-                                        v.x += x[u].x * g; v.y += x[u].y * g; v.z += x[u].z * g; v.w += x[u].w * g;
+                                    for (int k = 0; k < JOINED; k++) {
+                                        const float g = exp2_approx(ml[k].x - base);
+                                        sum += ml[k].y * g;
+                                        v.x += x[k].x * g; v.y += x[k].y * g; v.z += x[k].z * g; v.w += x[k].w * g;
                                     }
                                     top = now;
                                 }
@@ -490,25 +528,55 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
                             if (ways > 1) {                 // (the loop is entered once then)
                                 join_v[tid] = v;
                                 join_ml[tid] = make_float2(top, sum);
-                            } else if (way < ways) write(i, top, sum, v);
-                        }
-                        if (ways > 1) {
-                            __syncthreads();
-                            if (tid < pieces) {
-                                float top = -CUDART_INF_F, sum = 0.0f;
-                                float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                                for (int w = 0; w < ways; w++) top = fmaxf(top, join_ml[w * per + tid].x);
+                                __syncthreads();
+                                if (tid >= pieces) continue;
+                                top = -CUDART_INF_F; sum = 0.0f;
+                                v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                                for (int k = 0; k < ways; k++) top = fmaxf(top, join_ml[k * per + tid].x);
                                 const float base = top == -CUDART_INF_F ? 0.0f : top;
-                                for (int w = 0; w < ways; w++) {
-                                    const float2 ml = join_ml[w * per + tid];
-                                    const float4 x = join_v[w * per + tid];
+                                for (int k = 0; k < ways; k++) {
+                                    const float2 ml = join_ml[k * per + tid];
+                                    const float4 x = join_v[k * per + tid];
                                     const float g = exp2_approx(ml.x - base);
                                     sum += ml.y * g;
                                     v.x += x.x * g; v.y += x.y * g; v.z += x.z * g; v.w += x.w * g;
                                 }
-                                write(tid, top, sum, v);
+                            } else if (way >= ways) continue;
+                            if (final) write(i, top, sum, v);
+                            else {                          // (others may still read the maxima and sums there)
+                                __stcg(reinterpret_cast<float4 *>(p.parts + (long long)(w == w_first ? first_slot : 2 * w) * PART + MAX_GROUP * 2) + i, v);
+                                if (i % (D / 4) == 0) new_ml[h] = make_float2(top, sum);
                             }
+                        }
+                        __syncthreads();
+                        if (!final) {
+                            if (tid < of_heads) __stcg(reinterpret_cast<float2 *>(p.parts + (long long)(w == w_first ? first_slot : 2 * w) * PART) + tid, new_ml[tid]);
                             __syncthreads();
+                        }
+                    };
+                    // whether this CTA is the last of `many` at a counter, which is zero again then; what they wrote before is seen behind it
+                    auto is_last = [&](unsigned *counter, int many) {
+                        if (tid == 0) {
+                            __threadfence();
+                            const bool last = atomicAdd(counter, 1u) == (unsigned)(many - 1);
+                            if (last) *counter = 0;
+                            last_s = last;
+                            __threadfence();
+                        }
+                        __syncthreads();
+                        const bool last = last_s;
+                        __syncthreads();
+                        return last;
+                    };
+                    // Few parts are joined at once; many by eights first, each eight by the last of them: one trip to memory for eight results
+                    // at a time.
+                    if (count <= 2 * JOINED) {
+                        if (is_last(p.counters + first_slot, count)) join(w_first, 1, count, true);
+                    } else {
+                        const int g = ((int)blockIdx.x - w_first) / JOINED, leader = w_first + g * JOINED, groups = (count + JOINED - 1) / JOINED, many = min(JOINED, count - g * JOINED);
+                        if (is_last(p.group_counters + (leader == w_first ? first_slot : 2 * leader), many)) {
+                            join(leader, 1, many, false);
+                            if (is_last(p.counters + first_slot, groups)) join(w_first, JOINED, groups, true);
                         }
                     }
                 }
@@ -525,21 +593,22 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
 }
 
 template <typename T, int D, int NT, bool SAME, int STAGES, int CTAS>
-int launch(const Params &p, long long most_tiles, cudaStream_t stream) {
+int launch(Params &p, long long most_tiles, cudaStream_t stream) {
     static kvc_launch_slot slot;
     constexpr size_t shared = (size_t)WARPS * STAGES * 64 * D;
     auto *kernel = paged_attn_kernel<T, D, NT, SAME, STAGES, CTAS>;
     int occ = 0;
     if (int rc = kvc_prepare(slot, reinterpret_cast<const void *>(kernel), THREADS, shared, &occ)) return rc;
     KVC_REQUIRE(occ > 0, "kvc_paged_attn: the kernel does not fit this device");
-    const long long grid = std::min<long long>(most_tiles, (long long)std::min(occ, MAX_CTAS_PER_SM) * kvc_sm_count());
-    kernel<<<(unsigned)std::max<long long>(grid, 1), THREADS, shared, stream>>>(p);
+    const long long grid = std::max<long long>(std::min<long long>(most_tiles, (long long)std::min(occ, MAX_CTAS_PER_SM) * kvc_sm_count()), 1);
+    p.per_cta = (float)(0.9999997 / grid);
+    kernel<<<(unsigned)grid, THREADS, shared, stream>>>(p);
     KVC_LAUNCH_OK();
     return KVC_OK;
 }
 
 template <typename T, int D, int STAGES, int CTAS, int WIDE_STAGES, int WIDE_CTAS>
-int choose_heads(const Params &p, bool same, long long most, cudaStream_t s) {
+int choose_heads(Params &p, bool same, long long most, cudaStream_t s) {
     if constexpr (WIDE_STAGES > 0) {
         if (p.group > 8) return same ? launch<T, D, 2, true, WIDE_STAGES, WIDE_CTAS>(p, most, s) : launch<T, D, 2, false, WIDE_STAGES, WIDE_CTAS>(p, most, s);
     }
@@ -547,7 +616,7 @@ int choose_heads(const Params &p, bool same, long long most, cudaStream_t s) {
 }
 
 template <typename T>
-int choose(const Params &p, bool same, long long most, cudaStream_t s) {
+int choose(Params &p, bool same, long long most, cudaStream_t s) {
     switch (p.a.D) {
         case 64: return choose_heads<T, 64, KVC_SC>(p, same, most, s);
         case 96: return choose_heads<T, 96, KVC_SC96>(p, same, most, s);
@@ -559,14 +628,16 @@ int choose(const Params &p, bool same, long long most, cudaStream_t s) {
 // query heads that a column takes at most: 16 where they fit the registers beside the accumulators
 int group_of(int64_t Hq, int64_t Hkv, int64_t D) { return (int)std::min<int64_t>(Hq / Hkv, D > 128 ? 8 : MAX_GROUP); }
 int64_t columns_of(int64_t Hq, int64_t Hkv, int64_t D) { return Hkv * ((Hq / Hkv + group_of(Hq, Hkv, D) - 1) / group_of(Hq, Hkv, D)); }
-int64_t counter_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t D) { return (B * columns_of(Hq, Hkv, D) * 4 + 255) / 256 * 256; }
+int64_t places() { return 2ll * MAX_CTAS_PER_SM * kvc_sm_count(); }             // of partial results: two for every CTA that the device holds
+// Two counters for a place: of the column whose first result lies there, of the eight results that begin there.  They lie in front, the same for
+// calls of all shapes: a workspace may serve one after the other.
+int64_t counter_bytes() { return (2 * places() * 4 + 255) / 256 * 256; }
 
 }  // namespace
 
-// a counter per column; two partial results for every CTA that the device holds
 extern "C" int64_t kvc_paged_attn_workspace(int64_t B, int64_t Hq, int64_t Hkv, int64_t D) {
     if (B < 0 || Hkv <= 0 || Hq < Hkv || D <= 0) return 0;
-    return counter_bytes(B, Hq, Hkv, D) + 2ll * MAX_CTAS_PER_SM * kvc_sm_count() * MAX_GROUP * (D + 2) * 4;
+    return counter_bytes() + places() * MAX_GROUP * (D + 2) * 4;
 }
 
 extern "C" int kvc_paged_attn(const kvc_paged_attn_args *args, kvc_stream_t stream) {
@@ -607,10 +678,11 @@ extern "C" int kvc_paged_attn(const kvc_paged_attn_args *args, kvc_stream_t stre
     p.sign = a.scaling < 0.0f ? 0x80008000u : 0;
     p.log2_scaling = std::max(fabsf(a.scaling) * 1.4426950408889634f, 1e-37f);      // (0 times the -inf of a token that is left out is none)
     p.counters = reinterpret_cast<unsigned *>(a.workspace);
-    p.parts = reinterpret_cast<float *>(reinterpret_cast<uint8_t *>(a.workspace) + counter_bytes(a.B, a.Hq, a.Hkv, a.D));
+    p.group_counters = p.counters + places();
+    p.parts = reinterpret_cast<float *>(reinterpret_cast<uint8_t *>(a.workspace) + counter_bytes());
     const long long most = a.B * p.columns * ((a.table_width * a.page_size + TILE - 1) / TILE);
     cudaStream_t s = kvc_cu(stream);
-    KVC_REQUIRE(most / kvc_sm_count() < (1ll << 31), "kvc_paged_attn: too many tokens");
+    KVC_REQUIRE(a.B * p.columns < (1ll << 31) && most < (1ll << 31) - (1 << 20), "kvc_paged_attn: requests, KV heads and table rows of more than 2^31 tiles of %d tokens", TILE);
     p.v_less_k = reinterpret_cast<const uint8_t *>(a.vpages) - reinterpret_cast<const uint8_t *>(a.kpages);
     const bool same = a.kp_page == a.vp_page && a.kp_row == a.vp_row && a.kp_head == a.vp_head;
     return a.type == KVC_TYPE_FP16 ? choose<__half>(p, same, most, s) : choose<__nv_bfloat16>(p, same, most, s);
