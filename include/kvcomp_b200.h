@@ -448,8 +448,8 @@ int kvc_rotary_store(const kvc_rotary_args *args, kvc_stream_t stream);
  * `window` of them), out = sum exp(s_t) v_t / sum exp(s_t) and lse = log sum exp(s_t) (fp32 [B, Hq], may be null).  No
  * tokens: out = 0, lse = -inf.  q, out: [B, Hq, D], D 64, 96, 128 or 256, query head h reads KV head h / (Hq / Hkv).  Rows of q and of the
  * pools start on 16 bytes (pointers and strides).  Tokens behind a length are never read.
- * workspace: kvc_paged_attn_workspace() bytes, 16-byte aligned, zeroed once before its first use; every call leaves what has to be zero at zero.  A workspace
- * serves one launch at a time: concurrent streams need their own. */
+ * workspace: kvc_paged_attn_workspace() bytes, 16-byte aligned, the first kvc_paged_attn_cleared() of them zeroed once before the first use; every call
+ * leaves these at zero, for calls of any shape.  A workspace serves one launch at a time: concurrent streams need their own. */
 typedef struct {
     const void *q, *kpages, *vpages;
     const int32_t *table, *lengths;
@@ -463,6 +463,7 @@ typedef struct {
     float scaling;
     int32_t type;
 } kvc_paged_attn_args;
+int64_t kvc_paged_attn_cleared(void);
 int64_t kvc_paged_attn_workspace(int64_t B, int64_t Hq, int64_t Hkv, int64_t D);
 int kvc_paged_attn(const kvc_paged_attn_args *args, kvc_stream_t stream);
 

@@ -114,6 +114,7 @@ _SIGNATURES = {
     "kvc_page_plan": (_i32, [C.c_char_p, _vp]),
     "kvc_page_release": (_i32, [C.c_char_p, _vp]),
     "kvc_rotary_store": (_i32, [C.c_char_p, _vp]),
+    "kvc_paged_attn_cleared": (_i64, []),
     "kvc_paged_attn_workspace": (_i64, [_i64, _i64, _i64, _i64]),
     "kvc_paged_attn": (_i32, [C.c_char_p, _vp]),
     "kvc_k_matvec": (_i32, [_vp, _vp, _vp, _i64, _i64, _vp]),

@@ -33,6 +33,10 @@ namespace {
 constexpr int WARPS = 4, THREADS = WARPS * 32;
 constexpr int TILE = 16 * WARPS;                // tokens of a tile
 constexpr int MAX_CTAS_PER_SM = 4;
+constexpr int DRAWN_REQUESTS = 1024;            // of more requests nothing is drawn: where a tile belongs is looked up in shared memory
+#ifndef DRAWN_SHARE
+#define DRAWN_SHARE 96
+#endif
 constexpr int JOINED = 8;                       // partial results that are asked for at once
 constexpr int MIN_TILES = 2;                    // of a share
 #ifndef KVC_SC
@@ -52,13 +56,16 @@ constexpr int MAX_GROUP = 16;                   // query heads that a column ser
 struct Params {
     kvc_paged_attn_args a;
     kvc_div page;
+    int chunk;                                  // requests of a lane
     int group, columns, per_head;               // query heads of a column at most, columns of a request, columns of a KV head
     int most_tokens;                            // of a table row
     unsigned n_pages;
     uint32_t sign;                              // of the scaling, for two values: the scores' maximum is taken before they are scaled
     float log2_scaling, per_cta;                // per_cta: a little less than one over the number of CTAs
     long long v_less_k;                         // bytes from the keys' pool to the values'
+    int *drawn;                                 // how many pieces have been drawn
     unsigned *counters, *group_counters;        // of the places of partial results
+    int part;                                   // floats of a place: sums of values, maxima and sums of weights
     float *parts;
 };
 
@@ -125,6 +132,14 @@ __device__ __forceinline__ Span span_of(const Params &p, int b, int &flags) {
 }
 __device__ __forceinline__ int tiles_of(const Span &s) { return (s.len - s.first + TILE - 1) / TILE; }
 
+// n / d of numbers that are not negative, through a float that a step or two put right
+__device__ __forceinline__ int quotient(int n, int d) {
+    int q = (int)((float)n * __frcp_rn((float)d));
+    while ((unsigned)q * (unsigned)d > (unsigned)n) q--;
+    while ((unsigned)n - (unsigned)q * (unsigned)d >= (unsigned)d) q++;
+    return q;
+}
+
 // A place in the row of tiles: tile `i` of column `c` of request `b`
 struct Place { int b, c, i, n; Span span; };
 __device__ __forceinline__ void next_tile(const Params &p, Place &at) {
@@ -144,16 +159,16 @@ template <typename T, int D, int NT, bool SAME, int STAGES, int CTAS>
 __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_constant__ Params p) {
     constexpr int KS = D / 16;                              // steps of 16 channels
     constexpr uint32_t HALF_STAGE = 16 * D * 2, STAGE = 2 * HALF_STAGE;
-    constexpr int PART = MAX_GROUP * (D + 2);               // floats of a partial result: maxima and sums, sums of values
     constexpr float LIFT = Pair<T>::LIFT;
+    static_assert(STAGES + 2 <= DRAWN_SHARE - DRAWN_SHARE / 8, "a share is long enough for the first draw");
     extern __shared__ __align__(128) uint8_t smem[];        // [warp][stage]: 16 rows of keys, 16 of values
     __shared__ uint32_t masks[WARPS][STAGES];
     __shared__ float2 ml_s[WARPS][8 * NT];                  // maximum and sum
     __shared__ float4 join_v[THREADS];
     __shared__ float2 join_ml[THREADS], new_ml[MAX_GROUP];
-    __shared__ int4 scan_s[3][WARPS];
-    __shared__ Place start_s;
-    __shared__ int last_s;
+    __shared__ Place next_start_s[WARPS];
+    __shared__ unsigned before_s[CTAS >= 3 ? DRAWN_REQUESTS : 1];           // tiles of a column in front of a request
+    __shared__ int last_s, next_s;
     const kvc_paged_attn_args &a = p.a;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, B = (int)a.B;
     int flags = 0;
@@ -161,10 +176,18 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
     // ---- this CTA's share
     // Whole parts of columns, one for each CTA, where all columns together have no more of them than there are CTAs (few columns): no CTA has two to finish then.  Else
     // equal shares of the row of all columns' tiles.  (All of it is on the way of the first byte: 32 bits, no division by what is known before.)
+    // Of long shares an eighth is drawn from a counter instead, in pieces of a sixteenth of a share, then halves of it: the SMs do not get the same out of the
+    // memory (of 444 CTAs with 295 tiles each the first was done at 235 us, half at 285, the last at 319).  Where columns are few all of these pieces would be
+    // joined by few CTAs, and a CTA alone on its SM pauses at the end of every piece: equal shares there.
+    constexpr bool DRAWS = CTAS >= 3;
+    // (All of this is on the way of the first byte.  Every warp does it by itself, for its lanes' requests: no barrier, no division but by a reciprocal.)
     int r0, r1, size;                                       // tiles [r0, r1) of the row, shares of `size`; or with even != 0: CTA r0, r1 = r0 + 1
-    int even = 0, parts = 1;                                // tiles of a part at most; this column's parts
+    float even = 0.0f;                                      // one over the tiles of a part at most
+    int unit = 0, least = 0, drawn_from = 0x7fffffff, all_tiles;       // tiles of the first and the last pieces that are drawn, the first tile that is not in a share
+    Place at;
+    auto parts_of = [&](int tiles) { return __float2int_ru((float)tiles * even); };
     {
-        const int chunk = B <= THREADS ? 1 : (B + THREADS - 1) / THREADS, b0 = min(B, tid * chunk), b1 = min(B, b0 + chunk);
+        const int b0 = min(B, lane * p.chunk), b1 = min(B, b0 + p.chunk);
         const int n0 = b0 < b1 ? tiles_of(span_of(p, b0, flags)) : 0;
         unsigned mine = n0, some = n0 > 0;
         for (int b = b0 + 1; b < b1; b++) {
@@ -172,68 +195,63 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
             mine += n;
             some += n > 0;
         }
-        const unsigned sum = __reduce_add_sync(0xffffffffu, mine), columns = __reduce_add_sync(0xffffffffu, some);
-        if (lane == 0) scan_s[0][warp] = make_int4((int)sum, (int)columns, 0, 0);
-        __syncthreads();
-        unsigned total = 0, there = 0;
-#pragma unroll
-        for (int w = 0; w < WARPS; w++) { total += scan_s[0][w].x; there += scan_s[0][w].y; }
-        total *= p.columns;
+        const unsigned total = __reduce_add_sync(0xffffffffu, mine) * p.columns, there = __reduce_add_sync(0xffffffffu, some) * p.columns;
         size = max(MIN_TILES, (int)((float)total * p.per_cta));
         while ((unsigned)size * gridDim.x < total) size += 1 + (size >> 20);       // (the float is a little below the quotient)
-        // the tiles that a part of `tiles` tiles at most needs, for this thread's requests
-        auto count = [&](int tiles) {
-            unsigned k = ((unsigned)n0 + tiles - 1) / (unsigned)tiles;
-            int unused = 0;
-            for (int b = b0 + 1; b < b1; b++) k += ((unsigned)tiles_of(span_of(p, b, unused)) + tiles - 1) / (unsigned)tiles;
-            return k;
-        };
-        if (there * p.columns <= gridDim.x) {
+        int unused = 0;
+        if (DRAWS && B <= DRAWN_REQUESTS && size >= DRAWN_SHARE && there * 8 >= gridDim.x) {
+            least = max(STAGES + 2, size / 64);
+            unit = max(least, size / 16);
+            size -= size / 8;
+            drawn_from = size * (int)gridDim.x;
+        } else if (there <= gridDim.x) {
             const int step = max(1, size / 16);
-            const unsigned k0 = __reduce_add_sync(0xffffffffu, count(size)), k1 = __reduce_add_sync(0xffffffffu, count(size + step)), k2 = __reduce_add_sync(0xffffffffu, count(size + 2 * step));
-            if (lane == 0) scan_s[1][warp] = make_int4((int)k0, (int)k1, (int)k2, 0);
-            __syncthreads();
-            unsigned all0 = 0, all1 = 0, all2 = 0;
-#pragma unroll
-            for (int w = 0; w < WARPS; w++) { all0 += scan_s[1][w].x; all1 += scan_s[1][w].y; all2 += scan_s[1][w].z; }
-            if (all0 * p.columns <= gridDim.x) even = size;
-            else if (all1 * p.columns <= gridDim.x) even = size + step;
-            else if (all2 * p.columns <= gridDim.x) even = size + 2 * step;
-            if (even) mine = count(even);
+#pragma unroll 1
+            for (int tiles = size; tiles <= size + 2 * step; tiles += step) {
+                even = __frcp_rn((float)tiles);
+                unsigned k = parts_of(n0);
+                for (int b = b0 + 1; b < b1; b++) k += parts_of(tiles_of(span_of(p, b, unused)));
+                if (__reduce_add_sync(0xffffffffu, k) * p.columns <= gridDim.x) {
+                    mine = k;
+                    break;
+                }
+                even = 0.0f;
+            }
         }
-        unsigned upto = mine;
+        unsigned before = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const unsigned u = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += u;
+            const unsigned u = __shfl_up_sync(0xffffffffu, before, o);
+            if (lane >= o) before += u;
         }
-        if (lane == 31) scan_s[2][warp] = make_int4((int)upto, 0, 0, 0);
-        __syncthreads();
-        unsigned before = upto - mine, all = 0;
-#pragma unroll
-        for (int w = 0; w < WARPS; w++) {
-            if (w < warp) before += scan_s[2][w].x;
-            all += scan_s[2][w].x;
+        const unsigned all = __shfl_sync(0xffffffffu, before, 31) * p.columns;
+        before -= mine;
+        if (DRAWS && unit && warp == 0) {                   // (it is read behind the barriers at which pieces become known)
+            unsigned tiles = before;
+            for (int b = b0; b < b1; b++) { before_s[b] = tiles; tiles += tiles_of(span_of(p, b, unused)); }
         }
-        before *= p.columns; all *= p.columns;
-        r0 = (int)min((unsigned long long)all, (unsigned long long)(even ? 1 : size) * blockIdx.x);
-        r1 = (int)min(all, (unsigned)r0 + (even ? 1 : size));
-        if ((unsigned)r0 >= before && (unsigned)r0 < before + mine * p.columns) {
-            Place at;
-            int unused = 0;
-            unsigned rest = r0 - before, units;
-            for (at.b = b0; ; at.b++) {
-                at.span = span_of(p, at.b, unused);
-                at.n = tiles_of(at.span);
-                units = even ? ((unsigned)at.n + even - 1) / (unsigned)even : at.n;
-                if (rest < units * p.columns) break;
-                rest -= units * p.columns;
+        all_tiles = (int)all;
+        r0 = (int)min((unsigned long long)all, (unsigned long long)(even != 0.0f ? 1 : size) * blockIdx.x);
+        r1 = (int)min(all, (unsigned)r0 + (even != 0.0f ? 1 : size));
+        // the lane that has the request of r0, and the request
+        unsigned rest = (unsigned)r0 - before * p.columns;
+        const bool here = (unsigned)r0 >= before * p.columns && rest < mine * p.columns;
+        at.b = b0;
+        if (here)
+            for (;; at.b++) {
+                const int n = tiles_of(span_of(p, at.b, unused));
+                const unsigned units = (unsigned)(even != 0.0f ? parts_of(n) : n) * p.columns;
+                if (rest < units) break;
+                rest -= units;
             }
-            at.c = (int)(rest / units);
-            at.i = (int)(rest - at.c * units);              // the tile, or the part
-            start_s = at;
-        }
-        __syncthreads();
+        const int from = max(__ffs(__ballot_sync(0xffffffffu, here)) - 1, 0);
+        at.b = min(__shfl_sync(0xffffffffu, at.b, from), B - 1);
+        rest = __shfl_sync(0xffffffffu, rest, from);
+        at.span = span_of(p, at.b, unused);
+        at.n = tiles_of(at.span);
+        const int units = max(even != 0.0f ? parts_of(at.n) : at.n, 1);
+        at.c = quotient((int)rest, units);
+        at.i = (int)rest - at.c * units;                    // the tile, or the part
     }
     // requests without tokens
     for (int b = blockIdx.x; b < B; b += gridDim.x) {
@@ -248,19 +266,38 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
     }
 
     // ---- the copies
-    Place at = start_s;
-    int share = r1 - r0;
-    if (even) {                                             // part `i` of a column: the same number of tiles for each, the first ones have one more
+    int share = r1 - r0, column_first = 0, parts = 1;       // column_first: the first CTA of this column's parts
+    if (even != 0.0f) {                                     // part `i` of a column: the same number of tiles for each, the first ones have one more
         const int i = at.i;
-        parts = (int)(((unsigned)at.n + even - 1) / (unsigned)even);
-        share = (int)((unsigned)at.n / (unsigned)parts);
+        parts = parts_of(at.n);
+        share = quotient(at.n, parts);
         const int more = at.n - share * parts;
         at.i = i * share + min(i, more);
         share += i < more;
-        r0 = (int)blockIdx.x - i;                           // the column's first CTA
+        column_first = (int)blockIdx.x - i;
     }
+    // pieces: the shares, then rounds of as many that are drawn, of half the size each time
+    auto piece_of = [&](int tile) {
+        if (!DRAWS || tile < drawn_from) return quotient(tile, size);
+        int first = gridDim.x, tiles = unit;
+        for (tile -= drawn_from; tiles > least && tile >= tiles * (int)gridDim.x; tiles = max(tiles / 2, least)) { tile -= tiles * (int)gridDim.x; first += gridDim.x; }
+        return first + quotient(tile, tiles);
+    };
+    auto start_of = [&](int g, int &tiles) {
+        tiles = size;
+        if (!DRAWS || g < (int)gridDim.x) return g * size;
+        int from = drawn_from;
+        tiles = unit;
+        for (g -= gridDim.x; tiles > least && g >= (int)gridDim.x; tiles = max(tiles / 2, least)) { from += tiles * (int)gridDim.x; g -= gridDim.x; }
+        from += g * tiles;
+        tiles = min(tiles, all_tiles - from);
+        return from;
+    };
+    int piece = blockIdx.x, next = -1;                      // next: the piece behind this one, once it is known
+    const int pieces_end = DRAWS && unit ? piece_of(all_tiles - 1) + 1 : 0;
     Place ahead = at;
     int to_copy = share;
+    bool taken = false;                                     // `next` is being copied
     int page = -1;                                          // lanes 0 .. 15: the page of their token of the tile that is copied next
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * STAGES * STAGE;
     auto ask = [&]() {
@@ -302,7 +339,23 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
                 }
             }
             next_tile(p, ahead);
-            to_copy--;
+            if (--to_copy == 0 && DRAWS && next >= 0 && !taken) {
+                const int tile = start_of(next, to_copy);
+                int lo = 0, hi = B;
+                while (hi - lo > 1) {                       // the last request with before_s * columns <= tile
+                    const int mid = (lo + hi) >> 1;
+                    if (before_s[mid] * p.columns <= (unsigned)tile) lo = mid; else hi = mid;
+                }
+                int unused = 0;
+                const unsigned rest = (unsigned)tile - before_s[lo] * p.columns;
+                ahead.b = lo;
+                ahead.span = span_of(p, lo, unused);
+                ahead.n = tiles_of(ahead.span);
+                ahead.c = quotient((int)rest, ahead.n);
+                ahead.i = (int)rest - ahead.c * ahead.n;
+                if (lane == 0) next_start_s[warp] = ahead;
+                taken = true;
+            }
         }
         copies_commit();
         ask();
@@ -347,9 +400,23 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
     ask();
     begin_column();
     clear();
+    int drawn = 0;
 #pragma unroll 1
-    for (int n = -STAGES; n < share; n++) {
+    for (int n = -STAGES;; n++) {                           // tile n of the piece
         if (n >= 0) {
+            if (DRAWS && unit) {
+                // The next piece is drawn as late as the copies allow: they are STAGES tiles ahead, and it takes a tile's time to know it.
+                if (n == max(0, share - STAGES - 2) && tid == 0) drawn = atomicAdd(p.drawn, 1);
+                if (n == max(min(1, share - 1), share - STAGES - 1)) {
+                    if (tid == 0) {
+                        next_s = (int)gridDim.x + drawn < pieces_end ? (int)gridDim.x + drawn : -1;
+                        if (drawn == pieces_end - 1) *p.drawn = 0;                   // every CTA draws once in vain: this was the last of all
+                    }
+                    __syncthreads();
+                    next = next_s;
+                    taken = false;
+                }
+            }
             copies_wait<STAGES - 1>();
             __syncwarp();
             const uint32_t mask = masks[warp][stage], from = ring + stage * STAGE;
@@ -448,12 +515,20 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
                 const int of_b = at.b, of_h0 = h0, of_heads = heads, pieces = heads * (D / 4);
                 const bool whole = first_i == 0 && at.i == at.n - 1;        // the column lies in this share
                 const int begin = r0 + n - at.i;            // its first tile in the row of tiles
-                const int tiles = at.n, slot = 2 * blockIdx.x + (n - (at.i - first_i) > 0);
+                const int tiles = at.n, of_piece = piece, place = 2 * piece + (n - (at.i - first_i) > 0);
+                first_i = 0;
                 if (n < share - 1) {
                     next_tile(p, at);
                     begin_column();                         // on their way while the sums are joined
-                }
-                first_i = 0;
+                } else if (DRAWS && next >= 0) {
+                    piece = next;
+                    next = -1;
+                    r0 = start_of(piece, share);
+                    at = next_start_s[warp];
+                    first_i = at.i;
+                    begin_column();
+                    n = -1;                                 // (the loop goes on with 0)
+                } else n = share;                           // (it ends)
                 clear();
                 __syncthreads();
                 auto write = [&](int i, float top, float sum, const float4 &v) {       // four channels of a result
@@ -463,7 +538,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
                         make_uint2(Pair<T>::pack(v.x * f, v.y * f), Pair<T>::pack(v.z * f, v.w * f));
                     if (d == 0 && a.lse) a.lse[of_b * a.Hq + h] = sum == 0.0f ? -CUDART_INF_F : (top + log2f(sum) - LIFT) * 0.69314718055994531f;
                 };
-                float *part = p.parts + (long long)slot * PART;
+                float *part = p.parts + (long long)place * p.part;
                 for (int i = tid; i < pieces; i += THREADS) {
                     const int h = i / (D / 4), d = i % (D / 4) * 4;
                     float2 ml[WARPS];
@@ -481,15 +556,16 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
                     }
                     if (whole) write(i, top, sum, v);
                     else {
-                        __stcg(reinterpret_cast<float4 *>(part + MAX_GROUP * 2) + i, v);
-                        if (d == 0) __stcg(reinterpret_cast<float2 *>(part) + h, make_float2(top, sum));
+                        __stcg(reinterpret_cast<float4 *>(part) + i, v);
+                        if (d == 0) __stcg(reinterpret_cast<float2 *>(part + p.group * D) + h, make_float2(top, sum));
                     }
                 }
                 __syncthreads();
                 if (!whole) {
-                    const int w_first = even ? r0 : begin / size, count = even ? parts : (begin + tiles - 1) / size - w_first + 1;
-                    const int first_slot = 2 * w_first + (!even && begin > size * w_first);
-                    // the results of every step-th of `many` CTAs from w on become one: the column's, or one in the first of their places
+                    const int w_first = even != 0.0f ? column_first : piece_of(begin), count = even != 0.0f ? parts : piece_of(begin + tiles - 1) - w_first + 1;
+                    int unused;
+                    const int first_place = 2 * w_first + (even == 0.0f && begin > start_of(w_first, unused));
+                    // the results of every step-th of `many` pieces from w on become one: the column's, or one in the first of their places
                     auto join = [&](int w, int step, int many, bool final) {
                         const int per = min(pieces, THREADS), ways = THREADS / per, way = tid / per;
                         for (int i = tid - way * per; i < pieces; i += per) {
@@ -503,12 +579,12 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
 #pragma unroll
                                     for (int k = 0; k < JOINED; k++) {
                                         const int u = u0 + k * ways, from_w = w + u * step;
-                                        const float *from = p.parts + (long long)(from_w == w_first ? first_slot : 2 * from_w) * PART;
+                                        const float *from = p.parts + (long long)(from_w == w_first ? first_place : 2 * from_w) * p.part;
                                         ml[k] = make_float2(-CUDART_INF_F, 0.0f);
                                         x[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                                         if (u < many) {
-                                            ml[k] = __ldcg(reinterpret_cast<const float2 *>(from) + h);
-                                            x[k] = __ldcg(reinterpret_cast<const float4 *>(from + MAX_GROUP * 2) + i);
+                                            ml[k] = __ldcg(reinterpret_cast<const float2 *>(from + p.group * D) + h);
+                                            x[k] = __ldcg(reinterpret_cast<const float4 *>(from) + i);
                                         }
                                     }
                                     float now = top;
@@ -544,13 +620,13 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
                             } else if (way >= ways) continue;
                             if (final) write(i, top, sum, v);
                             else {                          // (others may still read the maxima and sums there)
-                                __stcg(reinterpret_cast<float4 *>(p.parts + (long long)(w == w_first ? first_slot : 2 * w) * PART + MAX_GROUP * 2) + i, v);
+                                __stcg(reinterpret_cast<float4 *>(p.parts + (long long)(w == w_first ? first_place : 2 * w) * p.part) + i, v);
                                 if (i % (D / 4) == 0) new_ml[h] = make_float2(top, sum);
                             }
                         }
                         __syncthreads();
                         if (!final) {
-                            if (tid < of_heads) __stcg(reinterpret_cast<float2 *>(p.parts + (long long)(w == w_first ? first_slot : 2 * w) * PART) + tid, new_ml[tid]);
+                            if (tid < of_heads) __stcg(reinterpret_cast<float2 *>(p.parts + (long long)(w == w_first ? first_place : 2 * w) * p.part + p.group * D) + tid, new_ml[tid]);
                             __syncthreads();
                         }
                     };
@@ -571,12 +647,12 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
                     // Few parts are joined at once; many by eights first, each eight by the last of them: one trip to memory for eight results
                     // at a time.
                     if (count <= 2 * JOINED) {
-                        if (is_last(p.counters + first_slot, count)) join(w_first, 1, count, true);
+                        if (is_last(p.counters + first_place, count)) join(w_first, 1, count, true);
                     } else {
-                        const int g = ((int)blockIdx.x - w_first) / JOINED, leader = w_first + g * JOINED, groups = (count + JOINED - 1) / JOINED, many = min(JOINED, count - g * JOINED);
-                        if (is_last(p.group_counters + (leader == w_first ? first_slot : 2 * leader), many)) {
+                        const int g = (of_piece - w_first) / JOINED, leader = w_first + g * JOINED, groups = (count + JOINED - 1) / JOINED, many = min(JOINED, count - g * JOINED);
+                        if (is_last(p.group_counters + (leader == w_first ? first_place : 2 * leader), many)) {
                             join(leader, 1, many, false);
-                            if (is_last(p.counters + first_slot, groups)) join(w_first, JOINED, groups, true);
+                            if (is_last(p.counters + first_place, groups)) join(w_first, JOINED, groups, true);
                         }
                     }
                 }
@@ -584,6 +660,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
                 at.i++;
             }
         }
+        if (n == share) break;
         // the stage that was read is filled again; nothing is read in the first rounds
         copy_tile(stage);
         stage = stage + 1 == STAGES ? 0 : stage + 1;
@@ -628,16 +705,20 @@ int choose(Params &p, bool same, long long most, cudaStream_t s) {
 // query heads that a column takes at most: 16 where they fit the registers beside the accumulators
 int group_of(int64_t Hq, int64_t Hkv, int64_t D) { return (int)std::min<int64_t>(Hq / Hkv, D > 128 ? 8 : MAX_GROUP); }
 int64_t columns_of(int64_t Hq, int64_t Hkv, int64_t D) { return Hkv * ((Hq / Hkv + group_of(Hq, Hkv, D) - 1) / group_of(Hq, Hkv, D)); }
-int64_t places() { return 2ll * MAX_CTAS_PER_SM * kvc_sm_count(); }             // of partial results: two for every CTA that the device holds
-// Two counters for a place: of the column whose first result lies there, of the eight results that begin there.  They lie in front, the same for
-// calls of all shapes: a workspace may serve one after the other.
-int64_t counter_bytes() { return (2 * places() * 4 + 255) / 256 * 256; }
+// Of partial results: two for every piece.  Of s tiles for a CTA s / 8 and those left by rounding down are drawn, in rounds of s / 16, s / 32, s / 64 (at least) and what these leave:
+// a CTA's share and five pieces more.
+int64_t places(int64_t D) { return 2ll * 6 * (D == 64 ? 4 : 3) * kvc_sm_count(); }
+int64_t part_floats(int64_t group, int64_t D) { return std::max<int64_t>(group, 8) * (D + 2); }       // (room for eight heads at least: one workspace for more shapes)
+// The counter of what is drawn, and two counters for a place: of the column whose first result lies there, of the eight results that begin there.  They lie in
+// front, the same for calls of all shapes: a workspace may serve one after the other.
+int64_t counter_bytes() { return 256 + (2 * places(64) * 4 + 255) / 256 * 256; }
 
 }  // namespace
 
+extern "C" int64_t kvc_paged_attn_cleared(void) { return counter_bytes(); }
 extern "C" int64_t kvc_paged_attn_workspace(int64_t B, int64_t Hq, int64_t Hkv, int64_t D) {
     if (B < 0 || Hkv <= 0 || Hq < Hkv || D <= 0) return 0;
-    return counter_bytes() + places() * MAX_GROUP * (D + 2) * 4;
+    return counter_bytes() + places(D) * part_floats(group_of(Hq, Hkv, D), D) * 4;
 }
 
 extern "C" int kvc_paged_attn(const kvc_paged_attn_args *args, kvc_stream_t stream) {
@@ -673,12 +754,15 @@ extern "C" int kvc_paged_attn(const kvc_paged_attn_args *args, kvc_stream_t stre
     p.group = group_of(a.Hq, a.Hkv, a.D);
     p.columns = (int)columns_of(a.Hq, a.Hkv, a.D);
     p.per_head = p.columns / (int)a.Hkv;
+    p.chunk = (int)((a.B + 31) / 32);
     p.most_tokens = (int)(a.table_width * a.page_size);
     p.n_pages = (unsigned)a.n_pages;
     p.sign = a.scaling < 0.0f ? 0x80008000u : 0;
     p.log2_scaling = std::max(fabsf(a.scaling) * 1.4426950408889634f, 1e-37f);      // (0 times the -inf of a token that is left out is none)
-    p.counters = reinterpret_cast<unsigned *>(a.workspace);
-    p.group_counters = p.counters + places();
+    p.part = (int)part_floats(p.group, a.D);
+    p.drawn = reinterpret_cast<int *>(a.workspace);
+    p.counters = reinterpret_cast<unsigned *>(a.workspace) + 64;
+    p.group_counters = p.counters + places(64);
     p.parts = reinterpret_cast<float *>(reinterpret_cast<uint8_t *>(a.workspace) + counter_bytes());
     const long long most = a.B * p.columns * ((a.table_width * a.page_size + TILE - 1) / TILE);
     cudaStream_t s = kvc_cu(stream);

@@ -893,13 +893,15 @@ def rotary_paged_store(q, k, v, positions, slots, frequencies, kpages, vpages, l
 
 
 def paged_attn_workspace(B, Hq, Hkv, D, device):
-    """Zeroed workspace for paged_attn (reusable across calls that follow one another; concurrent streams need their own)."""
+    """Workspace for paged_attn, its counters zeroed (reusable across calls that follow one another; concurrent streams need their own)."""
     index = torch.empty(0, device=device).get_device()
     if index < 0:
         raise KvcError("paged_attn_workspace: %s is no CUDA device" % (device,))
     with _on(torch.device("cuda", index)):
-        n = _lib.load().kvc_paged_attn_workspace(B, Hq, Hkv, D)
-    return torch.zeros(n, dtype=torch.uint8, device=torch.device("cuda", index))
+        lib = _lib.load()
+        workspace = torch.empty(lib.kvc_paged_attn_workspace(B, Hq, Hkv, D), dtype=torch.uint8, device=torch.device("cuda", index))
+        workspace[:lib.kvc_paged_attn_cleared()].zero_()
+    return workspace
 
 
 def paged_attn(q, kpages, vpages, table, lengths, scaling, window=0, out=None, return_lse=False, workspace=None, status=None):
