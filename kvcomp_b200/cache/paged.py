@@ -1,0 +1,87 @@
+"""PagedKVCache: the cache of a serving batch, whose requests have lengths of their own and come and go.  Beside KVCompCache, which compresses a
+rectangular batch: here tokens stay fp16 or bf16, in pages that requests take from a common pool and give back.
+
+    cache = PagedKVCache(requests, pages, layer_num, kv_heads, head_dim, frequencies=..., ...)
+    plan = cache.begin(new, tokens)                        # once a step: new[b] tokens of request b, packed one request behind the other
+    for layer in range(layer_num):
+        q = cache.append(q, k, v, layer)                   # q, k rotated, k and v into their pages
+        out = cache.attend(q, layer)                       # a decode step: one token per request
+    cache.release(done)                                    # the pages of finished requests go back
+
+Everything is launched and nothing waited for or asked of the device: a step of one token per request can be captured into a CUDA graph and
+replayed, with the lengths, the tables and the free list going on from replay to replay.  (The prompt's own attention is the model's: its keys and
+values are in hand there.)"""
+import math
+
+import torch
+
+from .. import ops
+from .._lib import KvcError
+
+
+class PagedKVCache:
+    def __init__(self, requests, pages, layer_num, kv_heads, head_dim, page_size=64, max_tokens=None, dtype=torch.float16, device="cuda",
+                 frequencies=None, layout="half", factor=1.0, window=0):
+        """A pool of `pages` pages of `page_size` tokens for `requests` requests of up to max_tokens tokens each (all of the pool where it is not given).
+        frequencies, layout, factor: the rotation (utils.rotary.frequencies; None: keys and queries come rotated).  window > 0: attention over the
+        last `window` tokens."""
+        if min(requests, pages, layer_num, kv_heads, head_dim, page_size) <= 0:
+            raise KvcError("PagedKVCache: sizes must be positive")
+        if dtype not in (torch.float16, torch.bfloat16):
+            raise KvcError("PagedKVCache: fp16 or bf16, got %s" % dtype)
+        device = torch.empty(0, device=device).device
+        if device.type != "cuda":
+            raise KvcError("PagedKVCache: kvcomp_b200 has no CPU path")
+        self.requests, self.pages, self.layer_num, self.kv_heads, self.head_dim, self.page_size = requests, pages, layer_num, kv_heads, head_dim, page_size
+        self.max_tokens = pages * page_size if max_tokens is None else max_tokens
+        self.dtype, self.device, self.layout, self.factor, self.window = dtype, device, layout, float(factor), window
+        self.frequencies = None if frequencies is None else frequencies.to(device=device, dtype=torch.float64)
+        # (zeros: rows that no token was written to are never read, but a pool can be saved and compared)
+        self.keys, self.values = (torch.zeros(layer_num, pages, page_size, kv_heads, head_dim, dtype=dtype, device=device) for _ in range(2))
+        self.lengths = torch.zeros(requests, dtype=torch.int32, device=device)
+        self.table = torch.full((requests, -(-self.max_tokens // page_size)), -1, dtype=torch.int32, device=device)
+        self.free = torch.arange(pages, dtype=torch.int32, device=device)
+        self.head = torch.zeros(1, dtype=torch.int32, device=device)
+        self.status = ops.new_status(device)
+        self.plan = None
+        self._workspace = {}
+
+    def begin(self, new, tokens):
+        """A step that brings new[b] tokens (int32[requests], on the device) of each request, `tokens` rows in all.  Returns the plan (ops.PagePlan):
+        slots, positions, the requests' first rows; taken[b] = -1 where request b was refused: its tokens have no slot and it keeps its length.  The
+        cache's lengths, tables and free list are behind the step from here on."""
+        plan = ops.PagePlan(self.lengths, self.head, *(torch.empty(n, dtype=torch.int32, device=self.device) for n in (self.requests + 1, self.requests, tokens, tokens)))
+        self.plan = ops.page_plan(self.lengths, new, self.table, self.free, self.head, self.page_size, tokens, out=plan, status=self.status)
+        return self.plan
+
+    def append(self, query_states, key_states, value_states, layer_idx):
+        """The step's rows of a layer: queries [tokens, Hq, D] (or None), keys and values [tokens, Hkv, D].  Keys go rotated into their pages, values as they are;
+        returns the rotated queries."""
+        if self.plan is None:
+            raise KvcError("append before any begin")
+        return ops.rotary_paged_store(query_states, key_states, value_states, self.plan.positions, self.plan.slots, self.frequencies, self.keys[layer_idx],
+                                      self.values[layer_idx], layout=self.layout, factor=self.factor, status=self.status)
+
+    def attend(self, query_states, layer_idx, scaling=None, return_lse=False):
+        """One token per request: rotated queries [requests, Hq, D] -> [requests, Hq, D] over the tokens that each request has (0 for one that has none)."""
+        heads = query_states.shape[1]
+        workspace = self._workspace.get(heads)
+        if workspace is None:
+            workspace = self._workspace[heads] = ops.paged_attn_workspace(self.requests, heads, self.kv_heads, self.head_dim, self.device)
+        return ops.paged_attn(query_states, self.keys[layer_idx], self.values[layer_idx], self.table, self.lengths,
+                              1.0 / math.sqrt(self.head_dim) if scaling is None else scaling, window=self.window, return_lse=return_lse, workspace=workspace, status=self.status)
+
+    def release(self, done):
+        """The requests with done[b] (bool[requests], on the device) end: their pages go back, their lengths are 0."""
+        ops.page_release(self.lengths, done, self.table, self.free, self.head, self.page_size, out=(self.lengths, self.head), status=self.status)
+
+    def check(self):
+        """The conditions reported since the last check (_lib.FLAG_*; FLAG_NO_PAGES: a request was refused).  Raises where a page or a length was bad.
+        Synchronises; nothing else here does."""
+        flags = int(self.status.item())
+        self.status.zero_()
+        return ops.check_flags(flags, what="PagedKVCache")
+
+    def get_seq_length(self, request=0):
+        """Tokens of a request (synchronises)."""
+        return int(self.lengths[request].item())
