@@ -393,6 +393,35 @@ def test_attend_again_and_workspaces(ops):
     assert ops.paged_attn(*args, out=mine, workspace=ws) is mine and torch.equal(mine, out)
 
 
+@pytest.mark.parametrize("D,tokens", [(64, 60000), (96, 46000), (128, 46000)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_attend_long_shares(ops, D, tokens, dtype):
+    """So many tokens that CTAs draw the last of them (96 tiles of 64 for each CTA, up to four of which are on an SM).  The requests share their pages, one reads
+    another's backwards; some are short or empty.  The same bits again."""
+    Hq, Hkv, page = 16, 8, 64
+    lengths = [tokens, tokens - 1, 0, tokens + 777, tokens, 64, tokens, tokens - 4000, tokens, tokens + 1, 1]
+    assert sum(lengths) * Hkv > 96 * 64 * (4 if D == 64 else 3) * torch.cuda.get_device_properties(0).multi_processor_count
+    gen = torch.Generator(device="cuda").manual_seed(D)
+    pages = -(-max(lengths) // page)
+    rows = np.random.RandomState(D).permutation(pages).astype(np.int32)
+    table = np.stack([rows if b % 3 else rows[::-1] for b in range(len(lengths))])
+    kp, vp = (plain.pool(gen, pages, page, Hkv, D, dtype, "cuda") for _ in range(2))
+    q = torch.randn(len(lengths), Hq, D, generator=gen, device="cuda").to(dtype)
+    ws = ops.paged_attn_workspace(len(lengths), Hq, Hkv, D, "cuda")
+    args = (q, kp, vp, dev(table), dev(lengths), 0.3)
+    status = ops.new_status("cuda")
+    out, lse = ops.paged_attn(*args, return_lse=True, workspace=ws, status=status)
+    assert status.item() == 0
+    for _ in range(3):
+        again, lse2 = ops.paged_attn(*args, return_lse=True, workspace=ws)
+        assert torch.equal(out, again) and torch.equal(lse, lse2)
+    some = [0, 2, 3, 5, 9, 10]
+    want, want_lse, bound, lse_bound = plain.attend(q[some], kp, vp, dev(table[some]), [lengths[b] for b in some], 0.3)
+    near(out[some], want, bound)
+    there = [i for i, b in enumerate(some) if lengths[b]]
+    near(lse[some][there], want_lse[there], lse_bound[there])
+
+
 def test_attend_long_offsets(ops):
     """Pages whose offsets pass 32 bits: a pool of 5 GB of keys, the request's pages at both ends."""
     page, D = 64, 128
