@@ -6,8 +6,8 @@
 // What bounds it: every key and value is read once and used for Hq / Hkv heads, 4 (Hq / Hkv) operations per 4 bytes: HBM, for any
 // number of heads that a model has.  Everything else is arranged so that the loads never pause:
 //
-// Work is cut into tiles of 64 tokens of a column (a request's KV head), all tiles of all columns in one row; each CTA takes an equal, contiguous
-// share of the row, found from the lengths in the kernel (the host does not know them).  Lengths may be as unequal as they like, and a
+// Work is cut into tiles of 64 tokens of a column (a request's KV head; or 32 tokens of two heads, see choose_heads), all tiles of all columns in one row; each CTA takes
+// an equal, contiguous share of the row, found from the lengths in the kernel (the host does not know them).  Lengths may be as unequal as they like, and a
 // single long request is spread over the device.  A column that lies in one share is written at once; one that was cut leaves partial results {m, l,
 // sums} in the workspace, and the CTA that finishes last (a counter, put back to zero) joins them in the order of the shares, so that
 // the result does not depend on who that was.
@@ -31,27 +31,15 @@
 namespace {
 
 constexpr int WARPS = 4, THREADS = WARPS * 32;
-constexpr int TILE = 16 * WARPS;                // tokens of a tile
 constexpr int MAX_CTAS_PER_SM = 4;
 constexpr int DRAWN_REQUESTS = 1024;            // of more requests nothing is drawn: where a tile belongs is looked up in shared memory
-#ifndef DRAWN_SHARE
-#define DRAWN_SHARE 96
-#endif
+// Tiles of a share from which on the last eighth is drawn.  295 tiles (16 x 32768 tokens of 8 KV heads): 317 us, 333 undrawn; about 50 (64 requests of up to 4096 tokens,
+// 10 KV heads): 157 and 148, 37 (8 x 4096 of 32): 89.3 and 89.6.
+constexpr int DRAWN_SHARE = 96;
 constexpr int JOINED = 8;                       // partial results that are asked for at once
-constexpr int MIN_TILES = 2;                    // of a share
-#ifndef KVC_SC
-#define KVC_SC 3, 4, 4, 3
-#endif
-#ifndef KVC_SC96
-#define KVC_SC96 3, 3, 4, 2
-#endif
-#ifndef KVC_SC128
-#define KVC_SC128 2, 3, 3, 2
-#endif
-#ifndef KVC_SC256
-#define KVC_SC256 3, 1
-#endif
-constexpr int MAX_GROUP = 16;                   // query heads that a column serves
+// Tiles of a share at least: a tile more takes less than joining two parts (8 heads of 100 tokens 5.6 us, with 1 7.5, with 4, of 777 tokens of 32 heads, 12.2 for 10.9).
+constexpr int MIN_TILES = 2;
+constexpr int MAX_GROUP = 16;                   // query heads that a column serves (of all its KV heads)
 
 struct Params {
     kvc_paged_attn_args a;
@@ -130,7 +118,7 @@ __device__ __forceinline__ Span span_of(const Params &p, int b, int &flags) {
     s.first = p.a.window > 0 && len > p.a.window ? len - (int)p.a.window : 0;
     return s;
 }
-__device__ __forceinline__ int tiles_of(const Span &s) { return (s.len - s.first + TILE - 1) / TILE; }
+template <int TILE> __device__ __forceinline__ int tiles_of(const Span &s) { return (s.len - s.first + TILE - 1) / TILE; }
 
 // n / d of numbers that are not negative, through a float that a step or two put right
 __device__ __forceinline__ int quotient(int n, int d) {
@@ -142,7 +130,7 @@ __device__ __forceinline__ int quotient(int n, int d) {
 
 // A place in the row of tiles: tile `i` of column `c` of request `b`
 struct Place { int b, c, i, n; Span span; };
-__device__ __forceinline__ void next_tile(const Params &p, Place &at) {
+template <int TILE> __device__ __forceinline__ void next_tile(const Params &p, Place &at) {
     if (++at.i < at.n) return;
     at.i = 0;
     if (++at.c < p.columns) return;
@@ -151,13 +139,14 @@ __device__ __forceinline__ void next_tile(const Params &p, Place &at) {
     at.n = 0;
     while (++at.b < (int)p.a.B) {
         at.span = span_of(p, at.b, unused);
-        if ((at.n = tiles_of(at.span)) > 0) return;
+        if ((at.n = tiles_of<TILE>(at.span)) > 0) return;
     }
 }
 
-template <typename T, int D, int NT, bool SAME, int STAGES, int CTAS>
+template <typename T, int D, int NT, int WH, bool SAME, int STAGES, int CTAS>
 __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_constant__ Params p) {
     constexpr int KS = D / 16;                              // steps of 16 channels
+    constexpr int TEAM = WARPS / WH, TILE = 16 * TEAM;      // warps of a KV head, tokens of a tile
     constexpr uint32_t HALF_STAGE = 16 * D * 2, STAGE = 2 * HALF_STAGE;
     constexpr float LIFT = Pair<T>::LIFT;
     static_assert(STAGES + 2 <= DRAWN_SHARE - DRAWN_SHARE / 8, "a share is long enough for the first draw");
@@ -188,10 +177,10 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
     auto parts_of = [&](int tiles) { return __float2int_ru((float)tiles * even); };
     {
         const int b0 = min(B, lane * p.chunk), b1 = min(B, b0 + p.chunk);
-        const int n0 = b0 < b1 ? tiles_of(span_of(p, b0, flags)) : 0;
+        const int n0 = b0 < b1 ? tiles_of<TILE>(span_of(p, b0, flags)) : 0;
         unsigned mine = n0, some = n0 > 0;
         for (int b = b0 + 1; b < b1; b++) {
-            const int n = tiles_of(span_of(p, b, flags));
+            const int n = tiles_of<TILE>(span_of(p, b, flags));
             mine += n;
             some += n > 0;
         }
@@ -210,7 +199,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
             for (int tiles = size; tiles <= size + 2 * step; tiles += step) {
                 even = __frcp_rn((float)tiles);
                 unsigned k = parts_of(n0);
-                for (int b = b0 + 1; b < b1; b++) k += parts_of(tiles_of(span_of(p, b, unused)));
+                for (int b = b0 + 1; b < b1; b++) k += parts_of(tiles_of<TILE>(span_of(p, b, unused)));
                 if (__reduce_add_sync(0xffffffffu, k) * p.columns <= gridDim.x) {
                     mine = k;
                     break;
@@ -228,7 +217,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
         before -= mine;
         if (DRAWS && unit && warp == 0) {                   // (it is read behind the barriers at which pieces become known)
             unsigned tiles = before;
-            for (int b = b0; b < b1; b++) { before_s[b] = tiles; tiles += tiles_of(span_of(p, b, unused)); }
+            for (int b = b0; b < b1; b++) { before_s[b] = tiles; tiles += tiles_of<TILE>(span_of(p, b, unused)); }
         }
         all_tiles = (int)all;
         r0 = (int)min((unsigned long long)all, (unsigned long long)(even != 0.0f ? 1 : size) * blockIdx.x);
@@ -239,7 +228,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
         at.b = b0;
         if (here)
             for (;; at.b++) {
-                const int n = tiles_of(span_of(p, at.b, unused));
+                const int n = tiles_of<TILE>(span_of(p, at.b, unused));
                 const unsigned units = (unsigned)(even != 0.0f ? parts_of(n) : n) * p.columns;
                 if (rest < units) break;
                 rest -= units;
@@ -248,14 +237,14 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
         at.b = min(__shfl_sync(0xffffffffu, at.b, from), B - 1);
         rest = __shfl_sync(0xffffffffu, rest, from);
         at.span = span_of(p, at.b, unused);
-        at.n = tiles_of(at.span);
+        at.n = tiles_of<TILE>(at.span);
         const int units = max(even != 0.0f ? parts_of(at.n) : at.n, 1);
         at.c = quotient((int)rest, units);
         at.i = (int)rest - at.c * units;                    // the tile, or the part
     }
     // requests without tokens
     for (int b = blockIdx.x; b < B; b += gridDim.x) {
-        if (tiles_of(span_of(p, b, flags)) > 0) continue;
+        if (tiles_of<TILE>(span_of(p, b, flags)) > 0) continue;
         for (int i = tid; i < (int)a.Hq * (D / 8); i += THREADS)
             *reinterpret_cast<uint4 *>(reinterpret_cast<T *>(a.out) + b * a.out_token + i / (D / 8) * a.out_head + i % (D / 8) * 8) = make_uint4(0, 0, 0, 0);
         if (a.lse) for (int h = tid; h < (int)a.Hq; h += THREADS) a.lse[b * a.Hq + h] = -CUDART_INF_F;
@@ -303,19 +292,19 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
     auto ask = [&]() {
         page = -1;
         if (to_copy > 0 && lane < 16) {
-            const int t = ahead.span.first + ahead.i * TILE + warp * 16 + lane;
+            const int t = ahead.span.first + ahead.i * TILE + warp % TEAM * 16 + lane;
             if (t < ahead.span.len) page = __ldg(a.table + ahead.b * a.table_stride + kvc_divide(t, p.page));
         }
     };
     auto copy_tile = [&](int stage) {
         if (to_copy > 0) {
-            const int t = ahead.span.first + ahead.i * TILE + warp * 16 + lane;
+            const int t = ahead.span.first + ahead.i * TILE + warp % TEAM * 16 + lane;
             const bool there = lane < 16 && t < ahead.span.len, good = there && (unsigned)page < p.n_pages;
             if (there && !good) flags |= KVC_FLAG_BAD_PAGE;
             const uint32_t mask = __ballot_sync(0xffffffffu, good);
             if (lane == 0) masks[warp][stage] = mask;
             if (mask) {
-                const int hk = p.per_head == 1 ? ahead.c : ahead.c / p.per_head, row = t - kvc_divide(t, p.page) * (int)a.page_size;
+                const int hk = WH > 1 ? ahead.c * WH + warp / TEAM : (p.per_head == 1 ? ahead.c : ahead.c / p.per_head), row = t - kvc_divide(t, p.page) * (int)a.page_size;
                 const T *k16 = reinterpret_cast<const T *>(a.kpages), *v16 = reinterpret_cast<const T *>(a.vpages);
                 if (good) {
                     k16 += page * a.kp_page + row * (int)a.kp_row + hk * (int)a.kp_head;
@@ -338,7 +327,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
                     }
                 }
             }
-            next_tile(p, ahead);
+            next_tile<TILE>(p, ahead);
             if (--to_copy == 0 && DRAWS && next >= 0 && !taken) {
                 const int tile = start_of(next, to_copy);
                 int lo = 0, hi = B;
@@ -350,7 +339,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
                 const unsigned rest = (unsigned)tile - before_s[lo] * p.columns;
                 ahead.b = lo;
                 ahead.span = span_of(p, lo, unused);
-                ahead.n = tiles_of(ahead.span);
+                ahead.n = tiles_of<TILE>(ahead.span);
                 ahead.c = quotient((int)rest, ahead.n);
                 ahead.i = (int)rest - ahead.c * ahead.n;
                 if (lane == 0) next_start_s[warp] = ahead;
@@ -366,9 +355,14 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
     float o[KS][NT][4], m[NT][2], l[NT][2];
     int h0 = 0, heads = 0;
     auto begin_column = [&]() {                             // (the queries are asked for; they are first used behind the next wait)
-        const int hk = p.per_head == 1 ? at.c : at.c / p.per_head, g = (int)(a.Hq / a.Hkv), sub = (at.c - hk * p.per_head) * p.group;
-        h0 = hk * g + sub;
-        heads = min(p.group, g - sub);
+        if (WH > 1) {
+            h0 = (at.c * WH + warp / TEAM) * p.group;
+            heads = p.group;
+        } else {
+            const int hk = p.per_head == 1 ? at.c : at.c / p.per_head, g = (int)(a.Hq / a.Hkv), sub = (at.c - hk * p.per_head) * p.group;
+            h0 = hk * g + sub;
+            heads = min(p.group, g - sub);
+        }
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
             const int h = nt * 8 + (lane >> 2);
@@ -512,13 +506,13 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
                             }
                         }
                     }
-                const int of_b = at.b, of_h0 = h0, of_heads = heads, pieces = heads * (D / 4);
+                const int of_b = at.b, of_h0 = WH > 1 ? at.c * WH * p.group : h0, of_heads = WH * heads, pieces = of_heads * (D / 4);      // of all its KV heads
                 const bool whole = first_i == 0 && at.i == at.n - 1;        // the column lies in this share
                 const int begin = r0 + n - at.i;            // its first tile in the row of tiles
                 const int tiles = at.n, of_piece = piece, place = 2 * piece + (n - (at.i - first_i) > 0);
                 first_i = 0;
                 if (n < share - 1) {
-                    next_tile(p, at);
+                    next_tile<TILE>(p, at);
                     begin_column();                         // on their way while the sums are joined
                 } else if (DRAWS && next >= 0) {
                     piece = next;
@@ -539,25 +533,27 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
                     if (d == 0 && a.lse) a.lse[of_b * a.Hq + h] = sum == 0.0f ? -CUDART_INF_F : (top + log2f(sum) - LIFT) * 0.69314718055994531f;
                 };
                 float *part = p.parts + (long long)place * p.part;
-                for (int i = tid; i < pieces; i += THREADS) {
+                // the warps of a KV head join their sums
+                const int mine = of_heads / WH, sub = warp / TEAM * mine;       // a KV head's query heads, the first of them among the column's
+                for (int i = tid % (TEAM * 32); i < mine * (D / 4); i += TEAM * 32) {
                     const int h = i / (D / 4), d = i % (D / 4) * 4;
-                    float2 ml[WARPS];
+                    float2 ml[TEAM];
                     float top = -CUDART_INF_F, sum = 0.0f;
 #pragma unroll
-                    for (int w = 0; w < WARPS; w++) { ml[w] = ml_s[w][h]; top = fmaxf(top, ml[w].x); }
+                    for (int w = 0; w < TEAM; w++) { ml[w] = ml_s[warp / TEAM * TEAM + w][h]; top = fmaxf(top, ml[w].x); }
                     const float base = top == -CUDART_INF_F ? 0.0f : top;
                     float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-                    for (int w = 0; w < WARPS; w++) {
+                    for (int w = 0; w < TEAM; w++) {
                         const float f = exp2_approx(ml[w].x - base);
-                        const float4 x = *reinterpret_cast<const float4 *>(smem + w * STAGES * STAGE + scratch + (h * D + (d ^ ((h >> 1 & 3) * 8))) * 4);
+                        const float4 x = *reinterpret_cast<const float4 *>(smem + (warp / TEAM * TEAM + w) * STAGES * STAGE + scratch + (h * D + (d ^ ((h >> 1 & 3) * 8))) * 4);
                         sum += f * ml[w].y;
                         v.x += f * x.x; v.y += f * x.y; v.z += f * x.z; v.w += f * x.w;
                     }
-                    if (whole) write(i, top, sum, v);
+                    if (whole) write(sub * (D / 4) + i, top, sum, v);
                     else {
-                        __stcg(reinterpret_cast<float4 *>(part) + i, v);
-                        if (d == 0) __stcg(reinterpret_cast<float2 *>(part + p.group * D) + h, make_float2(top, sum));
+                        __stcg(reinterpret_cast<float4 *>(part) + sub * (D / 4) + i, v);
+                        if (d == 0) __stcg(reinterpret_cast<float2 *>(part + WH * p.group * D) + sub + h, make_float2(top, sum));
                     }
                 }
                 __syncthreads();
@@ -583,7 +579,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
                                         ml[k] = make_float2(-CUDART_INF_F, 0.0f);
                                         x[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                                         if (u < many) {
-                                            ml[k] = __ldcg(reinterpret_cast<const float2 *>(from + p.group * D) + h);
+                                            ml[k] = __ldcg(reinterpret_cast<const float2 *>(from + WH * p.group * D) + h);
                                             x[k] = __ldcg(reinterpret_cast<const float4 *>(from) + i);
                                         }
                                     }
@@ -626,7 +622,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
                         }
                         __syncthreads();
                         if (!final) {
-                            if (tid < of_heads) __stcg(reinterpret_cast<float2 *>(p.parts + (long long)(w == w_first ? first_place : 2 * w) * p.part + p.group * D) + tid, new_ml[tid]);
+                            if (tid < of_heads) __stcg(reinterpret_cast<float2 *>(p.parts + (long long)(w == w_first ? first_place : 2 * w) * p.part + WH * p.group * D) + tid, new_ml[tid]);
                             __syncthreads();
                         }
                     };
@@ -669,14 +665,18 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
     if (flags && a.status) atomicOr(a.status, flags);
 }
 
-template <typename T, int D, int NT, bool SAME, int STAGES, int CTAS>
-int launch(Params &p, long long most_tiles, cudaStream_t stream) {
+template <typename T, int D, int NT, int WH, bool SAME, int STAGES, int CTAS>
+int launch(Params &p, cudaStream_t stream) {
     static kvc_launch_slot slot;
     constexpr size_t shared = (size_t)WARPS * STAGES * 64 * D;
-    auto *kernel = paged_attn_kernel<T, D, NT, SAME, STAGES, CTAS>;
+    auto *kernel = paged_attn_kernel<T, D, NT, WH, SAME, STAGES, CTAS>;
     int occ = 0;
     if (int rc = kvc_prepare(slot, reinterpret_cast<const void *>(kernel), THREADS, shared, &occ)) return rc;
     KVC_REQUIRE(occ > 0, "kvc_paged_attn: the kernel does not fit this device");
+    constexpr int TILE = 16 * WARPS / WH;
+    p.columns /= WH;
+    const long long most_tiles = p.a.B * p.columns * ((p.a.table_width * p.a.page_size + TILE - 1) / TILE);
+    KVC_REQUIRE(p.a.B * p.columns < (1ll << 31) && most_tiles < (1ll << 31) - (1 << 20), "kvc_paged_attn: requests, KV heads and table rows of more than 2^31 tiles of %d tokens", TILE);
     const long long grid = std::max<long long>(std::min<long long>(most_tiles, (long long)std::min(occ, MAX_CTAS_PER_SM) * kvc_sm_count()), 1);
     p.per_cta = (float)(0.9999997 / grid);
     kernel<<<(unsigned)grid, THREADS, shared, stream>>>(p);
@@ -684,21 +684,29 @@ int launch(Params &p, long long most_tiles, cudaStream_t stream) {
     return KVC_OK;
 }
 
+// Stages of a warp's ring and CTAs of an SM, for up to 8 query heads of a KV head and for up to 16 (their accumulators take the registers of the third CTA): as many copies
+// under way as the shared memory holds.  128 channels: three CTAs of two stages, 89.5 us for 8 x 4096 tokens of 32 heads and 33.5 for 256 requests of up to 300,
+// two of three 95.5 and 46.8.
 template <typename T, int D, int STAGES, int CTAS, int WIDE_STAGES, int WIDE_CTAS>
-int choose_heads(Params &p, bool same, long long most, cudaStream_t s) {
+int choose_heads(Params &p, bool same, cudaStream_t s) {
     if constexpr (WIDE_STAGES > 0) {
-        if (p.group > 8) return same ? launch<T, D, 2, true, WIDE_STAGES, WIDE_CTAS>(p, most, s) : launch<T, D, 2, false, WIDE_STAGES, WIDE_CTAS>(p, most, s);
+        if (p.group > 8) return same ? launch<T, D, 2, 1, true, WIDE_STAGES, WIDE_CTAS>(p, s) : launch<T, D, 2, 1, false, WIDE_STAGES, WIDE_CTAS>(p, s);
     }
-    return same ? launch<T, D, 1, true, STAGES, CTAS>(p, most, s) : launch<T, D, 1, false, STAGES, CTAS>(p, most, s);
+    // Rows of 64 and 96 channels that lie head by head behind one another leave half of what the memory delivers at a time to the neighbour's row: two KV heads are read
+    // together.  32 x 8192 tokens of 8 heads: of 96 channels 151 us, 181 one by one, of 64 101 and 110.  (Of 128: 326 and 317 us for 16 x 32768.)
+    if constexpr (D < 128) {
+        if (same && p.per_head == 1 && p.a.Hkv % 2 == 0 && p.a.kp_head < p.a.kp_row) return launch<T, D, 1, 2, true, STAGES, CTAS>(p, s);
+    }
+    return same ? launch<T, D, 1, 1, true, STAGES, CTAS>(p, s) : launch<T, D, 1, 1, false, STAGES, CTAS>(p, s);
 }
 
 template <typename T>
-int choose(Params &p, bool same, long long most, cudaStream_t s) {
+int choose(Params &p, bool same, cudaStream_t s) {
     switch (p.a.D) {
-        case 64: return choose_heads<T, 64, KVC_SC>(p, same, most, s);
-        case 96: return choose_heads<T, 96, KVC_SC96>(p, same, most, s);
-        case 128: return choose_heads<T, 128, KVC_SC128>(p, same, most, s);
-        default: return choose_heads<T, 256, KVC_SC256, 0, 0>(p, same, most, s);
+        case 64: return choose_heads<T, 64, 3, 4, 4, 3>(p, same, s);
+        case 96: return choose_heads<T, 96, 3, 3, 4, 2>(p, same, s);
+        case 128: return choose_heads<T, 128, 2, 3, 3, 2>(p, same, s);
+        default: return choose_heads<T, 256, 3, 1, 0, 0>(p, same, s);
     }
 }
 
@@ -708,7 +716,7 @@ int64_t columns_of(int64_t Hq, int64_t Hkv, int64_t D) { return Hkv * ((Hq / Hkv
 // Of partial results: two for every piece.  Of s tiles for a CTA s / 8 and those left by rounding down are drawn, in rounds of s / 16, s / 32, s / 64 (at least) and what these leave:
 // a CTA's share and five pieces more.
 int64_t places(int64_t D) { return 2ll * 6 * (D == 64 ? 4 : 3) * kvc_sm_count(); }
-int64_t part_floats(int64_t group, int64_t D) { return std::max<int64_t>(group, 8) * (D + 2); }       // (room for eight heads at least: one workspace for more shapes)
+int64_t part_floats(int64_t group, int64_t D) { return std::max<int64_t>(group <= 8 && D < 128 ? 2 * group : group, 8) * (D + 2); }       // (of two KV heads where they are read together; room for eight heads at least: one workspace for more shapes)
 // The counter of what is drawn, and two counters for a place: of the column whose first result lies there, of the eight results that begin there.  They lie in
 // front, the same for calls of all shapes: a workspace may serve one after the other.
 int64_t counter_bytes() { return 256 + (2 * places(64) * 4 + 255) / 256 * 256; }
@@ -764,10 +772,8 @@ extern "C" int kvc_paged_attn(const kvc_paged_attn_args *args, kvc_stream_t stre
     p.counters = reinterpret_cast<unsigned *>(a.workspace) + 64;
     p.group_counters = p.counters + places(64);
     p.parts = reinterpret_cast<float *>(reinterpret_cast<uint8_t *>(a.workspace) + counter_bytes());
-    const long long most = a.B * p.columns * ((a.table_width * a.page_size + TILE - 1) / TILE);
     cudaStream_t s = kvc_cu(stream);
-    KVC_REQUIRE(a.B * p.columns < (1ll << 31) && most < (1ll << 31) - (1 << 20), "kvc_paged_attn: requests, KV heads and table rows of more than 2^31 tiles of %d tokens", TILE);
     p.v_less_k = reinterpret_cast<const uint8_t *>(a.vpages) - reinterpret_cast<const uint8_t *>(a.kpages);
     const bool same = a.kp_page == a.vp_page && a.kp_row == a.vp_row && a.kp_head == a.vp_head;
-    return a.type == KVC_TYPE_FP16 ? choose<__half>(p, same, most, s) : choose<__nv_bfloat16>(p, same, most, s);
+    return a.type == KVC_TYPE_FP16 ? choose<__half>(p, same, s) : choose<__nv_bfloat16>(p, same, s);
 }
