@@ -148,6 +148,29 @@ def load():
     return lib
 
 
+_torch_calls = None
+
+
+def torch_calls():
+    """The paged cache's calls for torch (csrc/kvc_torch.cpp), built first when the source is newer, with this library's entries.  Raises if it cannot."""
+    global _torch_calls
+    if _torch_calls is not None:
+        return _torch_calls
+    import importlib.machinery
+    import importlib.util
+
+    import torch  # noqa: F401  (its libraries are loaded first)
+    path = _build.build_binding()
+    loader = importlib.machinery.ExtensionFileLoader("kvc_torch", path)
+    module = importlib.util.module_from_spec(importlib.util.spec_from_file_location("kvc_torch", path, loader=loader))
+    loader.exec_module(module)
+    lib = load()
+    module.init(KvcError, *(C.cast(getattr(lib, name), C.c_void_p).value
+                            for name in ("kvc_page_plan", "kvc_page_release", "kvc_rotary_store", "kvc_paged_attn", "kvc_last_error")))
+    _torch_calls = module
+    return module
+
+
 def check(rc, what):
     if rc != KVC_OK:
         msg = load().kvc_last_error()

@@ -1,4 +1,5 @@
-"""Compile kvcomp_b200/csrc/*.cu into kvcomp_b200/lib/libkvcomp_b200.so for sm_100a.
+"""Compile kvcomp_b200/csrc/*.cu into kvcomp_b200/lib/libkvcomp_b200.so for sm_100a, and kvcomp_b200/csrc/kvc_torch.cpp, the paged cache's calls for torch, into
+kvcomp_b200/lib/kvc_torch.so.
 
     python -m kvcomp_b200.build [--force] [--verbose]
 
@@ -10,11 +11,14 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB_DIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIB_DIR, "libkvcomp_b200.so")
+BINDING = os.path.join(LIB_DIR, "kvc_torch.so")
+BINDING_SOURCE = os.path.join(CSRC, "kvc_torch.cpp")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
@@ -36,6 +40,42 @@ def is_stale():
     return any(os.path.getmtime(f) > t for f in _deps())
 
 
+def binding_is_stale():
+    if not os.path.exists(BINDING):
+        return True
+    t = os.path.getmtime(BINDING)
+    return any(os.path.getmtime(f) > t for f in [BINDING_SOURCE] + glob.glob(os.path.join(INCLUDE, "*.h")))
+
+
+def _run(cmd, to, verbose):
+    """Run a compiler that writes `to`.  It writes beside it first: a process that starts meanwhile sees the old file or the new one."""
+    made = "%s.%d.tmp" % (to, os.getpid())
+    r = subprocess.run(cmd + ["-o", made], capture_output=True, text=True)
+    if verbose:
+        sys.stderr.write(r.stdout + r.stderr)
+    if r.returncode != 0:
+        raise RuntimeError("%s failed:\n%s\n%s" % (os.path.basename(cmd[0]), " ".join(cmd), r.stderr[-4000:]))
+    os.replace(made, to)
+    return to
+
+
+def build_binding(force=False, verbose=False):
+    if not force and not binding_is_stale():
+        return BINDING
+    import torch
+    root = os.path.dirname(torch.__file__)
+    cuda = os.path.join(os.path.dirname(os.path.dirname(nvcc_path())), "include")
+    os.makedirs(LIB_DIR, exist_ok=True)
+    compiler = shutil.which(os.environ.get("CXX", "g++"))
+    if not compiler:
+        raise RuntimeError("no C++ compiler found; kvc_torch.so cannot be built")
+    cmd = [compiler, "-std=c++17", "-O2", "-shared", "-fPIC", "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI]
+    for d in (os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"), cuda, sysconfig.get_paths()["include"]):
+        cmd += ["-isystem", d]
+    cmd += [BINDING_SOURCE, "-L" + os.path.join(root, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
+    return _run(cmd, BINDING, verbose)
+
+
 def nvcc_path():
     for c in (os.environ.get("NVCC"), shutil.which("nvcc"), "/usr/local/cuda/bin/nvcc"):
         if c and os.path.exists(c):
@@ -44,16 +84,12 @@ def nvcc_path():
 
 
 def build(force=False, verbose=False):
+    """The library, and the binding where it is stale too."""
+    build_binding(force, verbose)
     if not force and not is_stale():
         return LIB
     os.makedirs(LIB_DIR, exist_ok=True)
-    cmd = [nvcc_path()] + NVCC_FLAGS + (["-Xptxas", "-v"] if verbose else []) + ["-o", LIB] + sources()
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if verbose:
-        sys.stderr.write(r.stdout + r.stderr)
-    if r.returncode != 0:
-        raise RuntimeError("nvcc failed:\n%s\n%s" % (" ".join(cmd), r.stderr[-4000:]))
-    return LIB
+    return _run([nvcc_path()] + NVCC_FLAGS + (["-Xptxas", "-v"] if verbose else []) + sources(), LIB, verbose)
 
 
 if __name__ == "__main__":

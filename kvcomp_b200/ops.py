@@ -709,64 +709,10 @@ def k_matvec(k, q, out):
 
 # ---- paged caches ----------------------------------------------------------------------------------------------------
 # Requests of different lengths share a pool of pages.  Lengths, block tables and the free list are device tensors: no call
-# below waits or asks the device for anything, and each can be captured into a graph.  A decode step makes three of these calls a layer: their
-# checks ask a tensor for as little as they can (50 to 200 ns each time), and temporaries are few (1 to 2 us each).
+# below waits or asks the device for anything, and each can be captured into a graph.  A decode step makes three of these calls a layer: tensors
+# are checked, results made and arguments packed by csrc/kvc_torch.cpp.
 
-_TYPES = {torch.float16: _lib.TYPE_FP16, torch.bfloat16: _lib.TYPE_BF16}
 _LAYOUTS = {"half": _lib.ROTARY_HALF, "interleaved": _lib.ROTARY_INTERLEAVED}
-_I32, _F64, _DENSE = torch.int32, torch.float64, torch.contiguous_format
-
-
-def _device_index(t, name):
-    """The number of the device that a call's first tensor lies on; all others have to lie there."""
-    i = t.get_device() if isinstance(t, torch.Tensor) else -1
-    if i < 0 or not t.is_cuda:
-        raise KvcError("%s must be a CUDA tensor (kvcomp_b200 has no CPU path)" % name)
-    return i
-
-
-def _words(t, n, name, index, dtype=_I32):
-    """The address of a vector of n words."""
-    if not isinstance(t, torch.Tensor) or t.get_device() != index or t.dtype is not dtype or t.shape != (n,) or not t.is_contiguous():
-        raise KvcError("%s must be a contiguous %s[%d] on cuda:%d" % (name, dtype, n, index))
-    return t.data_ptr()
-
-
-def _rows(t, shape, dtype, name, index):
-    """The address and strides of a tensor whose last dimension is contiguous."""
-    if not isinstance(t, torch.Tensor) or t.get_device() != index or t.dtype is not dtype or t.shape != shape:
-        raise KvcError("%s must be %s %s on cuda:%d" % (name, dtype, tuple(shape), index))
-    stride = t.stride()
-    if stride[-1] != 1 and shape[-1] > 1 and t.numel() > 0:
-        raise KvcError("%s must have its last dimension contiguous, got strides %s" % (name, stride))
-    return (t.data_ptr(), *stride[:-1])
-
-
-def _status_at(status, index):
-    return 0 if status is None else _words(status, 1, "status", index)
-
-
-def _table_at(table, B, index):
-    """Address, stride of the rows and their length of a block table."""
-    if not isinstance(table, torch.Tensor) or table.get_device() != index or table.dtype is not _I32 or table.dim() != 2:
-        raise KvcError("table must be int32 [%d, pages of a request] on cuda:%d" % (B, index))
-    rows, width = table.shape
-    stride, step = table.stride()
-    if rows != B or (step != 1 and width > 1 and B > 0):
-        raise KvcError("table must be int32 [%d, pages of a request], rows contiguous" % B)
-    return table.data_ptr(), stride if B > 1 else width, width
-
-
-def _launch(name, args, index):
-    """The call `name` of the library with packed arguments on the current stream of the device."""
-    call = getattr(_lib.load(), name)
-    if _raw_stream is not None and _get_device is not None and _get_device() == index:
-        rc = call(args, _raw_stream(index))
-    else:
-        with _on(torch.device("cuda", index)):
-            rc = call(args, _stream())
-    if rc:
-        _lib.check(rc, name)
 
 
 class PagePlan:
@@ -783,113 +729,34 @@ def page_plan(lengths, new, table, free, head, page_size, tokens, out=None, stat
     pages; free int32[pages of the pool]: the free list, a stack whose first head[0] (int32[1]) entries are taken.  tokens: rows of the step, at least
     sum(new); a request that finds no pages, no room in its table row or no rows is refused as a whole and keeps its length.  Returns a PagePlan;
     out: one to write into, whose lengths and head may be the ones given (a step that is captured goes on from its own result)."""
-    index = _device_index(lengths, "lengths")
-    B, pool, tokens = lengths.shape[0], free.numel(), int(tokens)
-    if tokens < 0:
-        raise KvcError("tokens must not be negative, got %d" % tokens)
+    call = _lib.torch_calls().page_plan
     if out is None:
-        # slots and positions first: they are written 16 bytes at a time where they can be
-        room = (tokens + 3) // 4 * 4
-        buf = torch.empty(2 * room + 3 * B + 2, dtype=_I32, device=lengths.device)
-        slots, a, positions, b, new_lengths, starts, taken, new_head = torch.split_with_sizes(buf, (tokens, room - tokens, tokens, room - tokens, B, B + 1, B, 1))
-        out = PagePlan(new_lengths, new_head, starts, taken, slots, positions)
-        at = buf.data_ptr()
-        at_lengths = at + 8 * room
-        outs = at_lengths, at_lengths + 4 * (3 * B + 1), at_lengths + 4 * B, at_lengths + 4 * (2 * B + 1), at, at + 4 * room
-    else:
-        outs = (_words(out.lengths, B, "out.lengths", index), _words(out.head, 1, "out.head", index), _words(out.starts, B + 1, "out.starts", index),
-                _words(out.taken, B, "out.taken", index), _words(out.slots, tokens, "out.slots", index), _words(out.positions, tokens, "out.positions", index))
-    _launch("kvc_page_plan", _lib.PAGE_PLAN_ARGS.pack(
-        _words(lengths, B, "lengths", index), _words(new, B, "new", index), _words(free, pool, "free", index), _words(head, 1, "head", index),
-        *_table_at(table, B, index), B, pool, page_size, tokens, *outs, _status_at(status, index)), index)
+        return PagePlan(*call(lengths, new, table, free, head, page_size, tokens, None, status))
+    call(lengths, new, table, free, head, page_size, tokens, (out.lengths, out.head, out.starts, out.taken, out.slots, out.positions), status)
     return out
 
 
 def page_release(lengths, done, table, free, head, page_size, out=None, status=None):
     """The pages of the requests with done[b] (bool[B]) go back to the free list, in place; (lengths, head) behind it: theirs 0.  out: (lengths, head) to
     write, which may be the ones given."""
-    index = _device_index(lengths, "lengths")
-    B, pool = lengths.shape[0], free.numel()
-    buf = torch.empty(2 * B + 2, dtype=_I32, device=lengths.device)
-    at = buf.data_ptr()
-    outs = at + 4 * (B + 1), at + 4 * (2 * B + 1)           # (behind the scratch of B + 1 words)
-    if out is None:
-        out = torch.split_with_sizes(buf, (B + 1, B, 1))[1:]
-    else:
-        outs = _words(out[0], B, "out lengths", index), _words(out[1], 1, "out head", index)
-    _launch("kvc_page_release", _lib.PAGE_RELEASE_ARGS.pack(
-        _words(lengths, B, "lengths", index), _words(done, B, "done", index, torch.bool), *_table_at(table, B, index), _words(free, pool, "free", index),
-        _words(head, 1, "head", index), B, pool, page_size, *outs, at, _status_at(status, index)), index)
-    return out
-
-
-def _turns(frequencies, positions, N, D, layout, index):
-    """Addresses of positions and frequencies, the number of rotated channels, the layout's number."""
-    lay = _LAYOUTS.get(layout)
-    if lay is None:
-        raise KvcError("layout must be 'half' or 'interleaved', got %r" % (layout,))
-    if frequencies is None:
-        return 0, 0, 0, lay
-    n = frequencies.numel() if isinstance(frequencies, torch.Tensor) else -1
-    if n < 0 or 2 * n > D:
-        raise KvcError("frequencies must be float64[rotated channels / 2], at most %d" % (D // 2))
-    return _words(positions, N, "positions", index), _words(frequencies, n, "frequencies", index, _F64), 2 * n, lay
+    out_lengths, out_head = (None, None) if out is None else out
+    return _lib.torch_calls().page_release(lengths, done, table, free, head, page_size, out_lengths, out_head, status)
 
 
 def rotary(x, positions, frequencies, layout="half", factor=1.0, inverse=False, out=None):
     """x fp16 or bf16 [N, H, D] rotated: the first 2 * len(frequencies) channels of each head in pairs by positions[n] * frequencies[i] (int32[N], float64),
     the others copied.  layout: "half" pairs channel i with i + half of the rotated ones, "interleaved" 2i with 2i + 1.  factor multiplies cos and
     sin.  inverse turns back (the gradient of the rotation, too).  out may be x.  utils.rotary.frequencies gives the frequencies of the usual scalings."""
-    index = _device_index(x, "x")
-    dtype, shape = x.dtype, x.shape
-    if len(shape) != 3 or dtype not in _TYPES:
-        raise KvcError("x must be fp16 or bf16 [N, H, D]")
-    N, H, D = shape
-    xa, x_token, x_head = _rows(x, shape, dtype, "x", index)
-    pos, freq, rotated, lay = _turns(frequencies, positions, N, D, layout, index)
-    out = torch.empty_like(x, memory_format=_DENSE) if out is None else out
-    oa, o_token, o_head = _rows(out, shape, dtype, "out", index)
-    _launch("kvc_rotary_store", _lib.ROTARY_ARGS.pack(
-        xa, 0, 0, oa, 0, 0, pos, 0, freq, N, H, 0, D, rotated, 0, 0, x_token, x_head, 0, 0, 0, 0, o_token, o_head, 0, 0, 0, 0, 0, 0, 0,
-        lay, 1 if inverse else 0, _TYPES[dtype], factor), index)
-    return out
+    return _lib.torch_calls().rotary_store(x, None, None, positions, None, frequencies, None, None, _LAYOUTS.get(layout), factor, inverse, out, None)
 
 
 def rotary_paged_store(q, k, v, positions, slots, frequencies, kpages, vpages, layout="half", factor=1.0, out=None, status=None):
     """A step's tokens: q [N, Hq, D] rotated (returned; out may be q, q may be None), k [N, Hkv, D] rotated into and v copied into the rows `slots`
     (int32[N], page * page_size + row; below 0: not stored) of the pools [pages, page_size, Hkv, D].  fp16 or bf16, any strides but a contiguous last
     dimension.  positions, frequencies, layout, factor: as for rotary; frequencies None: nothing is rotated.  Tokens of one call have slots of their own."""
-    index = _device_index(k, "k")
-    dtype, shape = k.dtype, k.shape
-    if len(shape) != 3 or dtype not in _TYPES or not isinstance(kpages, torch.Tensor) or kpages.dim() != 4:
-        raise KvcError("k must be fp16 or bf16 [N, Hkv, D], the pools [pages, page_size, Hkv, D]")
-    N, Hkv, D = shape
-    pool = kpages.shape
-    pages, page_size, pool_heads, pool_dim = pool
-    if pool_heads != Hkv or pool_dim != D:
-        raise KvcError("the pools must be [pages, page_size, %d, %d], got %s" % (Hkv, D, tuple(pool)))
-    ka, k_token, k_head = _rows(k, shape, dtype, "k", index)
-    va, v_token, v_head = _rows(v, shape, dtype, "v", index)
-    kp, kp_page, kp_row, kp_head = _rows(kpages, pool, dtype, "kpages", index)
-    vp, vp_page, vp_row, vp_head = _rows(vpages, pool, dtype, "vpages", index)
-    pos, freq, rotated, lay = _turns(frequencies, positions, N, D, layout, index)
-    qa = q_token = q_head = oa = o_token = o_head = Hq = 0
-    if q is None:
-        out = None
-    else:
-        Hq = q.shape[1] if isinstance(q, torch.Tensor) and q.dim() == 3 else 0
-        shape = (N, Hq, D)
-        qa, q_token, q_head = _rows(q, shape, dtype, "q", index)
-        if out is None:
-            out = torch.empty_like(q, memory_format=_DENSE)
-            oa, o_token, o_head = out.data_ptr(), Hq * D, D
-        else:
-            oa, o_token, o_head = _rows(out, shape, dtype, "out", index)
-    _launch("kvc_rotary_store", _lib.ROTARY_ARGS.pack(
-        qa, ka, va, oa, kp, vp, pos, _words(slots, N, "slots", index), freq, N, Hq, Hkv, D, rotated, pages, page_size,
-        q_token, q_head, k_token, k_head, v_token, v_head, o_token, o_head, kp_page, kp_row, kp_head, vp_page, vp_row, vp_head,
-        _status_at(status, index), lay, 0, _TYPES[dtype], factor), index)
-    return out
+    if k is None:
+        raise KvcError("k must be a tensor")
+    return _lib.torch_calls().rotary_store(q, k, v, positions, slots, frequencies, kpages, vpages, _LAYOUTS.get(layout), factor, False, out, status)
 
 
 def paged_attn_workspace(B, Hq, Hkv, D, device):
@@ -909,29 +776,8 @@ def paged_attn(q, kpages, vpages, table, lengths, scaling, window=0, out=None, r
     request has in the pages table[b] (int32 [B, pages]) of the pools [pages, page_size, Hkv, D]; window > 0: over the last `window` of them.  Requests
     without tokens: 0.  return_lse: (out, fp32 [B, Hq] log of the sum of exponentials, -inf without tokens).  D: 64, 96, 128, 256.
     workspace: paged_attn_workspace's, for one call at a time; None: one is made, and cleared, for this call."""
-    index = _device_index(q, "q")
-    dtype, shape = q.dtype, q.shape
-    if len(shape) != 3 or dtype not in _TYPES or not isinstance(kpages, torch.Tensor) or kpages.dim() != 4:
-        raise KvcError("q must be fp16 or bf16 [B, Hq, D], the pools [pages, page_size, Hkv, D]")
-    B, Hq, D = shape
-    pool = kpages.shape
-    pages, page_size, Hkv, pool_dim = pool
-    if pool_dim != D:
-        raise KvcError("the pools' heads have %d channels, q's %d" % (pool_dim, D))
-    qa, q_token, q_head = _rows(q, shape, dtype, "q", index)
-    kp, kp_page, kp_row, kp_head = _rows(kpages, pool, dtype, "kpages", index)
-    vp, vp_page, vp_row, vp_head = _rows(vpages, pool, dtype, "vpages", index)
-    if out is None:
-        out = torch.empty_like(q, memory_format=_DENSE)
-        oa, o_token, o_head = out.data_ptr(), Hq * D, D
-    else:
-        oa, o_token, o_head = _rows(out, shape, dtype, "out", index)
-    lse = torch.empty(B, Hq, dtype=torch.float32, device=q.device) if return_lse else None
     if workspace is None:
-        workspace = paged_attn_workspace(B, Hq, Hkv, D, q.device)
-    size = workspace.numel()
-    _launch("kvc_paged_attn", _lib.PAGED_ATTN_ARGS.pack(
-        qa, kp, vp, (at_table := _table_at(table, B, index))[0], _words(lengths, B, "lengths", index), oa, lse.data_ptr() if return_lse else 0,
-        _words(workspace, size, "workspace", index, torch.uint8), size, B, Hq, Hkv, D, pages, page_size, at_table[1], at_table[2], window,
-        q_token, q_head, o_token, o_head, kp_page, kp_row, kp_head, vp_page, vp_row, vp_head, _status_at(status, index), scaling, _TYPES[dtype]), index)
-    return (out, lse) if return_lse else out
+        if not isinstance(q, torch.Tensor) or not q.is_cuda or q.dim() != 3 or not isinstance(kpages, torch.Tensor) or kpages.dim() != 4:
+            raise KvcError("q must be a CUDA tensor [B, Hq, D], the pools [pages, page_size, Hkv, D] (kvcomp_b200 has no CPU path)")
+        workspace = paged_attn_workspace(q.shape[0], q.shape[1], kpages.shape[2], q.shape[2], q.device)
+    return _lib.torch_calls().paged_attn(q, kpages, vpages, table, lengths, scaling, window, out, return_lse, workspace, status)
