@@ -33,7 +33,7 @@ namespace {
 constexpr int WARPS = 4, THREADS = WARPS * 32;
 constexpr int MAX_CTAS_PER_SM = 4;
 constexpr int DRAWN_REQUESTS = 1024;            // of more requests nothing is drawn: where a tile belongs is looked up in shared memory
-// Tiles of a share from which on the last eighth is drawn.  295 tiles (16 x 32768 tokens of 8 KV heads): 317 us, 333 undrawn; about 50 (64 requests of up to 4096 tokens,
+// Tiles of a share from which on the last eighth is drawn.  148 tiles (16 x 32768 tokens of 8 KV heads): 317 us, 333 undrawn; 64 (64 requests of up to 4096 tokens,
 // 10 KV heads): 157 and 148, 37 (8 x 4096 of 32): 89.3 and 89.6.
 constexpr int DRAWN_SHARE = 96;
 constexpr int JOINED = 8;                       // partial results that are asked for at once
@@ -163,11 +163,13 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
     int flags = 0;
 
     // ---- this CTA's share
-    // Whole parts of columns, one for each CTA, where all columns together have no more of them than there are CTAs (few columns): no CTA has two to finish then.  Else
-    // equal shares of the row of all columns' tiles.  (All of it is on the way of the first byte: 32 bits, no division by what is known before.)
+    // Whole parts of columns, one for each CTA, where parts of up to 7 / 4 of an equal share do (few columns): no CTA has two to finish then, and fewer are joined; so many
+    // CTAs less still have as much under way as the memory gives (8 requests of 32 heads of 128 channels, one CTA a column: 512 tokens 15.7 us, 2048 45.6, 4096 85; in equal
+    // shares 19.6, 49.4, 90).  Tiles of shorter rows are less to have under way: 5 / 4 (11 x 4096 tokens of 32 heads of 96 channels 92 us, with 7 / 4 125); where an SM
+    // holds one CTA, 9 / 8.  Else equal shares of the row of all columns' tiles.
     // Of long shares an eighth is drawn from a counter instead, in pieces of a sixteenth of a share, then halves of it: the SMs do not get the same out of the
-    // memory (of 444 CTAs with 295 tiles each the first was done at 235 us, half at 285, the last at 319).  Where columns are few all of these pieces would be
-    // joined by few CTAs, and a CTA alone on its SM pauses at the end of every piece: equal shares there.
+    // memory (of 444 CTAs with 148 tiles each the first was done at 235 us, half at 285, the last at 319).  Where columns are few all of these pieces would be
+    // joined by few CTAs, and a CTA alone on its SM pauses at the end of every piece: not there.
     constexpr bool DRAWS = CTAS >= 3;
     // (All of this is on the way of the first byte.  Every warp does it by itself, for its lanes' requests: no barrier, no division but by a reciprocal.)
     int r0, r1, size;                                       // tiles [r0, r1) of the row, shares of `size`; or with even != 0: CTA r0, r1 = r0 + 1
@@ -194,9 +196,9 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
             size -= size / 8;
             drawn_from = size * (int)gridDim.x;
         } else if (there <= gridDim.x) {
-            const int step = max(1, size / 16);
+            const int step = max(1, size / (CTAS > 1 ? 4 : 16)), most = CTAS > 1 ? size * (D < 128 ? 5 : 7) / 4 + 2 : size + 2 * step;
 #pragma unroll 1
-            for (int tiles = size; tiles <= size + 2 * step; tiles += step) {
+            for (int tiles = size; tiles <= most; tiles += step) {
                 even = __frcp_rn((float)tiles);
                 unsigned k = parts_of(n0);
                 for (int b = b0 + 1; b < b1; b++) k += parts_of(tiles_of<TILE>(span_of(p, b, unused)));
