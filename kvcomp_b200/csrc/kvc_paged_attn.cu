@@ -32,7 +32,7 @@ namespace {
 
 constexpr int WARPS = 4, THREADS = WARPS * 32;
 constexpr int MAX_CTAS_PER_SM = 4;
-constexpr int DRAWN_REQUESTS = 1024;            // of more requests nothing is drawn: where a tile belongs is looked up in shared memory
+constexpr int DRAWN_REQUESTS = 512;             // of more requests nothing is drawn: where a tile belongs is looked up in shared memory
 // Tiles of a share from which on the last eighth is drawn.  148 tiles (16 x 32768 tokens of 8 KV heads): 317 us, 333 undrawn; 64 (64 requests of up to 4096 tokens,
 // 10 KV heads): 157 and 148, 37 (8 x 4096 of 32): 89.3 and 89.6.
 constexpr int DRAWN_SHARE = 96;
@@ -153,8 +153,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
     extern __shared__ __align__(128) uint8_t smem[];        // [warp][stage]: 16 rows of keys, 16 of values
     __shared__ uint32_t masks[WARPS][STAGES];
     __shared__ float2 ml_s[WARPS][8 * NT];                  // maximum and sum
-    __shared__ float4 join_v[THREADS];
-    __shared__ float2 join_ml[THREADS], new_ml[MAX_GROUP];
+    __shared__ float2 new_ml[MAX_GROUP];
     __shared__ Place next_start_s[WARPS];
     __shared__ unsigned before_s[CTAS >= 3 ? DRAWN_REQUESTS : 1];           // tiles of a column in front of a request
     __shared__ int last_s, next_s;
@@ -563,6 +562,9 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
                     const int w_first = even != 0.0f ? column_first : piece_of(begin), count = even != 0.0f ? parts : piece_of(begin + tiles - 1) - w_first + 1;
                     int unused;
                     const int first_place = 2 * w_first + (even == 0.0f && begin > start_of(w_first, unused));
+                    float4 *const join_v = reinterpret_cast<float4 *>(smem + scratch);       // (the stage that held the sums)
+                    float2 *const join_ml = reinterpret_cast<float2 *>(join_v + THREADS);
+                    static_assert(THREADS * 24 <= STAGE, "a stage has room for what is joined");
                     // the results of every step-th of `many` pieces from w on become one: the column's, or one in the first of their places
                     auto join = [&](int w, int step, int many, bool final) {
                         const int per = min(pieces, THREADS), ways = THREADS / per, way = tid / per;
