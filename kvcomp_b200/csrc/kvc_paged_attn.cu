@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
     // ---- this CTA's share
     // Whole parts of columns, one for each CTA, where parts of up to 7 / 4 of an equal share do (few columns): no CTA has two to finish then, and fewer are joined; so many
     // CTAs less still have as much under way as the memory gives (8 requests of 32 heads of 128 channels, one CTA a column: 512 tokens 15.7 us, 2048 45.6, 4096 85; in equal
-    // shares 19.6, 49.4, 90).  Tiles of shorter rows are less to have under way: 5 / 4 (11 x 4096 tokens of 32 heads of 96 channels 92 us, with 7 / 4 125); where an SM
+    // shares 19.6, 49.4, 90).  Tiles of shorter rows are less to have under way: 5 / 4 (11 x 4096 tokens of 32 heads of 96 channels 94 us, with 7 / 4 99); where an SM
     // holds one CTA, 9 / 8.  Else equal shares of the row of all columns' tiles.
     // Of long shares an eighth is drawn from a counter instead, in pieces of a sixteenth of a share, then halves of it: the SMs do not get the same out of the
     // memory (of 444 CTAs with 148 tiles each the first was done at 235 us, half at 285, the last at 319).  Where columns are few all of these pieces would be
@@ -697,7 +697,8 @@ int choose_heads(Params &p, bool same, cudaStream_t s) {
         if (p.group > 8) return same ? launch<T, D, 2, 1, true, WIDE_STAGES, WIDE_CTAS>(p, s) : launch<T, D, 2, 1, false, WIDE_STAGES, WIDE_CTAS>(p, s);
     }
     // Rows of 64 and 96 channels that lie head by head behind one another leave half of what the memory delivers at a time to the neighbour's row: two KV heads are read
-    // together.  32 x 8192 tokens of 8 heads: of 96 channels 151 us, 181 one by one, of 64 101 and 110.  (Of 128: 326 and 317 us for 16 x 32768.)
+    // together.  32 x 8192 tokens of 8 heads: of 96 channels 134 us, 177 one by one, of 64 89.5 and 91.4; 11 x 4096 of 32 heads of 96 94 and 126.  (Of 128: 326 and 317 us
+    // for 16 x 32768.)
     if constexpr (D < 128) {
         if (same && p.per_head == 1 && p.a.Hkv % 2 == 0 && p.a.kp_head < p.a.kp_row) return launch<T, D, 1, 2, true, STAGES, CTAS>(p, s);
     }

@@ -131,6 +131,42 @@ def test_release_of_more_than_was_taken(ops):
     assert np.array_equal(df.cpu().numpy(), want["free"]) and status.item() == _lib.FLAG_NO_PAGES
 
 
+def test_plan_and_release_in_a_graph(ops):
+    """Prompts admitted and given back by replays, in place, with rows and pages enough for the second kernels."""
+    rng = np.random.RandomState(5)
+    page, B, pages = 4, 70, 9000
+    new = rng.randint(0, 300, B)
+    tokens = int(new.sum())
+    table, free, _ = plain.tables(rng, [0] * B, page, pages, extra=200)
+    state = [dev([0] * B), dev(table), dev(free), dev([0])]
+    done = dev(rng.rand(B) < 0.5, torch.bool)
+    out = ops.PagePlan(state[0], state[3], *torch.zeros(2 * B + 1 + 2 * tokens, dtype=torch.int32, device="cuda").split((B + 1, B, tokens, tokens)))
+    status = ops.new_status("cuda")
+    dnew = dev(new)
+
+    def step():
+        ops.page_plan(state[0], dnew, state[1], state[2], state[3], page, tokens, out=out, status=status)
+        ops.page_release(state[0], done, state[1], state[2], state[3], page, out=(state[0], state[3]), status=status)
+
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    from kvcomp_b200 import _lib
+    lengths, head, refused = [0] * B, 0, False
+    for _ in range(3):
+        want = plain.plan(lengths, list(new), table, list(free), head, page, tokens)
+        refused |= want["refused"]                          # (the third time some table rows are full)
+        table = want["table"]
+        graph.replay()
+        assert out.slots.tolist() == want["slots"] and out.positions.tolist() == want["positions"] and out.starts.tolist() == want["starts"]
+        back = plain.release(want["lengths"], done.tolist(), table, free, want["head"], page)
+        lengths, head, free = back["lengths"], back["head"], back["free"]
+        assert state[0].tolist() == lengths and state[3].item() == head
+        assert np.array_equal(state[1].cpu().numpy(), table) and np.array_equal(state[2].cpu().numpy(), free)
+    assert status.item() == (_lib.FLAG_NO_PAGES if refused else 0)
+
+
 # ---- rotation ---------------------------------------------------------------------------------------------------
 
 def freqs(n, base=10000.0):
@@ -420,6 +456,24 @@ def test_attend_long_shares(ops, D, tokens, dtype):
     near(out[some], want, bound)
     there = [i for i, b in enumerate(some) if lengths[b]]
     near(lse[some][there], want_lse[there], lse_bound[there])
+
+
+def test_attend_on_two_streams(ops):
+    """Two calls at once with workspaces of their own; out may be q."""
+    args, out, _ = attend(ops, [5000, 70, 9000, 0], 8, 2, 128, torch.float16)
+    args2, out2, _ = attend(ops, [3000] * 6, 16, 1, 64, torch.bfloat16, seed=3)
+    streams, ws = [torch.cuda.Stream() for _ in range(2)], [ops.paged_attn_workspace(4, 8, 2, 128, "cuda"), ops.paged_attn_workspace(6, 16, 1, 64, "cuda")]
+    got = [[], []]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for i, a in enumerate((args, args2)):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(ops.paged_attn(*a, workspace=ws[i]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, out) for x in got[0]) and all(torch.equal(x, out2) for x in got[1])
+    q = args[0].clone()
+    ops.paged_attn(q, *args[1:], out=q, workspace=ws[0])
+    assert torch.equal(q, out)
 
 
 def test_attend_long_offsets(ops):
