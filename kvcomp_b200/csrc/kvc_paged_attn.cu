@@ -120,11 +120,13 @@ __device__ __forceinline__ Span span_of(const Params &p, int b, int &flags) {
 }
 template <int TILE> __device__ __forceinline__ int tiles_of(const Span &s) { return (s.len - s.first + TILE - 1) / TILE; }
 
-// n / d of numbers that are not negative, through a float that a step or two put right
+// n / d of numbers that are not negative, through a float that some steps put right (16 of them: it is off by 3 2^-24, and quotients are below 2^26).  Lengths are read more
+// than once: should a caller change them meanwhile, d may be 0 and results are anything, but every loop ends and nothing outside the arguments' tensors is touched.
 __device__ __forceinline__ int quotient(int n, int d) {
+    if (d <= 0) return 0;
     int q = (int)((float)n * __frcp_rn((float)d));
-    while ((unsigned)q * (unsigned)d > (unsigned)n) q--;
-    while ((unsigned)n - (unsigned)q * (unsigned)d >= (unsigned)d) q++;
+    for (int k = 0; k < 16 && (unsigned)q * (unsigned)d > (unsigned)n; k++) q--;
+    for (int k = 0; k < 16 && (unsigned)n - (unsigned)q * (unsigned)d >= (unsigned)d; k++) q++;
     return q;
 }
 
@@ -141,6 +143,8 @@ template <int TILE> __device__ __forceinline__ void next_tile(const Params &p, P
         at.span = span_of(p, at.b, unused);
         if ((at.n = tiles_of<TILE>(at.span)) > 0) return;
     }
+    at.b = (int)p.a.B - 1;                                  // (behind the last: a place without tokens)
+    at.span = {0, 0};
 }
 
 template <typename T, int D, int NT, int WH, bool SAME, int STAGES, int CTAS>
@@ -228,7 +232,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
         const bool here = (unsigned)r0 >= before * p.columns && rest < mine * p.columns;
         at.b = b0;
         if (here)
-            for (;; at.b++) {
+            for (; at.b < b1 - 1; at.b++) {
                 const int n = tiles_of<TILE>(span_of(p, at.b, unused));
                 const unsigned units = (unsigned)(even != 0.0f ? parts_of(n) : n) * p.columns;
                 if (rest < units) break;
