@@ -1,7 +1,7 @@
 // The paged cache's calls for torch: tensors checked, results allocated, arguments packed, the C ABI called.
 //
 // A decode step makes these calls for every layer, and its kernels take 3 to 10 us.  Asked for one by one from Python, what a call has to know of its tensors took longer than
-// that (13 to 15 us of the host for a call; here 6 to 8).  Nothing is computed here: torch carries memory and streams, the library's addresses are given by
+// that (13 to 15 us of the host for a call; here 5 to 6).  Nothing is computed here: torch carries memory and streams, the library's addresses are given by
 // init(), so that this file knows the ABI's structures and no symbol of the library.
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -111,6 +111,13 @@ void launch(int (*call)(const Args *, kvc_stream_t), const Args &args, int devic
 }
 
 at::Tensor ints(int64_t n, const at::Tensor &like) { return at::empty({n}, like.options()); }
+// a part of a buffer of words, as a tensor: a tenth of what a tensor of its own, or the buffer's narrow(), takes
+at::Tensor part(const at::Tensor &buffer, int64_t first, int64_t n) {
+    auto impl = c10::make_intrusive<c10::TensorImpl>(c10::TensorImpl::VIEW, c10::Storage(buffer.storage()), buffer.key_set(), buffer.dtype());
+    impl->set_storage_offset(first);
+    impl->set_sizes_contiguous({n});
+    return at::Tensor(std::move(impl));
+}
 int32_t *int_at(const at::Tensor &t) { return static_cast<int32_t *>(t.data_ptr()); }
 
 PyObject *tuple(std::initializer_list<at::Tensor> parts) {
@@ -150,8 +157,9 @@ PyObject *py_page_plan(PyObject *, PyObject *const *args, Py_ssize_t n) {
         launch(page_plan, a, device, "kvc_page_plan");
         result = Py_NewRef(Py_None);
     } else {
-        const at::Tensor out_lengths = ints(a.B, lengths), head = ints(1, lengths), starts = ints(a.B + 1, lengths), taken = ints(a.B, lengths), slots = ints(a.tokens, lengths),
-                         positions = ints(a.tokens, lengths);
+        const int64_t room = (a.tokens + 3) / 4 * 4;        // (slots and positions are written 16 bytes at a time)
+        const at::Tensor all = ints(2 * room + 3 * a.B + 2, lengths), slots = part(all, 0, a.tokens), positions = part(all, room, a.tokens), out_lengths = part(all, 2 * room, a.B),
+                         head = part(all, 2 * room + a.B, 1), starts = part(all, 2 * room + a.B + 1, a.B + 1), taken = part(all, 2 * room + 2 * a.B + 2, a.B);
         a.lengths_out = int_at(out_lengths); a.head_out = int_at(head); a.starts = int_at(starts); a.taken = int_at(taken);
         a.slots = int_at(slots); a.positions = int_at(positions);
         launch(page_plan, a, device, "kvc_page_plan");
@@ -178,15 +186,15 @@ PyObject *py_page_release(PyObject *, PyObject *const *args, Py_ssize_t n) {
     a.head = static_cast<int32_t *>(words(args[4], 1, "head", device));
     a.page_size = number(args[5]);
     a.status = status_of(args[8], device);
-    const at::Tensor first = ints(a.B + 1, lengths);
-    a.first = int_at(first);
+    const at::Tensor all = ints(2 * a.B + 2, lengths);      // scratch of B + 1 words, lengths, head
+    a.first = int_at(all);
     if (given(args[6])) {
         a.lengths_out = static_cast<int32_t *>(words(args[6], a.B, "out lengths", device));
         a.head_out = static_cast<int32_t *>(words(args[7], 1, "out head", device));
         launch(page_release, a, device, "kvc_page_release");
         return PyTuple_Pack(2, args[6], args[7]);
     }
-    const at::Tensor out_lengths = ints(a.B, lengths), head = ints(1, lengths);
+    const at::Tensor out_lengths = part(all, a.B + 1, a.B), head = part(all, 2 * a.B + 1, 1);
     a.lengths_out = int_at(out_lengths); a.head_out = int_at(head);
     launch(page_release, a, device, "kvc_page_release");
     return tuple({out_lengths, head});
