@@ -48,7 +48,7 @@ struct Params {
     int group, columns, per_head;               // query heads of a column at most, columns of a request, columns of a KV head
     int most_tokens;                            // of a table row
     unsigned n_pages;
-    uint32_t sign;                              // of the scaling, for two values: the scores' maximum is taken before they are scaled
+    int negative;                               // scaling: the scores' maximum is taken before they are scaled
     float log2_scaling, per_cta;                // per_cta: a little less than one over the number of CTAs
     long long v_less_k;                         // bytes from the keys' pool to the values'
     int *drawn;                                 // how many pieces have been drawn
@@ -374,8 +374,8 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
             const T *from = reinterpret_cast<const T *>(a.q) + at.b * a.q_token + (h0 + h) * a.q_head + (lane & 3) * 2;
 #pragma unroll
             for (int k = 0; k < KS; k++) {
-                q[k][nt][0] = h < heads ? *reinterpret_cast<const uint32_t *>(from + k * 16) ^ p.sign : 0;
-                q[k][nt][1] = h < heads ? *reinterpret_cast<const uint32_t *>(from + k * 16 + 8) ^ p.sign : 0;
+                q[k][nt][0] = h < heads ? *reinterpret_cast<const uint32_t *>(from + k * 16) : 0;
+                q[k][nt][1] = h < heads ? *reinterpret_cast<const uint32_t *>(from + k * 16 + 8) : 0;
             }
         }
     };
@@ -432,6 +432,12 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
                 for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                     for (int e = 0; e < 4; e++) s[0][nt][e] += s[1][nt][e];
+                if (p.negative) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) s[0][nt][e] = -s[0][nt][e];
+                }
                 if (mask != 0xffff) {
                     const bool on0 = mask >> (lane >> 2) & 1, on1 = mask >> (8 + (lane >> 2)) & 1;
 #pragma unroll
@@ -518,16 +524,15 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
                 first_i = 0;
                 if (n < share - 1) {
                     next_tile<TILE>(p, at);
-                    begin_column();                         // on their way while the sums are joined
                 } else if (DRAWS && next >= 0) {
                     piece = next;
                     next = -1;
                     r0 = start_of(piece, share);
                     at = next_start_s[warp];
                     first_i = at.i;
-                    begin_column();
                     n = -1;                                 // (the loop goes on with 0)
                 } else n = share;                           // (it ends)
+                if (n != share) begin_column();             // on their way while the sums are joined
                 clear();
                 __syncthreads();
                 auto write = [&](int i, float top, float sum, const float4 &v) {       // four channels of a result
@@ -774,7 +779,7 @@ extern "C" int kvc_paged_attn(const kvc_paged_attn_args *args, kvc_stream_t stre
     p.chunk = (int)((a.B + 31) / 32);
     p.most_tokens = (int)(a.table_width * a.page_size);
     p.n_pages = (unsigned)a.n_pages;
-    p.sign = a.scaling < 0.0f ? 0x80008000u : 0;
+    p.negative = a.scaling < 0.0f;
     p.log2_scaling = std::max(fabsf(a.scaling) * 1.4426950408889634f, 1e-37f);      // (0 times the -inf of a token that is left out is none)
     p.part = (int)part_floats(p.group, a.D);
     p.drawn = reinterpret_cast<int *>(a.workspace);
