@@ -62,7 +62,6 @@ template <> struct Pair<__half> {
     static constexpr float LIFT = 14.0f;
     static __device__ __forceinline__ uint32_t pack(float a, float b) { const __half2 r = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t *>(&r); }
     static __device__ __forceinline__ float2 unpack(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2 *>(&v)); }
-    static __device__ __forceinline__ __half one(float a) { return __float2half_rn(a); }
     static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -72,7 +71,6 @@ template <> struct Pair<__nv_bfloat16> {
     static constexpr float LIFT = 0.0f;
     static __device__ __forceinline__ uint32_t pack(float a, float b) { const __nv_bfloat162 r = __floats2bfloat162_rn(a, b); return *reinterpret_cast<const uint32_t *>(&r); }
     static __device__ __forceinline__ float2 unpack(uint32_t v) { return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&v)); }
-    static __device__ __forceinline__ __nv_bfloat16 one(float a) { return __float2bfloat16_rn(a); }
     static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -642,11 +640,11 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
                     // whether this CTA is the last of `many` at a counter, which is zero again then; what they wrote before is seen behind it
                     auto is_last = [&](unsigned *counter, int many) {
                         if (tid == 0) {
-                            __threadfence();
-                            const bool last = atomicAdd(counter, 1u) == (unsigned)(many - 1);
+                            unsigned before;                // (the barrier ahead made the CTA's writes this thread's: it releases them, and acquires the others')
+                            asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(before) : "l"(counter) : "memory");
+                            const bool last = before == (unsigned)(many - 1);
                             if (last) *counter = 0;
                             last_s = last;
-                            __threadfence();
                         }
                         __syncthreads();
                         const bool last = last_s;
@@ -751,7 +749,7 @@ extern "C" int kvc_paged_attn(const kvc_paged_attn_args *args, kvc_stream_t stre
     KVC_REQUIRE(a.D == 64 || a.D == 96 || a.D == 128 || a.D == 256, "kvc_paged_attn: heads of 64, 96, 128 or 256 channels, got %lld", (long long)a.D);
     KVC_REQUIRE(a.B >= 0 && a.Hkv > 0 && a.Hq > 0 && a.Hq % a.Hkv == 0 && a.Hq < 65536, "kvc_paged_attn: %lld query heads over %lld", (long long)a.Hq, (long long)a.Hkv);
     KVC_REQUIRE(a.page_size > 0 && a.page_size <= KVC_MAX_PAGE && a.n_pages >= 0 && a.n_pages < (1ll << 31) && a.table_width >= 0 && a.window >= 0, "kvc_paged_attn: bad sizes");
-    KVC_REQUIRE(a.table_width * a.page_size < (1ll << 31), "kvc_paged_attn: a table row holds %lld tokens, lengths have 32 bits", (long long)(a.table_width * a.page_size));
+    KVC_REQUIRE(a.table_width * a.page_size < (1ll << 31) - 256, "kvc_paged_attn: a table row holds %lld tokens, lengths have 32 bits", (long long)(a.table_width * a.page_size));
     if (a.B == 0) return KVC_OK;
     KVC_REQUIRE(a.B < (1 << 24), "kvc_paged_attn: %lld requests", (long long)a.B);
     KVC_REQUIRE(a.q && a.out && a.lengths && (a.table || a.table_width == 0) && ((a.kpages && a.vpages) || a.n_pages == 0), "kvc_paged_attn: null pointer");
