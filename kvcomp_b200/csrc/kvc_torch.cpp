@@ -1,6 +1,6 @@
 // The paged cache's calls for torch: tensors checked, results allocated, arguments packed, the C ABI called.
 //
-// A decode step makes these calls for every layer, and its kernels take 3 to 10 us.  Asked for one by one from Python, what a call has to know of its tensors took longer than
+// A decode step makes these calls for every layer, and its kernels take 2 to 10 us.  Asked for one by one from Python, what a call has to know of its tensors took longer than
 // that (13 to 15 us of the host for a call; here 5 to 6).  Nothing is computed here: torch carries memory and streams, the library's addresses are given by
 // init(), so that this file knows the ABI's structures and no symbol of the library.
 #include <torch/csrc/Exceptions.h>
