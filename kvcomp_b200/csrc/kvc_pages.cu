@@ -124,7 +124,7 @@ __global__ void __launch_bounds__(THREADS) page_plan_kernel(const __grid_constan
     kvc_behind();
     const int B = (int)a.B;
     const long long head = min(max((long long)a.head[0], 0ll), (long long)a.n_pages);
-    long long rows = 0, pages = 0, given = 0;               // in front of this round's requests; what this thread's have been given, with all before them
+    long long rows = 0, pages = 0, given = 0;               // in front of these 1024 requests; what this thread's have been given, with all before them
     int flags = a.head[0] != head ? KVC_FLAG_BAD_LENGTH : 0;
     for (int b0 = 0; b0 < B; b0 += THREADS) {
         const int b = b0 + threadIdx.x;

@@ -153,6 +153,42 @@ def test_a_step_in_a_graph(Cache):
     assert a.lengths.tolist() == [9 + 13, 5, 17 + 13, 4 + 13, 5] and a.check() == 0
 
 
+def test_a_step_captured_behind_two_streams(Cache):
+    """The step's first kernels follow a copy, a memset and another stream's kernels in one graph."""
+    from kvcomp_b200 import ops
+    R, D = 3, 64
+    cache = Cache(R, 30, 1, 2, D, page_size=8, frequencies=frequencies(D)[0])
+    rows, new = torch.randn(R, 6, D, device="cuda").half(), dev([0] * R)
+    counts, scratch = dev([2, 1, 3]).cpu().pin_memory(), torch.ones(100000, device="cuda")
+    x = torch.randn(6, 6, D, device="cuda").half()
+    cache.attend(rows[:, :2], 0)                           # (the workspace)
+    torch.cuda.synchronize()
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph):
+        main = torch.cuda.current_stream()
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            for _ in range(20):
+                scratch.mul_(1.0)
+            turned = ops.rotary(x, cache_positions := torch.zeros(6, dtype=torch.int32, device="cuda"), cache.frequencies)
+        new.copy_(counts, non_blocking=True)
+        main.wait_stream(side)
+        plan = cache.begin(new, 6)
+        cache_positions.zero_()
+        q = cache.append(turned[:, :2], x[:, 2:4], x[:, 4:], 0)
+        out = cache.attend(rows[:, :2], 0)
+    want, lengths = None, [0] * R
+    for _ in range(4):
+        graph.replay()
+        lengths = [n + k for n, k in zip(lengths, [2, 1, 3])]
+        assert cache.lengths.tolist() == lengths and plan.positions.tolist() == [n - k + j for n, k in zip(lengths, [2, 1, 3]) for j in range(k)]
+        want, _, bound, _ = plain.attend(rows[:, :2], cache.keys[0], cache.values[0], cache.table, lengths, 1 / math.sqrt(D))
+        assert bool(((out.cpu().double() - want).abs() <= bound).all())
+        rot = plain.rotate(x[:, :2].cpu(), plan.positions.cpu(), cache.frequencies.cpu(), "half")
+        assert bool(((q.cpu().double() - rot).abs() <= plain.rotate_bound(x[:, :2].cpu(), rot, cache.frequencies, "half", 1.0)).all())
+    assert cache.check() == 0
+
+
 def test_refusals(Cache):
     from kvcomp_b200._lib import KvcError
     for kw in (dict(dtype=torch.float32), dict(device="cpu"), dict(page_size=0)):
