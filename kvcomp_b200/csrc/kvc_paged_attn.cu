@@ -728,7 +728,9 @@ int64_t columns_of(int64_t Hq, int64_t Hkv, int64_t D) { return Hkv * ((Hq / Hkv
 // Of partial results: two for every piece.  Of s tiles for a CTA s / 8 and those left by rounding down are drawn, in rounds of s / 16, s / 32, s / 64 (at least) and what these leave:
 // a CTA's share and five pieces more.
 int64_t places(int64_t D) { return 2ll * 6 * (D == 64 ? 4 : 3) * kvc_sm_count(); }
-int64_t part_floats(int64_t group, int64_t D) { return std::max<int64_t>(group <= 8 && D < 128 ? 2 * group : group, 8) * (D + 2); }       // (of two KV heads where they are read together; room for eight heads at least: one workspace for more shapes)
+// Floats of a place: of two KV heads where they are read together; room for eight heads at least, so that one workspace serves more shapes.  A multiple of four: values are
+// written and read sixteen bytes at a time, and n (D + 2) is two more than one for odd n.
+int64_t part_floats(int64_t group, int64_t D) { return (std::max<int64_t>(group <= 8 && D < 128 ? 2 * group : group, 8) * (D + 2) + 3) / 4 * 4; }
 // The counter of what is drawn, and two counters for a place: of the column whose first result lies there, of the eight results that begin there.  They lie in
 // front, the same for calls of all shapes: a workspace may serve one after the other.
 int64_t counter_bytes() { return 256 + (2 * places(64) * 4 + 255) / 256 * 256; }
