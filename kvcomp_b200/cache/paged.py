@@ -9,13 +9,14 @@ rectangular batch: here tokens stay fp16 or bf16, in pages that requests take fr
     cache.release(done)                                    # the pages of finished requests go back
 
 Everything is launched and nothing waited for or asked of the device: a step of one token per request can be captured into a CUDA graph and
-replayed, with the lengths, the tables and the free list going on from replay to replay.  (The prompt's own attention is the model's: its keys and
+replayed, with the lengths, the tables and the free list going on from replay to replay; nothing has to be called before it.  Layers may be attended on streams of
+their own (each keeps a workspace of 15 to 45 MB, and so does each graph).  (The prompt's own attention is the model's: its keys and
 values are in hand there.)"""
 import math
 
 import torch
 
-from .. import ops
+from .. import _lib, ops
 from .._lib import KvcError
 
 
@@ -44,7 +45,10 @@ class PagedKVCache:
         self.head = torch.zeros(1, dtype=torch.int32, device=device)
         self.status = ops.new_status(device)
         self.plan = None
-        self._workspace = {}
+        self._workspaces = {}
+
+    def __getstate__(self):
+        return dict(self.__dict__, _workspaces={})                   # (a copy makes its own)
 
     def begin(self, new, tokens):
         """A step that brings new[b] tokens (int32[requests], on the device) of each request, `tokens` rows in all.  Returns the plan (ops.PagePlan):
@@ -64,12 +68,20 @@ class PagedKVCache:
 
     def attend(self, query_states, layer_idx, scaling=None, return_lse=False):
         """One token per request: rotated queries [requests, Hq, D] -> [requests, Hq, D] over the tokens that each request has (0 for one that has none)."""
-        heads = query_states.shape[1]
-        workspace = self._workspace.get(heads)
-        if workspace is None:
-            workspace = self._workspace[heads] = ops.paged_attn_workspace(self.requests, heads, self.kv_heads, self.head_dim, self.device)
+        workspace = self._workspace(query_states.shape[1])
         return ops.paged_attn(query_states, self.keys[layer_idx], self.values[layer_idx], self.table, self.lengths,
                               1.0 / math.sqrt(self.head_dim) if scaling is None else scaling, window=self.window, return_lse=return_lse, workspace=workspace, status=self.status)
+
+    def _workspace(self, heads):
+        """The attention's workspace, cleared, for the current stream: calls on streams of their own may run at once.  A capture has its own too, cleared by the
+        graph where the capture's first call lies (a launch more for a graph): an eager call or another graph neither finds it uncleared nor in use."""
+        stream, capture = _lib.torch_calls().stream_of(self.device.index)
+        workspace = self._workspaces.get((heads, stream, capture))
+        if workspace is None:
+            if capture:                                              # captures on this stream before are over: their memory is their graphs'
+                self._workspaces = {key: w for key, w in self._workspaces.items() if key[1] != stream or key[2] in (0, capture)}
+            workspace = self._workspaces[heads, stream, capture] = ops.paged_attn_workspace(self.requests, heads, self.kv_heads, self.head_dim, self.device)
+        return workspace
 
     def release(self, done):
         """The requests with done[b] (bool[requests], on the device) end: their pages go back, their lengths are 0."""

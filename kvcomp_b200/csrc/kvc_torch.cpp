@@ -304,6 +304,19 @@ PyObject *py_paged_attn(PyObject *, PyObject *const *args, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// device -> (handle of its current stream, number of the capture that it is in or 0)
+PyObject *py_stream_of(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    count(n, 1);
+    const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(number(args[0]))).stream();
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    unsigned long long capture = 0;
+    // (the legacy stream does not answer while another thread captures: it is in none then)
+    if (cudaStreamGetCaptureInfo(stream, &status, &capture) != cudaSuccess) (void)cudaGetLastError(), status = cudaStreamCaptureStatusNone;
+    return Py_BuildValue("KK", static_cast<unsigned long long>(reinterpret_cast<uintptr_t>(stream)), status == cudaStreamCaptureStatusNone ? 0ull : capture);
+    END_HANDLE_TH_ERRORS
+}
+
 // the error's class and the addresses of the library's entries
 PyObject *py_init(PyObject *, PyObject *const *args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
@@ -326,6 +339,7 @@ PyMethodDef methods[] = {{"init", fast<py_init>(), METH_FASTCALL, nullptr},
                          {"page_release", fast<py_page_release>(), METH_FASTCALL, nullptr},
                          {"rotary_store", fast<py_rotary_store>(), METH_FASTCALL, nullptr},
                          {"paged_attn", fast<py_paged_attn>(), METH_FASTCALL, nullptr},
+                         {"stream_of", fast<py_stream_of>(), METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "kvc_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -760,7 +760,8 @@ def rotary_paged_store(q, k, v, positions, slots, frequencies, kpages, vpages, l
 
 
 def paged_attn_workspace(B, Hq, Hkv, D, device):
-    """Workspace for paged_attn, its counters zeroed (reusable across calls that follow one another; concurrent streams need their own)."""
+    """Workspace for paged_attn, its counters zeroed (reusable across calls that follow one another; concurrent streams need their own, and so do graphs that may run at
+    once).  Made while a graph is captured it is zeroed by the graph, and serves that graph only."""
     index = torch.empty(0, device=device).get_device()
     if index < 0:
         raise KvcError("paged_attn_workspace: %s is no CUDA device" % (device,))
