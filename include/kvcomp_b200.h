@@ -466,6 +466,9 @@ typedef struct {
 int64_t kvc_paged_attn_cleared(void);
 int64_t kvc_paged_attn_workspace(int64_t B, int64_t Hq, int64_t Hkv, int64_t D);
 int kvc_paged_attn(const kvc_paged_attn_args *args, kvc_stream_t stream);
+/* The same where not every request has a row: q and out have `rows` rows, request b's are starts[b] .. starts[b + 1] - 1 (B + 1 numbers in order, on the device: a
+ * plan's).  A request without a row is left out.  Rows behind the last request's, and those of a request that has more than one (KVC_FLAG_BAD_LENGTH), get 0 and -inf. */
+int kvc_paged_attn_rows(const kvc_paged_attn_args *args, const int32_t *starts, int64_t rows, kvc_stream_t stream);
 
 #ifdef __cplusplus
 }

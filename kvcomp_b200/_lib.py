@@ -117,6 +117,7 @@ _SIGNATURES = {
     "kvc_paged_attn_cleared": (_i64, []),
     "kvc_paged_attn_workspace": (_i64, [_i64, _i64, _i64, _i64]),
     "kvc_paged_attn": (_i32, [C.c_char_p, _vp]),
+    "kvc_paged_attn_rows": (_i32, [C.c_char_p, _vp, _i64, _vp]),
     "kvc_k_matvec": (_i32, [_vp, _vp, _vp, _i64, _i64, _vp]),
 }
 
@@ -166,7 +167,7 @@ def torch_calls():
     loader.exec_module(module)
     lib = load()
     module.init(KvcError, *(C.cast(getattr(lib, name), C.c_void_p).value
-                            for name in ("kvc_page_plan", "kvc_page_release", "kvc_rotary_store", "kvc_paged_attn", "kvc_last_error")))
+                            for name in ("kvc_page_plan", "kvc_page_release", "kvc_rotary_store", "kvc_paged_attn", "kvc_paged_attn_rows", "kvc_last_error")))
     _torch_calls = module
     return module
 

@@ -5,11 +5,11 @@ rectangular batch: here tokens stay fp16 or bf16, in pages that requests take fr
     plan = cache.begin(new, tokens)                        # once a step: new[b] tokens of request b, packed one request behind the other
     for layer in range(layer_num):
         q = cache.append(q, k, v, layer)                   # q, k rotated, k and v into their pages
-        out = cache.attend(q, layer)                       # a decode step: one token per request
+        out = cache.attend(q, layer)                       # a decode step: one token per request, or none; row by row as the step is packed
     cache.release(done)                                    # the pages of finished requests go back
 
 Everything is launched and nothing waited for or asked of the device: a step of one token per request can be captured into a CUDA graph and
-replayed, with the lengths, the tables and the free list going on from replay to replay; nothing has to be called before it.  Layers may be attended on streams of
+replayed, with the lengths, the tables and the free list going on from replay to replay (new[b] may be 0 in any of them); nothing has to be called before it.  Layers may be attended on streams of
 their own (each keeps a workspace of 15 to 45 MB, and so does each graph).  (The prompt's own attention is the model's: its keys and
 values are in hand there.)"""
 import math
@@ -66,11 +66,19 @@ class PagedKVCache:
         return ops.rotary_paged_store(query_states, key_states, value_states, self.plan.positions, self.plan.slots, self.frequencies, self.keys[layer_idx],
                                       self.values[layer_idx], layout=self.layout, factor=self.factor, status=self.status)
 
-    def attend(self, query_states, layer_idx, scaling=None, return_lse=False):
-        """One token per request: rotated queries [requests, Hq, D] -> [requests, Hq, D] over the tokens that each request has (0 for one that has none)."""
+    def attend(self, query_states, layer_idx, scaling=None, return_lse=False, by_request=False):
+        """The step's rows as append returns them, at most one of a request: [tokens, Hq, D] -> [tokens, Hq, D], each over the tokens that its request has.  Rows behind the last
+        are 0 (a captured step has as many as there are requests, whatever they bring), and so are those of a request that brought more than one (reported: check).
+        by_request, or as many rows as requests where the step had another number: row b is request b's, whatever it brought; 0 for one without tokens."""
+        rows, starts = query_states.shape[0], None
+        if not by_request and self.plan is not None and rows == self.plan.slots.shape[0]:
+            if rows > self.requests:
+                raise KvcError("attend: one token per request, got %d rows of %d requests" % (rows, self.requests))
+            starts = self.plan.starts
         workspace = self._workspace(query_states.shape[1])
         return ops.paged_attn(query_states, self.keys[layer_idx], self.values[layer_idx], self.table, self.lengths,
-                              1.0 / math.sqrt(self.head_dim) if scaling is None else scaling, window=self.window, return_lse=return_lse, workspace=workspace, status=self.status)
+                              1.0 / math.sqrt(self.head_dim) if scaling is None else scaling, window=self.window, return_lse=return_lse, workspace=workspace, status=self.status,
+                              starts=starts)
 
     def _workspace(self, heads):
         """The attention's workspace, cleared, for the current stream: calls on streams of their own may run at once.  A capture has its own too, cleared by the

@@ -21,6 +21,7 @@ decltype(&kvc_page_plan) page_plan = nullptr;
 decltype(&kvc_page_release) page_release = nullptr;
 decltype(&kvc_rotary_store) rotary_store = nullptr;
 decltype(&kvc_paged_attn) paged_attn = nullptr;
+decltype(&kvc_paged_attn_rows) paged_attn_rows = nullptr;
 decltype(&kvc_last_error) last_error = nullptr;
 
 [[noreturn]] void fail(const std::string &why) {
@@ -98,14 +99,14 @@ Table table_of(PyObject *o, int64_t B, int device) {
 int32_t *status_of(PyObject *o, int device) { return given(o) ? static_cast<int32_t *>(words(o, 1, "status", device)) : nullptr; }
 
 // the call on the device's current stream, other threads running meanwhile (a full queue makes a launch wait)
-template <typename Args>
-void launch(int (*call)(const Args *, kvc_stream_t), const Args &args, int device, const char *name) {
+template <typename Call, typename Args, typename... More>
+void launch(Call *call, const Args &args, int device, const char *name, More... more) {
     if (!call) fail("kvc_torch: init() has not been called");
     const c10::cuda::OptionalCUDAGuard guard(c10::Device(c10::kCUDA, static_cast<c10::DeviceIndex>(device)));
     const kvc_stream_t stream = c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(device)).stream();
     int rc;
     Py_BEGIN_ALLOW_THREADS
-    rc = call(&args, stream);
+    rc = call(&args, more..., stream);
     Py_END_ALLOW_THREADS
     if (rc != KVC_OK) fail(std::string(name) + " failed (code " + std::to_string(rc) + "): " + last_error());
 }
@@ -259,10 +260,10 @@ PyObject *py_rotary_store(PyObject *, PyObject *const *args, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-// q, kpages, vpages, table, lengths, scaling, window, out or None, return_lse, workspace, status
+// q, kpages, vpages, table, lengths, scaling, window, out or None, return_lse, workspace, status, starts or None
 PyObject *py_paged_attn(PyObject *, PyObject *const *args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    count(n, 11);
+    count(n, 12);
     const at::Tensor &q0 = tensor(args[0], "q"), &pool = tensor(args[1], "kpages");
     const int device = device_of(q0, "q");
     kvc_paged_attn_args a = {};
@@ -271,7 +272,10 @@ PyObject *py_paged_attn(PyObject *, PyObject *const *args, Py_ssize_t n) {
     if (q0.dim() != 3 || pool.dim() != 4 || pool.size(3) != q0.size(2))
         fail("q must be [B, Hq, D], the pools [pages, page_size, Hkv, D], got " + shape_of(q0.sizes()) + " and " + shape_of(pool.sizes()));
     const at::Tensor &q = rows(args[0], q0.sizes(), type, "q", device), &kp = rows(args[1], pool.sizes(), type, "kpages", device), &vp = rows(args[2], pool.sizes(), type, "vpages", device);
-    a.B = q.size(0); a.Hq = q.size(1); a.D = q.size(2);
+    const bool by_row = given(args[11]);
+    const at::Tensor &lengths = tensor(args[4], "lengths");
+    a.B = !by_row ? q.size(0) : lengths.dim() == 1 ? lengths.size(0) : -1;
+    a.Hq = q.size(1); a.D = q.size(2);
     a.n_pages = pool.size(0); a.page_size = pool.size(1); a.Hkv = pool.size(2);
     a.q = q.data_ptr(); a.q_token = q.stride(0); a.q_head = q.stride(1);
     a.kpages = kp.data_ptr(); a.kp_page = kp.stride(0); a.kp_row = kp.stride(1); a.kp_head = kp.stride(2);
@@ -290,10 +294,11 @@ PyObject *py_paged_attn(PyObject *, PyObject *const *args, Py_ssize_t n) {
     a.out = out.data_ptr(); a.out_token = out.stride(0); a.out_head = out.stride(1);
     at::Tensor lse;
     if (PyObject_IsTrue(args[8])) {
-        lse = at::empty({a.B, a.Hq}, q.options().dtype(at::kFloat));
+        lse = at::empty({q.size(0), a.Hq}, q.options().dtype(at::kFloat));
         a.lse = static_cast<float *>(lse.data_ptr());
     }
-    launch(paged_attn, a, device, "kvc_paged_attn");
+    if (by_row) launch(paged_attn_rows, a, device, "kvc_paged_attn_rows", static_cast<const int32_t *>(words(args[11], a.B + 1, "starts", device)), q.size(0));
+    else launch(paged_attn, a, device, "kvc_paged_attn");
     PyObject *const result = own ? THPVariable_Wrap(out) : Py_NewRef(args[7]);
     if (!lse.defined() || !result) return result;
     PyObject *const more = THPVariable_Wrap(lse);
@@ -320,14 +325,15 @@ PyObject *py_stream_of(PyObject *, PyObject *const *args, Py_ssize_t n) {
 // the error's class and the addresses of the library's entries
 PyObject *py_init(PyObject *, PyObject *const *args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    count(n, 6);
+    count(n, 7);
     error_class = Py_NewRef(args[0]);
     auto address = [&](int i) { return reinterpret_cast<void *>(static_cast<uintptr_t>(number(args[i]))); };
     page_plan = reinterpret_cast<decltype(page_plan)>(address(1));
     page_release = reinterpret_cast<decltype(page_release)>(address(2));
     rotary_store = reinterpret_cast<decltype(rotary_store)>(address(3));
     paged_attn = reinterpret_cast<decltype(paged_attn)>(address(4));
-    last_error = reinterpret_cast<decltype(last_error)>(address(5));
+    paged_attn_rows = reinterpret_cast<decltype(paged_attn_rows)>(address(5));
+    last_error = reinterpret_cast<decltype(last_error)>(address(6));
     Py_RETURN_NONE;
     END_HANDLE_TH_ERRORS
 }

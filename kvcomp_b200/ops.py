@@ -772,13 +772,15 @@ def paged_attn_workspace(B, Hq, Hkv, D, device):
     return workspace
 
 
-def paged_attn(q, kpages, vpages, table, lengths, scaling, window=0, out=None, return_lse=False, workspace=None, status=None):
+def paged_attn(q, kpages, vpages, table, lengths, scaling, window=0, out=None, return_lse=False, workspace=None, status=None, starts=None):
     """One new token per request: q fp16 or bf16 [B, Hq, D] -> out [B, Hq, D] = softmax(scaling * q . k) v over the lengths[b] (int32[B]) tokens that the
     request has in the pages table[b] (int32 [B, pages]) of the pools [pages, page_size, Hkv, D]; window > 0: over the last `window` of them.  Requests
     without tokens: 0.  return_lse: (out, fp32 [B, Hq] log of the sum of exponentials, -inf without tokens).  D: 64, 96, 128, 256.
-    workspace: paged_attn_workspace's, for one call at a time; None: one is made, and cleared, for this call."""
+    workspace: paged_attn_workspace's, for one call at a time; None: one is made, and cleared, for this call.
+    starts (int32[B + 1], a plan's): q and out have a row for each token of a step, request b's at starts[b]; requests without one are left out, rows that are nobody's
+    are 0, and so are those of a request that has more than one (FLAG_BAD_LENGTH)."""
     if workspace is None:
         if not isinstance(q, torch.Tensor) or not q.is_cuda or q.dim() != 3 or not isinstance(kpages, torch.Tensor) or kpages.dim() != 4:
             raise KvcError("q must be a CUDA tensor [B, Hq, D], the pools [pages, page_size, Hkv, D] (kvcomp_b200 has no CPU path)")
         workspace = paged_attn_workspace(q.shape[0], q.shape[1], kpages.shape[2], q.shape[2], q.device)
-    return _lib.torch_calls().paged_attn(q, kpages, vpages, table, lengths, scaling, window, out, return_lse, workspace, status)
+    return _lib.torch_calls().paged_attn(q, kpages, vpages, table, lengths, scaling, window, out, return_lse, workspace, status, starts)
