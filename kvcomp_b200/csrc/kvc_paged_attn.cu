@@ -20,7 +20,8 @@
 // heads, so that few heads waste little.  (tcgen05 wants 64 rows and its operands in shared memory behind barriers of the whole CTA; here the tensor
 // work is a few per cent of the time that the bytes need.)  P is split into two 16-bit pieces, hi + lo, and multiplied twice: the weights keep 21
 // (fp16) or 16 bits (bf16), and the result is rounded once, at the end.  fp16 weights are carried times 2^14, so that the pieces of weights down to 2^-28
-// of the largest are normal numbers and many small ones are not lost.
+// of the largest are normal numbers and many small ones are not lost.  Two pieces make no number of an infinite value (0 times it, or pieces of two signs), and neither does a
+// weight that is nothing in 32 bits: a column whose sums are no numbers although its weights are is looked at again (infinite_values).
 #include <math_constants.h>
 #include <string.h>
 
@@ -62,6 +63,7 @@ struct Params {
 template <typename T> struct Pair;
 template <> struct Pair<__half> {
     static constexpr float LIFT = 14.0f;
+    static constexpr uint32_t INFINITE = 0x7c00;
     static __device__ __forceinline__ uint32_t pack(float a, float b) { const __half2 r = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t *>(&r); }
     static __device__ __forceinline__ float2 unpack(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2 *>(&v)); }
     static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -71,6 +73,7 @@ template <> struct Pair<__half> {
 };
 template <> struct Pair<__nv_bfloat16> {
     static constexpr float LIFT = 0.0f;
+    static constexpr uint32_t INFINITE = 0x7f80;
     static __device__ __forceinline__ uint32_t pack(float a, float b) { const __nv_bfloat162 r = __floats2bfloat162_rn(a, b); return *reinterpret_cast<const uint32_t *>(&r); }
     static __device__ __forceinline__ float2 unpack(uint32_t v) { return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&v)); }
     static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -155,6 +158,75 @@ template <int TILE, bool ROWS> __device__ __forceinline__ void next_tile(const P
     at.span = {0, 0};
 }
 
+// The channels of query heads [h0, h0 + heads) of request b that came out as no numbers although their weights are some (`odd`: a bit for each such head), by the definition:
+// a value of +inf or -inf that counts makes the sum that, both, or one that is no number itself, or one of weight 0 (a score of -inf), none.  The CTA reads the column's values
+// again, 16 bytes a thread and eight of them at a time; `seen` (heads * D bytes of shared memory) has for each channel 1: +inf, 2: -inf.  All threads call it, behind a barrier.
+template <typename T, int D, bool ROWS>
+__device__ __noinline__ void infinite_values(const Params &p, int b, int row, int h0, int heads, unsigned odd, uint32_t *seen) {
+    constexpr uint32_t INFINITE = Pair<T>::INFINITE;
+    const kvc_paged_attn_args &a = p.a;
+    const int tid = threadIdx.x, g = (int)(a.Hq / a.Hkv), hk0 = h0 / g, kv_heads = (h0 + heads - 1) / g - hk0 + 1, pieces = kv_heads * (D / 8);
+    for (int i = tid; i < heads * (D / 4); i += THREADS) seen[i] = 0;
+    __syncthreads();
+    int unused = 0;
+    const Span span = span_of<ROWS>(p, b, unused);
+    const long long end = (long long)(span.len - span.first) * pieces;
+    auto at = [&](const void *pool, long long of_page, long long of_row, long long of_head, int page, int t, int hk) {
+        return reinterpret_cast<const T *>(pool) + page * of_page + (t - kvc_divide(t, p.page) * (int)a.page_size) * of_row + hk * of_head;
+    };
+    auto odd_pair = [](uint32_t v) { return (v & INFINITE) == INFINITE || (v >> 16 & INFINITE) == INFINITE; };
+    auto odd_piece = [&](const uint4 &v) { return odd_pair(v.x) || odd_pair(v.y) || odd_pair(v.z) || odd_pair(v.w); };
+    for (long long i0 = tid; i0 < end; i0 += 8 * THREADS) {
+        uint4 v[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            const long long i = i0 + k * THREADS;
+            v[k] = make_uint4(0, 0, 0, 0);
+            if (i < end) {
+                const int t = span.first + (int)(i / pieces), piece = (int)(i % pieces);
+                const int page = a.table[b * a.table_stride + kvc_divide(t, p.page)];
+                if ((unsigned)page < p.n_pages)
+                    v[k] = *reinterpret_cast<const uint4 *>(at(a.vpages, a.vp_page, a.vp_row, a.vp_head, page, t, hk0 + piece / (D / 8)) + piece % (D / 8) * 8);
+            }
+        }
+#pragma unroll 1
+        for (int k = 0; k < 8; k++) {
+            const uint4 mine = k == 0 ? v[0] : k == 1 ? v[1] : k == 2 ? v[2] : k == 3 ? v[3] : k == 4 ? v[4] : k == 5 ? v[5] : k == 6 ? v[6] : v[7];
+            if (!odd_piece(mine)) continue;
+            const long long i = i0 + k * THREADS;
+            const int t = span.first + (int)(i / pieces), piece = (int)(i % pieces), hk = hk0 + piece / (D / 8);
+            const T *const key = at(a.kpages, a.kp_page, a.kp_row, a.kp_head, a.table[b * a.table_stride + kvc_divide(t, p.page)], t, hk);
+            bool weighed = false;                           // whether a weight may be 0
+            for (int c = 0; c < D / 8 && !weighed; c++) weighed = odd_piece(*reinterpret_cast<const uint4 *>(key + c * 8));
+            for (int h = max(h0, hk * g); h < min(h0 + heads, (hk + 1) * g); h++) {
+                if (!(odd >> (h - h0) & 1)) continue;
+                bool none = false;
+                if (weighed && a.q == a.out) none = true;   // (the result is where the query was: no number stays none)
+                else if (weighed) {
+                    const T *const q = reinterpret_cast<const T *>(a.q) + row * a.q_token + h * a.q_head;
+                    float s = 0.0f;
+                    for (int c = 0; c < D; c++) s = fmaf((float)q[c], (float)key[c], s);
+                    none = (p.negative ? -s : s) == -CUDART_INF_F;
+                }
+                for (int c = 0; c < 8; c++) {
+                    const uint32_t pair = c < 2 ? mine.x : c < 4 ? mine.y : c < 6 ? mine.z : mine.w, x = pair >> c % 2 * 16 & 0xffff;
+                    if ((x & INFINITE) != INFINITE) continue;
+                    const uint32_t code = none || (x & 0x7fff) != INFINITE ? 3 : (x & 0x8000 ? 2 : 1);
+                    const int channel = (h - h0) * D + piece % (D / 8) * 8 + c;
+                    atomicOr(seen + channel / 4, code << channel % 4 * 8);
+                }
+            }
+        }
+    }
+    __syncthreads();
+    for (int i = tid; i < heads * D; i += THREADS) {
+        const uint32_t code = seen[i / 4] >> i % 4 * 8 & 3;
+        uint16_t *const out = reinterpret_cast<uint16_t *>(reinterpret_cast<T *>(a.out) + row * a.out_token + (h0 + i / D) * a.out_head + i % D);
+        if ((odd >> i / D & 1) && (code == 1 || code == 2) && (*out & 0x7fff) > INFINITE) *out = (uint16_t)(code == 1 ? INFINITE : INFINITE | 0x8000);
+    }
+    __syncthreads();
+}
+
 template <typename T, int D, int NT, int WH, bool SAME, int STAGES, int CTAS, bool ROWS>
 __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_constant__ Params p) {
     constexpr int KS = D / 16;                              // steps of 16 channels
@@ -169,9 +241,11 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
     __shared__ Place next_start_s[WARPS];
     __shared__ unsigned before_s[CTAS >= 3 ? DRAWN_REQUESTS : 1];           // tiles of a column in front of a request
     __shared__ int last_s, next_s;
+    __shared__ unsigned odd_s;                              // whether a thread has seen such a result (and which heads', while they are looked at)
     const kvc_paged_attn_args &a = p.a;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, B = (int)a.B;
     int flags = 0;
+    if (tid == 0) odd_s = 0;                                // (the first result is written behind a barrier)
 
     // ---- this CTA's share
     // Whole parts of columns, one for each CTA, where parts of up to 7 / 4 of an equal share do (few columns): no CTA has two to finish then, and fewer are joined; so many
@@ -530,7 +604,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
                             }
                         }
                     }
-                const int of_row = ROWS ? min(row_of<ROWS>(p, at.b), p.rows - 1) : at.b, of_h0 = WH > 1 ? at.c * WH * p.group : h0, of_heads = WH * heads, pieces = of_heads * (D / 4);      // of all its KV heads
+                const int of_b = at.b, of_row = ROWS ? min(row_of<ROWS>(p, at.b), p.rows - 1) : at.b, of_h0 = WH > 1 ? at.c * WH * p.group : h0, of_heads = WH * heads, pieces = of_heads * (D / 4);      // of all its KV heads
                 const bool whole = first_i == 0 && at.i == at.n - 1;        // the column lies in this share
                 const int begin = r0 + n - at.i;            // its first tile in the row of tiles
                 const int tiles = at.n, of_piece = piece, place = 2 * piece + (n - (at.i - first_i) > 0);
@@ -548,9 +622,11 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
                 if (n != share) begin_column();             // on their way while the sums are joined
                 clear();
                 __syncthreads();
+                unsigned odd = 0;                           // query heads whose result has channels that are no numbers although its weights are: a bit for each
                 auto write = [&](int i, float top, float sum, const float4 &v) {       // four channels of a result
                     const int h = of_h0 + i / (D / 4), d = i % (D / 4) * 4;
-                    const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
+                    const float f = sum == 0.0f ? 0.0f : 1.0f / sum, any = v.x + v.y + v.z + v.w;
+                    odd |= any != any && sum == sum ? 1u << (h - of_h0) : 0;
                     *reinterpret_cast<uint2 *>(reinterpret_cast<T *>(a.out) + of_row * a.out_token + h * a.out_head + d) =
                         make_uint2(Pair<T>::pack(v.x * f, v.y * f), Pair<T>::pack(v.z * f, v.w * f));
                     if (d == 0 && a.lse) a.lse[of_row * a.Hq + h] = sum == 0.0f ? -CUDART_INF_F : (top + log2f(sum) - LIFT) * 0.69314718055994531f;
@@ -579,6 +655,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
                         if (d == 0) __stcg(reinterpret_cast<float2 *>(part + WH * p.group * D) + sub + h, make_float2(top, sum));
                     }
                 }
+                if (odd) odd_s = 1;
                 __syncthreads();
                 if (!whole) {
                     const int w_first = even != 0.0f ? column_first : piece_of(begin), count = even != 0.0f ? parts : piece_of(begin + tiles - 1) - w_first + 1;
@@ -586,7 +663,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
                     const int first_place = 2 * w_first + (even == 0.0f && begin > start_of(w_first, unused));
                     float4 *const join_v = reinterpret_cast<float4 *>(smem + scratch);       // (the stage that held the sums)
                     float2 *const join_ml = reinterpret_cast<float2 *>(join_v + THREADS);
-                    static_assert(THREADS * 24 <= STAGE, "a stage has room for what is joined");
+                    static_assert(THREADS * 24 <= STAGE && MAX_GROUP * D <= STAGE, "a stage has room for what is joined, and for what infinite_values keeps");
                     // the results of every step-th of `many` pieces from w on become one: the column's, or one in the first of their places
                     auto join = [&](int w, int step, int many, bool final) {
                         const int per = min(pieces, THREADS), ways = THREADS / per, way = tid / per;
@@ -646,6 +723,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
                                 if (i % (D / 4) == 0) new_ml[h] = make_float2(top, sum);
                             }
                         }
+                        if (odd) odd_s = 1;
                         __syncthreads();
                         if (!final) {
                             if (tid < of_heads) __stcg(reinterpret_cast<float2 *>(p.parts + (long long)(w == w_first ? first_place : 2 * w) * p.part + WH * p.group * D) + tid, new_ml[tid]);
@@ -677,6 +755,15 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
                             if (is_last(p.counters + first_place, groups)) join(w_first, JOINED, groups, true);
                         }
                     }
+                }
+                if (odd_s) {                                // (of 256 requests of 64 tokens, a column of one tile, asking takes 0.5 of 17.6 us, 8 x 4096 84.6 with and without)
+                    __syncthreads();
+                    if (tid == 0) odd_s = 0;
+                    __syncthreads();
+                    if (odd) atomicOr(&odd_s, odd);
+                    __syncthreads();
+                    infinite_values<T, D, ROWS>(p, of_b, of_row, of_h0, of_heads, odd_s, reinterpret_cast<uint32_t *>(smem + scratch));
+                    if (tid == 0) odd_s = 0;
                 }
             } else {
                 at.i++;
