@@ -121,6 +121,15 @@ at::Tensor part(const at::Tensor &buffer, int64_t first, int64_t n) {
 }
 int32_t *int_at(const at::Tensor &t) { return static_cast<int32_t *>(t.data_ptr()); }
 
+// tensors of the caller's that a call has written: autograd refuses to go back through what it had kept of them
+void written(std::initializer_list<PyObject *> given_tensors) {
+    for (PyObject *o : given_tensors) {
+        if (!given(o)) continue;
+        const at::Tensor &t = THPVariable_Unpack(o);
+        if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+    }
+}
+
 PyObject *tuple(std::initializer_list<at::Tensor> parts) {
     PyObject *r = PyTuple_New(static_cast<Py_ssize_t>(parts.size()));
     if (!r) throw python_error();
@@ -156,6 +165,7 @@ PyObject *py_page_plan(PyObject *, PyObject *const *args, Py_ssize_t n) {
         int32_t **const to[6] = {&a.lengths_out, &a.head_out, &a.starts, &a.taken, &a.slots, &a.positions};
         for (int i = 0; i < 6; i++) *to[i] = static_cast<int32_t *>(words(PyTuple_GET_ITEM(args[7], i), sizes[i], names[i], device));
         launch(page_plan, a, device, "kvc_page_plan");
+        for (int i = 0; i < 6; i++) written({PyTuple_GET_ITEM(args[7], i)});
         result = Py_NewRef(Py_None);
     } else {
         const int64_t room = (a.tokens + 3) / 4 * 4;        // (slots and positions are written 16 bytes at a time)
@@ -166,6 +176,7 @@ PyObject *py_page_plan(PyObject *, PyObject *const *args, Py_ssize_t n) {
         launch(page_plan, a, device, "kvc_page_plan");
         result = tuple({out_lengths, head, starts, taken, slots, positions});
     }
+    written({args[2]});
     return result;
     END_HANDLE_TH_ERRORS
 }
@@ -193,11 +204,13 @@ PyObject *py_page_release(PyObject *, PyObject *const *args, Py_ssize_t n) {
         a.lengths_out = static_cast<int32_t *>(words(args[6], a.B, "out lengths", device));
         a.head_out = static_cast<int32_t *>(words(args[7], 1, "out head", device));
         launch(page_release, a, device, "kvc_page_release");
+        written({args[3], args[6], args[7]});
         return PyTuple_Pack(2, args[6], args[7]);
     }
     const at::Tensor out_lengths = part(all, a.B + 1, a.B), head = part(all, 2 * a.B + 1, 1);
     a.lengths_out = int_at(out_lengths); a.head_out = int_at(head);
     launch(page_release, a, device, "kvc_page_release");
+    written({args[3]});
     return tuple({out_lengths, head});
     END_HANDLE_TH_ERRORS
 }
@@ -244,6 +257,7 @@ PyObject *py_rotary_store(PyObject *, PyObject *const *args, Py_ssize_t n) {
     a.status = status_of(args[12], device);
     if (!has_q) {
         launch(rotary_store, a, device, "kvc_rotary_store");
+        written({args[6], args[7]});
         Py_RETURN_NONE;
     }
     const at::Tensor &q0 = tensor(args[0], q_name);
@@ -256,6 +270,7 @@ PyObject *py_rotary_store(PyObject *, PyObject *const *args, Py_ssize_t n) {
     const at::Tensor out = own ? at::empty(q.sizes(), q.options()) : rows(args[11], q.sizes(), type, "out", device);
     a.q_out = out.data_ptr(); a.out_token = out.stride(0); a.out_head = out.stride(1);
     launch(rotary_store, a, device, "kvc_rotary_store");
+    written({args[6], args[7], args[11]});
     return own ? THPVariable_Wrap(out) : Py_NewRef(args[11]);
     END_HANDLE_TH_ERRORS
 }
@@ -299,6 +314,7 @@ PyObject *py_paged_attn(PyObject *, PyObject *const *args, Py_ssize_t n) {
     }
     if (by_row) launch(paged_attn_rows, a, device, "kvc_paged_attn_rows", static_cast<const int32_t *>(words(args[11], a.B + 1, "starts", device)), q.size(0));
     else launch(paged_attn, a, device, "kvc_paged_attn");
+    written({args[7]});
     PyObject *const result = own ? THPVariable_Wrap(out) : Py_NewRef(args[7]);
     if (!lse.defined() || !result) return result;
     PyObject *const more = THPVariable_Wrap(lse);

@@ -743,17 +743,40 @@ def page_release(lengths, done, table, free, head, page_size, out=None, status=N
     return _lib.torch_calls().page_release(lengths, done, table, free, head, page_size, out_lengths, out_head, status)
 
 
+class _Rotary(torch.autograd.Function):
+    """The rotation is linear: a gradient goes back through the rotation the other way."""
+
+    @staticmethod
+    def forward(ctx, x, positions, frequencies, layout, factor, inverse):
+        ctx.save_for_backward(positions, frequencies)
+        ctx.form = layout, factor, inverse
+        return rotary(x, positions, frequencies, layout, factor, inverse)
+
+    @staticmethod
+    def backward(ctx, grad):
+        positions, frequencies = ctx.saved_tensors
+        layout, factor, inverse = ctx.form
+        grad = grad if grad.stride(-1) == 1 else grad.contiguous()
+        return rotary(grad, positions, frequencies, layout, factor, not inverse), None, None, None, None, None
+
+
 def rotary(x, positions, frequencies, layout="half", factor=1.0, inverse=False, out=None):
     """x fp16 or bf16 [N, H, D] rotated: the first 2 * len(frequencies) channels of each head in pairs by positions[n] * frequencies[i] (int32[N], float64),
     the others copied.  layout: "half" pairs channel i with i + half of the rotated ones, "interleaved" 2i with 2i + 1.  factor multiplies cos and
-    sin.  inverse turns back (the gradient of the rotation, too).  out may be x.  utils.rotary.frequencies gives the frequencies of the usual scalings."""
+    sin.  inverse turns back (the gradient of the rotation, too).  out may be x.  utils.rotary.frequencies gives the frequencies of the usual scalings.
+    Gradients go through it, to x; not through out."""
+    if isinstance(x, torch.Tensor) and x.requires_grad and torch.is_grad_enabled():
+        if out is not None:
+            raise KvcError("rotary: out carries no gradient, and x requires one")
+        return _Rotary.apply(x, positions, frequencies, layout, factor, inverse)
     return _lib.torch_calls().rotary_store(x, None, None, positions, None, frequencies, None, None, _LAYOUTS.get(layout), factor, inverse, out, None)
 
 
 def rotary_paged_store(q, k, v, positions, slots, frequencies, kpages, vpages, layout="half", factor=1.0, out=None, status=None):
     """A step's tokens: q [N, Hq, D] rotated (returned; out may be q, q may be None), k [N, Hkv, D] rotated into and v copied into the rows `slots`
     (int32[N], page * page_size + row; below 0: not stored) of the pools [pages, page_size, Hkv, D].  fp16 or bf16, any strides but a contiguous last
-    dimension.  positions, frequencies, layout, factor: as for rotary; frequencies None: nothing is rotated.  Tokens of one call have slots of their own."""
+    dimension.  positions, frequencies, layout, factor: as for rotary; frequencies None: nothing is rotated.  Tokens of one call have slots of their own.
+    For serving: no gradient goes through it."""
     if k is None:
         raise KvcError("k must be a tensor")
     return _lib.torch_calls().rotary_store(q, k, v, positions, slots, frequencies, kpages, vpages, _LAYOUTS.get(layout), factor, False, out, status)
@@ -776,7 +799,7 @@ def paged_attn(q, kpages, vpages, table, lengths, scaling, window=0, out=None, r
     """One new token per request: q fp16 or bf16 [B, Hq, D] -> out [B, Hq, D] = softmax(scaling * q . k) v over the lengths[b] (int32[B]) tokens that the
     request has in the pages table[b] (int32 [B, pages]) of the pools [pages, page_size, Hkv, D]; window > 0: over the last `window` of them.  Requests
     without tokens: 0.  return_lse: (out, fp32 [B, Hq] log of the sum of exponentials, -inf without tokens).  D: 64, 96, 128, 256.
-    workspace: paged_attn_workspace's, for one call at a time; None: one is made, and cleared, for this call.
+    workspace: paged_attn_workspace's, for one call at a time; None: one is made, and cleared, for this call.  For serving: no gradient goes through it.
     starts (int32[B + 1], a plan's): q and out have a row for each token of a step, request b's at starts[b]; requests without one are left out, rows that are nobody's
     are 0, and so are those of a request that has more than one (FLAG_BAD_LENGTH)."""
     if workspace is None:
