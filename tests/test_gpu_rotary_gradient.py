@@ -77,3 +77,24 @@ def test_versions(ops):  # noqa: F811
         ops.rotary(x, pos, f, out=kept)
         ops.rotary(x, pos, f, out=out)
     ops.rotary(x, pos, f, out=kept)
+
+
+def test_captured(ops):  # noqa: F811
+    """Forward and backward in a graph.  (No eager graph of the same leaf may live then: torch gives up such a capture of any operator, since it keeps the leaf's node on
+    the stream that it was made on.)"""
+    pos, f = dev([9, 40, 2]), freqs(32).cuda()
+    x, g = (torch.randn(3, 2, 64, device="cuda").half() for _ in range(2))
+    x.requires_grad_()
+    torch.autograd.grad(ops.rotary(x, pos, f), x, g)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = ops.rotary(x, pos, f)
+        (gx,) = torch.autograd.grad(y, x, g)
+    for _ in range(3):
+        with torch.no_grad():
+            x.copy_(torch.randn_like(x)), g.copy_(torch.randn_like(g))
+        pos += 5
+        graph.replay()
+        with torch.no_grad():
+            assert torch.equal(y, ops.rotary(x, pos, f)) and torch.equal(gx, ops.rotary(g, pos, f, inverse=True))
