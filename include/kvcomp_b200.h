@@ -427,7 +427,8 @@ int kvc_page_release(const kvc_page_release_args *args, kvc_stream_t stream);
  *   q [N, Hq, D] -> q_out, which may be q; Hq = 0: none.
  *   k, v [N, Hkv, D] -> the rows `slots` of the pools, k rotated and v not; Hkv = 0: none.  A slot below 0 is not stored, one
  *   behind the pool raises KVC_FLAG_BAD_PAGE and is not stored.  Of two tokens with one slot either may be what stays.
- * Strides count elements; channels are next to each other.  frequencies: rotary / 2 of them. */
+ * Strides count elements; channels are next to each other.  frequencies: rotary / 2 of them.  Rows that are written must not overlap: those of q_out or of a pool one another, q_out
+ * what is read (q itself may be it), one pool the other (unless both get the same: v is k and rotary 0). */
 #define KVC_ROTARY_HALF 0
 #define KVC_ROTARY_INTERLEAVED 1
 typedef struct {
@@ -447,7 +448,7 @@ int kvc_rotary_store(const kvc_rotary_args *args, kvc_stream_t stream);
 /* One new token per request over its pages: with s_t = scaling * (q . k_t) over the tokens t < lengths[b] (with window > 0 only the last
  * `window` of them), out = sum exp(s_t) v_t / sum exp(s_t) and lse = log sum exp(s_t) (fp32 [B, Hq], may be null).  No
  * tokens: out = 0, lse = -inf.  q, out: [B, Hq, D], D 64, 96, 128 or 256, query head h reads KV head h / (Hq / Hkv).  Rows of q and of the
- * pools start on 16 bytes (pointers and strides).  Tokens behind a length are never read.
+ * pools start on 16 bytes (pointers and strides).  Rows of out must not overlap one another, nor q's unless out is q.  Tokens behind a length are never read.
  * workspace: kvc_paged_attn_workspace() bytes, 16-byte aligned, the first kvc_paged_attn_cleared() of them zeroed once before the first use; every call
  * leaves these at zero, for calls of any shape.  A workspace serves one launch at a time: concurrent streams need their own. */
 typedef struct {

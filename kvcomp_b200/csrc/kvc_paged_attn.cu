@@ -882,6 +882,9 @@ static int paged_attn(const kvc_paged_attn_args *args, const int32_t *starts, in
         kvc_set_error("kvc_paged_attn: the workspace must hold what kvc_paged_attn_workspace says");
         return KVC_ERR_CAPACITY;
     }
+    const kvc_rows q = kvc_make_rows(a.q, a.D, rows, a.q_token, a.Hq, a.q_head), out = kvc_make_rows(a.out, a.D, rows, a.out_token, a.Hq, a.out_head);
+    KVC_REQUIRE(out.apart, "kvc_paged_attn: rows of the output overlap");
+    KVC_REQUIRE(kvc_rows_equal(q, out) || !kvc_rows_overlap(q, out), "kvc_paged_attn: the output overlaps the queries and is not them");
     Params p;
     p.a = a;
     p.page = kvc_make_div((uint32_t)a.page_size);

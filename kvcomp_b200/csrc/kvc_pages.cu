@@ -483,6 +483,16 @@ extern "C" int kvc_rotary_store(const kvc_rotary_args *args, kvc_stream_t stream
     if (a.N == 1 || a.Hkv == 0) a.k_token = a.v_token = 0;
     if (a.page_size <= 1 || a.Hkv == 0) a.kp_row = a.vp_row = 0;
     if (a.n_pages <= 1 || a.Hkv == 0) a.kp_page = a.vp_page = 0;
+    // What is written in no order must not overlap: rows of the results or of a pool each other, a result what another thread reads.
+    const kvc_rows q = kvc_make_rows(a.q, a.D, a.N, a.q_token, a.Hq, a.q_head), out = kvc_make_rows(a.q_out, a.D, a.N, a.out_token, a.Hq, a.out_head);
+    const kvc_rows k = kvc_make_rows(a.k, a.D, a.N, a.k_token, a.Hkv, a.k_head), v = kvc_make_rows(a.v, a.D, a.N, a.v_token, a.Hkv, a.v_head);
+    const kvc_rows kp = kvc_make_rows(a.kpages, a.D, a.n_pages, a.kp_page, a.page_size, a.kp_row, a.Hkv, a.kp_head);
+    const kvc_rows vp = kvc_make_rows(a.vpages, a.D, a.n_pages, a.vp_page, a.page_size, a.vp_row, a.Hkv, a.vp_head);
+    KVC_REQUIRE(a.Hq == 0 || out.apart, "kvc_rotary_store: rows of the output overlap");
+    KVC_REQUIRE(a.Hq == 0 || kvc_rows_equal(q, out) || !kvc_rows_overlap(q, out), "kvc_rotary_store: the output overlaps the queries and is not them");
+    KVC_REQUIRE(a.Hq == 0 || a.Hkv == 0 || !(kvc_rows_overlap(k, out) || kvc_rows_overlap(v, out)), "kvc_rotary_store: the output overlaps the keys or the values");
+    KVC_REQUIRE(a.Hkv == 0 || (kp.apart && vp.apart), "kvc_rotary_store: rows of a pool overlap");
+    KVC_REQUIRE(a.Hkv == 0 || !kvc_rows_overlap(kp, vp) || (a.rotary == 0 && kvc_rows_equal(kp, vp) && kvc_rows_equal(k, v)), "kvc_rotary_store: the pools overlap");
     const uintptr_t at = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.q_out) | reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) |
                          reinterpret_cast<uintptr_t>(a.kpages) | reinterpret_cast<uintptr_t>(a.vpages);
     const int64_t strides = a.q_token | a.q_head | a.k_token | a.k_head | a.v_token | a.v_head | a.out_token | a.out_head | a.kp_page | a.kp_row | a.kp_head | a.vp_page | a.vp_row | a.vp_head;

@@ -776,7 +776,7 @@ def rotary_paged_store(q, k, v, positions, slots, frequencies, kpages, vpages, l
     """A step's tokens: q [N, Hq, D] rotated (returned; out may be q, q may be None), k [N, Hkv, D] rotated into and v copied into the rows `slots`
     (int32[N], page * page_size + row; below 0: not stored) of the pools [pages, page_size, Hkv, D].  fp16 or bf16, any strides but a contiguous last
     dimension.  positions, frequencies, layout, factor: as for rotary; frequencies None: nothing is rotated.  Tokens of one call have slots of their own.
-    For serving: no gradient goes through it."""
+    Outputs and pools must not overlap (views of one tensor that lie in one another are fine).  For serving: no gradient goes through it."""
     if k is None:
         raise KvcError("k must be a tensor")
     return _lib.torch_calls().rotary_store(q, k, v, positions, slots, frequencies, kpages, vpages, _LAYOUTS.get(layout), factor, False, out, status)
