@@ -23,11 +23,14 @@ from .._lib import KvcError
 class PagedKVCache:
     def __init__(self, requests, pages, layer_num, kv_heads, head_dim, page_size=64, max_tokens=None, dtype=torch.float16, device="cuda",
                  frequencies=None, layout="half", factor=1.0, window=0):
-        """A pool of `pages` pages of `page_size` tokens for `requests` requests of up to max_tokens tokens each (all of the pool where it is not given).
+        """A pool of `pages` pages of `page_size` tokens for `requests` requests of up to max_tokens tokens each (all of the pool where it is not given).  head_dim: 64, 96, 128 or
+        256, what the attention takes (ops.rotary_paged_store alone takes any).
         frequencies, layout, factor: the rotation (utils.rotary.frequencies; None: keys and queries come rotated).  window > 0: attention over the
         last `window` tokens."""
         if min(requests, pages, layer_num, kv_heads, head_dim, page_size) <= 0:
             raise KvcError("PagedKVCache: sizes must be positive")
+        if head_dim not in ops.PAGED_HEADS:
+            raise KvcError("PagedKVCache: heads of 64, 96, 128 or 256 channels, got %d" % head_dim)
         if dtype not in (torch.float16, torch.bfloat16):
             raise KvcError("PagedKVCache: fp16 or bf16, got %s" % dtype)
         device = torch.empty(0, device=device).device

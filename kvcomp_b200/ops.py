@@ -712,6 +712,7 @@ def k_matvec(k, q, out):
 # below waits or asks the device for anything, and each can be captured into a graph.  A decode step makes three of these calls a layer: tensors
 # are checked, results made and arguments packed by csrc/kvc_torch.cpp.
 
+PAGED_HEADS = (64, 96, 128, 256)                # channels that paged_attn takes
 _LAYOUTS = {"half": _lib.ROTARY_HALF, "interleaved": _lib.ROTARY_INTERLEAVED}
 
 
