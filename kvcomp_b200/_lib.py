@@ -137,7 +137,7 @@ def load():
     if not path:
         path = _build.LIB
         if _build.is_stale():
-            path = _build.build()
+            path = _build.build(binding=False)
     if not os.path.exists(path):
         raise KvcError("libkvcomp_b200.so is missing and could not be built; there is no CPU fallback")
     lib = C.CDLL(path)

@@ -1,12 +1,13 @@
 """Compile kvcomp_b200/csrc/*.cu into kvcomp_b200/lib/libkvcomp_b200.so for sm_100a, and kvcomp_b200/csrc/kvc_torch.cpp, the paged cache's calls for torch, into
-kvcomp_b200/lib/kvc_torch.so.
+kvcomp_b200/lib/kvc_torch.<torch's version, Python's tag, ABI>.so.
 
-    python -m kvcomp_b200.build [--force] [--verbose]
+    python -m kvcomp_b200.build [--force] [--verbose] [--library]          # --library: the library alone, which needs no torch
 
 nvcc cross-compiles without a GPU.  The library is kept in-tree so that it ships with the
 source snapshot; it is rebuilt when any source is newer than it.
 """
 import glob
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -17,7 +18,6 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB_DIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIB_DIR, "libkvcomp_b200.so")
-BINDING = os.path.join(LIB_DIR, "kvc_torch.so")
 BINDING_SOURCE = os.path.join(CSRC, "kvc_torch.cpp")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 
@@ -40,10 +40,17 @@ def is_stale():
     return any(os.path.getmtime(f) > t for f in _deps())
 
 
+def binding_path():
+    """Where the binding for this torch and this Python lies: it is compiled against the classes of the one and the headers of the other."""
+    import torch
+    return os.path.join(LIB_DIR, "kvc_torch.%s.%s.abi%d.so" % (torch.__version__, sysconfig.get_config_var("SOABI"), torch._C._GLIBCXX_USE_CXX11_ABI))
+
+
 def binding_is_stale():
-    if not os.path.exists(BINDING):
+    path = binding_path()
+    if not os.path.exists(path):
         return True
-    t = os.path.getmtime(BINDING)
+    t = os.path.getmtime(path)
     return any(os.path.getmtime(f) > t for f in [BINDING_SOURCE] + glob.glob(os.path.join(INCLUDE, "*.h")))
 
 
@@ -60,20 +67,21 @@ def _run(cmd, to, verbose):
 
 
 def build_binding(force=False, verbose=False):
-    if not force and not binding_is_stale():
-        return BINDING
     import torch
+    path = binding_path()
+    if not force and not binding_is_stale():
+        return path
     root = os.path.dirname(torch.__file__)
     cuda = os.path.join(os.path.dirname(os.path.dirname(nvcc_path())), "include")
     os.makedirs(LIB_DIR, exist_ok=True)
     compiler = shutil.which(os.environ.get("CXX", "g++"))
     if not compiler:
-        raise RuntimeError("no C++ compiler found; kvc_torch.so cannot be built")
+        raise RuntimeError("no C++ compiler found; kvc_torch cannot be built")
     cmd = [compiler, "-std=c++17", "-O2", "-shared", "-fPIC", "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI]
     for d in (os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"), cuda, sysconfig.get_paths()["include"]):
         cmd += ["-isystem", d]
     cmd += [BINDING_SOURCE, "-L" + os.path.join(root, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
-    return _run(cmd, BINDING, verbose)
+    return _run(cmd, path, verbose)
 
 
 def nvcc_path():
@@ -83,14 +91,18 @@ def nvcc_path():
     raise RuntimeError("nvcc not found; libkvcomp_b200.so cannot be built")
 
 
-def build(force=False, verbose=False):
-    """The library, and the binding where it is stale too."""
-    build_binding(force, verbose)
-    if not force and not is_stale():
-        return LIB
-    os.makedirs(LIB_DIR, exist_ok=True)
-    return _run([nvcc_path()] + NVCC_FLAGS + (["-Xptxas", "-v"] if verbose else []) + sources(), LIB, verbose)
+def build(force=False, verbose=False, binding=True):
+    """The library, and then the binding where there is torch to bind to.  Each is left as it is where nothing is newer."""
+    if force or is_stale():
+        os.makedirs(LIB_DIR, exist_ok=True)
+        _run([nvcc_path()] + NVCC_FLAGS + (["-Xptxas", "-v"] if verbose else []) + sources(), LIB, verbose)
+    if binding:
+        if importlib.util.find_spec("torch") is not None:
+            build_binding(force, verbose)
+        else:
+            sys.stderr.write("no torch here: kvc_torch, through which kvcomp_b200.ops makes the paged cache's calls, is not built\n")
+    return LIB
 
 
 if __name__ == "__main__":
-    print(build(force="--force" in sys.argv, verbose="--verbose" in sys.argv))
+    print(build(force="--force" in sys.argv, verbose="--verbose" in sys.argv, binding="--library" not in sys.argv))
