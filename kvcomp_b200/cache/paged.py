@@ -51,7 +51,11 @@ class PagedKVCache:
         self._workspaces = {}
 
     def __getstate__(self):
-        return dict(self.__dict__, _workspaces={})                   # (a copy makes its own)
+        return {name: value for name, value in self.__dict__.items() if name != "_workspaces"}                           # (a copy makes its own)
+
+    def __setstate__(self, state):
+        self.__dict__.update(state, _workspaces={})
+        self.__dict__.pop("_workspace", None)                        # (what it was once kept under)
 
     def begin(self, new, tokens):
         """A step that brings new[b] tokens (int32[requests], on the device) of each request, `tokens` rows in all.  Returns the plan (ops.PagePlan):

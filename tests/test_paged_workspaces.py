@@ -64,3 +64,12 @@ def test_copies_make_their_own(attend):
     mine = attend(0)
     other = copy.copy(attend.cache)
     assert attend(0, cache=other) != mine and attend(0) == mine
+
+
+def test_states_of_older_caches(attend):
+    """One that was pickled with its workspaces, under the name that they had."""
+    state = dict(vars(attend.cache), _workspace={4: "workspace of another process"})
+    del state["_workspaces"]
+    other = object.__new__(PagedKVCache)
+    other.__setstate__(state)
+    assert attend(0, cache=other) == "workspace 1"
