@@ -51,12 +51,12 @@ CACHE_FIELDS = "7q2i4q2i"
 KV_STORE_ARGS = struct.Struct("<11q")
 ATTN_ARGS = struct.Struct("<" + 2 * CACHE_FIELDS + "12qfi")
 STORE_ARGS = struct.Struct("<29q6ifi")
+# (ops makes these calls through csrc/kvc_torch.cpp; for callers of the library by ctypes)
 PAGE_PLAN_ARGS = struct.Struct("<18q")
 PAGE_RELEASE_ARGS = struct.Struct("<14q")
 ROTARY_ARGS = struct.Struct("<31q3if")
 PAGED_ATTN_ARGS = struct.Struct("<29qfi")
 
-TYPE_FP16, TYPE_BF16 = 0, 1
 ROTARY_HALF, ROTARY_INTERLEAVED = 0, 1
 
 

@@ -5,7 +5,9 @@
 
 #include "kvc_common.cuh"
 
-struct kvc_div { uint32_t magic, shift; };      // n / d by a divisor that the host knows, 0 <= n < 2^31, 1 <= d <= 2^31
+// n / d by a divisor that the host knows, 0 <= n < 2^31, 1 <= d <= 2^31: a product's high word, a sum and a shift (Granlund and Montgomery, Division by Invariant Integers using
+// Multiplication, 1994)
+struct kvc_div { uint32_t magic, shift; };
 
 static inline kvc_div kvc_make_div(uint32_t d) {
     kvc_div r;

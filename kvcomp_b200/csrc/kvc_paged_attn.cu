@@ -132,7 +132,7 @@ template <bool ROWS> __device__ __forceinline__ Span span_of(const Params &p, in
 template <int TILE> __device__ __forceinline__ int tiles_of(const Span &s) { return (s.len - s.first + TILE - 1) / TILE; }
 
 // n / d of numbers that are not negative, through a float that some steps put right (16 of them: it is off by 3 2^-24, and quotients are below 2^26).  Lengths are read more
-// than once: should a caller change them meanwhile, d may be 0 and results are anything, but every loop ends and nothing outside the arguments' tensors is touched.
+// than once and must not change while the kernel runs: its warps would take different numbers of turns between the CTA's barriers.
 __device__ __forceinline__ int quotient(int n, int d) {
     if (d <= 0) return 0;
     int q = (int)((float)n * __frcp_rn((float)d));

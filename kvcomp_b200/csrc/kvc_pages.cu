@@ -253,7 +253,7 @@ __device__ __forceinline__ uint32_t pack(float a, float b, __nv_bfloat16) { cons
 
 // cos and sin of a position, given the turns of one step.  The turns are counted in fp64: what is left of a far position's angle after its whole
 // turns keeps 2^-53 of the angle, 1e-10 at a million radians; fp32 would keep 0.06.  Of the rest the nearest quarter is taken off, and the series of sine and cosine on
-// [-pi / 4, pi / 4] are left, to the terms below 2^-31.
+// [-pi / 4, pi / 4] are left, to x^9 and x^10: the first terms left out are below 2^-29 and 2^-33 (fp32's half step there: 2^-25).
 constexpr double TURNS_OF_RADIANS = 0.15915494309189533576888;
 __device__ __forceinline__ float2 turn(double position, double turns, float factor) {
     double whole = position * turns;
