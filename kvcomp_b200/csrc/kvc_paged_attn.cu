@@ -160,69 +160,86 @@ template <int TILE, bool ROWS> __device__ __forceinline__ void next_tile(const P
 
 // The channels of query heads [h0, h0 + heads) of request b that came out as no numbers although their weights are some (`odd`: a bit for each such head), by the definition:
 // a value of +inf or -inf that counts makes the sum that, both, or one that is no number itself, or one of weight 0 (a score of -inf), none.  The CTA reads the column's values
-// again, 16 bytes a thread and eight of them at a time; `seen` (heads * D bytes of shared memory) has for each channel 1: +inf, 2: -inf.  All threads call it, behind a barrier.
+// again, of the 16-byte pieces that hold such a channel, eight at a time a thread; `seen` (heads * D bytes of shared memory and a word) has for each channel 1: +inf, 2: -inf.  All
+// threads call it, behind a barrier.  (One infinity among 131072 tokens of 8 KV heads: a call of 90 us takes 1200; 8 x 4096 of 32
+// heads, one for each, 87 and 123; values that are all no numbers 140 and 133.)
 template <typename T, int D, bool ROWS>
 __device__ __noinline__ void infinite_values(const Params &p, int b, int row, int h0, int heads, unsigned odd, uint32_t *seen) {
     constexpr uint32_t INFINITE = Pair<T>::INFINITE;
     const kvc_paged_attn_args &a = p.a;
-    const int tid = threadIdx.x, g = (int)(a.Hq / a.Hkv), hk0 = h0 / g, kv_heads = (h0 + heads - 1) / g - hk0 + 1, pieces = kv_heads * (D / 8);
-    for (int i = tid; i < heads * (D / 4); i += THREADS) seen[i] = 0;
+    const int tid = threadIdx.x, g = (int)(a.Hq / a.Hkv), hk0 = h0 / g;
+    uint32_t *const pieces_s = seen + heads * (D / 4);      // a bit for each piece of the KV heads' rows (32 at most)
+    auto result = [&](int i) { return reinterpret_cast<uint16_t *>(reinterpret_cast<T *>(a.out) + row * a.out_token + (h0 + i / D) * a.out_head + i % D); };
+    auto no_number = [&](int i) { return (odd >> i / D & 1) && (*result(i) & 0x7fff) > INFINITE; };
+    for (int i = tid; i <= heads * (D / 4); i += THREADS) seen[i] = 0;
     __syncthreads();
+    for (int i = tid; i < heads * D; i += THREADS)
+        if (no_number(i)) atomicOr(pieces_s, 1u << (((h0 + i / D) / g - hk0) * (D / 8) + i % D / 8));
+    __syncthreads();
+    const unsigned pieces = *pieces_s;
+    if (pieces == 0) return;                                // (infinities of two signs in one thread's channels)
+    const int many = max(__popc(pieces), 1), ways = THREADS / many, way = tid / many;
+    int piece = 0;
+    for (int left = tid % many; piece < 31 && !((pieces >> piece & 1) && left-- == 0); piece++) {}
+    const int hk = hk0 + piece / (D / 8), channel = piece % (D / 8) * 8, from = max(h0, hk * g), to = min(h0 + heads, (hk + 1) * g);
     int unused = 0;
     const Span span = span_of<ROWS>(p, b, unused);
-    const long long end = (long long)(span.len - span.first) * pieces;
-    auto at = [&](const void *pool, long long of_page, long long of_row, long long of_head, int page, int t, int hk) {
+    auto page_of = [&](int t) { return a.table[b * a.table_stride + kvc_divide(t, p.page)]; };
+    auto row_at = [&](const void *pool, long long of_page, long long of_row, long long of_head, int page, int t) {
         return reinterpret_cast<const T *>(pool) + page * of_page + (t - kvc_divide(t, p.page) * (int)a.page_size) * of_row + hk * of_head;
     };
     auto odd_pair = [](uint32_t v) { return (v & INFINITE) == INFINITE || (v >> 16 & INFINITE) == INFINITE; };
     auto odd_piece = [&](const uint4 &v) { return odd_pair(v.x) || odd_pair(v.y) || odd_pair(v.z) || odd_pair(v.w); };
-    for (long long i0 = tid; i0 < end; i0 += 8 * THREADS) {
+    uint32_t plus = 0, minus = 0;                           // this thread's channels, a bit for each; none: both
+    auto keep = [&](int h, uint32_t up, uint32_t down) {
+        for (int c = 0; c < 8; c++) {
+            const uint32_t code = (up >> c & 1) | (down >> c & 1) << 1;
+            if (code) atomicOr(seen + ((h - h0) * D + channel + c) / 4, code << c % 4 * 8);
+        }
+    };
+#pragma unroll 1
+    for (long long t0 = span.first + way; way < ways && t0 < span.len && (plus & minus) != 0xff; t0 += 8 * ways) {
         uint4 v[8];
 #pragma unroll
         for (int k = 0; k < 8; k++) {
-            const long long i = i0 + k * THREADS;
-            v[k] = make_uint4(0, 0, 0, 0);
-            if (i < end) {
-                const int t = span.first + (int)(i / pieces), piece = (int)(i % pieces);
-                const int page = a.table[b * a.table_stride + kvc_divide(t, p.page)];
-                if ((unsigned)page < p.n_pages)
-                    v[k] = *reinterpret_cast<const uint4 *>(at(a.vpages, a.vp_page, a.vp_row, a.vp_head, page, t, hk0 + piece / (D / 8)) + piece % (D / 8) * 8);
-            }
+            const long long t = t0 + k * ways;
+            const int page = t < span.len ? page_of((int)t) : -1;
+            v[k] = (unsigned)page < p.n_pages ? *reinterpret_cast<const uint4 *>(row_at(a.vpages, a.vp_page, a.vp_row, a.vp_head, page, (int)t) + channel) : make_uint4(0, 0, 0, 0);
         }
-#pragma unroll 1
+#pragma unroll
         for (int k = 0; k < 8; k++) {
-            const uint4 mine = k == 0 ? v[0] : k == 1 ? v[1] : k == 2 ? v[2] : k == 3 ? v[3] : k == 4 ? v[4] : k == 5 ? v[5] : k == 6 ? v[6] : v[7];
-            if (!odd_piece(mine)) continue;
-            const long long i = i0 + k * THREADS;
-            const int t = span.first + (int)(i / pieces), piece = (int)(i % pieces), hk = hk0 + piece / (D / 8);
-            const T *const key = at(a.kpages, a.kp_page, a.kp_row, a.kp_head, a.table[b * a.table_stride + kvc_divide(t, p.page)], t, hk);
-            bool weighed = false;                           // whether a weight may be 0
+            if (!odd_piece(v[k])) continue;
+            const int t = (int)(t0 + k * ways);
+            uint32_t up = 0, down = 0;
+            for (int c = 0; c < 8; c++) {
+                const uint32_t pair = c < 2 ? v[k].x : c < 4 ? v[k].y : c < 6 ? v[k].z : v[k].w, x = pair >> c % 2 * 16 & 0xffff;
+                if ((x & INFINITE) != INFINITE) continue;
+                const bool number = (x & 0x7fff) == INFINITE;
+                up |= (!number || !(x & 0x8000)) << c;
+                down |= (!number || (x & 0x8000)) << c;
+            }
+            plus |= up;
+            minus |= down;
+            const T *const key = row_at(a.kpages, a.kp_page, a.kp_row, a.kp_head, page_of(t), t);
+            bool weighed = false;                           // whether the weight may be 0
             for (int c = 0; c < D / 8 && !weighed; c++) weighed = odd_piece(*reinterpret_cast<const uint4 *>(key + c * 8));
-            for (int h = max(h0, hk * g); h < min(h0 + heads, (hk + 1) * g); h++) {
-                if (!(odd >> (h - h0) & 1)) continue;
-                bool none = false;
-                if (weighed && a.q == a.out) none = true;   // (the result is where the query was: no number stays none)
-                else if (weighed) {
+            for (int h = from; weighed && h < to; h++) {
+                bool none = a.q == a.out;                   // (the result is where the query was: no number stays none)
+                if (!none) {
                     const T *const q = reinterpret_cast<const T *>(a.q) + row * a.q_token + h * a.q_head;
                     float s = 0.0f;
                     for (int c = 0; c < D; c++) s = fmaf((float)q[c], (float)key[c], s);
                     none = (p.negative ? -s : s) == -CUDART_INF_F;
                 }
-                for (int c = 0; c < 8; c++) {
-                    const uint32_t pair = c < 2 ? mine.x : c < 4 ? mine.y : c < 6 ? mine.z : mine.w, x = pair >> c % 2 * 16 & 0xffff;
-                    if ((x & INFINITE) != INFINITE) continue;
-                    const uint32_t code = none || (x & 0x7fff) != INFINITE ? 3 : (x & 0x8000 ? 2 : 1);
-                    const int channel = (h - h0) * D + piece % (D / 8) * 8 + c;
-                    atomicOr(seen + channel / 4, code << channel % 4 * 8);
-                }
+                if (none) keep(h, up | down, up | down);
             }
         }
     }
+    for (int h = from; way < ways && h < to; h++) keep(h, plus, minus);
     __syncthreads();
     for (int i = tid; i < heads * D; i += THREADS) {
         const uint32_t code = seen[i / 4] >> i % 4 * 8 & 3;
-        uint16_t *const out = reinterpret_cast<uint16_t *>(reinterpret_cast<T *>(a.out) + row * a.out_token + (h0 + i / D) * a.out_head + i % D);
-        if ((odd >> i / D & 1) && (code == 1 || code == 2) && (*out & 0x7fff) > INFINITE) *out = (uint16_t)(code == 1 ? INFINITE : INFINITE | 0x8000);
+        if ((code == 1 || code == 2) && no_number(i)) *result(i) = (uint16_t)(code == 1 ? INFINITE : INFINITE | 0x8000);
     }
     __syncthreads();
 }
@@ -663,7 +680,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
                     const int first_place = 2 * w_first + (even == 0.0f && begin > start_of(w_first, unused));
                     float4 *const join_v = reinterpret_cast<float4 *>(smem + scratch);       // (the stage that held the sums)
                     float2 *const join_ml = reinterpret_cast<float2 *>(join_v + THREADS);
-                    static_assert(THREADS * 24 <= STAGE && MAX_GROUP * D <= STAGE, "a stage has room for what is joined, and for what infinite_values keeps");
+                    static_assert(THREADS * 24 <= STAGE && MAX_GROUP * D + 4 <= STAGE && WH * D / 8 <= 32, "a stage has room for what is joined, and for what infinite_values keeps");
                     // the results of every step-th of `many` pieces from w on become one: the column's, or one in the first of their places
                     auto join = [&](int w, int step, int many, bool final) {
                         const int per = min(pieces, THREADS), ways = THREADS / per, way = tid / per;

@@ -84,3 +84,18 @@ def test_keys(ops, dtype):  # noqa: F811
         put(1, 3, 0, 11, INF)
         put(2, 5, 0, 2, NAN, keys=True)
     check(ops, [50, 1000, 30], 4, 1, 64, dtype, plant, seed=5)
+
+
+@pytest.mark.parametrize("Hq,Hkv,D", [(8, 4, 64), (4, 4, 96), (16, 2, 128), (4, 2, 256)])
+def test_signs_side_by_side(ops, Hq, Hkv, D):  # noqa: F811
+    """Infinities of two signs in neighbouring channels, everywhere; whole rows that are infinite, or no numbers."""
+    lengths = [3, 700, 64, 2500]
+
+    def plant(put):
+        for h in range(Hkv):
+            for d in range(0, 16, 2):
+                put(0, 1, h, d, INF), put(0, 1, h, d + 1, -INF), put(1, 650, h, d, -INF), put(1, 2, h, d + 1, INF)
+            for d in range(D):
+                put(2, 63, h, d, INF if d % 3 else NAN), put(3, 2000, h, d, -INF)
+    for dtype in (torch.float16, torch.bfloat16):
+        check(ops, lengths, Hq, Hkv, D, dtype, plant)
