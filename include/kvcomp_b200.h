@@ -59,7 +59,8 @@ extern "C" {
 #define KVC_FLAG_NO_PAGES        0x800  /* page plan: a request was refused (no pages left, or its table row or the token rows are full);
                                          * page release: more pages than have been taken */
 #define KVC_FLAG_BAD_PAGE        0x1000 /* paged cache: a table entry or a slot outside the pool; its tokens are left out */
-#define KVC_FLAG_BAD_LENGTH      0x2000 /* paged cache: a length or a count of new tokens below 0, or beyond the table row */
+#define KVC_FLAG_BAD_LENGTH      0x2000 /* paged cache: a length or a count of new tokens below 0, or beyond the table row;
+                                         * attention of packed rows: a request with more than one */
 
 typedef void *kvc_stream_t;   /* a cudaStream_t; NULL = the legacy default stream */
 
