@@ -99,3 +99,26 @@ def test_signs_side_by_side(ops, Hq, Hkv, D):  # noqa: F811
                 put(2, 63, h, d, INF if d % 3 else NAN), put(3, 2000, h, d, -INF)
     for dtype in (torch.float16, torch.bfloat16):
         check(ops, lengths, Hq, Hkv, D, dtype, plant)
+
+
+@pytest.mark.parametrize("Hq,Hkv,D", [(8, 2, 64), (6, 3, 96), (16, 1, 128), (9, 1, 256)])
+def test_packed_rows_and_in_place(ops, Hq, Hkv, D):  # noqa: F811
+    """Infinities of requests whose rows are packed, some requests without one; where the result takes the queries' place."""
+    gen = torch.Generator(device="cuda").manual_seed(D)
+    lengths, page = [5000, 40, 1, 0, 9000, 300], 16
+    pages = sum(-(-n // page) for n in lengths) + 1
+    table, _, _ = plain.tables(np.random.RandomState(D), lengths, page, pages)
+    kp, vp = (plain.pool(gen, pages, page, Hkv, D, torch.float16, "cuda") for _ in range(2))
+    for b, n in enumerate(lengths):
+        for t in {0, n // 2, n - 1} if n else ():
+            vp[int(table[b, t // page]), t % page, :, 3 + b] = -INF if t and b > 3 else INF
+    q = torch.randn(6, Hq, D, generator=gen, device="cuda").half()
+    args = (kp, vp, dev(table), dev(lengths), 0.2)
+    want = ops.paged_attn(q, *args)
+    assert torch.isposinf(want).nonzero()[:, ::2].unique(dim=0).tolist() == [[0, 3], [1, 4], [2, 5]]
+    assert torch.isnan(want).nonzero()[:, ::2].unique(dim=0).tolist() == [[4, 7], [5, 8]]
+    rows = [0, 1, 2, 4, 5]
+    got = ops.paged_attn(q[rows], *args, starts=dev([0, 1, 2, 3, 3, 4, 5]))
+    torch.testing.assert_close(got, want[rows], rtol=0, atol=0, equal_nan=True)
+    assert ops.paged_attn(q, *args, out=q) is q
+    torch.testing.assert_close(q, want, rtol=0, atol=0, equal_nan=True)
