@@ -472,6 +472,62 @@ int kvc_paged_attn(const kvc_paged_attn_args *args, kvc_stream_t stream);
  * plan's).  A request without a row is left out.  Rows behind the last request's, and those of a request that has more than one (KVC_FLAG_BAD_LENGTH), get 0 and -inf. */
 int kvc_paged_attn_rows(const kvc_paged_attn_args *args, const int32_t *starts, int64_t rows, kvc_stream_t stream);
 
+/* Tokens in 8 bits.  A row (a token's channels of a KV head) has codes c of 8 bits and one scale s (fp32) and stands for the values c s:
+ *   KVC_CODES_INT8  s = max |x| / 127, c = x / s to the nearest whole number, ties to even
+ *   KVC_CODES_E4M3  s = the least power of two with max |x| / s <= 448, c = x / s to the nearest e4m3
+ * No scale is below 2^-100.  A row with an infinity or no number in it has the scale NaN.  The scales of a pool [n_pages, page_size, Hkv, D] are [n_pages, Hkv, page_size], the
+ * last dimension contiguous; strides count elements, those of a pool of codes bytes.  Rows of codes start on 16 bytes (pointers and strides), D is a multiple of 16. */
+#define KVC_CODES_NONE 0
+#define KVC_CODES_INT8 1
+#define KVC_CODES_E4M3 2
+typedef struct {
+    float *k, *v;
+    int64_t k_page, k_head, v_page, v_head;
+    int32_t codes, reserved;
+} kvc_scales;
+
+/* kvc_rotary_store into pools of codes: keys are coded from their rotated values in fp32, values from theirs; Hkv > 0.  Neither pools nor scales may overlap one another or what is
+ * read or written beside them. */
+int kvc_rotary_store_codes(const kvc_rotary_args *args, const kvc_scales *scales, kvc_stream_t stream);
+
+/* The slots of all tokens that requests have, packed request by request: starts[b] the first row of request b (B + 1 numbers), slots[row] = page * page_size + row of
+ * the page.  `tokens` rows; those behind the last request's have slot -1.  Requests beyond them are cut (KVC_FLAG_BAD_LENGTH, as for lengths that the table does not hold); a page
+ * below 0 gives -1 (KVC_FLAG_BAD_PAGE). */
+typedef struct {
+    const int32_t *lengths, *table;
+    int64_t table_stride, table_width, B, page_size, tokens;
+    int32_t *slots, *starts;
+    int32_t *status;
+} kvc_page_slots_args;
+int kvc_page_slots(const kvc_page_slots_args *args, kvc_stream_t stream);
+
+/* positions[row] += first[b] for the rows starts[b] .. starts[b + 1] - 1 of each request (a plan's positions, for requests whose tokens follow a prefix of first[b] tokens). */
+typedef struct {
+    const int32_t *starts, *first;
+    int32_t *positions;
+    int64_t B, tokens;
+} kvc_page_shift_args;
+int kvc_page_shift(const kvc_page_shift_args *args, kvc_stream_t stream);
+
+/* The rows `slots` of the pools, keys and values, as fp16 or bf16 rows k_out, v_out [N, Hkv, D]: codes times scales in fp32, rounded once, or (KVC_CODES_NONE) rows of 16 bits as they are.
+ * A slot below 0 gives zeros, one behind the pool zeros and KVC_FLAG_BAD_PAGE.  Everything starts on 16 bytes; outputs overlap neither one another nor a pool. */
+typedef struct {
+    const void *kpages, *vpages;
+    kvc_scales scales;
+    const int32_t *slots;
+    void *k_out, *v_out;
+    int64_t N, Hkv, D, n_pages, page_size;
+    int64_t kp_page, kp_row, kp_head, vp_page, vp_row, vp_head;
+    int64_t k_token, k_head, v_token, v_head;
+    int32_t *status;
+    int32_t type, reserved;
+} kvc_paged_rows_args;
+int kvc_paged_rows(const kvc_paged_rows_args *args, kvc_stream_t stream);
+
+/* kvc_paged_attn (starts null) or kvc_paged_attn_rows over pools of codes: a token's key is its codes times its scale, exactly, and its value too.  Both pools have the same strides, both
+ * arrays of scales too.  type: of q and out.  The same workspace. */
+int kvc_paged_attn_codes(const kvc_paged_attn_args *args, const kvc_scales *scales, const int32_t *starts, int64_t rows, kvc_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

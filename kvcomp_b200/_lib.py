@@ -56,8 +56,13 @@ PAGE_PLAN_ARGS = struct.Struct("<18q")
 PAGE_RELEASE_ARGS = struct.Struct("<14q")
 ROTARY_ARGS = struct.Struct("<31q3if")
 PAGED_ATTN_ARGS = struct.Struct("<29qfi")
+SCALES = struct.Struct("<6q2i")
+PAGE_SLOTS_ARGS = struct.Struct("<10q")
+PAGE_SHIFT_ARGS = struct.Struct("<5q")
+PAGED_ROWS_ARGS = struct.Struct("<2q6q2i19q2i")
 
 ROTARY_HALF, ROTARY_INTERLEAVED = 0, 1
+CODES_NONE, CODES_INT8, CODES_E4M3 = 0, 1, 2
 
 
 class KvcError(RuntimeError):
@@ -118,6 +123,11 @@ _SIGNATURES = {
     "kvc_paged_attn_workspace": (_i64, [_i64, _i64, _i64, _i64]),
     "kvc_paged_attn": (_i32, [C.c_char_p, _vp]),
     "kvc_paged_attn_rows": (_i32, [C.c_char_p, _vp, _i64, _vp]),
+    "kvc_rotary_store_codes": (_i32, [C.c_char_p, C.c_char_p, _vp]),
+    "kvc_page_slots": (_i32, [C.c_char_p, _vp]),
+    "kvc_page_shift": (_i32, [C.c_char_p, _vp]),
+    "kvc_paged_rows": (_i32, [C.c_char_p, _vp]),
+    "kvc_paged_attn_codes": (_i32, [C.c_char_p, C.c_char_p, _vp, _i64, _vp]),
     "kvc_k_matvec": (_i32, [_vp, _vp, _vp, _i64, _i64, _vp]),
 }
 
@@ -167,7 +177,8 @@ def torch_calls():
     loader.exec_module(module)
     lib = load()
     module.init(KvcError, *(C.cast(getattr(lib, name), C.c_void_p).value
-                            for name in ("kvc_page_plan", "kvc_page_release", "kvc_rotary_store", "kvc_paged_attn", "kvc_paged_attn_rows", "kvc_last_error")))
+                            for name in ("kvc_page_plan", "kvc_page_release", "kvc_rotary_store", "kvc_paged_attn", "kvc_paged_attn_rows", "kvc_last_error",
+                                         "kvc_rotary_store_codes", "kvc_page_slots", "kvc_page_shift", "kvc_paged_rows", "kvc_paged_attn_codes")))
     _torch_calls = module
     return module
 

@@ -112,3 +112,50 @@ __device__ __forceinline__ void kvc_behind() {
     cudaGridDependencySynchronize();
     cudaTriggerProgrammaticLaunchCompletion();
 }
+
+__device__ __forceinline__ void raise_flag(int32_t *status, int flags) {
+    if (flags && status) atomicOr(status, flags);
+}
+
+// ---- rotation
+template <typename T> __device__ __forceinline__ float to_float(T v);
+template <> __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+template <> __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> __device__ __forceinline__ T from_float(float v);
+template <> __device__ __forceinline__ __half from_float(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float(float v) { return __float2bfloat16_rn(v); }
+__device__ __forceinline__ float2 unpack(uint32_t v, __half) { return __half22float2(*reinterpret_cast<const __half2 *>(&v)); }
+__device__ __forceinline__ float2 unpack(uint32_t v, __nv_bfloat16) { return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&v)); }
+__device__ __forceinline__ uint32_t pack(float a, float b, __half) { const __half2 r = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t *>(&r); }
+__device__ __forceinline__ uint32_t pack(float a, float b, __nv_bfloat16) { const __nv_bfloat162 r = __floats2bfloat162_rn(a, b); return *reinterpret_cast<const uint32_t *>(&r); }
+
+// cos and sin of a position, given the turns of one step.  The turns are counted in fp64: what is left of a far position's angle after its whole
+// turns keeps 2^-53 of the angle, 1e-10 at a million radians; fp32 would keep 0.06.  Of the rest the nearest quarter is taken off, and the series of sine and cosine on
+// [-pi / 4, pi / 4] are left, to x^9 and x^10: the first terms left out are below 2^-29 and 2^-33 (fp32's half step there: 2^-25).
+constexpr double TURNS_OF_RADIANS = 0.15915494309189533576888;
+__device__ __forceinline__ float2 turn(double position, double turns, float factor) {
+    double whole = position * turns;
+    whole -= rint(whole);
+    const float t = (float)whole, quarter = rintf(4.0f * t), x = fmaf(-0.25f, quarter, t) * 6.2831853071795865f, y = x * x;
+    const int q = (int)quarter;
+    float s = fmaf(y, 1.0f / 362880, -1.0f / 5040), c = fmaf(y, -1.0f / 3628800, 1.0f / 40320);
+    s = fmaf(y, s, 1.0f / 120);
+    c = fmaf(y, c, -1.0f / 720);
+    s = fmaf(y, s, -1.0f / 6);
+    c = fmaf(y, c, 1.0f / 24);
+    s = fmaf(x * y, s, x);
+    c = fmaf(y, c, -0.5f);
+    c = fmaf(y, c, 1.0f);
+    const float a = q & 1 ? s : c, b = q & 1 ? c : s;
+    return make_float2(((q + 1) & 2 ? -a : a) * factor, (q & 2 ? -b : b) * factor);
+}
+
+// Queries, keys or values: a CTA has rows of one of them.  dst: token stride 0 for the pools, where `places` say where a token goes.
+struct Part {
+    const void *src;
+    void *dst;
+    int64_t src_token, src_head, dst_token, dst_head;
+    int heads, chunk, of_token, turned;                     // heads, those that a thread takes, threads' shares of a token, rotated units of a head
+    unsigned first;                                         // CTA
+    kvc_div chunks;                                         // by of_token
+};

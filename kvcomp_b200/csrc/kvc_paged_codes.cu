@@ -1,0 +1,475 @@
+// Paged caches whose tokens are held in 8 bits: rows are coded as they go to their slots, and read back.
+//
+// A row (a token's channels of a KV head, keys after their rotation) has one scale s in 32 bits.  int8: s = max |x| / 127, codes x / s to the nearest whole number, ties to even.
+// e4m3: s = the least power of two with max |x| / s <= 448, codes x / s to the nearest e4m3: a power of two costs a floating code nothing, and the quotient is exact.  No scale is
+// below 2^-100, so that its inverse and its products are numbers.  A row that holds an infinity or no number has no scale: NaN, and all of it reads back so.
+//
+// Every value is read once and written once: HBM for a prompt, latency for a step, as for rows of 16 bits; the codes are a part of the instructions only where that does not show.
+#include <cuda_fp8.h>
+#include <math_constants.h>
+#include <string.h>
+
+#include <algorithm>
+
+#include "kvc_paged.cuh"
+
+namespace {
+
+struct CodesParams {
+    kvc_rotary_args a;
+    kvc_scales s;
+    kvc_div page;
+    long long slots;                                        // of the pool
+    int lanes, units;                                       // lanes of a row (a power of two), those that have channels
+    Part parts[3];
+};
+
+constexpr int CODES_THREADS = 256, CHUNK = 4;
+constexpr float LEAST_SCALE = 7.888609052210118e-31f;       // 2^-100
+
+// bits of |x|, so that what is no number is the largest
+__device__ __forceinline__ uint32_t size_of(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+
+// The scale of a row by its largest size, and one over it.
+template <int KIND> __device__ __forceinline__ float scale_of(uint32_t top, float &inverse) {
+    float s;
+    if (KIND == KVC_CODES_INT8) {
+        s = fmaxf(__fdiv_rn(__uint_as_float(top), 127.0f), LEAST_SCALE);
+        inverse = __frcp_rn(s);
+    } else {                                                // top = m 2^e, 448 = 1.75 2^8: e - 8, one more where m is above 1.75
+        const int e = max((int)((top + 0x1fffffu) >> 23) - 8, 127 - 100);
+        s = __uint_as_float((uint32_t)e << 23);
+        inverse = __uint_as_float((uint32_t)(254 - e) << 23);
+    }
+    if (top >= 0x7f800000u) s = CUDART_NAN_F;
+    return s;
+}
+
+// Four codes of a row, packed.  int8: x times one over s is off by 127 1.5 2^-24 of a step at most, so the whole number next to it is right unless it lies that near the border
+// of two.  There the remainder x - q s says: it is a multiple of s's last bit and no larger than s, hence exact.
+template <int KIND> __device__ __forceinline__ uint32_t codes4(const float *x, float s, float inverse) {
+    if (KIND == KVC_CODES_INT8) {
+        constexpr float WHOLE = 12582912.0f;                // 1.5 2^23: a sum's last bits are a whole number's
+        uint32_t c[4];
+        float far = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float t = __fmul_rn(x[i], inverse), w = __fadd_rn(t, WHOLE);
+            c[i] = __float_as_uint(w);
+            far = fmaxf(far, fabsf(t - (w - WHOLE)));
+        }
+        if (far > 0.4999f) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float q = __uint_as_float(c[i]) - WHOLE, r = fmaf(-q, s, x[i]), d = 2.0f * fabsf(r);
+                if (d > s || (d == s && (c[i] & 1))) c[i] += r > 0.0f ? 1 : -1;
+            }
+        }
+        return __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+    } else {
+        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(x[0] * inverse, x[1] * inverse), __NV_SATFINITE, __NV_E4M3);
+        const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(x[2] * inverse, x[3] * inverse), __NV_SATFINITE, __NV_E4M3);
+        return lo | hi << 16;
+    }
+}
+
+// Where a token goes: its row in the pools (in codes) and its place among the scales; -1: nowhere
+struct Place { long long k, v, ks, vs; };
+__device__ __forceinline__ Place place_of(const CodesParams &p, long long n, int &flags) {
+    const kvc_rotary_args &a = p.a;
+    Place r = {-1, -1, 0, 0};
+    const int slot = a.slots[n];
+    if (slot < 0) return r;
+    if (slot >= p.slots) { flags = KVC_FLAG_BAD_PAGE; return r; }
+    const int page = kvc_divide(slot, p.page), row = slot - page * (int)a.page_size;
+    r.k = page * a.kp_page + row * a.kp_row;
+    r.v = page * a.vp_page + row * a.vp_row;
+    r.ks = page * p.s.k_page + row;
+    r.vs = page * p.s.v_page + row;
+    return r;
+}
+
+// Heads of 16 n channels, rotated by multiples of 16, everything on 16 bytes.  As for rows of 16 bits a thread has a unit of 16 channels (8 pairs) of up to CHUNK heads of a token, whose
+// angles it makes once; the lanes of a row are neighbours in a warp and find the row's largest value among them.
+template <typename T, int KIND>
+__global__ void __launch_bounds__(CODES_THREADS, 3) codes_rows_kernel(const __grid_constant__ CodesParams p) {
+    kvc_behind();
+    const kvc_rotary_args &a = p.a;
+    const int which = blockIdx.x >= p.parts[2].first ? 2 : (blockIdx.x >= p.parts[1].first ? 1 : 0);
+    const Part &part = p.parts[which];
+    const int turned = part.turned, id = (int)((blockIdx.x - part.first) * CODES_THREADS + threadIdx.x);
+    const int u = id & (p.lanes - 1), group = id / p.lanes, n = kvc_divide(group, part.chunks);       // (lanes: a power of two)
+    if (n >= a.N) return;
+    const bool on = u < p.units;
+    const int h0 = (group - n * part.of_token) * part.chunk, heads = min(part.chunk, part.heads - h0);
+    const bool half = a.layout == KVC_ROTARY_HALF && u < turned;
+    const int c0 = half ? 8 * u : 16 * u, apart = half ? 8 * turned : 8;
+    const T *src = reinterpret_cast<const T *>(part.src) + n * part.src_token + h0 * part.src_head + c0;
+    uint4 x[CHUNK][2];
+#pragma unroll
+    for (int j = 0; j < CHUNK; j++) {
+        x[j][0] = x[j][1] = make_uint4(0, 0, 0, 0);
+        if (on && j < heads) {
+            x[j][0] = *reinterpret_cast<const uint4 *>(src);
+            x[j][1] = *reinterpret_cast<const uint4 *>(src + apart);
+        }
+        src += part.src_head;
+    }
+    uint8_t *dst = nullptr;
+    float *scale = nullptr;
+    if (which > 0) {
+        int flags = 0;
+        const Place at = place_of(p, n, flags);
+        raise_flag(a.status, flags);
+        if (at.k < 0) return;                               // (a token's lanes all go)
+        dst = reinterpret_cast<uint8_t *>(part.dst) + (which == 1 ? at.k : at.v) + h0 * part.dst_head + c0;
+        scale = which == 1 ? p.s.k + at.ks + h0 * p.s.k_head : p.s.v + at.vs + h0 * p.s.v_head;
+    }
+    const bool turns = u < turned;
+    float2 cs[8];
+    if (turns) {
+        const double position = a.inverse ? -(double)a.positions[n] : (double)a.positions[n];
+#pragma unroll
+        for (int k = 0; k < 8; k++) cs[k] = turn(position, a.frequencies[8 * u + k] * TURNS_OF_RADIANS, a.factor);
+    }
+    const unsigned row_lanes = (p.lanes == 32 ? 0xffffffffu : (1u << p.lanes) - 1) << (threadIdx.x & 31 & ~(p.lanes - 1));
+#pragma unroll
+    for (int j = 0; j < CHUNK; j++) {
+        if (j < heads) {
+            const uint32_t w[8] = {x[j][0].x, x[j][0].y, x[j][0].z, x[j][0].w, x[j][1].x, x[j][1].y, x[j][1].z, x[j][1].w};
+            float f[16];
+#pragma unroll
+            for (int m = 0; m < 8; m++) {
+                const float2 v = unpack(w[m], T());
+                f[2 * m] = v.x; f[2 * m + 1] = v.y;
+            }
+            if (turns) {
+                // pairs: with halves a value of the first piece and its like of the second, else neighbours
+if (half) {
+#pragma unroll
+                    for (int m = 0; m < 8; m++) {
+                        const float f0 = f[m], f1 = f[8 + m];
+                        f[m] = f0 * cs[m].x - f1 * cs[m].y;
+                        f[8 + m] = f1 * cs[m].x + f0 * cs[m].y;
+                    }
+                } else {
+#pragma unroll
+                    for (int m = 0; m < 8; m++) {
+                        const float f0 = f[2 * m], f1 = f[2 * m + 1];
+                        f[2 * m] = f0 * cs[m].x - f1 * cs[m].y;
+                        f[2 * m + 1] = f1 * cs[m].x + f0 * cs[m].y;
+                    }
+                }
+            }
+            if (which == 0) {
+                T *to = reinterpret_cast<T *>(part.dst) + n * part.dst_token + (h0 + j) * part.dst_head + c0;
+                if (on) {
+                    *reinterpret_cast<uint4 *>(to) = make_uint4(pack(f[0], f[1], T()), pack(f[2], f[3], T()), pack(f[4], f[5], T()), pack(f[6], f[7], T()));
+                    *reinterpret_cast<uint4 *>(to + apart) = make_uint4(pack(f[8], f[9], T()), pack(f[10], f[11], T()), pack(f[12], f[13], T()), pack(f[14], f[15], T()));
+                }
+                continue;
+            }
+            uint32_t top = 0;
+#pragma unroll
+            for (int m = 0; m < 16; m++) top = max(top, size_of(f[m]));
+            for (int o = p.lanes / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(row_lanes, top, o));
+            float inverse;
+            const float s = scale_of<KIND>(top, inverse);
+            if (on) {
+                *reinterpret_cast<uint2 *>(dst) = make_uint2(codes4<KIND>(f, s, inverse), codes4<KIND>(f + 4, s, inverse));
+                *reinterpret_cast<uint2 *>(dst + apart) = make_uint2(codes4<KIND>(f + 8, s, inverse), codes4<KIND>(f + 12, s, inverse));
+                if (u == 0) *scale = s;
+            }
+            dst += part.dst_head;
+            scale += which == 1 ? p.s.k_head : p.s.v_head;
+        }
+    }
+}
+
+// Any sizes and strides of what is read: a warp per row, a lane every 32nd channel.
+template <typename T, int KIND>
+__global__ void __launch_bounds__(CODES_THREADS) codes_any_kernel(const __grid_constant__ CodesParams p) {
+    kvc_behind();
+    const kvc_rotary_args &a = p.a;
+    const long long heads = a.Hq + 2 * a.Hkv, row = (long long)blockIdx.x * (CODES_THREADS / 32) + (threadIdx.x >> 5);
+    if (row >= a.N * heads) return;
+    const int lane = threadIdx.x & 31, h = (int)(row % heads), D = (int)a.D, rotary = h < a.Hq + a.Hkv ? (int)a.rotary : 0;
+    const long long n = row / heads;
+    const T *x;
+    T *y = nullptr;
+    uint8_t *dst = nullptr;
+    float *scale = nullptr;
+    if (h < a.Hq) {
+        x = reinterpret_cast<const T *>(a.q) + n * a.q_token + h * a.q_head;
+        y = reinterpret_cast<T *>(a.q_out) + n * a.out_token + h * a.out_head;
+    } else {
+        const bool key = h < a.Hq + a.Hkv;
+        const long long hk = h - a.Hq - (key ? 0 : a.Hkv);
+        int flags = 0;
+        const Place at = place_of(p, n, flags);
+        if (lane == 0) raise_flag(a.status, flags);
+        if (at.k < 0) return;
+        x = key ? reinterpret_cast<const T *>(a.k) + n * a.k_token + hk * a.k_head : reinterpret_cast<const T *>(a.v) + n * a.v_token + hk * a.v_head;
+        dst = key ? reinterpret_cast<uint8_t *>(a.kpages) + at.k + hk * a.kp_head : reinterpret_cast<uint8_t *>(a.vpages) + at.v + hk * a.vp_head;
+        scale = key ? p.s.k + at.ks + hk * p.s.k_head : p.s.v + at.vs + hk * p.s.v_head;
+    }
+    const double position = rotary == 0 ? 0.0 : a.inverse ? -(double)a.positions[n] : (double)a.positions[n];
+    auto pair_of = [&](int i, int &other, bool &second) {   // a rotated channel's pair
+        const int half = rotary / 2;
+        second = a.layout == KVC_ROTARY_HALF ? i >= half : i & 1;
+        other = a.layout == KVC_ROTARY_HALF ? (second ? i - half : i + half) : i ^ 1;
+        return a.layout == KVC_ROTARY_HALF ? (second ? other : i) : i >> 1;
+    };
+    auto value = [&](int i) {
+        if (i >= rotary) return to_float(x[i]);
+        int other;
+        bool second;
+        const int k = pair_of(i, other, second);
+        const float2 cs = turn(position, a.frequencies[k] * TURNS_OF_RADIANS, a.factor);
+        const float f0 = to_float(x[second ? other : i]), f1 = to_float(x[second ? i : other]);
+        return second ? f1 * cs.x + f0 * cs.y : f0 * cs.x - f1 * cs.y;
+    };
+    if (h < a.Hq) {                                         // (the result may lie where the query does: 32 channels and their partners are read before any is written)
+        for (int i = lane; i < D; i += 32) {
+            if (i >= rotary) { y[i] = x[i]; continue; }
+            int other;
+            bool second;
+            const int k = pair_of(i, other, second);
+            if (second) continue;
+            const float2 cs = turn(position, a.frequencies[k] * TURNS_OF_RADIANS, a.factor);
+            const float f0 = to_float(x[i]), f1 = to_float(x[other]);
+            y[i] = from_float<T>(f0 * cs.x - f1 * cs.y);
+            y[other] = from_float<T>(f1 * cs.x + f0 * cs.y);
+        }
+        return;
+    }
+    uint32_t top = 0;
+    for (int i = lane; i < D; i += 32) top = max(top, size_of(value(i)));
+    top = __reduce_max_sync(0xffffffffu, top);
+    float inverse;
+    const float s = scale_of<KIND>(top, inverse);
+    for (int i = lane; i < D; i += 32) {
+        const float v[4] = {value(i), 0.0f, 0.0f, 0.0f};
+        dst[i] = (uint8_t)codes4<KIND>(v, s, inverse);
+    }
+    if (lane == 0) *scale = s;
+}
+
+// ---- rows out of pages ----------------------------------------------------------------------------------------------
+
+struct RowsParams {
+    kvc_paged_rows_args a;
+    kvc_div page, units, chunks;                            // divisors: page size, units of a row, threads' shares of a token
+    long long slots;
+    int of_token, chunk;
+};
+
+template <int KIND> __device__ __forceinline__ void values4(uint32_t c, float s, float *v) {
+    if (KIND == KVC_CODES_INT8) {
+        // a byte becomes the last bits of 2^23 + 128 + code
+        const uint32_t b = c ^ 0x80808080u;
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = (__uint_as_float(__byte_perm(b, 0x4b000000u, 0x7440 + i)) - 8388736.0f) * s;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(c >> 16 * i), __NV_E4M3);
+            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h));
+            v[2 * i] = f.x * s; v[2 * i + 1] = f.y * s;
+        }
+    }
+}
+
+// A thread has 16 channels of up to CHUNK heads of a token, keys or values.  KIND 0: rows of 16 bits, copied.
+template <typename T, int KIND>
+__global__ void __launch_bounds__(CODES_THREADS) paged_rows_kernel(const __grid_constant__ RowsParams p) {
+    kvc_behind();
+    const kvc_paged_rows_args &a = p.a;
+    const bool values = blockIdx.y;
+    const int id = (int)(blockIdx.x * CODES_THREADS + threadIdx.x), group = kvc_divide(id, p.units), u = id - group * (int)(a.D / 16), n = kvc_divide(group, p.chunks);
+    if (n >= a.N) return;
+    const int h0 = (group - n * p.of_token) * p.chunk, heads = min(p.chunk, (int)a.Hkv - h0);
+    T *out = reinterpret_cast<T *>(values ? a.v_out : a.k_out) + n * (values ? a.v_token : a.k_token) + h0 * (values ? a.v_head : a.k_head) + 16 * u;
+    const long long out_head = values ? a.v_head : a.k_head;
+    const int slot = a.slots[n];
+    const bool there = slot >= 0 && slot < p.slots;
+    if (slot >= p.slots) raise_flag(a.status, KVC_FLAG_BAD_PAGE);
+    const int page = there ? kvc_divide(slot, p.page) : 0, row = there ? slot - page * (int)a.page_size : 0;
+    const long long at = (values ? page * a.vp_page + row * a.vp_row + h0 * a.vp_head : page * a.kp_page + row * a.kp_row + h0 * a.kp_head) + 16 * u;
+    const long long head = values ? a.vp_head : a.kp_head;
+    const void *pool = values ? a.vpages : a.kpages;
+    constexpr int WORDS = KIND ? 1 : 2;
+    uint4 c[CHUNK][WORDS];
+    float s[CHUNK];
+#pragma unroll
+    for (int j = 0; j < CHUNK; j++) {
+        if (!there || j >= heads) continue;
+        if (KIND) {
+            c[j][0] = *reinterpret_cast<const uint4 *>(reinterpret_cast<const uint8_t *>(pool) + at + j * head);
+            s[j] = values ? a.scales.v[page * a.scales.v_page + (h0 + j) * a.scales.v_head + row] : a.scales.k[page * a.scales.k_page + (h0 + j) * a.scales.k_head + row];
+        } else {
+            const uint4 *from = reinterpret_cast<const uint4 *>(reinterpret_cast<const T *>(pool) + at + j * head);
+            c[j][0] = from[0];
+            c[j][WORDS - 1] = from[1];
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < CHUNK; j++) {
+        if (j >= heads) continue;
+        uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
+        if (there && KIND) {
+            float v[16];
+            values4<KIND>(c[j][0].x, s[j], v);
+            values4<KIND>(c[j][0].y, s[j], v + 4);
+            values4<KIND>(c[j][0].z, s[j], v + 8);
+            values4<KIND>(c[j][0].w, s[j], v + 12);
+            lo = make_uint4(pack(v[0], v[1], T()), pack(v[2], v[3], T()), pack(v[4], v[5], T()), pack(v[6], v[7], T()));
+            hi = make_uint4(pack(v[8], v[9], T()), pack(v[10], v[11], T()), pack(v[12], v[13], T()), pack(v[14], v[15], T()));
+        } else if (there) {
+            lo = c[j][0];
+            hi = c[j][WORDS - 1];
+        }
+        reinterpret_cast<uint4 *>(out + j * out_head)[0] = lo;
+        reinterpret_cast<uint4 *>(out + j * out_head)[1] = hi;
+    }
+}
+
+bool known_codes(int codes) { return codes == KVC_CODES_INT8 || codes == KVC_CODES_E4M3; }
+
+}  // namespace
+
+extern "C" int kvc_rotary_store_codes(const kvc_rotary_args *args, const kvc_scales *scales, kvc_stream_t stream) {
+    KVC_REQUIRE(args && scales, "kvc_rotary_store_codes: null pointer");
+    CodesParams p;
+    memcpy(&p.a, args, sizeof(p.a));
+    memcpy(&p.s, scales, sizeof(p.s));
+    kvc_rotary_args &a = p.a;
+    kvc_scales &s = p.s;
+    KVC_REQUIRE(a.type == KVC_TYPE_FP16 || a.type == KVC_TYPE_BF16, "kvc_rotary_store_codes: unknown type %d", a.type);
+    KVC_REQUIRE(known_codes(s.codes), "kvc_rotary_store_codes: unknown codes %d", s.codes);
+    KVC_REQUIRE(a.layout == KVC_ROTARY_HALF || a.layout == KVC_ROTARY_INTERLEAVED, "kvc_rotary_store_codes: unknown layout %d", a.layout);
+    KVC_REQUIRE(a.N >= 0 && a.Hq >= 0 && a.Hkv > 0 && a.D > 0 && a.D <= 65536 && a.D % 16 == 0 && a.rotary >= 0 && a.rotary <= a.D && a.rotary % 2 == 0,
+                "kvc_rotary_store_codes: bad sizes (head of %lld channels, %lld rotated)", (long long)a.D, (long long)a.rotary);
+    KVC_REQUIRE(a.page_size > 0 && a.page_size <= KVC_MAX_PAGE && a.n_pages >= 0 && a.n_pages * a.page_size < (1ll << 31), "kvc_rotary_store_codes: bad pool");
+    if (a.N == 0) return KVC_OK;
+    KVC_REQUIRE((a.Hq == 0 || (a.q && a.q_out)) && a.k && a.v && a.slots && ((a.kpages && a.vpages && s.k && s.v) || a.n_pages == 0) && (a.rotary == 0 || (a.positions && a.frequencies)),
+                "kvc_rotary_store_codes: null pointer");
+    KVC_REQUIRE(a.Hq < (1 << 20) && a.Hkv < (1 << 20) && a.N < (1ll << 31), "kvc_rotary_store_codes: too many heads or tokens");
+    const long long H = a.Hq + 2 * a.Hkv, rows = a.N * H;
+    p.page = kvc_make_div((uint32_t)a.page_size);
+    p.slots = a.n_pages * a.page_size;
+    // (the stride of a dimension of one, and what a part that is not there says, may be anything)
+    if (a.Hq == 0) a.q = nullptr, a.q_out = nullptr;
+    if (a.Hq <= 1) a.q_head = a.out_head = 0;
+    if (a.N == 1 || a.Hq == 0) a.q_token = a.out_token = 0;
+    if (a.Hkv == 1) a.k_head = a.v_head = a.kp_head = a.vp_head = s.k_head = s.v_head = 0;
+    if (a.N == 1) a.k_token = a.v_token = 0;
+    if (a.page_size == 1) a.kp_row = a.vp_row = 0;
+    if (a.n_pages <= 1) a.kp_page = a.vp_page = s.k_page = s.v_page = 0;
+    const uintptr_t pools = reinterpret_cast<uintptr_t>(a.kpages) | reinterpret_cast<uintptr_t>(a.vpages);
+    KVC_REQUIRE(((pools | a.kp_page | a.kp_row | a.kp_head | a.vp_page | a.vp_row | a.vp_head) & 15) == 0, "kvc_rotary_store_codes: rows of codes must start on 16 bytes");
+    KVC_REQUIRE(((reinterpret_cast<uintptr_t>(s.k) | reinterpret_cast<uintptr_t>(s.v)) & 3) == 0, "kvc_rotary_store_codes: scales must start on 4 bytes");
+    // What is written in no order must not overlap: rows of the results, of a pool or of the scales each other, a result what another thread reads.  (Sizes in halves of 16 bits.)
+    const kvc_rows q = kvc_make_rows(a.q, a.D, a.N, a.q_token, a.Hq, a.q_head), out = kvc_make_rows(a.q_out, a.D, a.N, a.out_token, a.Hq, a.out_head);
+    const kvc_rows k = kvc_make_rows(a.k, a.D, a.N, a.k_token, a.Hkv, a.k_head), v = kvc_make_rows(a.v, a.D, a.N, a.v_token, a.Hkv, a.v_head);
+    const kvc_rows written[4] = {kvc_make_rows(a.kpages, a.D / 2, a.n_pages, a.kp_page / 2, a.page_size, a.kp_row / 2, a.Hkv, a.kp_head / 2),
+                                 kvc_make_rows(a.vpages, a.D / 2, a.n_pages, a.vp_page / 2, a.page_size, a.vp_row / 2, a.Hkv, a.vp_head / 2),
+                                 kvc_make_rows(s.k, 2 * a.page_size, a.n_pages, 2 * s.k_page, a.Hkv, 2 * s.k_head),
+                                 kvc_make_rows(s.v, 2 * a.page_size, a.n_pages, 2 * s.v_page, a.Hkv, 2 * s.v_head)};
+    KVC_REQUIRE(a.Hq == 0 || out.apart, "kvc_rotary_store_codes: rows of the output overlap");
+    KVC_REQUIRE(a.Hq == 0 || kvc_rows_equal(q, out) || !kvc_rows_overlap(q, out), "kvc_rotary_store_codes: the output overlaps the queries and is not them");
+    KVC_REQUIRE(a.Hq == 0 || !(kvc_rows_overlap(k, out) || kvc_rows_overlap(v, out)), "kvc_rotary_store_codes: the output overlaps the keys or the values");
+    for (int i = 0; i < 4; i++) {
+        KVC_REQUIRE(written[i].apart, "kvc_rotary_store_codes: rows of a pool or of its scales overlap");
+        for (int j = 0; j < i; j++) KVC_REQUIRE(!kvc_rows_overlap(written[i], written[j]), "kvc_rotary_store_codes: the pools or their scales overlap");
+        KVC_REQUIRE(!kvc_rows_overlap(written[i], k) && !kvc_rows_overlap(written[i], v) && (a.Hq == 0 || (!kvc_rows_overlap(written[i], q) && !kvc_rows_overlap(written[i], out))),
+                    "kvc_rotary_store_codes: a pool overlaps what is read or the output");
+    }
+    const uintptr_t at = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.q_out) | reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v);
+    const int64_t strides = a.q_token | a.q_head | a.k_token | a.k_head | a.v_token | a.v_head | a.out_token | a.out_head;
+    cudaStream_t st = kvc_cu(stream);
+    const bool fp16 = a.type == KVC_TYPE_FP16, whole = s.codes == KVC_CODES_INT8;
+    p.units = (int)(a.D / 16);
+    p.lanes = 1;
+    while (p.lanes < p.units) p.lanes *= 2;
+    if ((at & 15) == 0 && (strides & 7) == 0 && a.rotary % 16 == 0 && p.lanes <= 32 && rows * p.lanes < (1ll << 31) - CODES_THREADS) {
+        p.parts[0] = {a.q, a.q_out, a.q_token, a.q_head, a.out_token, a.out_head, (int)a.Hq};
+        p.parts[1] = {a.k, a.kpages, a.k_token, a.k_head, 0, a.kp_head, (int)a.Hkv};
+        p.parts[2] = {a.v, a.vpages, a.v_token, a.v_head, 0, a.vp_head, (int)a.Hkv};
+        // heads of a thread: CHUNK share its angles, unless that leaves too few threads for the device's latency
+        const long long threads = 3ll * CODES_THREADS * kvc_sm_count();
+        const int chunk = (int)std::max<long long>(1, std::min<long long>(CHUNK, rows * p.lanes / threads));
+        int64_t grid = 0;
+        for (int i = 0; i < 3; i++) {
+            Part &part = p.parts[i];
+            const int chunks = std::max((part.heads + chunk - 1) / chunk, 1);
+            part.chunk = std::max((part.heads + chunks - 1) / chunks, 1);
+            part.of_token = chunks;
+            part.chunks = kvc_make_div((uint32_t)chunks);
+            part.turned = i < 2 ? (int)a.rotary / 16 : 0;
+            part.first = (unsigned)grid;
+            if (part.heads > 0) grid += (a.N * chunks * p.lanes + CODES_THREADS - 1) / CODES_THREADS;
+        }
+        auto *kernel = fp16 ? (whole ? codes_rows_kernel<__half, KVC_CODES_INT8> : codes_rows_kernel<__half, KVC_CODES_E4M3>)
+                            : (whole ? codes_rows_kernel<__nv_bfloat16, KVC_CODES_INT8> : codes_rows_kernel<__nv_bfloat16, KVC_CODES_E4M3>);
+        return kvc_launch_early(kernel, (unsigned)grid, CODES_THREADS, st, p);
+    }
+    const long long ctas = (rows + CODES_THREADS / 32 - 1) / (CODES_THREADS / 32);
+    KVC_REQUIRE(ctas < (1ll << 31), "kvc_rotary_store_codes: too many rows");
+    auto *kernel = fp16 ? (whole ? codes_any_kernel<__half, KVC_CODES_INT8> : codes_any_kernel<__half, KVC_CODES_E4M3>)
+                        : (whole ? codes_any_kernel<__nv_bfloat16, KVC_CODES_INT8> : codes_any_kernel<__nv_bfloat16, KVC_CODES_E4M3>);
+    return kvc_launch_early(kernel, (unsigned)ctas, CODES_THREADS, st, p);
+}
+
+extern "C" int kvc_paged_rows(const kvc_paged_rows_args *args, kvc_stream_t stream) {
+    KVC_REQUIRE(args, "kvc_paged_rows: null pointer");
+    RowsParams p;
+    memcpy(&p.a, args, sizeof(p.a));
+    kvc_paged_rows_args &a = p.a;
+    const int codes = a.scales.codes;
+    KVC_REQUIRE(a.type == KVC_TYPE_FP16 || a.type == KVC_TYPE_BF16, "kvc_paged_rows: unknown type %d", a.type);
+    KVC_REQUIRE(codes == KVC_CODES_NONE || known_codes(codes), "kvc_paged_rows: unknown codes %d", codes);
+    KVC_REQUIRE(a.N >= 0 && a.N < (1ll << 31) && a.Hkv > 0 && a.Hkv < (1 << 20) && a.D > 0 && a.D <= 65536 && a.D % 16 == 0, "kvc_paged_rows: bad sizes (head of %lld channels)", (long long)a.D);
+    KVC_REQUIRE(a.page_size > 0 && a.page_size <= KVC_MAX_PAGE && a.n_pages >= 0 && a.n_pages * a.page_size < (1ll << 31), "kvc_paged_rows: bad pool");
+    if (a.N == 0) return KVC_OK;
+    KVC_REQUIRE(a.slots && a.k_out && a.v_out && ((a.kpages && a.vpages && (codes == KVC_CODES_NONE || (a.scales.k && a.scales.v))) || a.n_pages == 0), "kvc_paged_rows: null pointer");
+    if (a.N == 1) a.k_token = a.v_token = 0;
+    if (a.Hkv == 1) a.k_head = a.v_head = a.kp_head = a.vp_head = a.scales.k_head = a.scales.v_head = 0;
+    if (a.page_size == 1) a.kp_row = a.vp_row = 0;
+    if (a.n_pages <= 1) a.kp_page = a.vp_page = a.scales.k_page = a.scales.v_page = 0;
+    const int64_t of_pools = a.kp_page | a.kp_row | a.kp_head | a.vp_page | a.vp_row | a.vp_head, of_rows = a.k_token | a.k_head | a.v_token | a.v_head;
+    const uintptr_t at = reinterpret_cast<uintptr_t>(a.kpages) | reinterpret_cast<uintptr_t>(a.vpages) | reinterpret_cast<uintptr_t>(a.k_out) | reinterpret_cast<uintptr_t>(a.v_out);
+    KVC_REQUIRE((at & 15) == 0 && (of_rows & 7) == 0 && (of_pools & (codes == KVC_CODES_NONE ? 7 : 15)) == 0, "kvc_paged_rows: rows must start on 16 bytes");
+    KVC_REQUIRE(((reinterpret_cast<uintptr_t>(a.scales.k) | reinterpret_cast<uintptr_t>(a.scales.v)) & 3) == 0, "kvc_paged_rows: scales must start on 4 bytes");
+    const int64_t half = codes == KVC_CODES_NONE ? 1 : 2;   // (sizes in halves of 16 bits)
+    const kvc_rows k = kvc_make_rows(a.k_out, a.D, a.N, a.k_token, a.Hkv, a.k_head), v = kvc_make_rows(a.v_out, a.D, a.N, a.v_token, a.Hkv, a.v_head);
+    const kvc_rows kp = kvc_make_rows(a.kpages, a.D / half, a.n_pages, a.kp_page / half, a.page_size, a.kp_row / half, a.Hkv, a.kp_head / half);
+    const kvc_rows vp = kvc_make_rows(a.vpages, a.D / half, a.n_pages, a.vp_page / half, a.page_size, a.vp_row / half, a.Hkv, a.vp_head / half);
+    KVC_REQUIRE(k.apart && v.apart && !kvc_rows_overlap(k, v), "kvc_paged_rows: rows of the outputs overlap");
+    for (const kvc_rows &out : {k, v}) KVC_REQUIRE(!kvc_rows_overlap(out, kp) && !kvc_rows_overlap(out, vp), "kvc_paged_rows: an output overlaps a pool");
+    p.page = kvc_make_div((uint32_t)a.page_size);
+    p.slots = a.n_pages * a.page_size;
+    const int64_t units = a.D / 16;
+    const long long threads = 4ll * CODES_THREADS * kvc_sm_count();
+    const int64_t chunk = std::max<int64_t>(1, std::min<int64_t>(CHUNK, a.N * a.Hkv * units / threads)), chunks = (a.Hkv + chunk - 1) / chunk;
+    p.units = kvc_make_div((uint32_t)units);
+    p.chunk = (int)((a.Hkv + chunks - 1) / chunks);
+    p.of_token = (int)chunks;
+    p.chunks = kvc_make_div((uint32_t)chunks);
+    KVC_REQUIRE(a.N * chunks * units < (1ll << 31) - CODES_THREADS, "kvc_paged_rows: too many rows");
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((a.N * chunks * units + CODES_THREADS - 1) / CODES_THREADS), 2);
+    cfg.blockDim = dim3(CODES_THREADS);
+    cfg.stream = kvc_cu(stream);
+    cudaLaunchAttribute early;
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &early;
+    cfg.numAttrs = 1;
+    const bool fp16 = a.type == KVC_TYPE_FP16;
+    auto *kernel = codes == KVC_CODES_NONE ? paged_rows_kernel<__half, 0>                          // (copied, whatever they are)
+                   : codes == KVC_CODES_INT8 ? (fp16 ? paged_rows_kernel<__half, KVC_CODES_INT8> : paged_rows_kernel<__nv_bfloat16, KVC_CODES_INT8>)
+                                             : (fp16 ? paged_rows_kernel<__half, KVC_CODES_E4M3> : paged_rows_kernel<__nv_bfloat16, KVC_CODES_E4M3>);
+    KVC_CUDA_OK(cudaLaunchKernelEx(&cfg, kernel, (const RowsParams)p));
+    return KVC_OK;
+}

@@ -8,10 +8,6 @@
 
 namespace {
 
-__device__ __forceinline__ void raise_flag(int32_t *status, int flags) {
-    if (flags && status) atomicOr(status, flags);
-}
-
 // ---- pages ----------------------------------------------------------------------------------------------------------
 //
 // Two sums over the requests in their order (tokens, pages) say where each one's rows and pages begin; one CTA makes them, 1024
@@ -235,52 +231,83 @@ __global__ void __launch_bounds__(FILL_THREADS) release_rows_kernel(const __grid
         release_rows(p, (int)i, freed, p.a.free_pages + p.a.head_out[0]);
 }
 
+struct SlotsParams { kvc_page_slots_args a; kvc_div page; };
+
+// slots of rows [first, first + 4)
+__device__ __forceinline__ void slot_rows(const SlotsParams &p, const int32_t *starts, int first, int end) {
+    const kvc_page_slots_args &a = p.a;
+    int b = -1, flags = 0;
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        const int n = first + k;
+        if (n >= a.tokens) continue;
+        int slot = -1;
+        if (n < end) {
+            if (b < 0) b = find_row(starts, (int)a.B, n);
+            else while (starts[b + 1] <= n) b++;
+            const int t = n - starts[b], at = kvc_divide(t, p.page), page = a.table[b * a.table_stride + at];
+            const long long wide = (long long)page * a.page_size + t - at * (int)a.page_size;
+            if (page >= 0 && wide < (1ll << 31)) slot = (int)wide;
+            else flags = KVC_FLAG_BAD_PAGE;
+        }
+        a.slots[n] = slot;
+    }
+    raise_flag(a.status, flags);
+}
+
+template <int THREADS, bool ALONE>
+__global__ void __launch_bounds__(THREADS) page_slots_kernel(const __grid_constant__ SlotsParams p) {
+    __shared__ longlong2 warps[32];
+    __shared__ int32_t starts_s[ALONE ? THREADS + 1 : 1];
+    const kvc_page_slots_args &a = p.a;
+    const bool near = ALONE && a.B <= THREADS;
+    kvc_behind();
+    const int B = (int)a.B;
+    long long rows = 0;
+    int flags = 0;
+    for (int b0 = 0; b0 < B; b0 += THREADS) {
+        const int b = b0 + threadIdx.x;
+        int held = b < B ? a.lengths[b] : 0;
+        const long long most = a.table_width * a.page_size;
+        if (held < 0 || held > most) { flags |= KVC_FLAG_BAD_LENGTH; held = held < 0 ? 0 : (int)most; }
+        long long start = held, zero = 0, total, unused;
+        block_scan2(start, zero, total, unused, warps);
+        start += rows;
+        if (start + held > a.tokens) flags |= KVC_FLAG_BAD_LENGTH;
+        if (b < B) {
+            a.starts[b] = (int32_t)min(start, (long long)a.tokens);
+            if (near) starts_s[b] = (int32_t)min(start, (long long)a.tokens);
+        }
+        rows += total;
+    }
+    const int end = (int)min(rows, (long long)a.tokens);
+    if (threadIdx.x == 0) {
+        a.starts[B] = end;
+        if (near) starts_s[B] = end;
+    }
+    raise_flag(a.status, flags);
+    if (ALONE) {
+        __syncthreads();
+        for (int n = threadIdx.x * 4; n < (int)a.tokens; n += THREADS * 4) slot_rows(p, near ? starts_s : a.starts, n, end);
+    }
+}
+
+__global__ void __launch_bounds__(FILL_THREADS) slot_rows_kernel(const __grid_constant__ SlotsParams p) {
+    kvc_behind();
+    const long long n = 4 * ((long long)blockIdx.x * FILL_THREADS + threadIdx.x);
+    if (n < p.a.tokens) slot_rows(p, p.a.starts, (int)n, p.a.starts[p.a.B]);
+}
+
+__global__ void __launch_bounds__(FILL_THREADS) page_shift_kernel(const __grid_constant__ kvc_page_shift_args p) {
+    kvc_behind();
+    const long long n = (long long)blockIdx.x * FILL_THREADS + threadIdx.x;
+    if (n < p.tokens && n < p.starts[p.B]) p.positions[n] += p.first[find_row(p.starts, (int)p.B, (int)n)];
+}
+
 // ---- rotation ---------------------------------------------------------------------------------------------------
 //
 // Every value is read once and written once: HBM for a prompt, latency for a step.  cos and sin are made once for a token and several of its
 // heads, in registers, while the first of these are on their way.
-
-template <typename T> __device__ __forceinline__ float to_float(T v);
-template <> __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
-template <> __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <typename T> __device__ __forceinline__ T from_float(float v);
-template <> __device__ __forceinline__ __half from_float(float v) { return __float2half_rn(v); }
-template <> __device__ __forceinline__ __nv_bfloat16 from_float(float v) { return __float2bfloat16_rn(v); }
-__device__ __forceinline__ float2 unpack(uint32_t v, __half) { return __half22float2(*reinterpret_cast<const __half2 *>(&v)); }
-__device__ __forceinline__ float2 unpack(uint32_t v, __nv_bfloat16) { return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&v)); }
-__device__ __forceinline__ uint32_t pack(float a, float b, __half) { const __half2 r = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t *>(&r); }
-__device__ __forceinline__ uint32_t pack(float a, float b, __nv_bfloat16) { const __nv_bfloat162 r = __floats2bfloat162_rn(a, b); return *reinterpret_cast<const uint32_t *>(&r); }
-
-// cos and sin of a position, given the turns of one step.  The turns are counted in fp64: what is left of a far position's angle after its whole
-// turns keeps 2^-53 of the angle, 1e-10 at a million radians; fp32 would keep 0.06.  Of the rest the nearest quarter is taken off, and the series of sine and cosine on
-// [-pi / 4, pi / 4] are left, to x^9 and x^10: the first terms left out are below 2^-29 and 2^-33 (fp32's half step there: 2^-25).
-constexpr double TURNS_OF_RADIANS = 0.15915494309189533576888;
-__device__ __forceinline__ float2 turn(double position, double turns, float factor) {
-    double whole = position * turns;
-    whole -= rint(whole);
-    const float t = (float)whole, quarter = rintf(4.0f * t), x = fmaf(-0.25f, quarter, t) * 6.2831853071795865f, y = x * x;
-    const int q = (int)quarter;
-    float s = fmaf(y, 1.0f / 362880, -1.0f / 5040), c = fmaf(y, -1.0f / 3628800, 1.0f / 40320);
-    s = fmaf(y, s, 1.0f / 120);
-    c = fmaf(y, c, -1.0f / 720);
-    s = fmaf(y, s, -1.0f / 6);
-    c = fmaf(y, c, 1.0f / 24);
-    s = fmaf(x * y, s, x);
-    c = fmaf(y, c, -0.5f);
-    c = fmaf(y, c, 1.0f);
-    const float a = q & 1 ? s : c, b = q & 1 ? c : s;
-    return make_float2(((q + 1) & 2 ? -a : a) * factor, (q & 2 ? -b : b) * factor);
-}
-
-// Queries, keys or values: a CTA has rows of one of them.  dst: token stride 0 for the pools, where `places` say where a token goes.
-struct Part {
-    const void *src;
-    void *dst;
-    int64_t src_token, src_head, dst_token, dst_head;
-    int heads, chunk, of_token, turned;                     // heads, those that a thread takes, threads' shares of a token, rotated units of a head
-    unsigned first;                                         // CTA
-    kvc_div chunks;                                         // by of_token
-};
 
 struct RotaryParams {
     kvc_rotary_args a;
@@ -455,6 +482,35 @@ extern "C" int kvc_page_release(const kvc_page_release_args *args, kvc_stream_t 
     }
     if (a.B <= SMALL_THREADS && most <= 8 * SMALL_THREADS) return kvc_launch_early(page_release_kernel<SMALL_THREADS, true>, 1, SMALL_THREADS, s, p);
     return kvc_launch_early(page_release_kernel<SCAN_THREADS, true>, 1, SCAN_THREADS, s, p);
+}
+
+extern "C" int kvc_page_slots(const kvc_page_slots_args *args, kvc_stream_t stream) {
+    KVC_REQUIRE(args, "kvc_page_slots: null pointer");
+    SlotsParams p;
+    memcpy(&p.a, args, sizeof(p.a));
+    const kvc_page_slots_args &a = p.a;
+    KVC_REQUIRE(a.B >= 0 && a.B < (1 << 24) && a.page_size > 0 && a.page_size <= KVC_MAX_PAGE && a.tokens >= 0 && a.tokens < (1ll << 31) - 4, "kvc_page_slots: bad sizes");
+    KVC_REQUIRE(a.table_width >= 0 && a.table_width * a.page_size < (1ll << 31) && (a.B <= 1 || a.table_stride >= 0), "kvc_page_slots: a table row holds %lld tokens, lengths have 32 bits",
+                (long long)(a.table_width * a.page_size));
+    KVC_REQUIRE(a.starts && (a.B == 0 || a.lengths) && (a.table || a.B == 0 || a.table_width == 0) && (a.tokens == 0 || a.slots), "kvc_page_slots: null pointer");
+    p.page = kvc_make_div((uint32_t)a.page_size);
+    cudaStream_t s = kvc_cu(stream);
+    if (a.tokens > FILL_ALONE) {
+        if (int rc = kvc_launch_early(page_slots_kernel<SCAN_THREADS, false>, 1, SCAN_THREADS, s, p)) return rc;
+        return kvc_launch_early(slot_rows_kernel, (unsigned)((a.tokens + 4 * FILL_THREADS - 1) / (4 * FILL_THREADS)), FILL_THREADS, s, p);
+    }
+    if (a.B <= SMALL_THREADS && a.tokens <= 4 * SMALL_THREADS) return kvc_launch_early(page_slots_kernel<SMALL_THREADS, true>, 1, SMALL_THREADS, s, p);
+    return kvc_launch_early(page_slots_kernel<SCAN_THREADS, true>, 1, SCAN_THREADS, s, p);
+}
+
+extern "C" int kvc_page_shift(const kvc_page_shift_args *args, kvc_stream_t stream) {
+    KVC_REQUIRE(args, "kvc_page_shift: null pointer");
+    kvc_page_shift_args p;
+    memcpy(&p, args, sizeof(p));
+    KVC_REQUIRE(p.B >= 0 && p.B < (1 << 24) && p.tokens >= 0 && p.tokens < (1ll << 31) - 4, "kvc_page_shift: bad sizes");
+    if (p.B == 0 || p.tokens == 0) return KVC_OK;
+    KVC_REQUIRE(p.starts && p.first && p.positions, "kvc_page_shift: null pointer");
+    return kvc_launch_early(page_shift_kernel, (unsigned)((p.tokens + FILL_THREADS - 1) / FILL_THREADS), FILL_THREADS, kvc_cu(stream), p);
 }
 
 extern "C" int kvc_rotary_store(const kvc_rotary_args *args, kvc_stream_t stream) {

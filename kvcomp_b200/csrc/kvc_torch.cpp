@@ -23,6 +23,11 @@ decltype(&kvc_rotary_store) rotary_store = nullptr;
 decltype(&kvc_paged_attn) paged_attn = nullptr;
 decltype(&kvc_paged_attn_rows) paged_attn_rows = nullptr;
 decltype(&kvc_last_error) last_error = nullptr;
+decltype(&kvc_rotary_store_codes) rotary_store_codes = nullptr;
+decltype(&kvc_page_slots) page_slots = nullptr;
+decltype(&kvc_page_shift) page_shift = nullptr;
+decltype(&kvc_paged_rows) paged_rows = nullptr;
+decltype(&kvc_paged_attn_codes) paged_attn_codes = nullptr;
 
 [[noreturn]] void fail(const std::string &why) {
     PyErr_SetString(error_class ? error_class : PyExc_RuntimeError, why.c_str());
@@ -138,6 +143,25 @@ PyObject *tuple(std::initializer_list<at::Tensor> parts) {
     return r;
 }
 
+// The type of a pool's rows: the other tensors' type, or, where there are scales, codes'.  The scales of [pages, page_size, heads, channels] are [pages, heads, page_size].
+kvc_scales scales_of(const at::Tensor &pool, PyObject *k, PyObject *v, at::ScalarType &type, int device) {
+    kvc_scales s = {};
+    const bool codes = pool.scalar_type() == at::kChar || pool.scalar_type() == at::kFloat8_e4m3fn;
+    if (!given(k) && !given(v)) {
+        if (codes) fail("pools of codes need kscales and vscales");
+        return s;
+    }
+    if (!given(k) || !given(v)) fail("kscales and vscales must be given together");
+    if (!codes) fail(std::string("with scales the pools must be int8 or float8_e4m3fn, got ") + c10::toString(pool.scalar_type()));
+    type = pool.scalar_type();
+    s.codes = type == at::kChar ? KVC_CODES_INT8 : KVC_CODES_E4M3;
+    const int64_t shape[3] = {pool.size(0), pool.size(2), pool.size(1)};
+    const at::Tensor &ks = rows(k, shape, at::kFloat, "kscales", device), &vs = rows(v, shape, at::kFloat, "vscales", device);
+    s.k = static_cast<float *>(ks.data_ptr()); s.k_page = ks.stride(0); s.k_head = ks.stride(1);
+    s.v = static_cast<float *>(vs.data_ptr()); s.v_page = vs.stride(0); s.v_head = vs.stride(1);
+    return s;
+}
+
 // lengths, new, table, free, head, page_size, tokens, out (six tensors or None), status
 PyObject *py_page_plan(PyObject *, PyObject *const *args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
@@ -215,10 +239,10 @@ PyObject *py_page_release(PyObject *, PyObject *const *args, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-// q or None, k or None, v, positions, slots, frequencies or None, kpages, vpages, layout, factor, inverse, out or None, status; q's name for messages is x without k
+// q or None, k or None, v, positions, slots, frequencies or None, kpages, vpages, layout, factor, inverse, out or None, status, kscales or None, vscales or None; q's name for messages is x without k
 PyObject *py_rotary_store(PyObject *, PyObject *const *args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    count(n, 13);
+    count(n, 15);
     const bool has_q = given(args[0]), has_k = given(args[1]);
     const char *const q_name = has_k ? "q" : "x", *const first_name = has_k ? "k" : "x";
     const at::Tensor &first = tensor(has_k ? args[1] : args[0], first_name);
@@ -226,6 +250,7 @@ PyObject *py_rotary_store(PyObject *, PyObject *const *args, Py_ssize_t n) {
     if (first.dim() != 3) fail(std::string(first_name) + " must be [N, heads, D], got " + shape_of(first.sizes()));
     const at::ScalarType type = first.scalar_type();
     kvc_rotary_args a = {};
+    kvc_scales scales = {};
     a.type = value_type(first, first_name);
     a.N = first.size(0); a.D = first.size(2);
     if (has_k) {
@@ -234,7 +259,9 @@ PyObject *py_rotary_store(PyObject *, PyObject *const *args, Py_ssize_t n) {
         const at::Tensor &pool = tensor(args[6], "kpages");
         if (pool.dim() != 4 || pool.size(2) != a.Hkv || pool.size(3) != a.D)
             fail("the pools must be [pages, page_size, " + std::to_string(a.Hkv) + ", " + std::to_string(a.D) + "], got " + shape_of(pool.sizes()));
-        const at::Tensor &kp = rows(args[6], pool.sizes(), type, "kpages", device), &vp = rows(args[7], pool.sizes(), type, "vpages", device);
+        at::ScalarType of_pool = type;
+        scales = scales_of(pool, args[13], args[14], of_pool, device);
+        const at::Tensor &kp = rows(args[6], pool.sizes(), of_pool, "kpages", device), &vp = rows(args[7], pool.sizes(), of_pool, "vpages", device);
         a.k = k.data_ptr(); a.k_token = k.stride(0); a.k_head = k.stride(1);
         a.v = v.data_ptr(); a.v_token = v.stride(0); a.v_head = v.stride(1);
         a.kpages = kp.data_ptr(); a.kp_page = kp.stride(0); a.kp_row = kp.stride(1); a.kp_head = kp.stride(2);
@@ -255,9 +282,13 @@ PyObject *py_rotary_store(PyObject *, PyObject *const *args, Py_ssize_t n) {
         a.rotary = 2 * pairs;
     }
     a.status = status_of(args[12], device);
+    const auto call = [&] {
+        if (scales.codes) launch(rotary_store_codes, a, device, "kvc_rotary_store_codes", static_cast<const kvc_scales *>(&scales));
+        else launch(rotary_store, a, device, "kvc_rotary_store");
+    };
     if (!has_q) {
-        launch(rotary_store, a, device, "kvc_rotary_store");
-        written({args[6], args[7]});
+        call();
+        written({args[6], args[7], args[13], args[14]});
         Py_RETURN_NONE;
     }
     const at::Tensor &q0 = tensor(args[0], q_name);
@@ -269,16 +300,94 @@ PyObject *py_rotary_store(PyObject *, PyObject *const *args, Py_ssize_t n) {
     const bool own = !given(args[11]);
     const at::Tensor out = own ? at::empty(q.sizes(), q.options()) : rows(args[11], q.sizes(), type, "out", device);
     a.q_out = out.data_ptr(); a.out_token = out.stride(0); a.out_head = out.stride(1);
-    launch(rotary_store, a, device, "kvc_rotary_store");
-    written({args[6], args[7], args[11]});
+    call();
+    written({args[6], args[7], args[11], args[13], args[14]});
     return own ? THPVariable_Wrap(out) : Py_NewRef(args[11]);
     END_HANDLE_TH_ERRORS
 }
 
-// q, kpages, vpages, table, lengths, scaling, window, out or None, return_lse, workspace, status, starts or None
+// table, lengths, page_size, tokens, status -> (slots, starts)
+PyObject *py_page_slots(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    count(n, 5);
+    const at::Tensor &lengths = tensor(args[1], "lengths");
+    const int device = device_of(lengths, "lengths");
+    kvc_page_slots_args a = {};
+    a.B = lengths.dim() == 1 ? lengths.size(0) : -1;
+    a.lengths = static_cast<int32_t *>(words(args[1], a.B, "lengths", device));
+    const Table table = table_of(args[0], a.B, device);
+    a.table = table.at; a.table_stride = table.stride; a.table_width = table.width;
+    a.page_size = number(args[2]);
+    a.tokens = number(args[3]);
+    if (a.tokens < 0) fail("tokens must not be negative, got " + std::to_string(a.tokens));
+    a.status = status_of(args[4], device);
+    const at::Tensor slots = ints(a.tokens, lengths), starts = ints(a.B + 1, lengths);
+    a.slots = int_at(slots); a.starts = int_at(starts);
+    launch(page_slots, a, device, "kvc_page_slots");
+    return tuple({slots, starts});
+    END_HANDLE_TH_ERRORS
+}
+
+// starts, first, positions: positions of each request's rows go up by first, in place
+PyObject *py_page_shift(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    count(n, 3);
+    const at::Tensor &first = tensor(args[1], "first"), &positions = tensor(args[2], "positions");
+    const int device = device_of(positions, "positions");
+    kvc_page_shift_args a = {};
+    a.B = first.dim() == 1 ? first.size(0) : -1;
+    a.tokens = positions.numel();
+    a.positions = static_cast<int32_t *>(words(args[2], a.tokens, "positions", device));
+    a.first = static_cast<int32_t *>(words(args[1], a.B, "first", device));
+    a.starts = static_cast<int32_t *>(words(args[0], a.B + 1, "starts", device));
+    launch(page_shift, a, device, "kvc_page_shift");
+    written({args[2]});
+    Py_RETURN_NONE;
+    END_HANDLE_TH_ERRORS
+}
+
+// kpages, vpages, slots, kscales or None, vscales or None, bfloat16 or not or None, out (two tensors) or None, status -> (k, v)
+PyObject *py_paged_rows(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    count(n, 8);
+    const at::Tensor &pool = tensor(args[0], "kpages"), &slots = tensor(args[2], "slots");
+    const int device = device_of(pool, "kpages");
+    if (pool.dim() != 4) fail("the pools must be [pages, page_size, Hkv, D], got " + shape_of(pool.sizes()));
+    kvc_paged_rows_args a = {};
+    at::ScalarType type = pool.scalar_type(), of_rows = type;
+    a.scales = scales_of(pool, args[3], args[4], type, device);
+    if (a.scales.codes) {
+        if (!given(args[5])) fail("dtype must be fp16 or bf16: codes are of neither");
+        of_rows = PyObject_IsTrue(args[5]) ? at::kBFloat16 : at::kHalf;
+    } else {
+        value_type(pool, "kpages");
+        if (given(args[5]) && (PyObject_IsTrue(args[5]) ? at::kBFloat16 : at::kHalf) != type) fail(std::string("dtype must be the pools', ") + c10::toString(type));
+    }
+    const at::Tensor &kp = rows(args[0], pool.sizes(), type, "kpages", device), &vp = rows(args[1], pool.sizes(), type, "vpages", device);
+    a.type = of_rows == at::kHalf ? KVC_TYPE_FP16 : KVC_TYPE_BF16;
+    a.N = slots.numel(); a.n_pages = pool.size(0); a.page_size = pool.size(1); a.Hkv = pool.size(2); a.D = pool.size(3);
+    a.slots = static_cast<int32_t *>(words(args[2], a.N, "slots", device));
+    a.kpages = kp.data_ptr(); a.kp_page = kp.stride(0); a.kp_row = kp.stride(1); a.kp_head = kp.stride(2);
+    a.vpages = vp.data_ptr(); a.vp_page = vp.stride(0); a.vp_row = vp.stride(1); a.vp_head = vp.stride(2);
+    a.status = status_of(args[7], device);
+    const int64_t shape[3] = {a.N, a.Hkv, a.D};
+    const bool own = !given(args[6]);
+    if (!own && (!PyTuple_Check(args[6]) || PyTuple_GET_SIZE(args[6]) != 2)) fail("out must be a tuple of two tensors");
+    const at::Tensor k = own ? at::empty(shape, pool.options().dtype(of_rows)) : rows(PyTuple_GET_ITEM(args[6], 0), shape, of_rows, "out[0]", device);
+    const at::Tensor v = own ? at::empty(shape, pool.options().dtype(of_rows)) : rows(PyTuple_GET_ITEM(args[6], 1), shape, of_rows, "out[1]", device);
+    a.k_out = k.data_ptr(); a.k_token = k.stride(0); a.k_head = k.stride(1);
+    a.v_out = v.data_ptr(); a.v_token = v.stride(0); a.v_head = v.stride(1);
+    launch(paged_rows, a, device, "kvc_paged_rows");
+    if (own) return tuple({k, v});
+    written({PyTuple_GET_ITEM(args[6], 0), PyTuple_GET_ITEM(args[6], 1)});
+    return Py_NewRef(args[6]);
+    END_HANDLE_TH_ERRORS
+}
+
+// q, kpages, vpages, table, lengths, scaling, window, out or None, return_lse, workspace, status, starts or None, kscales or None, vscales or None
 PyObject *py_paged_attn(PyObject *, PyObject *const *args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    count(n, 12);
+    count(n, 14);
     const at::Tensor &q0 = tensor(args[0], "q"), &pool = tensor(args[1], "kpages");
     const int device = device_of(q0, "q");
     kvc_paged_attn_args a = {};
@@ -286,7 +395,9 @@ PyObject *py_paged_attn(PyObject *, PyObject *const *args, Py_ssize_t n) {
     const at::ScalarType type = q0.scalar_type();
     if (q0.dim() != 3 || pool.dim() != 4 || pool.size(3) != q0.size(2))
         fail("q must be [B, Hq, D], the pools [pages, page_size, Hkv, D], got " + shape_of(q0.sizes()) + " and " + shape_of(pool.sizes()));
-    const at::Tensor &q = rows(args[0], q0.sizes(), type, "q", device), &kp = rows(args[1], pool.sizes(), type, "kpages", device), &vp = rows(args[2], pool.sizes(), type, "vpages", device);
+    at::ScalarType of_pool = type;
+    const kvc_scales scales = scales_of(pool, args[12], args[13], of_pool, device);
+    const at::Tensor &q = rows(args[0], q0.sizes(), type, "q", device), &kp = rows(args[1], pool.sizes(), of_pool, "kpages", device), &vp = rows(args[2], pool.sizes(), of_pool, "vpages", device);
     const bool by_row = given(args[11]);
     const at::Tensor &lengths = tensor(args[4], "lengths");
     a.B = !by_row ? q.size(0) : lengths.dim() == 1 ? lengths.size(0) : -1;
@@ -312,7 +423,9 @@ PyObject *py_paged_attn(PyObject *, PyObject *const *args, Py_ssize_t n) {
         lse = at::empty({q.size(0), a.Hq}, q.options().dtype(at::kFloat));
         a.lse = static_cast<float *>(lse.data_ptr());
     }
-    if (by_row) launch(paged_attn_rows, a, device, "kvc_paged_attn_rows", static_cast<const int32_t *>(words(args[11], a.B + 1, "starts", device)), q.size(0));
+    if (scales.codes)
+        launch(paged_attn_codes, a, device, "kvc_paged_attn_codes", &scales, by_row ? static_cast<const int32_t *>(words(args[11], a.B + 1, "starts", device)) : nullptr, q.size(0));
+    else if (by_row) launch(paged_attn_rows, a, device, "kvc_paged_attn_rows", static_cast<const int32_t *>(words(args[11], a.B + 1, "starts", device)), q.size(0));
     else launch(paged_attn, a, device, "kvc_paged_attn");
     written({args[7]});
     PyObject *const result = own ? THPVariable_Wrap(out) : Py_NewRef(args[7]);
@@ -341,7 +454,7 @@ PyObject *py_stream_of(PyObject *, PyObject *const *args, Py_ssize_t n) {
 // the error's class and the addresses of the library's entries
 PyObject *py_init(PyObject *, PyObject *const *args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    count(n, 7);
+    count(n, 12);
     error_class = Py_NewRef(args[0]);
     auto address = [&](int i) { return reinterpret_cast<void *>(static_cast<uintptr_t>(number(args[i]))); };
     page_plan = reinterpret_cast<decltype(page_plan)>(address(1));
@@ -350,6 +463,11 @@ PyObject *py_init(PyObject *, PyObject *const *args, Py_ssize_t n) {
     paged_attn = reinterpret_cast<decltype(paged_attn)>(address(4));
     paged_attn_rows = reinterpret_cast<decltype(paged_attn_rows)>(address(5));
     last_error = reinterpret_cast<decltype(last_error)>(address(6));
+    rotary_store_codes = reinterpret_cast<decltype(rotary_store_codes)>(address(7));
+    page_slots = reinterpret_cast<decltype(page_slots)>(address(8));
+    page_shift = reinterpret_cast<decltype(page_shift)>(address(9));
+    paged_rows = reinterpret_cast<decltype(paged_rows)>(address(10));
+    paged_attn_codes = reinterpret_cast<decltype(paged_attn_codes)>(address(11));
     Py_RETURN_NONE;
     END_HANDLE_TH_ERRORS
 }
@@ -361,6 +479,9 @@ PyMethodDef methods[] = {{"init", fast<py_init>(), METH_FASTCALL, nullptr},
                          {"page_release", fast<py_page_release>(), METH_FASTCALL, nullptr},
                          {"rotary_store", fast<py_rotary_store>(), METH_FASTCALL, nullptr},
                          {"paged_attn", fast<py_paged_attn>(), METH_FASTCALL, nullptr},
+                         {"page_slots", fast<py_page_slots>(), METH_FASTCALL, nullptr},
+                         {"page_shift", fast<py_page_shift>(), METH_FASTCALL, nullptr},
+                         {"paged_rows", fast<py_paged_rows>(), METH_FASTCALL, nullptr},
                          {"stream_of", fast<py_stream_of>(), METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "kvc_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

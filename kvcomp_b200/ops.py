@@ -770,17 +770,40 @@ def rotary(x, positions, frequencies, layout="half", factor=1.0, inverse=False, 
         if out is not None:
             raise KvcError("rotary: out carries no gradient, and x requires one")
         return _Rotary.apply(x, positions, frequencies, layout, factor, inverse)
-    return _lib.torch_calls().rotary_store(x, None, None, positions, None, frequencies, None, None, _LAYOUTS.get(layout), factor, inverse, out, None)
+    return _lib.torch_calls().rotary_store(x, None, None, positions, None, frequencies, None, None, _LAYOUTS.get(layout), factor, inverse, out, None,
+                                           None, None)
 
 
-def rotary_paged_store(q, k, v, positions, slots, frequencies, kpages, vpages, layout="half", factor=1.0, out=None, status=None):
+def rotary_paged_store(q, k, v, positions, slots, frequencies, kpages, vpages, layout="half", factor=1.0, out=None, status=None, kscales=None, vscales=None):
     """A step's tokens: q [N, Hq, D] rotated (returned; out may be q, q may be None), k [N, Hkv, D] rotated into and v copied into the rows `slots`
     (int32[N], page * page_size + row; below 0: not stored) of the pools [pages, page_size, Hkv, D].  fp16 or bf16, any strides but a contiguous last
     dimension.  positions, frequencies, layout, factor: as for rotary; frequencies None: nothing is rotated.  Tokens of one call have slots of their own.
-    Outputs and pools must not overlap (views of one tensor that lie in one another are fine).  For serving: no gradient goes through it."""
+    Outputs and pools must not overlap (views of one tensor that lie in one another are fine).  For serving: no gradient goes through it.
+    kscales, vscales (fp32 [pages, Hkv, page_size], last dimension contiguous): the pools hold 8-bit codes, torch.int8 or torch.float8_e4m3fn, and a token's row of a head has one scale:
+    int8 max |x| / 127, e4m3 the least power of two with max |x| / scale <= 448, none below 2^-100; a row that holds an infinity or no number has the scale NaN.  D is a multiple of 16 then."""
     if k is None:
         raise KvcError("k must be a tensor")
-    return _lib.torch_calls().rotary_store(q, k, v, positions, slots, frequencies, kpages, vpages, _LAYOUTS.get(layout), factor, False, out, status)
+    return _lib.torch_calls().rotary_store(q, k, v, positions, slots, frequencies, kpages, vpages, _LAYOUTS.get(layout), factor, False, out, status, kscales, vscales)
+
+
+def page_slots(table, lengths, page_size, tokens, status=None):
+    """The slots (page * page_size + row) of all tokens that requests have, packed request by request: (slots int32[tokens], starts int32[B + 1], the requests' first rows).  tokens: at
+    least sum(lengths); rows behind the last have slot -1.  For paged_rows, of all layers."""
+    return _lib.torch_calls().page_slots(table, lengths, page_size, tokens, status)
+
+
+def page_shift(starts, first, positions):
+    """positions[row] += first[b] for the rows of each request b, in place: a plan's positions where requests follow prefixes of first[b] tokens (int32[B])."""
+    _lib.torch_calls().page_shift(starts, first, positions)
+
+
+def paged_rows(kpages, vpages, slots, kscales=None, vscales=None, dtype=None, out=None, status=None):
+    """(k, v): the rows `slots` (int32[N], page * page_size + row; below 0: zeros) of the pools [pages, page_size, Hkv, D] as [N, Hkv, D], fp16 or bf16.  Of codes (kscales, vscales, dtype
+    given) codes times scales in fp32, rounded once.  out: the two tensors to write, any strides but a contiguous last dimension, rows on 16 bytes.  D is a multiple of 16.  For a prompt in
+    chunks: its keys and values so far, in a row.  For serving: no gradient goes through it."""
+    if dtype not in (None, torch.float16, torch.bfloat16):
+        raise KvcError("dtype must be fp16 or bf16, got %s" % (dtype,))
+    return _lib.torch_calls().paged_rows(kpages, vpages, slots, kscales, vscales, None if dtype is None else dtype == torch.bfloat16, None if out is None else tuple(out), status)
 
 
 def paged_attn_workspace(B, Hq, Hkv, D, device):
@@ -796,15 +819,16 @@ def paged_attn_workspace(B, Hq, Hkv, D, device):
     return workspace
 
 
-def paged_attn(q, kpages, vpages, table, lengths, scaling, window=0, out=None, return_lse=False, workspace=None, status=None, starts=None):
+def paged_attn(q, kpages, vpages, table, lengths, scaling, window=0, out=None, return_lse=False, workspace=None, status=None, starts=None, kscales=None, vscales=None):
     """One new token per request: q fp16 or bf16 [B, Hq, D] -> out [B, Hq, D] = softmax(scaling * q . k) v over the lengths[b] (int32[B]) tokens that the
     request has in the pages table[b] (int32 [B, pages]) of the pools [pages, page_size, Hkv, D]; window > 0: over the last `window` of them.  Requests
     without tokens: 0.  return_lse: (out, fp32 [B, Hq] log of the sum of exponentials, -inf without tokens).  D: 64, 96, 128, 256.
     workspace: paged_attn_workspace's, for one call at a time; None: one is made, and cleared, for this call.  For serving: no gradient goes through it.
     starts (int32[B + 1], a plan's): q and out have a row for each token of a step, request b's at starts[b]; requests without one are left out, rows that are nobody's
-    are 0, and so are those of a request that has more than one (FLAG_BAD_LENGTH)."""
+    are 0, and so are those of a request that has more than one (FLAG_BAD_LENGTH).
+    kscales, vscales: the pools hold codes (rotary_paged_store), keys and values with the same strides."""
     if workspace is None:
         if not isinstance(q, torch.Tensor) or not q.is_cuda or q.dim() != 3 or not isinstance(kpages, torch.Tensor) or kpages.dim() != 4:
             raise KvcError("q must be a CUDA tensor [B, Hq, D], the pools [pages, page_size, Hkv, D] (kvcomp_b200 has no CPU path)")
         workspace = paged_attn_workspace(q.shape[0], q.shape[1], kpages.shape[2], q.shape[2], q.device)
-    return _lib.torch_calls().paged_attn(q, kpages, vpages, table, lengths, scaling, window, out, return_lse, workspace, status, starts)
+    return _lib.torch_calls().paged_attn(q, kpages, vpages, table, lengths, scaling, window, out, return_lse, workspace, status, starts, kscales, vscales)
