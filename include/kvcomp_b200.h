@@ -528,6 +528,24 @@ int kvc_paged_rows(const kvc_paged_rows_args *args, kvc_stream_t stream);
  * arrays of scales too.  type: of q and out.  The same workspace. */
 int kvc_paged_attn_codes(const kvc_paged_attn_args *args, const kvc_scales *scales, const int32_t *starts, int64_t rows, kvc_stream_t stream);
 
+/* Requests that continue a common prefix.  parents[b] is the request whose first shared[b] tokens come before b's own (below 0: none); requests with the same two numbers are a group.  plan:
+ * kvc_prefix_plan_words(B) words; it holds as long as parents and shared do.  Whoever is followed follows no one: what it follows is not seen by its followers (KVC_FLAG_BAD_LENGTH, as for a
+ * parent that is no request, or the request itself, and a negative length: none are followed then).  B is at most 16384. */
+typedef struct {
+    const int32_t *parents, *shared;
+    int64_t B;
+    int32_t *plan;
+    int32_t *status;
+} kvc_prefix_plan_args;
+int64_t kvc_prefix_plan_words(int64_t B);
+int kvc_prefix_plan(const kvc_prefix_plan_args *args, kvc_stream_t stream);
+
+/* kvc_paged_attn (starts null) or kvc_paged_attn_rows over prefix and own tokens: lengths and the block table are of own tokens, a request's prefix are the first shared tokens (of those
+ * that it has: KVC_FLAG_BAD_LENGTH if it has fewer) of its parent, whose pages are read once for the whole group.  D is 64, 96 or 128, window 0.  workspace: kvc_paged_attn_shared_workspace()
+ * bytes, not cleared; it serves one call at a time.  An infinite value that counts may give no number where its weight is 0 in 16 bits. */
+int64_t kvc_paged_attn_shared_workspace(int64_t B, int64_t Hq, int64_t Hkv, int64_t D);
+int kvc_paged_attn_shared(const kvc_paged_attn_args *args, const int32_t *plan, const int32_t *starts, int64_t rows, kvc_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -59,6 +59,7 @@ PAGED_ATTN_ARGS = struct.Struct("<29qfi")
 SCALES = struct.Struct("<6q2i")
 PAGE_SLOTS_ARGS = struct.Struct("<10q")
 PAGE_SHIFT_ARGS = struct.Struct("<5q")
+PREFIX_PLAN_ARGS = struct.Struct("<5q")
 PAGED_ROWS_ARGS = struct.Struct("<2q6q2i19q2i")
 
 ROTARY_HALF, ROTARY_INTERLEAVED = 0, 1
@@ -128,6 +129,10 @@ _SIGNATURES = {
     "kvc_page_shift": (_i32, [C.c_char_p, _vp]),
     "kvc_paged_rows": (_i32, [C.c_char_p, _vp]),
     "kvc_paged_attn_codes": (_i32, [C.c_char_p, C.c_char_p, _vp, _i64, _vp]),
+    "kvc_prefix_plan_words": (_i64, [_i64]),
+    "kvc_prefix_plan": (_i32, [C.c_char_p, _vp]),
+    "kvc_paged_attn_shared_workspace": (_i64, [_i64, _i64, _i64, _i64]),
+    "kvc_paged_attn_shared": (_i32, [C.c_char_p, _vp, _vp, _i64, _vp]),
     "kvc_k_matvec": (_i32, [_vp, _vp, _vp, _i64, _i64, _vp]),
 }
 
@@ -178,7 +183,8 @@ def torch_calls():
     lib = load()
     module.init(KvcError, *(C.cast(getattr(lib, name), C.c_void_p).value
                             for name in ("kvc_page_plan", "kvc_page_release", "kvc_rotary_store", "kvc_paged_attn", "kvc_paged_attn_rows", "kvc_last_error",
-                                         "kvc_rotary_store_codes", "kvc_page_slots", "kvc_page_shift", "kvc_paged_rows", "kvc_paged_attn_codes")))
+                                         "kvc_rotary_store_codes", "kvc_page_slots", "kvc_page_shift", "kvc_paged_rows", "kvc_paged_attn_codes", "kvc_prefix_plan_words", "kvc_prefix_plan",
+                                         "kvc_paged_attn_shared")))
     _torch_calls = module
     return module
 

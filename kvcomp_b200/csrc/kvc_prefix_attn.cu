@@ -1,0 +1,775 @@
+// Attention of one new token per request where requests continue a common prefix: the prefix is read once for all that follow it.
+//
+// out = sum_t w_t v_t / sum_t w_t with w_t = exp(scaling q . k_t - m), over the tokens of the prefix and the request's own ones.  The sums of both, and of any parts of them, are kept
+// with their maxima and joined: the tokens are a prefix's, times all queries that follow it, or a request's own, times its queries.
+//
+// What bounds it: of n requests with g query heads on a KV head, n g rows meet every key and value of the prefix, 4 n g D operations for 4 D bytes: HBM up to some 250 rows, the tensor
+// cores and the exponentials beyond.  mma.sync (what the attention without prefixes uses, at 8 rows) gives a quarter of that; so here tcgen05: 128 rows by 128 tokens, the scores in tensor
+// memory, the weights in 16 bits beside them as the second product's operand, the sums there too.  Two sets of 128 rows take turns: while the exponentials of one are made the other's
+// products run.  Columns of more than 128 rows use both sets with the same tokens; columns of fewer give them every other tile.
+//
+// Work is cut into tiles of 128 tokens of a column (an item's KV head and up to 256 of its rows; an item is a prefix or a request's own tokens), all tiles of all columns in one row; each CTA, one
+// on an SM, takes an equal, contiguous share, found from the lengths in the kernel.  What a CTA finds for a column goes to the workspace; a second kernel joins the
+// parts, in the order of the shares, so that results do not depend on timing.
+//
+// Keys and values come by 16-byte asynchronous copies (pages end anywhere, any strides) into a ring in shared memory, in the 128-byte swizzled layout that the products read: keys
+// channel by channel, values as they lie (token by token: the product's second operand turned).  Rounding: the weights are fp16 (times 2^7: 2^-21 of the largest are still normal numbers) or bf16,
+// the sums of weights are taken before that; everything joined is 32 bits and the result is rounded once.
+#include <math_constants.h>
+#include <string.h>
+
+#include <algorithm>
+
+#include "kvc_paged.cuh"
+
+namespace {
+
+constexpr int THREADS = 384, ROWS = 128, TOKENS = 128, ATOM = 16384;       // ATOM: 128 rows of 128 bytes
+constexpr int MASKS = 16;
+constexpr int MAX_REQUESTS = 16384;
+
+// places in a plan of B requests
+__host__ __device__ constexpr int64_t plan_first(int64_t) { return 1; }                    // groups' first members [B + 1]
+__host__ __device__ constexpr int64_t plan_parent(int64_t B) { return B + 2; }             // a group's prefix: whose it is, how long [B] each
+__host__ __device__ constexpr int64_t plan_shared(int64_t B) { return 2 * B + 2; }
+__host__ __device__ constexpr int64_t plan_order(int64_t B) { return 3 * B + 2; }          // members, group by group [B]
+__host__ __device__ constexpr int64_t plan_group(int64_t B) { return 4 * B + 2; }          // a request's group (-1: none) and its place there [B] each
+__host__ __device__ constexpr int64_t plan_rank(int64_t B) { return 5 * B + 2; }
+__host__ __device__ constexpr int64_t plan_leader(int64_t B) { return 6 * B + 2; }         // scratch: the first of those with the same prefix, their number [B] each
+__host__ __device__ constexpr int64_t plan_count(int64_t B) { return 7 * B + 2; }
+__host__ __device__ constexpr int64_t plan_words(int64_t B) { return 8 * B + 2; }
+
+// ---- the plan: requests with the same prefix become a group ---------------------------------------------------------
+
+constexpr int FIND_THREADS = 256, SCAN_THREADS = 1024;
+
+struct Wish { int parent, shared; };
+__device__ __forceinline__ Wish wish_of(const kvc_prefix_plan_args &a, int b, int &flags) {
+    Wish w = {a.parents[b], a.shared[b]};
+    if (w.parent < 0) return {-1, 0};
+    if (w.parent >= a.B || w.parent == b || w.shared < 0) { flags |= KVC_FLAG_BAD_LENGTH; return {-1, 0}; }
+    return w;
+}
+
+// For each request the first with the same prefix, how many of these are before it and how many there are: all are looked at, which for 1024 requests takes a few us and is done when
+// requests come, not for every step.
+__global__ void __launch_bounds__(FIND_THREADS) prefix_find_kernel(const __grid_constant__ kvc_prefix_plan_args a) {
+    __shared__ Wish wishes[FIND_THREADS];
+    kvc_behind();
+    const int B = (int)a.B, b = blockIdx.x * FIND_THREADS + threadIdx.x;
+    int flags = 0, ignored = 0;
+    const Wish mine = b < B ? wish_of(a, b, flags) : Wish{-1, 0};
+    if (mine.parent >= 0 && a.parents[mine.parent] >= 0) flags |= KVC_FLAG_BAD_LENGTH;     // who is followed follows no one
+    int leader = -1, rank = 0, count = 0;
+    for (int first = 0; first < B; first += FIND_THREADS) {
+        __syncthreads();
+        wishes[threadIdx.x] = first + (int)threadIdx.x < B ? wish_of(a, first + threadIdx.x, ignored) : Wish{-1, 0};
+        __syncthreads();
+        const int n = min(FIND_THREADS, B - first);
+        for (int i = 0; i < n; i++) {
+            if (wishes[i].parent != mine.parent || wishes[i].shared != mine.shared) continue;
+            if (leader < 0) leader = first + i;
+            rank += first + i < b;
+            count++;
+        }
+    }
+    if (b < B) {
+        a.plan[plan_leader(B) + b] = mine.parent < 0 ? -1 : leader;
+        a.plan[plan_rank(B) + b] = rank;
+        a.plan[plan_count(B) + b] = count;
+    }
+    raise_flag(a.status, flags);
+}
+
+__global__ void __launch_bounds__(SCAN_THREADS) prefix_scan_kernel(const __grid_constant__ kvc_prefix_plan_args a) {
+    __shared__ int2 warps[SCAN_THREADS / 32];
+    __shared__ int2 before_s;
+    kvc_behind();
+    const int B = (int)a.B, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int ignored = 0;
+    if (threadIdx.x == 0) before_s = make_int2(0, 0);
+    for (int b0 = 0; b0 < B; b0 += SCAN_THREADS) {
+        const int b = b0 + threadIdx.x;
+        const bool leads = b < B && a.plan[plan_leader(B) + b] == b;
+        const int count = leads ? a.plan[plan_count(B) + b] : 0;
+        int2 sum = make_int2(leads, count);
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, sum.x, o), y = __shfl_up_sync(0xffffffffu, sum.y, o);
+            if (lane >= o) { sum.x += x; sum.y += y; }
+        }
+        if (lane == 31) warps[warp] = sum;
+        __syncthreads();
+        int2 before = before_s;
+        for (int w = 0; w < warp; w++) { before.x += warps[w].x; before.y += warps[w].y; }
+        const int group = before.x + sum.x - leads, first = before.y + sum.y - count;
+        if (leads) {
+            const Wish w = wish_of(a, b, ignored);
+            a.plan[plan_first(B) + group] = first;
+            a.plan[plan_parent(B) + group] = w.parent;
+            a.plan[plan_shared(B) + group] = w.shared;
+            a.plan[plan_group(B) + b] = group;
+        }
+        __syncthreads();
+        if (threadIdx.x == SCAN_THREADS - 1) before_s = make_int2(before.x + sum.x, before.y + sum.y);
+        __syncthreads();
+    }
+    const int2 all = before_s;
+    if (threadIdx.x == 0) {
+        a.plan[0] = all.x;
+        a.plan[plan_first(B) + all.x] = all.y;
+    }
+    __syncthreads();
+    for (int b = threadIdx.x; b < B; b += SCAN_THREADS) {
+        const int leader = a.plan[plan_leader(B) + b];
+        if (leader < 0) { a.plan[plan_group(B) + b] = -1; continue; }
+        const int group = a.plan[plan_group(B) + leader];                    // (written by this CTA ahead of a barrier)
+        if (leader != b) a.plan[plan_group(B) + b] = group;
+        a.plan[plan_order(B) + a.plan[plan_first(B) + group] + a.plan[plan_rank(B) + b]] = b;
+    }
+}
+
+// ---- the attention --------------------------------------------------------------------------------------------------
+
+struct Params {
+    kvc_paged_attn_args a;
+    const int32_t *plan, *starts;                           // starts null: row b is request b's
+    kvc_div page, group;                                    // divisors: page size, query heads of a KV head
+    int g, rows, most_tokens, grid;                         // query heads of a KV head, rows of q, tokens of a table row, CTAs
+    unsigned n_pages;
+    int negative;
+    float log2_scaling;
+    int32_t *item_first, *share;                            // (workspace) the items' first tiles, and the tiles of a share
+    float *sums;                                            // (workspace) of places of D floats
+    float2 *maxima;                                         // maximum and sum of weights of a place
+};
+
+// Places: of column parts that begin with the column [prefix or own][request][head][2]; behind them of those that begin with a CTA's share [CTA][256].
+__device__ __forceinline__ long long place_of(const Params &p, bool own, int b, int h, int i) { return (((own ? p.a.B : 0) + b) * p.a.Hq + h) * 2 + i; }
+__device__ __forceinline__ long long cta_place(const Params &p, int cta, int i) { return p.a.B * p.a.Hq * 4 + (long long)cta * 256 + i; }
+
+__device__ __forceinline__ int row_at(const Params &p, int b) { return p.starts ? min(max(p.starts[b], 0), p.rows) : b; }
+__device__ __forceinline__ int member_at(const Params &p, int i) { return min(max(p.plan[plan_order(p.a.B) + i], 0), (int)p.a.B - 1); }
+// the row of a request's token, -1: it has none, or more than one
+__device__ __forceinline__ int row_of(const Params &p, int b) {
+    if (!p.starts) return b;
+    const int row = row_at(p, b);
+    return row_at(p, b + 1) - row == 1 ? row : -1;
+}
+__device__ __forceinline__ int length_of(const Params &p, int b) { return min(max(p.a.lengths[b], 0), p.most_tokens); }
+
+struct Item { int table, first, rows, len, tiles, parts; };  // whose pages, the first member in the order (or the request itself), rows of a KV head, tokens, tiles of a column, columns of a KV head
+__device__ __forceinline__ Item item_of(const Params &p, int i, int groups) {
+    Item r;
+    const int B = (int)p.a.B;
+    if (i < groups) {
+        r.first = min(max(p.plan[plan_first(B) + i], 0), B);               // (kept inside the arrays whatever the plan holds, as lengths are)
+        r.rows = min(max(p.plan[plan_first(B) + i + 1] - r.first, 0), B - r.first) * p.g;
+        r.table = min(max(p.plan[plan_parent(B) + i], 0), B - 1);
+        r.len = r.rows == 0 ? 0 : min(max(p.plan[plan_shared(B) + i], 0), length_of(p, r.table));
+    } else {
+        r.first = r.table = i - groups;
+        r.rows = p.g;
+        r.len = row_of(p, r.table) >= 0 ? length_of(p, r.table) : 0;
+    }
+    r.tiles = (r.len + TOKENS - 1) / TOKENS;
+    r.parts = (r.rows + 2 * ROWS - 1) / (2 * ROWS);
+    return r;
+}
+
+// A CTA's way through its share, tile by tile; the same for all its warps.
+struct Walk {
+    int item, column, tile, left;                           // left: tiles of the share
+    int of_column, in_part;                                 // (of the column's part in this share) its first tile, how many tiles it has
+    int first_job, jobs;                                    // its first job, those before this tile's
+    int k_head, part;
+    Item it;
+    bool wide;
+};
+__device__ __forceinline__ void begin_column(Walk &w) {
+    w.k_head = w.column / w.it.parts;
+    w.part = w.column - w.k_head * w.it.parts;
+    w.wide = w.it.rows - w.part * 2 * ROWS > ROWS;
+    w.of_column = w.tile;
+    w.in_part = min(w.it.tiles - w.tile, w.left);
+    w.first_job = w.jobs;
+}
+__device__ __forceinline__ void next_tile(const Params &p, Walk &w, int groups) {
+    w.jobs += w.wide ? 2 : 1;
+    if (--w.left == 0) return;
+    if (++w.tile < w.it.tiles) return;
+    w.tile = 0;
+    if (++w.column == w.it.parts * (int)p.a.Hkv) {
+        w.column = 0;
+        const int items = groups + (int)p.a.B;
+        do {
+            if (++w.item >= items) { w.left = 0; return; }      // (lengths that changed meanwhile)
+            w.it = item_of(p, w.item, groups);
+        } while (w.it.tiles == 0);
+    }
+    begin_column(w);
+}
+
+// ---- what the hardware is asked for
+__device__ __forceinline__ uint32_t shared_at(const void *v) { return (uint32_t)__cvta_generic_to_shared(v); }
+__device__ __forceinline__ void bar_init(uint64_t *bar, int count) { asm volatile("mbarrier.init.shared.b64 [%0], %1;" ::"r"(shared_at(bar)), "r"(count)); }
+__device__ __forceinline__ void bar_arrive(uint64_t *bar) { asm volatile("mbarrier.arrive.shared.b64 _, [%0];" ::"r"(shared_at(bar)) : "memory"); }
+__device__ __forceinline__ bool bar_try(uint64_t *bar, uint32_t parity, uint32_t ns) {
+    uint32_t done;
+    asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared.b64 p, [%1], %2, %3; selp.u32 %0, 1, 0, p; }" : "=r"(done) : "r"(shared_at(bar)), "r"(parity), "r"(ns) : "memory");
+    return done;
+}
+// Waits up to about a second; what runs out is said in *failed, and nothing waits any more then.
+__device__ __forceinline__ void bar_wait(uint64_t *bar, uint32_t parity, volatile int *failed) {
+    for (int n = 0; n < 1 << 20; n++) {
+        if (bar_try(bar, parity, 1000)) return;
+        if (*failed) return;
+    }
+    *failed = 1;
+}
+__device__ __forceinline__ void copy16(uint32_t to, const void *from, bool on) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(on ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void seen_by_products() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void commit_to(uint64_t *bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(shared_at(bar)) : "memory");
+}
+// operands in shared memory, 128-byte swizzle: of 1024-byte pieces (8 rows) that follow one another; `other` bytes to the next 64 channels where rows are not what is summed over
+__device__ __forceinline__ uint64_t operand_at(uint32_t at, uint32_t other) {
+    return (uint64_t)((at & 0x3ffff) >> 4) | (uint64_t)(other >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | 1ull << 46 | 2ull << 61;
+}
+__device__ __forceinline__ void product(uint32_t d, uint64_t a, uint64_t b, uint32_t kind, bool add) {
+    asm volatile("{ .reg .pred p; setp.ne.u32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }" ::"r"(d), "l"(a), "l"(b), "r"(kind), "r"((uint32_t)add) : "memory");
+}
+__device__ __forceinline__ void product_of_weights(uint32_t d, uint32_t a, uint64_t b, uint32_t kind, bool add) {
+    asm volatile("{ .reg .pred p; setp.ne.u32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(d), "r"(a), "l"(b), "r"(kind), "r"((uint32_t)add) : "memory");
+}
+#define KVC_32(X) X(0), X(1), X(2), X(3), X(4), X(5), X(6), X(7), X(8), X(9), X(10), X(11), X(12), X(13), X(14), X(15), X(16), X(17), X(18), X(19), X(20), X(21), X(22), X(23), X(24), X(25), X(26), X(27), X(28), X(29), X(30), X(31)
+__device__ __forceinline__ void load32(uint32_t *r, uint32_t at) {
+#define KVC_OUT(i) "=r"(r[i])
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, "
+                 "%28, %29, %30, %31}, [%32];" : KVC_32(KVC_OUT) : "r"(at));
+#undef KVC_OUT
+}
+__device__ __forceinline__ void store32(uint32_t at, const uint32_t *r) {
+#define KVC_IN(i) "r"(r[i])
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, "
+                 "%28, %29, %30, %31};" ::KVC_32(KVC_IN), "r"(at) : "memory");
+#undef KVC_IN
+}
+__device__ __forceinline__ void loads_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void stores_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ float exp2_approx(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+template <typename T> struct Weight;
+template <> struct Weight<__half> { static constexpr float LIFT = 7.0f; static constexpr uint32_t KIND = 0; };
+template <> struct Weight<__nv_bfloat16> { static constexpr float LIFT = 0.0f; static constexpr uint32_t KIND = 1; };
+constexpr float SLACK = 8.0f;                               // the maximum that weights go by is put up when it is 2^8 too low: the sums are touched once or twice a column, not every tile
+
+template <int D> struct Shape {
+    static constexpr int ATOMS = (D + 63) / 64, UNIT = ATOMS * ATOM, RING = ATOMS == 1 ? 10 : 5;      // a tile of keys or values; how many lie in the ring
+    static constexpr size_t SHARED = (size_t)(2 + RING) * UNIT + 1024;
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(THREADS, 1) prefix_attn_kernel(const __grid_constant__ Params p) {
+    constexpr int ATOMS = Shape<D>::ATOMS, UNIT = Shape<D>::UNIT, RING = Shape<D>::RING;
+    constexpr float LIFT = Weight<T>::LIFT;
+    extern __shared__ uint8_t raw[];
+    __shared__ __align__(8) uint64_t full[RING], empty[RING], scores_there[2], weights_there[2], sums_there[2], queries_free[2];
+    __shared__ uint32_t masks[MASKS][4], tensor_s;
+    __shared__ int failed_s, warp_sums[THREADS / 32], start_item, start_rest;
+    const kvc_paged_attn_args &a = p.a;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, B = (int)a.B;
+    volatile int *failed = &failed_s;
+    const uint32_t base = (shared_at(raw) + 1023) & ~1023u, ring = base + 2 * UNIT;
+
+    if (warp == 8) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(shared_at(&tensor_s)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    if (tid == 0) {
+        for (int i = 0; i < RING; i++) { bar_init(full + i, 1); bar_init(empty + i, 1); }
+        for (int i = 0; i < 2; i++) { bar_init(scores_there + i, 1); bar_init(weights_there + i, 4); bar_init(sums_there + i, 1); bar_init(queries_free + i, 1); }
+        failed_s = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+
+    // ---- this CTA's share
+    const int groups = min(max(p.plan[0], 0), B), items = groups + B;
+    int flags = 0, total = 0;
+    auto scan = [&](int i0, int &tiles) {                   // (first tile of item i0 + tid, its tiles; `total` grows)
+        Item it = {};
+        if (i0 + tid < items) it = item_of(p, i0 + tid, groups);
+        tiles = it.tiles * it.parts * (int)a.Hkv;
+        int sum = tiles;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += x;
+        }
+        __syncthreads();
+        if (lane == 31) warp_sums[warp] = sum;
+        __syncthreads();
+        int before = total;
+        for (int w = 0; w < THREADS / 32; w++) {
+            if (w < warp) before += warp_sums[w];
+            total += warp_sums[w];
+        }
+        return before + sum - tiles;
+    };
+    int tiles = 0, first = 0;
+    for (int i0 = 0; i0 < items; i0 += THREADS) {
+        first = scan(i0, tiles);
+        if (blockIdx.x == 0 && i0 + tid < items) p.item_first[i0 + tid] = first;
+    }
+    const int all = total, size = max(1, (all + p.grid - 1) / p.grid), r0 = (int)min((long long)all, (long long)size * blockIdx.x), r1 = min(all, r0 + size);
+    if (blockIdx.x == 0 && tid == 0) *p.share = size;
+    if (r0 < r1) {
+        if (items > THREADS) total = 0;
+        for (int i0 = 0; i0 < items; i0 += THREADS) {
+            if (items > THREADS) first = scan(i0, tiles);
+            if (r0 >= first && r0 < first + tiles) { start_item = i0 + tid; start_rest = r0 - first; }
+        }
+    }
+    if (blockIdx.x == gridDim.x - 1) {                      // lengths and rows that are none
+        for (int b = tid; b < B; b += THREADS) {
+            if (a.lengths[b] < 0 || a.lengths[b] > p.most_tokens || (p.starts && row_at(p, b + 1) - row_at(p, b) > 1)) flags |= KVC_FLAG_BAD_LENGTH;
+            const int group = p.plan[plan_group(B) + b];
+            if (group >= 0 && group < groups && item_of(p, group, groups).len < p.plan[plan_shared(B) + group]) flags |= KVC_FLAG_BAD_LENGTH;
+        }
+    }
+    before_sync();
+    __syncthreads();
+    after_sync();
+    const uint32_t tensor = tensor_s;
+
+    if (r0 < r1) {
+        Walk w;
+        w.left = r1 - r0;
+        w.jobs = 0;
+        w.item = start_item;
+        w.it = item_of(p, w.item, groups);
+        w.column = start_rest / w.it.tiles;
+        w.tile = start_rest - w.column * w.it.tiles;
+        begin_column(w);
+
+        if (warp < 8) {
+            asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+            // ---- a set of rows: scores -> weights, and the sums' way out
+            const int set = warp >> 2, r = tid & 127;
+            const uint32_t lanes = (uint32_t)(warp & 3) << 21, scores = tensor + lanes + set * 128, sums = tensor + lanes + 256 + set * 128;
+            float m = -CUDART_INF_F, l = 0.0f;
+            int n_set = 0, tile_n = 0;                      // jobs of this set, tiles
+            bool mine = false;
+            float *to = nullptr;
+            float2 *to_max = nullptr;
+            for (; w.left > 0; next_tile(p, w, groups), tile_n++) {
+                const int idx = (set - w.jobs) & 1;         // which of the tile's jobs is this set's
+                if (!w.wide && idx != 0) continue;
+                const int half = w.wide ? idx : 0, part_i = w.wide ? half : (w.jobs - w.first_job) & 1, nth = w.tile - w.of_column;
+                const bool begins = w.wide ? nth == 0 : nth < 2, ends = w.wide ? nth == w.in_part - 1 : nth + 2 >= w.in_part;
+                if (begins) {
+                    const int R = w.part * 2 * ROWS + half * ROWS + r;
+                    mine = R < w.it.rows;
+                    if (mine) {
+                        const int member = kvc_divide(R, p.group), h = w.k_head * p.g + R - member * p.g, b = w.item < groups ? member_at(p, w.it.first + member) : w.it.first;
+                        mine = row_of(p, b) >= 0;
+                        const long long place = w.of_column == 0 ? place_of(p, w.item >= groups, b, h, w.wide ? 0 : part_i) : cta_place(p, blockIdx.x, part_i * ROWS + r);
+                        to = p.sums + place * D;
+                        to_max = p.maxima + place;
+                    }
+                    m = -CUDART_INF_F;
+                    l = 0.0f;
+                }
+                bar_wait(scores_there + set, n_set & 1, failed);
+                after_sync();
+                if (__any_sync(0xffffffffu, mine)) {
+                    uint32_t s[128];
+#pragma unroll
+                    for (int c = 0; c < 4; c++) load32(s + 32 * c, scores + 32 * c);
+                    loads_wait();
+                    if (p.negative) {
+#pragma unroll
+                        for (int i = 0; i < 128; i++) s[i] ^= 0x80000000u;
+                    }
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        const uint32_t mask = masks[tile_n % MASKS][c];
+                        if (mask == 0xffffffffu) continue;
+#pragma unroll
+                        for (int i = 0; i < 32; i++) s[32 * c + i] = mask >> i & 1 ? s[32 * c + i] : 0xff800000u;
+                    }
+                    float top[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
+#pragma unroll
+                    for (int i = 0; i < 128; i++) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(s[i]));
+                    const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.log2_scaling;
+                    const bool up = high > m + SLACK || (m == -CUDART_INF_F && high > m);
+                    if (__any_sync(0xffffffffu, up)) {
+                        const float now = up ? high : m, f = up ? exp2_approx(m - now) : 1.0f;
+                        m = now;
+                        l *= f;
+                        if (!begins) {
+                            bar_wait(sums_there + set, (n_set - 1) & 1, failed);
+                            after_sync();
+#pragma unroll
+                            for (int c = 0; c < D / 32; c++) {
+                                uint32_t o[32];
+                                load32(o, sums + 32 * c);
+                                loads_wait();
+#pragma unroll
+                                for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                                store32(sums + 32 * c, o);
+                            }
+                        }
+                    }
+                    const float less = LIFT - (m == -CUDART_INF_F ? 0.0f : m);
+                    float sum[4] = {};
+#pragma unroll
+                    for (int c = 0; c < 2; c++) {
+                        uint32_t weights[32];
+#pragma unroll
+                        for (int i = 0; i < 32; i++) {
+                            const float w0 = exp2_approx(fmaf(__uint_as_float(s[64 * c + 2 * i]), p.log2_scaling, less)), w1 = exp2_approx(fmaf(__uint_as_float(s[64 * c + 2 * i + 1]), p.log2_scaling, less));
+                            sum[i & 1] += w0;
+                            sum[2 + (i & 1)] += w1;
+                            weights[i] = pack(w0, w1, T());
+                        }
+                        store32(scores + 32 * c, weights);
+                    }
+                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    stores_wait();
+                }
+                before_sync();
+                __syncwarp();
+                if (lane == 0) bar_arrive(weights_there + set);
+                if (ends) {
+                    bar_wait(sums_there + set, n_set & 1, failed);
+                    after_sync();
+                    if (__any_sync(0xffffffffu, mine)) {
+#pragma unroll
+                        for (int c = 0; c < D / 32; c++) {
+                            uint32_t o[32];
+                            load32(o, sums + 32 * c);
+                            loads_wait();
+                            if (mine) {
+#pragma unroll
+                                for (int i = 0; i < 8; i++)
+                                    __stcg(reinterpret_cast<uint4 *>(to) + 8 * c + i, make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]));
+                            }
+                        }
+                        if (mine) __stcg(to_max, make_float2(m, l));
+                    }
+                    before_sync();
+                }
+                n_set++;
+            }
+        } else {
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+            if (warp == 8) {
+                // ---- the products, by one thread
+                constexpr uint32_t KIND = 1u << 4 | Weight<T>::KIND << 7 | Weight<T>::KIND << 10 | (uint32_t)(ROWS >> 4) << 24;
+                constexpr uint32_t SCORES = KIND | (uint32_t)(TOKENS >> 3) << 17, VALUES = KIND | 1u << 16 | (uint32_t)(D >> 3) << 17;
+                if (lane == 0) {
+                    struct { int set, unit, n; bool first, last_of_unit; } late = {-1, 0, 0, false, false};
+                    int n_set[2] = {0, 0}, tile_n = 0;
+                    auto values_of = [&]() {                // the second product of the job before
+                        if (late.set < 0) return;
+                        bar_wait(weights_there + late.set, late.n & 1, failed);
+                        const int unit = late.unit, slot = unit % RING;
+                        bar_wait(full + slot, unit / RING & 1, failed);
+                        after_sync();
+                        const uint32_t at = ring + slot * UNIT;
+#pragma unroll
+                        for (int k = 0; k < TOKENS / 16; k++)
+                            product_of_weights(tensor + 256 + late.set * 128, tensor + late.set * 128 + 8 * k, operand_at(at + k * 2048, ATOM), VALUES, !late.first || k > 0);
+                        if (late.last_of_unit) commit_to(empty + slot);
+                        commit_to(sums_there + late.set);   // (the last that comes back)
+                    };
+                    for (; w.left > 0; next_tile(p, w, groups), tile_n++) {
+                        const int nth = w.tile - w.of_column, unit = 2 * tile_n, slot = unit % RING;
+                        bar_wait(full + slot, unit / RING & 1, failed);
+                        for (int j = 0; j < (w.wide ? 2 : 1); j++) {
+                            const int set = (w.jobs + j) & 1;
+                            const bool begins = w.wide ? nth == 0 : nth < 2, ends = w.wide ? nth == w.in_part - 1 : nth + 2 >= w.in_part, last = !w.wide || j == 1;
+                            after_sync();
+#pragma unroll
+                            for (int k = 0; k < D / 16; k++) {
+                                const uint32_t off = (k >> 2) * ATOM + (k & 3) * 32;
+                                product(tensor + set * 128, operand_at(base + set * UNIT + off, 16), operand_at(ring + slot * UNIT + off, 16), SCORES, k > 0);
+                            }
+                            commit_to(scores_there + set);
+                            if (ends) commit_to(queries_free + set);
+                            if (last) commit_to(empty + slot);
+                            values_of();
+                            late = {set, unit + 1, n_set[set]++, begins, last};
+                        }
+                    }
+                    values_of();
+                    // all products are done before anything is given back
+                    if (late.set >= 0) bar_wait(sums_there + late.set, late.n & 1, failed);
+                }
+                __syncwarp();
+            } else {
+                // ---- the copies: a warp takes every third tile of keys or values
+                const int mine = warp - 9;
+                int signal = -1, tile_n = 0, loads[2] = {0, 0};     // the tile whose copies are on their way and not said to be there, times the sets' queries were loaded
+                auto drain = [&]() {
+                    if (signal < 0) return;
+                    copies_wait<0>();
+                    seen_by_products();
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(full + signal % RING);
+                    signal = -1;
+                };
+                auto wait = [&](uint64_t *bar, uint32_t parity) {   // (what is waited for may need what this warp has copied)
+                    if (__all_sync(0xffffffffu, bar_try(bar, parity, 0))) return;
+                    drain();
+                    bar_wait(bar, parity, failed);
+                    __syncwarp();
+                };
+                for (; w.left > 0; next_tile(p, w, groups), tile_n++) {
+                    const int nth = w.tile - w.of_column;
+                    const bool begins = w.wide ? nth == 0 : nth < 2;
+#pragma unroll 1
+                    for (int values = 0; values < 2; values++) {
+                        const int unit = 2 * tile_n + values;
+                        if (unit % 3 != mine) {
+                            if (values == 0 && begins) for (int j = 0; j < (w.wide ? 2 : 1); j++) loads[(w.jobs + j) & 1]++;
+                            continue;
+                        }
+                        // pages of the tile's tokens: lane's are lane, lane + 32, ..
+                        int pages[4];
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const int t = w.tile * TOKENS + 32 * i + lane;
+                            pages[i] = t < w.it.len ? a.table[w.it.table * a.table_stride + kvc_divide(t, p.page)] : -1;
+                        }
+                        if (unit >= RING) wait(empty + unit % RING, (unit / RING - 1) & 1);
+                        if (values == 0) {
+                            if (begins) {
+                                for (int j = 0; j < (w.wide ? 2 : 1); j++) {
+                                    const int set = (w.jobs + j) & 1, from = w.part * 2 * ROWS + j * ROWS, n = min(ROWS, w.it.rows - from);
+                                    if (loads[set] > 0) wait(queries_free + set, (loads[set] - 1) & 1);
+                                    loads[set]++;
+                                    for (int i = lane; i < n * (D / 8); i += 32) {
+                                        const int r = i / (D / 8), c = i % (D / 8), R = from + r, member = kvc_divide(R, p.group), h = w.k_head * p.g + R - member * p.g;
+                                        const int b = w.item < groups ? member_at(p, w.it.first + member) : w.it.first, row = row_of(p, b);
+                                        copy16(base + set * UNIT + (c >> 3) * ATOM + r * 128 + ((c & 7) ^ (r & 7)) * 16,
+                                               reinterpret_cast<const T *>(a.q) + (long long)max(row, 0) * a.q_token + h * a.q_head + c * 8, row >= 0);
+                                    }
+                                }
+                            }
+                        }
+                        const uint32_t to = ring + unit % RING * UNIT;
+                        const T *pool = reinterpret_cast<const T *>(values ? a.vpages : a.kpages);
+                        const long long of_page = values ? a.vp_page : a.kp_page, of_row = values ? a.vp_row : a.kp_row, of_head = values ? a.vp_head : a.kp_head;
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const bool good = (unsigned)pages[i] < p.n_pages;
+                            if (!good && w.tile * TOKENS + 32 * i + lane < w.it.len) flags |= KVC_FLAG_BAD_PAGE;
+                            const uint32_t mask = __ballot_sync(0xffffffffu, good);
+                            if (values == 0 && lane == 0) masks[tile_n % MASKS][i] = mask;
+                            const int t = w.tile * TOKENS + 32 * i + lane, row = t - kvc_divide(t, p.page) * (int)a.page_size;
+                            const T *from = pool + (good ? pages[i] * of_page + row * of_row + w.k_head * of_head : 0);
+                            constexpr int SIDE = D == 96 ? 4 : D / 8 > 16 ? 16 : D / 8;       // lanes of a row
+#pragma unroll 4
+                            for (int k = 0; k < SIDE; k++) {
+                                const int j = k * (32 / SIDE) + lane / SIDE;
+                                const T *row_from = reinterpret_cast<const T *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(from), j));
+                                const int r = 32 * i + j;
+#pragma unroll
+                                for (int c0 = 0; c0 < D / 8; c0 += SIDE) {
+                                    const int c = c0 + lane % SIDE;
+                                    copy16(to + (c >> 3) * ATOM + r * 128 + ((c & 7) ^ (r & 7)) * 16, row_from + c * 8, mask >> j & 1);
+                                }
+                            }
+                        }
+                        copies_commit();
+                        if (signal >= 0) {
+                            copies_wait<1>();
+                            seen_by_products();
+                            __syncwarp();
+                            if (lane == 0) bar_arrive(full + signal % RING);
+                        }
+                        signal = unit;
+                    }
+                }
+                drain();
+                copies_wait<0>();
+            }
+        }
+    }
+    if (flags && a.status) atomicOr(a.status, flags);
+    before_sync();
+    __syncthreads();
+    after_sync();
+    if (tid == 0 && failed_s && a.status) atomicOr(a.status, KVC_FLAG_WAIT_TIMEOUT);
+    if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tensor));
+}
+
+// ---- the parts of a row's sums are joined ---------------------------------------------------------------------------
+
+template <typename T, int D>
+__global__ void __launch_bounds__(128) prefix_join_kernel(const __grid_constant__ Params p) {
+    kvc_behind();
+    const kvc_paged_attn_args &a = p.a;
+    const int lane = threadIdx.x & 31, B = (int)a.B, quads = (int)(a.Hq + 3) / 4, b = blockIdx.x / quads, h = (blockIdx.x - b * quads) * 4 + (threadIdx.x >> 5);
+    if (h >= a.Hq) return;
+    const bool on = lane < D / 4;
+    auto nothing = [&](int row) {
+        if (on) *reinterpret_cast<uint2 *>(reinterpret_cast<T *>(a.out) + row * a.out_token + h * a.out_head + lane * 4) = make_uint2(0, 0);
+        if (lane == 0 && a.lse) a.lse[row * a.Hq + h] = -CUDART_INF_F;
+    };
+    if (b == B) {                                           // rows behind the last
+        for (int row = row_at(p, B); row < p.rows; row++) nothing(row);
+        return;
+    }
+    const int row = row_of(p, b);
+    if (row < 0) {
+        for (int i = row_at(p, b); i < row_at(p, b + 1); i++) nothing(i);
+        return;
+    }
+    const int groups = min(max(p.plan[0], 0), B), group = min(p.plan[plan_group(B) + b], groups - 1), size = *p.share, k_head = kvc_divide(h, p.group);
+    float top = -CUDART_INF_F, sum = 0.0f;
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    auto add = [&](float2 ml, float4 x) {
+        const float now = fmaxf(top, ml.x), less = now == -CUDART_INF_F ? 0.0f : now, f = exp2_approx(top - less), g = exp2_approx(ml.x - less);
+        sum = sum * f + ml.y * g;
+        // (what nothing was added to may hold anything)
+        v.x = v.x * f + x.x * g; v.y = v.y * f + x.y * g; v.z = v.z * f + x.z * g; v.w = v.w * f + x.w * g;
+        top = now;
+    };
+    for (int own = 0; own < 2; own++) {
+        if (!own && group < 0) continue;
+        const int i = own ? groups + b : group;
+        const Item it = item_of(p, i, groups);
+        if (it.tiles == 0) continue;
+        const int R = (own ? 0 : min(max(p.plan[plan_rank(B) + b], 0), it.rows / p.g - 1)) * p.g + h - k_head * p.g, part = R / (2 * ROWS), in_part = R - part * 2 * ROWS;
+        const bool wide = it.rows - part * 2 * ROWS > ROWS;
+        const int from = p.item_first[i] + (k_head * it.parts + part) * it.tiles, to = from + it.tiles;
+        // a column's parts: each in a CTA's share, of narrow columns two (every other tile) where it has more than one
+        const int cta0 = from / size, cta1 = (to - 1) / size, each = wide ? 1 : 2;
+        constexpr int AT_ONCE = 4;
+        for (int k0 = 0; k0 < (cta1 - cta0 + 1) * each; k0 += AT_ONCE) {
+            float2 ml[AT_ONCE];
+            float4 x[AT_ONCE];
+#pragma unroll
+            for (int k = 0; k < AT_ONCE; k++) {
+                const int cta = cta0 + (k0 + k) / each, which = (k0 + k) % each;
+                const int there = min(to, (cta + 1) * size) - max(from, cta * size);
+                ml[k] = make_float2(-CUDART_INF_F, 0.0f);
+                x[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (cta <= cta1 && which < there) {
+                    const long long place = cta == cta0 ? place_of(p, own, b, h, which) : cta_place(p, cta, wide ? in_part : which * ROWS + in_part);
+                    ml[k] = __ldcg(p.maxima + place);
+                    if (on) x[k] = __ldcg(reinterpret_cast<const float4 *>(p.sums + place * D) + lane);
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < AT_ONCE; k++)
+                if (ml[k].x != -CUDART_INF_F || ml[k].y != 0.0f) add(ml[k], x[k]);
+        }
+    }
+    const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
+    if (on) *reinterpret_cast<uint2 *>(reinterpret_cast<T *>(a.out) + row * a.out_token + h * a.out_head + lane * 4) = make_uint2(pack(v.x * f, v.y * f, T()), pack(v.z * f, v.w * f, T()));
+    if (lane == 0 && a.lse) a.lse[row * a.Hq + h] = sum == 0.0f ? -CUDART_INF_F : (top + log2f(sum) - Weight<T>::LIFT) * 0.69314718055994531f;
+}
+
+template <typename T, int D>
+int launch(Params &p, cudaStream_t s) {
+    static kvc_launch_slot slot;
+    int occ = 0;
+    if (int rc = kvc_prepare(slot, reinterpret_cast<const void *>(prefix_attn_kernel<T, D>), THREADS, Shape<D>::SHARED, &occ)) return rc;
+    KVC_REQUIRE(occ > 0, "kvc_paged_attn_shared: the kernel does not fit this device");
+    prefix_attn_kernel<T, D><<<(unsigned)p.grid, THREADS, Shape<D>::SHARED, s>>>(p);
+    KVC_LAUNCH_OK();
+    return kvc_launch_early(prefix_join_kernel<T, D>, (unsigned)((p.a.B + 1) * ((p.a.Hq + 3) / 4)), 128, s, p);
+}
+
+int64_t item_bytes(int64_t B) { return (4 * (2 * B + 1) + 255) / 256 * 256; }
+int64_t places(int64_t B, int64_t Hq) { return 4 * B * Hq + 256ll * kvc_sm_count(); }
+
+}  // namespace
+
+extern "C" int64_t kvc_prefix_plan_words(int64_t B) { return B < 0 ? 0 : plan_words(B); }
+
+extern "C" int kvc_prefix_plan(const kvc_prefix_plan_args *args, kvc_stream_t stream) {
+    KVC_REQUIRE(args, "kvc_prefix_plan: null pointer");
+    kvc_prefix_plan_args a;
+    memcpy(&a, args, sizeof(a));
+    KVC_REQUIRE(a.B >= 0 && a.B <= MAX_REQUESTS, "kvc_prefix_plan: %lld requests, %d at most", (long long)a.B, MAX_REQUESTS);
+    KVC_REQUIRE(a.plan && (a.B == 0 || (a.parents && a.shared)), "kvc_prefix_plan: null pointer");
+    cudaStream_t s = kvc_cu(stream);
+    if (a.B > 0)
+        if (int rc = kvc_launch_early(prefix_find_kernel, (unsigned)((a.B + FIND_THREADS - 1) / FIND_THREADS), FIND_THREADS, s, a)) return rc;
+    return kvc_launch_early(prefix_scan_kernel, 1, SCAN_THREADS, s, a);
+}
+
+extern "C" int64_t kvc_paged_attn_shared_workspace(int64_t B, int64_t Hq, int64_t Hkv, int64_t D) {
+    if (B < 0 || Hkv <= 0 || Hq < Hkv || D <= 0) return 0;
+    return item_bytes(B) + places(B, Hq) * (4 * D + 8);
+}
+
+extern "C" int kvc_paged_attn_shared(const kvc_paged_attn_args *args, const int32_t *plan, const int32_t *starts, int64_t rows, kvc_stream_t stream) {
+    KVC_REQUIRE(args && plan, "kvc_paged_attn_shared: null pointer");
+    Params p;
+    memcpy(&p.a, args, sizeof(p.a));
+    kvc_paged_attn_args &a = p.a;
+    KVC_REQUIRE(a.type == KVC_TYPE_FP16 || a.type == KVC_TYPE_BF16, "kvc_paged_attn_shared: unknown type %d", a.type);
+    KVC_REQUIRE(a.D == 64 || a.D == 96 || a.D == 128, "kvc_paged_attn_shared: heads of 64, 96 or 128 channels, got %lld", (long long)a.D);
+    KVC_REQUIRE(a.B >= 0 && a.B <= MAX_REQUESTS && a.Hkv > 0 && a.Hq > 0 && a.Hq % a.Hkv == 0 && a.Hq < 65536, "kvc_paged_attn_shared: %lld query heads over %lld", (long long)a.Hq, (long long)a.Hkv);
+    KVC_REQUIRE(a.page_size > 0 && a.page_size <= KVC_MAX_PAGE && a.n_pages >= 0 && a.n_pages < (1ll << 31) && a.table_width >= 0, "kvc_paged_attn_shared: bad sizes");
+    KVC_REQUIRE(a.window == 0, "kvc_paged_attn_shared: no window (it would end inside the prefix)");
+    KVC_REQUIRE(a.table_width * a.page_size < (1ll << 31) - 256, "kvc_paged_attn_shared: a table row holds %lld tokens, lengths have 32 bits", (long long)(a.table_width * a.page_size));
+    if (!starts) rows = a.B;
+    KVC_REQUIRE(rows >= 0 && rows < (1 << 24) && (a.B > 0 || rows == 0), "kvc_paged_attn_shared: %lld rows of %lld requests", (long long)rows, (long long)a.B);
+    if (rows == 0) return KVC_OK;
+    KVC_REQUIRE(a.q && a.out && a.lengths && (a.table || a.table_width == 0) && ((a.kpages && a.vpages) || a.n_pages == 0), "kvc_paged_attn_shared: null pointer");
+    const int64_t g = a.Hq / a.Hkv, most_tiles = (a.table_width * a.page_size + TOKENS - 1) / TOKENS;
+    KVC_REQUIRE(a.Hkv * (2 * a.B + a.B * g / (2 * ROWS)) < (1ll << 31) / std::max<int64_t>(most_tiles, 1), "kvc_paged_attn_shared: requests, KV heads and table rows of more than 2^31 tiles");
+    const uintptr_t at = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.kpages) | reinterpret_cast<uintptr_t>(a.vpages) | reinterpret_cast<uintptr_t>(a.out);
+    if (a.Hq == 1) a.q_head = a.out_head = 0;              // (the stride of a dimension of one may be anything)
+    if (rows == 1) a.q_token = a.out_token = 0;
+    if (a.Hkv == 1) a.kp_head = a.vp_head = 0;
+    if (a.page_size == 1) a.kp_row = a.vp_row = 0;
+    if (a.n_pages <= 1) a.kp_page = a.vp_page = 0;
+    const int64_t strides = a.q_token | a.q_head | a.out_token | a.out_head | a.kp_page | a.kp_row | a.kp_head | a.vp_page | a.vp_row | a.vp_head;
+    KVC_REQUIRE((at & 15) == 0 && (strides & 7) == 0, "kvc_paged_attn_shared: rows must start on 16 bytes");
+    KVC_REQUIRE(a.workspace && (reinterpret_cast<uintptr_t>(a.workspace) & 15) == 0, "kvc_paged_attn_shared: the workspace must be 16-byte aligned");
+    if (a.workspace_bytes < kvc_paged_attn_shared_workspace(a.B, a.Hq, a.Hkv, a.D)) {
+        kvc_set_error("kvc_paged_attn_shared: the workspace must hold what kvc_paged_attn_shared_workspace says");
+        return KVC_ERR_CAPACITY;
+    }
+    const kvc_rows q = kvc_make_rows(a.q, a.D, rows, a.q_token, a.Hq, a.q_head), out = kvc_make_rows(a.out, a.D, rows, a.out_token, a.Hq, a.out_head);
+    KVC_REQUIRE(out.apart, "kvc_paged_attn_shared: rows of the output overlap");
+    KVC_REQUIRE(kvc_rows_equal(q, out) || !kvc_rows_overlap(q, out), "kvc_paged_attn_shared: the output overlaps the queries and is not them");
+    p.plan = plan;
+    p.starts = starts;
+    p.page = kvc_make_div((uint32_t)a.page_size);
+    p.group = kvc_make_div((uint32_t)g);
+    p.g = (int)g;
+    p.rows = (int)rows;
+    p.most_tokens = (int)(a.table_width * a.page_size);
+    p.grid = kvc_sm_count();
+    p.n_pages = (unsigned)a.n_pages;
+    p.negative = a.scaling < 0.0f;
+    p.log2_scaling = std::max(fabsf(a.scaling) * 1.4426950408889634f, 1e-37f);      // (0 times the -inf of a token that is left out is none)
+    p.item_first = reinterpret_cast<int32_t *>(a.workspace);
+    p.share = p.item_first + 2 * a.B;
+    p.sums = reinterpret_cast<float *>(reinterpret_cast<uint8_t *>(a.workspace) + item_bytes(a.B));
+    p.maxima = reinterpret_cast<float2 *>(p.sums + places(a.B, a.Hq) * a.D);
+    cudaStream_t s = kvc_cu(stream);
+    const bool fp16 = a.type == KVC_TYPE_FP16;
+    if (a.D == 64) return fp16 ? launch<__half, 64>(p, s) : launch<__nv_bfloat16, 64>(p, s);
+    if (a.D == 96) return fp16 ? launch<__half, 96>(p, s) : launch<__nv_bfloat16, 96>(p, s);
+    return fp16 ? launch<__half, 128>(p, s) : launch<__nv_bfloat16, 128>(p, s);
+}

@@ -28,6 +28,9 @@ decltype(&kvc_page_slots) page_slots = nullptr;
 decltype(&kvc_page_shift) page_shift = nullptr;
 decltype(&kvc_paged_rows) paged_rows = nullptr;
 decltype(&kvc_paged_attn_codes) paged_attn_codes = nullptr;
+decltype(&kvc_prefix_plan_words) prefix_plan_words = nullptr;
+decltype(&kvc_prefix_plan) prefix_plan = nullptr;
+decltype(&kvc_paged_attn_shared) paged_attn_shared = nullptr;
 
 [[noreturn]] void fail(const std::string &why) {
     PyErr_SetString(error_class ? error_class : PyExc_RuntimeError, why.c_str());
@@ -384,10 +387,10 @@ PyObject *py_paged_rows(PyObject *, PyObject *const *args, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-// q, kpages, vpages, table, lengths, scaling, window, out or None, return_lse, workspace, status, starts or None, kscales or None, vscales or None
+// q, kpages, vpages, table, lengths, scaling, window, out or None, return_lse, workspace, status, starts or None, kscales or None, vscales or None, a prefix plan or None
 PyObject *py_paged_attn(PyObject *, PyObject *const *args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    count(n, 14);
+    count(n, 15);
     const at::Tensor &q0 = tensor(args[0], "q"), &pool = tensor(args[1], "kpages");
     const int device = device_of(q0, "q");
     kvc_paged_attn_args a = {};
@@ -398,7 +401,8 @@ PyObject *py_paged_attn(PyObject *, PyObject *const *args, Py_ssize_t n) {
     at::ScalarType of_pool = type;
     const kvc_scales scales = scales_of(pool, args[12], args[13], of_pool, device);
     const at::Tensor &q = rows(args[0], q0.sizes(), type, "q", device), &kp = rows(args[1], pool.sizes(), of_pool, "kpages", device), &vp = rows(args[2], pool.sizes(), of_pool, "vpages", device);
-    const bool by_row = given(args[11]);
+    const bool by_row = given(args[11]), with_prefix = given(args[14]);
+    if (with_prefix && scales.codes) fail("prefixes of pools of codes are not attended");
     const at::Tensor &lengths = tensor(args[4], "lengths");
     a.B = !by_row ? q.size(0) : lengths.dim() == 1 ? lengths.size(0) : -1;
     a.Hq = q.size(1); a.D = q.size(2);
@@ -423,7 +427,10 @@ PyObject *py_paged_attn(PyObject *, PyObject *const *args, Py_ssize_t n) {
         lse = at::empty({q.size(0), a.Hq}, q.options().dtype(at::kFloat));
         a.lse = static_cast<float *>(lse.data_ptr());
     }
-    if (scales.codes)
+    if (with_prefix)
+        launch(paged_attn_shared, a, device, "kvc_paged_attn_shared", static_cast<const int32_t *>(words(args[14], prefix_plan_words ? prefix_plan_words(a.B) : 0, "plan", device)),
+               by_row ? static_cast<const int32_t *>(words(args[11], a.B + 1, "starts", device)) : nullptr, q.size(0));
+    else if (scales.codes)
         launch(paged_attn_codes, a, device, "kvc_paged_attn_codes", &scales, by_row ? static_cast<const int32_t *>(words(args[11], a.B + 1, "starts", device)) : nullptr, q.size(0));
     else if (by_row) launch(paged_attn_rows, a, device, "kvc_paged_attn_rows", static_cast<const int32_t *>(words(args[11], a.B + 1, "starts", device)), q.size(0));
     else launch(paged_attn, a, device, "kvc_paged_attn");
@@ -435,6 +442,29 @@ PyObject *py_paged_attn(PyObject *, PyObject *const *args, Py_ssize_t n) {
     Py_DECREF(result);
     Py_XDECREF(more);
     return both;
+    END_HANDLE_TH_ERRORS
+}
+
+// parents, shared, out or None, status -> the plan
+PyObject *py_prefix_plan(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    count(n, 4);
+    const at::Tensor &parents = tensor(args[0], "parents");
+    const int device = device_of(parents, "parents");
+    kvc_prefix_plan_args a = {};
+    a.B = parents.dim() == 1 ? parents.size(0) : -1;
+    a.parents = static_cast<int32_t *>(words(args[0], a.B, "parents", device));
+    a.shared = static_cast<int32_t *>(words(args[1], a.B, "shared", device));
+    if (!prefix_plan_words) fail("kvc_torch: init() has not been called");
+    const int64_t all = prefix_plan_words(a.B);
+    const bool own = !given(args[2]);
+    const at::Tensor plan = own ? ints(all, parents) : (words(args[2], all, "out", device), tensor(args[2], "out"));
+    a.plan = int_at(plan);
+    a.status = status_of(args[3], device);
+    launch(prefix_plan, a, device, "kvc_prefix_plan");
+    if (own) return THPVariable_Wrap(plan);
+    written({args[2]});
+    return Py_NewRef(args[2]);
     END_HANDLE_TH_ERRORS
 }
 
@@ -454,7 +484,7 @@ PyObject *py_stream_of(PyObject *, PyObject *const *args, Py_ssize_t n) {
 // the error's class and the addresses of the library's entries
 PyObject *py_init(PyObject *, PyObject *const *args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    count(n, 12);
+    count(n, 15);
     error_class = Py_NewRef(args[0]);
     auto address = [&](int i) { return reinterpret_cast<void *>(static_cast<uintptr_t>(number(args[i]))); };
     page_plan = reinterpret_cast<decltype(page_plan)>(address(1));
@@ -468,6 +498,9 @@ PyObject *py_init(PyObject *, PyObject *const *args, Py_ssize_t n) {
     page_shift = reinterpret_cast<decltype(page_shift)>(address(9));
     paged_rows = reinterpret_cast<decltype(paged_rows)>(address(10));
     paged_attn_codes = reinterpret_cast<decltype(paged_attn_codes)>(address(11));
+    prefix_plan_words = reinterpret_cast<decltype(prefix_plan_words)>(address(12));
+    prefix_plan = reinterpret_cast<decltype(prefix_plan)>(address(13));
+    paged_attn_shared = reinterpret_cast<decltype(paged_attn_shared)>(address(14));
     Py_RETURN_NONE;
     END_HANDLE_TH_ERRORS
 }
@@ -482,6 +515,7 @@ PyMethodDef methods[] = {{"init", fast<py_init>(), METH_FASTCALL, nullptr},
                          {"page_slots", fast<py_page_slots>(), METH_FASTCALL, nullptr},
                          {"page_shift", fast<py_page_shift>(), METH_FASTCALL, nullptr},
                          {"paged_rows", fast<py_paged_rows>(), METH_FASTCALL, nullptr},
+                         {"prefix_plan", fast<py_prefix_plan>(), METH_FASTCALL, nullptr},
                          {"stream_of", fast<py_stream_of>(), METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "kvc_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

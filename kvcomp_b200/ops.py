@@ -831,4 +831,42 @@ def paged_attn(q, kpages, vpages, table, lengths, scaling, window=0, out=None, r
         if not isinstance(q, torch.Tensor) or not q.is_cuda or q.dim() != 3 or not isinstance(kpages, torch.Tensor) or kpages.dim() != 4:
             raise KvcError("q must be a CUDA tensor [B, Hq, D], the pools [pages, page_size, Hkv, D] (kvcomp_b200 has no CPU path)")
         workspace = paged_attn_workspace(q.shape[0], q.shape[1], kpages.shape[2], q.shape[2], q.device)
-    return _lib.torch_calls().paged_attn(q, kpages, vpages, table, lengths, scaling, window, out, return_lse, workspace, status, starts, kscales, vscales)
+    return _lib.torch_calls().paged_attn(q, kpages, vpages, table, lengths, scaling, window, out, return_lse, workspace, status, starts, kscales, vscales, None)
+
+
+class PrefixPlan:
+    """What prefix_plan answers: which requests continue the same prefix (a device tensor of the library's layout), for `requests` of them."""
+    __slots__ = ("words", "requests")
+
+    def __init__(self, words, requests):
+        self.words, self.requests = words, requests
+
+
+def prefix_plan(parents, shared, out=None, status=None):
+    """Requests that continue a common prefix: parents[b] (int32[B], below 0: none) is the request whose first shared[b] (int32[B]) tokens come before b's own.  Requests with the same two numbers
+    are attended to together (paged_attn_shared).  A request that is followed follows no one, and nobody itself (FLAG_BAD_LENGTH).  Holds for all steps and layers until either changes.  out: a
+    PrefixPlan of as many requests, written in place (a captured step goes by what is in it).  At most 16384 requests."""
+    words = _lib.torch_calls().prefix_plan(parents, shared, None if out is None else out.words, status)
+    return PrefixPlan(words, parents.shape[0]) if out is None else out
+
+
+def paged_attn_shared_workspace(B, Hq, Hkv, D, device):
+    """Workspace for paged_attn_shared (reusable across calls that follow one another; concurrent streams need their own, and so do graphs that may run at once)."""
+    index = torch.empty(0, device=device).get_device()
+    if index < 0:
+        raise KvcError("paged_attn_shared_workspace: %s is no CUDA device" % (device,))
+    with _on(torch.device("cuda", index)):
+        return torch.empty(_lib.load().kvc_paged_attn_shared_workspace(B, Hq, Hkv, D), dtype=torch.uint8, device=torch.device("cuda", index))
+
+
+def paged_attn_shared(q, kpages, vpages, table, lengths, plan, scaling, out=None, return_lse=False, workspace=None, status=None, starts=None):
+    """paged_attn where requests continue prefixes: request b's token attends to the first shared[b] tokens of its parent (of those that it has: FLAG_BAD_LENGTH if it has fewer) and to b's own
+    lengths[b].  plan: prefix_plan's, of these B requests.  The pages of a prefix are read once for all that follow it (once for 256 rows of a KV head).  D: 64, 96, 128; no window.  workspace:
+    paged_attn_shared_workspace's, for one call at a time.  Values that count are finite (0 times an infinite one is no number).  The other arguments are paged_attn's."""
+    if not isinstance(plan, PrefixPlan):
+        raise KvcError("plan must be prefix_plan's")
+    if not isinstance(q, torch.Tensor) or not q.is_cuda or q.dim() != 3 or not isinstance(kpages, torch.Tensor) or kpages.dim() != 4:
+        raise KvcError("q must be a CUDA tensor [B, Hq, D], the pools [pages, page_size, Hkv, D] (kvcomp_b200 has no CPU path)")
+    if workspace is None:
+        workspace = paged_attn_shared_workspace(plan.requests, q.shape[1], kpages.shape[2], q.shape[2], q.device)
+    return _lib.torch_calls().paged_attn(q, kpages, vpages, table, lengths, scaling, 0, out, return_lse, workspace, status, starts, None, None, plan.words)
