@@ -32,19 +32,6 @@ int choose(Params &p, bool same, cudaStream_t s) {
     }
 }
 
-// query heads that a column takes at most: 16 where they fit the registers beside the accumulators
-int group_of(int64_t Hq, int64_t Hkv, int64_t D) { return (int)std::min<int64_t>(Hq / Hkv, D > 128 ? 8 : MAX_GROUP); }
-int64_t columns_of(int64_t Hq, int64_t Hkv, int64_t D) { return Hkv * ((Hq / Hkv + group_of(Hq, Hkv, D) - 1) / group_of(Hq, Hkv, D)); }
-// Of partial results: two for every piece.  Of s tiles for a CTA s / 8 and those left by rounding down are drawn, in rounds of s / 16, s / 32, s / 64 (at least) and what these leave:
-// a CTA's share and five pieces more.
-int64_t places(int64_t D) { return 2ll * 6 * (D == 64 ? 4 : 3) * kvc_sm_count(); }
-// Floats of a place: of two KV heads where they are read together; room for eight heads at least, so that one workspace serves more shapes.  A multiple of four: values are
-// written and read sixteen bytes at a time, and n (D + 2) is two more than one for odd n.
-int64_t part_floats(int64_t group, int64_t D) { return (std::max<int64_t>(group <= 8 && D < 128 ? 2 * group : group, 8) * (D + 2) + 3) / 4 * 4; }
-// The counter of what is drawn, and two counters for a place: of the column whose first result lies there, of the eight results that begin there.  They lie in
-// front, the same for calls of all shapes: a workspace may serve one after the other.
-int64_t counter_bytes() { return 256 + (2 * places(64) * 4 + 255) / 256 * 256; }
-
 }  // namespace
 
 extern "C" int64_t kvc_paged_attn_cleared(void) { return counter_bytes(); }
@@ -89,26 +76,9 @@ static int paged_attn(const kvc_paged_attn_args *args, const kvc_scales *scales,
     const kvc_rows q = kvc_make_rows(a.q, a.D, rows, a.q_token, a.Hq, a.q_head), out = kvc_make_rows(a.out, a.D, rows, a.out_token, a.Hq, a.out_head);
     KVC_REQUIRE(out.apart, "kvc_paged_attn: rows of the output overlap");
     KVC_REQUIRE(kvc_rows_equal(q, out) || !kvc_rows_overlap(q, out), "kvc_paged_attn: the output overlaps the queries and is not them");
-    Params p;
-    p.a = a;
-    p.page = kvc_make_div((uint32_t)a.page_size);
-    p.group = group_of(a.Hq, a.Hkv, a.D);
-    p.columns = (int)columns_of(a.Hq, a.Hkv, a.D);
-    p.per_head = p.columns / (int)a.Hkv;
-    p.chunk = (int)((a.B + 31) / 32);
-    p.most_tokens = (int)(a.table_width * a.page_size);
-    p.n_pages = (unsigned)a.n_pages;
-    p.starts = starts;
-    p.rows = (int)rows;
-    p.negative = a.scaling < 0.0f;
-    p.log2_scaling = std::max(fabsf(a.scaling) * 1.4426950408889634f, 1e-37f);      // (0 times the -inf of a token that is left out is none)
-    p.part = (int)part_floats(p.group, a.D);
-    p.drawn = reinterpret_cast<int *>(a.workspace);
-    p.counters = reinterpret_cast<unsigned *>(a.workspace) + 64;
-    p.group_counters = p.counters + places(64);
-    p.parts = reinterpret_cast<float *>(reinterpret_cast<uint8_t *>(a.workspace) + counter_bytes());
+    Params p = {};
+    set_params(p, a, starts, rows);
     cudaStream_t s = kvc_cu(stream);
-    p.v_less_k = reinterpret_cast<const uint8_t *>(a.vpages) - reinterpret_cast<const uint8_t *>(a.kpages);
     const bool same = a.kp_page == a.vp_page && a.kp_row == a.vp_row && a.kp_head == a.vp_head;
     if (scales) {
         if (a.Hkv == 1) c.k_head = c.v_head = 0;

@@ -62,6 +62,7 @@ struct Params {
     int part;                                   // floats of a place: sums of values, maxima and sums of weights
     float *parts;
     kvc_scales s;                               // of pools of codes
+    float *wide;                                // WIDE_RESULTS: [request][query head][D], as the logarithms are by request then
 };
 
 template <typename T> struct Pair;
@@ -138,7 +139,7 @@ template <int KIND, int FIRST, int STEP> __device__ __forceinline__ uint32_t two
 template <int KIND> __device__ __forceinline__ uint32_t offset_codes(uint32_t c) { return KIND == KVC_CODES_INT8 ? c ^ 0x80808080u : c; }
 
 // The first of a request's rows of q and out, for b = B the first that is nobody's.  (Kept inside the tensors whatever `starts` hold, as lengths are.)
-template <bool ROWS> __device__ __forceinline__ int row_of(const Params &p, int b) { return ROWS ? min(max(p.starts[b], 0), p.rows) : b; }
+template <bool ROWS> __device__ __forceinline__ int row_of(const Params &p, int b) { return ROWS && p.starts ? min(max(p.starts[b], 0), p.rows) : b; }
 
 // The tokens of a request that count: [first, len).  None where it has no row, or more than one.
 struct Span { int first, len; };
@@ -270,10 +271,12 @@ __device__ __noinline__ void infinite_values(const Params &p, int b, int row, in
     __syncthreads();
 }
 
-// What a kernel's tiles are, by its channels and the kind of its rows (0: T).
+// What a kernel's tiles are, by its channels and the kind of its rows: T, codes, or T with results of 32 bits for whoever joins them with others (a call with prefixes).
+constexpr int WIDE_RESULTS = 3;
 template <int D, int KIND> struct Tiles {
-    static constexpr int TOKENS = KIND ? 32 : 16, ROW = KIND ? D : 2 * D;                   // tokens of a warp's tile, bytes of a row
-    static constexpr uint32_t HALF_STAGE = TOKENS * ROW, STAGE = 2 * HALF_STAGE + (KIND ? 8 * TOKENS : 0);     // keys, values; of codes their scales
+    static constexpr bool CODED = KIND == KVC_CODES_INT8 || KIND == KVC_CODES_E4M3;
+    static constexpr int TOKENS = CODED ? 32 : 16, ROW = CODED ? D : 2 * D;                 // tokens of a warp's tile, bytes of a row
+    static constexpr uint32_t HALF_STAGE = TOKENS * ROW, STAGE = 2 * HALF_STAGE + (CODED ? 8 * TOKENS : 0);     // keys, values; of codes their scales
 };
 
 // Rows of codes: a warp's tile has 32 tokens, as many bytes as 16 of 16 bits.  A token's score is its codes' times its key's scale.  Its weight is multiplied with its value's scale before
@@ -281,7 +284,7 @@ template <int D, int KIND> struct Tiles {
 // times a power of two for each head (what is 2^29 below the head's largest value loses bits, no less than a sum in 32 bits does).
 template <typename T, int D, int NT, int WH, bool SAME, int STAGES, int CTAS, bool ROWS, int KIND>
 __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_constant__ Params p) {
-    constexpr bool CODED = KIND != 0;
+    constexpr bool CODED = Tiles<D, KIND>::CODED;
     constexpr int KS = D / 16;                              // steps of 16 channels
     constexpr int TOKENS = Tiles<D, KIND>::TOKENS, ROW = Tiles<D, KIND>::ROW;
     constexpr int TEAM = WARPS / WH, TILE = TOKENS * TEAM;  // warps of a KV head, tokens of a tile
@@ -388,16 +391,20 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
     }
     // rows without tokens, and those that are nobody's
     auto nothing = [&](int row) {
-        for (int i = tid; i < (int)a.Hq * (D / 8); i += THREADS)
+        if (KIND != WIDE_RESULTS) for (int i = tid; i < (int)a.Hq * (D / 8); i += THREADS)
             *reinterpret_cast<uint4 *>(reinterpret_cast<T *>(a.out) + row * a.out_token + i / (D / 8) * a.out_head + i % (D / 8) * 8) = make_uint4(0, 0, 0, 0);
         if (a.lse) for (int h = tid; h < (int)a.Hq; h += THREADS) a.lse[row * a.Hq + h] = -CUDART_INF_F;
     };
     for (int b = blockIdx.x; b < B; b += gridDim.x) {
         if (tiles_of<TILE>(span_of<ROWS>(p, b, flags)) > 0) continue;
-        for (int row = row_of<ROWS>(p, b), end = ROWS ? row_of<ROWS>(p, b + 1) : b + 1; row < end; row++) nothing(row);
+        if (KIND == WIDE_RESULTS) nothing(b);
+        else for (int row = row_of<ROWS>(p, b), end = ROWS ? row_of<ROWS>(p, b + 1) : b + 1; row < end; row++) nothing(row);
     }
-    if (ROWS) for (int row = row_of<ROWS>(p, B) + (int)blockIdx.x; row < p.rows; row += (int)gridDim.x) nothing(row);
+    if (ROWS && KIND != WIDE_RESULTS) for (int row = row_of<ROWS>(p, B) + (int)blockIdx.x; row < p.rows; row += (int)gridDim.x) nothing(row);
+    // (in a call with prefixes what is ahead may still run, but not when this kernel has ended)
+    auto behind = [&]() { if (KIND == WIDE_RESULTS && blockIdx.x == gridDim.x - 1) cudaGridDependencySynchronize(); };
     if (r0 >= r1) {
+        behind();
         if (flags && a.status) atomicOr(a.status, flags);
         return;
     }
@@ -818,7 +825,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
                             }
                         }
                     }
-                const int of_b = at.b, of_row = ROWS ? min(row_of<ROWS>(p, at.b), p.rows - 1) : at.b, of_h0 = WH > 1 ? at.c * WH * p.group : h0, of_heads = WH * heads, pieces = of_heads * (D / 4);      // of all its KV heads
+                const int of_b = at.b, of_row = KIND == WIDE_RESULTS ? at.b : ROWS ? min(row_of<ROWS>(p, at.b), p.rows - 1) : at.b, of_h0 = WH > 1 ? at.c * WH * p.group : h0, of_heads = WH * heads, pieces = of_heads * (D / 4);      // of all its KV heads
                 const bool whole = first_i == 0 && at.i == at.n - 1;        // the column lies in this share
                 const int begin = r0 + n - at.i;            // its first tile in the row of tiles
                 const int tiles = at.n, of_piece = piece, place = 2 * piece + (n - (at.i - first_i) > 0);
@@ -840,8 +847,9 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
                 auto write = [&](int i, float top, float sum, const float4 &v) {       // four channels of a result
                     const int h = of_h0 + i / (D / 4), d = i % (D / 4) * 4;
                     const float f = sum == 0.0f ? 0.0f : 1.0f / sum, any = v.x + v.y + v.z + v.w;
-                    if (!CODED) odd |= any != any && sum == sum ? 1u << (h - of_h0) : 0;
-                    *reinterpret_cast<uint2 *>(reinterpret_cast<T *>(a.out) + of_row * a.out_token + h * a.out_head + d) =
+                    if (!CODED && KIND != WIDE_RESULTS) odd |= any != any && sum == sum ? 1u << (h - of_h0) : 0;
+                    if constexpr (KIND == WIDE_RESULTS) __stcg(reinterpret_cast<float4 *>(p.wide + ((long long)of_row * a.Hq + h) * D + d), make_float4(v.x * f, v.y * f, v.z * f, v.w * f));
+                    else *reinterpret_cast<uint2 *>(reinterpret_cast<T *>(a.out) + of_row * a.out_token + h * a.out_head + d) =
                         make_uint2(Pair<T>::pack(v.x * f, v.y * f), Pair<T>::pack(v.z * f, v.w * f));
                     if (d == 0 && a.lse) a.lse[of_row * a.Hq + h] = sum == 0.0f ? -CUDART_INF_F : (top + log2f(sum) - RESULT_LIFT) * 0.69314718055994531f;
                 };
@@ -970,7 +978,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
                         }
                     }
                 }
-                if constexpr (!CODED) if (odd_s) {          // (of 256 requests of 64 tokens, a column of one tile, asking takes 0.5 of 17.6 us, 8 x 4096 84.6 with and without)
+                if constexpr (!CODED && KIND != WIDE_RESULTS) if (odd_s) {      // (of 256 requests of 64 tokens, a column of one tile, asking takes 0.5 of 17.6 us, 8 x 4096 84.6 with and without)
                     __syncthreads();
                     if (tid == 0) odd_s = 0;
                     __syncthreads();
@@ -989,6 +997,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
         stage = stage + 1 == STAGES ? 0 : stage + 1;
     }
     copies_wait<0>();
+    behind();
     if (flags && a.status) atomicOr(a.status, flags);
 }
 
@@ -1008,6 +1017,20 @@ int launch_kernel(Params &p, cudaStream_t stream) {
     KVC_REQUIRE(p.a.B * p.columns < (1ll << 31) && most_tiles < (1ll << 31) - (1 << 20), "kvc_paged_attn: requests, KV heads and table rows of more than 2^31 tiles of %d tokens", TILE);
     const long long grid = std::max<long long>(std::min<long long>(most_tiles, (long long)std::min(occ, MAX_CTAS_PER_SM) * kvc_sm_count()), 1);
     p.per_cta = (float)(0.9999997 / grid);
+    if (KIND == WIDE_RESULTS) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)grid);
+        cfg.blockDim = dim3(THREADS);
+        cfg.dynamicSmemBytes = shared;
+        cfg.stream = stream;
+        cudaLaunchAttribute early;
+        early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        early.val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = &early;
+        cfg.numAttrs = 1;
+        KVC_CUDA_OK(cudaLaunchKernelEx(&cfg, kernel, (const Params)p));
+        return KVC_OK;
+    }
     kernel<<<(unsigned)grid, THREADS, shared, stream>>>(p);
     KVC_LAUNCH_OK();
     return KVC_OK;
@@ -1018,8 +1041,44 @@ int launch(Params &p, cudaStream_t s) {
     return p.starts ? launch_kernel<T, D, NT, WH, SAME, STAGES, CTAS, true, KIND>(p, s) : launch_kernel<T, D, NT, WH, SAME, STAGES, CTAS, false, KIND>(p, s);
 }
 
-// the kernels for rows of codes (a file of their own: they take as long to compile as the others)
+// the kernels for rows of codes, and those with results of 32 bits (files of their own: they take as long to compile as the others)
 int launch_codes(Params &p, cudaStream_t s);
+int launch_wide(Params &p, cudaStream_t s);
+
+// query heads that a column takes at most: 16 where they fit the registers beside the accumulators
+inline int group_of(int64_t Hq, int64_t Hkv, int64_t D) { return (int)std::min<int64_t>(Hq / Hkv, D > 128 ? 8 : MAX_GROUP); }
+inline int64_t columns_of(int64_t Hq, int64_t Hkv, int64_t D) { return Hkv * ((Hq / Hkv + group_of(Hq, Hkv, D) - 1) / group_of(Hq, Hkv, D)); }
+// Of partial results: two for every piece.  Of s tiles for a CTA s / 8 and those left by rounding down are drawn, in rounds of s / 16, s / 32, s / 64 (at least) and what these leave:
+// a CTA's share and five pieces more.
+inline int64_t places(int64_t D) { return 2ll * 6 * (D == 64 ? 4 : 3) * kvc_sm_count(); }
+// Floats of a place: of two KV heads where they are read together; room for eight heads at least, so that one workspace serves more shapes.  A multiple of four: values are
+// written and read sixteen bytes at a time, and n (D + 2) is two more than one for odd n.
+inline int64_t part_floats(int64_t group, int64_t D) { return (std::max<int64_t>(group <= 8 && D < 128 ? 2 * group : group, 8) * (D + 2) + 3) / 4 * 4; }
+// The counter of what is drawn, and two counters for a place: of the column whose first result lies there, of the eight results that begin there.  They lie in
+// front, the same for calls of all shapes: a workspace may serve one after the other.
+inline int64_t counter_bytes() { return 256 + (2 * places(64) * 4 + 255) / 256 * 256; }
+
+// What a call's arguments say, for a kernel: sizes have been checked.
+inline void set_params(Params &p, const kvc_paged_attn_args &a, const int32_t *starts, int64_t rows) {
+    p.a = a;
+    p.page = kvc_make_div((uint32_t)a.page_size);
+    p.group = group_of(a.Hq, a.Hkv, a.D);
+    p.columns = (int)columns_of(a.Hq, a.Hkv, a.D);
+    p.per_head = p.columns / (int)a.Hkv;
+    p.chunk = (int)((a.B + 31) / 32);
+    p.most_tokens = (int)(a.table_width * a.page_size);
+    p.n_pages = (unsigned)a.n_pages;
+    p.starts = starts;
+    p.rows = (int)rows;
+    p.negative = a.scaling < 0.0f;
+    p.log2_scaling = std::max(fabsf(a.scaling) * 1.4426950408889634f, 1e-37f);      // (0 times the -inf of a token that is left out is none)
+    p.part = (int)part_floats(p.group, a.D);
+    p.drawn = reinterpret_cast<int *>(a.workspace);
+    p.counters = reinterpret_cast<unsigned *>(a.workspace) + 64;
+    p.group_counters = p.counters + places(64);
+    p.parts = reinterpret_cast<float *>(reinterpret_cast<uint8_t *>(a.workspace) + counter_bytes());
+    p.v_less_k = reinterpret_cast<const uint8_t *>(a.vpages) - reinterpret_cast<const uint8_t *>(a.kpages);
+}
 
 }  // namespace kvc_paged
 

@@ -1,16 +1,16 @@
 // Attention of one new token per request where requests continue a common prefix: the prefix is read once for all that follow it.
 //
-// out = sum_t w_t v_t / sum_t w_t with w_t = exp(scaling q . k_t - m), over the tokens of the prefix and the request's own ones.  The sums of both, and of any parts of them, are kept
-// with their maxima and joined: the tokens are a prefix's, times all queries that follow it, or a request's own, times its queries.
+// out = sum_t w_t v_t / sum_t w_t with w_t = exp(scaling q . k_t - m), over the tokens of the prefix and the request's own ones.  The sums of any parts of the tokens are kept with their
+// maxima and joined.  Three kernels: prefixes, times all queries that follow them; the requests' own tokens (the kernel of calls without prefixes, with results of 32 bits); the joining.
 //
-// What bounds it: of n requests with g query heads on a KV head, n g rows meet every key and value of the prefix, 4 n g D operations for 4 D bytes: HBM up to some 250 rows, the tensor
-// cores and the exponentials beyond.  mma.sync (what the attention without prefixes uses, at 8 rows) gives a quarter of that; so here tcgen05: 128 rows by 128 tokens, the scores in tensor
-// memory, the weights in 16 bits beside them as the second product's operand, the sums there too.  Two sets of 128 rows take turns: while the exponentials of one are made the other's
+// What bounds the first: of n requests with g query heads on a KV head, n g rows meet every key and value of the prefix, 4 n g D operations for 4 D bytes: HBM up to some 250 rows, the tensor
+// cores and the exponentials beyond.  mma.sync (what the second kernel uses, at 8 rows) gives a quarter of that; so here tcgen05: 128 rows by 128 tokens, the scores in tensor
+// memory, the weights in 16 bits in their place as the second product's operand, the sums there too.  Two sets of 128 rows take turns: while the exponentials of one are made the other's
 // products run.  Columns of more than 128 rows use both sets with the same tokens; columns of fewer give them every other tile.
 //
-// Work is cut into tiles of 128 tokens of a column (an item's KV head and up to 256 of its rows; an item is a prefix or a request's own tokens), all tiles of all columns in one row; each CTA, one
-// on an SM, takes an equal, contiguous share, found from the lengths in the kernel.  What a CTA finds for a column goes to the workspace; a second kernel joins the
-// parts, in the order of the shares, so that results do not depend on timing.
+// Work is cut into tiles of 128 tokens of a column (a prefix's KV head and up to 256 of its followers' rows), all tiles of all columns in one row; each CTA, one on an SM, takes an
+// equal, contiguous share, found from the lengths in the kernel.  What a CTA finds for a column goes to the workspace; the third kernel joins the parts, in the order of the
+// shares, so that results do not depend on timing.
 //
 // Keys and values come by 16-byte asynchronous copies (pages end anywhere, any strides) into a ring in shared memory, in the 128-byte swizzled layout that the products read: keys
 // channel by channel, values as they lie (token by token: the product's second operand turned).  Rounding: the weights are fp16 (times 2^7: 2^-21 of the largest are still normal numbers) or bf16,
@@ -20,11 +20,13 @@
 
 #include <algorithm>
 
-#include "kvc_paged.cuh"
+#include "kvc_paged_attn.cuh"
 
 namespace {
 
-constexpr int THREADS = 384, ROWS = 128, TOKENS = 128, ATOM = 16384;       // ATOM: 128 rows of 128 bytes
+using kvc_paged::Params, kvc_paged::set_params, kvc_paged::launch_wide, kvc_paged::counter_bytes, kvc_paged::places, kvc_paged::group_of, kvc_paged::part_floats, kvc_paged::columns_of;
+
+constexpr int PREFIX_THREADS = 384, ROWS = 128, TOKENS = 128, ATOM = 16384;       // ATOM: 128 rows of 128 bytes
 constexpr int MASKS = 16;
 constexpr int MAX_REQUESTS = 16384;
 
@@ -131,7 +133,7 @@ __global__ void __launch_bounds__(SCAN_THREADS) prefix_scan_kernel(const __grid_
 
 // ---- the attention --------------------------------------------------------------------------------------------------
 
-struct Params {
+struct Prefix {
     kvc_paged_attn_args a;
     const int32_t *plan, *starts;                           // starts null: row b is request b's
     kvc_div page, group;                                    // divisors: page size, query heads of a KV head
@@ -140,38 +142,33 @@ struct Params {
     int negative;
     float log2_scaling;
     int32_t *item_first, *share;                            // (workspace) the items' first tiles, and the tiles of a share
+    float *own, *own_lse;                                   // (workspace) results of the requests' own tokens [request][query head][D], logarithms of their sums
     float *sums;                                            // (workspace) of places of D floats
     float2 *maxima;                                         // maximum and sum of weights of a place
 };
 
-// Places: of column parts that begin with the column [prefix or own][request][head][2]; behind them of those that begin with a CTA's share [CTA][256].
-__device__ __forceinline__ long long place_of(const Params &p, bool own, int b, int h, int i) { return (((own ? p.a.B : 0) + b) * p.a.Hq + h) * 2 + i; }
-__device__ __forceinline__ long long cta_place(const Params &p, int cta, int i) { return p.a.B * p.a.Hq * 4 + (long long)cta * 256 + i; }
+// Places: of column parts that begin with the column [request][head][2]; behind them of those that begin with a CTA's share [CTA][256].
+__device__ __forceinline__ long long place_of(const Prefix &p, int b, int h, int i) { return (b * p.a.Hq + h) * 2 + i; }
+__device__ __forceinline__ long long cta_place(const Prefix &p, int cta, int i) { return p.a.B * p.a.Hq * 2 + (long long)cta * 256 + i; }
 
-__device__ __forceinline__ int row_at(const Params &p, int b) { return p.starts ? min(max(p.starts[b], 0), p.rows) : b; }
-__device__ __forceinline__ int member_at(const Params &p, int i) { return min(max(p.plan[plan_order(p.a.B) + i], 0), (int)p.a.B - 1); }
+__device__ __forceinline__ int row_at(const Prefix &p, int b) { return p.starts ? min(max(p.starts[b], 0), p.rows) : b; }
+__device__ __forceinline__ int member_at(const Prefix &p, int i) { return min(max(p.plan[plan_order(p.a.B) + i], 0), (int)p.a.B - 1); }
 // the row of a request's token, -1: it has none, or more than one
-__device__ __forceinline__ int row_of(const Params &p, int b) {
+__device__ __forceinline__ int row_of(const Prefix &p, int b) {
     if (!p.starts) return b;
     const int row = row_at(p, b);
     return row_at(p, b + 1) - row == 1 ? row : -1;
 }
-__device__ __forceinline__ int length_of(const Params &p, int b) { return min(max(p.a.lengths[b], 0), p.most_tokens); }
+__device__ __forceinline__ int length_of(const Prefix &p, int b) { return min(max(p.a.lengths[b], 0), p.most_tokens); }
 
-struct Item { int table, first, rows, len, tiles, parts; };  // whose pages, the first member in the order (or the request itself), rows of a KV head, tokens, tiles of a column, columns of a KV head
-__device__ __forceinline__ Item item_of(const Params &p, int i, int groups) {
+struct Item { int table, first, rows, len, tiles, parts; };  // whose pages, the first member in the order, rows of a KV head, tokens, tiles of a column, columns of a KV head
+__device__ __forceinline__ Item item_of(const Prefix &p, int i) {
     Item r;
     const int B = (int)p.a.B;
-    if (i < groups) {
-        r.first = min(max(p.plan[plan_first(B) + i], 0), B);               // (kept inside the arrays whatever the plan holds, as lengths are)
-        r.rows = min(max(p.plan[plan_first(B) + i + 1] - r.first, 0), B - r.first) * p.g;
-        r.table = min(max(p.plan[plan_parent(B) + i], 0), B - 1);
-        r.len = r.rows == 0 ? 0 : min(max(p.plan[plan_shared(B) + i], 0), length_of(p, r.table));
-    } else {
-        r.first = r.table = i - groups;
-        r.rows = p.g;
-        r.len = row_of(p, r.table) >= 0 ? length_of(p, r.table) : 0;
-    }
+    r.first = min(max(p.plan[plan_first(B) + i], 0), B);               // (kept inside the arrays whatever the plan holds, as lengths are)
+    r.rows = min(max(p.plan[plan_first(B) + i + 1] - r.first, 0), B - r.first) * p.g;
+    r.table = min(max(p.plan[plan_parent(B) + i], 0), B - 1);
+    r.len = r.rows == 0 ? 0 : min(max(p.plan[plan_shared(B) + i], 0), length_of(p, r.table));
     r.tiles = (r.len + TOKENS - 1) / TOKENS;
     r.parts = (r.rows + 2 * ROWS - 1) / (2 * ROWS);
     return r;
@@ -194,17 +191,16 @@ __device__ __forceinline__ void begin_column(Walk &w) {
     w.in_part = min(w.it.tiles - w.tile, w.left);
     w.first_job = w.jobs;
 }
-__device__ __forceinline__ void next_tile(const Params &p, Walk &w, int groups) {
+__device__ __forceinline__ void next_tile(const Prefix &p, Walk &w, int groups) {
     w.jobs += w.wide ? 2 : 1;
     if (--w.left == 0) return;
     if (++w.tile < w.it.tiles) return;
     w.tile = 0;
     if (++w.column == w.it.parts * (int)p.a.Hkv) {
         w.column = 0;
-        const int items = groups + (int)p.a.B;
         do {
-            if (++w.item >= items) { w.left = 0; return; }      // (lengths that changed meanwhile)
-            w.it = item_of(p, w.item, groups);
+            if (++w.item >= groups) { w.left = 0; return; }     // (lengths that changed meanwhile)
+            w.it = item_of(p, w.item);
         } while (w.it.tiles == 0);
     }
     begin_column(w);
@@ -280,16 +276,17 @@ template <int D> struct Shape {
 };
 
 template <typename T, int D>
-__global__ void __launch_bounds__(THREADS, 1) prefix_attn_kernel(const __grid_constant__ Params p) {
-    constexpr int ATOMS = Shape<D>::ATOMS, UNIT = Shape<D>::UNIT, RING = Shape<D>::RING;
+__global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_attn_kernel(const __grid_constant__ Prefix p) {
+    constexpr int UNIT = Shape<D>::UNIT, RING = Shape<D>::RING;
     constexpr float LIFT = Weight<T>::LIFT;
     extern __shared__ uint8_t raw[];
     __shared__ __align__(8) uint64_t full[RING], empty[RING], scores_there[2], weights_there[2], sums_there[2], queries_free[2];
     __shared__ uint32_t masks[MASKS][4], tensor_s;
-    __shared__ int failed_s, warp_sums[THREADS / 32], start_item, start_rest;
+    __shared__ int failed_s, warp_sums[PREFIX_THREADS / 32], start_item, start_rest;
     const kvc_paged_attn_args &a = p.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, B = (int)a.B;
     volatile int *failed = &failed_s;
+    cudaTriggerProgrammaticLaunchCompletion();              // (the kernel of the requests' own tokens, which reads nothing of this one's, may begin where there is room)
     const uint32_t base = (shared_at(raw) + 1023) & ~1023u, ring = base + 2 * UNIT;
 
     if (warp == 8) {
@@ -304,11 +301,11 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_attn_kernel(const __grid_co
     }
 
     // ---- this CTA's share
-    const int groups = min(max(p.plan[0], 0), B), items = groups + B;
+    const int groups = min(max(p.plan[0], 0), B);
     int flags = 0, total = 0;
     auto scan = [&](int i0, int &tiles) {                   // (first tile of item i0 + tid, its tiles; `total` grows)
         Item it = {};
-        if (i0 + tid < items) it = item_of(p, i0 + tid, groups);
+        if (i0 + tid < groups) it = item_of(p, i0 + tid);
         tiles = it.tiles * it.parts * (int)a.Hkv;
         int sum = tiles;
 #pragma unroll
@@ -320,33 +317,29 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_attn_kernel(const __grid_co
         if (lane == 31) warp_sums[warp] = sum;
         __syncthreads();
         int before = total;
-        for (int w = 0; w < THREADS / 32; w++) {
+        for (int w = 0; w < PREFIX_THREADS / 32; w++) {
             if (w < warp) before += warp_sums[w];
             total += warp_sums[w];
         }
         return before + sum - tiles;
     };
     int tiles = 0, first = 0;
-    for (int i0 = 0; i0 < items; i0 += THREADS) {
+    for (int i0 = 0; i0 < groups; i0 += PREFIX_THREADS) {
         first = scan(i0, tiles);
-        if (blockIdx.x == 0 && i0 + tid < items) p.item_first[i0 + tid] = first;
+        if (blockIdx.x == 0 && i0 + tid < groups) p.item_first[i0 + tid] = first;
     }
     const int all = total, size = max(1, (all + p.grid - 1) / p.grid), r0 = (int)min((long long)all, (long long)size * blockIdx.x), r1 = min(all, r0 + size);
     if (blockIdx.x == 0 && tid == 0) *p.share = size;
     if (r0 < r1) {
-        if (items > THREADS) total = 0;
-        for (int i0 = 0; i0 < items; i0 += THREADS) {
-            if (items > THREADS) first = scan(i0, tiles);
+        if (groups > PREFIX_THREADS) total = 0;
+        for (int i0 = 0; i0 < groups; i0 += PREFIX_THREADS) {
+            if (groups > PREFIX_THREADS) first = scan(i0, tiles);
             if (r0 >= first && r0 < first + tiles) { start_item = i0 + tid; start_rest = r0 - first; }
         }
     }
-    if (blockIdx.x == gridDim.x - 1) {                      // lengths and rows that are none
-        for (int b = tid; b < B; b += THREADS) {
-            if (a.lengths[b] < 0 || a.lengths[b] > p.most_tokens || (p.starts && row_at(p, b + 1) - row_at(p, b) > 1)) flags |= KVC_FLAG_BAD_LENGTH;
-            const int group = p.plan[plan_group(B) + b];
-            if (group >= 0 && group < groups && item_of(p, group, groups).len < p.plan[plan_shared(B) + group]) flags |= KVC_FLAG_BAD_LENGTH;
-        }
-    }
+    if (blockIdx.x == gridDim.x - 1)                        // prefixes that are longer than what there is
+        for (int i = tid; i < groups; i += PREFIX_THREADS)
+            if (item_of(p, i).len < p.plan[plan_shared(B) + i]) flags |= KVC_FLAG_BAD_LENGTH;
     before_sync();
     __syncthreads();
     after_sync();
@@ -357,7 +350,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_attn_kernel(const __grid_co
         w.left = r1 - r0;
         w.jobs = 0;
         w.item = start_item;
-        w.it = item_of(p, w.item, groups);
+        w.it = item_of(p, w.item);
         w.column = start_rest / w.it.tiles;
         w.tile = start_rest - w.column * w.it.tiles;
         begin_column(w);
@@ -381,9 +374,9 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_attn_kernel(const __grid_co
                     const int R = w.part * 2 * ROWS + half * ROWS + r;
                     mine = R < w.it.rows;
                     if (mine) {
-                        const int member = kvc_divide(R, p.group), h = w.k_head * p.g + R - member * p.g, b = w.item < groups ? member_at(p, w.it.first + member) : w.it.first;
+                        const int member = kvc_divide(R, p.group), h = w.k_head * p.g + R - member * p.g, b = member_at(p, w.it.first + member);
                         mine = row_of(p, b) >= 0;
-                        const long long place = w.of_column == 0 ? place_of(p, w.item >= groups, b, h, w.wide ? 0 : part_i) : cta_place(p, blockIdx.x, part_i * ROWS + r);
+                        const long long place = w.of_column == 0 ? place_of(p, b, h, w.wide ? 0 : part_i) : cta_place(p, blockIdx.x, part_i * ROWS + r);
                         to = p.sums + place * D;
                         to_max = p.maxima + place;
                     }
@@ -466,7 +459,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_attn_kernel(const __grid_co
                                     __stcg(reinterpret_cast<uint4 *>(to) + 8 * c + i, make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]));
                             }
                         }
-                        if (mine) __stcg(to_max, make_float2(m, l));
+                        if (mine) __stcg(to_max, make_float2(m - LIFT, l));     // (weights were 2^LIFT times what the maximum says)
                     }
                     before_sync();
                 }
@@ -562,7 +555,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_attn_kernel(const __grid_co
                                     loads[set]++;
                                     for (int i = lane; i < n * (D / 8); i += 32) {
                                         const int r = i / (D / 8), c = i % (D / 8), R = from + r, member = kvc_divide(R, p.group), h = w.k_head * p.g + R - member * p.g;
-                                        const int b = w.item < groups ? member_at(p, w.it.first + member) : w.it.first, row = row_of(p, b);
+                                        const int b = member_at(p, w.it.first + member), row = row_of(p, b);
                                         copy16(base + set * UNIT + (c >> 3) * ATOM + r * 128 + ((c & 7) ^ (r & 7)) * 16,
                                                reinterpret_cast<const T *>(a.q) + (long long)max(row, 0) * a.q_token + h * a.q_head + c * 8, row >= 0);
                                     }
@@ -619,7 +612,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefix_attn_kernel(const __grid_co
 // ---- the parts of a row's sums are joined ---------------------------------------------------------------------------
 
 template <typename T, int D>
-__global__ void __launch_bounds__(128) prefix_join_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(128) prefix_join_kernel(const __grid_constant__ Prefix p) {
     kvc_behind();
     const kvc_paged_attn_args &a = p.a;
     const int lane = threadIdx.x & 31, B = (int)a.B, quads = (int)(a.Hq + 3) / 4, b = blockIdx.x / quads, h = (blockIdx.x - b * quads) * 4 + (threadIdx.x >> 5);
@@ -639,8 +632,11 @@ __global__ void __launch_bounds__(128) prefix_join_kernel(const __grid_constant_
         return;
     }
     const int groups = min(max(p.plan[0], 0), B), group = min(p.plan[plan_group(B) + b], groups - 1), size = *p.share, k_head = kvc_divide(h, p.group);
-    float top = -CUDART_INF_F, sum = 0.0f;
+    // the request's own tokens: a result and the logarithm of its weights' sum
+    const float own = p.own_lse[b * a.Hq + h];
+    float top = own * 1.4426950408889634f, sum = own == -CUDART_INF_F ? 0.0f : 1.0f;
     float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (on && own != -CUDART_INF_F) v = __ldcg(reinterpret_cast<const float4 *>(p.own + (b * a.Hq + h) * D) + lane);
     auto add = [&](float2 ml, float4 x) {
         const float now = fmaxf(top, ml.x), less = now == -CUDART_INF_F ? 0.0f : now, f = exp2_approx(top - less), g = exp2_approx(ml.x - less);
         sum = sum * f + ml.y * g;
@@ -648,18 +644,15 @@ __global__ void __launch_bounds__(128) prefix_join_kernel(const __grid_constant_
         v.x = v.x * f + x.x * g; v.y = v.y * f + x.y * g; v.z = v.z * f + x.z * g; v.w = v.w * f + x.w * g;
         top = now;
     };
-    for (int own = 0; own < 2; own++) {
-        if (!own && group < 0) continue;
-        const int i = own ? groups + b : group;
-        const Item it = item_of(p, i, groups);
-        if (it.tiles == 0) continue;
-        const int R = (own ? 0 : min(max(p.plan[plan_rank(B) + b], 0), it.rows / p.g - 1)) * p.g + h - k_head * p.g, part = R / (2 * ROWS), in_part = R - part * 2 * ROWS;
+    if (group >= 0) {
+        const Item it = item_of(p, group);
+        const int R = min(max(p.plan[plan_rank(B) + b], 0), it.rows / p.g - 1) * p.g + h - k_head * p.g, part = R / (2 * ROWS), in_part = R - part * 2 * ROWS;
         const bool wide = it.rows - part * 2 * ROWS > ROWS;
-        const int from = p.item_first[i] + (k_head * it.parts + part) * it.tiles, to = from + it.tiles;
+        const int from = p.item_first[group] + (k_head * it.parts + part) * it.tiles, to = from + it.tiles;
         // a column's parts: each in a CTA's share, of narrow columns two (every other tile) where it has more than one
         const int cta0 = from / size, cta1 = (to - 1) / size, each = wide ? 1 : 2;
         constexpr int AT_ONCE = 4;
-        for (int k0 = 0; k0 < (cta1 - cta0 + 1) * each; k0 += AT_ONCE) {
+        for (int k0 = 0; it.tiles > 0 && k0 < (cta1 - cta0 + 1) * each; k0 += AT_ONCE) {
             float2 ml[AT_ONCE];
             float4 x[AT_ONCE];
 #pragma unroll
@@ -669,7 +662,7 @@ __global__ void __launch_bounds__(128) prefix_join_kernel(const __grid_constant_
                 ml[k] = make_float2(-CUDART_INF_F, 0.0f);
                 x[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                 if (cta <= cta1 && which < there) {
-                    const long long place = cta == cta0 ? place_of(p, own, b, h, which) : cta_place(p, cta, wide ? in_part : which * ROWS + in_part);
+                    const long long place = cta == cta0 ? place_of(p, b, h, which) : cta_place(p, cta, wide ? in_part : which * ROWS + in_part);
                     ml[k] = __ldcg(p.maxima + place);
                     if (on) x[k] = __ldcg(reinterpret_cast<const float4 *>(p.sums + place * D) + lane);
                 }
@@ -681,22 +674,24 @@ __global__ void __launch_bounds__(128) prefix_join_kernel(const __grid_constant_
     }
     const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
     if (on) *reinterpret_cast<uint2 *>(reinterpret_cast<T *>(a.out) + row * a.out_token + h * a.out_head + lane * 4) = make_uint2(pack(v.x * f, v.y * f, T()), pack(v.z * f, v.w * f, T()));
-    if (lane == 0 && a.lse) a.lse[row * a.Hq + h] = sum == 0.0f ? -CUDART_INF_F : (top + log2f(sum) - Weight<T>::LIFT) * 0.69314718055994531f;
+    if (lane == 0 && a.lse) a.lse[row * a.Hq + h] = sum == 0.0f ? -CUDART_INF_F : (top + log2f(sum)) * 0.69314718055994531f;
 }
 
 template <typename T, int D>
-int launch(Params &p, cudaStream_t s) {
+int launch(Prefix &p, Params &own, cudaStream_t s) {
     static kvc_launch_slot slot;
     int occ = 0;
-    if (int rc = kvc_prepare(slot, reinterpret_cast<const void *>(prefix_attn_kernel<T, D>), THREADS, Shape<D>::SHARED, &occ)) return rc;
+    if (int rc = kvc_prepare(slot, reinterpret_cast<const void *>(prefix_attn_kernel<T, D>), PREFIX_THREADS, Shape<D>::SHARED, &occ)) return rc;
     KVC_REQUIRE(occ > 0, "kvc_paged_attn_shared: the kernel does not fit this device");
-    prefix_attn_kernel<T, D><<<(unsigned)p.grid, THREADS, Shape<D>::SHARED, s>>>(p);
+    prefix_attn_kernel<T, D><<<(unsigned)p.grid, PREFIX_THREADS, Shape<D>::SHARED, s>>>(p);
     KVC_LAUNCH_OK();
+    if (int rc = launch_wide(own, s)) return rc;
     return kvc_launch_early(prefix_join_kernel<T, D>, (unsigned)((p.a.B + 1) * ((p.a.Hq + 3) / 4)), 128, s, p);
 }
 
-int64_t item_bytes(int64_t B) { return (4 * (2 * B + 1) + 255) / 256 * 256; }
-int64_t places(int64_t B, int64_t Hq) { return 4 * B * Hq + 256ll * kvc_sm_count(); }
+int64_t rounded(int64_t bytes) { return (bytes + 255) / 256 * 256; }
+int64_t prefix_places(int64_t B, int64_t Hq) { return 2 * B * Hq + 256ll * kvc_sm_count(); }
+int64_t own_bytes(int64_t Hq, int64_t Hkv, int64_t D) { return rounded(counter_bytes() + places(D) * part_floats(group_of(Hq, Hkv, D), D) * 4); }      // of the kernel for own tokens
 
 }  // namespace
 
@@ -716,12 +711,12 @@ extern "C" int kvc_prefix_plan(const kvc_prefix_plan_args *args, kvc_stream_t st
 
 extern "C" int64_t kvc_paged_attn_shared_workspace(int64_t B, int64_t Hq, int64_t Hkv, int64_t D) {
     if (B < 0 || Hkv <= 0 || Hq < Hkv || D <= 0) return 0;
-    return item_bytes(B) + places(B, Hq) * (4 * D + 8);
+    return own_bytes(Hq, Hkv, D) + rounded(4 * (B + 1)) + rounded(4 * B * Hq * (D + 1)) + prefix_places(B, Hq) * (4 * D + 8);
 }
 
 extern "C" int kvc_paged_attn_shared(const kvc_paged_attn_args *args, const int32_t *plan, const int32_t *starts, int64_t rows, kvc_stream_t stream) {
     KVC_REQUIRE(args && plan, "kvc_paged_attn_shared: null pointer");
-    Params p;
+    Prefix p;
     memcpy(&p.a, args, sizeof(p.a));
     kvc_paged_attn_args &a = p.a;
     KVC_REQUIRE(a.type == KVC_TYPE_FP16 || a.type == KVC_TYPE_BF16, "kvc_paged_attn_shared: unknown type %d", a.type);
@@ -736,6 +731,7 @@ extern "C" int kvc_paged_attn_shared(const kvc_paged_attn_args *args, const int3
     KVC_REQUIRE(a.q && a.out && a.lengths && (a.table || a.table_width == 0) && ((a.kpages && a.vpages) || a.n_pages == 0), "kvc_paged_attn_shared: null pointer");
     const int64_t g = a.Hq / a.Hkv, most_tiles = (a.table_width * a.page_size + TOKENS - 1) / TOKENS;
     KVC_REQUIRE(a.Hkv * (2 * a.B + a.B * g / (2 * ROWS)) < (1ll << 31) / std::max<int64_t>(most_tiles, 1), "kvc_paged_attn_shared: requests, KV heads and table rows of more than 2^31 tiles");
+    KVC_REQUIRE(a.B * columns_of(a.Hq, a.Hkv, a.D) * ((a.table_width * a.page_size + 31) / 32) < (1ll << 31) - (1 << 20), "kvc_paged_attn_shared: requests, KV heads and table rows of more than 2^31 tiles");
     const uintptr_t at = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.kpages) | reinterpret_cast<uintptr_t>(a.vpages) | reinterpret_cast<uintptr_t>(a.out);
     if (a.Hq == 1) a.q_head = a.out_head = 0;              // (the stride of a dimension of one may be anything)
     if (rows == 1) a.q_token = a.out_token = 0;
@@ -763,13 +759,22 @@ extern "C" int kvc_paged_attn_shared(const kvc_paged_attn_args *args, const int3
     p.n_pages = (unsigned)a.n_pages;
     p.negative = a.scaling < 0.0f;
     p.log2_scaling = std::max(fabsf(a.scaling) * 1.4426950408889634f, 1e-37f);      // (0 times the -inf of a token that is left out is none)
-    p.item_first = reinterpret_cast<int32_t *>(a.workspace);
-    p.share = p.item_first + 2 * a.B;
-    p.sums = reinterpret_cast<float *>(reinterpret_cast<uint8_t *>(a.workspace) + item_bytes(a.B));
-    p.maxima = reinterpret_cast<float2 *>(p.sums + places(a.B, a.Hq) * a.D);
+    uint8_t *at_ws = reinterpret_cast<uint8_t *>(a.workspace) + own_bytes(a.Hq, a.Hkv, a.D);
+    p.item_first = reinterpret_cast<int32_t *>(at_ws);
+    p.share = p.item_first + a.B;
+    at_ws += rounded(4 * (a.B + 1));
+    p.own = reinterpret_cast<float *>(at_ws);
+    p.own_lse = p.own + a.B * a.Hq * a.D;
+    at_ws += rounded(4 * a.B * a.Hq * (a.D + 1));
+    p.sums = reinterpret_cast<float *>(at_ws);
+    p.maxima = reinterpret_cast<float2 *>(p.sums + prefix_places(a.B, a.Hq) * a.D);
+    Params own = {};
+    set_params(own, a, starts, rows);
+    own.wide = p.own;
+    own.a.lse = p.own_lse;
     cudaStream_t s = kvc_cu(stream);
     const bool fp16 = a.type == KVC_TYPE_FP16;
-    if (a.D == 64) return fp16 ? launch<__half, 64>(p, s) : launch<__nv_bfloat16, 64>(p, s);
-    if (a.D == 96) return fp16 ? launch<__half, 96>(p, s) : launch<__nv_bfloat16, 96>(p, s);
-    return fp16 ? launch<__half, 128>(p, s) : launch<__nv_bfloat16, 128>(p, s);
+    if (a.D == 64) return fp16 ? launch<__half, 64>(p, own, s) : launch<__nv_bfloat16, 64>(p, own, s);
+    if (a.D == 96) return fp16 ? launch<__half, 96>(p, own, s) : launch<__nv_bfloat16, 96>(p, own, s);
+    return fp16 ? launch<__half, 128>(p, own, s) : launch<__nv_bfloat16, 128>(p, own, s);
 }

@@ -851,12 +851,16 @@ def prefix_plan(parents, shared, out=None, status=None):
 
 
 def paged_attn_shared_workspace(B, Hq, Hkv, D, device):
-    """Workspace for paged_attn_shared (reusable across calls that follow one another; concurrent streams need their own, and so do graphs that may run at once)."""
+    """Workspace for paged_attn_shared, its counters zeroed (reusable across calls that follow one another; concurrent streams need their own, and so do graphs that may run at once).  Made
+    while a graph is captured it is zeroed by the graph, and serves that graph only."""
     index = torch.empty(0, device=device).get_device()
     if index < 0:
         raise KvcError("paged_attn_shared_workspace: %s is no CUDA device" % (device,))
     with _on(torch.device("cuda", index)):
-        return torch.empty(_lib.load().kvc_paged_attn_shared_workspace(B, Hq, Hkv, D), dtype=torch.uint8, device=torch.device("cuda", index))
+        lib = _lib.load()
+        workspace = torch.empty(lib.kvc_paged_attn_shared_workspace(B, Hq, Hkv, D), dtype=torch.uint8, device=torch.device("cuda", index))
+        workspace[:lib.kvc_paged_attn_cleared()].zero_()
+    return workspace
 
 
 def paged_attn_shared(q, kpages, vpages, table, lengths, plan, scaling, out=None, return_lse=False, workspace=None, status=None, starts=None):

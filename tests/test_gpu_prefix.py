@@ -93,7 +93,8 @@ def attend(ops, prefixes, members, own, Hq, Hkv, D, dtype, page=16, seed=0, shar
     status = ops.new_status(torch.device("cuda"))
     plan = ops.prefix_plan(dev(parents), dev(shared), status=status)
     workspace = ops.paged_attn_shared_workspace(n, Hq, Hkv, D, "cuda")
-    workspace.view(torch.int32).fill_(0x7fc00000)                   # (nothing relies on what was there: NaN)
+    from kvcomp_b200 import _lib
+    workspace[_lib.load().kvc_paged_attn_cleared():].view(torch.int32).fill_(0x7fc00000)            # (nothing relies on what was there: NaN)
     call = lambda: ops.paged_attn_shared(q, kp, vp, dev(table), dev(lengths), plan, scaling, return_lse=True, workspace=workspace, status=status, starts=None if starts is None else dev(starts))  # noqa: E731
     out, lse = call()
     assert int(status.item()) == 0
