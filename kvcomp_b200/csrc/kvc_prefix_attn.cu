@@ -26,7 +26,7 @@ namespace {
 
 using kvc_paged::Params, kvc_paged::set_params, kvc_paged::launch_wide, kvc_paged::counter_bytes, kvc_paged::places, kvc_paged::group_of, kvc_paged::part_floats, kvc_paged::columns_of;
 
-constexpr int PREFIX_THREADS = 384, ROWS = 128, TOKENS = 128, ATOM = 16384;       // ATOM: 128 rows of 128 bytes
+constexpr int PREFIX_THREADS = 512, LOADERS = 7, ROWS = 128, TOKENS = 128, ATOM = 16384;       // ATOM: 128 rows of 128 bytes
 constexpr int MASKS = 16;
 constexpr int MAX_REQUESTS = 16384;
 
@@ -210,18 +210,19 @@ __device__ __forceinline__ void next_tile(const Prefix &p, Walk &w, int groups) 
 __device__ __forceinline__ uint32_t shared_at(const void *v) { return (uint32_t)__cvta_generic_to_shared(v); }
 __device__ __forceinline__ void bar_init(uint64_t *bar, int count) { asm volatile("mbarrier.init.shared.b64 [%0], %1;" ::"r"(shared_at(bar)), "r"(count)); }
 __device__ __forceinline__ void bar_arrive(uint64_t *bar) { asm volatile("mbarrier.arrive.shared.b64 _, [%0];" ::"r"(shared_at(bar)) : "memory"); }
-__device__ __forceinline__ bool bar_try(uint64_t *bar, uint32_t parity, uint32_t ns) {
+__device__ __forceinline__ bool bar_try(uint64_t *bar, uint32_t parity) {
     uint32_t done;
-    asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared.b64 p, [%1], %2, %3; selp.u32 %0, 1, 0, p; }" : "=r"(done) : "r"(shared_at(bar)), "r"(parity), "r"(ns) : "memory");
+    asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }" : "=r"(done) : "r"(shared_at(bar)), "r"(parity) : "memory");
     return done;
 }
 // Waits up to about a second; what runs out is said in *failed, and nothing waits any more then.
 __device__ __forceinline__ void bar_wait(uint64_t *bar, uint32_t parity, volatile int *failed) {
-    for (int n = 0; n < 1 << 20; n++) {
-        if (bar_try(bar, parity, 1000)) return;
+    if (bar_try(bar, parity)) return;
+    const long long until = clock64() + (1ll << 31);
+    while (!bar_try(bar, parity)) {
         if (*failed) return;
+        if (clock64() > until) { *failed = 1; return; }
     }
-    *failed = 1;
 }
 __device__ __forceinline__ void copy16(uint32_t to, const void *from, bool on) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(on ? 16 : 0) : "memory");
@@ -265,6 +266,21 @@ __device__ __forceinline__ float exp2_approx(float x) {
     return r;
 }
 
+// Rows 32 i .. 32 i + 31 of a tile, by a warp: `from` is the lane's own row, mask says which there are (the others become zeros).
+template <typename T, int D> __device__ __forceinline__ void copy_rows(uint32_t to, int i, const T *from, uint32_t mask, int lane) {
+    constexpr int SIDE = D == 96 ? 4 : D / 8 > 16 ? 16 : D / 8;                           // lanes of a row
+#pragma unroll 4
+    for (int k = 0; k < SIDE; k++) {
+        const int j = k * (32 / SIDE) + lane / SIDE, r = 32 * i + j;
+        const T *row = reinterpret_cast<const T *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(from), j));
+#pragma unroll
+        for (int c0 = 0; c0 < D / 8; c0 += SIDE) {
+            const int c = c0 + lane % SIDE;
+            copy16(to + (c >> 3) * ATOM + r * 128 + ((c & 7) ^ (r & 7)) * 16, row + c * 8, mask >> j & 1);
+        }
+    }
+}
+
 template <typename T> struct Weight;
 template <> struct Weight<__half> { static constexpr float LIFT = 7.0f; static constexpr uint32_t KIND = 0; };
 template <> struct Weight<__nv_bfloat16> { static constexpr float LIFT = 0.0f; static constexpr uint32_t KIND = 1; };
@@ -294,7 +310,7 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_attn_kernel(const __
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
     if (tid == 0) {
-        for (int i = 0; i < RING; i++) { bar_init(full + i, 1); bar_init(empty + i, 1); }
+        for (int i = 0; i < RING; i++) { bar_init(full + i, 4); bar_init(empty + i, 1); }
         for (int i = 0; i < 2; i++) { bar_init(scores_there + i, 1); bar_init(weights_there + i, 4); bar_init(sums_there + i, 1); bar_init(queries_free + i, 1); }
         failed_s = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -356,7 +372,7 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_attn_kernel(const __
         begin_column(w);
 
         if (warp < 8) {
-            asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+            asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
             // ---- a set of rows: scores -> weights, and the sums' way out
             const int set = warp >> 2, r = tid & 127;
             const uint32_t lanes = (uint32_t)(warp & 3) << 21, scores = tensor + lanes + set * 128, sums = tensor + lanes + 256 + set * 128;
@@ -466,7 +482,7 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_attn_kernel(const __
                 n_set++;
             }
         } else {
-            asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
             if (warp == 8) {
                 // ---- the products, by one thread
                 constexpr uint32_t KIND = 1u << 4 | Weight<T>::KIND << 7 | Weight<T>::KIND << 10 | (uint32_t)(ROWS >> 4) << 24;
@@ -512,88 +528,62 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_attn_kernel(const __
                 }
                 __syncwarp();
             } else {
-                // ---- the copies: a warp takes every third tile of keys or values
+                // ---- the copies: of each tile of keys or values four times 32 rows, which the warps take in turn
                 const int mine = warp - 9;
-                int signal = -1, tile_n = 0, loads[2] = {0, 0};     // the tile whose copies are on their way and not said to be there, times the sets' queries were loaded
+                int signal = -1, tile_n = 0, loads0 = 0, loads1 = 0;          // the tile whose copies are on their way and not said to be there, times the sets' queries were loaded
+                auto say = [&](int unit) {
+                    seen_by_products();
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(full + unit % RING);
+                };
                 auto drain = [&]() {
                     if (signal < 0) return;
                     copies_wait<0>();
-                    seen_by_products();
-                    __syncwarp();
-                    if (lane == 0) bar_arrive(full + signal % RING);
+                    say(signal);
                     signal = -1;
                 };
                 auto wait = [&](uint64_t *bar, uint32_t parity) {   // (what is waited for may need what this warp has copied)
-                    if (__all_sync(0xffffffffu, bar_try(bar, parity, 0))) return;
+                    if (__all_sync(0xffffffffu, bar_try(bar, parity))) return;
                     drain();
                     bar_wait(bar, parity, failed);
                     __syncwarp();
                 };
                 for (; w.left > 0; next_tile(p, w, groups), tile_n++) {
-                    const int nth = w.tile - w.of_column;
+                    const int nth = w.tile - w.of_column, sets = w.wide ? 2 : 1;
                     const bool begins = w.wide ? nth == 0 : nth < 2;
 #pragma unroll 1
-                    for (int values = 0; values < 2; values++) {
-                        const int unit = 2 * tile_n + values;
-                        if (unit % 3 != mine) {
-                            if (values == 0 && begins) for (int j = 0; j < (w.wide ? 2 : 1); j++) loads[(w.jobs + j) & 1]++;
-                            continue;
-                        }
-                        // pages of the tile's tokens: lane's are lane, lane + 32, ..
-                        int pages[4];
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const int t = w.tile * TOKENS + 32 * i + lane;
-                            pages[i] = t < w.it.len ? a.table[w.it.table * a.table_stride + kvc_divide(t, p.page)] : -1;
-                        }
+                    for (int k = (mine + LOADERS - 8 * tile_n % LOADERS) % LOADERS; k < 8; k += LOADERS) {
+                        const int values = k >> 2, i = k & 3, unit = 2 * tile_n + values, t = w.tile * TOKENS + 32 * i + lane, at_page = kvc_divide(t, p.page);
+                        const int page = t < w.it.len ? a.table[w.it.table * a.table_stride + at_page] : -1;
                         if (unit >= RING) wait(empty + unit % RING, (unit / RING - 1) & 1);
-                        if (values == 0) {
-                            if (begins) {
-                                for (int j = 0; j < (w.wide ? 2 : 1); j++) {
-                                    const int set = (w.jobs + j) & 1, from = w.part * 2 * ROWS + j * ROWS, n = min(ROWS, w.it.rows - from);
-                                    if (loads[set] > 0) wait(queries_free + set, (loads[set] - 1) & 1);
-                                    loads[set]++;
-                                    for (int i = lane; i < n * (D / 8); i += 32) {
-                                        const int r = i / (D / 8), c = i % (D / 8), R = from + r, member = kvc_divide(R, p.group), h = w.k_head * p.g + R - member * p.g;
-                                        const int b = member_at(p, w.it.first + member), row = row_of(p, b);
-                                        copy16(base + set * UNIT + (c >> 3) * ATOM + r * 128 + ((c & 7) ^ (r & 7)) * 16,
-                                               reinterpret_cast<const T *>(a.q) + (long long)max(row, 0) * a.q_token + h * a.q_head + c * 8, row >= 0);
-                                    }
-                                }
+                        if (values == 0 && begins)
+                            for (int j = 0; j < sets; j++) {
+                                const int set = (w.jobs + j) & 1, loads = set ? loads1 : loads0, from = w.part * 2 * ROWS + j * ROWS, R = from + 32 * i + lane, member = kvc_divide(R, p.group);
+                                int row = R < w.it.rows ? member_at(p, w.it.first + member) : -1;
+                                if (row >= 0) row = row_of(p, row);
+                                if (loads > 0) wait(queries_free + set, (loads - 1) & 1);
+                                const uint32_t mask = __ballot_sync(0xffffffffu, row >= 0);
+                                if (mask) copy_rows<T, D>(base + set * UNIT, i, reinterpret_cast<const T *>(a.q) + (row >= 0 ? (long long)row * a.q_token + (w.k_head * p.g + R - member * p.g) * a.q_head : 0), mask, lane);
                             }
-                        }
-                        const uint32_t to = ring + unit % RING * UNIT;
-                        const T *pool = reinterpret_cast<const T *>(values ? a.vpages : a.kpages);
-                        const long long of_page = values ? a.vp_page : a.kp_page, of_row = values ? a.vp_row : a.kp_row, of_head = values ? a.vp_head : a.kp_head;
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const bool good = (unsigned)pages[i] < p.n_pages;
-                            if (!good && w.tile * TOKENS + 32 * i + lane < w.it.len) flags |= KVC_FLAG_BAD_PAGE;
-                            const uint32_t mask = __ballot_sync(0xffffffffu, good);
-                            if (values == 0 && lane == 0) masks[tile_n % MASKS][i] = mask;
-                            const int t = w.tile * TOKENS + 32 * i + lane, row = t - kvc_divide(t, p.page) * (int)a.page_size;
-                            const T *from = pool + (good ? pages[i] * of_page + row * of_row + w.k_head * of_head : 0);
-                            constexpr int SIDE = D == 96 ? 4 : D / 8 > 16 ? 16 : D / 8;       // lanes of a row
-#pragma unroll 4
-                            for (int k = 0; k < SIDE; k++) {
-                                const int j = k * (32 / SIDE) + lane / SIDE;
-                                const T *row_from = reinterpret_cast<const T *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(from), j));
-                                const int r = 32 * i + j;
-#pragma unroll
-                                for (int c0 = 0; c0 < D / 8; c0 += SIDE) {
-                                    const int c = c0 + lane % SIDE;
-                                    copy16(to + (c >> 3) * ATOM + r * 128 + ((c & 7) ^ (r & 7)) * 16, row_from + c * 8, mask >> j & 1);
-                                }
-                            }
-                        }
+                        const bool good = (unsigned)page < p.n_pages;
+                        if (!good && t < w.it.len) flags |= KVC_FLAG_BAD_PAGE;
+                        const uint32_t mask = __ballot_sync(0xffffffffu, good);
+                        if (values == 0 && lane == 0) masks[tile_n % MASKS][i] = mask;
+                        const T *from = reinterpret_cast<const T *>(values ? a.vpages : a.kpages);
+                        const int row = t - at_page * (int)a.page_size;
+                        if (good) from += values ? page * a.vp_page + row * a.vp_row + w.k_head * a.vp_head : page * a.kp_page + row * a.kp_row + w.k_head * a.kp_head;
+                        copy_rows<T, D>(ring + unit % RING * UNIT, i, from, mask, lane);
                         copies_commit();
                         if (signal >= 0) {
                             copies_wait<1>();
-                            seen_by_products();
-                            __syncwarp();
-                            if (lane == 0) bar_arrive(full + signal % RING);
+                            say(signal);
                         }
                         signal = unit;
+                    }
+                    if (begins) {
+                        if (w.wide) loads0++, loads1++;
+                        else if (w.jobs & 1) loads1++;
+                        else loads0++;
                     }
                 }
                 drain();
