@@ -174,27 +174,24 @@ __device__ __forceinline__ Item item_of(const Prefix &p, int i) {
     return r;
 }
 
-// A CTA's way through its share, tile by tile; the same for all its warps.
+// A CTA's way through its share, column by column; the same for all its warps.
 struct Walk {
-    int item, column, tile, left;                           // left: tiles of the share
-    int of_column, in_part;                                 // (of the column's part in this share) its first tile, how many tiles it has
-    int first_job, jobs;                                    // its first job, those before this tile's
+    int item, column, tile, left, in_part;                  // the first tile of the column's part in this share, tiles of the share that are left, of the part
+    int tiles_before, jobs;                                 // of the share, before the part
     int k_head, part;
     Item it;
-    bool wide;
+    bool wide;                                              // more than one set's rows: a tile is two jobs, else one, of the sets in turn
 };
-__device__ __forceinline__ void begin_column(Walk &w) {
+__device__ __forceinline__ void begin_part(Walk &w) {
     w.k_head = w.column / w.it.parts;
     w.part = w.column - w.k_head * w.it.parts;
     w.wide = w.it.rows - w.part * 2 * ROWS > ROWS;
-    w.of_column = w.tile;
     w.in_part = min(w.it.tiles - w.tile, w.left);
-    w.first_job = w.jobs;
 }
-__device__ __forceinline__ void next_tile(const Prefix &p, Walk &w, int groups) {
-    w.jobs += w.wide ? 2 : 1;
-    if (--w.left == 0) return;
-    if (++w.tile < w.it.tiles) return;
+__device__ __forceinline__ void next_part(const Prefix &p, Walk &w, int groups) {
+    w.jobs += w.wide ? 2 * w.in_part : w.in_part;
+    w.tiles_before += w.in_part;
+    if ((w.left -= w.in_part) == 0) return;
     w.tile = 0;
     if (++w.column == w.it.parts * (int)p.a.Hkv) {
         w.column = 0;
@@ -203,7 +200,7 @@ __device__ __forceinline__ void next_tile(const Prefix &p, Walk &w, int groups) 
             w.it = item_of(p, w.item);
         } while (w.it.tiles == 0);
     }
-    begin_column(w);
+    begin_part(w);
 }
 
 // ---- what the hardware is asked for
@@ -235,7 +232,8 @@ __device__ __forceinline__ void before_sync() { asm volatile("tcgen05.fence::bef
 __device__ __forceinline__ void commit_to(uint64_t *bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(shared_at(bar)) : "memory");
 }
-// operands in shared memory, 128-byte swizzle: of 1024-byte pieces (8 rows) that follow one another; `other` bytes to the next 64 channels where rows are not what is summed over
+// operands in shared memory, 128-byte swizzle: of 1024-byte pieces (8 rows) that follow one another; `other` bytes to the next 64 channels where rows are not what is summed over.  Sixteen
+// bytes further: one more.
 __device__ __forceinline__ uint64_t operand_at(uint32_t at, uint32_t other) {
     return (uint64_t)((at & 0x3ffff) >> 4) | (uint64_t)(other >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | 1ull << 46 | 2ull << 61;
 }
@@ -245,6 +243,7 @@ __device__ __forceinline__ void product(uint32_t d, uint64_t a, uint64_t b, uint
 __device__ __forceinline__ void product_of_weights(uint32_t d, uint32_t a, uint64_t b, uint32_t kind, bool add) {
     asm volatile("{ .reg .pred p; setp.ne.u32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(d), "r"(a), "l"(b), "r"(kind), "r"((uint32_t)add) : "memory");
 }
+#define KVC_16(X) X(0), X(1), X(2), X(3), X(4), X(5), X(6), X(7), X(8), X(9), X(10), X(11), X(12), X(13), X(14), X(15)
 #define KVC_32(X) X(0), X(1), X(2), X(3), X(4), X(5), X(6), X(7), X(8), X(9), X(10), X(11), X(12), X(13), X(14), X(15), X(16), X(17), X(18), X(19), X(20), X(21), X(22), X(23), X(24), X(25), X(26), X(27), X(28), X(29), X(30), X(31)
 __device__ __forceinline__ void load32(uint32_t *r, uint32_t at) {
 #define KVC_OUT(i) "=r"(r[i])
@@ -258,7 +257,16 @@ __device__ __forceinline__ void store32(uint32_t at, const uint32_t *r) {
                  "%28, %29, %30, %31};" ::KVC_32(KVC_IN), "r"(at) : "memory");
 #undef KVC_IN
 }
-__device__ __forceinline__ void loads_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void loads_wait(uint32_t *r) {    // (nothing of r is used before)
+#define KVC_BOTH(i) "+r"(r[i])
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : KVC_32(KVC_BOTH)::"memory");
+#undef KVC_BOTH
+}
+__device__ __forceinline__ void store16(uint32_t at, const uint32_t *r) {
+#define KVC_IN(i) "r"(r[i])
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::KVC_16(KVC_IN), "r"(at) : "memory");
+#undef KVC_IN
+}
 __device__ __forceinline__ void stores_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ float exp2_approx(float x) {
     float r;
@@ -299,6 +307,7 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_attn_kernel(const __
     __shared__ __align__(8) uint64_t full[RING], empty[RING], scores_there[2], weights_there[2], sums_there[2], queries_free[2];
     __shared__ uint32_t masks[MASKS][4], tensor_s;
     __shared__ int failed_s, warp_sums[PREFIX_THREADS / 32], start_item, start_rest;
+    __shared__ Item start_it;
     const kvc_paged_attn_args &a = p.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, B = (int)a.B;
     volatile int *failed = &failed_s;
@@ -319,8 +328,9 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_attn_kernel(const __
     // ---- this CTA's share
     const int groups = min(max(p.plan[0], 0), B);
     int flags = 0, total = 0;
+    Item it = {};
     auto scan = [&](int i0, int &tiles) {                   // (first tile of item i0 + tid, its tiles; `total` grows)
-        Item it = {};
+        it.tiles = it.parts = 0;
         if (i0 + tid < groups) it = item_of(p, i0 + tid);
         tiles = it.tiles * it.parts * (int)a.Hkv;
         int sum = tiles;
@@ -350,7 +360,7 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_attn_kernel(const __
         if (groups > PREFIX_THREADS) total = 0;
         for (int i0 = 0; i0 < groups; i0 += PREFIX_THREADS) {
             if (groups > PREFIX_THREADS) first = scan(i0, tiles);
-            if (r0 >= first && r0 < first + tiles) { start_item = i0 + tid; start_rest = r0 - first; }
+            if (r0 >= first && r0 < first + tiles) { start_item = i0 + tid; start_rest = r0 - first; start_it = it; }
         }
     }
     if (blockIdx.x == gridDim.x - 1)                        // prefixes that are longer than what there is
@@ -364,167 +374,171 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_attn_kernel(const __
     if (r0 < r1) {
         Walk w;
         w.left = r1 - r0;
-        w.jobs = 0;
+        w.jobs = w.tiles_before = 0;
         w.item = start_item;
-        w.it = item_of(p, w.item);
+        w.it = start_it;
         w.column = start_rest / w.it.tiles;
         w.tile = start_rest - w.column * w.it.tiles;
-        begin_column(w);
+        begin_part(w);
 
         if (warp < 8) {
-            asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
             // ---- a set of rows: scores -> weights, and the sums' way out
             const int set = warp >> 2, r = tid & 127;
             const uint32_t lanes = (uint32_t)(warp & 3) << 21, scores = tensor + lanes + set * 128, sums = tensor + lanes + 256 + set * 128;
-            float m = -CUDART_INF_F, l = 0.0f;
-            int n_set = 0, tile_n = 0;                      // jobs of this set, tiles
-            bool mine = false;
-            float *to = nullptr;
-            float2 *to_max = nullptr;
-            for (; w.left > 0; next_tile(p, w, groups), tile_n++) {
-                const int idx = (set - w.jobs) & 1;         // which of the tile's jobs is this set's
-                if (!w.wide && idx != 0) continue;
-                const int half = w.wide ? idx : 0, part_i = w.wide ? half : (w.jobs - w.first_job) & 1, nth = w.tile - w.of_column;
-                const bool begins = w.wide ? nth == 0 : nth < 2, ends = w.wide ? nth == w.in_part - 1 : nth + 2 >= w.in_part;
-                if (begins) {
-                    const int R = w.part * 2 * ROWS + half * ROWS + r;
-                    mine = R < w.it.rows;
-                    if (mine) {
-                        const int member = kvc_divide(R, p.group), h = w.k_head * p.g + R - member * p.g, b = member_at(p, w.it.first + member);
-                        mine = row_of(p, b) >= 0;
-                        const long long place = w.of_column == 0 ? place_of(p, b, h, w.wide ? 0 : part_i) : cta_place(p, blockIdx.x, part_i * ROWS + r);
-                        to = p.sums + place * D;
-                        to_max = p.maxima + place;
-                    }
-                    m = -CUDART_INF_F;
-                    l = 0.0f;
+            int phase = 0;                                  // of this set's jobs
+            for (; w.left > 0; next_part(p, w, groups)) {
+                const int idx = (set - w.jobs) & 1, half = w.wide ? idx : 0, first_n = w.wide ? 0 : idx, step = w.wide ? 1 : 2;
+                if (first_n >= w.in_part) continue;
+                const int R = w.part * 2 * ROWS + half * ROWS + r;
+                bool mine = R < w.it.rows;
+                long long place = 0;
+                if (mine) {
+                    const int member = kvc_divide(R, p.group), h = w.k_head * p.g + R - member * p.g, b = member_at(p, w.it.first + member);
+                    mine = row_of(p, b) >= 0;
+                    place = w.tile == 0 ? place_of(p, b, h, first_n) : cta_place(p, blockIdx.x, (w.wide ? half : first_n) * ROWS + r);
                 }
-                bar_wait(scores_there + set, n_set & 1, failed);
-                after_sync();
-                if (__any_sync(0xffffffffu, mine)) {
-                    uint32_t s[128];
-#pragma unroll
-                    for (int c = 0; c < 4; c++) load32(s + 32 * c, scores + 32 * c);
-                    loads_wait();
-                    if (p.negative) {
-#pragma unroll
-                        for (int i = 0; i < 128; i++) s[i] ^= 0x80000000u;
-                    }
-#pragma unroll
-                    for (int c = 0; c < 4; c++) {
-                        const uint32_t mask = masks[tile_n % MASKS][c];
-                        if (mask == 0xffffffffu) continue;
-#pragma unroll
-                        for (int i = 0; i < 32; i++) s[32 * c + i] = mask >> i & 1 ? s[32 * c + i] : 0xff800000u;
-                    }
-                    float top[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
-#pragma unroll
-                    for (int i = 0; i < 128; i++) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(s[i]));
-                    const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.log2_scaling;
-                    const bool up = high > m + SLACK || (m == -CUDART_INF_F && high > m);
-                    if (__any_sync(0xffffffffu, up)) {
-                        const float now = up ? high : m, f = up ? exp2_approx(m - now) : 1.0f;
-                        m = now;
-                        l *= f;
-                        if (!begins) {
-                            bar_wait(sums_there + set, (n_set - 1) & 1, failed);
-                            after_sync();
-#pragma unroll
-                            for (int c = 0; c < D / 32; c++) {
-                                uint32_t o[32];
-                                load32(o, sums + 32 * c);
-                                loads_wait();
-#pragma unroll
-                                for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                                store32(sums + 32 * c, o);
-                            }
-                        }
-                    }
-                    const float less = LIFT - (m == -CUDART_INF_F ? 0.0f : m);
-                    float sum[4] = {};
-#pragma unroll
-                    for (int c = 0; c < 2; c++) {
-                        uint32_t weights[32];
-#pragma unroll
-                        for (int i = 0; i < 32; i++) {
-                            const float w0 = exp2_approx(fmaf(__uint_as_float(s[64 * c + 2 * i]), p.log2_scaling, less)), w1 = exp2_approx(fmaf(__uint_as_float(s[64 * c + 2 * i + 1]), p.log2_scaling, less));
-                            sum[i & 1] += w0;
-                            sum[2 + (i & 1)] += w1;
-                            weights[i] = pack(w0, w1, T());
-                        }
-                        store32(scores + 32 * c, weights);
-                    }
-                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                    stores_wait();
-                }
-                before_sync();
-                __syncwarp();
-                if (lane == 0) bar_arrive(weights_there + set);
-                if (ends) {
-                    bar_wait(sums_there + set, n_set & 1, failed);
+                const bool some = __any_sync(0xffffffffu, mine);
+                float m = -CUDART_INF_F, l = 0.0f;
+                for (int n = first_n; n < w.in_part; n += step) {
+                    bar_wait(scores_there + set, phase, failed);
                     after_sync();
-                    if (__any_sync(0xffffffffu, mine)) {
+                    if (some) {
+                        // Twice over the scores, 32 at a time (all 128 at once would not leave registers enough): their maximum, then the weights
+                        const uint32_t *const mask = masks[(w.tiles_before + n) % MASKS];
+                        uint32_t s[2][32];
+                        auto chunk = [&](int c) {           // 32 scores are here, the next 32 are asked for
+                            loads_wait(s[c & 1]);
+                            if (c < 3) load32(s[(c + 1) & 1], scores + 32 * (c + 1));
+                            if (p.negative) {
 #pragma unroll
-                        for (int c = 0; c < D / 32; c++) {
-                            uint32_t o[32];
-                            load32(o, sums + 32 * c);
-                            loads_wait();
-                            if (mine) {
+                                for (int i = 0; i < 32; i++) s[c & 1][i] ^= 0x80000000u;
+                            }
+                            if (mask[c] != 0xffffffffu) {
+                                const uint32_t on = mask[c];
 #pragma unroll
-                                for (int i = 0; i < 8; i++)
-                                    __stcg(reinterpret_cast<uint4 *>(to) + 8 * c + i, make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]));
+                                for (int i = 0; i < 32; i++) s[c & 1][i] = on >> i & 1 ? s[c & 1][i] : 0xff800000u;
+                            }
+                        };
+                        load32(s[0], scores);
+                        float top[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
+#pragma unroll
+                        for (int c = 0; c < 4; c++) {
+                            chunk(c);
+#pragma unroll
+                            for (int i = 0; i < 32; i++) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(s[c & 1][i]));
+                        }
+                        load32(s[0], scores);
+                        const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.log2_scaling;
+                        const bool up = high > m + SLACK || (m == -CUDART_INF_F && high > m);
+                        if (__any_sync(0xffffffffu, up)) {
+                            const float now = up ? high : m, f = up ? exp2_approx(m - now) : 1.0f;
+                            m = now;
+                            l *= f;
+                            if (n != first_n) {
+                                bar_wait(sums_there + set, phase ^ 1, failed);
+                                after_sync();
+                                loads_wait(s[0]);
+#pragma unroll
+                                for (int c = 0; c < D / 32; c++) {
+                                    load32(s[1], sums + 32 * c);
+                                    loads_wait(s[1]);
+#pragma unroll
+                                    for (int i = 0; i < 32; i++) s[1][i] = __float_as_uint(__uint_as_float(s[1][i]) * f);
+                                    store32(sums + 32 * c, s[1]);
+                                }
                             }
                         }
-                        if (mine) __stcg(to_max, make_float2(m - LIFT, l));     // (weights were 2^LIFT times what the maximum says)
+                        const float less = LIFT - (m == -CUDART_INF_F ? 0.0f : m);
+                        float sum[4] = {};
+#pragma unroll
+                        for (int c = 0; c < 4; c++) {
+                            chunk(c);
+                            uint32_t weights[16];           // (they take the place of scores that have been read)
+#pragma unroll
+                            for (int i = 0; i < 16; i++) {
+                                const float w0 = exp2_approx(fmaf(__uint_as_float(s[c & 1][2 * i]), p.log2_scaling, less)), w1 = exp2_approx(fmaf(__uint_as_float(s[c & 1][2 * i + 1]), p.log2_scaling, less));
+                                sum[i & 1] += w0;
+                                sum[2 + (i & 1)] += w1;
+                                weights[i] = pack(w0, w1, T());
+                            }
+                            store16(scores + 16 * c, weights);
+                        }
+                        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                        stores_wait();
                     }
                     before_sync();
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(weights_there + set);
+                    phase ^= 1;
                 }
-                n_set++;
+                bar_wait(sums_there + set, phase ^ 1, failed);
+                after_sync();
+                if (some) {
+                    uint32_t o[2][32];
+                    load32(o[0], sums);
+#pragma unroll
+                    for (int c = 0; c < D / 32; c++) {
+                        loads_wait(o[c & 1]);
+                        if (c + 1 < D / 32) load32(o[(c + 1) & 1], sums + 32 * (c + 1));
+                        if (mine) {
+#pragma unroll
+                            for (int i = 0; i < 8; i++)
+                                __stcg(reinterpret_cast<uint4 *>(p.sums + place * D) + 8 * c + i, make_uint4(o[c & 1][4 * i], o[c & 1][4 * i + 1], o[c & 1][4 * i + 2], o[c & 1][4 * i + 3]));
+                        }
+                    }
+                    if (mine) __stcg(p.maxima + place, make_float2(m - LIFT, l));          // (weights were 2^LIFT times what the maximum says)
+                }
+                before_sync();
             }
         } else {
-            asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
             if (warp == 8) {
                 // ---- the products, by one thread
                 constexpr uint32_t KIND = 1u << 4 | Weight<T>::KIND << 7 | Weight<T>::KIND << 10 | (uint32_t)(ROWS >> 4) << 24;
                 constexpr uint32_t SCORES = KIND | (uint32_t)(TOKENS >> 3) << 17, VALUES = KIND | 1u << 16 | (uint32_t)(D >> 3) << 17;
                 if (lane == 0) {
-                    struct { int set, unit, n; bool first, last_of_unit; } late = {-1, 0, 0, false, false};
-                    int n_set[2] = {0, 0}, tile_n = 0;
-                    auto values_of = [&]() {                // the second product of the job before
-                        if (late.set < 0) return;
-                        bar_wait(weights_there + late.set, late.n & 1, failed);
-                        const int unit = late.unit, slot = unit % RING;
-                        bar_wait(full + slot, unit / RING & 1, failed);
+                    const uint64_t queries = operand_at(base, 16), keys = operand_at(ring, 16), values = operand_at(ring, ATOM);
+                    int slot = 0, round = 0;                // of the ring: the next unit's place, and how often it has been through (its last bit)
+                    int phases = 0;                         // a bit for each set: its jobs
+                    int late = -1, late_slot = 0, late_round = 0;          // the job before: its set and what its second product needs
+                    bool late_first = false, late_last = false;
+                    auto second = [&]() {
+                        if (late < 0) return;
+                        bar_wait(weights_there + late, phases >> late & 1, failed);
+                        phases ^= 1 << late;
+                        bar_wait(full + late_slot, late_round, failed);
                         after_sync();
-                        const uint32_t at = ring + slot * UNIT;
+                        const uint64_t b = values + (uint32_t)late_slot * (UNIT / 16);
+                        const uint32_t d = tensor + 256 + late * 128, a_at = tensor + late * 128;
 #pragma unroll
-                        for (int k = 0; k < TOKENS / 16; k++)
-                            product_of_weights(tensor + 256 + late.set * 128, tensor + late.set * 128 + 8 * k, operand_at(at + k * 2048, ATOM), VALUES, !late.first || k > 0);
-                        if (late.last_of_unit) commit_to(empty + slot);
-                        commit_to(sums_there + late.set);   // (the last that comes back)
+                        for (int k = 0; k < TOKENS / 16; k++) product_of_weights(d, a_at + 8 * k, b + k * (2048 / 16), VALUES, k > 0 || !late_first);
+                        if (late_last) commit_to(empty + late_slot);
+                        commit_to(sums_there + late);       // (the last that comes back)
                     };
-                    for (; w.left > 0; next_tile(p, w, groups), tile_n++) {
-                        const int nth = w.tile - w.of_column, unit = 2 * tile_n, slot = unit % RING;
-                        bar_wait(full + slot, unit / RING & 1, failed);
-                        for (int j = 0; j < (w.wide ? 2 : 1); j++) {
-                            const int set = (w.jobs + j) & 1;
-                            const bool begins = w.wide ? nth == 0 : nth < 2, ends = w.wide ? nth == w.in_part - 1 : nth + 2 >= w.in_part, last = !w.wide || j == 1;
-                            after_sync();
+                    for (; w.left > 0; next_part(p, w, groups)) {
+                        for (int n = 0; n < w.in_part; n++) {
+                            const int v_slot = slot + 1 == RING ? 0 : slot + 1, v_round = slot + 1 == RING ? round ^ 1 : round;
+                            const bool begins = w.wide ? n == 0 : n < 2, ends = w.wide ? n == w.in_part - 1 : n + 2 >= w.in_part;
+                            bar_wait(full + slot, round, failed);
+                            for (int j = 0; j < (w.wide ? 2 : 1); j++) {
+                                const int set = (w.jobs + (w.wide ? j : n)) & 1;
+                                const bool last = !w.wide || j == 1;
+                                after_sync();
+                                const uint64_t q_at = queries + set * (UNIT / 16), k_at = keys + (uint32_t)slot * (UNIT / 16);
 #pragma unroll
-                            for (int k = 0; k < D / 16; k++) {
-                                const uint32_t off = (k >> 2) * ATOM + (k & 3) * 32;
-                                product(tensor + set * 128, operand_at(base + set * UNIT + off, 16), operand_at(ring + slot * UNIT + off, 16), SCORES, k > 0);
+                                for (int k = 0; k < D / 16; k++) product(tensor + set * 128, q_at + ((k >> 2) * ATOM + (k & 3) * 32) / 16, k_at + ((k >> 2) * ATOM + (k & 3) * 32) / 16, SCORES, k > 0);
+                                commit_to(scores_there + set);
+                                if (ends) commit_to(queries_free + set);
+                                if (last) commit_to(empty + slot);
+                                second();
+                                late = set; late_slot = v_slot; late_round = v_round; late_first = begins; late_last = last;
                             }
-                            commit_to(scores_there + set);
-                            if (ends) commit_to(queries_free + set);
-                            if (last) commit_to(empty + slot);
-                            values_of();
-                            late = {set, unit + 1, n_set[set]++, begins, last};
+                            slot = v_slot + 1; round = v_round;
+                            if (slot == RING) { slot = 0; round ^= 1; }
                         }
                     }
-                    values_of();
+                    second();
                     // all products are done before anything is given back
-                    if (late.set >= 0) bar_wait(sums_there + late.set, late.n & 1, failed);
+                    if (late >= 0) bar_wait(sums_there + late, phases >> late & 1 ^ 1, failed);
                 }
                 __syncwarp();
             } else {
@@ -548,17 +562,17 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_attn_kernel(const __
                     bar_wait(bar, parity, failed);
                     __syncwarp();
                 };
-                for (; w.left > 0; next_tile(p, w, groups), tile_n++) {
-                    const int nth = w.tile - w.of_column, sets = w.wide ? 2 : 1;
-                    const bool begins = w.wide ? nth == 0 : nth < 2;
+                for (; w.left > 0; next_part(p, w, groups)) for (int n = 0; n < w.in_part; n++, tile_n++) {
+                    const int sets = w.wide ? 2 : 1, first_job = w.jobs + n * sets;
+                    const bool begins = w.wide ? n == 0 : n < 2;
 #pragma unroll 1
                     for (int k = (mine + LOADERS - 8 * tile_n % LOADERS) % LOADERS; k < 8; k += LOADERS) {
-                        const int values = k >> 2, i = k & 3, unit = 2 * tile_n + values, t = w.tile * TOKENS + 32 * i + lane, at_page = kvc_divide(t, p.page);
+                        const int values = k >> 2, i = k & 3, unit = 2 * tile_n + values, t = (w.tile + n) * TOKENS + 32 * i + lane, at_page = kvc_divide(t, p.page);
                         const int page = t < w.it.len ? a.table[w.it.table * a.table_stride + at_page] : -1;
                         if (unit >= RING) wait(empty + unit % RING, (unit / RING - 1) & 1);
                         if (values == 0 && begins)
                             for (int j = 0; j < sets; j++) {
-                                const int set = (w.jobs + j) & 1, loads = set ? loads1 : loads0, from = w.part * 2 * ROWS + j * ROWS, R = from + 32 * i + lane, member = kvc_divide(R, p.group);
+                                const int set = (first_job + j) & 1, loads = set ? loads1 : loads0, from = w.part * 2 * ROWS + j * ROWS, R = from + 32 * i + lane, member = kvc_divide(R, p.group);
                                 int row = R < w.it.rows ? member_at(p, w.it.first + member) : -1;
                                 if (row >= 0) row = row_of(p, row);
                                 if (loads > 0) wait(queries_free + set, (loads - 1) & 1);
@@ -582,7 +596,7 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_attn_kernel(const __
                     }
                     if (begins) {
                         if (w.wide) loads0++, loads1++;
-                        else if (w.jobs & 1) loads1++;
+                        else if (first_job & 1) loads1++;
                         else loads0++;
                     }
                 }
