@@ -229,19 +229,26 @@ template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("c
 __device__ __forceinline__ void seen_by_products() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void commit_to(uint64_t *bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(shared_at(bar)) : "memory");
+// One lane of the warp asks for products and what follows them; all lanes come along, so that what these take is the warp's (uniform registers) and not put together by a lane for every one:
+// 32 products and commits of a tile took 6000 cycles of one lane alone.
+__device__ __forceinline__ uint32_t one_lane() {
+    uint32_t is;
+    asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p; }" : "=r"(is));
+    return is;
+}
+__device__ __forceinline__ void commit_to(uint32_t one, uint64_t *bar) {
+    asm volatile("{ .reg .pred e; setp.ne.u32 e, %1, 0; @e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0]; }" ::"r"(shared_at(bar)), "r"(one) : "memory");
 }
 // operands in shared memory, 128-byte swizzle: of 1024-byte pieces (8 rows) that follow one another; `other` bytes to the next 64 channels where rows are not what is summed over.  Sixteen
 // bytes further: one more.
 __device__ __forceinline__ uint64_t operand_at(uint32_t at, uint32_t other) {
     return (uint64_t)((at & 0x3ffff) >> 4) | (uint64_t)(other >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | 1ull << 46 | 2ull << 61;
 }
-__device__ __forceinline__ void product(uint32_t d, uint64_t a, uint64_t b, uint32_t kind, bool add) {
-    asm volatile("{ .reg .pred p; setp.ne.u32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }" ::"r"(d), "l"(a), "l"(b), "r"(kind), "r"((uint32_t)add) : "memory");
+__device__ __forceinline__ void product(uint32_t one, uint32_t d, uint64_t a, uint64_t b, uint32_t kind, bool add) {
+    asm volatile("{ .reg .pred p, e; setp.ne.u32 p, %4, 0; setp.ne.u32 e, %5, 0; @e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }" ::"r"(d), "l"(a), "l"(b), "r"(kind), "r"((uint32_t)add), "r"(one) : "memory");
 }
-__device__ __forceinline__ void product_of_weights(uint32_t d, uint32_t a, uint64_t b, uint32_t kind, bool add) {
-    asm volatile("{ .reg .pred p; setp.ne.u32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(d), "r"(a), "l"(b), "r"(kind), "r"((uint32_t)add) : "memory");
+__device__ __forceinline__ void product_of_weights(uint32_t one, uint32_t d, uint32_t a, uint64_t b, uint32_t kind, bool add) {
+    asm volatile("{ .reg .pred p, e; setp.ne.u32 p, %4, 0; setp.ne.u32 e, %5, 0; @e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(d), "r"(a), "l"(b), "r"(kind), "r"((uint32_t)add), "r"(one) : "memory");
 }
 #define KVC_16(X) X(0), X(1), X(2), X(3), X(4), X(5), X(6), X(7), X(8), X(9), X(10), X(11), X(12), X(13), X(14), X(15)
 #define KVC_32(X) X(0), X(1), X(2), X(3), X(4), X(5), X(6), X(7), X(8), X(9), X(10), X(11), X(12), X(13), X(14), X(15), X(16), X(17), X(18), X(19), X(20), X(21), X(22), X(23), X(24), X(25), X(26), X(27), X(28), X(29), X(30), X(31)
@@ -311,7 +318,6 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_attn_kernel(const __
     const kvc_paged_attn_args &a = p.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, B = (int)a.B;
     volatile int *failed = &failed_s;
-    cudaTriggerProgrammaticLaunchCompletion();              // (the kernel of the requests' own tokens, which reads nothing of this one's, may begin where there is room)
     const uint32_t base = (shared_at(raw) + 1023) & ~1023u, ring = base + 2 * UNIT;
 
     if (warp == 8) {
@@ -326,6 +332,7 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_attn_kernel(const __
     }
 
     // ---- this CTA's share
+    kvc_behind();                                           // (from here on the kernel of the requests' own tokens, which reads nothing of this one's, may begin where there is room)
     const int groups = min(max(p.plan[0], 0), B);
     int flags = 0, total = 0;
     Item it = {};
@@ -492,54 +499,65 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_attn_kernel(const __
             }
         } else {
             if (warp == 8) {
-                // ---- the products, by one thread
+                // ---- the products
                 constexpr uint32_t KIND = 1u << 4 | Weight<T>::KIND << 7 | Weight<T>::KIND << 10 | (uint32_t)(ROWS >> 4) << 24;
                 constexpr uint32_t SCORES = KIND | (uint32_t)(TOKENS >> 3) << 17, VALUES = KIND | 1u << 16 | (uint32_t)(D >> 3) << 17;
-                if (lane == 0) {
-                    const uint64_t queries = operand_at(base, 16), keys = operand_at(ring, 16), values = operand_at(ring, ATOM);
-                    int slot = 0, round = 0;                // of the ring: the next unit's place, and how often it has been through (its last bit)
-                    int phases = 0;                         // a bit for each set: its jobs
-                    int late = -1, late_slot = 0, late_round = 0;          // the job before: its set and what its second product needs
-                    bool late_first = false, late_last = false;
-                    auto second = [&]() {
-                        if (late < 0) return;
-                        bar_wait(weights_there + late, phases >> late & 1, failed);
-                        phases ^= 1 << late;
-                        bar_wait(full + late_slot, late_round, failed);
-                        after_sync();
-                        const uint64_t b = values + (uint32_t)late_slot * (UNIT / 16);
-                        const uint32_t d = tensor + 256 + late * 128, a_at = tensor + late * 128;
+                auto all_lanes = [](int v) { return __shfl_sync(0xffffffffu, v, 0); };
+                const uint32_t one = one_lane(), t_at = (uint32_t)all_lanes((int)tensor);
+                const uint64_t queries = operand_at(base, 16), keys = operand_at(ring, 16), values = operand_at(ring, ATOM);
+                int slot = 0, round = 0;                    // of the ring: the next unit's place, and how often it has been through (its last bit)
+                auto next_unit = [&]() { if (++slot == RING) { slot = 0; round ^= 1; } };
+                int phases = 0;                             // a bit for each set: its jobs
+                int late = -1, late_slot = 0, late_round = 0;          // the job before: its set and what its second product needs
+                bool late_first = false, late_last = false, late_waits = false;
+                auto second = [&]() {
+                    if (late < 0) return;
+                    bar_wait(weights_there + late, phases >> late & 1, failed);
+                    phases ^= 1 << late;
+                    bar_wait(full + late_slot, late_round, failed);
+                    after_sync();
+                    const uint64_t b = values + (uint32_t)late_slot * (UNIT / 16);
+                    const uint32_t d = t_at + 256 + late * 128, a_at = t_at + late * 128;
 #pragma unroll
-                        for (int k = 0; k < TOKENS / 16; k++) product_of_weights(d, a_at + 8 * k, b + k * (2048 / 16), VALUES, k > 0 || !late_first);
-                        if (late_last) commit_to(empty + late_slot);
-                        commit_to(sums_there + late);       // (the last that comes back)
-                    };
-                    for (; w.left > 0; next_part(p, w, groups)) {
-                        for (int n = 0; n < w.in_part; n++) {
-                            const int v_slot = slot + 1 == RING ? 0 : slot + 1, v_round = slot + 1 == RING ? round ^ 1 : round;
-                            const bool begins = w.wide ? n == 0 : n < 2, ends = w.wide ? n == w.in_part - 1 : n + 2 >= w.in_part;
-                            bar_wait(full + slot, round, failed);
-                            for (int j = 0; j < (w.wide ? 2 : 1); j++) {
-                                const int set = (w.jobs + (w.wide ? j : n)) & 1;
-                                const bool last = !w.wide || j == 1;
-                                after_sync();
-                                const uint64_t q_at = queries + set * (UNIT / 16), k_at = keys + (uint32_t)slot * (UNIT / 16);
-#pragma unroll
-                                for (int k = 0; k < D / 16; k++) product(tensor + set * 128, q_at + ((k >> 2) * ATOM + (k & 3) * 32) / 16, k_at + ((k >> 2) * ATOM + (k & 3) * 32) / 16, SCORES, k > 0);
-                                commit_to(scores_there + set);
-                                if (ends) commit_to(queries_free + set);
-                                if (last) commit_to(empty + slot);
-                                second();
-                                late = set; late_slot = v_slot; late_round = v_round; late_first = begins; late_last = last;
-                            }
-                            slot = v_slot + 1; round = v_round;
-                            if (slot == RING) { slot = 0; round ^= 1; }
+                    for (int k = 0; k < TOKENS / 16; k++) product_of_weights(one, d, a_at + 8 * k, b + k * (2048 / 16), VALUES, k > 0 || !late_first);
+                    if (late_last) commit_to(one, empty + late_slot);
+                    commit_to(one, sums_there + late);      // (the last that comes back)
+                };
+                for (; all_lanes(w.left) > 0; next_part(p, w, groups)) {
+                    const int in_part = all_lanes(w.in_part), jobs = all_lanes(w.jobs);
+                    const bool wide = all_lanes(w.wide);
+                    for (int n = 0; n < in_part; n++) {
+                        const bool begins = wide ? n == 0 : n < 2, ends = wide ? n == in_part - 1 : n + 2 >= in_part;
+                        const int k_slot = slot;
+                        bar_wait(full + slot, round, failed);
+                        next_unit();
+                        if (late_waits) {                   // the values of the tile before come behind this one's keys
+                            late_slot = slot; late_round = round;
+                            next_unit();
                         }
+                        const int v_slot = slot, v_round = round;       // (wide)
+                        if (wide) next_unit();
+                        for (int j = 0; j < (wide ? 2 : 1); j++) {
+                            const int set = (jobs + (wide ? j : n)) & 1;
+                            const bool last = !wide || j == 1;
+                            after_sync();
+                            const uint64_t q_at = queries + set * (UNIT / 16), k_at = keys + (uint32_t)k_slot * (UNIT / 16);
+                            const uint32_t d = t_at + set * 128;
+#pragma unroll
+                            for (int k = 0; k < D / 16; k++) product(one, d, q_at + ((k >> 2) * ATOM + (k & 3) * 32) / 16, k_at + ((k >> 2) * ATOM + (k & 3) * 32) / 16, SCORES, k > 0);
+                            commit_to(one, scores_there + set);
+                            if (ends) commit_to(one, queries_free + set);
+                            if (last) commit_to(one, empty + k_slot);
+                            second();
+                            late = set; late_slot = v_slot; late_round = v_round; late_first = begins; late_last = last;
+                        }
+                        late_waits = !wide;
                     }
-                    second();
-                    // all products are done before anything is given back
-                    if (late >= 0) bar_wait(sums_there + late, phases >> late & 1 ^ 1, failed);
                 }
+                if (late_waits) { late_slot = slot; late_round = round; }
+                second();
+                // all products are done before anything is given back
+                if (late >= 0) bar_wait(sums_there + late, phases >> late & 1 ^ 1, failed);
                 __syncwarp();
             } else {
                 // ---- the copies: of each tile of keys or values four times 32 rows, which the warps take in turn
@@ -562,15 +580,48 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_attn_kernel(const __
                     bar_wait(bar, parity, failed);
                     __syncwarp();
                 };
+                // Units of the ring in the order of their use: a tile's keys, and its values behind the next tile's keys (narrow: the next job's first product runs before them) or behind
+                // its own (wide).
+                int block = 0;                              // 32 rows of a unit, of all that came before
+                int v_tile = -1, v_table = 0, v_len = 0, v_head = 0;                       // values that are still to come: of which tile
+                auto rows_of = [&](int values, int unit, int i, int tile, int table, int len, int k_head) {
+                    const int t = tile * TOKENS + 32 * i + lane, at_page = kvc_divide(t, p.page), row = t - at_page * (int)a.page_size;
+                    const int page = t < len ? a.table[table * a.table_stride + at_page] : -1;
+                    if (unit >= RING) wait(empty + unit % RING, (unit / RING - 1) & 1);
+                    const bool good = (unsigned)page < p.n_pages;
+                    if (!good && t < len) flags |= KVC_FLAG_BAD_PAGE;
+                    const uint32_t mask = __ballot_sync(0xffffffffu, good);
+                    if (values == 0 && lane == 0) masks[tile_n % MASKS][i] = mask;
+                    const T *from = reinterpret_cast<const T *>(values ? a.vpages : a.kpages);
+                    if (good) from += values ? page * a.vp_page + row * a.vp_row + k_head * a.vp_head : page * a.kp_page + row * a.kp_row + k_head * a.kp_head;
+                    copy_rows<T, D>(ring + unit % RING * UNIT, i, from, mask, lane);
+                };
+                auto sent = [&](int unit) {                 // what was copied is said to be there when the next rows are on their way
+                    copies_commit();
+                    if (signal >= 0) {
+                        copies_wait<1>();
+                        say(signal);
+                    }
+                    signal = unit;
+                };
+                auto values_of = [&]() {
+                    const int unit = block / 4;
+#pragma unroll 1
+                    for (int i = 0; i < 4; i++, block++) {
+                        if (block % LOADERS != mine) continue;
+                        rows_of(1, unit, i, v_tile, v_table, v_len, v_head);
+                        sent(unit);
+                    }
+                    v_tile = -1;
+                };
                 for (; w.left > 0; next_part(p, w, groups)) for (int n = 0; n < w.in_part; n++, tile_n++) {
-                    const int sets = w.wide ? 2 : 1, first_job = w.jobs + n * sets;
+                    const int sets = w.wide ? 2 : 1, first_job = w.jobs + n * sets, unit = block / 4;
                     const bool begins = w.wide ? n == 0 : n < 2;
 #pragma unroll 1
-                    for (int k = (mine + LOADERS - 8 * tile_n % LOADERS) % LOADERS; k < 8; k += LOADERS) {
-                        const int values = k >> 2, i = k & 3, unit = 2 * tile_n + values, t = (w.tile + n) * TOKENS + 32 * i + lane, at_page = kvc_divide(t, p.page);
-                        const int page = t < w.it.len ? a.table[w.it.table * a.table_stride + at_page] : -1;
-                        if (unit >= RING) wait(empty + unit % RING, (unit / RING - 1) & 1);
-                        if (values == 0 && begins)
+                    for (int i = 0; i < 4; i++, block++) {
+                        if (block % LOADERS != mine) continue;
+                        rows_of(0, unit, i, w.tile + n, w.it.table, w.it.len, w.k_head);
+                        if (begins)
                             for (int j = 0; j < sets; j++) {
                                 const int set = (first_job + j) & 1, loads = set ? loads1 : loads0, from = w.part * 2 * ROWS + j * ROWS, R = from + 32 * i + lane, member = kvc_divide(R, p.group);
                                 int row = R < w.it.rows ? member_at(p, w.it.first + member) : -1;
@@ -579,27 +630,18 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_attn_kernel(const __
                                 const uint32_t mask = __ballot_sync(0xffffffffu, row >= 0);
                                 if (mask) copy_rows<T, D>(base + set * UNIT, i, reinterpret_cast<const T *>(a.q) + (row >= 0 ? (long long)row * a.q_token + (w.k_head * p.g + R - member * p.g) * a.q_head : 0), mask, lane);
                             }
-                        const bool good = (unsigned)page < p.n_pages;
-                        if (!good && t < w.it.len) flags |= KVC_FLAG_BAD_PAGE;
-                        const uint32_t mask = __ballot_sync(0xffffffffu, good);
-                        if (values == 0 && lane == 0) masks[tile_n % MASKS][i] = mask;
-                        const T *from = reinterpret_cast<const T *>(values ? a.vpages : a.kpages);
-                        const int row = t - at_page * (int)a.page_size;
-                        if (good) from += values ? page * a.vp_page + row * a.vp_row + w.k_head * a.vp_head : page * a.kp_page + row * a.kp_row + w.k_head * a.kp_head;
-                        copy_rows<T, D>(ring + unit % RING * UNIT, i, from, mask, lane);
-                        copies_commit();
-                        if (signal >= 0) {
-                            copies_wait<1>();
-                            say(signal);
-                        }
-                        signal = unit;
+                        sent(unit);
                     }
                     if (begins) {
                         if (w.wide) loads0++, loads1++;
                         else if (first_job & 1) loads1++;
                         else loads0++;
                     }
+                    if (v_tile >= 0) values_of();
+                    v_tile = w.tile + n; v_table = w.it.table; v_len = w.it.len; v_head = w.k_head;
+                    if (w.wide) values_of();
                 }
+                if (v_tile >= 0) values_of();
                 drain();
                 copies_wait<0>();
             }
@@ -655,7 +697,7 @@ __global__ void __launch_bounds__(128) prefix_join_kernel(const __grid_constant_
         const int from = p.item_first[group] + (k_head * it.parts + part) * it.tiles, to = from + it.tiles;
         // a column's parts: each in a CTA's share, of narrow columns two (every other tile) where it has more than one
         const int cta0 = from / size, cta1 = (to - 1) / size, each = wide ? 1 : 2;
-        constexpr int AT_ONCE = 4;
+        constexpr int AT_ONCE = 8;
         for (int k0 = 0; it.tiles > 0 && k0 < (cta1 - cta0 + 1) * each; k0 += AT_ONCE) {
             float2 ml[AT_ONCE];
             float4 x[AT_ONCE];
@@ -687,8 +729,17 @@ int launch(Prefix &p, Params &own, cudaStream_t s) {
     int occ = 0;
     if (int rc = kvc_prepare(slot, reinterpret_cast<const void *>(prefix_attn_kernel<T, D>), PREFIX_THREADS, Shape<D>::SHARED, &occ)) return rc;
     KVC_REQUIRE(occ > 0, "kvc_paged_attn_shared: the kernel does not fit this device");
-    prefix_attn_kernel<T, D><<<(unsigned)p.grid, PREFIX_THREADS, Shape<D>::SHARED, s>>>(p);
-    KVC_LAUNCH_OK();
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)p.grid);
+    cfg.blockDim = dim3(PREFIX_THREADS);
+    cfg.dynamicSmemBytes = Shape<D>::SHARED;
+    cfg.stream = s;
+    cudaLaunchAttribute early;
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &early;
+    cfg.numAttrs = 1;
+    KVC_CUDA_OK(cudaLaunchKernelEx(&cfg, prefix_attn_kernel<T, D>, (const Prefix)p));
     if (int rc = launch_wide(own, s)) return rc;
     return kvc_launch_early(prefix_join_kernel<T, D>, (unsigned)((p.a.B + 1) * ((p.a.Hq + 3) / 4)), 128, s, p);
 }
