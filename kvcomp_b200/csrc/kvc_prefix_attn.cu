@@ -212,6 +212,11 @@ __device__ __forceinline__ bool bar_try(uint64_t *bar, uint32_t parity) {
     asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }" : "=r"(done) : "r"(shared_at(bar)), "r"(parity) : "memory");
     return done;
 }
+__device__ __forceinline__ bool bar_done(uint64_t *bar, uint32_t parity) {                // (try_wait may take some 10000 cycles to say no)
+    uint32_t done;
+    asm volatile("{ .reg .pred p; mbarrier.test_wait.parity.shared.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }" : "=r"(done) : "r"(shared_at(bar)), "r"(parity) : "memory");
+    return done;
+}
 // Waits up to about a second; what runs out is said in *failed, and nothing waits any more then.
 __device__ __forceinline__ void bar_wait(uint64_t *bar, uint32_t parity, volatile int *failed) {
     if (bar_try(bar, parity)) return;
@@ -275,6 +280,20 @@ __device__ __forceinline__ void store16(uint32_t at, const uint32_t *r) {
 #undef KVC_IN
 }
 __device__ __forceinline__ void stores_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// two at a time
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 r;
+    asm("{ .reg .b64 x, y, z; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; mov.b64 z, {%6, %7}; fma.rn.f32x2 x, x, y, z; mov.b64 {%0, %1}, x; }" : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 r;
+    asm("{ .reg .b64 x, y; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; add.rn.f32x2 x, x, y; mov.b64 {%0, %1}, x; }" : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+__device__ __forceinline__ void store_sector(void *to, const uint32_t *r) {               // 32 bytes, of a lane's own row: a whole sector
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
+}
 __device__ __forceinline__ float exp2_approx(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -311,7 +330,7 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_attn_kernel(const __
     constexpr int UNIT = Shape<D>::UNIT, RING = Shape<D>::RING;
     constexpr float LIFT = Weight<T>::LIFT;
     extern __shared__ uint8_t raw[];
-    __shared__ __align__(8) uint64_t full[RING], empty[RING], scores_there[2], weights_there[2], sums_there[2], queries_free[2];
+    __shared__ __align__(8) uint64_t full[RING], empty[RING], scores_there[2], weights_there[2], sums_there[2], queries_there[2], queries_free[2], over;
     __shared__ uint32_t masks[MASKS][4], tensor_s;
     __shared__ int failed_s, warp_sums[PREFIX_THREADS / 32], start_item, start_rest;
     __shared__ Item start_it;
@@ -326,7 +345,8 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_attn_kernel(const __
     }
     if (tid == 0) {
         for (int i = 0; i < RING; i++) { bar_init(full + i, 4); bar_init(empty + i, 1); }
-        for (int i = 0; i < 2; i++) { bar_init(scores_there + i, 1); bar_init(weights_there + i, 4); bar_init(sums_there + i, 1); bar_init(queries_free + i, 1); }
+        for (int i = 0; i < 2; i++) { bar_init(scores_there + i, 1); bar_init(weights_there + i, 4); bar_init(sums_there + i, 1); bar_init(queries_there + i, 4); bar_init(queries_free + i, 1); }
+        bar_init(&over, 1);
         failed_s = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -392,7 +412,7 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_attn_kernel(const __
             // ---- a set of rows: scores -> weights, and the sums' way out
             const int set = warp >> 2, r = tid & 127;
             const uint32_t lanes = (uint32_t)(warp & 3) << 21, scores = tensor + lanes + set * 128, sums = tensor + lanes + 256 + set * 128;
-            int phase = 0;                                  // of this set's jobs
+            int phase = 0, parts = 0;                       // of this set's jobs, of its columns' parts
             for (; w.left > 0; next_part(p, w, groups)) {
                 const int idx = (set - w.jobs) & 1, half = w.wide ? idx : 0, first_n = w.wide ? 0 : idx, step = w.wide ? 1 : 2;
                 if (first_n >= w.in_part) continue;
@@ -441,9 +461,7 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_attn_kernel(const __
                             const float now = up ? high : m, f = up ? exp2_approx(m - now) : 1.0f;
                             m = now;
                             l *= f;
-                            if (n != first_n) {
-                                bar_wait(sums_there + set, phase ^ 1, failed);
-                                after_sync();
+                            if (n != first_n) {             // (the sums are there: what was asked for behind them is)
                                 loads_wait(s[0]);
 #pragma unroll
                                 for (int c = 0; c < D / 32; c++) {
@@ -456,21 +474,22 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_attn_kernel(const __
                             }
                         }
                         const float less = LIFT - (m == -CUDART_INF_F ? 0.0f : m);
-                        float sum[4] = {};
+                        const float2 scale2 = make_float2(p.log2_scaling, p.log2_scaling), less2 = make_float2(less, less);
+                        float2 sum[2] = {};
 #pragma unroll
                         for (int c = 0; c < 4; c++) {
                             chunk(c);
                             uint32_t weights[16];           // (they take the place of scores that have been read)
 #pragma unroll
                             for (int i = 0; i < 16; i++) {
-                                const float w0 = exp2_approx(fmaf(__uint_as_float(s[c & 1][2 * i]), p.log2_scaling, less)), w1 = exp2_approx(fmaf(__uint_as_float(s[c & 1][2 * i + 1]), p.log2_scaling, less));
-                                sum[i & 1] += w0;
-                                sum[2 + (i & 1)] += w1;
-                                weights[i] = pack(w0, w1, T());
+                                const float2 x = fma2(make_float2(__uint_as_float(s[c & 1][2 * i]), __uint_as_float(s[c & 1][2 * i + 1])), scale2, less2);
+                                const float2 y = make_float2(exp2_approx(x.x), exp2_approx(x.y));
+                                sum[i & 1] = add2(sum[i & 1], y);
+                                weights[i] = pack(y.x, y.y, T());
                             }
                             store16(scores + 16 * c, weights);
                         }
-                        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                        l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                         stores_wait();
                     }
                     before_sync();
@@ -478,7 +497,8 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_attn_kernel(const __
                     if (lane == 0) bar_arrive(weights_there + set);
                     phase ^= 1;
                 }
-                bar_wait(sums_there + set, phase ^ 1, failed);
+                bar_wait(sums_there + set, parts, failed);
+                parts ^= 1;
                 after_sync();
                 if (some) {
                     uint32_t o[2][32];
@@ -489,8 +509,7 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_attn_kernel(const __
                         if (c + 1 < D / 32) load32(o[(c + 1) & 1], sums + 32 * (c + 1));
                         if (mine) {
 #pragma unroll
-                            for (int i = 0; i < 8; i++)
-                                __stcg(reinterpret_cast<uint4 *>(p.sums + place * D) + 8 * c + i, make_uint4(o[c & 1][4 * i], o[c & 1][4 * i + 1], o[c & 1][4 * i + 2], o[c & 1][4 * i + 3]));
+                            for (int i = 0; i < 4; i++) store_sector(p.sums + place * D + 32 * c + 8 * i, o[c & 1] + 8 * i);
                         }
                     }
                     if (mine) __stcg(p.maxima + place, make_float2(m - LIFT, l));          // (weights were 2^LIFT times what the maximum says)
@@ -507,39 +526,46 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_attn_kernel(const __
                 const uint64_t queries = operand_at(base, 16), keys = operand_at(ring, 16), values = operand_at(ring, ATOM);
                 int slot = 0, round = 0;                    // of the ring: the next unit's place, and how often it has been through (its last bit)
                 auto next_unit = [&]() { if (++slot == RING) { slot = 0; round ^= 1; } };
-                int phases = 0;                             // a bit for each set: its jobs
-                int late = -1, late_slot = 0, late_round = 0;          // the job before: its set and what its second product needs
-                bool late_first = false, late_last = false, late_waits = false;
-                auto second = [&]() {
-                    if (late < 0) return;
-                    bar_wait(weights_there + late, phases >> late & 1, failed);
-                    phases ^= 1 << late;
-                    bar_wait(full + late_slot, late_round, failed);
+                int phases = 0;                             // a bit for each set: its jobs, the lowest two; the next two: its queries
+                // Of each set the job that waits for its second product, and where its values lie.  A set's scores may be written again when its weights have been read: its next first product
+                // is asked for right behind its second one, and products are made in order.
+                struct { int slot, round; bool there, first, last, ends; } late[2] = {};
+                auto second = [&](int set) {
+                    const auto &job = late[set];
+                    if (!job.there) return;
+                    bar_wait(full + job.slot, job.round, failed);
+                    bar_wait(weights_there + set, phases >> set & 1, failed);
+                    phases ^= 1 << set;
                     after_sync();
-                    const uint64_t b = values + (uint32_t)late_slot * (UNIT / 16);
-                    const uint32_t d = t_at + 256 + late * 128, a_at = t_at + late * 128;
+                    const uint64_t b = values + (uint32_t)job.slot * (UNIT / 16);
+                    const uint32_t d = t_at + 256 + set * 128, a_at = t_at + set * 128;
 #pragma unroll
-                    for (int k = 0; k < TOKENS / 16; k++) product_of_weights(one, d, a_at + 8 * k, b + k * (2048 / 16), VALUES, k > 0 || !late_first);
-                    if (late_last) commit_to(one, empty + late_slot);
-                    commit_to(one, sums_there + late);      // (the last that comes back)
+                    for (int k = 0; k < TOKENS / 16; k++) product_of_weights(one, d, a_at + 8 * k, b + k * (2048 / 16), VALUES, k > 0 || !job.first);
+                    if (job.last) commit_to(one, empty + job.slot);
+                    if (job.ends) commit_to(one, sums_there + set);
                 };
+                int odd = 0, pending = -1;                  // the next job's set; the set whose values are still to come
                 for (; all_lanes(w.left) > 0; next_part(p, w, groups)) {
-                    const int in_part = all_lanes(w.in_part), jobs = all_lanes(w.jobs);
+                    const int in_part = all_lanes(w.in_part);
                     const bool wide = all_lanes(w.wide);
                     for (int n = 0; n < in_part; n++) {
                         const bool begins = wide ? n == 0 : n < 2, ends = wide ? n == in_part - 1 : n + 2 >= in_part;
                         const int k_slot = slot;
                         bar_wait(full + slot, round, failed);
                         next_unit();
-                        if (late_waits) {                   // the values of the tile before come behind this one's keys
-                            late_slot = slot; late_round = round;
+                        if (pending >= 0) {                 // the values of the tile before come behind this one's keys
+                            if (pending) late[1].slot = slot, late[1].round = round;
+                            else late[0].slot = slot, late[0].round = round;
                             next_unit();
                         }
                         const int v_slot = slot, v_round = round;       // (wide)
                         if (wide) next_unit();
-                        for (int j = 0; j < (wide ? 2 : 1); j++) {
-                            const int set = (jobs + (wide ? j : n)) & 1;
-                            const bool last = !wide || j == 1;
+                        auto job = [&](int set, bool last) {
+                            second(set);
+                            if (begins) {
+                                bar_wait(queries_there + set, phases >> (2 + set) & 1, failed);
+                                phases ^= 4 << set;
+                            }
                             after_sync();
                             const uint64_t q_at = queries + set * (UNIT / 16), k_at = keys + (uint32_t)k_slot * (UNIT / 16);
                             const uint32_t d = t_at + set * 128;
@@ -548,41 +574,51 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_attn_kernel(const __
                             commit_to(one, scores_there + set);
                             if (ends) commit_to(one, queries_free + set);
                             if (last) commit_to(one, empty + k_slot);
-                            second();
-                            late = set; late_slot = v_slot; late_round = v_round; late_first = begins; late_last = last;
+                            late[set] = {v_slot, v_round, true, begins, last, ends};
+                            odd ^= 1;
+                        };
+                        for (int j = 0; j < (wide ? 2 : 1); j++) {
+                            const bool last = !wide || j == 1;
+                            if (odd) job(1, last);
+                            else job(0, last);
                         }
-                        late_waits = !wide;
+                        pending = wide ? -1 : odd ^ 1;
                     }
                 }
-                if (late_waits) { late_slot = slot; late_round = round; }
-                second();
-                // all products are done before anything is given back
-                if (late >= 0) bar_wait(sums_there + late, phases >> late & 1 ^ 1, failed);
+                if (pending >= 0) {
+                    if (pending) late[1].slot = slot, late[1].round = round;
+                    else late[0].slot = slot, late[0].round = round;
+                }
+                if (odd) { second(1); second(0); }
+                else { second(0); second(1); }
+                commit_to(one, &over);                      // all products are done before anything is given back
+                bar_wait(&over, 0, failed);
                 __syncwarp();
             } else {
                 // ---- the copies: of each tile of keys or values four times 32 rows, which the warps take in turn
                 const int mine = warp - 9;
-                int signal = -1, tile_n = 0, loads0 = 0, loads1 = 0;          // the tile whose copies are on their way and not said to be there, times the sets' queries were loaded
-                auto say = [&](int unit) {
+                uint64_t *signal = nullptr;                 // where to say that the copies on their way are there
+                int tile_n = 0, loads0 = 0, loads1 = 0;     // times the sets' queries were loaded
+                auto say = [&]() {
                     seen_by_products();
                     __syncwarp();
-                    if (lane == 0) bar_arrive(full + unit % RING);
+                    if (lane == 0) bar_arrive(signal);
                 };
                 auto drain = [&]() {
-                    if (signal < 0) return;
+                    if (!signal) return;
                     copies_wait<0>();
-                    say(signal);
-                    signal = -1;
+                    say();
+                    signal = nullptr;
                 };
                 auto wait = [&](uint64_t *bar, uint32_t parity) {   // (what is waited for may need what this warp has copied)
-                    if (__all_sync(0xffffffffu, bar_try(bar, parity))) return;
+                    if (__all_sync(0xffffffffu, bar_done(bar, parity))) return;
                     drain();
                     bar_wait(bar, parity, failed);
                     __syncwarp();
                 };
                 // Units of the ring in the order of their use: a tile's keys, and its values behind the next tile's keys (narrow: the next job's first product runs before them) or behind
                 // its own (wide).
-                int block = 0;                              // 32 rows of a unit, of all that came before
+                int block = 0, unit = 0;                    // 32 rows of a unit or of queries, units: all that came before
                 int v_tile = -1, v_table = 0, v_len = 0, v_head = 0;                       // values that are still to come: of which tile
                 auto rows_of = [&](int values, int unit, int i, int tile, int table, int len, int k_head) {
                     const int t = tile * TOKENS + 32 * i + lane, at_page = kvc_divide(t, p.page), row = t - at_page * (int)a.page_size;
@@ -596,42 +632,49 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_attn_kernel(const __
                     if (good) from += values ? page * a.vp_page + row * a.vp_row + k_head * a.vp_head : page * a.kp_page + row * a.kp_row + k_head * a.kp_head;
                     copy_rows<T, D>(ring + unit % RING * UNIT, i, from, mask, lane);
                 };
-                auto sent = [&](int unit) {                 // what was copied is said to be there when the next rows are on their way
+                auto sent = [&](uint64_t *bar) {            // what was copied is said to be there when the next rows are on their way
                     copies_commit();
-                    if (signal >= 0) {
+                    if (signal) {
                         copies_wait<1>();
-                        say(signal);
+                        say();
                     }
-                    signal = unit;
+                    signal = bar;
                 };
                 auto values_of = [&]() {
-                    const int unit = block / 4;
 #pragma unroll 1
                     for (int i = 0; i < 4; i++, block++) {
                         if (block % LOADERS != mine) continue;
                         rows_of(1, unit, i, v_tile, v_table, v_len, v_head);
-                        sent(unit);
+                        sent(full + unit % RING);
                     }
+                    unit++;
                     v_tile = -1;
                 };
                 for (; w.left > 0; next_part(p, w, groups)) for (int n = 0; n < w.in_part; n++, tile_n++) {
-                    const int sets = w.wide ? 2 : 1, first_job = w.jobs + n * sets, unit = block / 4;
+                    const int sets = w.wide ? 2 : 1, first_job = w.jobs + n * sets;
                     const bool begins = w.wide ? n == 0 : n < 2;
+                    if (begins)
+                        for (int j = 0; j < sets; j++) {
+                            const int set = (first_job + j) & 1, loads = set ? loads1 : loads0;
 #pragma unroll 1
-                    for (int i = 0; i < 4; i++, block++) {
-                        if (block % LOADERS != mine) continue;
-                        rows_of(0, unit, i, w.tile + n, w.it.table, w.it.len, w.k_head);
-                        if (begins)
-                            for (int j = 0; j < sets; j++) {
-                                const int set = (first_job + j) & 1, loads = set ? loads1 : loads0, from = w.part * 2 * ROWS + j * ROWS, R = from + 32 * i + lane, member = kvc_divide(R, p.group);
+                            for (int i = 0; i < 4; i++, block++) {
+                                if (block % LOADERS != mine) continue;
+                                const int R = w.part * 2 * ROWS + j * ROWS + 32 * i + lane, member = kvc_divide(R, p.group);
                                 int row = R < w.it.rows ? member_at(p, w.it.first + member) : -1;
                                 if (row >= 0) row = row_of(p, row);
                                 if (loads > 0) wait(queries_free + set, (loads - 1) & 1);
                                 const uint32_t mask = __ballot_sync(0xffffffffu, row >= 0);
                                 if (mask) copy_rows<T, D>(base + set * UNIT, i, reinterpret_cast<const T *>(a.q) + (row >= 0 ? (long long)row * a.q_token + (w.k_head * p.g + R - member * p.g) * a.q_head : 0), mask, lane);
+                                sent(queries_there + set);
                             }
-                        sent(unit);
+                        }
+#pragma unroll 1
+                    for (int i = 0; i < 4; i++, block++) {
+                        if (block % LOADERS != mine) continue;
+                        rows_of(0, unit, i, w.tile + n, w.it.table, w.it.len, w.k_head);
+                        sent(full + unit % RING);
                     }
+                    unit++;
                     if (begins) {
                         if (w.wide) loads0++, loads1++;
                         else if (first_job & 1) loads1++;
