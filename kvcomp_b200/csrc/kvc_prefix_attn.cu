@@ -286,6 +286,11 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
     asm("{ .reg .b64 x, y, z; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; mov.b64 z, {%6, %7}; fma.rn.f32x2 x, x, y, z; mov.b64 {%0, %1}, x; }" : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
     return r;
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     float2 r;
     asm("{ .reg .b64 x, y; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; add.rn.f32x2 x, x, y; mov.b64 {%0, %1}, x; }" : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
@@ -412,6 +417,7 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_attn_kernel(const __
             // ---- a set of rows: scores -> weights, and the sums' way out
             const int set = warp >> 2, r = tid & 127;
             const uint32_t lanes = (uint32_t)(warp & 3) << 21, scores = tensor + lanes + set * 128, sums = tensor + lanes + 256 + set * 128;
+            const uint32_t lowest = p.negative ? 0x7f800000u : 0xff800000u;                // (before they are scaled)
             int phase = 0, parts = 0;                       // of this set's jobs, of its columns' parts
             for (; w.left > 0; next_part(p, w, groups)) {
                 const int idx = (set - w.jobs) & 1, half = w.wide ? idx : 0, first_n = w.wide ? 0 : idx, step = w.wide ? 1 : 2;
@@ -430,64 +436,83 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_attn_kernel(const __
                     bar_wait(scores_there + set, phase, failed);
                     after_sync();
                     if (some) {
-                        // Twice over the scores, 32 at a time (all 128 at once would not leave registers enough): their maximum, then the weights
                         const uint32_t *const mask = masks[(w.tiles_before + n) % MASKS];
-                        uint32_t s[2][32];
-                        auto chunk = [&](int c) {           // 32 scores are here, the next 32 are asked for
-                            loads_wait(s[c & 1]);
-                            if (c < 3) load32(s[(c + 1) & 1], scores + 32 * (c + 1));
-                            if (p.negative) {
-#pragma unroll
-                                for (int i = 0; i < 32; i++) s[c & 1][i] ^= 0x80000000u;
-                            }
-                            if (mask[c] != 0xffffffffu) {
+                        if ((mask[0] & mask[1] & mask[2] & mask[3]) != 0xffffffffu) {      // tokens that are none (a column's last tile, bad pages): their scores become the lowest
+#pragma unroll 1
+                            for (int c = 0; c < 4; c++) {
+                                uint32_t x[32];
+                                load32(x, scores + 32 * c);
+                                loads_wait(x);
                                 const uint32_t on = mask[c];
 #pragma unroll
-                                for (int i = 0; i < 32; i++) s[c & 1][i] = on >> i & 1 ? s[c & 1][i] : 0xff800000u;
+                                for (int i = 0; i < 32; i++) x[i] = on >> i & 1 ? x[i] : lowest;
+                                store32(scores + 32 * c, x);
+                            }
+                            stores_wait();
+                        }
+                        // Twice over the scores, 32 at a time (all 128 at once would not leave registers enough): their maximum, then the weights.  Loops of two steps: all four in a row are
+                        // more instructions than are at hand when the sets come by (64 requests behind 16384 tokens 48 us, so 40).
+                        uint32_t x[32], y[32];
+                        float top[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
+                        auto highest = [&](const uint32_t *v) {
+                            if (p.negative) {
+#pragma unroll
+                                for (int i = 0; i < 32; i++) top[i & 3] = fmaxf(top[i & 3], -__uint_as_float(v[i]));
+                            } else {
+#pragma unroll
+                                for (int i = 0; i < 16; i++) top[i & 3] = max3(top[i & 3], __uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
                             }
                         };
-                        load32(s[0], scores);
-                        float top[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
-#pragma unroll
-                        for (int c = 0; c < 4; c++) {
-                            chunk(c);
-#pragma unroll
-                            for (int i = 0; i < 32; i++) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(s[c & 1][i]));
+                        load32(x, scores);
+#pragma unroll 1
+                        for (int c = 0; c < 2; c++) {
+                            loads_wait(x);
+                            load32(y, scores + 64 * c + 32);
+                            highest(x);
+                            loads_wait(y);
+                            load32(x, scores + (c == 0 ? 64 : 0));       // (and the first again)
+                            highest(y);
                         }
-                        load32(s[0], scores);
-                        const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.log2_scaling;
+                        const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * fabsf(p.log2_scaling);
                         const bool up = high > m + SLACK || (m == -CUDART_INF_F && high > m);
                         if (__any_sync(0xffffffffu, up)) {
                             const float now = up ? high : m, f = up ? exp2_approx(m - now) : 1.0f;
                             m = now;
                             l *= f;
                             if (n != first_n) {             // (the sums are there: what was asked for behind them is)
-                                loads_wait(s[0]);
-#pragma unroll
+                                loads_wait(x);
+#pragma unroll 1
                                 for (int c = 0; c < D / 32; c++) {
-                                    load32(s[1], sums + 32 * c);
-                                    loads_wait(s[1]);
+                                    load32(y, sums + 32 * c);
+                                    loads_wait(y);
 #pragma unroll
-                                    for (int i = 0; i < 32; i++) s[1][i] = __float_as_uint(__uint_as_float(s[1][i]) * f);
-                                    store32(sums + 32 * c, s[1]);
+                                    for (int i = 0; i < 32; i++) y[i] = __float_as_uint(__uint_as_float(y[i]) * f);
+                                    store32(sums + 32 * c, y);
                                 }
                             }
                         }
                         const float less = LIFT - (m == -CUDART_INF_F ? 0.0f : m);
                         const float2 scale2 = make_float2(p.log2_scaling, p.log2_scaling), less2 = make_float2(less, less);
                         float2 sum[2] = {};
-#pragma unroll
-                        for (int c = 0; c < 4; c++) {
-                            chunk(c);
+                        auto weigh = [&](const uint32_t *v, uint32_t to) {
                             uint32_t weights[16];           // (they take the place of scores that have been read)
 #pragma unroll
                             for (int i = 0; i < 16; i++) {
-                                const float2 x = fma2(make_float2(__uint_as_float(s[c & 1][2 * i]), __uint_as_float(s[c & 1][2 * i + 1])), scale2, less2);
-                                const float2 y = make_float2(exp2_approx(x.x), exp2_approx(x.y));
-                                sum[i & 1] = add2(sum[i & 1], y);
-                                weights[i] = pack(y.x, y.y, T());
+                                const float2 e = fma2(make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), scale2, less2);
+                                const float2 f = make_float2(exp2_approx(e.x), exp2_approx(e.y));
+                                sum[i & 1] = add2(sum[i & 1], f);
+                                weights[i] = pack(f.x, f.y, T());
                             }
-                            store16(scores + 16 * c, weights);
+                            store16(to, weights);
+                        };
+#pragma unroll 1
+                        for (int c = 0; c < 2; c++) {
+                            loads_wait(x);
+                            load32(y, scores + 64 * c + 32);
+                            weigh(x, scores + 32 * c);
+                            loads_wait(y);
+                            if (c == 0) load32(x, scores + 64);
+                            weigh(y, scores + 32 * c + 16);
                         }
                         l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                         stores_wait();
@@ -856,7 +881,7 @@ extern "C" int kvc_paged_attn_shared(const kvc_paged_attn_args *args, const int3
     p.grid = kvc_sm_count();
     p.n_pages = (unsigned)a.n_pages;
     p.negative = a.scaling < 0.0f;
-    p.log2_scaling = std::max(fabsf(a.scaling) * 1.4426950408889634f, 1e-37f);      // (0 times the -inf of a token that is left out is none)
+    p.log2_scaling = std::max(fabsf(a.scaling) * 1.4426950408889634f, 1e-37f) * (p.negative ? -1.0f : 1.0f);      // (0 times the infinite score of a token that is left out is none)
     uint8_t *at_ws = reinterpret_cast<uint8_t *>(a.workspace) + own_bytes(a.Hq, a.Hkv, a.D);
     p.item_first = reinterpret_cast<int32_t *>(at_ws);
     p.share = p.item_first + a.B;
