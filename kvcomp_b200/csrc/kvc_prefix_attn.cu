@@ -26,7 +26,7 @@ namespace {
 
 using kvc_paged::Params, kvc_paged::set_params, kvc_paged::launch_wide, kvc_paged::counter_bytes, kvc_paged::places, kvc_paged::group_of, kvc_paged::part_floats, kvc_paged::columns_of;
 
-constexpr int PREFIX_THREADS = 512, LOADERS = 7, ROWS = 128, TOKENS = 128, ATOM = 16384;       // ATOM: 128 rows of 128 bytes
+constexpr int PREFIX_THREADS = 512, QUERY_LOADERS = 3, ROWS = 128, TOKENS = 128, ATOM = 16384;       // ATOM: 128 rows of 128 bytes
 constexpr int MASKS = 16;
 constexpr int MAX_REQUESTS = 16384;
 
@@ -305,18 +305,22 @@ __device__ __forceinline__ float exp2_approx(float x) {
     return r;
 }
 
-// Rows 32 i .. 32 i + 31 of a tile, by a warp: `from` is the lane's own row, mask says which there are (the others become zeros).
-template <typename T, int D> __device__ __forceinline__ void copy_rows(uint32_t to, int i, const T *from, uint32_t mask, int lane) {
+// Rows 32 i .. 32 i + 31 of a tile, by a warp: `from` is the lane's own row, mask says which there are (the others become zeros).  between() is called when a quarter is on its way.
+template <typename T, int D, typename F> __device__ __forceinline__ void copy_rows(uint32_t to, int i, const T *from, uint32_t mask, int lane, F between) {
     constexpr int SIDE = D == 96 ? 4 : D / 8 > 16 ? 16 : D / 8;                           // lanes of a row
-#pragma unroll 4
-    for (int k = 0; k < SIDE; k++) {
-        const int j = k * (32 / SIDE) + lane / SIDE, r = 32 * i + j;
-        const T *row = reinterpret_cast<const T *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(from), j));
+#pragma unroll 1
+    for (int k0 = 0; k0 < SIDE; k0 += 4) {
 #pragma unroll
-        for (int c0 = 0; c0 < D / 8; c0 += SIDE) {
-            const int c = c0 + lane % SIDE;
-            copy16(to + (c >> 3) * ATOM + r * 128 + ((c & 7) ^ (r & 7)) * 16, row + c * 8, mask >> j & 1);
+        for (int k = 0; k < 4; k++) {
+            const int j = (k0 + k) * (32 / SIDE) + lane / SIDE, r = 32 * i + j;
+            const T *row = reinterpret_cast<const T *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(from), j));
+#pragma unroll
+            for (int c0 = 0; c0 < D / 8; c0 += SIDE) {
+                const int c = c0 + lane % SIDE;
+                copy16(to + (c >> 3) * ATOM + r * 128 + ((c & 7) ^ (r & 7)) * 16, row + c * 8, mask >> j & 1);
+            }
         }
+        if (k0 == 0) between();
     }
 }
 
@@ -619,99 +623,82 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_attn_kernel(const __
                 commit_to(one, &over);                      // all products are done before anything is given back
                 bar_wait(&over, 0, failed);
                 __syncwarp();
-            } else {
-                // ---- the copies: of each tile of keys or values four times 32 rows, which the warps take in turn
-                const int mine = warp - 9;
+            } else if (warp < 13) {
+                // ---- the copies of keys and values: each of four warps has 32 rows of every tile, whose pages it asks for a tile ahead
+                const int i = warp - 9;
                 uint64_t *signal = nullptr;                 // where to say that the copies on their way are there
-                int tile_n = 0, loads0 = 0, loads1 = 0;     // times the sets' queries were loaded
-                auto say = [&]() {
+                auto say = [&]() {                          // (of what has been committed; it is called when the first of the next rows are on their way)
+                    if (!signal) return;
+                    copies_wait<0>();
                     seen_by_products();
                     __syncwarp();
                     if (lane == 0) bar_arrive(signal);
-                };
-                auto drain = [&]() {
-                    if (!signal) return;
-                    copies_wait<0>();
-                    say();
                     signal = nullptr;
-                };
-                auto wait = [&](uint64_t *bar, uint32_t parity) {   // (what is waited for may need what this warp has copied)
-                    if (__all_sync(0xffffffffu, bar_done(bar, parity))) return;
-                    drain();
-                    bar_wait(bar, parity, failed);
-                    __syncwarp();
                 };
                 // Units of the ring in the order of their use: a tile's keys, and its values behind the next tile's keys (narrow: the next job's first product runs before them) or behind
                 // its own (wide).
-                int block = 0, unit = 0;                    // 32 rows of a unit or of queries, units: all that came before
-                int v_tile = -1, v_table = 0, v_len = 0, v_head = 0;                       // values that are still to come: of which tile
-                auto rows_of = [&](int values, int unit, int i, int tile, int table, int len, int k_head) {
-                    const int t = tile * TOKENS + 32 * i + lane, at_page = kvc_divide(t, p.page), row = t - at_page * (int)a.page_size;
-                    const int page = t < len ? a.table[table * a.table_stride + at_page] : -1;
-                    if (unit >= RING) wait(empty + unit % RING, (unit / RING - 1) & 1);
-                    const bool good = (unsigned)page < p.n_pages;
-                    if (!good && t < len) flags |= KVC_FLAG_BAD_PAGE;
-                    const uint32_t mask = __ballot_sync(0xffffffffu, good);
-                    if (values == 0 && lane == 0) masks[tile_n % MASKS][i] = mask;
+                int slot = 0, round = 1;                    // the next unit's place; the bit to wait for there (1: the first time round there is nothing to wait for)
+                auto send = [&](bool values, int page, uint32_t mask, int t, int k_head) {
+                    if (!__all_sync(0xffffffffu, bar_done(empty + slot, round))) {
+                        say();                              // (what is waited for may need what this warp has copied)
+                        bar_wait(empty + slot, round, failed);
+                        __syncwarp();
+                    }
                     const T *from = reinterpret_cast<const T *>(values ? a.vpages : a.kpages);
-                    if (good) from += values ? page * a.vp_page + row * a.vp_row + k_head * a.vp_head : page * a.kp_page + row * a.kp_row + k_head * a.kp_head;
-                    copy_rows<T, D>(ring + unit % RING * UNIT, i, from, mask, lane);
-                };
-                auto sent = [&](uint64_t *bar) {            // what was copied is said to be there when the next rows are on their way
+                    const int row = t - kvc_divide(t, p.page) * (int)a.page_size;
+                    if (mask >> lane & 1) from += values ? page * a.vp_page + row * a.vp_row + k_head * a.vp_head : page * a.kp_page + row * a.kp_row + k_head * a.kp_head;
+                    copy_rows<T, D>(ring + slot * UNIT, i, from, mask, lane, say);
                     copies_commit();
-                    if (signal) {
-                        copies_wait<1>();
-                        say();
-                    }
-                    signal = bar;
+                    signal = full + slot;
+                    if (++slot == RING) { slot = 0; round ^= 1; }
                 };
-                auto values_of = [&]() {
-#pragma unroll 1
-                    for (int i = 0; i < 4; i++, block++) {
-                        if (block % LOADERS != mine) continue;
-                        rows_of(1, unit, i, v_tile, v_table, v_len, v_head);
-                        sent(full + unit % RING);
+                int tile_n = 0, late_page = 0, late_t = 0, late_head = 0;
+                uint32_t late_mask = 0;
+                bool late = false;                          // values that are still to come
+                for (; w.left > 0; next_part(p, w, groups)) {
+                    const int32_t *const pages = a.table + w.it.table * a.table_stride;
+                    int t = w.tile * TOKENS + 32 * i + lane, page = t < w.it.len ? pages[kvc_divide(t, p.page)] : -1;
+                    for (int n = 0; n < w.in_part; n++, tile_n++, t += TOKENS) {
+                        const int behind = t + TOKENS, next = n + 1 < w.in_part && behind < w.it.len ? pages[kvc_divide(behind, p.page)] : -1;
+                        const bool good = (unsigned)page < p.n_pages;
+                        if (!good && t < w.it.len) flags |= KVC_FLAG_BAD_PAGE;
+                        const uint32_t mask = __ballot_sync(0xffffffffu, good);
+                        if (lane == 0) masks[tile_n % MASKS][i] = mask;
+                        send(false, page, mask, t, w.k_head);
+                        if (late) send(true, late_page, late_mask, late_t, late_head);
+                        late = !w.wide;
+                        if (w.wide) send(true, page, mask, t, w.k_head);
+                        late_page = page; late_mask = mask; late_t = t; late_head = w.k_head;
+                        page = next;
                     }
-                    unit++;
-                    v_tile = -1;
-                };
-                for (; w.left > 0; next_part(p, w, groups)) for (int n = 0; n < w.in_part; n++, tile_n++) {
-                    const int sets = w.wide ? 2 : 1, first_job = w.jobs + n * sets;
-                    const bool begins = w.wide ? n == 0 : n < 2;
-                    if (begins)
-                        for (int j = 0; j < sets; j++) {
-                            const int set = (first_job + j) & 1, loads = set ? loads1 : loads0;
-#pragma unroll 1
-                            for (int i = 0; i < 4; i++, block++) {
-                                if (block % LOADERS != mine) continue;
-                                const int R = w.part * 2 * ROWS + j * ROWS + 32 * i + lane, member = kvc_divide(R, p.group);
-                                int row = R < w.it.rows ? member_at(p, w.it.first + member) : -1;
-                                if (row >= 0) row = row_of(p, row);
-                                if (loads > 0) wait(queries_free + set, (loads - 1) & 1);
-                                const uint32_t mask = __ballot_sync(0xffffffffu, row >= 0);
-                                if (mask) copy_rows<T, D>(base + set * UNIT, i, reinterpret_cast<const T *>(a.q) + (row >= 0 ? (long long)row * a.q_token + (w.k_head * p.g + R - member * p.g) * a.q_head : 0), mask, lane);
-                                sent(queries_there + set);
-                            }
-                        }
-#pragma unroll 1
-                    for (int i = 0; i < 4; i++, block++) {
-                        if (block % LOADERS != mine) continue;
-                        rows_of(0, unit, i, w.tile + n, w.it.table, w.it.len, w.k_head);
-                        sent(full + unit % RING);
-                    }
-                    unit++;
-                    if (begins) {
-                        if (w.wide) loads0++, loads1++;
-                        else if (first_job & 1) loads1++;
-                        else loads0++;
-                    }
-                    if (v_tile >= 0) values_of();
-                    v_tile = w.tile + n; v_table = w.it.table; v_len = w.it.len; v_head = w.k_head;
-                    if (w.wide) values_of();
                 }
-                if (v_tile >= 0) values_of();
-                drain();
-                copies_wait<0>();
+                if (late) send(true, late_page, late_mask, late_t, late_head);
+                say();
+            } else {
+                // ---- the copies of queries: the columns' rows, 32 at a time, by three warps in turn
+                int block = warp - 13, loads0 = 0, loads1 = 0;      // times the sets' queries were loaded
+                for (; w.left > 0; next_part(p, w, groups)) {
+                    const int sets = w.wide || w.in_part > 1 ? 2 : 1;           // (narrow: both sets have the same rows)
+                    for (; block < 4 * sets; block += QUERY_LOADERS) {
+                        const int j = block >> 2, i = block & 3, set = (w.jobs + j) & 1, loads = set ? loads1 : loads0;
+                        const int R = w.part * 2 * ROWS + (w.wide ? j * ROWS : 0) + 32 * i + lane, member = kvc_divide(R, p.group);
+                        int row = R < w.it.rows ? member_at(p, w.it.first + member) : -1;
+                        if (row >= 0) row = row_of(p, row);
+                        if (loads > 0) bar_wait(queries_free + set, (loads - 1) & 1, failed);
+                        __syncwarp();
+                        const uint32_t mask = __ballot_sync(0xffffffffu, row >= 0);
+                        if (mask) copy_rows<T, D>(base + set * UNIT, i, reinterpret_cast<const T *>(a.q) + (row >= 0 ? (long long)row * a.q_token + (w.k_head * p.g + R - member * p.g) * a.q_head : 0), mask, lane, []() {});
+                        copies_commit();
+                        copies_wait<0>();
+                        seen_by_products();
+                        __syncwarp();
+                        if (lane == 0) bar_arrive(queries_there + set);
+                    }
+                    block -= 4 * sets;
+                    if (sets == 2) loads0++, loads1++;
+                    else if (w.jobs & 1) loads1++;
+                    else loads0++;
+                }
             }
         }
     }
