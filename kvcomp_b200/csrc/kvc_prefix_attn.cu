@@ -626,30 +626,43 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_attn_kernel(const __
             } else if (warp < 13) {
                 // ---- the copies of keys and values: each of four warps has 32 rows of every tile, whose pages it asks for a tile ahead
                 const int i = warp - 9;
-                uint64_t *signal = nullptr;                 // where to say that the copies on their way are there
-                auto say = [&]() {                          // (of what has been committed; it is called when the first of the next rows are on their way)
-                    if (!signal) return;
-                    copies_wait<0>();
+                constexpr int ON_THE_WAY = RING > 5 ? 4 : 2;               // units whose copies are on their way while the next ones are asked for
+                uint64_t *signals[ON_THE_WAY] = {};         // where to say that they are there, the oldest first
+                auto say = [&](uint64_t *bar) {
                     seen_by_products();
                     __syncwarp();
-                    if (lane == 0) bar_arrive(signal);
-                    signal = nullptr;
+                    if (lane == 0) bar_arrive(bar);
+                };
+                auto drain = [&]() {
+                    copies_wait<0>();
+#pragma unroll
+                    for (int k = 0; k < ON_THE_WAY; k++) {
+                        if (signals[k]) say(signals[k]);
+                        signals[k] = nullptr;
+                    }
+                };
+                auto oldest = [&]() {                       // (called when the first copies of the next unit are on their way)
+                    if (!signals[0]) return;
+                    copies_wait<ON_THE_WAY - 1>();
+                    say(signals[0]);
                 };
                 // Units of the ring in the order of their use: a tile's keys, and its values behind the next tile's keys (narrow: the next job's first product runs before them) or behind
                 // its own (wide).
                 int slot = 0, round = 1;                    // the next unit's place; the bit to wait for there (1: the first time round there is nothing to wait for)
                 auto send = [&](bool values, int page, uint32_t mask, int t, int k_head) {
                     if (!__all_sync(0xffffffffu, bar_done(empty + slot, round))) {
-                        say();                              // (what is waited for may need what this warp has copied)
+                        drain();                            // (what is waited for may need what this warp has copied)
                         bar_wait(empty + slot, round, failed);
                         __syncwarp();
                     }
                     const T *from = reinterpret_cast<const T *>(values ? a.vpages : a.kpages);
                     const int row = t - kvc_divide(t, p.page) * (int)a.page_size;
                     if (mask >> lane & 1) from += values ? page * a.vp_page + row * a.vp_row + k_head * a.vp_head : page * a.kp_page + row * a.kp_row + k_head * a.kp_head;
-                    copy_rows<T, D>(ring + slot * UNIT, i, from, mask, lane, say);
+                    copy_rows<T, D>(ring + slot * UNIT, i, from, mask, lane, oldest);
                     copies_commit();
-                    signal = full + slot;
+#pragma unroll
+                    for (int k = 0; k + 1 < ON_THE_WAY; k++) signals[k] = signals[k + 1];
+                    signals[ON_THE_WAY - 1] = full + slot;
                     if (++slot == RING) { slot = 0; round ^= 1; }
                 };
                 int tile_n = 0, late_page = 0, late_t = 0, late_head = 0;
@@ -673,7 +686,7 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_attn_kernel(const __
                     }
                 }
                 if (late) send(true, late_page, late_mask, late_t, late_head);
-                say();
+                drain();
             } else {
                 // ---- the copies of queries: the columns' rows, 32 at a time, by three warps in turn
                 int block = warp - 13, loads0 = 0, loads1 = 0;      // times the sets' queries were loaded
