@@ -713,6 +713,7 @@ def k_matvec(k, q, out):
 # are checked, results made and arguments packed by csrc/kvc_torch.cpp.
 
 PAGED_HEADS = (64, 96, 128, 256)                # channels that paged_attn takes
+SHARED_HEADS = (64, 96, 128)                    # and paged_attn_shared
 _LAYOUTS = {"half": _lib.ROTARY_HALF, "interleaved": _lib.ROTARY_INTERLEAVED}
 
 
