@@ -20,11 +20,13 @@ struct CodesParams {
     kvc_scales s;
     kvc_div page;
     long long slots;                                        // of the pool
-    int lanes, units;                                       // lanes of a row (a power of two), those that have channels
+    int lanes, units, tokens;                               // lanes of a row (a power of two), those that have channels; tokens of a CTA
     Part parts[3];
+    int ctas;                                               // for these tokens: one for every few heads
+    kvc_div by_ctas;
 };
 
-constexpr int CODES_THREADS = 256, CHUNK = 4;
+constexpr int CODES_THREADS = 128, CODES_CTAS = 5, CHUNK = 4;
 constexpr float LEAST_SCALE = 7.888609052210118e-31f;       // 2^-100
 
 // bits of |x|, so that what is no number is the largest
@@ -34,8 +36,12 @@ __device__ __forceinline__ uint32_t size_of(float x) { return __float_as_uint(x)
 template <int KIND> __device__ __forceinline__ float scale_of(uint32_t top, float &inverse) {
     float s;
     if (KIND == KVC_CODES_INT8) {
-        s = fmaxf(__fdiv_rn(__uint_as_float(top), 127.0f), LEAST_SCALE);
-        inverse = __frcp_rn(s);
+        // top / 127 rounded: a product with the rounded reciprocal, and its remainder, exact, times that (Markstein, Computation of elementary functions on the IBM RISC System/6000
+        // processor, 1990)
+        constexpr float LESS = 1.0f / 127.0f;
+        const float t = __uint_as_float(top), q = t * LESS;
+        s = fmaxf(fmaf(fmaf(-127.0f, q, t), LESS, q), LEAST_SCALE);
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inverse) : "f"(s));
     } else {                                                // top = m 2^e, 448 = 1.75 2^8: e - 8, one more where m is above 1.75
         const int e = max((int)((top + 0x1fffffu) >> 23) - 8, 127 - 100);
         s = __uint_as_float((uint32_t)e << 23);
@@ -45,40 +51,68 @@ template <int KIND> __device__ __forceinline__ float scale_of(uint32_t top, floa
     return s;
 }
 
-// Four codes of a row, packed.  int8: x times one over s is off by 127 1.5 2^-24 of a step at most, so the whole number next to it is right unless it lies that near the border
+// two at a time, each rounded
+__device__ __forceinline__ float2 mul2(float2 a, float b) {
+    float2 r;
+    asm("{ .reg .b64 x, y; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %4}; mul.rn.f32x2 x, x, y; mov.b64 {%0, %1}, x; }" : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 r;
+    asm("{ .reg .b64 x, y; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; add.rn.f32x2 x, x, y; mov.b64 {%0, %1}, x; }" : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+// the largest size of three; no number if one is none
+__device__ __forceinline__ float largest(float a, float b, float c) {
+    float r;
+    asm("{ .reg .f32 x, y; abs.f32 x, %2; abs.f32 y, %3; max.NaN.f32 %0, %1, x, y; }" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+__device__ __forceinline__ float larger(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+// Codes of 4 N values of a row, packed.  int8: x times one over s (off by 2^-23 of it) is off by 127 1.5 2^-23 of a step at most, so the whole number next to it is right unless it lies that near the border
 // of two.  There the remainder x - q s says: it is a multiple of s's last bit and no larger than s, hence exact.
-template <int KIND> __device__ __forceinline__ uint32_t codes4(const float *x, float s, float inverse) {
+template <int KIND, int N> __device__ __forceinline__ void codes_of(const float *x, float s, float inverse, uint32_t *packed) {
     if (KIND == KVC_CODES_INT8) {
         constexpr float WHOLE = 12582912.0f;                // 1.5 2^23: a sum's last bits are a whole number's
-        uint32_t c[4];
+        float2 w[2 * N];
         float far = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const float t = __fmul_rn(x[i], inverse), w = __fadd_rn(t, WHOLE);
-            c[i] = __float_as_uint(w);
-            far = fmaxf(far, fabsf(t - (w - WHOLE)));
+        for (int i = 0; i < 2 * N; i++) {
+            const float2 t = mul2(make_float2(x[2 * i], x[2 * i + 1]), inverse);
+            w[i] = add2(t, make_float2(WHOLE, WHOLE));
+            const float2 q = add2(w[i], make_float2(-WHOLE, -WHOLE)), rest = add2(t, make_float2(-q.x, -q.y));
+            far = largest(far, rest.x, rest.y);
         }
         if (far > 0.4999f) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float q = __uint_as_float(c[i]) - WHOLE, r = fmaf(-q, s, x[i]), d = 2.0f * fabsf(r);
-                if (d > s || (d == s && (c[i] & 1))) c[i] += r > 0.0f ? 1 : -1;
+            for (int i = 0; i < 4 * N; i++) {
+                float &c = i & 1 ? w[i / 2].y : w[i / 2].x;
+                const float q = c - WHOLE, r = fmaf(-q, s, x[i]), d = 2.0f * fabsf(r);
+                if (d > s || (d == s && (__float_as_uint(c) & 1))) c += r > 0.0f ? 1.0f : -1.0f;
             }
         }
-        return __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+#pragma unroll
+        for (int i = 0; i < N; i++)
+            packed[i] = __byte_perm(__byte_perm(__float_as_uint(w[2 * i].x), __float_as_uint(w[2 * i].y), 0x0040), __byte_perm(__float_as_uint(w[2 * i + 1].x), __float_as_uint(w[2 * i + 1].y), 0x0040), 0x5410);
     } else {
-        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(x[0] * inverse, x[1] * inverse), __NV_SATFINITE, __NV_E4M3);
-        const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(x[2] * inverse, x[3] * inverse), __NV_SATFINITE, __NV_E4M3);
-        return lo | hi << 16;
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const float2 a = mul2(make_float2(x[4 * i], x[4 * i + 1]), inverse), b = mul2(make_float2(x[4 * i + 2], x[4 * i + 3]), inverse);
+            packed[i] = (uint32_t)__nv_cvt_float2_to_fp8x2(a, __NV_SATFINITE, __NV_E4M3) | (uint32_t)__nv_cvt_float2_to_fp8x2(b, __NV_SATFINITE, __NV_E4M3) << 16;
+        }
     }
 }
 
 // Where a token goes: its row in the pools (in codes) and its place among the scales; -1: nowhere
 struct Place { long long k, v, ks, vs; };
-__device__ __forceinline__ Place place_of(const CodesParams &p, long long n, int &flags) {
+__device__ __forceinline__ Place place_of(const CodesParams &p, int slot, int &flags) {
     const kvc_rotary_args &a = p.a;
     Place r = {-1, -1, 0, 0};
-    const int slot = a.slots[n];
     if (slot < 0) return r;
     if (slot >= p.slots) { flags = KVC_FLAG_BAD_PAGE; return r; }
     const int page = kvc_divide(slot, p.page), row = slot - page * (int)a.page_size;
@@ -90,21 +124,30 @@ __device__ __forceinline__ Place place_of(const CodesParams &p, long long n, int
 }
 
 // Heads of 16 n channels, rotated by multiples of 16, everything on 16 bytes.  As for rows of 16 bits a thread has a unit of 16 channels (8 pairs) of up to CHUNK heads of a token, whose
-// angles it makes once; the lanes of a row are neighbours in a warp and find the row's largest value among them.
+// angles it makes once; the lanes of a row are neighbours in a warp and find the row's largest value among them.  A CTA has the same few heads of several tokens, the next one the next
+// heads of these: queries, which are bytes alone, and keys and values, which take instructions, run at the same time.
+// Measured: 16384 tokens of 40 + 10 + 10 heads of 128 channels in int8 (463 MB) 94 us, 5.0 TB/s, one kind behind the other and one head at a time 147; four or six CTAs per SM (the latter
+// spilling) 112, two heads of a thread 104, six 116.  e4m3, 4099 tokens of 32 + 8 + 8 heads (93 MB) 19 us.
 template <typename T, int KIND>
-__global__ void __launch_bounds__(CODES_THREADS, 3) codes_rows_kernel(const __grid_constant__ CodesParams p) {
+__global__ void __launch_bounds__(CODES_THREADS, CODES_CTAS) codes_rows_kernel(const __grid_constant__ CodesParams p) {
     kvc_behind();
     const kvc_rotary_args &a = p.a;
-    const int which = blockIdx.x >= p.parts[2].first ? 2 : (blockIdx.x >= p.parts[1].first ? 1 : 0);
+    const int of_tokens = kvc_divide((int)blockIdx.x, p.by_ctas), cta = (int)blockIdx.x - of_tokens * p.ctas;
+    const int which = cta >= (int)p.parts[2].first ? 2 : (cta >= (int)p.parts[1].first ? 1 : 0);
     const Part &part = p.parts[which];
-    const int turned = part.turned, id = (int)((blockIdx.x - part.first) * CODES_THREADS + threadIdx.x);
-    const int u = id & (p.lanes - 1), group = id / p.lanes, n = kvc_divide(group, part.chunks);       // (lanes: a power of two)
+    const int turned = part.turned, u = (int)threadIdx.x & (p.lanes - 1), n = of_tokens * p.tokens + (int)threadIdx.x / p.lanes;        // (lanes: a power of two)
     if (n >= a.N) return;
     const bool on = u < p.units;
-    const int h0 = (group - n * part.of_token) * part.chunk, heads = min(part.chunk, part.heads - h0);
+    const int h0 = (cta - (int)part.first) * part.chunk, heads = min(part.chunk, part.heads - h0);
     const bool half = a.layout == KVC_ROTARY_HALF && u < turned;
     const int c0 = half ? 8 * u : 16 * u, apart = half ? 8 * turned : 8;
     const T *src = reinterpret_cast<const T *>(part.src) + n * part.src_token + h0 * part.src_head + c0;
+    // everything is asked for before anything is waited for: place, position and frequencies one after the other took half of the time
+    const bool turns = u < turned;
+    const int slot = which > 0 ? a.slots[n] : 0, position = turns ? a.positions[n] : 0;
+    double2 f2[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) f2[k] = turns ? reinterpret_cast<const double2 *>(a.frequencies)[4 * u + k] : make_double2(0.0, 0.0);
     uint4 x[CHUNK][2];
 #pragma unroll
     for (int j = 0; j < CHUNK; j++) {
@@ -119,66 +162,86 @@ __global__ void __launch_bounds__(CODES_THREADS, 3) codes_rows_kernel(const __gr
     float *scale = nullptr;
     if (which > 0) {
         int flags = 0;
-        const Place at = place_of(p, n, flags);
+        const Place at = place_of(p, slot, flags);
         raise_flag(a.status, flags);
         if (at.k < 0) return;                               // (a token's lanes all go)
         dst = reinterpret_cast<uint8_t *>(part.dst) + (which == 1 ? at.k : at.v) + h0 * part.dst_head + c0;
         scale = which == 1 ? p.s.k + at.ks + h0 * p.s.k_head : p.s.v + at.vs + h0 * p.s.v_head;
     }
-    const bool turns = u < turned;
     float2 cs[8];
     if (turns) {
-        const double position = a.inverse ? -(double)a.positions[n] : (double)a.positions[n];
+        const double at = a.inverse ? -(double)position : (double)position;
 #pragma unroll
-        for (int k = 0; k < 8; k++) cs[k] = turn(position, a.frequencies[8 * u + k] * TURNS_OF_RADIANS, a.factor);
+        for (int k = 0; k < 8; k++) cs[k] = turn(at, (k & 1 ? f2[k / 2].y : f2[k / 2].x) * TURNS_OF_RADIANS, a.factor);
     }
     const unsigned row_lanes = (p.lanes == 32 ? 0xffffffffu : (1u << p.lanes) - 1) << (threadIdx.x & 31 & ~(p.lanes - 1));
+    auto values_of = [&](const uint4 (&v)[2], float (&f)[16]) {
+        const uint32_t w[8] = {v[0].x, v[0].y, v[0].z, v[0].w, v[1].x, v[1].y, v[1].z, v[1].w};
 #pragma unroll
-    for (int j = 0; j < CHUNK; j++) {
-        if (j < heads) {
-            const uint32_t w[8] = {x[j][0].x, x[j][0].y, x[j][0].z, x[j][0].w, x[j][1].x, x[j][1].y, x[j][1].z, x[j][1].w};
-            float f[16];
+        for (int m = 0; m < 8; m++) {
+            const float2 g = unpack(w[m], T());
+            f[2 * m] = g.x; f[2 * m + 1] = g.y;
+        }
+        if (!turns) return;
+        // pairs: with halves a value of the first piece and its like of the second, else neighbours
+        if (half) {
 #pragma unroll
             for (int m = 0; m < 8; m++) {
-                const float2 v = unpack(w[m], T());
-                f[2 * m] = v.x; f[2 * m + 1] = v.y;
+                const float f0 = f[m], f1 = f[8 + m];
+                f[m] = f0 * cs[m].x - f1 * cs[m].y;
+                f[8 + m] = f1 * cs[m].x + f0 * cs[m].y;
             }
-            if (turns) {
-                // pairs: with halves a value of the first piece and its like of the second, else neighbours
-if (half) {
+        } else {
 #pragma unroll
-                    for (int m = 0; m < 8; m++) {
-                        const float f0 = f[m], f1 = f[8 + m];
-                        f[m] = f0 * cs[m].x - f1 * cs[m].y;
-                        f[8 + m] = f1 * cs[m].x + f0 * cs[m].y;
-                    }
-                } else {
-#pragma unroll
-                    for (int m = 0; m < 8; m++) {
-                        const float f0 = f[2 * m], f1 = f[2 * m + 1];
-                        f[2 * m] = f0 * cs[m].x - f1 * cs[m].y;
-                        f[2 * m + 1] = f1 * cs[m].x + f0 * cs[m].y;
-                    }
-                }
+            for (int m = 0; m < 8; m++) {
+                const float f0 = f[2 * m], f1 = f[2 * m + 1];
+                f[2 * m] = f0 * cs[m].x - f1 * cs[m].y;
+                f[2 * m + 1] = f1 * cs[m].x + f0 * cs[m].y;
             }
-            if (which == 0) {
-                T *to = reinterpret_cast<T *>(part.dst) + n * part.dst_token + (h0 + j) * part.dst_head + c0;
-                if (on) {
-                    *reinterpret_cast<uint4 *>(to) = make_uint4(pack(f[0], f[1], T()), pack(f[2], f[3], T()), pack(f[4], f[5], T()), pack(f[6], f[7], T()));
-                    *reinterpret_cast<uint4 *>(to + apart) = make_uint4(pack(f[8], f[9], T()), pack(f[10], f[11], T()), pack(f[12], f[13], T()), pack(f[14], f[15], T()));
-                }
-                continue;
-            }
-            uint32_t top = 0;
+        }
+    };
+    if (which == 0) {
+        T *to = reinterpret_cast<T *>(part.dst) + n * part.dst_token + h0 * part.dst_head + c0;
 #pragma unroll
-            for (int m = 0; m < 16; m++) top = max(top, size_of(f[m]));
-            for (int o = p.lanes / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(row_lanes, top, o));
-            float inverse;
-            const float s = scale_of<KIND>(top, inverse);
-            if (on) {
-                *reinterpret_cast<uint2 *>(dst) = make_uint2(codes4<KIND>(f, s, inverse), codes4<KIND>(f + 4, s, inverse));
-                *reinterpret_cast<uint2 *>(dst + apart) = make_uint2(codes4<KIND>(f + 8, s, inverse), codes4<KIND>(f + 12, s, inverse));
-                if (u == 0) *scale = s;
+        for (int j = 0; j < CHUNK; j++) {
+            if (on && j < heads) {
+                float f[16];
+                values_of(x[j], f);
+                *reinterpret_cast<uint4 *>(to) = make_uint4(pack(f[0], f[1], T()), pack(f[2], f[3], T()), pack(f[4], f[5], T()), pack(f[6], f[7], T()));
+                *reinterpret_cast<uint4 *>(to + apart) = make_uint4(pack(f[8], f[9], T()), pack(f[10], f[11], T()), pack(f[12], f[13], T()), pack(f[14], f[15], T()));
+            }
+            to += part.dst_head;
+        }
+        return;
+    }
+    // Two heads at a time: the way from a row's values to its scale is a chain, and two take little more than one.
+#pragma unroll
+    for (int j = 0; j < CHUNK; j += 2) {
+        if (j >= heads) break;
+        float f[2][16], top[2] = {0.0f, 0.0f}, s[2], inverse[2];
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            values_of(x[j + i], f[i]);
+#pragma unroll
+            for (int m = 0; m < 8; m++) top[i] = largest(top[i], f[i][2 * m], f[i][2 * m + 1]);
+        }
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2) {
+            if (o >= p.lanes) break;
+            const float other[2] = {__shfl_xor_sync(row_lanes, top[0], o), __shfl_xor_sync(row_lanes, top[1], o)};
+            top[0] = larger(top[0], other[0]);
+            top[1] = larger(top[1], other[1]);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            s[i] = scale_of<KIND>(size_of(top[i]), inverse[i]);
+            if (on && j + i < heads) {
+                uint32_t c[4];
+                codes_of<KIND, 2>(f[i], s[i], inverse[i], c);
+                codes_of<KIND, 2>(f[i] + 8, s[i], inverse[i], c + 2);
+                *reinterpret_cast<uint2 *>(dst) = make_uint2(c[0], c[1]);
+                *reinterpret_cast<uint2 *>(dst + apart) = make_uint2(c[2], c[3]);
+                if (u == 0) *scale = s[i];
             }
             dst += part.dst_head;
             scale += which == 1 ? p.s.k_head : p.s.v_head;
@@ -206,7 +269,7 @@ __global__ void __launch_bounds__(CODES_THREADS) codes_any_kernel(const __grid_c
         const bool key = h < a.Hq + a.Hkv;
         const long long hk = h - a.Hq - (key ? 0 : a.Hkv);
         int flags = 0;
-        const Place at = place_of(p, n, flags);
+        const Place at = place_of(p, a.slots[n], flags);
         if (lane == 0) raise_flag(a.status, flags);
         if (at.k < 0) return;
         x = key ? reinterpret_cast<const T *>(a.k) + n * a.k_token + hk * a.k_head : reinterpret_cast<const T *>(a.v) + n * a.v_token + hk * a.v_head;
@@ -250,7 +313,9 @@ __global__ void __launch_bounds__(CODES_THREADS) codes_any_kernel(const __grid_c
     const float s = scale_of<KIND>(top, inverse);
     for (int i = lane; i < D; i += 32) {
         const float v[4] = {value(i), 0.0f, 0.0f, 0.0f};
-        dst[i] = (uint8_t)codes4<KIND>(v, s, inverse);
+        uint32_t c;
+        codes_of<KIND, 1>(v, s, inverse, &c);
+        dst[i] = (uint8_t)c;
     }
     if (lane == 0) *scale = s;
 }
@@ -385,31 +450,34 @@ extern "C" int kvc_rotary_store_codes(const kvc_rotary_args *args, const kvc_sca
         KVC_REQUIRE(!kvc_rows_overlap(written[i], k) && !kvc_rows_overlap(written[i], v) && (a.Hq == 0 || (!kvc_rows_overlap(written[i], q) && !kvc_rows_overlap(written[i], out))),
                     "kvc_rotary_store_codes: a pool overlaps what is read or the output");
     }
-    const uintptr_t at = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.q_out) | reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v);
+    const uintptr_t at = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.q_out) | reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) |
+                         (a.rotary ? reinterpret_cast<uintptr_t>(a.frequencies) : 0);
     const int64_t strides = a.q_token | a.q_head | a.k_token | a.k_head | a.v_token | a.v_head | a.out_token | a.out_head;
     cudaStream_t st = kvc_cu(stream);
     const bool fp16 = a.type == KVC_TYPE_FP16, whole = s.codes == KVC_CODES_INT8;
     p.units = (int)(a.D / 16);
     p.lanes = 1;
     while (p.lanes < p.units) p.lanes *= 2;
-    if ((at & 15) == 0 && (strides & 7) == 0 && a.rotary % 16 == 0 && p.lanes <= 32 && rows * p.lanes < (1ll << 31) - CODES_THREADS) {
+    if ((at & 15) == 0 && (strides & 7) == 0 && a.rotary % 16 == 0 && p.lanes <= 32) {
         p.parts[0] = {a.q, a.q_out, a.q_token, a.q_head, a.out_token, a.out_head, (int)a.Hq};
         p.parts[1] = {a.k, a.kpages, a.k_token, a.k_head, 0, a.kp_head, (int)a.Hkv};
         p.parts[2] = {a.v, a.vpages, a.v_token, a.v_head, 0, a.vp_head, (int)a.Hkv};
         // heads of a thread: CHUNK share its angles, unless that leaves too few threads for the device's latency
-        const long long threads = 3ll * CODES_THREADS * kvc_sm_count();
+        const long long threads = (long long)CODES_CTAS * CODES_THREADS * kvc_sm_count();
         const int chunk = (int)std::max<long long>(1, std::min<long long>(CHUNK, rows * p.lanes / threads));
-        int64_t grid = 0;
+        p.ctas = 0;
         for (int i = 0; i < 3; i++) {
             Part &part = p.parts[i];
-            const int chunks = std::max((part.heads + chunk - 1) / chunk, 1);
-            part.chunk = std::max((part.heads + chunks - 1) / chunks, 1);
-            part.of_token = chunks;
-            part.chunks = kvc_make_div((uint32_t)chunks);
+            const int chunks = (part.heads + chunk - 1) / chunk;
+            part.chunk = chunks > 0 ? (part.heads + chunks - 1) / chunks : 1;
             part.turned = i < 2 ? (int)a.rotary / 16 : 0;
-            part.first = (unsigned)grid;
-            if (part.heads > 0) grid += (a.N * chunks * p.lanes + CODES_THREADS - 1) / CODES_THREADS;
+            part.first = (unsigned)p.ctas;
+            p.ctas += chunks > 0 ? (part.heads + part.chunk - 1) / part.chunk : 0;
         }
+        p.by_ctas = kvc_make_div((uint32_t)p.ctas);
+        p.tokens = CODES_THREADS / p.lanes;
+        const long long grid = (a.N + p.tokens - 1) / p.tokens * p.ctas;
+        KVC_REQUIRE(grid < (1ll << 31), "kvc_rotary_store_codes: too many rows");
         auto *kernel = fp16 ? (whole ? codes_rows_kernel<__half, KVC_CODES_INT8> : codes_rows_kernel<__half, KVC_CODES_E4M3>)
                             : (whole ? codes_rows_kernel<__nv_bfloat16, KVC_CODES_INT8> : codes_rows_kernel<__nv_bfloat16, KVC_CODES_E4M3>);
         return kvc_launch_early(kernel, (unsigned)grid, CODES_THREADS, st, p);
