@@ -130,13 +130,16 @@ template <int KIND, int FIRST, int STEP> __device__ __forceinline__ uint32_t two
         const __half2 r = __hsub2(*reinterpret_cast<const __half2 *>(&v), __float2half2_rn(1152.0f));
         return *reinterpret_cast<const uint32_t *>(&r);
     } else {
-        uint32_t r;
-        const uint16_t v = (uint16_t)__byte_perm(c, 0, 0x4400 + FIRST + ((FIRST + STEP) << 4));
-        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(v));
+        uint32_t r;                                         // (c: as asked for, each pair in a half)
+        asm("{ .reg .b16 l, h; mov.b32 {l, h}, %1; cvt.rn.f16x2.e4m3x2 %0, " "l; }" : "=r"(r) : "r"((STEP == 1 ? FIRST : 2 * FIRST) == 0 ? c : c >> 16));
         return r;
     }
 }
-template <int KIND> __device__ __forceinline__ uint32_t offset_codes(uint32_t c) { return KIND == KVC_CODES_INT8 ? c ^ 0x80808080u : c; }
+// a register of codes as two_codes of that STEP wants it
+template <int KIND, int STEP> __device__ __forceinline__ uint32_t offset_codes(uint32_t c) {
+    if constexpr (KIND == KVC_CODES_INT8) return c ^ 0x80808080u;
+    return STEP == 1 ? c : __byte_perm(c, 0, 0x3120);
+}
 
 // The first of a request's rows of q and out, for b = B the first that is nobody's.  (Kept inside the tensors whatever `starts` hold, as lengths are.)
 template <bool ROWS> __device__ __forceinline__ int row_of(const Params &p, int b) { return ROWS && p.starts ? min(max(p.starts[b], 0), p.rows) : b; }
@@ -292,6 +295,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
     constexpr float LIFT = CODED ? Pair<__half>::LIFT : Pair<T>::LIFT, RESULT_LIFT = CODED ? 0.0f : LIFT;
     typedef std::conditional_t<CODED, uint8_t, T> Element;
     typedef std::conditional_t<CODED, Pair<__half>, Pair<T>> Operand;
+    constexpr int EVEN_MOST = CODED ? 10 : D < 128 ? 10 : 14;
     static_assert(!CODED || SAME, "pools of codes have the same strides");
     static_assert(STAGES + 2 <= DRAWN_SHARE - DRAWN_SHARE / 8, "a share is long enough for the first draw");
     extern __shared__ __align__(128) uint8_t smem[];        // [warp][stage]: 16 rows of keys, 16 of values
@@ -341,7 +345,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
             size -= size / 8;
             drawn_from = size * (int)gridDim.x;
         } else if (there <= gridDim.x) {
-            const int step = max(1, size / (CTAS > 1 ? 4 : 16)), most = CTAS > 1 ? size * (D < 128 ? 5 : 7) / 4 + 2 : size + 2 * step;
+            const int step = max(1, size / (CTAS > 1 ? 4 : 16)), most = CTAS > 1 ? size * EVEN_MOST / 8 + 2 : size + 2 * step;
 #pragma unroll 1
             for (int tiles = size; tiles <= most; tiles += step) {
                 even = __frcp_rn((float)tiles);
@@ -472,6 +476,29 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
                 }
                 const uint32_t to = ring + stage * STAGE;
                 constexpr int PIECES = ROW / 16, SIDE = PIECES > 4 ? 8 : 4;                 // 16-byte pieces of a row, lanes that take a row's
+                bool one_page = false;                      // (CODED) all of the tile's tokens are there and in one page: nobody has to be asked where his row is
+                if constexpr (CODED) {
+                    const int page0 = __shfl_sync(0xffffffffu, page, 0);
+                    one_page = __all_sync(0xffffffffu, page == page0) && mask == ALL;
+                    if (one_page) {
+                        const uint8_t *k = reinterpret_cast<const uint8_t *>(a.kpages) + page0 * a.kp_page + __shfl_sync(0xffffffffu, row, 0) * (int)a.kp_row + hk * (int)a.kp_head + lane / SIDE * (int)a.kp_row +
+                                           lane % SIDE * 16;
+                        const int step = 32 / SIDE * (int)a.kp_row;
+#pragma unroll
+                        for (int j = 0; j < TOKENS * SIDE / 32; j++) {
+#pragma unroll
+                            for (int c = 0; c < (PIECES + SIDE - 1) / SIDE; c++) {
+                                if (PIECES % SIDE == 0 || c * SIDE + lane % SIDE < PIECES) {
+                                    const uint32_t at = to + piece_at<ROW>(32 / SIDE * j + lane / SIDE, c * SIDE + lane % SIDE);
+                                    copy16(at, k + c * SIDE * 16, true);
+                                    copy16(at + HALF_STAGE, k + c * SIDE * 16 + p.v_less_k, true);
+                                }
+                            }
+                            k += step;
+                        }
+                    }
+                }
+                if (!one_page)
 #pragma unroll
                 for (int j = 0; j < TOKENS * SIDE / 32; j++) {
                     const int r = 32 / SIDE * j + lane / SIDE;
@@ -621,23 +648,31 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
                         ldmatrix4(f, from + half * 16 * ROW + key_at[k & 3] + (k >> 2) * 128);
 #pragma unroll
                         for (int j = 0; j < 2; j++) {
-                            const uint32_t c0 = offset_codes<KIND>(f[2 * j]), c1 = offset_codes<KIND>(f[2 * j + 1]);
+                            const uint32_t c0 = offset_codes<KIND, 1>(f[2 * j]), c1 = offset_codes<KIND, 1>(f[2 * j + 1]);
                             const uint32_t operand[4] = {two_codes<KIND, 0, 1>(c0), two_codes<KIND, 0, 1>(c1), two_codes<KIND, 2, 1>(c0), two_codes<KIND, 2, 1>(c1)};
 #pragma unroll
                             for (int nt = 0; nt < NT; nt++) Operand::mma(t[j][nt], operand, q[2 * k + j][nt][0], q[2 * k + j][nt][1]);
                         }
                     }
-                    const float k0 = scales[half * 16 + (lane >> 2)], k1 = scales[half * 16 + 8 + (lane >> 2)];
-                    const bool on0 = mask >> (half * 16 + (lane >> 2)) & 1, on1 = mask >> (half * 16 + 8 + (lane >> 2)) & 1;
+                    float k0 = scales[half * 16 + (lane >> 2)], k1 = scales[half * 16 + 8 + (lane >> 2)];
+                    if (p.negative) k0 = -k0, k1 = -k1;
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
-                            float v = (t[0][nt][e] + t[1][nt][e]) * (e < 2 ? k0 : k1);
-                            if constexpr (std::is_same_v<T, __nv_bfloat16>) v *= head_scale[nt][e & 1];
-                            if (p.negative) v = -v;
-                            s[half][nt][e] = (e < 2 ? on0 : on1) ? v : -CUDART_INF_F;
+                            s[half][nt][e] = (t[0][nt][e] + t[1][nt][e]) * (e < 2 ? k0 : k1);
+                            if constexpr (std::is_same_v<T, __nv_bfloat16>) s[half][nt][e] *= head_scale[nt][e & 1];
                         }
+                }
+                if (mask != ALL) {
+#pragma unroll
+                    for (int half = 0; half < 2; half++) {
+                        const bool on0 = mask >> (half * 16 + (lane >> 2)) & 1, on1 = mask >> (half * 16 + 8 + (lane >> 2)) & 1;
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) s[half][nt][e] = (e < 2 ? on0 : on1) ? s[half][nt][e] : -CUDART_INF_F;
+                    }
                 }
                 // the largest scale of these tokens' values (left out ones have 0)
                 const int top_here = min((int)__reduce_max_sync(0xffffffffu, __float_as_uint(scales[TOKENS + lane])) >> 23, 253);
@@ -700,7 +735,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
                         ldmatrix4_trans(f, from + half * 16 * ROW + value_at[k & 3] + (k >> 2) * 128);
 #pragma unroll
                         for (int j = 0; j < 2; j++) {       // rows of the operand: even channels, odd ones
-                            const uint32_t c0 = offset_codes<KIND>(f[2 * j]), c1 = offset_codes<KIND>(f[2 * j + 1]);
+                            const uint32_t c0 = offset_codes<KIND, 2>(f[2 * j]), c1 = offset_codes<KIND, 2>(f[2 * j + 1]);
                             const uint32_t operand[4] = {two_codes<KIND, 0, 2>(c0), two_codes<KIND, 1, 2>(c0), two_codes<KIND, 0, 2>(c1), two_codes<KIND, 1, 2>(c1)};
 #pragma unroll
                             for (int nt = 0; nt < NT; nt++) {
