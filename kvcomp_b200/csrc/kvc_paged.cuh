@@ -133,11 +133,8 @@ __device__ __forceinline__ uint32_t pack(float a, float b, __nv_bfloat16) { cons
 // turns keeps 2^-53 of the angle, 1e-10 at a million radians; fp32 would keep 0.06.  Of the rest the nearest quarter is taken off, and the series of sine and cosine on
 // [-pi / 4, pi / 4] are left, to x^9 and x^10: the first terms left out are below 2^-29 and 2^-33 (fp32's half step there: 2^-25).
 constexpr double TURNS_OF_RADIANS = 0.15915494309189533576888;
-__device__ __forceinline__ float2 turn(double position, double turns, float factor) {
-    double whole = position * turns;
-    whole -= rint(whole);
-    const float t = (float)whole, quarter = rintf(4.0f * t), x = fmaf(-0.25f, quarter, t) * 6.2831853071795865f, y = x * x;
-    const int q = (int)quarter;
+__device__ __forceinline__ float2 turn_by(float x, int q, float factor) {
+    const float y = x * x;
     float s = fmaf(y, 1.0f / 362880, -1.0f / 5040), c = fmaf(y, -1.0f / 3628800, 1.0f / 40320);
     s = fmaf(y, s, 1.0f / 120);
     c = fmaf(y, c, -1.0f / 720);
@@ -148,6 +145,20 @@ __device__ __forceinline__ float2 turn(double position, double turns, float fact
     c = fmaf(y, c, 1.0f);
     const float a = q & 1 ? s : c, b = q & 1 ? c : s;
     return make_float2(((q + 1) & 2 ? -a : a) * factor, (q & 2 ? -b : b) * factor);
+}
+__device__ __forceinline__ float2 turn(double position, double turns, float factor) {
+    double whole = position * turns;
+    whole -= rint(whole);
+    const float t = (float)whole, quarter = rintf(4.0f * t);
+    return turn_by(fmaf(-0.25f, quarter, t) * 6.2831853071795865f, (int)quarter, factor);
+}
+// The same with the rest of a quarter taken in fp64 too: it is off by 2^-26, not by pi 2^-25 (the turn's own rounding), and cos and sin by little more than their last bit.  For keys that are
+// coded next, of which what lies at the border of two codes is decided by that.
+__device__ __forceinline__ float2 turn_closely(double position, double turns, float factor) {
+    double whole = position * turns;
+    whole -= rint(whole);
+    const float quarter = rintf(4.0f * (float)whole);
+    return turn_by((float)((whole - 0.25 * (double)quarter) * 6.283185307179586476925), (int)quarter, factor);
 }
 
 // Queries, keys or values: a CTA has rows of one of them.  dst: token stride 0 for the pools, where `places` say where a token goes.

@@ -108,6 +108,35 @@ template <int KIND, int N> __device__ __forceinline__ void codes_of(const float 
     }
 }
 
+// NEAR at most: a value in 32 bits, off by some of its last bits, that may lie on the other side of a border between two e4m3.  (A scale is a power of two, and a border a number of five bits, the
+// last one 1; those between the smallest codes have fewer and are let be.)
+constexpr uint32_t NEAR = 12;
+__device__ __forceinline__ uint32_t to_border(float x) { return (__float_as_uint(x) - 0x80000u + NEAR / 2) & 0xfffff; }
+// Such a value rotated in 64 bits, cut to 24, the last one 1 where something was cut off: it rounds to fewer as the value itself does.
+__device__ __noinline__ float rotated_closely(double position, double frequency, float factor, float f0, float f1, bool second) {
+    double turns = position * (frequency * TURNS_OF_RADIANS), c, s;
+    turns -= rint(turns);
+    sincospi(2.0 * turns, &s, &c);
+    const double exact = (second ? f1 * c + f0 * s : f0 * c - f1 * s) * factor;
+    const float cut = __double2float_rz(exact);
+    return (double)cut == exact ? cut : __uint_as_float(__float_as_uint(cut) | 1);
+}
+// The codes of such values among a thread's 8 pairs.  One of 80000 values; without it some keys in a million get the code beside theirs.
+template <typename T> __device__ __noinline__ void code_again(const T *src, uint8_t *dst, int apart, bool half, double position, const double *frequencies, float factor, float inverse) {
+#pragma unroll 1
+    for (int k = 0; k < 8; k++) {
+        const int i0 = half ? k : 2 * k, i1 = half ? apart + k : 2 * k + 1;
+        const float f0 = to_float(src[i0]), f1 = to_float(src[i1]);
+        const float2 cs = turn_closely(position, frequencies[k] * TURNS_OF_RADIANS, factor);
+        const float y[2] = {f0 * cs.x - f1 * cs.y, f1 * cs.x + f0 * cs.y};
+        for (int second = 0; second < 2; second++) {
+            if (to_border(y[second]) > NEAR) continue;
+            const float cut = rotated_closely(position, frequencies[k], factor, f0, f1, second);
+            dst[second ? i1 : i0] = (uint8_t)__nv_cvt_float_to_fp8(cut * inverse, __NV_SATFINITE, __NV_E4M3);
+        }
+    }
+}
+
 // Where a token goes: its row in the pools (in codes) and its place among the scales; -1: nowhere
 struct Place { long long k, v, ks, vs; };
 __device__ __forceinline__ Place place_of(const CodesParams &p, int slot, int &flags) {
@@ -172,7 +201,7 @@ __global__ void __launch_bounds__(CODES_THREADS, CODES_CTAS) codes_rows_kernel(c
     if (turns) {
         const double at = a.inverse ? -(double)position : (double)position;
 #pragma unroll
-        for (int k = 0; k < 8; k++) cs[k] = turn(at, (k & 1 ? f2[k / 2].y : f2[k / 2].x) * TURNS_OF_RADIANS, a.factor);
+        for (int k = 0; k < 8; k++) cs[k] = turn_closely(at, (k & 1 ? f2[k / 2].y : f2[k / 2].x) * TURNS_OF_RADIANS, a.factor);
     }
     const unsigned row_lanes = (p.lanes == 32 ? 0xffffffffu : (1u << p.lanes) - 1) << (threadIdx.x & 31 & ~(p.lanes - 1));
     auto values_of = [&](const uint4 (&v)[2], float (&f)[16]) {
@@ -242,6 +271,14 @@ __global__ void __launch_bounds__(CODES_THREADS, CODES_CTAS) codes_rows_kernel(c
                 *reinterpret_cast<uint2 *>(dst) = make_uint2(c[0], c[1]);
                 *reinterpret_cast<uint2 *>(dst + apart) = make_uint2(c[2], c[3]);
                 if (u == 0) *scale = s[i];
+                if (KIND == KVC_CODES_E4M3 && turns) {
+                    uint32_t near = 0xffffffffu;
+#pragma unroll
+                    for (int m = 0; m < 16; m++) near = min(near, to_border(f[i][m]));
+                    if (near <= NEAR && position != 0)
+                        code_again<T>(reinterpret_cast<const T *>(part.src) + n * part.src_token + (h0 + j + i) * part.src_head + c0, dst, apart, half, a.inverse ? -(double)position : (double)position,
+                                      a.frequencies + 8 * u, a.factor, inverse[i]);
+                }
             }
             dst += part.dst_head;
             scale += which == 1 ? p.s.k_head : p.s.v_head;
@@ -288,9 +325,10 @@ __global__ void __launch_bounds__(CODES_THREADS) codes_any_kernel(const __grid_c
         int other;
         bool second;
         const int k = pair_of(i, other, second);
-        const float2 cs = turn(position, a.frequencies[k] * TURNS_OF_RADIANS, a.factor);
+        const float2 cs = turn_closely(position, a.frequencies[k] * TURNS_OF_RADIANS, a.factor);
         const float f0 = to_float(x[second ? other : i]), f1 = to_float(x[second ? i : other]);
-        return second ? f1 * cs.x + f0 * cs.y : f0 * cs.x - f1 * cs.y;
+        const float y = second ? f1 * cs.x + f0 * cs.y : f0 * cs.x - f1 * cs.y;
+        return KIND == KVC_CODES_E4M3 && to_border(y) <= NEAR ? rotated_closely(position, a.frequencies[k], a.factor, f0, f1, second) : y;
     };
     if (h < a.Hq) {                                         // (the result may lie where the query does: 32 channels and their partners are read before any is written)
         for (int i = lane; i < D; i += 32) {
@@ -299,7 +337,7 @@ __global__ void __launch_bounds__(CODES_THREADS) codes_any_kernel(const __grid_c
             bool second;
             const int k = pair_of(i, other, second);
             if (second) continue;
-            const float2 cs = turn(position, a.frequencies[k] * TURNS_OF_RADIANS, a.factor);
+            const float2 cs = turn_closely(position, a.frequencies[k] * TURNS_OF_RADIANS, a.factor);
             const float f0 = to_float(x[i]), f1 = to_float(x[other]);
             y[i] = from_float<T>(f0 * cs.x - f1 * cs.y);
             y[other] = from_float<T>(f1 * cs.x + f0 * cs.y);
