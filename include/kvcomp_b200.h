@@ -529,7 +529,7 @@ int kvc_paged_rows(const kvc_paged_rows_args *args, kvc_stream_t stream);
 int kvc_paged_attn_codes(const kvc_paged_attn_args *args, const kvc_scales *scales, const int32_t *starts, int64_t rows, kvc_stream_t stream);
 
 /* Requests that continue a common prefix.  parents[b] is the request whose first shared[b] tokens come before b's own (below 0: none); requests with the same two numbers are a group.  plan:
- * kvc_prefix_plan_words(B) words; it holds as long as parents and shared do.  Whoever is followed follows no one: what it follows is not seen by its followers (KVC_FLAG_BAD_LENGTH, as for a
+ * kvc_prefix_plan_words(B) words on 16 bytes; it holds as long as parents and shared do.  Whoever is followed follows no one: what it follows is not seen by its followers (KVC_FLAG_BAD_LENGTH, as for a
  * parent that is no request, or the request itself, and a negative length: none are followed then).  B is at most 16384. */
 typedef struct {
     const int32_t *parents, *shared;

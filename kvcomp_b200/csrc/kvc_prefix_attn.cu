@@ -30,16 +30,13 @@ constexpr int PREFIX_THREADS = 512, QUERY_LOADERS = 3, ROWS = 128, TOKENS = 128,
 constexpr int MASKS = 16;
 constexpr int MAX_REQUESTS = 16384;
 
-// places in a plan of B requests
-__host__ __device__ constexpr int64_t plan_first(int64_t) { return 1; }                    // groups' first members [B + 1]
-__host__ __device__ constexpr int64_t plan_parent(int64_t B) { return B + 2; }             // a group's prefix: whose it is, how long [B] each
-__host__ __device__ constexpr int64_t plan_shared(int64_t B) { return 2 * B + 2; }
-__host__ __device__ constexpr int64_t plan_order(int64_t B) { return 3 * B + 2; }          // members, group by group [B]
-__host__ __device__ constexpr int64_t plan_group(int64_t B) { return 4 * B + 2; }          // a request's group (-1: none) and its place there [B] each
-__host__ __device__ constexpr int64_t plan_rank(int64_t B) { return 5 * B + 2; }
-__host__ __device__ constexpr int64_t plan_leader(int64_t B) { return 6 * B + 2; }         // scratch: the first of those with the same prefix, their number [B] each
-__host__ __device__ constexpr int64_t plan_count(int64_t B) { return 7 * B + 2; }
-__host__ __device__ constexpr int64_t plan_words(int64_t B) { return 8 * B + 2; }
+// Places in a plan of B requests, in words: what is asked for together lies together.
+__host__ __device__ constexpr int64_t plan_groups(int64_t) { return 4; }                   // groups [B][4]: first member, members (0 behind the last group), whose prefix it is, how long
+__host__ __device__ constexpr int64_t plan_owners(int64_t B) { return 4 + 4 * B; }         // requests [B][2]: group (-1: none), place among its members
+__host__ __device__ constexpr int64_t plan_order(int64_t B) { return 4 + 6 * B; }          // members, group by group [B]
+__host__ __device__ constexpr int64_t plan_leader(int64_t B) { return 4 + 7 * B; }         // scratch: the first of those with the same prefix, their number [B] each
+__host__ __device__ constexpr int64_t plan_count(int64_t B) { return 4 + 8 * B; }
+__host__ __device__ constexpr int64_t plan_words(int64_t B) { return 4 + 9 * B; }          // (the first: groups)
 
 // ---- the plan: requests with the same prefix become a group ---------------------------------------------------------
 
@@ -77,7 +74,7 @@ __global__ void __launch_bounds__(FIND_THREADS) prefix_find_kernel(const __grid_
     }
     if (b < B) {
         a.plan[plan_leader(B) + b] = mine.parent < 0 ? -1 : leader;
-        a.plan[plan_rank(B) + b] = rank;
+        a.plan[plan_owners(B) + 2 * b + 1] = rank;
         a.plan[plan_count(B) + b] = count;
     }
     raise_flag(a.status, flags);
@@ -107,27 +104,23 @@ __global__ void __launch_bounds__(SCAN_THREADS) prefix_scan_kernel(const __grid_
         const int group = before.x + sum.x - leads, first = before.y + sum.y - count;
         if (leads) {
             const Wish w = wish_of(a, b, ignored);
-            a.plan[plan_first(B) + group] = first;
-            a.plan[plan_parent(B) + group] = w.parent;
-            a.plan[plan_shared(B) + group] = w.shared;
-            a.plan[plan_group(B) + b] = group;
+            int32_t *const to = a.plan + plan_groups(B) + 4 * group;
+            to[0] = first; to[1] = count; to[2] = w.parent; to[3] = w.shared;
+            a.plan[plan_owners(B) + 2 * b] = group;
         }
         __syncthreads();
         if (threadIdx.x == SCAN_THREADS - 1) before_s = make_int2(before.x + sum.x, before.y + sum.y);
         __syncthreads();
     }
-    const int2 all = before_s;
-    if (threadIdx.x == 0) {
-        a.plan[0] = all.x;
-        a.plan[plan_first(B) + all.x] = all.y;
-    }
-    __syncthreads();
+    const int groups = before_s.x;
+    if (threadIdx.x == 0) a.plan[0] = groups;
+    for (int i = 4 * groups + threadIdx.x; i < 4 * B; i += SCAN_THREADS) a.plan[plan_groups(B) + i] = 0;
     for (int b = threadIdx.x; b < B; b += SCAN_THREADS) {
         const int leader = a.plan[plan_leader(B) + b];
-        if (leader < 0) { a.plan[plan_group(B) + b] = -1; continue; }
-        const int group = a.plan[plan_group(B) + leader];                    // (written by this CTA ahead of a barrier)
-        if (leader != b) a.plan[plan_group(B) + b] = group;
-        a.plan[plan_order(B) + a.plan[plan_first(B) + group] + a.plan[plan_rank(B) + b]] = b;
+        if (leader < 0) { a.plan[plan_owners(B) + 2 * b] = -1; continue; }
+        const int group = a.plan[plan_owners(B) + 2 * leader];               // (written by this CTA ahead of a barrier)
+        if (leader != b) a.plan[plan_owners(B) + 2 * b] = group;
+        a.plan[plan_order(B) + a.plan[plan_groups(B) + 4 * group] + a.plan[plan_owners(B) + 2 * b + 1]] = b;
     }
 }
 
@@ -141,7 +134,7 @@ struct Prefix {
     unsigned n_pages;
     int negative;
     float log2_scaling;
-    int32_t *item_first, *share;                            // (workspace) the items' first tiles, and the tiles of a share
+    int4 *items;                                            // (workspace) the groups' first tiles, tiles of a column, rows of a KV head, tiles of a share
     float *own, *own_lse;                                   // (workspace) results of the requests' own tokens [request][query head][D], logarithms of their sums
     float *sums;                                            // (workspace) of places of D floats
     float2 *maxima;                                         // maximum and sum of weights of a place
@@ -161,14 +154,16 @@ __device__ __forceinline__ int row_of(const Prefix &p, int b) {
 }
 __device__ __forceinline__ int length_of(const Prefix &p, int b) { return min(max(p.a.lengths[b], 0), p.most_tokens); }
 
-struct Item { int table, first, rows, len, tiles, parts; };  // whose pages, the first member in the order, rows of a KV head, tokens, tiles of a column, columns of a KV head
+struct Item { int table, first, rows, len, tiles, parts; bool cut; };       // whose pages, the first member in the order, rows of a KV head, tokens, tiles of a column, columns of a KV head; fewer tokens than are shared
 __device__ __forceinline__ Item item_of(const Prefix &p, int i) {
     Item r;
     const int B = (int)p.a.B;
-    r.first = min(max(p.plan[plan_first(B) + i], 0), B);               // (kept inside the arrays whatever the plan holds, as lengths are)
-    r.rows = min(max(p.plan[plan_first(B) + i + 1] - r.first, 0), B - r.first) * p.g;
-    r.table = min(max(p.plan[plan_parent(B) + i], 0), B - 1);
-    r.len = r.rows == 0 ? 0 : min(max(p.plan[plan_shared(B) + i], 0), length_of(p, r.table));
+    const int4 group = *reinterpret_cast<const int4 *>(p.plan + plan_groups(B) + 4 * i);
+    r.first = min(max(group.x, 0), B);                      // (kept inside the arrays whatever the plan holds, as lengths are)
+    r.rows = min(max(group.y, 0), B - r.first) * p.g;
+    r.table = min(max(group.z, 0), B - 1);
+    r.len = r.rows == 0 ? 0 : min(max(group.w, 0), length_of(p, r.table));
+    r.cut = r.rows > 0 && r.len < group.w;
     r.tiles = (r.len + TOKENS - 1) / TOKENS;
     r.parts = (r.rows + 2 * ROWS - 1) / (2 * ROWS);
     return r;
@@ -362,12 +357,14 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_attn_kernel(const __
 
     // ---- this CTA's share
     kvc_behind();                                           // (from here on the kernel of the requests' own tokens, which reads nothing of this one's, may begin where there is room)
-    const int groups = min(max(p.plan[0], 0), B);
+    const int groups = min(max(p.plan[0], 0), B), looked_at = max(groups, min(B, PREFIX_THREADS));       // (those behind the last have no members: the first are looked at before their number is there)
     int flags = 0, total = 0;
     Item it = {};
     auto scan = [&](int i0, int &tiles) {                   // (first tile of item i0 + tid, its tiles; `total` grows)
         it.tiles = it.parts = 0;
-        if (i0 + tid < groups) it = item_of(p, i0 + tid);
+        it.cut = false;
+        if (i0 + tid < B) it = item_of(p, i0 + tid);
+        if (it.cut) flags |= KVC_FLAG_BAD_LENGTH;
         tiles = it.tiles * it.parts * (int)a.Hkv;
         int sum = tiles;
 #pragma unroll
@@ -386,22 +383,17 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_attn_kernel(const __
         return before + sum - tiles;
     };
     int tiles = 0, first = 0;
-    for (int i0 = 0; i0 < groups; i0 += PREFIX_THREADS) {
-        first = scan(i0, tiles);
-        if (blockIdx.x == 0 && i0 + tid < groups) p.item_first[i0 + tid] = first;
-    }
+    for (int i0 = 0; i0 < looked_at; i0 += PREFIX_THREADS) first = scan(i0, tiles);
     const int all = total, size = max(1, (all + p.grid - 1) / p.grid), r0 = (int)min((long long)all, (long long)size * blockIdx.x), r1 = min(all, r0 + size);
-    if (blockIdx.x == 0 && tid == 0) *p.share = size;
-    if (r0 < r1) {
+    if (r0 < r1 || blockIdx.x == 0) {                       // (of more groups than threads the first CTA and those with work look twice)
         if (groups > PREFIX_THREADS) total = 0;
         for (int i0 = 0; i0 < groups; i0 += PREFIX_THREADS) {
             if (groups > PREFIX_THREADS) first = scan(i0, tiles);
+            if (blockIdx.x == 0 && i0 + tid < groups) p.items[i0 + tid] = make_int4(first, it.tiles, it.rows, size);
             if (r0 >= first && r0 < first + tiles) { start_item = i0 + tid; start_rest = r0 - first; start_it = it; }
         }
     }
-    if (blockIdx.x == gridDim.x - 1)                        // prefixes that are longer than what there is
-        for (int i = tid; i < groups; i += PREFIX_THREADS)
-            if (item_of(p, i).len < p.plan[plan_shared(B) + i]) flags |= KVC_FLAG_BAD_LENGTH;
+    if (blockIdx.x > 0) flags = 0;                          // (one says it)
     before_sync();
     __syncthreads();
     after_sync();
@@ -740,17 +732,19 @@ __global__ void __launch_bounds__(128) prefix_join_kernel(const __grid_constant_
         for (int row = row_at(p, B); row < p.rows; row++) nothing(row);
         return;
     }
-    const int row = row_of(p, b);
-    if (row < 0) {
-        for (int i = row_at(p, b); i < row_at(p, b + 1); i++) nothing(i);
+    // (what does not wait for anything else is asked for together: the request's row and group, the result of its own tokens and the logarithm of their weights' sum)
+    const int2 owner = *reinterpret_cast<const int2 *>(p.plan + plan_owners(B) + 2 * b);
+    const int row = row_at(p, b), behind = p.starts ? row_at(p, b + 1) : b + 1, groups = min(p.plan[0], B);
+    const float own = __ldcg(p.own_lse + b * a.Hq + h);
+    float4 v = on ? __ldcg(reinterpret_cast<const float4 *>(p.own + (b * a.Hq + h) * D) + lane) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const int4 it = p.items[min(max(owner.x, 0), B - 1)];
+    if (behind - row != 1) {
+        for (int i = row; i < behind; i++) nothing(i);
         return;
     }
-    const int groups = min(max(p.plan[0], 0), B), group = min(p.plan[plan_group(B) + b], groups - 1), size = *p.share, k_head = kvc_divide(h, p.group);
-    // the request's own tokens: a result and the logarithm of its weights' sum
-    const float own = p.own_lse[b * a.Hq + h];
+    const int k_head = kvc_divide(h, p.group);
     float top = own * 1.4426950408889634f, sum = own == -CUDART_INF_F ? 0.0f : 1.0f;
-    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (on && own != -CUDART_INF_F) v = __ldcg(reinterpret_cast<const float4 *>(p.own + (b * a.Hq + h) * D) + lane);
+    if (own == -CUDART_INF_F) v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     auto add = [&](float2 ml, float4 x) {
         const float now = fmaxf(top, ml.x), less = now == -CUDART_INF_F ? 0.0f : now, f = exp2_approx(top - less), g = exp2_approx(ml.x - less);
         sum = sum * f + ml.y * g;
@@ -758,15 +752,15 @@ __global__ void __launch_bounds__(128) prefix_join_kernel(const __grid_constant_
         v.x = v.x * f + x.x * g; v.y = v.y * f + x.y * g; v.z = v.z * f + x.z * g; v.w = v.w * f + x.w * g;
         top = now;
     };
-    if (group >= 0) {
-        const Item it = item_of(p, group);
-        const int R = min(max(p.plan[plan_rank(B) + b], 0), it.rows / p.g - 1) * p.g + h - k_head * p.g, part = R / (2 * ROWS), in_part = R - part * 2 * ROWS;
-        const bool wide = it.rows - part * 2 * ROWS > ROWS;
-        const int from = p.item_first[group] + (k_head * it.parts + part) * it.tiles, to = from + it.tiles;
+    if (owner.x >= 0 && owner.x < groups && it.y > 0) {
+        const int size = max(it.w, 1), parts = (it.z + 2 * ROWS - 1) / (2 * ROWS);
+        const int R = min(max(owner.y, 0), it.z / p.g - 1) * p.g + h - k_head * p.g, part = R / (2 * ROWS), in_part = R - part * 2 * ROWS;
+        const bool wide = it.z - part * 2 * ROWS > ROWS;
+        const int from = it.x + (k_head * parts + part) * it.y, to = from + it.y;
         // a column's parts: each in a CTA's share, of narrow columns two (every other tile) where it has more than one
         const int cta0 = from / size, cta1 = (to - 1) / size, each = wide ? 1 : 2;
         constexpr int AT_ONCE = 8;
-        for (int k0 = 0; it.tiles > 0 && k0 < (cta1 - cta0 + 1) * each; k0 += AT_ONCE) {
+        for (int k0 = 0; k0 < (cta1 - cta0 + 1) * each; k0 += AT_ONCE) {
             float2 ml[AT_ONCE];
             float4 x[AT_ONCE];
 #pragma unroll
@@ -825,6 +819,7 @@ extern "C" int kvc_prefix_plan(const kvc_prefix_plan_args *args, kvc_stream_t st
     kvc_prefix_plan_args a;
     memcpy(&a, args, sizeof(a));
     KVC_REQUIRE(a.B >= 0 && a.B <= MAX_REQUESTS, "kvc_prefix_plan: %lld requests, %d at most", (long long)a.B, MAX_REQUESTS);
+    KVC_REQUIRE((reinterpret_cast<uintptr_t>(a.plan) & 15) == 0, "kvc_prefix_plan: the plan must be 16-byte aligned");
     KVC_REQUIRE(a.plan && (a.B == 0 || (a.parents && a.shared)), "kvc_prefix_plan: null pointer");
     cudaStream_t s = kvc_cu(stream);
     if (a.B > 0)
@@ -834,11 +829,12 @@ extern "C" int kvc_prefix_plan(const kvc_prefix_plan_args *args, kvc_stream_t st
 
 extern "C" int64_t kvc_paged_attn_shared_workspace(int64_t B, int64_t Hq, int64_t Hkv, int64_t D) {
     if (B < 0 || Hkv <= 0 || Hq < Hkv || D <= 0) return 0;
-    return own_bytes(Hq, Hkv, D) + rounded(4 * (B + 1)) + rounded(4 * B * Hq * (D + 1)) + prefix_places(B, Hq) * (4 * D + 8);
+    return own_bytes(Hq, Hkv, D) + rounded(16 * B) + rounded(4 * B * Hq * (D + 1)) + prefix_places(B, Hq) * (4 * D + 8);
 }
 
 extern "C" int kvc_paged_attn_shared(const kvc_paged_attn_args *args, const int32_t *plan, const int32_t *starts, int64_t rows, kvc_stream_t stream) {
     KVC_REQUIRE(args && plan, "kvc_paged_attn_shared: null pointer");
+    KVC_REQUIRE((reinterpret_cast<uintptr_t>(plan) & 15) == 0, "kvc_paged_attn_shared: the plan must be 16-byte aligned");
     Prefix p;
     memcpy(&p.a, args, sizeof(p.a));
     kvc_paged_attn_args &a = p.a;
@@ -883,9 +879,8 @@ extern "C" int kvc_paged_attn_shared(const kvc_paged_attn_args *args, const int3
     p.negative = a.scaling < 0.0f;
     p.log2_scaling = std::max(fabsf(a.scaling) * 1.4426950408889634f, 1e-37f) * (p.negative ? -1.0f : 1.0f);      // (0 times the infinite score of a token that is left out is none)
     uint8_t *at_ws = reinterpret_cast<uint8_t *>(a.workspace) + own_bytes(a.Hq, a.Hkv, a.D);
-    p.item_first = reinterpret_cast<int32_t *>(at_ws);
-    p.share = p.item_first + a.B;
-    at_ws += rounded(4 * (a.B + 1));
+    p.items = reinterpret_cast<int4 *>(at_ws);
+    at_ws += rounded(16 * a.B);
     p.own = reinterpret_cast<float *>(at_ws);
     p.own_lse = p.own + a.B * a.Hq * a.D;
     at_ws += rounded(4 * a.B * a.Hq * (a.D + 1));

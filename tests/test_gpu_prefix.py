@@ -27,9 +27,10 @@ def dev(a, dtype=torch.int32):
 def groups_of(plan):
     """{(parent, shared): members in order} and each request's (group, rank) of a plan."""
     w, B = plan.words.tolist(), plan.requests
-    n = w[0]
-    first, parent, shared, order = w[1:B + 2], w[B + 2:2 * B + 2], w[2 * B + 2:3 * B + 2], w[3 * B + 2:4 * B + 2]
-    return {(parent[i], shared[i]): order[first[i]:first[i + 1]] for i in range(n)}, list(zip(w[4 * B + 2:5 * B + 2], w[5 * B + 2:6 * B + 2]))
+    groups = [w[4 + 4 * i:8 + 4 * i] for i in range(B)]             # first member, members, parent, shared
+    assert all(g == [0] * 4 for g in groups[w[0]:])
+    owners, order = w[4 + 4 * B:4 + 6 * B], w[4 + 6 * B:4 + 7 * B]
+    return {(parent, shared): order[first:first + n] for first, n, parent, shared in groups[:w[0]]}, list(zip(owners[::2], owners[1::2]))
 
 
 @pytest.mark.parametrize("B,holders", [(1, 1), (2, 1), (40, 3), (257, 5), (1025, 1), (2100, 700)])
