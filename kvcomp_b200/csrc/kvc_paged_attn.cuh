@@ -285,6 +285,8 @@ template <int D, int KIND> struct Tiles {
 // Rows of codes: a warp's tile has 32 tokens, as many bytes as 16 of 16 bits.  A token's score is its codes' times its key's scale.  Its weight is multiplied with its value's scale before
 // it meets the codes; in fp16 that leaves no room, so the largest power of two among the scales seen is kept beside the sums as the maximum is, and taken out of them.  bf16 queries become fp16
 // times a power of two for each head (what is 2^29 below the head's largest value loses bits, no less than a sum in 32 bits does).
+// What bounds them is no longer HBM but instructions, about 980 for a tile of 32 tokens of 128 channels, a third of them codes that become numbers: 8 x 4096 tokens of 32 heads in int8 61 us (4.5 TB/s;
+// fp16 rows 85), 16 x 32768 of 8 KV heads in e4m3 207 (5.3 TB/s; 317).  So CTAs have equal work sooner than with rows of 16 bits: one CTA a column of 8 x 4096 took 82 us.
 template <typename T, int D, int NT, int WH, bool SAME, int STAGES, int CTAS, bool ROWS, int KIND>
 __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_constant__ Params p) {
     constexpr bool CODED = Tiles<D, KIND>::CODED;
@@ -314,8 +316,8 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
     // ---- this CTA's share
     // Whole parts of columns, one for each CTA, where parts of up to 7 / 4 of an equal share do (few columns): no CTA has two to finish then, and fewer are joined; so many
     // CTAs less still have as much under way as the memory gives (8 requests of 32 heads of 128 channels, one CTA a column: 512 tokens 15.7 us, 2048 45.6, 4096 85; in equal
-    // shares 19.6, 49.4, 90).  Tiles of shorter rows are less to have under way: 5 / 4 (11 x 4096 tokens of 32 heads of 96 channels 94 us, with 7 / 4 99); where an SM
-    // holds one CTA, 9 / 8.  Else equal shares of the row of all columns' tiles.
+    // shares 19.6, 49.4, 90).  Tiles of shorter rows are less to have under way: 5 / 4 (11 x 4096 tokens of 32 heads of 96 channels 94 us, with 7 / 4 99), and so
+    // do codes; where an SM holds one CTA, 9 / 8.  Else equal shares of the row of all columns' tiles.
     // Of long shares an eighth is drawn from a counter instead, in pieces of a sixteenth of a share, then halves of it: the SMs do not get the same out of the
     // memory (of 444 CTAs with 148 tiles each the first was done at 235 us, half at 285, the last at 319).  Where columns are few all of these pieces would be
     // joined by few CTAs, and a CTA alone on its SM pauses at the end of every piece: not there.

@@ -4,6 +4,8 @@
 namespace kvc_paged {
 namespace {
 
+// As for rows of 16 bits (a stage has twice the tokens and the same bytes, and their scales); 96 channels with a stage less, which three CTAs need to fit an SM.  Rows of 64 and 96 channels of two KV
+// heads are read together, as there.
 template <typename T, int D, int STAGES, int CTAS, int WIDE_STAGES, int WIDE_CTAS, int KIND>
 int choose_heads(Params &p, cudaStream_t s) {
     if constexpr (WIDE_STAGES > 0) {

@@ -156,7 +156,7 @@ __device__ __forceinline__ Place place_of(const CodesParams &p, int slot, int &f
 // angles it makes once; the lanes of a row are neighbours in a warp and find the row's largest value among them.  A CTA has the same few heads of several tokens, the next one the next
 // heads of these: queries, which are bytes alone, and keys and values, which take instructions, run at the same time.
 // Measured: 16384 tokens of 40 + 10 + 10 heads of 128 channels in int8 (463 MB) 94 us, 5.0 TB/s, one kind behind the other and one head at a time 147; four or six CTAs per SM (the latter
-// spilling) 112, two heads of a thread 104, six 116.  e4m3, 4099 tokens of 32 + 8 + 8 heads (93 MB) 19 us.
+// spilling) 112, two heads of a thread 104, six 116.  e4m3, 4099 tokens of 32 + 8 + 8 heads (93 MB) 22 us, 3 of them the second look at values next to a border.
 template <typename T, int KIND>
 __global__ void __launch_bounds__(CODES_THREADS, CODES_CTAS) codes_rows_kernel(const __grid_constant__ CodesParams p) {
     kvc_behind();
@@ -383,7 +383,8 @@ template <int KIND> __device__ __forceinline__ void values4(uint32_t c, float s,
     }
 }
 
-// A thread has 16 channels of up to CHUNK heads of a token, keys or values.  KIND 0: rows of 16 bits, copied.
+// A thread has 16 channels of up to CHUNK heads of a token, keys or values.  KIND 0: rows of 16 bits, copied.  HBM: 16 requests of up to 16384 tokens of 8 heads out of e4m3 (705 MB) 112 us, 6.3
+// TB/s (CTAs of 256 threads 125); 777 tokens of 32 heads 8 us, latency: slots, then codes and scales.
 template <typename T, int KIND>
 __global__ void __launch_bounds__(CODES_THREADS) paged_rows_kernel(const __grid_constant__ RowsParams p) {
     kvc_behind();

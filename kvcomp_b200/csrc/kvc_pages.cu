@@ -231,6 +231,7 @@ __global__ void __launch_bounds__(FILL_THREADS) release_rows_kernel(const __grid
         release_rows(p, (int)i, freed, p.a.free_pages + p.a.head_out[0]);
 }
 
+// The slots of all tokens that requests have, as a plan makes them for the new ones: a scan, and four rows a thread behind it.
 struct SlotsParams { kvc_page_slots_args a; kvc_div page; };
 
 // slots of rows [first, first + 4)

@@ -14,7 +14,13 @@
 //
 // Keys and values come by 16-byte asynchronous copies (pages end anywhere, any strides) into a ring in shared memory, in the 128-byte swizzled layout that the products read: keys
 // channel by channel, values as they lie (token by token: the product's second operand turned).  Rounding: the weights are fp16 (times 2^7: 2^-21 of the largest are still normal numbers) or bf16,
-// the sums of weights are taken before that; everything joined is 32 bits and the result is rounded once.
+// the sums of weights are taken before that; everything joined is 32 bits and the result is rounded once.  (Weights in 16 bits are off as the result's own rounding is: the error against 64 bits
+// is 1.35 times the plain form's, 2.3e-3 bf16, 2.8e-4 fp16.)
+//
+// Measured, device times of one B200: 64 requests of 32 heads behind 16384 tokens of 8 KV heads (256 rows a KV head), 1 to 500 own tokens each, 61 us: prefix 35, own tokens 23 (some of it beside the
+// prefix's end), joining 9.5.  Of the 35, 5 pass before the first tile's scores (lengths, pages, first bytes, one behind the other) and 4 with 19 MB of parts; a tile takes 4500 cycles, its
+// exponentials alone 2048, its products 2048.  8 times 16 requests of 40 heads behind 8000 tokens of 10 (64 rows a KV head) 133 us: prefix 62 (280 MB, 4.5 TB/s), own tokens 64, joining 9.5.  4
+// requests of 32 heads behind 777 tokens 16.6 us: three kernels' starts.
 #include <math_constants.h>
 #include <string.h>
 
