@@ -865,7 +865,7 @@ extern "C" int kvc_paged_attn_shared(const kvc_paged_attn_args *args, const int3
     if (a.n_pages <= 1) a.kp_page = a.vp_page = 0;
     const int64_t strides = a.q_token | a.q_head | a.out_token | a.out_head | a.kp_page | a.kp_row | a.kp_head | a.vp_page | a.vp_row | a.vp_head;
     KVC_REQUIRE((at & 15) == 0 && (strides & 7) == 0, "kvc_paged_attn_shared: rows must start on 16 bytes");
-    KVC_REQUIRE(a.workspace && (reinterpret_cast<uintptr_t>(a.workspace) & 15) == 0, "kvc_paged_attn_shared: the workspace must be 16-byte aligned");
+    KVC_REQUIRE(a.workspace && (reinterpret_cast<uintptr_t>(a.workspace) & 31) == 0, "kvc_paged_attn_shared: the workspace must be 32-byte aligned");         // (sums are written by whole sectors)
     if (a.workspace_bytes < kvc_paged_attn_shared_workspace(a.B, a.Hq, a.Hkv, a.D)) {
         kvc_set_error("kvc_paged_attn_shared: the workspace must hold what kvc_paged_attn_shared_workspace says");
         return KVC_ERR_CAPACITY;

@@ -374,3 +374,48 @@ def test_store_rows_and_attention_in_a_graph(ops):
         torch.cuda.synchronize()
         kept = [t.clone() for t in got]
         assert all(torch.equal(a, b) for a, b in zip(kept, step()))
+
+
+@pytest.mark.parametrize("codes", CODES)
+def test_long_offsets(ops, codes):
+    """Pages that lie behind 2^32 codes of the pool: stored, read back and attended."""
+    pages, page, Hkv, D = 36000, 64, 16, 128
+    kp, vp = (torch.zeros(pages, page, Hkv, D, dtype=torch.int8, device="cuda").view(codes_plain.TYPES[codes]) for _ in range(2))
+    ks, vs = (torch.zeros(pages, Hkv, page, device="cuda") for _ in range(2))
+    slots = dev(np.concatenate([35999 * page + np.arange(64), 7 * page + np.arange(40)]))
+    x = torch.randn(104, Hkv, D, device="cuda").half()
+    ops.rotary_paged_store(None, x, x, None, slots, None, kp, vp, kscales=ks, vscales=vs)
+    s = codes_plain.scale(x.double(), codes)
+    held = (codes_plain.code(x.double(), s, codes).float() * s.float()).half()
+    k, v = ops.paged_rows(kp, vp, slots, ks, vs, dtype=torch.float16)
+    assert torch.equal(k, held) and torch.equal(v, held)
+    q = torch.randn(1, Hkv, D, device="cuda").half()
+    out = ops.paged_attn(q, kp, vp, dev([[35999, 7]]), dev([104]), 0.1, kscales=ks, vscales=vs)
+    rows = codes_plain.code(x.double(), s, codes).float().double() * s
+    want = torch.einsum("ht,thd->hd", torch.softmax(0.1 * torch.einsum("hd,thd->ht", q[0].double(), rows), -1), rows)
+    assert bool(((out[0].double() - want).abs() <= 2.0 ** -10 * rows.abs().max()).all())
+
+
+def test_refusals(ops):
+    from kvcomp_b200._lib import KvcError
+    kp, vp, ks, vs = pools(4, 16, 2, 128, "int8")
+    x, i, q, table, lengths = torch.randn(3, 2, 128, device="cuda").half(), dev([0, 1, 2]), torch.randn(2, 4, 128, device="cuda").half(), dev([[0], [1]]), dev([3, 4])
+    store = dict(q=None, k=x, v=x, positions=None, slots=i, frequencies=None, kpages=kp, vpages=vp, kscales=ks, vscales=vs)
+    rows = dict(kpages=kp, vpages=vp, slots=i, kscales=ks, vscales=vs, dtype=torch.float16)
+    attn = dict(q=q, kpages=kp, vpages=vp, table=table, lengths=lengths, scaling=0.1, kscales=ks, vscales=vs)
+    ops.rotary_paged_store(**store), ops.paged_rows(**rows), ops.paged_attn(**attn)
+    both = [dict(kscales=None), dict(kscales=None, vscales=None), dict(kscales=ks.double()), dict(kscales=ks[:3]), dict(vscales=vs.transpose(1, 2)), dict(kscales=ks.cpu()), dict(vpages=vp.view(torch.float8_e4m3fn)),
+            dict(kpages=kp.half(), vpages=vp.half()), dict(kpages=kp[..., :120], vpages=vp[..., :120]), dict(vpages=vp[:2])]
+    for call, good, more in ((ops.rotary_paged_store, store, [dict(vscales=ks), dict(vpages=kp), dict(k=x.float()), dict(slots=i.long())]),
+                             (ops.paged_rows, rows, [dict(dtype=None), dict(dtype=torch.float32), dict(out=(x, x)), dict(out=(x, x[:1])), dict(slots=i[None])]),
+                             (ops.paged_attn, attn, [dict(kscales=torch.cat([ks, ks], 1)[:, :2]), dict(vpages=torch.cat([vp, vp], 2)[:, :, :2])])):
+        for change in both + more:
+            with pytest.raises(KvcError):
+                call(**{**good, **change})
+    with pytest.raises(KvcError):
+        ops.paged_rows(x[None].contiguous(), x[None].contiguous(), i, dtype=torch.bfloat16)          # (rows of 16 bits come as they are)
+    assert ops.paged_rows(kp, vp, i[:0], ks, vs, dtype=torch.float16)[0].shape == (0, 2, 128)
+    slots, starts = ops.page_slots(table[:0], lengths[:0], 16, 3)
+    assert slots.tolist() == [-1, -1, -1] and starts.tolist() == [0]
+    ops.page_shift(starts, lengths[:0], slots)
+    assert slots.tolist() == [-1, -1, -1]

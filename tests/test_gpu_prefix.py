@@ -218,3 +218,62 @@ def test_bad_pages_and_lengths(ops):
     status.zero_()
     out = ops.paged_attn_shared(q, kp, vp, dev([[0, 1], [2, 2], [3, 3]]), dev([20, 20, 3]), plan, 0.1, status=status, starts=dev([0, 0, 2, 3]))       # two rows of one request
     assert int(status.item()) == _lib.FLAG_BAD_LENGTH and not bool(out[:2].any()) and bool(out[2].any())
+
+
+def test_many_groups(ops):
+    """More groups than a CTA has threads, of one request each."""
+    attend(ops, [17] * 600, [1] * 600, [2, 0], 2, 1, 64, torch.bfloat16, page=8)
+
+
+def test_many_heads_of_one_request(ops):
+    """One follower with more query heads on a KV head than both sets have rows."""
+    attend(ops, [500], [1], [30], 300, 1, 64, torch.float16)
+    attend(ops, [500], [2], [30], 260, 2, 128, torch.bfloat16)
+
+
+def test_the_result_in_the_queries_place(ops):
+    kp, vp = (torch.randn(8, 16, 2, 128, device="cuda").half() for _ in range(2))
+    q, plan = torch.randn(3, 8, 128, device="cuda").half(), ops.prefix_plan(dev([-1, 0, 0]), dev([0, 40, 40]))
+    args = kp, vp, dev([[0, 1, 2], [3, 4, 5], [6, 7, 7]]), dev([40, 33, 1]), plan, 0.1
+    want = ops.paged_attn_shared(q, *args)
+    wide = torch.randn(3, 10, 128, device="cuda").half()
+    into = ops.paged_attn_shared(q, *args, out=wide[:, 1:9])
+    assert into.data_ptr() == wide[:, 1:9].data_ptr() and torch.equal(into, want)
+    assert torch.equal(ops.paged_attn_shared(q, *args, out=q), want) and torch.equal(q, want)
+
+
+def test_long_offsets(ops):
+    """Pages that lie behind 2^32 elements of the pool."""
+    pages, page, Hkv, D = 36000, 64, 16, 128
+    pool = torch.zeros(pages, page, Hkv, D, dtype=torch.float16, device="cuda")
+    table = np.array([[35999, 35000, 1, 35998], [35997, 2, 35996, 0], [3, 35995, 0, 0]])
+    for p in np.unique(table):
+        pool[int(p)] = torch.randn(page, Hkv, D, device="cuda").half()
+    q = torch.randn(3, 2 * Hkv, D, device="cuda").half()
+    plan = ops.prefix_plan(dev([-1, 0, 0]), dev([0, 250, 250]))
+    out = ops.paged_attn_shared(q, pool, pool, dev(table), dev([250, 200, 70]), plan, 0.1)
+    for b, own in ((1, 200), (2, 70)):
+        for h in (0, 31):
+            rows = torch.cat([torch.cat([pool[int(p), :, h // 2] for p in table[i]])[:n] for i, n in ((0, 250), (b, own))]).double()
+            want = torch.softmax(0.1 * (q[b, h].double() @ rows.T), -1) @ rows
+            assert bool(((out[b, h].double() - want).abs() <= 2.0 ** -9 * rows.abs().max()).all())
+
+
+def test_refusals(ops):
+    from kvcomp_b200._lib import KvcError
+    kp, vp = (torch.randn(4, 16, 2, 128, device="cuda").half() for _ in range(2))
+    q, table, lengths, plan = torch.randn(2, 4, 128, device="cuda").half(), dev([[0], [1]]), dev([3, 4]), ops.prefix_plan(dev([-1, 0]), dev([0, 3]))
+    good = dict(q=q, kpages=kp, vpages=vp, table=table, lengths=lengths, plan=plan, scaling=0.1)
+    workspace = ops.paged_attn_shared_workspace(2, 4, 2, 128, "cuda")
+    ops.paged_attn_shared(**good, workspace=workspace)
+    odd = torch.empty(workspace.numel() + 16, dtype=torch.uint8, device="cuda")[16:]
+    bad_pool = torch.randn(4, 16, 2, 256, device="cuda").half()
+    for change in (dict(plan=ops.prefix_plan(dev([-1]), dev([0]))), dict(plan=None), dict(plan=ops.PrefixPlan(plan.words.cpu(), 2)), dict(lengths=lengths[:1]), dict(table=table.long()), dict(kpages=kp.float()),
+                   dict(q=q.bfloat16()), dict(workspace=workspace[:-32]), dict(workspace=odd), dict(q=torch.randn(2, 4, 256, device="cuda").half(), kpages=bad_pool, vpages=bad_pool), dict(starts=dev([0, 1])),
+                   dict(out=torch.empty(2, 4, 64, device="cuda").half()), dict(out=q.expand(2, 4, 128).as_strided((2, 4, 128), (128, 128, 1)))):
+        with pytest.raises(KvcError):
+            ops.paged_attn_shared(**{**good, **change})
+    for parents, shared in ((dev([0]), dev([0, 1])), (dev([0]).long(), dev([0])), (dev([0]), dev([0]).cpu())):
+        with pytest.raises(KvcError):
+            ops.prefix_plan(parents, shared)
+    assert ops.paged_attn_shared(q[:0], kp, vp, table[:0], lengths[:0], ops.prefix_plan(dev([]), dev([])), 0.1).shape == (0, 4, 128)
