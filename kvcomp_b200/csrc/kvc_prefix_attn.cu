@@ -20,7 +20,8 @@
 // Measured, device times of one B200: 64 requests of 32 heads behind 16384 tokens of 8 KV heads (256 rows a KV head), 1 to 500 own tokens each, 61 us: prefix 35, own tokens 23 (some of it beside the
 // prefix's end), joining 9.5.  Of the 35, 5 pass before the first tile's scores (lengths, pages, first bytes, one behind the other) and 4 with 19 MB of parts; a tile takes 4500 cycles, its
 // exponentials alone 2048, its products 2048.  8 times 16 requests of 40 heads behind 8000 tokens of 10 (64 rows a KV head) 133 us: prefix 62 (280 MB, 4.5 TB/s), own tokens 64, joining 9.5.  4
-// requests of 32 heads behind 777 tokens 16.6 us: three kernels' starts.
+// requests of 32 heads behind 777 tokens 16.6 us: three kernels' starts.  (Joined where the own tokens' columns end, without a third kernel: 78, 155 and 18.5 us: few threads read many
+// parts then, and hold what others need meanwhile.)
 #include <math_constants.h>
 #include <string.h>
 
