@@ -391,7 +391,7 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_attn_kernel(const __
     };
     int tiles = 0, first = 0;
     for (int i0 = 0; i0 < looked_at; i0 += PREFIX_THREADS) first = scan(i0, tiles);
-    const int all = total, size = max(1, (all + p.grid - 1) / p.grid), r0 = (int)min((long long)all, (long long)size * blockIdx.x), r1 = min(all, r0 + size);
+    const int all = total, size = max(1, (all + p.grid - 1) / p.grid), r0 = (int)min((long long)all, (long long)size * blockIdx.x), r1 = r0 + min(size, all - r0);
     if (r0 < r1 || blockIdx.x == 0) {                       // (of more groups than threads the first CTA and those with work look twice)
         if (groups > PREFIX_THREADS) total = 0;
         for (int i0 = 0; i0 < groups; i0 += PREFIX_THREADS) {
@@ -856,7 +856,7 @@ extern "C" int kvc_paged_attn_shared(const kvc_paged_attn_args *args, const int3
     if (rows == 0) return KVC_OK;
     KVC_REQUIRE(a.q && a.out && a.lengths && (a.table || a.table_width == 0) && ((a.kpages && a.vpages) || a.n_pages == 0), "kvc_paged_attn_shared: null pointer");
     const int64_t g = a.Hq / a.Hkv, most_tiles = (a.table_width * a.page_size + TOKENS - 1) / TOKENS;
-    KVC_REQUIRE(a.Hkv * (2 * a.B + a.B * g / (2 * ROWS)) < (1ll << 31) / std::max<int64_t>(most_tiles, 1), "kvc_paged_attn_shared: requests, KV heads and table rows of more than 2^31 tiles");
+    KVC_REQUIRE(a.Hkv * (2 * a.B + a.B * g / (2 * ROWS)) < (1ll << 30) / std::max<int64_t>(most_tiles, 1), "kvc_paged_attn_shared: requests, KV heads and table rows of more than 2^30 tiles");
     KVC_REQUIRE(a.B * columns_of(a.Hq, a.Hkv, a.D) * ((a.table_width * a.page_size + 31) / 32) < (1ll << 31) - (1 << 20), "kvc_paged_attn_shared: requests, KV heads and table rows of more than 2^31 tiles");
     const uintptr_t at = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.kpages) | reinterpret_cast<uintptr_t>(a.vpages) | reinterpret_cast<uintptr_t>(a.out);
     if (a.Hq == 1) a.q_head = a.out_head = 0;              // (the stride of a dimension of one may be anything)
