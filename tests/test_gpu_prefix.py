@@ -194,6 +194,15 @@ def test_long_prefixes(ops, dtype):
     attend(ops, [9000], [40], [100, 300, 0], 8, 1, 64, dtype, page=64)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("prefix", [128, 500, 640, 5000, 20001])
+def test_few_rows_behind_long_prefixes(ops, prefix, dtype):
+    """Few rows, whose columns are cut into one to more than a hundred parts: these are joined by four warps a head, from some number of rows on by one."""
+    attend(ops, [prefix, prefix // 2], [3, 1], [25, 0, 7], 14, 2, 128, dtype, page=24)
+    attend(ops, [prefix], [2], [0], 36, 1, 64, dtype, page=24)
+    attend(ops, [prefix], [2], [3], 38, 1, 96, dtype, page=24, sharp=20.0)
+
+
 def test_many_requests(ops):
     """More items than a CTA looks at at once."""
     attend(ops, [200] * 5, [90] * 5, [1, 0, 3], 2, 1, 64, torch.float16, page=8)
