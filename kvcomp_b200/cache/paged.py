@@ -14,7 +14,7 @@ tokens come before theirs, and attend reads them once for all.
 Everything is launched and nothing waited for or asked of the device: a step of at most one token per request can be captured into a CUDA graph and
 replayed, with the lengths, the tables and the free list going on from replay to replay (new[b] may be 0 in any of them); nothing has to be called
 before it.  append and attend go by the last begin, captured or not.  Layers may be attended on streams of their own: each keeps a workspace of 15
-to 45 MB (with followers 30 to 100), and so does each graph.  Streams are ordered by the caller: begin and release change what the attention reads, and may run only behind all
+to 45 MB (with followers 30 to 100), and so does each graph.  Streams are ordered by the caller: begin, follow and release change what the attention reads, and may run only behind all
 of it (Stream.wait_stream).  (The prompt's own attention is the model's: its keys and values are in hand there.)  No gradient goes through a cache;
 tensors that a call writes are known to autograd as changed."""
 import math
