@@ -94,6 +94,7 @@ __global__ void __launch_bounds__(SCAN_THREADS) prefix_scan_kernel(const __grid_
     const int B = (int)a.B, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int ignored = 0;
     if (threadIdx.x == 0) before_s = make_int2(0, 0);
+    __syncthreads();                                        // (of no requests the loop, and its barriers, are left out)
     for (int b0 = 0; b0 < B; b0 += SCAN_THREADS) {
         const int b = b0 + threadIdx.x;
         const bool leads = b < B && a.plan[plan_leader(B) + b] == b;

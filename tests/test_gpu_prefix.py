@@ -64,6 +64,18 @@ def test_plan_of_bad_parents(ops):
         assert got == want and int(status.item()) == _lib.FLAG_BAD_LENGTH
 
 
+def test_a_plan_of_no_requests(ops):
+    """It says so, and touches nothing around it, whatever the kernels ahead of it left in shared memory."""
+    all_words = torch.full((1 << 16,), 7, dtype=torch.int32, device="cuda")
+    plan = ops.PrefixPlan(all_words[1 << 15:(1 << 15) + 4], 0)
+    want = all_words.clone()
+    want[1 << 15] = 0
+    for i in range(50):
+        torch.sort(torch.full((1 << 14,), -1 - i, dtype=torch.int32, device="cuda"))
+        plan.words[0] = 7
+        assert ops.prefix_plan(dev([]), dev([]), out=plan) is plan and torch.equal(all_words, want)
+
+
 def attend(ops, prefixes, members, own, Hq, Hkv, D, dtype, page=16, seed=0, sharp=1.0, scaling=None, order="token", rows="followers", shares=None, alone=0):
     """prefixes[i] tokens that members[i] requests follow, own tokens of each request from `own` in turn; `alone` requests follow no one."""
     rng = np.random.RandomState(seed + sum(prefixes) + page)
