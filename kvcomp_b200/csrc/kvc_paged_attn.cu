@@ -58,24 +58,13 @@ static int paged_attn(const kvc_paged_attn_args *args, const kvc_scales *scales,
     if (rows == 0) return KVC_OK;
     KVC_REQUIRE(a.B < (1 << 24), "kvc_paged_attn: %lld requests", (long long)a.B);
     KVC_REQUIRE(a.q && a.out && a.lengths && (a.table || a.table_width == 0) && ((a.kpages && a.vpages) || a.n_pages == 0), "kvc_paged_attn: null pointer");
-    const uintptr_t at = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.kpages) | reinterpret_cast<uintptr_t>(a.vpages) | reinterpret_cast<uintptr_t>(a.out);
-    if (a.Hq == 1) a.q_head = a.out_head = 0;              // (the stride of a dimension of one may be anything)
-    if (rows == 1) a.q_token = a.out_token = 0;
-    if (a.Hkv == 1) a.kp_head = a.vp_head = 0;
-    if (a.page_size == 1) a.kp_row = a.vp_row = 0;
-    if (a.n_pages <= 1) a.kp_page = a.vp_page = 0;
-    const int64_t strides = a.q_token | a.q_head | a.out_token | a.out_head, of_pools = a.kp_page | a.kp_row | a.kp_head | a.vp_page | a.vp_row | a.vp_head;
-    KVC_REQUIRE((at & 15) == 0 && (strides & 7) == 0 && (of_pools & (scales ? 15 : 7)) == 0, "kvc_paged_attn: rows must start on 16 bytes");
-    KVC_REQUIRE(a.kp_row >= 0 && a.kp_head >= 0 && a.vp_row >= 0 && a.vp_head >= 0 && a.kp_page >= 0 && a.vp_page >= 0 && a.kp_row * (a.page_size - 1) + a.kp_head * (a.Hkv - 1) < (1ll << 31) &&
-                    a.vp_row * (a.page_size - 1) + a.vp_head * (a.Hkv - 1) < (1ll << 31), "kvc_paged_attn: a page spans more than 2^31 elements");
+    if (int rc = check_rows(a, rows, scales ? 16 : 8, "kvc_paged_attn")) return rc;
     KVC_REQUIRE(a.workspace && (reinterpret_cast<uintptr_t>(a.workspace) & 15) == 0, "kvc_paged_attn: the workspace must be 16-byte aligned");
     if (a.workspace_bytes < kvc_paged_attn_workspace(a.B, a.Hq, a.Hkv, a.D)) {
         kvc_set_error("kvc_paged_attn: the workspace must hold what kvc_paged_attn_workspace says");
         return KVC_ERR_CAPACITY;
     }
-    const kvc_rows q = kvc_make_rows(a.q, a.D, rows, a.q_token, a.Hq, a.q_head), out = kvc_make_rows(a.out, a.D, rows, a.out_token, a.Hq, a.out_head);
-    KVC_REQUIRE(out.apart, "kvc_paged_attn: rows of the output overlap");
-    KVC_REQUIRE(kvc_rows_equal(q, out) || !kvc_rows_overlap(q, out), "kvc_paged_attn: the output overlaps the queries and is not them");
+    if (int rc = check_results(a, rows, "kvc_paged_attn")) return rc;
     Params p = {};
     set_params(p, a, starts, rows);
     cudaStream_t s = kvc_cu(stream);

@@ -1095,6 +1095,31 @@ inline int64_t part_floats(int64_t group, int64_t D) { return (std::max<int64_t>
 // front, the same for calls of all shapes: a workspace may serve one after the other.
 inline int64_t counter_bytes() { return 256 + (2 * places(64) * 4 + 255) / 256 * 256; }
 
+// Strides and places of rows, asked alike by all entries (name: which): rows start on 16 bytes, those of pools on `elements`, and a row's place in its page is a number of 32 bits.  The
+// stride of a dimension of one may be anything, and becomes 0.
+inline int check_rows(kvc_paged_attn_args &a, int64_t rows, int64_t elements, const char *name) {
+    if (a.Hq == 1) a.q_head = a.out_head = 0;
+    if (rows == 1) a.q_token = a.out_token = 0;
+    if (a.Hkv == 1) a.kp_head = a.vp_head = 0;
+    if (a.page_size == 1) a.kp_row = a.vp_row = 0;
+    if (a.n_pages <= 1) a.kp_page = a.vp_page = 0;
+    const uintptr_t at = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.kpages) | reinterpret_cast<uintptr_t>(a.vpages) | reinterpret_cast<uintptr_t>(a.out);
+    const int64_t strides = a.q_token | a.q_head | a.out_token | a.out_head, of_pools = a.kp_page | a.kp_row | a.kp_head | a.vp_page | a.vp_row | a.vp_head;
+    KVC_REQUIRE((at & 15) == 0 && (strides & 7) == 0 && (of_pools & (elements - 1)) == 0, "%s: rows must start on 16 bytes", name);
+    const int64_t last = a.page_size - 1, head = a.Hkv - 1, most = 1ll << 31;              // (each product by itself first: their sum is one of 64 bits then)
+    KVC_REQUIRE(a.kp_row >= 0 && a.kp_head >= 0 && a.vp_row >= 0 && a.vp_head >= 0 && a.kp_page >= 0 && a.vp_page >= 0, "%s: the pools have a negative stride", name);
+    KVC_REQUIRE(a.kp_row < most && a.kp_head < most && a.vp_row < most && a.vp_head < most && a.kp_row * last + a.kp_head * head < most && a.vp_row * last + a.vp_head * head < most,
+                "%s: a page spans more than 2^31 elements", name);
+    return KVC_OK;
+}
+// Results overlap neither one another nor queries that they are not.
+inline int check_results(const kvc_paged_attn_args &a, int64_t rows, const char *name) {
+    const kvc_rows q = kvc_make_rows(a.q, a.D, rows, a.q_token, a.Hq, a.q_head), out = kvc_make_rows(a.out, a.D, rows, a.out_token, a.Hq, a.out_head);
+    KVC_REQUIRE(out.apart, "%s: rows of the output overlap", name);
+    KVC_REQUIRE(kvc_rows_equal(q, out) || !kvc_rows_overlap(q, out), "%s: the output overlaps the queries and is not them", name);
+    return KVC_OK;
+}
+
 // What a call's arguments say, for a kernel: sizes have been checked.
 inline void set_params(Params &p, const kvc_paged_attn_args &a, const int32_t *starts, int64_t rows) {
     p.a = a;

@@ -31,7 +31,7 @@
 
 namespace {
 
-using kvc_paged::Params, kvc_paged::set_params, kvc_paged::launch_wide, kvc_paged::counter_bytes, kvc_paged::places, kvc_paged::group_of, kvc_paged::part_floats, kvc_paged::columns_of;
+using kvc_paged::Params, kvc_paged::set_params, kvc_paged::launch_wide, kvc_paged::counter_bytes, kvc_paged::places, kvc_paged::group_of, kvc_paged::part_floats, kvc_paged::columns_of, kvc_paged::check_rows, kvc_paged::check_results;
 
 constexpr int PREFIX_THREADS = 512, QUERY_LOADERS = 3, ROWS = 128, TOKENS = 128, ATOM = 16384;       // ATOM: 128 rows of 128 bytes
 constexpr int MASKS = 16;
@@ -879,22 +879,13 @@ extern "C" int kvc_paged_attn_shared(const kvc_paged_attn_args *args, const int3
     const int64_t g = a.Hq / a.Hkv, most_tiles = (a.table_width * a.page_size + TOKENS - 1) / TOKENS;
     KVC_REQUIRE(a.Hkv * (2 * a.B + a.B * g / (2 * ROWS)) < (1ll << 30) / std::max<int64_t>(most_tiles, 1), "kvc_paged_attn_shared: requests, KV heads and table rows of more than 2^30 tiles");
     KVC_REQUIRE(a.B * columns_of(a.Hq, a.Hkv, a.D) * ((a.table_width * a.page_size + 31) / 32) < (1ll << 31) - (1 << 20), "kvc_paged_attn_shared: requests, KV heads and table rows of more than 2^31 tiles");
-    const uintptr_t at = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.kpages) | reinterpret_cast<uintptr_t>(a.vpages) | reinterpret_cast<uintptr_t>(a.out);
-    if (a.Hq == 1) a.q_head = a.out_head = 0;              // (the stride of a dimension of one may be anything)
-    if (rows == 1) a.q_token = a.out_token = 0;
-    if (a.Hkv == 1) a.kp_head = a.vp_head = 0;
-    if (a.page_size == 1) a.kp_row = a.vp_row = 0;
-    if (a.n_pages <= 1) a.kp_page = a.vp_page = 0;
-    const int64_t strides = a.q_token | a.q_head | a.out_token | a.out_head | a.kp_page | a.kp_row | a.kp_head | a.vp_page | a.vp_row | a.vp_head;
-    KVC_REQUIRE((at & 15) == 0 && (strides & 7) == 0, "kvc_paged_attn_shared: rows must start on 16 bytes");
+    if (int rc = check_rows(a, rows, 8, "kvc_paged_attn_shared")) return rc;              // (the kernel for own tokens goes by them too)
     KVC_REQUIRE(a.workspace && (reinterpret_cast<uintptr_t>(a.workspace) & 31) == 0, "kvc_paged_attn_shared: the workspace must be 32-byte aligned");         // (sums are written by whole sectors)
     if (a.workspace_bytes < kvc_paged_attn_shared_workspace(a.B, a.Hq, a.Hkv, a.D)) {
         kvc_set_error("kvc_paged_attn_shared: the workspace must hold what kvc_paged_attn_shared_workspace says");
         return KVC_ERR_CAPACITY;
     }
-    const kvc_rows q = kvc_make_rows(a.q, a.D, rows, a.q_token, a.Hq, a.q_head), out = kvc_make_rows(a.out, a.D, rows, a.out_token, a.Hq, a.out_head);
-    KVC_REQUIRE(out.apart, "kvc_paged_attn_shared: rows of the output overlap");
-    KVC_REQUIRE(kvc_rows_equal(q, out) || !kvc_rows_overlap(q, out), "kvc_paged_attn_shared: the output overlaps the queries and is not them");
+    if (int rc = check_results(a, rows, "kvc_paged_attn_shared")) return rc;
     p.plan = plan;
     p.starts = starts;
     p.page = kvc_make_div((uint32_t)a.page_size);

@@ -38,6 +38,18 @@ def test_refusals(change):
     assert attn(**change) == 1 and b"kvc_paged_attn_shared" in _lib.load().kvc_last_error()
 
 
+@pytest.mark.parametrize("change", [dict(kp_head=1 << 31), dict(vp_head=1 << 31), dict(kp_head=1 << 32), dict(kp_row=1 << 28), dict(vp_row=1 << 28), dict(page_size=1 << 20, kp_row=1 << 12, kp_head=128),
+                                    dict(page_size=1 << 20, vp_row=1 << 12, vp_head=128), dict(kp_row=1 << 62), dict(vp_head=1 << 62), dict(kp_row=-256), dict(vp_row=-256), dict(kp_head=-128), dict(vp_head=-128),
+                                    dict(kp_page=-4096), dict(vp_page=-4096)], ids=str)
+@pytest.mark.parametrize("call", ["kvc_paged_attn_shared", "kvc_paged_attn", "kvc_paged_attn_rows"])
+def test_pages_that_reach_too_far(call, change):
+    """A row's place in its page is a number of 32 bits, for the requests' own tokens as in calls without prefixes."""
+    values = dict(good("kvc_paged_attn"), out=2 * AT, **change)
+    packed, lib = _lib.PAGED_ATTN_ARGS.pack(*(values[n] for n, _ in _header_fields("kvc_paged_attn_args"))), _lib.load()
+    rc = lib.kvc_paged_attn_shared(packed, AT, None, 0, None) if call.endswith("shared") else lib.kvc_paged_attn(packed, None) if call == "kvc_paged_attn" else lib.kvc_paged_attn_rows(packed, AT, 4, None)
+    assert rc == 1 and call.replace("_rows", "").encode() in lib.kvc_last_error()
+
+
 def test_workspaces_and_nothing_to_do():
     lib = _lib.load()
     need = lib.kvc_paged_attn_shared_workspace(4, 8, 2, 128)
