@@ -135,6 +135,10 @@ template <int KIND, int FIRST, int STEP> __device__ __forceinline__ uint32_t two
         return r;
     }
 }
+// the power of two that brings x to [2^14, 2^15), or a smaller one where there is none, and one over it
+__device__ __forceinline__ uint32_t exponent_of(float x) { return min(max(__float_as_uint(x) >> 23, 15u), 254u); }
+__device__ __forceinline__ float lifted(float x) { return __uint_as_float((268 - exponent_of(x)) << 23); }
+__device__ __forceinline__ float lifted_back(float x) { return __uint_as_float((exponent_of(x) - 14) << 23); }
 // a register of codes as two_codes of that STEP wants it
 template <int KIND, int STEP> __device__ __forceinline__ uint32_t offset_codes(uint32_t c) {
     if constexpr (KIND == KVC_CODES_INT8) return c ^ 0x80808080u;
@@ -283,8 +287,9 @@ template <int D, int KIND> struct Tiles {
 };
 
 // Rows of codes: a warp's tile has 32 tokens, as many bytes as 16 of 16 bits.  A token's score is its codes' times its key's scale.  Its weight is multiplied with its value's scale before
-// it meets the codes; in fp16 that leaves no room, so the largest power of two among the scales seen is kept beside the sums as the maximum is, and taken out of them.  bf16 queries become fp16
-// times a power of two for each head (what is 2^29 below the head's largest value loses bits, no less than a sum in 32 bits does).
+// it meets the codes, as two pieces of fp16, for which the product is too small or too large: a power of two that brings the largest product of a head so far to 2^14 is kept beside the sums as
+// the maximum is, and taken out of them.  (The largest product, not the largest scale: a row of large values that a head gives no weight takes no bits of the others.)  What is 2^-39 of that
+// product is lost, and a weight that is 2^-126 of the largest one.  bf16 queries become fp16 times a power of two for each head (what is 2^29 below the head's largest value loses bits, no less than a sum in 32 bits does).
 // What bounds them is no longer HBM but instructions, about 980 for a tile of 32 tokens of 128 channels, a third of them codes that become numbers: 8 x 4096 tokens of 32 heads in int8 61 us (4.5 TB/s;
 // fp16 rows 85), 16 x 32768 of 8 KV heads in e4m3 207 (5.3 TB/s; 317).  So CTAs have equal work sooner than with rows of 16 bits: one CTA a column of 8 x 4096 took 82 us.
 template <typename T, int D, int NT, int WH, bool SAME, int STAGES, int CTAS, bool ROWS, int KIND>
@@ -294,7 +299,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
     constexpr int TOKENS = Tiles<D, KIND>::TOKENS, ROW = Tiles<D, KIND>::ROW;
     constexpr int TEAM = WARPS / WH, TILE = TOKENS * TEAM;  // warps of a KV head, tokens of a tile
     constexpr uint32_t HALF_STAGE = Tiles<D, KIND>::HALF_STAGE, STAGE = Tiles<D, KIND>::STAGE, ALL = TOKENS == 32 ? 0xffffffffu : 0xffffu;
-    constexpr float LIFT = CODED ? Pair<__half>::LIFT : Pair<T>::LIFT, RESULT_LIFT = CODED ? 0.0f : LIFT;
+    constexpr float LIFT = CODED ? 0.0f : Pair<T>::LIFT;
     typedef std::conditional_t<CODED, uint8_t, T> Element;
     typedef std::conditional_t<CODED, Pair<__half>, Pair<T>> Operand;
     constexpr int EVEN_MOST = CODED ? 10 : D < 128 ? 10 : 14;
@@ -544,7 +549,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
     uint32_t q[KS][NT][2];
     float o[KS][NT][4], m[NT][2], l[NT][2];
     int h0 = 0, heads = 0;
-    int top_scale = 1;                                      // (CODED) the exponent's bits of the largest scale among the values so far: the sums are that power of two less
+    float most[NT][2];                                      // (CODED) the largest product of a weight and a value's scale so far: the sums are lifted(most) times what they are
     float head_scale[NT][2];                                // (CODED, bf16) what the queries were divided by, of this lane's heads
     bool fresh = true;                                      // (CODED, bf16) the queries have not become fp16 yet
     auto begin_column = [&]() {                             // (the queries are asked for; they are first used behind the next wait)
@@ -603,8 +608,8 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
             for (int k = 0; k < KS; k++) o[k][nt][0] = o[k][nt][1] = o[k][nt][2] = o[k][nt][3] = 0.0f;
             m[nt][0] = m[nt][1] = -CUDART_INF_F;
             l[nt][0] = l[nt][1] = 0.0f;
+            if (CODED) most[nt][0] = most[nt][1] = 0.0f;
         }
-        top_scale = 1;
     };
     // where this lane's rows of a matrix load lie, from the stage's start: keys 16 rows by two pieces, values two pieces by 16 rows
     uint32_t key_at[4], value_at[4];
@@ -676,19 +681,15 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
                             for (int e = 0; e < 4; e++) s[half][nt][e] = (e < 2 ? on0 : on1) ? s[half][nt][e] : -CUDART_INF_F;
                     }
                 }
-                // the largest scale of these tokens' values (left out ones have 0)
-                const int top_here = min((int)__reduce_max_sync(0xffffffffu, __float_as_uint(scales[TOKENS + lane])) >> 23, 253);
-                float rescale = 1.0f;
-                bool grows = false;
-                if (top_here > top_scale) {
-                    rescale = exp2_approx((float)(top_scale - top_here));
-                    top_scale = top_here;
-                    grows = true;
-                }
-                const float less = __uint_as_float((uint32_t)(254 - top_scale) << 23);
-                float scale[NT][2];
+                float v[2][2], scale[NT][2], lift[NT][2];   // scales of this lane's tokens' values (left out ones have 0)
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++)
+                for (int half = 0; half < 2; half++)
+#pragma unroll
+                    for (int r = 0; r < 2; r++) v[half][r] = scales[TOKENS + half * 16 + 8 * r + (lane >> 2)];
+                bool changes = false;
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+                    float largest[2];
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
                         float top = fmaxf(fmaxf(s[0][nt][e], s[0][nt][e + 2]), fmaxf(s[1][nt][e], s[1][nt][e + 2]));
@@ -696,18 +697,33 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
                         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
                         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16)) * p.log2_scaling;
                         top = fmaxf(top, m[nt][e]);
-                        grows |= top > m[nt][e];
                         const float base = top == -CUDART_INF_F ? 0.0f : top;
                         scale[nt][e] = exp2_approx(m[nt][e] - base);
                         m[nt][e] = top;
 #pragma unroll
                         for (int half = 0; half < 2; half++)
 #pragma unroll
-                            for (int i = e; i < 4; i += 2) s[half][nt][i] = exp2_approx(fmaf(s[half][nt][i], p.log2_scaling, LIFT - base));
+                            for (int i = e; i < 4; i += 2) s[half][nt][i] = exp2_approx(fmaf(s[half][nt][i], p.log2_scaling, -base));
                         l[nt][e] = fmaf(l[nt][e], scale[nt][e], (s[0][nt][e] + s[0][nt][e + 2]) + (s[1][nt][e] + s[1][nt][e + 2]));
-                        scale[nt][e] *= rescale;
+#pragma unroll
+                        for (int half = 0; half < 2; half++)
+#pragma unroll
+                            for (int r = 0; r < 2; r++) s[half][nt][e + 2 * r] *= v[half][r];
+                        largest[e] = fmaxf(fmaxf(fabsf(s[0][nt][e]), fabsf(s[0][nt][e + 2])), fmaxf(fabsf(s[1][nt][e]), fabsf(s[1][nt][e + 2])));
                     }
-                if (__any_sync(0xffffffffu, grows)) {
+                    uint32_t both = __byte_perm(__float_as_uint(largest[0]), __float_as_uint(largest[1]), 0x7632);      // (exponents are enough)
+#pragma unroll
+                    for (int i = 4; i < 32; i *= 2) both = __vmaxu2(both, __shfl_xor_sync(0xffffffffu, both, i));
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const float before = lifted_back(most[nt][e]);
+                        most[nt][e] = fmaxf(most[nt][e] * scale[nt][e], __uint_as_float(e ? both & 0xffff0000u : both << 16));
+                        lift[nt][e] = lifted(most[nt][e]);
+                        scale[nt][e] = scale[nt][e] * lift[nt][e] * before;                // (no more than 2: what it is the scale of was no more than `most`)
+                        changes |= scale[nt][e] != 1.0f;
+                    }
+                }
+                if (__any_sync(0xffffffffu, changes)) {
 #pragma unroll
                     for (int k = 0; k < KS; k++)
 #pragma unroll
@@ -721,10 +737,9 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
                     uint32_t hi[NT][2], lo[NT][2];
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
-                        const float v = scales[TOKENS + half * 16 + 8 * e + (lane >> 2)] * less;       // below 2
 #pragma unroll
                         for (int nt = 0; nt < NT; nt++) {
-                            const float w0 = s[half][nt][2 * e] * v, w1 = s[half][nt][2 * e + 1] * v;
+                            const float w0 = s[half][nt][2 * e] * lift[nt][0], w1 = s[half][nt][2 * e + 1] * lift[nt][1];      // below 2^15
                             const uint32_t top = Operand::pack(w0, w1);
                             const float2 f = Operand::unpack(top);
                             hi[nt][e] = transpose8x8(top);
@@ -827,16 +842,14 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
             if (at.i == at.n - 1 || n == share - 1) {
                 // ---- the column's end in this share: the warps' results are joined; the stage just read holds their sums meanwhile
                 const uint32_t scratch = stage * STAGE;
-                if constexpr (CODED) {                      // what was taken out of sums and weights
-                    constexpr float LESS = 1.0f / (1 << (int)LIFT);
-                    const float back = __uint_as_float((uint32_t)top_scale << 23);
+                if constexpr (CODED) {                      // what was taken out of the sums
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++) {
-                        l[nt][0] *= LESS; l[nt][1] *= LESS;
+                        const float back[2] = {lifted_back(most[nt][0]), lifted_back(most[nt][1])};
 #pragma unroll
                         for (int k = 0; k < KS; k++)
 #pragma unroll
-                            for (int e = 0; e < 4; e++) o[k][nt][e] = o[k][nt][e] * LESS * back;
+                            for (int e = 0; e < 4; e++) o[k][nt][e] *= back[e & 1];
                     }
                 }
 #pragma unroll
@@ -888,7 +901,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
                     if constexpr (KIND == WIDE_RESULTS) __stcg(reinterpret_cast<float4 *>(p.wide + ((long long)of_row * a.Hq + h) * D + d), make_float4(v.x * f, v.y * f, v.z * f, v.w * f));
                     else *reinterpret_cast<uint2 *>(reinterpret_cast<T *>(a.out) + of_row * a.out_token + h * a.out_head + d) =
                         make_uint2(Pair<T>::pack(v.x * f, v.y * f), Pair<T>::pack(v.z * f, v.w * f));
-                    if (d == 0 && a.lse) a.lse[of_row * a.Hq + h] = sum == 0.0f ? -CUDART_INF_F : (top + log2f(sum) - RESULT_LIFT) * 0.69314718055994531f;
+                    if (d == 0 && a.lse) a.lse[of_row * a.Hq + h] = sum == 0.0f ? -CUDART_INF_F : (top + log2f(sum) - LIFT) * 0.69314718055994531f;
                 };
                 float *part = p.parts + (long long)place * p.part;
                 // the warps of a KV head join their sums
