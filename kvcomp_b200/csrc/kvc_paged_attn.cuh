@@ -667,8 +667,9 @@ __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_
                     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
-                            s[half][nt][e] = (t[0][nt][e] + t[1][nt][e]) * (e < 2 ? k0 : k1);
-                            if constexpr (std::is_same_v<T, __nv_bfloat16>) s[half][nt][e] *= head_scale[nt][e & 1];
+                            float back = e < 2 ? k0 : k1;
+                            if constexpr (std::is_same_v<T, __nv_bfloat16>) back *= head_scale[nt][e & 1];      // (first: the products of codes and lifted queries may leave 32 bits with one of the two)
+                            s[half][nt][e] = (t[0][nt][e] + t[1][nt][e]) * back;
                         }
                 }
                 if (mask != ALL) {

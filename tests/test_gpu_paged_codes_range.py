@@ -129,3 +129,13 @@ def test_long_requests(ops, codes):
         v[0, at, head] *= 1e13
         k[0, at, head] = with_scores(q[0, 2 * head:2 * head + 2], [-200.0, -30.0], scaling).float()
     check(ops, q, k, v, codes, scaling, page=64)
+
+
+@pytest.mark.parametrize("codes", CODES)
+def test_keys_whose_products_leave_32_bits(ops, codes):
+    """Keys of 1e37 and queries of 1e-37 have scores like any other's."""
+    D, n = 64, 50
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    q = (rows(gen, 1, 2, D) * 1e-37).to(torch.bfloat16)
+    k, v = rows(gen, 1, n, 1, D) * 1e37, rows(gen, 1, n, 1, D)
+    check(ops, q, k, v, codes, 0.1)
