@@ -486,7 +486,7 @@ typedef struct {
     int32_t codes, reserved;
 } kvc_scales;
 
-/* kvc_rotary_store into pools of codes: keys are coded from their rotated values in fp32, values from theirs; Hkv > 0.  Neither pools nor scales may overlap one another or what is
+/* kvc_rotary_store into pools of codes: keys are coded as they are rotated, in fp32 (int8) or as if without any error (e4m3: the angle is position x frequency in fp64), values as they are; Hkv > 0.  Neither pools nor scales may overlap one another or what is
  * read or written beside them. */
 int kvc_rotary_store_codes(const kvc_rotary_args *args, const kvc_scales *scales, kvc_stream_t stream);
 

@@ -62,6 +62,11 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     asm("{ .reg .b64 x, y; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; add.rn.f32x2 x, x, y; mov.b64 {%0, %1}, x; }" : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
     return r;
 }
+__device__ __forceinline__ float2 fma2(float2 a, float b, float2 c) {
+    float2 r;
+    asm("{ .reg .b64 x, y, z; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %4}; mov.b64 z, {%5, %6}; fma.rn.f32x2 x, x, y, z; mov.b64 {%0, %1}, x; }" : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b), "f"(c.x), "f"(c.y));
+    return r;
+}
 // the largest size of three; no number if one is none
 __device__ __forceinline__ float largest(float a, float b, float c) {
     float r;
@@ -108,11 +113,19 @@ template <int KIND, int N> __device__ __forceinline__ void codes_of(const float 
     }
 }
 
-// NEAR at most: a value in 32 bits, off by some of its last bits, that may lie on the other side of a border between two e4m3.  (A scale is a power of two, and a border a number of five bits, the
-// last one 1; those between the smallest codes have fewer and are let be.)
-constexpr uint32_t NEAR = 12;
-__device__ __forceinline__ uint32_t to_border(float x) { return (__float_as_uint(x) - 0x80000u + NEAR / 2) & 0xfffff; }
-// Such a value rotated in 64 bits, cut to 24, the last one 1 where something was cut off: it rounds to fewer as the value itself does.
+// A pair y0, y1 rotated in 32 bits is off by NEAR times |y0| + |y1| at most (the sum of its products' sizes is their length, and that no more than this): 2.5 2^-24 of a product by cos or sin (their
+// argument's, their series' and their own rounding), three more for the factor, a product and the sum, one for the limits themselves.  e4m3 keys are those of a rotation without any error: where
+// both limits have the same code that is the key's, and the few others (one of some 15000; without it some keys in a million get the code beside theirs, and one of hundreds where a pair's products
+// cancel) are rotated in 64 bits.
+constexpr float NEAR = 7.0f / 16777216.0f;
+__device__ __forceinline__ uint32_t e4m3_of(float2 v) { return __nv_cvt_float2_to_fp8x2(v, __NV_SATFINITE, __NV_E4M3); }
+// Codes of four such values and the sizes |y0| + |y1| of their pairs; far: NEAR over the scale.  Returns where those of the limits differ.
+__device__ __forceinline__ uint32_t codes_within(const float *x, float s0, float s1, float s2, float s3, float inverse, float far, uint32_t &packed) {
+    const float2 a = mul2(make_float2(x[0], x[1]), inverse), b = mul2(make_float2(x[2], x[3]), inverse);
+    packed = e4m3_of(fma2(make_float2(s0, s1), -far, a)) | e4m3_of(fma2(make_float2(s2, s3), -far, b)) << 16;
+    return packed ^ (e4m3_of(fma2(make_float2(s0, s1), far, a)) | e4m3_of(fma2(make_float2(s2, s3), far, b)) << 16);
+}
+// A value rotated in 64 bits, cut to 24, the last one 1 where something was cut off: it rounds to fewer as the value itself does, and is above a number of fewer bits where the value is.
 __device__ __noinline__ float rotated_closely(double position, double frequency, float factor, float f0, float f1, bool second) {
     double turns = position * (frequency * TURNS_OF_RADIANS), c, s;
     turns -= rint(turns);
@@ -121,20 +134,41 @@ __device__ __noinline__ float rotated_closely(double position, double frequency,
     const float cut = __double2float_rz(exact);
     return (double)cut == exact ? cut : __uint_as_float(__float_as_uint(cut) | 1);
 }
-// The codes of such values among a thread's 8 pairs.  One of 80000 values; without it some keys in a million get the code beside theirs.
-template <typename T> __device__ __noinline__ void code_again(const T *src, uint8_t *dst, int apart, bool half, double position, const double *frequencies, float factor, float inverse) {
+// which bytes are not 0: a bit for each
+__device__ __forceinline__ uint32_t bits_of(uint32_t bytes) { return ((__vcmpne4(bytes, 0) & 0x01010101u) * 0x10204080u) >> 28; }
+// The codes of those of a thread's 16 values whose bit of `which` is set; turns: they are rotated.
+template <typename T> __device__ __noinline__ void code_closely(uint32_t which, const T *src, uint8_t *dst, int apart, bool half, bool turns, double position, const double *frequencies, float factor, float inverse) {
+#pragma unroll 1
+    for (; which; which &= which - 1) {
+        const int v = __ffs(which) - 1, k = half ? v & 7 : v >> 1, i0 = half ? k : 2 * k, i1 = half ? apart + k : 2 * k + 1;
+        const bool second = half ? v >= 8 : v & 1;
+        const float f0 = to_float(src[i0]), f1 = to_float(src[i1]);
+        const float y = turns ? rotated_closely(position, frequencies[k], factor, f0, f1, second) : second ? f1 : f0;
+        dst[second ? i1 : i0] = (uint8_t)__nv_cvt_float_to_fp8(y * inverse, __NV_SATFINITE, __NV_E4M3);
+    }
+}
+// A row's largest value decides on its scale, 448 times a power of two being the border: 1.75 2^e.  It is off by 2 NEAR of itself (|y0| + |y1| is no more than twice it), 13 of its last bits there;
+// next to the border one of the row's values may be above it and the largest in 32 bits not, or the other way round.
+constexpr uint32_t OF_BORDER = 0x600000, LAST_BITS = 13;
+__device__ __forceinline__ bool at_border(uint32_t top) { return ((top - OF_BORDER + LAST_BITS) & 0x7fffffu) <= 2 * LAST_BITS && top >> 23 >= 127 - 100 + 8; }       // (below, the scale is the least)
+__device__ __forceinline__ uint32_t border_of(uint32_t top) { return (top & 0x7f800000u) | OF_BORDER; }
+// whether one of a thread's 8 pairs has a value above it; turns: they are rotated
+template <typename T> __device__ __noinline__ bool above_border(uint32_t border, const T *src, int apart, bool half, bool turns, double position, const double *frequencies, float factor) {
+    bool above = false;
 #pragma unroll 1
     for (int k = 0; k < 8; k++) {
-        const int i0 = half ? k : 2 * k, i1 = half ? apart + k : 2 * k + 1;
-        const float f0 = to_float(src[i0]), f1 = to_float(src[i1]);
-        const float2 cs = turn_closely(position, frequencies[k] * TURNS_OF_RADIANS, factor);
-        const float y[2] = {f0 * cs.x - f1 * cs.y, f1 * cs.x + f0 * cs.y};
+        const float f0 = to_float(src[half ? k : 2 * k]), f1 = to_float(src[half ? apart + k : 2 * k + 1]);
         for (int second = 0; second < 2; second++) {
-            if (to_border(y[second]) > NEAR) continue;
-            const float cut = rotated_closely(position, frequencies[k], factor, f0, f1, second);
-            dst[second ? i1 : i0] = (uint8_t)__nv_cvt_float_to_fp8(cut * inverse, __NV_SATFINITE, __NV_E4M3);
+            float y = second ? f1 : f0;
+            if (turns) {
+                const float2 cs = turn_closely(position, frequencies[k] * TURNS_OF_RADIANS, factor);
+                y = second ? f1 * cs.x + f0 * cs.y : f0 * cs.x - f1 * cs.y;
+                if (size_of(y) + LAST_BITS >= border) y = rotated_closely(position, frequencies[k], factor, f0, f1, second);
+            }
+            above |= size_of(y) > border;
         }
     }
+    return above;
 }
 
 // Where a token goes: its row in the pools (in codes) and its place among the scales; -1: nowhere
@@ -156,7 +190,8 @@ __device__ __forceinline__ Place place_of(const CodesParams &p, int slot, int &f
 // angles it makes once; the lanes of a row are neighbours in a warp and find the row's largest value among them.  A CTA has the same few heads of several tokens, the next one the next
 // heads of these: queries, which are bytes alone, and keys and values, which take instructions, run at the same time.
 // Measured: 16384 tokens of 40 + 10 + 10 heads of 128 channels in int8 (463 MB) 94 us, 5.0 TB/s, one kind behind the other and one head at a time 147; four or six CTAs per SM (the latter
-// spilling) 112, two heads of a thread 104, six 116.  e4m3, 4099 tokens of 32 + 8 + 8 heads (93 MB) 22 us, 3 of them the second look at values next to a border.
+// spilling) 112, two heads of a thread 104, six 116.  e4m3 93, and 4099 tokens of 32 + 8 + 8 heads (93 MB) 21.
+// (Where the second looks at values next to a border were made in the loop, 135 and 26.)
 template <typename T, int KIND>
 __global__ void __launch_bounds__(CODES_THREADS, CODES_CTAS) codes_rows_kernel(const __grid_constant__ CodesParams p) {
     kvc_behind();
@@ -243,6 +278,8 @@ __global__ void __launch_bounds__(CODES_THREADS, CODES_CTAS) codes_rows_kernel(c
         }
         return;
     }
+    uint32_t exponents = 0, borders = 0, again[CHUNK / 2] = {};                             // (e4m3) of the heads' scales; rows at a border of scales; values at a border of codes
+    const bool sure = !turns || (position == 0 && a.factor == 1.0f);                       // (what is not turned is as it was)
     // Two heads at a time: the way from a row's values to its scale is a chain, and two take little more than one.
 #pragma unroll
     for (int j = 0; j < CHUNK; j += 2) {
@@ -264,29 +301,70 @@ __global__ void __launch_bounds__(CODES_THREADS, CODES_CTAS) codes_rows_kernel(c
 #pragma unroll
         for (int i = 0; i < 2; i++) {
             s[i] = scale_of<KIND>(size_of(top[i]), inverse[i]);
+            if (KIND == KVC_CODES_E4M3) {
+                uint32_t e = __float_as_uint(s[i]) >> 23;
+                if (part.turned > 0 && at_border(size_of(top[i]))) { borders |= 1u << (j + i); e = (size_of(top[i]) >> 23) - 8; }
+                exponents |= (e & 0xff) << 8 * (j + i);
+            }
             if (on && j + i < heads) {
-                uint32_t c[4];
-                codes_of<KIND, 2>(f[i], s[i], inverse[i], c);
-                codes_of<KIND, 2>(f[i] + 8, s[i], inverse[i], c + 2);
+                uint32_t c[4], unsure[4] = {};
+                if (KIND == KVC_CODES_E4M3 && part.turned > 0) {
+                    const float *const y = f[i], far = sure ? 0.0f : NEAR * inverse[i];
+                    auto size = [&](int a, int b) { return fabsf(y[a]) + fabsf(y[b]); };
+                    if (a.layout == KVC_ROTARY_HALF) {
+#pragma unroll
+                        for (int m = 0; m < 8; m += 4) {
+                            const float s0 = size(m, m + 8), s1 = size(m + 1, m + 9), s2 = size(m + 2, m + 10), s3 = size(m + 3, m + 11);
+                            unsure[m / 4] = codes_within(y + m, s0, s1, s2, s3, inverse[i], far, c[m / 4]);
+                            unsure[m / 4 + 2] = codes_within(y + m + 8, s0, s1, s2, s3, inverse[i], far, c[m / 4 + 2]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int m = 0; m < 16; m += 4) {
+                            const float s0 = size(m, m + 1), s1 = size(m + 2, m + 3);
+                            unsure[m / 4] = codes_within(y + m, s0, s0, s1, s1, inverse[i], far, c[m / 4]);
+                        }
+                    }
+                } else {
+                    codes_of<KIND, 2>(f[i], s[i], inverse[i], c);
+                    codes_of<KIND, 2>(f[i] + 8, s[i], inverse[i], c + 2);
+                }
                 *reinterpret_cast<uint2 *>(dst) = make_uint2(c[0], c[1]);
                 *reinterpret_cast<uint2 *>(dst + apart) = make_uint2(c[2], c[3]);
                 if (u == 0) *scale = s[i];
-                if (KIND == KVC_CODES_E4M3 && turns) {
-                    uint32_t near = 0xffffffffu;
-#pragma unroll
-                    for (int m = 0; m < 16; m++) near = min(near, to_border(f[i][m]));
-                    if (near <= NEAR && position != 0)
-                        code_again<T>(reinterpret_cast<const T *>(part.src) + n * part.src_token + (h0 + j + i) * part.src_head + c0, dst, apart, half, a.inverse ? -(double)position : (double)position,
-                                      a.frequencies + 8 * u, a.factor, inverse[i]);
-                }
+                if (KIND == KVC_CODES_E4M3 && (unsure[0] | unsure[1] | unsure[2] | unsure[3]))
+                    again[j / 2] |= (bits_of(unsure[0]) | bits_of(unsure[1]) << 4 | bits_of(unsure[2]) << 8 | bits_of(unsure[3]) << 12) << 16 * i;
             }
             dst += part.dst_head;
             scale += which == 1 ? p.s.k_head : p.s.v_head;
         }
     }
+    // Second looks, few, behind all else: in the loop what they need would have to be kept beside what it does.
+    if (KIND == KVC_CODES_E4M3 && which == 1 && (borders | again[0] | again[1])) {
+        int ignored = 0;
+        const Place at = place_of(p, slot, ignored);
+        const double turned_by = a.inverse ? -(double)position : (double)position;
+#pragma unroll 1
+        for (int j = 0; j < heads; j++) {
+            const T *const row = reinterpret_cast<const T *>(part.src) + n * part.src_token + (h0 + j) * part.src_head + c0;
+            int e = exponents >> 8 * j & 0xff;
+            uint32_t values = (j < 2 ? again[0] : again[1]) >> 16 * (j & 1) & 0xffff;
+            if (borders >> j & 1) {                         // (a row's lanes all, or none) all of its codes go by what is found
+                const uint32_t border = (uint32_t)(e + 8) << 23 | OF_BORDER;
+                const bool above = on && above_border<T>(border, row, apart, half, turns, turned_by, a.frequencies + 8 * u, a.factor);
+                e = max(e + (__any_sync(row_lanes, above) ? 1 : 0), 127 - 100);
+                if (u == 0) p.s.k[at.ks + (h0 + j) * p.s.k_head] = __uint_as_float((uint32_t)e << 23);
+                values = on ? 0xffff : 0;
+            }
+            if (values)
+                code_closely<T>(values, row, reinterpret_cast<uint8_t *>(part.dst) + at.k + (h0 + j) * part.dst_head + c0, apart, half, turns, turned_by, a.frequencies + 8 * u, a.factor,
+                                __uint_as_float((uint32_t)(254 - e) << 23));
+        }
+    }
 }
 
-// Any sizes and strides of what is read: a warp per row, a lane every 32nd channel.
+// Any sizes and strides of what is read: a warp per row, a lane every 32nd channel, whose angle it makes for itself, and again for its code.  4099 tokens of 32 + 8 + 8 heads of 96 channels, 24 of
+// them rotated, in e4m3 (70 MB) 71 us.
 template <typename T, int KIND>
 __global__ void __launch_bounds__(CODES_THREADS) codes_any_kernel(const __grid_constant__ CodesParams p) {
     kvc_behind();
@@ -320,15 +398,23 @@ __global__ void __launch_bounds__(CODES_THREADS) codes_any_kernel(const __grid_c
         other = a.layout == KVC_ROTARY_HALF ? (second ? i - half : i + half) : i ^ 1;
         return a.layout == KVC_ROTARY_HALF ? (second ? other : i) : i >> 1;
     };
+    struct Value { float y, size; };                        // (size: of its pair, 0 where nothing is turned)
     auto value = [&](int i) {
-        if (i >= rotary) return to_float(x[i]);
+        if (i >= rotary) return Value{to_float(x[i]), 0.0f};
         int other;
         bool second;
         const int k = pair_of(i, other, second);
         const float2 cs = turn_closely(position, a.frequencies[k] * TURNS_OF_RADIANS, a.factor);
         const float f0 = to_float(x[second ? other : i]), f1 = to_float(x[second ? i : other]);
-        const float y = second ? f1 * cs.x + f0 * cs.y : f0 * cs.x - f1 * cs.y;
-        return KIND == KVC_CODES_E4M3 && to_border(y) <= NEAR ? rotated_closely(position, a.frequencies[k], a.factor, f0, f1, second) : y;
+        const float y0 = f0 * cs.x - f1 * cs.y, y1 = f1 * cs.x + f0 * cs.y;
+        return Value{second ? y1 : y0, position == 0.0 && a.factor == 1.0f ? 0.0f : fabsf(y0) + fabsf(y1)};
+    };
+    auto value_closely = [&](int i) {
+        if (i >= rotary) return to_float(x[i]);
+        int other;
+        bool second;
+        const int k = pair_of(i, other, second);
+        return rotated_closely(position, a.frequencies[k], a.factor, to_float(x[second ? other : i]), to_float(x[second ? i : other]), second);
     };
     if (h < a.Hq) {                                         // (the result may lie where the query does: 32 channels and their partners are read before any is written)
         for (int i = lane; i < D; i += 32) {
@@ -345,14 +431,25 @@ __global__ void __launch_bounds__(CODES_THREADS) codes_any_kernel(const __grid_c
         return;
     }
     uint32_t top = 0;
-    for (int i = lane; i < D; i += 32) top = max(top, size_of(value(i)));
+    for (int i = lane; i < D; i += 32) top = max(top, size_of(value(i).y));
     top = __reduce_max_sync(0xffffffffu, top);
+    if (KIND == KVC_CODES_E4M3 && rotary > 0 && at_border(top)) {
+        bool above = false;
+        for (int i = lane; i < D; i += 32)
+            if (size_of(value(i).y) + LAST_BITS >= border_of(top)) above |= size_of(value_closely(i)) > border_of(top);
+        top = border_of(top) + (__any_sync(0xffffffffu, above) ? 1 : 0);
+    }
     float inverse;
     const float s = scale_of<KIND>(top, inverse);
     for (int i = lane; i < D; i += 32) {
-        const float v[4] = {value(i), 0.0f, 0.0f, 0.0f};
+        const Value of = value(i);
+        const float v[4] = {of.y, 0.0f, 0.0f, 0.0f};
         uint32_t c;
-        codes_of<KIND, 1>(v, s, inverse, &c);
+        if (KIND == KVC_CODES_E4M3) {
+            if (codes_within(v, of.size, 0.0f, 0.0f, 0.0f, inverse, NEAR * inverse, c)) c = __nv_cvt_float_to_fp8(value_closely(i) * inverse, __NV_SATFINITE, __NV_E4M3);
+        } else {
+            codes_of<KIND, 1>(v, s, inverse, &c);
+        }
         dst[i] = (uint8_t)c;
     }
     if (lane == 0) *scale = s;
