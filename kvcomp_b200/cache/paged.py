@@ -88,22 +88,25 @@ class PagedKVCache:
         """From here on request b's tokens come behind the first shared[b] tokens of request parents[b] (int32[requests] on the device; below 0: of none): their positions go on from there
         (begin), and attend covers both.  shared None: all tokens that the parent has now.  Requests that follow the same tokens are attended to together, and these are read once.  To be said
         before a follower's first tokens; for all requests at once, those that followed before included.  Who is followed brings no more tokens, stays until its followers have ended, and
-        follows no one; a follower that ends (release) follows no one any more.  Steps that are captured behind the first call go by the last one, captured or not.  Heads of 64, 96 or 128
-        channels, no window, no codes."""
+        follows no one; a follower that ends (release) follows no one any more; a parent that is no request, or the request itself, is none (reported: check).  Steps that are captured behind
+        the first call go by the last one, captured or not.  Heads of 64, 96 or 128 channels, no window, no codes."""
         if self.window or self.codes or self.head_dim not in ops.SHARED_HEADS:
             raise KvcError("PagedKVCache.follow: heads of 64, 96 or 128 channels, no window and no codes")
         if not isinstance(parents, torch.Tensor) or parents.dtype != torch.int32 or tuple(parents.shape) != (self.requests,) or parents.device != self.device:
             raise KvcError("parents must be int32[%d] on %s" % (self.requests, self.device))
         if shared is None:
-            shared = torch.where(parents >= 0, self.lengths[parents.clamp(0, self.requests - 1).long()], 0).int()
+            shared = self.lengths[parents.clamp(0, self.requests - 1).long()]
         elif not isinstance(shared, torch.Tensor) or shared.dtype != torch.int32 or tuple(shared.shape) != (self.requests,) or shared.device != self.device:
             raise KvcError("shared must be int32[%d] on %s" % (self.requests, self.device))
         if self.prefixes is None:
             if torch.cuda.is_current_stream_capturing():
                 raise KvcError("PagedKVCache.follow: the first call makes what all steps go by, and must not be captured")
             self.parents, self.shared = torch.empty_like(parents), torch.empty_like(parents)
-        self.parents.copy_(parents)
-        self.shared.copy_(torch.where(parents >= 0, shared, 0))
+        # whom nobody can follow is followed by none, in the plan, in positions and in lengths alike, and is reported (check raises)
+        valid = (parents >= 0) & (parents < self.requests) & (parents != torch.arange(self.requests, dtype=torch.int32, device=self.device)) & (shared >= 0)
+        self.status.bitwise_or_(((parents >= 0) & ~valid).any().int() * _lib.FLAG_BAD_LENGTH)
+        self.parents.copy_(torch.where(valid, parents, -1))
+        self.shared.copy_(torch.where(valid, shared, 0))
         self.prefixes = ops.prefix_plan(self.parents, self.shared, out=self.prefixes, status=self.status)
 
     def slots(self, tokens):
@@ -161,7 +164,7 @@ class PagedKVCache:
         ops.page_release(self.lengths, done, self.table, self.free, self.head, self.page_size, out=(self.lengths, self.head), status=self.status)
         if self.prefixes is not None:
             # those that ended follow no one; neither do those whose prefix has gone, which is reported (check raises)
-            lost = (self.parents >= 0) & done[self.parents.clamp(0, self.requests - 1).long()]
+            lost = (self.parents >= 0) & done[self.parents.clamp(min=0).long()]
             self.status.bitwise_or_((lost & ~done).any().int() * _lib.FLAG_BAD_LENGTH)
             self.parents.masked_fill_(lost | done, -1)
             self.shared.masked_fill_(lost | done, 0)

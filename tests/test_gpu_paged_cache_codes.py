@@ -180,6 +180,32 @@ def test_a_prefix_that_goes_too_early(Cache):  # noqa: F811
         cache.check()
 
 
+@pytest.mark.parametrize("parents,shared", [([-1, 0, 7, 0], None), ([-1, 0, 4, 0], [0, 9, 9, 9]), ([-1, 0, 2, 0], [0, 5, 5, 5]), ([-1, 0, 0, 0], [0, 9, -3, 9]), ([-1, 0, 1 << 30, 0], None)], ids=str)
+def test_parents_that_are_none(Cache, parents, shared):  # noqa: F811
+    """A request that says it follows no request, itself, or tokens below none is one that follows no one: positions, lengths, results and releases; check raises."""
+    from kvcomp_b200._lib import KvcError
+    R, Hq, Hkv, D = 4, 4, 2, 64
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    caches = [Cache(R, 40, 1, Hkv, D, page_size=8, max_tokens=80, frequencies=frequencies(D)[0]) for _ in range(2)]
+    k, v = randn(gen, torch.float16, 20, Hkv, D), randn(gen, torch.float16, 20, Hkv, D)
+    qkv = randn(gen, torch.float16, R, Hq + 2 * Hkv, D)
+    results = []
+    for cache, of in zip(caches, (parents, [p if b != 2 else -1 for b, p in enumerate(parents)])):
+        cache.begin(dev([20, 0, 0, 0]), 20)
+        cache.append(None, k, v, 0)
+        cache.follow(dev(of), None if shared is None else dev(shared))
+        plan = cache.begin(dev([0, 1, 1, 1]), 3)
+        q = cache.append(qkv[:3, :Hq], qkv[:3, Hq:Hq + Hkv], qkv[:3, Hq + Hkv:], 0)
+        results.append((plan.positions, q, cache.attend(q, 0), cache.parents.clone(), cache.shared.clone(), torch.tensor([cache.get_seq_length(b) for b in range(R)])))
+    assert all(torch.equal(a, b) for a, b in zip(*results)) and results[0][0][1] == 0 and results[0][5][2] == 1
+    with pytest.raises(KvcError):
+        caches[0].check()
+    assert caches[1].check() == 0
+    for cache in caches:                                            # the last request ends: nobody's prefix does
+        cache.release(dev([False, False, False, True], torch.bool))
+        assert cache.check() == 0 and cache.parents.tolist() == [-1, 0, -1, -1]
+
+
 def test_captured_steps_of_followers(Cache):  # noqa: F811
     """One graph: followers that change between replays are those that it goes by, also where the release is part of it."""
     R, Hq, Hkv, D = 4, 4, 2, 128
