@@ -98,16 +98,19 @@ class PagedKVCache:
             shared = self.lengths[parents.clamp(0, self.requests - 1).long()]
         elif not isinstance(shared, torch.Tensor) or shared.dtype != torch.int32 or tuple(shared.shape) != (self.requests,) or shared.device != self.device:
             raise KvcError("shared must be int32[%d] on %s" % (self.requests, self.device))
-        if self.prefixes is None:
-            if torch.cuda.is_current_stream_capturing():
-                raise KvcError("PagedKVCache.follow: the first call makes what all steps go by, and must not be captured")
-            self.parents, self.shared = torch.empty_like(parents), torch.empty_like(parents)
+        if self.prefixes is None and torch.cuda.is_current_stream_capturing():
+            raise KvcError("PagedKVCache.follow: the first call makes what all steps go by, and must not be captured")
         # whom nobody can follow is followed by none, in the plan, in positions and in lengths alike, and is reported (check raises)
         valid = (parents >= 0) & (parents < self.requests) & (parents != torch.arange(self.requests, dtype=torch.int32, device=self.device)) & (shared >= 0)
-        self.status.bitwise_or_(((parents >= 0) & ~valid).any().int() * _lib.FLAG_BAD_LENGTH)
-        self.parents.copy_(torch.where(valid, parents, -1))
-        self.shared.copy_(torch.where(valid, shared, 0))
-        self.prefixes = ops.prefix_plan(self.parents, self.shared, out=self.prefixes, status=self.status)
+        none = ((parents >= 0) & ~valid).any().int() * _lib.FLAG_BAD_LENGTH
+        parents, shared = torch.where(valid, parents, -1), torch.where(valid, shared, 0)
+        if self.prefixes is None:                                    # (a plan that cannot be made leaves the cache as it was)
+            self.prefixes, self.parents, self.shared = ops.prefix_plan(parents, shared, status=self.status), parents, shared
+        else:
+            self.parents.copy_(parents)
+            self.shared.copy_(shared)
+            ops.prefix_plan(self.parents, self.shared, out=self.prefixes, status=self.status)
+        self.status.bitwise_or_(none)
 
     def slots(self, tokens):
         """Where the tokens that requests have lie, request by request: (slots int32[tokens], starts int32[requests + 1]), for rows.  tokens: their number, as the host knows it; slots behind them

@@ -276,3 +276,38 @@ def test_refused(Cache):  # noqa: F811
     for parents, shared in ((i[:1], None), (i.long(), None), (i.cpu(), None), (i, i[:1]), ([-1, 0], None)):
         with pytest.raises(KvcError):
             cache.follow(parents, shared)
+
+
+def test_more_requests_than_a_plan_takes(Cache):  # noqa: F811
+    """A refused follow leaves a cache as it was: lengths, steps, copies; the largest number is taken."""
+    from kvcomp_b200._lib import KvcError
+    for R, taken in ((16385, False), (16384, True)):
+        cache = Cache(R, 8, 1, 1, 64, page_size=8, max_tokens=16)
+        k = torch.randn(9, 1, 64, device="cuda").half()
+        new = torch.zeros(R, dtype=torch.int32, device="cuda")
+        new[5] = 9
+        cache.begin(new, 9)
+        cache.append(None, k, k, 0)
+        parents = torch.full((R,), -1, dtype=torch.int32, device="cuda")
+        parents[7] = 5
+        if taken:
+            cache.follow(parents)
+        else:
+            with pytest.raises(KvcError):
+                cache.follow(parents)
+        assert cache.get_seq_length(7) == (9 if taken else 0) and (cache.prefixes is None) == (cache.parents is None) == (cache.shared is None) == (not taken)
+        new.zero_()
+        new[7] = 1
+        plan = cache.begin(new, 1)
+        q = cache.append(torch.randn(1, 2, 64, device="cuda").half(), k[:1], k[:1], 0)
+        assert plan.positions.tolist() == [9 if taken else 0]
+        near(cache.attend(q, 0), *plain_of(q, k if taken else k[:0], k[:1]))
+        cache.release(new.bool())
+        assert cache.check() == 0
+
+
+def plain_of(q, *tokens):
+    """(result, bound) of one request with these tokens as keys and values."""
+    x = torch.cat(tokens)[:, 0].double().cpu()
+    w = torch.softmax(q[0].double().cpu() @ x.T / math.sqrt(x.shape[1]), -1)
+    return (w @ x)[None], 2.0 ** -9 * x.abs().max()
