@@ -510,7 +510,7 @@ typedef struct {
 int kvc_page_shift(const kvc_page_shift_args *args, kvc_stream_t stream);
 
 /* The rows `slots` of the pools, keys and values, as fp16 or bf16 rows k_out, v_out [N, Hkv, D]: codes times scales in fp32, rounded once, or (KVC_CODES_NONE) rows of 16 bits as they are.
- * A slot below 0 gives zeros, one behind the pool zeros and KVC_FLAG_BAD_PAGE.  Everything starts on 16 bytes; outputs overlap neither one another nor a pool. */
+ * A slot below 0 gives zeros, one behind the pool zeros and KVC_FLAG_BAD_PAGE.  Everything starts on 16 bytes; outputs overlap neither one another nor what is read. */
 typedef struct {
     const void *kpages, *vpages;
     kvc_scales scales;

@@ -650,7 +650,13 @@ extern "C" int kvc_paged_rows(const kvc_paged_rows_args *args, kvc_stream_t stre
     const kvc_rows kp = kvc_make_rows(a.kpages, a.D / half, a.n_pages, a.kp_page / half, a.page_size, a.kp_row / half, a.Hkv, a.kp_head / half);
     const kvc_rows vp = kvc_make_rows(a.vpages, a.D / half, a.n_pages, a.vp_page / half, a.page_size, a.vp_row / half, a.Hkv, a.vp_head / half);
     KVC_REQUIRE(k.apart && v.apart && !kvc_rows_overlap(k, v), "kvc_paged_rows: rows of the outputs overlap");
-    for (const kvc_rows &out : {k, v}) KVC_REQUIRE(!kvc_rows_overlap(out, kp) && !kvc_rows_overlap(out, vp), "kvc_paged_rows: an output overlaps a pool");
+    const kvc_rows ks = kvc_make_rows(a.scales.k, 2 * a.page_size, a.n_pages, 2 * a.scales.k_page, a.Hkv, 2 * a.scales.k_head), vs = kvc_make_rows(a.scales.v, 2 * a.page_size, a.n_pages, 2 * a.scales.v_page, a.Hkv, 2 * a.scales.v_head);
+    const kvc_rows slots = kvc_make_rows(a.slots, 2 * a.N, 1, 0, 1, 0);
+    for (const kvc_rows &out : {k, v}) {
+        KVC_REQUIRE(!kvc_rows_overlap(out, kp) && !kvc_rows_overlap(out, vp), "kvc_paged_rows: an output overlaps a pool");
+        KVC_REQUIRE(codes == KVC_CODES_NONE || (!kvc_rows_overlap(out, ks) && !kvc_rows_overlap(out, vs)), "kvc_paged_rows: an output overlaps the scales");
+        KVC_REQUIRE(!kvc_rows_overlap(out, slots), "kvc_paged_rows: an output overlaps the slots");
+    }
     p.page = kvc_make_div((uint32_t)a.page_size);
     p.slots = a.n_pages * a.page_size;
     const int64_t units = a.D / 16;

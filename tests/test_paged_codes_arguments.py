@@ -87,6 +87,20 @@ def test_refusals(call, change):
     assert call.replace("_codes", "").encode() in _lib.load().kvc_last_error()
 
 
+@pytest.mark.parametrize("change,what", [(dict(k_out=7 * AT), "scales"), (dict(v_out=7 * AT + 16), "scales"), (dict(k_out=8 * AT), "scales"), (dict(v_out=8 * AT), "scales"), (dict(k_out=AT), "slots"),
+                                         (dict(v_out=AT - 16), "slots"), (dict(k_out=7 * AT - 32), "scales"), (dict(s_codes=0, v_out=AT), "slots")], ids=str)
+def test_rows_over_what_is_read(change, what):
+    assert make("kvc_paged_rows", **change) == 1 and _lib.load().kvc_last_error().decode() == "kvc_paged_rows: an output overlaps the %s" % what
+
+
+def test_rows_beside_what_is_read():
+    """Neighbours are no overlap.  (So many rows that the call is refused for their number, behind these checks: nothing is launched wherever this runs.)"""
+    far, n = dict(N=1 << 30, slots=1 << 48, s_k=1 << 49, s_v=(1 << 49) + AT, v_out=1 << 52), 1 << 50
+    for at, what in (((1 << 48) + (4 << 30), None), ((1 << 48) + (4 << 30) - 16, "slots"), ((1 << 49) + AT + 10 * 32 * 4, None), ((1 << 49) + AT + 10 * 32 * 4 - 16, "scales"), (n, None)):
+        assert make("kvc_paged_rows", **far, k_out=at) == 1
+        assert _lib.load().kvc_last_error().decode() == "kvc_paged_rows: " + ("an output overlaps the " + what if what else "too many rows")
+
+
 def test_null_and_nothing_to_do():
     lib = _lib.load()
     assert lib.kvc_rotary_store_codes(None, None, None) == 1 and lib.kvc_paged_rows(None, None) == 1 and lib.kvc_page_slots(None, None) == 1 and lib.kvc_page_shift(None, None) == 1
