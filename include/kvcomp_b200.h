@@ -542,7 +542,7 @@ int kvc_prefix_plan(const kvc_prefix_plan_args *args, kvc_stream_t stream);
 
 /* kvc_paged_attn (starts null) or kvc_paged_attn_rows over prefix and own tokens: lengths and the block table are of own tokens, a request's prefix are the first shared tokens (of those
  * that it has: KVC_FLAG_BAD_LENGTH if it has fewer) of its parent, whose pages are read once for the whole group.  D is 64, 96 or 128, window 0.  workspace: kvc_paged_attn_shared_workspace()
- * bytes, 32-byte aligned, the first kvc_paged_attn_cleared() zeroed once as there; it serves one call at a time.  An infinite value that counts may give no number where its weight is 0 in 16 bits. */
+ * bytes, 32-byte aligned, the first kvc_paged_attn_cleared() zeroed once as there; it serves one call at a time. */
 int64_t kvc_paged_attn_shared_workspace(int64_t B, int64_t Hq, int64_t Hkv, int64_t D);
 int kvc_paged_attn_shared(const kvc_paged_attn_args *args, const int32_t *plan, const int32_t *starts, int64_t rows, kvc_stream_t stream);
 

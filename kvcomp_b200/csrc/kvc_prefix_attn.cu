@@ -725,6 +725,60 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_attn_kernel(const __
 
 // ---- the parts of a row's sums are joined ---------------------------------------------------------------------------
 
+// Writes the result v of query head h of request b, four channels a lane, some of which came out as no numbers although the sum of weights is one, by the definition (as calls without prefixes have
+// it): a value of +inf or -inf that counts makes the result that, both, or one that is no number itself, or one of weight 0 (a score of -inf), none.  For each four channels that hold such a one the
+// warp reads these of the prefix's and the request's own values again, a token a lane, until nothing can change.  In line and small: behind a call, or with eight tokens a lane, all calls took 5 to
+// 7 us more (64 requests behind 16384 tokens).
+template <typename T, int D> __device__ __forceinline__ void write_with_infinities(const Prefix &p, int b, int row, int h, int owner, int groups, float4 v) {
+    constexpr uint32_t INFINITE = Weight<T>::KIND ? 0x7f80u : 0x7c00u;
+    const kvc_paged_attn_args &a = p.a;
+    const int lane = threadIdx.x & 31, hk = kvc_divide(h, p.group);
+    Item item = {};
+    if (owner >= 0 && owner < groups) item = item_of(p, owner);
+    const T *const q = reinterpret_cast<const T *>(a.q) + row * a.q_token + h * a.q_head;
+    const uint32_t none = lane >= D / 4 ? 0 : (v.x != v.x) | (v.y != v.y) << 1 | (v.z != v.z) << 2 | (v.w != v.w) << 3;
+    uint32_t sign = 0;                                      // of each channel: 1 +inf, 2 -inf, 3 none
+#pragma unroll 1
+    for (uint32_t pieces = __ballot_sync(0xffffffffu, none != 0); pieces; pieces &= pieces - 1) {
+        const int piece = __ffs(pieces) - 1;
+        uint32_t seen = 0;
+#pragma unroll 1
+        for (int part = 0; part < 2; part++) {
+            const int32_t *const pages = a.table + (part ? b : item.table) * a.table_stride;
+            const int len = part ? length_of(p, b) : item.len;
+#pragma unroll 1
+            for (int t0 = 0; t0 < len && seen != 0xff; t0 += 32) {
+                const int t = t0 + lane, page = t < len ? pages[kvc_divide(t, p.page)] : -1, r = t - kvc_divide(t, p.page) * (int)a.page_size;
+                uint32_t here = 0;
+                if ((unsigned)page < p.n_pages) {
+                    const uint2 x = *reinterpret_cast<const uint2 *>(reinterpret_cast<const T *>(a.vpages) + page * a.vp_page + r * a.vp_row + hk * a.vp_head + 4 * piece);
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        const uint32_t y = (c < 2 ? x.x : x.y) >> c % 2 * 16 & 0xffff;
+                        if ((y & INFINITE) == INFINITE) here |= ((y & 0x7fff) != INFINITE ? 3u : y & 0x8000 ? 2u : 1u) << 2 * c;
+                    }
+                    if (here) {
+                        const T *const key = reinterpret_cast<const T *>(a.kpages) + page * a.kp_page + r * a.kp_row + hk * a.kp_head;
+                        float score = 0.0f;
+#pragma unroll 1
+                        for (int c = 0; c < D; c++) score += (float)q[c] * (float)key[c];
+                        if ((p.negative ? -score : score) == -CUDART_INF_F) here |= (here >> 1 & 0x55) | (here << 1 & 0xaa);      // the weight is 0
+                    }
+                }
+                seen |= __reduce_or_sync(0xffffffffu, here);
+            }
+        }
+        if (lane == piece) sign = seen;
+    }
+    float r[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+        const uint32_t of = sign >> 2 * c & 3;
+        if (none >> c & 1) r[c] = of == 1 ? CUDART_INF_F : of == 2 ? -CUDART_INF_F : CUDART_NAN_F;
+    }
+    if (lane < D / 4) *reinterpret_cast<uint2 *>(reinterpret_cast<T *>(a.out) + row * a.out_token + h * a.out_head + lane * 4) = make_uint2(pack(r[0], r[1], T()), pack(r[2], r[3], T()));
+}
+
 // A warp for a row's head, or (TEAM 4) four, which take the parts in turn, their sums joined in the warps' order.  Few rows have columns of many parts, eight at a time in flight: the call for
 // 2 x 3 requests of 14 heads behind 31212 tokens, 148 parts a head, takes 35 us with four warps and 41 with one; 64 requests of 32 heads behind 16384, 18 parts a head, 70.5 with four and 67.6
 // with one.
@@ -807,8 +861,14 @@ __global__ void __launch_bounds__(128) prefix_join_kernel(const __grid_constant_
     }
     if (TEAM > 1 && warp > 0) return;
     const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
-    if (on) *reinterpret_cast<uint2 *>(reinterpret_cast<T *>(a.out) + row * a.out_token + h * a.out_head + lane * 4) = make_uint2(pack(v.x * f, v.y * f, T()), pack(v.z * f, v.w * f, T()));
+    v = make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
     if (lane == 0 && a.lse) a.lse[row * a.Hq + h] = sum == 0.0f ? -CUDART_INF_F : (top + log2f(sum)) * 0.69314718055994531f;
+    const float any = v.x + v.y + v.z + v.w;
+    if (__any_sync(0xffffffffu, any != any && sum == sum)) {
+        write_with_infinities<T, D>(p, b, row, h, owner.x, groups, v);
+        return;
+    }
+    if (on) *reinterpret_cast<uint2 *>(reinterpret_cast<T *>(a.out) + row * a.out_token + h * a.out_head + lane * 4) = make_uint2(pack(v.x, v.y, T()), pack(v.z, v.w, T()));
 }
 
 template <typename T, int D>

@@ -867,7 +867,7 @@ def paged_attn_shared_workspace(B, Hq, Hkv, D, device):
 def paged_attn_shared(q, kpages, vpages, table, lengths, plan, scaling, out=None, return_lse=False, workspace=None, status=None, starts=None):
     """paged_attn where requests continue prefixes: request b's token attends to the first shared[b] tokens of its parent (of those that it has: FLAG_BAD_LENGTH if it has fewer) and to b's own
     lengths[b].  plan: prefix_plan's, of these B requests.  The pages of a prefix are read once for all that follow it (once for 256 rows of a KV head).  D: 64, 96, 128; no window.  workspace:
-    paged_attn_shared_workspace's, for one call at a time.  Values that count are finite (0 times an infinite one is no number).  The other arguments are paged_attn's."""
+    paged_attn_shared_workspace's, for one call at a time.  The other arguments are paged_attn's."""
     if not isinstance(plan, PrefixPlan):
         raise KvcError("plan must be prefix_plan's")
     if not isinstance(q, torch.Tensor) or not q.is_cuda or q.dim() != 3 or not isinstance(kpages, torch.Tensor) or kpages.dim() != 4:
