@@ -13,15 +13,15 @@
 // shares, so that results do not depend on timing.
 //
 // Keys and values come by 16-byte asynchronous copies (pages end anywhere, any strides) into a ring in shared memory, in the 128-byte swizzled layout that the products read: keys
-// channel by channel, values as they lie (token by token: the product's second operand turned).  Rounding: the weights are fp16 (times 2^7: 2^-21 of the largest are still normal numbers) or bf16,
-// the sums of weights are taken before that; everything joined is 32 bits and the result is rounded once.  (Weights in 16 bits are off as the result's own rounding is: the error against 64 bits
-// is 1.35 times the plain form's, 2.3e-3 bf16, 2.8e-4 fp16.)
+// channel by channel, values as they lie (token by token: the product's second operand turned).  Rounding: a weight has two pieces of fp16
+// (times 2^7) or bf16, as in the kernel of calls without prefixes, and the second product is made with both: who follows a prefix has results as exact as who holds the same tokens.  Sums of weights
+// are taken before that; everything joined is 32 bits and the result is rounded once.  (Of one piece: 58.5 us for the first call below, and 1.35 times the error against 64 bits.)
 //
-// Measured, device times of one B200: 64 requests of 32 heads behind 16384 tokens of 8 KV heads (256 rows a KV head), 1 to 500 own tokens each, 61 us: prefix 35, own tokens 23 (some of it beside the
-// prefix's end), joining 9.5.  Of the 35, 5 pass before the first tile's scores (lengths, pages, first bytes, one behind the other) and 4 with 19 MB of parts; a tile takes 4500 cycles, its
-// exponentials alone 2048, its products 2048.  8 times 16 requests of 40 heads behind 8000 tokens of 10 (64 rows a KV head) 133 us: prefix 62 (280 MB, 4.5 TB/s), own tokens 64, joining 9.5.  4
-// requests of 32 heads behind 777 tokens 16.6 us: three kernels' starts.  (Joined where the own tokens' columns end, without a third kernel: 78, 155 and 18.5 us: few threads read many
-// parts then, and hold what others need meanwhile.)
+// Measured, device times of one B200: 64 requests of 32 heads behind 16384 tokens of 8 KV heads (256 rows a KV head), 1 to 500 own tokens each, 66 us: prefix 41, own tokens 23 (some of it beside the
+// prefix's end), joining 10.  Of the 41, 5 pass before the first tile's scores (lengths, pages, first bytes, one behind the other) and 4 with 19 MB of parts; a tile's exponentials alone take 2048
+// cycles, its products 3072.  8 times 16 requests of 40 heads behind 8000 tokens of 10 (64 rows a KV head) 137 us: prefix 70 (280 MB, 4 TB/s), own tokens 66, joining 10.  4 requests of 32 heads
+// behind 777 tokens 17.5 us: three kernels' starts.  (Joined where the own tokens' columns end, without a third kernel, 17 to 22 us more: few threads read many parts then, and hold what others
+// need meanwhile.)
 #include <math_constants.h>
 #include <string.h>
 
@@ -258,7 +258,6 @@ __device__ __forceinline__ void product(uint32_t one, uint32_t d, uint64_t a, ui
 __device__ __forceinline__ void product_of_weights(uint32_t one, uint32_t d, uint32_t a, uint64_t b, uint32_t kind, bool add) {
     asm volatile("{ .reg .pred p, e; setp.ne.u32 p, %4, 0; setp.ne.u32 e, %5, 0; @e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(d), "r"(a), "l"(b), "r"(kind), "r"((uint32_t)add), "r"(one) : "memory");
 }
-#define KVC_16(X) X(0), X(1), X(2), X(3), X(4), X(5), X(6), X(7), X(8), X(9), X(10), X(11), X(12), X(13), X(14), X(15)
 #define KVC_32(X) X(0), X(1), X(2), X(3), X(4), X(5), X(6), X(7), X(8), X(9), X(10), X(11), X(12), X(13), X(14), X(15), X(16), X(17), X(18), X(19), X(20), X(21), X(22), X(23), X(24), X(25), X(26), X(27), X(28), X(29), X(30), X(31)
 __device__ __forceinline__ void load32(uint32_t *r, uint32_t at) {
 #define KVC_OUT(i) "=r"(r[i])
@@ -276,11 +275,6 @@ __device__ __forceinline__ void loads_wait(uint32_t *r) {    // (nothing of r is
 #define KVC_BOTH(i) "+r"(r[i])
     asm volatile("tcgen05.wait::ld.sync.aligned;" : KVC_32(KVC_BOTH)::"memory");
 #undef KVC_BOTH
-}
-__device__ __forceinline__ void store16(uint32_t at, const uint32_t *r) {
-#define KVC_IN(i) "r"(r[i])
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::KVC_16(KVC_IN), "r"(at) : "memory");
-#undef KVC_IN
 }
 __device__ __forceinline__ void stores_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // two at a time
@@ -498,25 +492,27 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_attn_kernel(const __
                         const float less = LIFT - (m == -CUDART_INF_F ? 0.0f : m);
                         const float2 scale2 = make_float2(p.log2_scaling, p.log2_scaling), less2 = make_float2(less, less);
                         float2 sum[2] = {};
-                        auto weigh = [&](const uint32_t *v, uint32_t to) {
-                            uint32_t weights[16];           // (they take the place of scores that have been read)
+                        auto weigh = [&](const uint32_t *v, uint32_t to) {       // (weights take the scores' own place: 16 columns, and 16 of what is left of them)
+                            uint32_t weights[32];
 #pragma unroll
                             for (int i = 0; i < 16; i++) {
                                 const float2 e = fma2(make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), scale2, less2);
                                 const float2 f = make_float2(exp2_approx(e.x), exp2_approx(e.y));
                                 sum[i & 1] = add2(sum[i & 1], f);
                                 weights[i] = pack(f.x, f.y, T());
+                                const float2 g = unpack(weights[i], T()), r = add2(f, make_float2(-g.x, -g.y));
+                                weights[16 + i] = pack(r.x, r.y, T());
                             }
-                            store16(to, weights);
+                            store32(to, weights);
                         };
 #pragma unroll 1
                         for (int c = 0; c < 2; c++) {
                             loads_wait(x);
                             load32(y, scores + 64 * c + 32);
-                            weigh(x, scores + 32 * c);
+                            weigh(x, scores + 64 * c);
                             loads_wait(y);
                             if (c == 0) load32(x, scores + 64);
-                            weigh(y, scores + 32 * c + 16);
+                            weigh(y, scores + 64 * c + 32);
                         }
                         l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                         stores_wait();
@@ -569,7 +565,10 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_attn_kernel(const __
                     const uint64_t b = values + (uint32_t)job.slot * (UNIT / 16);
                     const uint32_t d = t_at + 256 + set * 128, a_at = t_at + set * 128;
 #pragma unroll
-                    for (int k = 0; k < TOKENS / 16; k++) product_of_weights(one, d, a_at + 8 * k, b + k * (2048 / 16), VALUES, k > 0 || !job.first);
+                    for (int k = 0; k < TOKENS / 16; k++) {         // (of 32 tokens the weights, 16 columns, then what is left of them)
+                        product_of_weights(one, d, a_at + k / 2 * 32 + k % 2 * 8, b + k * (2048 / 16), VALUES, k > 0 || !job.first);
+                        product_of_weights(one, d, a_at + k / 2 * 32 + k % 2 * 8 + 16, b + k * (2048 / 16), VALUES, true);
+                    }
                     if (job.last) commit_to(one, empty + job.slot);
                     if (job.ends) commit_to(one, sums_there + set);
                 };
@@ -728,7 +727,7 @@ __global__ void __launch_bounds__(PREFIX_THREADS, 1) prefix_attn_kernel(const __
 // Writes the result v of query head h of request b, four channels a lane, some of which came out as no numbers although the sum of weights is one, by the definition (as calls without prefixes have
 // it): a value of +inf or -inf that counts makes the result that, both, or one that is no number itself, or one of weight 0 (a score of -inf), none.  For each four channels that hold such a one the
 // warp reads these of the prefix's and the request's own values again, a token a lane, until nothing can change.  In line and small: behind a call, or with eight tokens a lane, all calls took 5 to
-// 7 us more (64 requests behind 16384 tokens).
+// 7 us more (64 requests behind 16384 tokens).  One infinity among these 364 us.
 template <typename T, int D> __device__ __forceinline__ void write_with_infinities(const Prefix &p, int b, int row, int h, int owner, int groups, float4 v) {
     constexpr uint32_t INFINITE = Weight<T>::KIND ? 0x7f80u : 0x7c00u;
     const kvc_paged_attn_args &a = p.a;

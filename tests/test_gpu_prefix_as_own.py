@@ -1,4 +1,4 @@
-"""Requests that follow a prefix have the results of requests that hold the same tokens themselves, where values are infinite too."""
+"""Requests that follow a prefix have the results of requests that hold the same tokens themselves: as exact, and the same where values are infinite."""
 import math
 
 import pytest
@@ -19,6 +19,40 @@ def ops():
 
 def ints(a):
     return torch.tensor(a, dtype=torch.int32, device="cuda")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [64, 96, 128])
+@pytest.mark.parametrize("members,Hq,tokens", [(1, 1, 512), (3, 4, 700), (40, 8, 900), (2, 1, 30000)])
+def test_weights_that_round_alike(ops, dtype, D, members, Hq, tokens):
+    """All but every 64th token have a weight next to the middle of two numbers of 16 bits: one rounding of weights is off by half a step, in one direction, beside the result's."""
+    eps = torch.finfo(dtype).eps / 2
+    weight = (1 + 0.97 * eps) / 8
+    scaling = -math.log(weight)
+    page = 64
+    pages = -(-tokens // page) + members
+    kp, vp = (torch.zeros(pages, page, 1, D, dtype=dtype, device="cuda") for _ in range(2))
+    kp[:, 1:, 0, 0] = -1.0
+    v = (1 + torch.arange(D, device="cuda") / D).to(dtype)
+    vp[:, 1:, 0] = v
+    q = torch.zeros(members + 1, Hq, D, dtype=dtype, device="cuda")
+    q[:, :, 0] = 1.0
+    table = torch.full((members + 1, pages), -1, dtype=torch.int32, device="cuda")
+    own = 33
+    table[0, :pages - members] = torch.arange(pages - members)
+    table[1:, 0] = torch.arange(pages - members, pages)
+    plan = ops.prefix_plan(ints([-1] + [0] * members), ints([0] + [tokens] * members))
+    out = ops.paged_attn_shared(q, kp, vp, table, ints([tokens] + [own] * members), plan, scaling)
+    large = -(-tokens // 64) + 1
+    small = tokens + own - large
+    want = v.double() * small * weight / (large + small * weight)
+    # A score is one product (the others are 0), scaled: with the sum's steps its weight is off by (D + 4) 2^-23 of 2.1 and 27 2^-22 (as in the tests of prefixes), two pieces of 16 bits by
+    # 2^-20 (fp16) and 2^-16 (bf16); the sums by 2^-23 a step, of up to 128 tokens' partial sums and the parts that are joined; then the result is rounded.
+    d = 2.1 * (D + 4) * 2.0 ** -23 + 27 * 2.0 ** -22
+    off = want * (2 * d + (2.0 ** -20 if dtype == torch.float16 else 2.0 ** -16) + (tokens / 8 + 512) * 2.0 ** -23)
+    bound = off + eps * (want + off)
+    error = (out[1:].double() - want).abs()
+    assert bool((error <= bound).all()), float((error / bound).max())
 
 
 def both(ops, kp, vp, q, prefix, owns, page, Hq):
