@@ -89,7 +89,8 @@ class PagedKVCache:
         (begin), and attend covers both.  shared None: all tokens that the parent has now.  Requests that follow the same tokens are attended to together, and these are read once.  To be said
         before a follower's first tokens; for all requests at once, those that followed before included.  Who is followed brings no more tokens, stays until its followers have ended, and
         follows no one; a follower that ends (release) follows no one any more; a parent that is no request, or the request itself, is none (reported: check).  Steps that are captured behind
-        the first call go by the last one, captured or not.  Heads of 64, 96 or 128 channels, no window, no codes."""
+        the first call go by the last one, captured or not.  Heads of 64, 96 or 128 channels, no window, no codes.  Pays from some 260000 on of followers x shared tokens x KV heads; one
+        follower alone costs more than the same tokens of its own."""
         if self.window or self.codes or self.head_dim not in ops.SHARED_HEADS:
             raise KvcError("PagedKVCache.follow: heads of 64, 96 or 128 channels, no window and no codes")
         if not isinstance(parents, torch.Tensor) or parents.dtype != torch.int32 or tuple(parents.shape) != (self.requests,) or parents.device != self.device:

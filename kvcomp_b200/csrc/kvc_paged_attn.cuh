@@ -290,8 +290,8 @@ template <int D, int KIND> struct Tiles {
 // it meets the codes, as two pieces of fp16, for which the product is too small or too large: a power of two that brings the largest product of a head so far to 2^14 is kept beside the sums as
 // the maximum is, and taken out of them.  (The largest product, not the largest scale: a row of large values that a head gives no weight takes no bits of the others.)  What is 2^-39 of that
 // product is lost, and a weight that is 2^-126 of the largest one.  bf16 queries become fp16 times a power of two for each head (what is 2^29 below the head's largest value loses bits, no less than a sum in 32 bits does).
-// What bounds them is no longer HBM but instructions, about 980 for a tile of 32 tokens of 128 channels, a third of them codes that become numbers: 8 x 4096 tokens of 32 heads in int8 61 us (4.5 TB/s;
-// fp16 rows 85), 16 x 32768 of 8 KV heads in e4m3 207 (5.3 TB/s; 317).  So CTAs have equal work sooner than with rows of 16 bits: one CTA a column of 8 x 4096 took 82 us.
+// What bounds them is no longer HBM but instructions, about 1020 for a tile of 32 tokens of 128 channels, a third of them codes that become numbers: 8 x 4096 tokens of 32 heads in int8 60 us (4.6 TB/s;
+// fp16 rows 85), 16 x 32768 of 8 KV heads in e4m3 213 (5.2 TB/s; 317), with other pools from call to call 220.  (By the largest scale of a warp instead of a head's largest product 2 to 4 % less.)  So CTAs have equal work sooner than with rows of 16 bits: one CTA a column of 8 x 4096 took 82 us.
 template <typename T, int D, int NT, int WH, bool SAME, int STAGES, int CTAS, bool ROWS, int KIND>
 __global__ void __launch_bounds__(THREADS, CTAS) paged_attn_kernel(const __grid_constant__ Params p) {
     constexpr bool CODED = Tiles<D, KIND>::CODED;

@@ -5,7 +5,7 @@ namespace kvc_paged {
 namespace {
 
 // As for rows of 16 bits (a stage has twice the tokens and the same bytes, and their scales); 96 channels with a stage less, which three CTAs need to fit an SM.  Rows of 64 and 96 channels of two KV
-// heads are read together, as there (16 x 16384 tokens of 8 heads of 64 channels in int8 77.9 us, one by one 79.6; of 96, 12288, 82.0 and 82.2).
+// heads are read together, as there (8 x 4096 tokens of 32 heads of 96 channels in int8 56 us, one by one 69; 16 x 16384 of 8 heads of 64 in e4m3 with a query head each 76 and 77.6, with eight 80.4 and 79.2).
 template <typename T, int D, int STAGES, int CTAS, int WIDE_STAGES, int WIDE_CTAS, int KIND>
 int choose_heads(Params &p, cudaStream_t s) {
     if constexpr (WIDE_STAGES > 0) {

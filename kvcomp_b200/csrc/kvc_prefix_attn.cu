@@ -17,10 +17,10 @@
 // (times 2^7) or bf16, as in the kernel of calls without prefixes, and the second product is made with both: who follows a prefix has results as exact as who holds the same tokens.  Sums of weights
 // are taken before that; everything joined is 32 bits and the result is rounded once.  (Of one piece: 58.5 us for the first call below, and 1.35 times the error against 64 bits.)
 //
-// Measured, device times of one B200: 64 requests of 32 heads behind 16384 tokens of 8 KV heads (256 rows a KV head), 1 to 500 own tokens each, 66 us: prefix 41, own tokens 23 (some of it beside the
+// Measured, device times of one B200: 64 requests of 32 heads behind 16384 tokens of 8 KV heads (256 rows a KV head), 1 to 500 own tokens each, 64 us: prefix 41, own tokens 23 (some of it beside the
 // prefix's end), joining 10.  Of the 41, 5 pass before the first tile's scores (lengths, pages, first bytes, one behind the other) and 4 with 19 MB of parts; a tile's exponentials alone take 2048
-// cycles, its products 3072.  8 times 16 requests of 40 heads behind 8000 tokens of 10 (64 rows a KV head) 137 us: prefix 70 (280 MB, 4 TB/s), own tokens 66, joining 10.  4 requests of 32 heads
-// behind 777 tokens 17.5 us: three kernels' starts.  (Joined where the own tokens' columns end, without a third kernel, 17 to 22 us more: few threads read many parts then, and hold what others
+// cycles, its products 3072.  8 times 16 requests of 40 heads behind 8000 tokens of 10 (64 rows a KV head) 135 us: prefix 70 (280 MB, 4 TB/s), own tokens 66, joining 10.  4 requests of 32 heads
+// behind 777 tokens 15.4 us: three kernels' starts.  (Joined where the own tokens' columns end, without a third kernel, 2 to 22 us more: few threads read many parts then, and hold what others
 // need meanwhile.)
 #include <math_constants.h>
 #include <string.h>
@@ -779,8 +779,8 @@ template <typename T, int D> __device__ __forceinline__ void write_with_infiniti
 }
 
 // A warp for a row's head, or (TEAM 4) four, which take the parts in turn, their sums joined in the warps' order.  Few rows have columns of many parts, eight at a time in flight: the call for
-// 2 x 3 requests of 14 heads behind 31212 tokens, 148 parts a head, takes 35 us with four warps and 41 with one; 64 requests of 32 heads behind 16384, 18 parts a head, 70.5 with four and 67.6
-// with one.
+// 2 x 3 requests of 14 heads behind 31212 tokens, 148 parts a head, takes 28 us with four warps and 34 with one; 64 requests of 32 heads behind 16384, 18 parts a head, 65.4 with four and 63 with
+// one.
 template <typename T, int D, int TEAM>
 __global__ void __launch_bounds__(128) prefix_join_kernel(const __grid_constant__ Prefix p) {
     kvc_behind();
