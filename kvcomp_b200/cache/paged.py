@@ -99,7 +99,7 @@ class PagedKVCache:
             shared = self.lengths[parents.clamp(0, self.requests - 1).long()]
         elif not isinstance(shared, torch.Tensor) or shared.dtype != torch.int32 or tuple(shared.shape) != (self.requests,) or shared.device != self.device:
             raise KvcError("shared must be int32[%d] on %s" % (self.requests, self.device))
-        if self.prefixes is None and torch.cuda.is_current_stream_capturing():
+        if self.prefixes is None and _lib.torch_calls().stream_of(self.device.index)[1]:         # (the capture of the cache's own device)
             raise KvcError("PagedKVCache.follow: the first call makes what all steps go by, and must not be captured")
         # whom nobody can follow is followed by none, in the plan, in positions and in lengths alike, and is reported (check raises)
         valid = (parents >= 0) & (parents < self.requests) & (parents != torch.arange(self.requests, dtype=torch.int32, device=self.device)) & (shared >= 0)
