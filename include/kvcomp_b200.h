@@ -486,8 +486,8 @@ typedef struct {
     int32_t codes, reserved;
 } kvc_scales;
 
-/* kvc_rotary_store into pools of codes: keys are coded as they are rotated, in fp32 (int8) or as if without any error (e4m3: the angle is position x frequency in fp64), values as they are; Hkv > 0.  Neither pools nor scales may overlap one another or what is
- * read or written beside them. */
+/* kvc_rotary_store into pools of codes: keys are coded as they are rotated, in fp32 (int8) or as if without any error (e4m3: the angle is position x frequency in fp64), values as they
+ * are; Hkv > 0.  Neither pools nor scales may overlap one another or what is read or written beside them. */
 int kvc_rotary_store_codes(const kvc_rotary_args *args, const kvc_scales *scales, kvc_stream_t stream);
 
 /* The slots of all tokens that requests have, packed request by request: starts[b] the first row of request b (B + 1 numbers), slots[row] = page * page_size + row of

@@ -19,7 +19,7 @@
 //
 // Measured, device times of one B200: 64 requests of 32 heads behind 16384 tokens of 8 KV heads (256 rows a KV head), 1 to 500 own tokens each, 64 us: prefix 41, own tokens 23 (some of it beside the
 // prefix's end), joining 10.  Of the 41, 5 pass before the first tile's scores (lengths, pages, first bytes, one behind the other) and 4 with 19 MB of parts; a tile's exponentials alone take 2048
-// cycles, its products 3072.  8 times 16 requests of 40 heads behind 8000 tokens of 10 (64 rows a KV head) 135 us: prefix 70 (280 MB, 4 TB/s), own tokens 66, joining 10.  4 requests of 32 heads
+// cycles, its products half as many again.  8 times 16 requests of 40 heads behind 8000 tokens of 10 (64 rows a KV head) 135 us: prefix 70 (280 MB, 4 TB/s), own tokens 66, joining 10.  4 requests of 32 heads
 // behind 777 tokens 15.4 us: three kernels' starts.  (Joined where the own tokens' columns end, without a third kernel, 2 to 22 us more: few threads read many parts then, and hold what others
 // need meanwhile.)
 #include <math_constants.h>

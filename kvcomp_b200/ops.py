@@ -781,7 +781,8 @@ def rotary_paged_store(q, k, v, positions, slots, frequencies, kpages, vpages, l
     dimension.  positions, frequencies, layout, factor: as for rotary; frequencies None: nothing is rotated.  Tokens of one call have slots of their own.
     Outputs and pools must not overlap (views of one tensor that lie in one another are fine).  For serving: no gradient goes through it.
     kscales, vscales (fp32 [pages, Hkv, page_size], last dimension contiguous): the pools hold 8-bit codes, torch.int8 or torch.float8_e4m3fn, and a token's row of a head has one scale:
-    int8 max |x| / 127, e4m3 the least power of two with max |x| / scale <= 448, none below 2^-100; a row that holds an infinity or no number has the scale NaN.  D is a multiple of 16 then."""
+    int8 max |x| / 127, e4m3 the least power of two with max |x| / scale <= 448, none below 2^-100; a row that holds an infinity or no number has the scale NaN.  Keys are coded as they are
+    rotated, e4m3 ones as if without any error.  D is a multiple of 16 then."""
     if k is None:
         raise KvcError("k must be a tensor")
     return _lib.torch_calls().rotary_store(q, k, v, positions, slots, frequencies, kpages, vpages, _LAYOUTS.get(layout), factor, False, out, status, kscales, vscales)
